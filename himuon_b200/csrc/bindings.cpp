@@ -279,6 +279,116 @@ static void flash_attn_bwd(const at::Tensor& d_o, const at::Tensor& q, const at:
   himuon::flash_attn_bwd(a, cur_stream());
 }
 
+// `plan`: (2, tiles, 4) int32, the batch's tiles in the two orders (himuon.h); its entries are bounded by the caller, which makes
+// them from the lengths on the host (`tokens` of them).
+static himuon::PackedAttnArgs packed_attn_args(const char* op, const at::Tensor& plan, int64_t tokens, const at::Tensor& q, const at::Tensor& k,
+                                               const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse, int64_t Hq, int64_t Hkv, double scale) {
+  const std::string at = std::string("himuon: ") + op;
+  TORCH_CHECK(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, at, ": heads");
+  TORCH_CHECK(q.dim() == 2 && q.size(1) % Hq == 0, at, ": (tokens, heads*head_dim) views expected");
+  const int64_t T = q.size(0), hd = q.size(1) / Hq;
+  TORCH_CHECK(hd > 0 && hd % 8 == 0 && hd <= 128, at, ": head_dim must be a multiple of 8 up to 128");
+  TORCH_CHECK(T > 0 && T < (1LL << 30) && tokens >= 0 && tokens <= T, at, ": fewer rows than the layout has tokens");
+  TORCH_CHECK(plan.device() == q.device() && plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.dim() == 3 && plan.size(0) == 2 && plan.size(2) == 4,
+              at, ": the plan must be a contiguous (2, tiles, 4) int32 tensor on the device of q");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0, at, ": misaligned plan");
+  himuon::PackedAttnArgs a{};
+  a.n_tiles = static_cast<int>(plan.size(1));
+  a.by_keys = reinterpret_cast<const himuon::PackedTile*>(plan.data_ptr<int>());
+  a.by_queries = a.by_keys + a.n_tiles;
+  a.rows = static_cast<int>(T); a.Hq = static_cast<int>(Hq); a.Hkv = static_cast<int>(Hkv); a.hd = static_cast<int>(hd);
+  a.scale = static_cast<float>(scale);
+  TORCH_CHECK(is_f32(lse) && lse.is_contiguous() && lse.device() == q.device() && lse.numel() == Hq * a.n_tiles * 128 &&
+                  reinterpret_cast<uintptr_t>(lse.data_ptr()) % 16 == 0, at, ": lse must be fp32, (heads, tiles * 128)");
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr(); a.lse = lse.data_ptr<float>();
+  a.ld_q = q.stride(0); a.ld_k = k.stride(0); a.ld_v = v.stride(0); a.ld_o = o.stride(0);
+  return a;
+}
+static void packed_rows(const char* op, const at::Tensor& t, const at::Tensor& q, int64_t cols) {
+  const std::string at = std::string("himuon: ") + op;
+  TORCH_CHECK(t.is_cuda() && t.device() == q.device() && is_bf16(t) && t.dim() == 2 && t.size(0) == q.size(0) && t.size(1) == cols && t.stride(1) == 1 &&
+                  t.stride(0) % 8 == 0 && (t.size(0) <= 1 || t.stride(0) >= cols) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              at, ": bf16 rows of heads * head_dim columns with unit inner stride, each on a 16-byte boundary, expected");
+}
+static void packed_attn_fwd(const at::Tensor& plan, int64_t tokens, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& o,
+                            at::Tensor& lse, int64_t Hq, int64_t Hkv, double scale) {
+  const himuon::PackedAttnArgs a = packed_attn_args("packed_attn_fwd", plan, tokens, q, k, v, o, lse, Hq, Hkv, scale);
+  packed_rows("packed_attn_fwd", q, q, Hq * a.hd); packed_rows("packed_attn_fwd", k, q, Hkv * a.hd);
+  packed_rows("packed_attn_fwd", v, q, Hkv * a.hd); packed_rows("packed_attn_fwd", o, q, Hq * a.hd);
+  const c10::cuda::CUDAGuard guard(q.device());
+  himuon::packed_attn_fwd(a, cur_stream());
+}
+static void packed_attn_bwd(const at::Tensor& plan, int64_t tokens, const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& o, const at::Tensor& lse, at::Tensor& dq, at::Tensor& dk, at::Tensor& dv, at::Tensor& delta,
+                            int64_t Hq, int64_t Hkv, double scale) {
+  himuon::PackedAttnArgs a = packed_attn_args("packed_attn_bwd", plan, tokens, q, k, v, o, lse, Hq, Hkv, scale);
+  for (const at::Tensor* t : {&q, &o, &d_o, static_cast<const at::Tensor*>(&dq)}) packed_rows("packed_attn_bwd", *t, q, Hq * a.hd);
+  for (const at::Tensor* t : {&k, &v, static_cast<const at::Tensor*>(&dk), static_cast<const at::Tensor*>(&dv)}) packed_rows("packed_attn_bwd", *t, q, Hkv * a.hd);
+  HM_CHECK(is_f32(delta) && delta.is_contiguous() && delta.device() == q.device() && delta.numel() == lse.numel() &&
+               reinterpret_cast<uintptr_t>(delta.data_ptr()) % 16 == 0, "packed_attn_bwd: delta must look like lse");
+  a.d_o = d_o.data_ptr(); a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr(); a.delta = delta.data_ptr<float>();
+  a.ld_do = d_o.stride(0); a.ld_dq = dq.stride(0); a.ld_dk = dk.stride(0); a.ld_dv = dv.stride(0);
+  const c10::cuda::CUDAGuard guard(q.device());
+  himuon::packed_attn_bwd(a, cur_stream());
+}
+
+// Checks what the forward and the gradient call share.
+static himuon::TokenScoreArgs token_score_args(const char* op, const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& entropy,
+                                               int64_t ignore_index) {
+  const std::string at = std::string("himuon: ") + op;
+  TORCH_CHECK(logits.is_cuda() && (is_bf16(logits) || is_f32(logits)) && logits.dim() == 2 && logits.stride(1) == 1 &&
+                  (logits.size(0) <= 1 || logits.stride(0) >= logits.size(1)), at, ": (rows, vocab) bf16 or fp32 logits with unit inner stride");
+  TORCH_CHECK(logits.size(1) > 0 && logits.size(1) < (1LL << 31), at, ": bad vocabulary");
+  TORCH_CHECK(ids.device() == logits.device() && ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == logits.size(0), at, ": one int64 id for each row");
+  TORCH_CHECK(entropy.device() == logits.device() && is_f32(entropy) && entropy.is_contiguous() && entropy.numel() == logits.size(0), at, ": entropy must be fp32, one for each row");
+  himuon::TokenScoreArgs a{};
+  a.logits = logits.data_ptr(); a.logits_fp32 = is_f32(logits) ? 1 : 0;
+  a.ids = reinterpret_cast<const long long*>(ids.data_ptr<int64_t>()); a.ignore = ignore_index;
+  a.rows = logits.size(0); a.ld = logits.stride(0); a.vocab = static_cast<int>(logits.size(1));
+  a.entropy = entropy.data_ptr<float>();
+  return a;
+}
+static void token_scores_fwd(const at::Tensor& logits, const at::Tensor& ids, at::Tensor& log_probs, at::Tensor& entropy,
+                             const c10::optional<at::Tensor>& stats, const c10::optional<at::Tensor>& top_log_probs,
+                             const c10::optional<at::Tensor>& top_ids, int64_t ignore_index) {
+  himuon::TokenScoreArgs a = token_score_args("token_scores_fwd", logits, ids, entropy, ignore_index);
+  HM_CHECK(log_probs.device() == logits.device() && is_f32(log_probs) && log_probs.is_contiguous() && log_probs.numel() == a.rows, "token_scores_fwd: log_probs must be fp32, one for each row");
+  a.log_probs = log_probs.data_ptr<float>();
+  if (stats.has_value()) {
+    HM_CHECK(stats->device() == logits.device() && is_f32(*stats) && stats->is_contiguous() && stats->numel() == 2 * a.rows, "token_scores_fwd: stats must be fp32, two for each row");
+    a.stats = stats->data_ptr<float>();
+  }
+  HM_CHECK(top_log_probs.has_value() == top_ids.has_value(), "token_scores_fwd: alternatives need values and ids");
+  if (top_ids.has_value()) {
+    HM_CHECK(top_ids->device() == logits.device() && top_log_probs->device() == logits.device() && top_ids->scalar_type() == at::kLong &&
+                 is_f32(*top_log_probs) && top_ids->is_contiguous() && top_log_probs->is_contiguous() && top_ids->dim() == 2 &&
+                 top_ids->size(0) == a.rows && top_log_probs->sizes() == top_ids->sizes() && top_ids->size(1) > 0 &&
+                 top_ids->size(1) <= himuon::kTopMax && top_ids->size(1) <= a.vocab,
+             "token_scores_fwd: alternatives must be (rows, 1..32) fp32 values and int64 ids");
+    a.top_k = static_cast<int>(top_ids->size(1));
+    a.top_log_probs = top_log_probs->data_ptr<float>();
+    a.top_ids = reinterpret_cast<long long*>(top_ids->data_ptr<int64_t>());
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  himuon::token_scores_fwd(a, cur_stream());
+}
+static void token_scores_bwd(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& entropy, const at::Tensor& stats,
+                             const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy, at::Tensor& grad,
+                             int64_t ignore_index) {
+  himuon::TokenScoreArgs a = token_score_args("token_scores_bwd", logits, ids, entropy, ignore_index);
+  HM_CHECK(stats.device() == logits.device() && is_f32(stats) && stats.is_contiguous() && stats.numel() == 2 * a.rows, "token_scores_bwd: stats must be fp32, two for each row");
+  HM_CHECK(grad.device() == logits.device() && grad.dim() == 2 && grad.sizes() == logits.sizes() && grad.stride(1) == 1 && (is_bf16(grad) || is_f32(grad)) &&
+               (grad.size(0) <= 1 || grad.stride(0) >= grad.size(1)), "token_scores_bwd: the gradient has the shape of the logits");
+  for (const auto* g : {&g_log_probs, &g_entropy})
+    if (g->has_value()) HM_CHECK((*g)->device() == logits.device() && is_f32(**g) && (*g)->is_contiguous() && (*g)->numel() == a.rows, "token_scores_bwd: incoming gradients must be fp32, one for each row");
+  a.stats = stats.data_ptr<float>();
+  a.g_log_probs = g_log_probs.has_value() ? g_log_probs->data_ptr<float>() : nullptr;
+  a.g_entropy = g_entropy.has_value() ? g_entropy->data_ptr<float>() : nullptr;
+  a.grad = grad.data_ptr(); a.grad_fp32 = is_f32(grad) ? 1 : 0; a.ld_grad = grad.stride(0);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  himuon::token_scores_bwd(a, cur_stream());
+}
+
 static bool ns5_fused_supported(int64_t m, int64_t n) { return himuon::ns5_fused_supported((int)m, (int)n); }
 static void ns5_fused(const at::Tensor& x, at::Tensor& out, int64_t steps, double eps, bool normalize) {
   HM_CHECK(x.is_cuda() && is_bf16(x) && is_bf16(out) && x.is_contiguous() && out.is_contiguous() && x.dim() == 3 && x.sizes() == out.sizes(), "ns5_fused: contiguous (B, m, n) bf16 tensors");
@@ -362,6 +472,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_fwd", &embedding_fwd);
   m.def("embedding_bwd", &embedding_bwd);
   m.def("cross_entropy", &cross_entropy);
+  m.def("packed_attn_fwd", &packed_attn_fwd);
+  m.def("packed_attn_bwd", &packed_attn_bwd);
+  m.def("token_scores_fwd", &token_scores_fwd);
+  m.def("token_scores_bwd", &token_scores_bwd);
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("flash_attn_bwd", &flash_attn_bwd);
   m.def("ns5_fused_supported", &ns5_fused_supported);

@@ -160,6 +160,38 @@ struct AttnArgs {
 void flash_attn_fwd(const AttnArgs& a, cudaStream_t s);
 void flash_attn_bwd(const AttnArgs& a, cudaStream_t s);
 
+// ---------------------------------------------------------------- packed attention (packed_attention_sm100.cu)
+// A tile of up to 128 tokens of one document: the document's first row and length, the tile's number in it and in the batch.
+struct PackedTile { int first, len, index, slot; };
+// q, o and their gradients: (rows, Hq * hd); k, v and theirs: (rows, Hkv * hd); bf16, row strides ld_*.  The tiles are listed
+// twice, by falling number of keys that their queries see and by falling number of queries that see their keys.  lse and delta:
+// (Hq, n_tiles * 128) fp32.  Rows of no document are left alone.
+struct PackedAttnArgs {
+  const PackedTile* by_keys; const PackedTile* by_queries;
+  int n_tiles, rows, Hq, Hkv, hd;
+  const void* q; const void* k; const void* v; void* o; float* lse;
+  const void* d_o; void* dq; void* dk; void* dv; float* delta;
+  long long ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv;
+  float scale;
+};
+void packed_attn_fwd(const PackedAttnArgs& a, cudaStream_t s);
+void packed_attn_bwd(const PackedAttnArgs& a, cudaStream_t s);
+
+// ---------------------------------------------------------------- token scores
+constexpr int kTopMax = 32;             // most alternatives a call returns
+// Log probabilities of given ids, entropy and the top_k likeliest ids of (rows, vocab) logits with row stride ld (token_scores.cu).
+struct TokenScoreArgs {
+  const void* logits; int logits_fp32;
+  const long long* ids; long long ignore;
+  long long rows, ld; int vocab, top_k;
+  float* log_probs; float* entropy; float* stats;          // stats: two per row (optional), kept for the gradient
+  float* top_log_probs; long long* top_ids;                // (rows, top_k)
+  void* grad; int grad_fp32; long long ld_grad;            // gradient only; the incoming gradients may be null
+  const float* g_log_probs; const float* g_entropy;
+};
+void token_scores_fwd(const TokenScoreArgs& a, cudaStream_t s);
+void token_scores_bwd(const TokenScoreArgs& a, cudaStream_t s);
+
 // ---------------------------------------------------------------- collectives over peer-mapped memory
 constexpr int kCommMaxBlocks = 256;
 // Flag area of one rank: int[2][kCommMaxBlocks][8] (phase, block slot, writing rank), zero-initialised.

@@ -764,3 +764,8 @@ def linear_cross_entropy(h2d, w, labels, ignore_index: int = -100, chunk: int = 
         return _LinearCrossEntropyFn.apply(h2d.contiguous(), w, labels, ignore_index, chunk, sink, param, loss_scale,
                                            torch.is_grad_enabled())
     return ref.linear_cross_entropy(h2d, w, labels, ignore_index)
+
+
+# ------------------------------------------------------------------------------------------- packed documents, token scores
+from .packed import PackedLayout, packed_attention  # noqa: E402
+from .scores import TokenLogProbs, linear_token_log_probs, token_log_probs  # noqa: E402

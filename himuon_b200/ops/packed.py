@@ -1,0 +1,191 @@
+"""Causal attention over documents of different lengths packed into one row of tokens.
+
+A batch of ``n`` documents is one ``(rows, features)`` matrix: document after document, padding (if any) behind the last one.
+:class:`PackedLayout` holds the documents' lengths and the list of 128-token tiles that the sm_100a kernels walk; it is made
+once for a batch and shared by every layer.  Padding rows attend to nothing and are attended by nothing: their output and
+their gradients are zero.
+"""
+
+from __future__ import annotations
+
+import math
+import operator
+
+import numpy as np
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _ext
+from . import _check_width, _count, _warn_torch_path, _with_kernel_rows, use_kernels
+from . import reference as ref
+
+TILE = 128          # tokens of one document that a block of the kernels takes
+
+
+def _tile_plan(lengths: np.ndarray) -> np.ndarray:
+    """``(2, tiles, 4)`` int32: every tile as (first row of its document, length of it, number in the document, number in
+    the batch), in the order of falling work of the passes over a tile's keys and of the pass over its queries."""
+    first = np.concatenate([[0], np.cumsum(lengths)[:-1]]) if lengths.size else lengths
+    per_doc = (lengths + TILE - 1) // TILE
+    doc = np.repeat(np.arange(lengths.size), per_doc)
+    slot = np.arange(doc.size)
+    index = slot - np.repeat(np.cumsum(per_doc) - per_doc, per_doc)
+    tiles = np.stack([first[doc], lengths[doc], index, slot], axis=1)
+    keys = np.minimum((index + 1) * TILE, lengths[doc])
+    queries = lengths[doc] - index * TILE
+    return np.stack([tiles[np.argsort(-keys, kind="stable")], tiles[np.argsort(-queries, kind="stable")]]).astype(np.int32)
+
+
+class PackedLayout:
+    """Where the documents of a packed batch lie.
+
+    ``lengths``: the documents' lengths in tokens, zero included (a sequence of whole numbers, or an integer tensor; one on a
+    GPU is read back, which waits for it).  ``device``: where the batch lives.  The device-side tables are copied without a wait on
+    the stream that is current here; calls on other streams wait for them.
+    """
+
+    def __init__(self, lengths, device="cuda"):
+        if isinstance(lengths, torch.Tensor):
+            if lengths.dim() != 1 or lengths.is_floating_point() or lengths.dtype == torch.bool:
+                raise RuntimeError("himuon_b200.ops.PackedLayout: lengths must be a 1-D integer tensor or a sequence of whole numbers")
+            lengths = lengths.tolist()
+        try:
+            self.lengths = tuple(operator.index(n) for n in lengths)
+        except TypeError as e:
+            raise RuntimeError(f"himuon_b200.ops.PackedLayout: lengths must be whole numbers: {e}") from None
+        if any(n < 0 for n in self.lengths):
+            raise RuntimeError("himuon_b200.ops.PackedLayout: a length is negative")
+        self.tokens = sum(self.lengths)
+        if self.tokens >= 2 ** 30:
+            raise RuntimeError(f"himuon_b200.ops.PackedLayout: {self.tokens} tokens in one batch (2**30 - 1 at most)")
+        self.max_length = max(self.lengths, default=0)
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        lens = np.asarray(self.lengths, dtype=np.int64)
+        self._position = np.arange(self.tokens) - np.repeat(np.cumsum(lens) - lens, lens)
+        self._tables: dict = {}
+        plan = _tile_plan(lens)
+        self.tiles = plan.shape[1]
+        self._table("plan", lambda: plan)
+
+    def _table(self, key, make) -> torch.Tensor:
+        """The device copy of a host table, safe to use on the current stream."""
+        entry = self._tables.get(key)
+        on_gpu = self.device.type == "cuda"
+        if entry is None:
+            host = torch.from_numpy(np.ascontiguousarray(make()))
+            if not on_gpu:
+                entry = (host.to(self.device), None, None)
+            else:
+                stream = torch.cuda.current_stream(self.device)
+                table = host.pin_memory().to(self.device, non_blocking=True)
+                event = torch.cuda.Event()
+                event.record(stream)
+                entry = (table, stream, event)
+            self._tables[key] = entry
+        table, stream, event = entry
+        if on_gpu and not torch.cuda.is_current_stream_capturing():
+            # (a stream that captures a graph has been synchronised with what came before)
+            here = torch.cuda.current_stream(self.device)
+            if here != stream:
+                here.wait_event(event)
+                table.record_stream(here)
+        return table
+
+    @property
+    def plan(self) -> torch.Tensor:
+        return self._table("plan", lambda: _tile_plan(np.asarray(self.lengths, dtype=np.int64)))
+
+    def _check_rows(self, op: str, rows: int) -> None:
+        if rows < self.tokens:
+            raise RuntimeError(f"himuon_b200.ops.{op}: {rows} rows for a layout of {self.tokens} tokens")
+
+    def positions(self, rows: int | None = None) -> torch.Tensor:
+        """Each row's position in its own document (int64), 0 for the padding of a batch of ``rows`` rows."""
+        rows = self.tokens if rows is None else rows
+        self._check_rows("PackedLayout.positions", rows)
+        return self._table(("positions", rows), lambda: np.concatenate([self._position, np.zeros(rows - self.tokens, dtype=np.int64)]))
+
+    def has_next(self, rows: int | None = None) -> torch.Tensor:
+        """Whether a row is followed by a token of its own document."""
+        rows = self.tokens if rows is None else rows
+        self._check_rows("PackedLayout.has_next", rows)
+
+        def make():
+            out = np.zeros(rows, dtype=bool)
+            out[: max(self.tokens - 1, 0)] = self._position[1:] > 0
+            return out
+        return self._table(("has_next", rows), make)
+
+    def next_ids(self, ids: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+        """For each row of a packed ``ids`` the id that follows it in its document, ``ignore_index`` where none does."""
+        flat = ids.reshape(-1)
+        return torch.where(self.has_next(flat.numel()), torch.roll(flat, -1), ignore_index)
+
+    def rope_table(self, cos_sin: torch.Tensor, rows: int | None = None) -> torch.Tensor:
+        """The rows of a rotary table ``(max position, head_dim / 2, 2)`` that the batch's tokens need, one for each row: what
+        :func:`head_norm_rope` takes as the table of one sequence of ``rows`` positions."""
+        if cos_sin.shape[0] < self.max_length:
+            raise RuntimeError(f"himuon_b200.ops.PackedLayout.rope_table: {cos_sin.shape[0]} positions, a document has {self.max_length}")
+        return cos_sin.index_select(0, self.positions(rows))
+
+
+class _PackedAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, layout, Hq, Hkv, scale):
+        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        if q.shape[0] > layout.tokens:
+            o[layout.tokens:].zero_()
+        lse = torch.empty(Hq * layout.tiles * TILE, device=q.device, dtype=torch.float32)
+        if layout.tiles:
+            _ext.ext().packed_attn_fwd(layout.plan, layout.tokens, q, k, v, o, lse, Hq, Hkv, scale)
+            _count()
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.layout, ctx.heads, ctx.scale = layout, (Hq, Hkv), scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        layout, (Hq, Hkv) = ctx.layout, ctx.heads
+        do = _with_kernel_rows(do)
+        D = q.shape[1] // Hq
+        # dq | dk | dv share one buffer, as in attention(): a fused projection sees a single contiguous gradient
+        dqkv = torch.empty(q.shape[0], (Hq + 2 * Hkv) * D, device=q.device, dtype=q.dtype)
+        if q.shape[0] > layout.tokens:
+            dqkv[layout.tokens:].zero_()
+        dq, dk, dv = dqkv[:, : Hq * D], dqkv[:, Hq * D: (Hq + Hkv) * D], dqkv[:, (Hq + Hkv) * D:]
+        if layout.tiles:
+            delta = torch.empty_like(lse)
+            _ext.ext().packed_attn_bwd(layout.plan, layout.tokens, do, q, k, v, o, lse, dq, dk, dv, delta, Hq, Hkv, ctx.scale)
+            _count(2)
+        return dq, dk, dv, None, None, None, None
+
+
+def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, head_dim: int, scale: float | None = None):
+    """Causal GQA attention within each document of a packed batch, on ``(rows, heads*head_dim)`` views (``rows`` at least
+    ``layout.tokens``; rows behind that are padding); returns ``(rows, Hq*head_dim)``.  ``scale`` defaults to
+    ``1/sqrt(head_dim)`` and must be positive.  bf16 CUDA tensors with heads of a multiple of 8 up to 128 run the sm_100a kernels,
+    forward and backward."""
+    if not isinstance(layout, PackedLayout):
+        raise RuntimeError("himuon_b200.ops.packed_attention: layout must be a PackedLayout")
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise RuntimeError(f"himuon_b200.ops.packed_attention: scale must be positive, got {scale}")
+    if Hq <= 0 or Hkv <= 0 or Hq % Hkv:
+        raise RuntimeError(f"himuon_b200.ops.packed_attention: {Hq} query heads over {Hkv}")
+    rows = q2d.shape[0]
+    for t, heads in ((q2d, Hq), (k2d, Hkv), (v2d, Hkv)):
+        if t.dim() != 2 or t.shape[0] != rows or t.device != q2d.device or t.dtype != q2d.dtype:
+            raise RuntimeError("himuon_b200.ops.packed_attention: q, k and v are (rows, heads*head_dim) of one type on one device")
+        _check_width("packed_attention", t, heads * head_dim)
+    layout._check_rows("packed_attention", rows)
+    if layout.device != q2d.device:
+        raise RuntimeError(f"himuon_b200.ops.packed_attention: the layout is on {layout.device}, the tensors on {q2d.device}")
+    if use_kernels(q2d) and head_dim <= 128 and head_dim % 8 == 0:
+        return _PackedAttnFn.apply(*(_with_kernel_rows(t) for t in (q2d, k2d, v2d)), layout, Hq, Hkv, scale)
+    if use_kernels(q2d):
+        _warn_torch_path("packed_attention", f"head_dim {head_dim} (the kernels take multiples of 8 up to 128)")
+    return ref.packed_attention(q2d, k2d, v2d, layout.lengths, Hq, Hkv, head_dim, scale)

@@ -111,3 +111,41 @@ def linear_cross_entropy(h, w, labels, ignore_index=-100):
     """Mean token cross-entropy of ``h @ w.T`` in fp32 (HF ``ForCausalLMLoss`` after the shift)."""
     logits = (h @ w.t()).float()
     return F.cross_entropy(logits, labels, ignore_index=ignore_index, reduction="mean")
+
+
+def packed_attention(q2d, k2d, v2d, lengths, Hq: int, Hkv: int, head_dim: int, scale=None):
+    """Causal attention within each of the documents of ``lengths`` that lie one after the other in ``(rows, heads*head_dim)``
+    views; rows behind the last one are padding, whose output is zero."""
+    parts, first = [], 0
+    for n in lengths:
+        if n:
+            q, k, v = (t[first: first + n].reshape(1, n, -1, head_dim) for t in (q2d, k2d, v2d))
+            parts.append(attention(q, k, v, scale).reshape(n, Hq * head_dim))
+        first += n
+    pad = q2d.shape[0] - first
+    if pad or not parts:
+        # (through an empty slice, so that an empty batch has a gradient as well)
+        parts.append(F.pad(q2d[first:first], (0, 0, 0, pad)))
+    return torch.cat(parts)
+
+
+def token_log_probs(logits, ids, top_k: int = 0, ignore_index: int = -100):
+    """``(log_probs, entropy, top_log_probs, top_ids)`` in fp32 (fp64 for fp64 logits): see ``ops.token_log_probs``."""
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    m = x.detach().amax(-1, keepdim=True)
+    empty = torch.isneginf(m)
+    d = x - torch.where(empty, torch.zeros_like(m), m)
+    e = d.exp()
+    s = torch.where(empty, torch.ones_like(m), e.sum(-1, keepdim=True))
+    t = (e * torch.where(e == 0, torch.zeros_like(d), d)).sum(-1, keepdim=True)
+    lp = d - s.log()
+    entropy = (s.log() - t / s)[:, 0]
+    counted, inside = ids != ignore_index, (ids >= 0) & (ids < x.shape[1])
+    picked = lp.gather(1, torch.where(inside, ids, torch.zeros_like(ids))[:, None])
+    picked = torch.where(empty, picked.detach(), picked)[:, 0]
+    picked = picked.masked_fill(~inside, float("nan"))
+    log_probs = torch.where(counted, picked, torch.zeros_like(picked))
+    if not top_k:
+        return log_probs, entropy, None, None
+    top_ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :top_k].contiguous()
+    return log_probs, entropy, lp.detach().gather(1, top_ids), top_ids

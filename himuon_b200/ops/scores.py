@@ -1,0 +1,151 @@
+"""Log probabilities of given tokens, with the entropy of their distribution and the likeliest alternatives.
+
+:func:`token_log_probs` takes logits, :func:`linear_token_log_probs` hidden states and the head's weight, whose logits it never
+keeps.  Both are differentiable in the log probabilities and the entropy (policy gradients, entropy bonuses, distillation).
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _ext
+from . import _count, gemm, use_kernels
+from . import reference as ref
+
+MAX_TOP_K = 32
+
+
+class TokenLogProbs(NamedTuple):
+    """``log_probs`` and ``entropy``: fp32, one for each row.  ``top_log_probs`` / ``top_ids``: ``(rows, top_k)``, likeliest
+    first, equal ones in the order of their ids; ``None`` without ``top_k``, and not differentiable."""
+
+    log_probs: torch.Tensor
+    entropy: torch.Tensor
+    top_log_probs: torch.Tensor | None = None
+    top_ids: torch.Tensor | None = None
+
+
+def _incoming(g: torch.Tensor | None):
+    return None if g is None else g.to(torch.float32).contiguous()
+
+
+class _TokenLogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, top_k, ignore_index):
+        ctx.set_materialize_grads(False)              # the gradient of an unused output arrives as None
+        rows, dev = logits.shape[0], logits.device
+        log_probs = torch.empty(rows, device=dev, dtype=torch.float32)
+        entropy = torch.empty_like(log_probs)
+        need = ctx.needs_input_grad[0]
+        stats = torch.empty(rows, 2, device=dev, dtype=torch.float32) if need else None
+        top_lp = torch.empty(rows, top_k, device=dev, dtype=torch.float32) if top_k else None
+        top_ids = torch.empty(rows, top_k, device=dev, dtype=torch.int64) if top_k else None
+        if rows:
+            _ext.ext().token_scores_fwd(logits, ids, log_probs, entropy, stats, top_lp, top_ids, ignore_index)
+            _count()
+        if need:
+            ctx.save_for_backward(logits, ids, entropy, stats)
+            ctx.ignore_index = ignore_index
+        if top_k:
+            ctx.mark_non_differentiable(top_lp, top_ids)
+        return log_probs, entropy, top_lp, top_ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_log_probs, g_entropy, *_):
+        if g_log_probs is None and g_entropy is None:
+            return None, None, None, None
+        logits, ids, entropy, stats = ctx.saved_tensors
+        grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        if grad.numel():
+            _ext.ext().token_scores_bwd(logits, ids, entropy, stats, _incoming(g_log_probs), _incoming(g_entropy), grad, ctx.ignore_index)
+            _count()
+        return grad, None, None, None
+
+
+def _check_ids(op: str, ids: torch.Tensor, rows: int, device) -> torch.Tensor:
+    if ids.dtype != torch.int64 or ids.numel() != rows or ids.dim() != 1 or ids.device != device:
+        raise RuntimeError(f"himuon_b200.ops.{op}: ids must be int64, one for each of the {rows} rows, on {device}")
+    return ids.contiguous()
+
+
+def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ignore_index: int = -100) -> TokenLogProbs:
+    """Scores of ``ids`` under the rows of ``(rows, vocab)`` logits.
+
+    A row whose id is ``ignore_index`` has log probability 0 and passes no gradient of it on; its entropy and alternatives
+    are those of the row.  An id outside the vocabulary has log probability NaN and no gradient.  Logits of ``-inf`` are masked tokens; a row of
+    nothing else has log probability ``-inf`` and entropy 0.  At most 32 alternatives.  bf16 and fp32 CUDA logits run the
+    sm_100a kernels.
+    """
+    if logits.dim() != 2 or logits.shape[1] == 0 or not logits.is_floating_point():
+        raise RuntimeError("himuon_b200.ops.token_log_probs: logits must be a (rows, vocab) matrix of floating point")
+    if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[1]):
+        raise RuntimeError(f"himuon_b200.ops.token_log_probs: top_k must lie in 0..{min(MAX_TOP_K, logits.shape[1])}, got {top_k}")
+    ids = _check_ids("token_log_probs", ids, logits.shape[0], logits.device)
+    if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32):
+        if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+            logits = logits.contiguous()
+        return TokenLogProbs(*_TokenLogProbsFn.apply(logits, ids, int(top_k), int(ignore_index)))
+    return TokenLogProbs(*ref.token_log_probs(logits, ids, top_k, ignore_index))
+
+
+class _LinearTokenLogProbsFn(torch.autograd.Function):
+    """Rows in chunks: fp32 logits of a chunk, their scores; the backward pass makes the logits again, turns them into
+    their gradient and multiplies that with both operands."""
+
+    CHUNK = 2 ** 29                                   # logits alive at once
+
+    @staticmethod
+    def forward(ctx, h, w, ids, ignore_index):
+        ctx.set_materialize_grads(False)
+        rows, vocab = h.shape[0], w.shape[0]
+        log_probs = torch.empty(rows, device=h.device, dtype=torch.float32)
+        entropy = torch.empty_like(log_probs)
+        stats = torch.empty(rows, 2, device=h.device, dtype=torch.float32)
+        step = max(128, _LinearTokenLogProbsFn.CHUNK // vocab)
+        for r in range(0, rows, step):
+            c = slice(r, min(rows, r + step))
+            logits = gemm(h[c], w, trans_b=True, out_dtype=torch.float32)
+            _ext.ext().token_scores_fwd(logits, ids[c], log_probs[c], entropy[c], stats[c], None, None, ignore_index)
+            _count()
+        ctx.save_for_backward(h, w, ids, entropy, stats)
+        ctx.ignore_index, ctx.step = ignore_index, step
+        return log_probs, entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_log_probs, g_entropy):
+        if g_log_probs is None and g_entropy is None:
+            return None, None, None, None
+        h, w, ids, entropy, stats = ctx.saved_tensors
+        rows, vocab = h.shape[0], w.shape[0]
+        g, ge = _incoming(g_log_probs), _incoming(g_entropy)
+        dh = torch.empty_like(h)
+        # a sum over several chunks is held in fp32
+        dw = torch.zeros(w.shape, device=w.device, dtype=torch.bfloat16 if rows <= ctx.step else torch.float32)
+        for r in range(0, rows, ctx.step):
+            c = slice(r, min(rows, r + ctx.step))
+            logits = gemm(h[c], w, trans_b=True, out_dtype=torch.float32)
+            dx = torch.empty(logits.shape[0], (vocab + 7) // 8 * 8, device=h.device, dtype=torch.bfloat16)[:, :vocab]
+            _ext.ext().token_scores_bwd(logits, ids[c], entropy[c], stats[c], None if g is None else g[c], None if ge is None else ge[c], dx, ctx.ignore_index)
+            _count()
+            gemm(dx, w, out=dh[c])
+            gemm(dx, h[c], trans_a=True, out=dw, aux=dw if r else None, beta=1.0 if r else 0.0)
+        return dh, dw.to(w.dtype), None, None
+
+
+def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, ignore_index: int = -100) -> TokenLogProbs:
+    """:func:`token_log_probs` of ``h2d @ w.T`` (logits in fp32) for ``(rows, hidden)`` hidden states and a ``(vocab,
+    hidden)`` head, without alternatives.  bf16 CUDA tensors whose hidden size is a multiple of 8 run the sm_100a kernels."""
+    if h2d.dim() != 2 or w.dim() != 2 or h2d.shape[1] != w.shape[1] or w.shape[0] == 0 or h2d.dtype != w.dtype or h2d.device != w.device:
+        raise RuntimeError("himuon_b200.ops.linear_token_log_probs: (rows, hidden) and (vocab, hidden) of one type on one device expected")
+    ids = _check_ids("linear_token_log_probs", ids, h2d.shape[0], h2d.device)
+    if use_kernels(h2d) and h2d.shape[1] % 8 == 0 and h2d.shape[1] > 0:
+        h2d, w = (t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+                  for t in (h2d, w))
+        return TokenLogProbs(*_LinearTokenLogProbsFn.apply(h2d, w, ids, int(ignore_index)))
+    logits = h2d @ w.t() if h2d.dtype in (torch.float32, torch.float64) else h2d.float() @ w.float().t()
+    return TokenLogProbs(*ref.token_log_probs(logits, ids, 0, ignore_index))

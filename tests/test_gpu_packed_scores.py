@@ -1,0 +1,460 @@
+"""Packed attention and token scores on the GPU against 64-bit formulas (GPU tier).
+
+The bounds are element by element and follow from the kernels' roundings: u = 2^-8 is what rounding to bf16 changes a value by
+at most (relative), and each product of rounded factors passes that on through the absolute values of the terms of its sum.
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -8          # bf16
+F = 1e-4               # fp32 sums, exponentials and differences of scores, relative to the terms' absolute values
+
+
+def _ops():
+    from himuon_b200 import ops
+
+    return ops
+
+
+def _clean():
+    from himuon_b200._ext import ext
+
+    torch.cuda.synchronize()
+    assert ext().status(True) == 0, "a bounded device wait ran out (status word set)"
+
+
+def _within(got, want, bound, what):
+    got = got.double()
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    over = (got - want).abs() - bound
+    assert (over <= 0).all(), f"{what}: {(over > 0).sum().item()} of {over.numel()} outside, worst by {over.max().item():.3g}"
+
+
+def _heads(t, hd):
+    return t.detach().double().view(t.shape[0], -1, hd).transpose(0, 1)
+
+
+def _flat(t):
+    return t.transpose(0, 1).reshape(t.shape[1], -1)
+
+
+def _attention64(q, k, v, lengths, Hq, Hkv, hd, scale, do=None):
+    """Results and bounds in 64 bits, one document at a time; zero for padding."""
+    T, G = q.shape[0], Hq // Hkv
+    q, k, v = (_heads(t, hd) for t in (q, k, v))
+    do = None if do is None else _heads(do, hd)
+    out = {n: torch.zeros(h, T, hd, dtype=torch.float64, device=q.device) for n, h in
+           (("o", Hq), ("dq", Hq), ("dk", Hkv), ("dv", Hkv), ("bo", Hq), ("bdq", Hq), ("bdk", Hkv), ("bdv", Hkv))}
+    first = 0
+    for n in lengths:
+        c = slice(first, first + n)
+        first += n
+        if n == 0:
+            continue
+        kk, vv = (t[:, c].repeat_interleave(G, 0) for t in (k, v))
+        qq = q[:, c]
+        s = scale * qq @ kk.transpose(1, 2)
+        p = torch.softmax(s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1), -math.inf), -1)
+        o = p @ vv
+        # P is rounded, and so is the sum of it that it is divided by; then the result
+        bo = U * o.abs() + (2 * U + F) * (p @ vv.abs())
+        out["o"][:, c], out["bo"][:, c] = o, bo
+        if do is None:
+            continue
+        g = do[:, c]
+        dp = g @ vv.transpose(1, 2)
+        delta = (g * o).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        # dS is rounded; delta has been summed from the rounded output
+        bds = U * ds.abs() + p * ((g.abs() * bo).sum(-1, keepdim=True) + F * (g.abs() @ vv.abs().transpose(1, 2) + (g * o).abs().sum(-1, keepdim=True)))
+        per = {"dq": (scale * ds @ kk, scale * bds @ kk.abs()),
+               "dk": (scale * ds.transpose(1, 2) @ qq, scale * bds.transpose(1, 2) @ qq.abs()),
+               "dv": (p.transpose(1, 2) @ g, (U + F) * p.transpose(1, 2) @ g.abs())}
+        for name, (val, bound) in per.items():
+            if name != "dq":
+                val, bound = (t.view(Hkv, G, n, hd).sum(1) for t in (val, bound))
+            out[name][:, c] = val
+            out["b" + name][:, c] = bound + U * (val.abs() + bound)
+    return {n: _flat(t) for n, t in out.items()}
+
+
+SHAPES = [(4, 2, 32), (2, 2, 64), (8, 2, 128), (3, 1, 128), (2, 1, 72), (1, 1, 8), (6, 3, 96)]
+BATCHES = [([1], 0), ([0, 0, 2], 5), ([128], 0), ([127, 1, 0, 64, 65], 7), ([129, 256, 3], 0), ([5, 1, 0, 700, 30, 513], 0), ([1100], 100)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", SHAPES)
+@pytest.mark.parametrize("lengths,pad", BATCHES)
+def test_packed_attention(Hq, Hkv, hd, lengths, pad):
+    ops = _ops()
+    torch.manual_seed(sum(lengths) + hd)
+    T = sum(lengths) + pad
+    q, k, v, do = (torch.randn(T, h * hd, device="cuda").bfloat16() for h in (Hq, Hkv, Hkv, Hq))
+    for t in (q, k, v):
+        t.requires_grad_()
+    layout = ops.PackedLayout(lengths)
+    before = ops.launch_count()
+    o = ops.packed_attention(q, k, v, layout, Hq, Hkv, hd)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
+    assert ops.launch_count() >= before + 3
+    _clean()
+    want = _attention64(q, k, v, lengths, Hq, Hkv, hd, 1 / math.sqrt(hd), do)
+    for name, got in (("o", o), ("dq", dq), ("dk", dk), ("dv", dv)):
+        _within(got, want[name], want["b" + name], name)
+        assert not got[sum(lengths):].any()                        # padding
+
+
+def test_packed_attention_of_peaked_scores_and_another_scale():
+    """Scores whose row maximum keeps growing along the document, so that the running maximum moves in every block."""
+    ops = _ops()
+    torch.manual_seed(3)
+    lengths, Hq, Hkv, hd = [400, 37], 2, 1, 128
+    T = sum(lengths)
+    ramp = torch.linspace(0, 6, T, device="cuda")[:, None]
+    q, k, v, do = (torch.randn(T, h * hd, device="cuda") for h in (Hq, Hkv, Hkv, Hq))
+    q, k = (1 + 0.1 * q).bfloat16().requires_grad_(), (ramp + 0.1 * k).bfloat16().requires_grad_()
+    v, do = v.bfloat16().requires_grad_(), do.bfloat16()
+    o = ops.packed_attention(q, k, v, ops.PackedLayout(lengths), Hq, Hkv, hd, scale=0.25)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    _clean()
+    want = _attention64(q, k, v, lengths, Hq, Hkv, hd, 0.25, do)
+    # a score of up to 200 rounds to 2^-17 in fp32, and e^x passes that on
+    for name, got in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+        _within(got, want[name], want["b" + name], name)
+
+
+def test_packed_attention_gradient_against_differences():
+    """The kernels' gradient along a direction against a central difference of the 64-bit formula."""
+    ops = _ops()
+    torch.manual_seed(5)
+    lengths, Hq, Hkv, hd = [150, 3, 90], 4, 2, 64
+    T = sum(lengths)
+    q, k, v, do = (torch.randn(T, h * hd, device="cuda").bfloat16() for h in (Hq, Hkv, Hkv, Hq))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.packed_attention(*leaves, ops.PackedLayout(lengths), Hq, Hkv, hd), leaves, do)
+    want = _attention64(q, k, v, lengths, Hq, Hkv, hd, hd ** -0.5, do)
+    base = [t.detach().double() for t in leaves]
+    for i, name in enumerate(("dq", "dk", "dv")):
+        d = torch.randn_like(base[i])
+        at = [[b + s * 1e-4 * d if j == i else b for j, b in enumerate(base)] for s in (1, -1)]
+        f = [(_attention64(*x, lengths, Hq, Hkv, hd, hd ** -0.5)["o"] * do.double()).sum().item() for x in at]
+        slope = (f[0] - f[1]) / 2e-4
+        got = (grads[i].double() * d).sum().item()
+        assert abs(got - slope) <= (want["b" + name] * d.abs()).sum().item() + 1e-5 * abs(slope)
+
+
+def test_packed_attention_keeps_documents_apart():
+    """NaN and infinities in one document and in the padding reach no other document, forward or backward."""
+    ops = _ops()
+    torch.manual_seed(7)
+    lengths, pad, Hq, Hkv, hd = [70, 50, 133, 9], 20, 4, 2, 128
+    T = sum(lengths) + pad
+    clean = [torch.randn(T, h * hd, device="cuda").bfloat16() for h in (Hq, Hkv, Hkv, Hq)]
+    bad = [t.clone() for t in clean]
+    for i, t in enumerate(bad):
+        t[70:120] = math.nan if i % 2 else math.inf
+        t[sum(lengths):] = math.nan
+    layout, got = ops.PackedLayout(lengths), []
+    for q, k, v, do in (clean, bad):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        o = ops.packed_attention(*leaves, layout, Hq, Hkv, hd)
+        got.append((o.detach(), *torch.autograd.grad(o, leaves, do)))
+    _clean()
+    others = torch.ones(T, dtype=torch.bool, device="cuda")
+    others[70:120] = False
+    for a, b in zip(*got):
+        assert torch.equal(a[others], b[others])
+
+
+def test_packed_attention_takes_slices_and_odd_rows():
+    """q, k, v as column slices of one projection, rows that start off the 16-byte grid, expanded gradients."""
+    ops = _ops()
+    torch.manual_seed(9)
+    lengths, Hq, Hkv, hd = [40, 200], 4, 2, 64
+    T = sum(lengths)
+    packed = torch.randn(T, (Hq + 2 * Hkv) * hd + 1, device="cuda").bfloat16()
+    layout = ops.PackedLayout(torch.tensor(lengths, device="cuda"))
+    for base in (packed[:, :-1].contiguous(), packed[:, 1:]):
+        q, k, v = base.split([Hq * hd, Hkv * hd, Hkv * hd], 1)
+        q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+        o = ops.packed_attention(q, k, v, layout, Hq, Hkv, hd)
+        grads = torch.autograd.grad(o.sum(), (q, k, v))
+        want = _attention64(q, k, v, lengths, Hq, Hkv, hd, hd ** -0.5, torch.ones(T, Hq * hd, device="cuda"))
+        for name, got in zip(("o", "dq", "dk", "dv"), (o, *grads)):
+            _within(got, want[name], want["b" + name], name)
+    _clean()
+
+
+def test_packed_attention_of_equal_documents_matches_the_unpacked_one():
+    ops = _ops()
+    torch.manual_seed(11)
+    B, S, Hq, Hkv, hd = 3, 256, 4, 2, 128
+    q, k, v = (torch.randn(B * S, h * hd, device="cuda").bfloat16() for h in (Hq, Hkv, Hkv))
+    a = ops.packed_attention(q, k, v, ops.PackedLayout([S] * B), Hq, Hkv, hd)
+    b = ops.attention(q, k, v, B, S, Hq, Hkv, hd)
+    assert (a.float() - b.float()).abs().max() <= 2 * U * (1 + v.float().abs().max())
+    _clean()
+
+
+def test_packed_attention_on_another_stream_and_in_a_graph():
+    ops = _ops()
+    torch.manual_seed(13)
+    lengths, H, hd = [90, 300], 2, 128
+    q, k, v = (torch.randn(390, H * hd, device="cuda").bfloat16() for _ in range(3))
+    layout = ops.PackedLayout(lengths)
+    want = ops.packed_attention(q, k, v, layout, H, H, hd)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = ops.packed_attention(q, k, v, ops.PackedLayout(lengths), H, H, hd)
+        got2 = ops.packed_attention(q, k, v, layout, H, H, hd)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(got2, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.packed_attention(q, k, v, layout, H, H, hd)
+    q.copy_(torch.randn_like(q))
+    graph.replay()
+    assert torch.equal(out, ops.packed_attention(q, k, v, layout, H, H, hd))
+    _clean()
+
+
+def test_packed_attention_repeats_its_bits():
+    ops = _ops()
+    torch.manual_seed(15)
+    lengths, Hq, Hkv, hd = [1000, 24, 600, 300], 8, 2, 128
+    leaves = [torch.randn(sum(lengths), h * hd, device="cuda").bfloat16().requires_grad_() for h in (Hq, Hkv, Hkv)]
+    do = torch.randn(sum(lengths), Hq * hd, device="cuda").bfloat16()
+    layout, seen = ops.PackedLayout(lengths), None
+    for _ in range(5):
+        o = ops.packed_attention(*leaves, layout, Hq, Hkv, hd)
+        got = (o, *torch.autograd.grad(o, leaves, do))
+        assert seen is None or all(torch.equal(a, b) for a, b in zip(seen, got))
+        seen = got
+    _clean()
+
+
+def test_packed_attention_refusals_of_the_kernel_path():
+    ops = _ops()
+    q = torch.randn(4, 64, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError, match="layout is on"):
+        ops.packed_attention(q, q, q, ops.PackedLayout([4], device="cpu"), 2, 2, 32)
+    from himuon_b200._ext import ext
+    plan, lse = ops.PackedLayout([4]).plan, torch.empty(256, device="cuda")
+    ok = (plan, 4, q, q, q, torch.empty_like(q), lse, 2, 2, 0.1)
+    ext().packed_attn_fwd(*ok)
+    for i, bad in [(0, plan.long()), (0, plan[:, :, :2].contiguous()), (0, plan.cpu()), (1, 5), (2, q.float()), (3, q[:, :32]), (4, q[:2]), (5, q.t()),
+                   (6, lse[:128]), (6, lse.double()), (7, 3), (8, 0), (2, torch.randn(5, 64, device="cuda").bfloat16().flatten()[4:260].view(4, 64))]:
+        with pytest.raises(RuntimeError, match="himuon"):
+            ext().packed_attn_fwd(*ok[:i], bad, *ok[i + 1:])
+    _clean()
+
+
+# ------------------------------------------------------------------------------------------- scores
+def _log_tolerance(vocab):
+    """Of a log probability: each thread adds up to vocab / 256 terms (and a row's sum at least one of 1), each exponential is
+    good to 2^-21, d and the result are rounded."""
+    return (vocab / 256 + 64) * 2.0 ** -24 + 2.0 ** -19
+
+
+def _scores64(x, ids, ignore=-100):
+    x = x.double()
+    lp = torch.log_softmax(x, -1)
+    counted = ids != ignore
+    log_probs = lp.gather(1, torch.where(counted, ids, 0)[:, None])[:, 0].masked_fill(~counted, 0.0)
+    entropy = -(lp.exp() * lp.clamp(min=-1e30)).sum(-1)
+    return lp, log_probs, entropy
+
+
+def _grad64(lp, entropy, ids, g, h, ignore=-100):
+    counted = ids != ignore
+    g = (g.double() * counted)[:, None]
+    h = h.double()[:, None]
+    p, l = lp.exp(), lp.clamp(min=-1e30)
+    dx = -p * (g + h * torch.where(p > 0, l + entropy[:, None], 0.0))
+    dx.scatter_add_(1, torch.where(counted, ids, 0)[:, None], g)
+    size = p * (g.abs() + h.abs() * (torch.where(p > 0, l.abs(), 0.0) + entropy[:, None]))
+    return dx, size
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (2, 33), (5, 1000), (40, 4097), (2, 151936), (3, 32003), (700, 2048)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", [0, 3])
+def test_token_log_probs(rows, vocab, dtype, offset):
+    ops = _ops()
+    torch.manual_seed(vocab + rows)
+    wide = (torch.randn(rows, vocab + offset + (8 if offset else 0), device="cuda") * 3).to(dtype)
+    x = wide[:, offset: offset + vocab].detach().requires_grad_()       # an offset: rows of a wider buffer, off the 16-byte grid
+    ids = torch.randint(0, vocab, (rows,), device="cuda")
+    ids[rows // 2] = -100 if rows > 2 else ids[rows // 2]
+    k = min(20, vocab)
+    s = ops.token_log_probs(x, ids, top_k=k)
+    lp, log_probs, entropy = _scores64(x.detach(), ids)
+    tol = _log_tolerance(vocab)
+    _within(s.log_probs, log_probs, tol + 2.0 ** -22 * log_probs.abs(), "log_probs")
+    _within(s.entropy, entropy, 2 * tol * (1 + entropy), "entropy")
+    order = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(s.top_ids, order)
+    _within(s.top_log_probs, lp.gather(1, order), tol + 2.0 ** -22 * lp.gather(1, order).abs(), "top")
+    g, h = torch.randn(rows, device="cuda"), torch.randn(rows, device="cuda")
+    for gg, hh in ((g, h), (g, None), (None, h)):
+        outs = [(o, d) for o, d in ((s.log_probs, gg), (s.entropy, hh)) if d is not None]
+        dx, = torch.autograd.grad([o for o, _ in outs], x, [d for _, d in outs], retain_graph=True)
+        zero = torch.zeros_like(g)
+        want, size = _grad64(lp, entropy, ids, zero if gg is None else gg, zero if hh is None else hh)
+        u = U if dtype == torch.bfloat16 else 2.0 ** -22
+        _within(dx, want, u * want.abs() + (4 * tol * (1 + entropy[:, None]) + 2.0 ** -18) * size + 1e-30, "gradient")
+    again = ops.token_log_probs(x, ids)                                  # without alternatives
+    assert again.top_ids is None and torch.allclose(again.log_probs, s.log_probs, rtol=0, atol=2 * tol + 2.0 ** -21 * 100)
+
+
+def test_token_log_probs_gradient_against_differences():
+    ops = _ops()
+    torch.manual_seed(21)
+    x = (2 * torch.randn(4, 500, device="cuda")).requires_grad_()
+    ids = torch.tensor([0, 499, -100, 77], device="cuda")
+    g, h = torch.randn(4, device="cuda"), torch.randn(4, device="cuda")
+
+    def f(t):
+        s = ops.token_log_probs(t, ids)
+        return (s.log_probs * g + s.entropy * h).sum()
+
+    dx, = torch.autograd.grad(f(x), x)
+    d = torch.randn_like(x)
+    slope = (f(x.detach() + 1e-2 * d).double() - f(x.detach() - 1e-2 * d).double()).item() / 2e-2
+    # values of about 7 to 2^-20 over a step of 2e-2, and the third derivative times 1e-4 / 6
+    assert abs((dx * d).sum().item() - slope) <= 4 * 7 * 2.0 ** -19 / 2e-2 + 1e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_log_probs_of_masks_and_extremes(dtype):
+    """-inf and the type's lowest value as masks, rows with nothing left, ties, ascending rows, one token that has it all, NaN."""
+    ops = _ops()
+    inf, low, V = math.inf, torch.finfo(dtype).min, 5000
+    torch.manual_seed(23)
+    x = torch.randn(9, V, device="cuda").to(dtype)
+    x[0, ::2] = -inf
+    x[1] = -inf
+    x[2, 10:] = low
+    x[3] = low
+    x[4] = 1.5
+    x[5] = torch.linspace(-8, 8, V, device="cuda").to(dtype)
+    x[6, 4321] = 200.0
+    x[7, 4999] = math.nan
+    x[8, 0], x[8, 1], x[8, 2:] = 0.0, -0.0, -1.0
+    x.requires_grad_()
+    ids = torch.tensor([1, 3, 12, 7, 4999, 2500, 4321, 0, 5000], device="cuda")
+    s = ops.token_log_probs(x, ids, top_k=32)
+    want = ops.token_log_probs(x.detach().double().cpu(), ids.cpu(), top_k=32)
+    tol = _log_tolerance(V)
+    assert torch.equal(s.top_ids.cpu(), want.top_ids)
+    for got, w in ((s.log_probs, want.log_probs), (s.entropy, want.entropy), (s.top_log_probs, want.top_log_probs)):
+        got, w = got.double().cpu(), w
+        assert torch.equal(got.isnan(), w.isnan()) and torch.equal(got == -inf, w == -inf)
+        ok = torch.isfinite(w) & (w.abs() < 1e30)
+        assert ((got - w).abs()[ok] <= 2 * tol * (1 + w.abs()[ok])).all()
+        far = torch.isfinite(w) & ~ok                    # a token at the lowest value: as far down as fp32 goes
+        assert ((got / w)[far] - 1).abs().max() <= 1e-6 if far.any() else True
+    keep = torch.tensor([0, 1, 2, 3, 4, 5, 6, 8], device="cuda")
+    g = torch.ones(9, device="cuda")
+    dx, = torch.autograd.grad((s.log_probs, s.entropy), x, (g, g))
+    assert torch.isfinite(dx[keep]).all() and not dx[1].any() and not dx[0, ::2].any() and dx[7].isnan().any()
+    _clean()
+
+
+def test_token_log_probs_refusals_of_the_kernel_path():
+    from himuon_b200._ext import ext
+    x = torch.randn(4, 64, device="cuda")
+    ids = torch.zeros(4, dtype=torch.int64, device="cuda")
+    lp, st = torch.empty(4, device="cuda"), torch.empty(4, 2, device="cuda")
+    top, tid = torch.empty(4, 5, device="cuda"), torch.empty(4, 5, device="cuda", dtype=torch.int64)
+    ok = (x, ids, lp, lp.clone(), st, top, tid, -100)
+    ext().token_scores_fwd(*ok)
+    for i, bad in [(0, x.half()), (0, x.t()), (0, x[:1].expand(4, 64)), (1, ids.int()), (1, ids[:3]), (2, lp[:3]), (3, lp.double()), (4, lp), (5, None), (6, tid[:, :4])]:
+        with pytest.raises(RuntimeError, match="himuon"):
+            ext().token_scores_fwd(*ok[:i], bad, *ok[i + 1:])
+    grad = torch.empty_like(x)
+    ok = (x, ids, lp, st, lp, lp, grad, -100)
+    ext().token_scores_bwd(*ok)
+    for i, bad in [(3, lp), (4, lp[:2]), (5, lp.double()), (6, grad[:2]), (6, grad.half()), (6, grad.t())]:
+        with pytest.raises(RuntimeError, match="himuon"):
+            ext().token_scores_bwd(*ok[:i], bad, *ok[i + 1:])
+
+
+def _logit_error(h, w):
+    """Largest error of a logit: fp32 sums of hidden / 16 steps, relative to the sum of the absolute products."""
+    return (h.shape[1] / 16 + 4) * 2.0 ** -22 * (h.double().abs() @ w.double().abs().t()).max().item()
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [(1, 8, 1), (1, 128, 1000), (8, 256, 5003), (100, 64, 264), (129, 136, 777), (300, 640, 4096), (777, 128, 2050)])
+def test_linear_token_log_probs(rows, hidden, vocab):
+    ops = _ops()
+    torch.manual_seed(rows + vocab)
+    h = torch.randn(rows, hidden, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn(vocab, hidden, device="cuda") * 2 / math.sqrt(hidden)).bfloat16().requires_grad_()
+    ids = torch.randint(0, vocab, (rows,), device="cuda")
+    ids[rows // 2] = -100 if rows > 2 else ids[rows // 2]
+    s = ops.linear_token_log_probs(h, w, ids)
+    g, e = torch.randn(rows, device="cuda"), 0.3 * torch.randn(rows, device="cuda")
+    dh, dw = torch.autograd.grad((s.log_probs, s.entropy), (h, w), (g, e))
+    _clean()
+    hd, wd = h.detach().double(), w.detach().double()
+    lp, log_probs, entropy = _scores64(hd @ wd.t(), ids)
+    dl = _logit_error(h.detach(), w.detach())
+    tol = _log_tolerance(vocab) + 2 * dl
+    _within(s.log_probs, log_probs, tol + 2.0 ** -22 * log_probs.abs(), "log_probs")
+    _within(s.entropy, entropy, 2 * tol * (1 + entropy), "entropy")
+    dx, size = _grad64(lp, entropy, ids, g, e)
+    bx = U * dx.abs() + (4 * tol * (1 + entropy[:, None]) + 2.0 ** -18) * size
+    for got, want, bound, what in ((dh, dx @ wd, bx @ wd.abs(), "dh"), (dw, dx.t() @ hd, bx.t() @ hd.abs(), "dw")):
+        _within(got, want, (1 + U) * bound + U * want.abs() + F * bound + 1e-30, what)
+
+
+def test_linear_token_log_probs_in_chunks(monkeypatch):
+    """Row by row nothing depends on how many rows a call has; the weight's gradient is summed over the chunks."""
+    ops = _ops()
+    from himuon_b200.ops import scores
+
+    torch.manual_seed(31)
+    h = torch.randn(600, 128, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn(1000, 128, device="cuda") * 0.2).bfloat16().requires_grad_()
+    ids = torch.randint(0, 1000, (600,), device="cuda")
+    g = torch.randn(600, device="cuda")
+
+    def both():
+        s = ops.linear_token_log_probs(h, w, ids)
+        return (s.log_probs, s.entropy, *torch.autograd.grad((s.log_probs, s.entropy), (h, w), (g, g)))
+
+    whole = both()
+    monkeypatch.setattr(scores._LinearTokenLogProbsFn, "CHUNK", 256 * 1000)
+    parts = both()
+    for a, b in zip(whole[:3], parts[:3]):
+        assert torch.equal(a, b)
+    # the same fp32 terms in another order, then one rounding
+    assert ((whole[3].float() - parts[3].float()).abs() <= 2 * U * whole[3].float().abs() + 1e-4).all()
+    _clean()
+
+
+def test_linear_token_log_probs_slices_and_partial_gradients():
+    ops = _ops()
+    torch.manual_seed(33)
+    buf = torch.randn(50, 200, device="cuda").bfloat16()
+    h, w = buf[:, 3:131].detach().requires_grad_(), torch.randn(300, 128, device="cuda").bfloat16()
+    ids = torch.randint(0, 300, (50,), device="cuda")
+    s = ops.linear_token_log_probs(h, w, ids)
+    dh, = torch.autograd.grad(s.log_probs.sum(), h)
+    lp, log_probs, entropy = _scores64(h.detach().double() @ w.double().t(), ids)
+    tol = _log_tolerance(300) + 2 * _logit_error(h.detach(), w)
+    _within(s.log_probs, log_probs, tol + 2.0 ** -22 * log_probs.abs(), "log_probs")
+    one, zero = torch.ones(50, device="cuda"), torch.zeros(50, device="cuda")
+    dx, size = _grad64(lp, entropy, ids, one, zero)
+    bound = (U * dx.abs() + (4 * tol + 2.0 ** -18) * size) @ w.double().abs()
+    _within(dh, dx @ w.double(), (1 + U + F) * bound + U * (dx @ w.double()).abs() + 1e-30, "dh")
+    assert ops.linear_token_log_probs(h[:0], w, ids[:0]).log_probs.shape == (0,)
+    with torch.no_grad():
+        assert torch.equal(ops.linear_token_log_probs(h, w, ids).log_probs, s.log_probs)
+    _clean()
