@@ -67,7 +67,7 @@ class Attention(nn.Module):
             self.q_norm = RMSNorm(D, cfg.rms_norm_eps)
             self.k_norm = RMSNorm(D, cfg.rms_norm_eps)
 
-    def forward(self, x2d, B: int, S: int, cos_sin):
+    def forward(self, x2d, B: int, S: int, cos_sin, layout=None):
         cfg = self.cfg
         Hq, Hkv, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         q = self.q_proj(x2d)
@@ -80,9 +80,14 @@ class Attention(nn.Module):
             v = self.v_proj(x2d)
         qw = self.q_norm.weight if cfg.qk_norm else None
         kw = self.k_norm.weight if cfg.qk_norm else None
+        if layout is not None:
+            S = x2d.shape[0]                    # the table has one row for each token of the packed batch
         q = ops.head_norm_rope(q, qw, cos_sin, Hq, S, D, cfg.rms_norm_eps, defer_dw=True, inplace_grad=True)
         k = ops.head_norm_rope(k, kw, cos_sin, Hkv, S, D, cfg.rms_norm_eps, defer_dw=True, inplace_grad=True)
-        o = ops.attention(q, k, v, B, S, Hq, Hkv, D)
+        if layout is not None:
+            o = ops.packed_attention(q, k, v, layout, Hq, Hkv, D)
+        else:
+            o = ops.attention(q, k, v, B, S, Hq, Hkv, D)
         return self.o_proj(o)
 
 
@@ -108,12 +113,12 @@ class DecoderLayer(nn.Module):
         self.input_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
         self.post_attention_layernorm = RMSNorm(cfg.hidden_size, cfg.rms_norm_eps)
 
-    def forward(self, h2d, delta, B: int, S: int, cos_sin):
+    def forward(self, h2d, delta, B: int, S: int, cos_sin, layout=None):
         """``delta`` is the previous block's output that has not been added to the residual stream yet (``None``
         for the first layer): every residual add is fused with the RMSNorm that follows it.  Returns the updated
         stream and this layer's own pending MLP output."""
         h2d, n1 = ops.add_rmsnorm(h2d, delta, self.input_layernorm.weight, self.input_layernorm.variance_epsilon, defer_dw=True)
-        a = self.self_attn(n1, B, S, cos_sin)
+        a = self.self_attn(n1, B, S, cos_sin, layout)
         h2d, n2 = ops.add_rmsnorm(h2d, a, self.post_attention_layernorm.weight,
                                       self.post_attention_layernorm.variance_epsilon, defer_dw=True)
         return h2d, self.mlp(n2)
@@ -174,9 +179,12 @@ class CausalLM(nn.Module):
             self._rope_cache[key] = ref.rope_tables(S, self.config.head_dim, self.config.rope_theta, device=device)
         return self._rope_cache[key]
 
-    def hidden_states(self, input_ids):
+    def hidden_states(self, input_ids, layout: ops.PackedLayout | None = None):
         B, S = input_ids.shape
-        cos_sin = self._rope(S, input_ids.device)
+        if layout is not None:
+            cos_sin = layout.rope_table(self._rope(max(layout.max_length, 1), input_ids.device), B * S)
+        else:
+            cos_sin = self._rope(S, input_ids.device)
         h = ops.embedding(input_ids, self.model.embed_tokens.weight).reshape(B * S, -1)
         delta = None
         # an engine that stages weights or reduces gradients per layer group is told where the layer loop stands
@@ -186,23 +194,31 @@ class CausalLM(nn.Module):
             if fenced:
                 h, delta = engine.pre_layer(i, h, delta)
             if self.gradient_checkpointing and self.training and torch.is_grad_enabled():
-                h, delta = checkpoint(layer, h, delta, B, S, cos_sin, use_reentrant=False)
+                h, delta = checkpoint(layer, h, delta, B, S, cos_sin, layout, use_reentrant=False)
             else:
-                h, delta = layer(h, delta, B, S, cos_sin)
+                h, delta = layer(h, delta, B, S, cos_sin, layout)
             if fenced:
                 h, delta = engine.post_layer(i, h, delta)
         return ops.add_rmsnorm(h, delta, self.model.norm.weight, self.model.norm.variance_epsilon, defer_dw=True)[1]
 
-    def forward(self, input_ids, attention_mask=None, labels=None, return_logits: bool = False, **_):
+    def forward(self, input_ids, attention_mask=None, labels=None, return_logits: bool = False,
+                layout: ops.PackedLayout | None = None, **_):
         """Causal LM forward.  With ``labels`` the shifted mean token cross-entropy is returned as
         ``.loss`` and, unless ``return_logits`` is set, logits are never materialised.  ``attention_mask``
-        is accepted for API compatibility; attention is causal and padding is not masked."""
+        is accepted for API compatibility; attention is causal and padding is not masked.
+
+        ``layout``: the rows of ``input_ids``, one after the other, are a packed batch of documents of these lengths
+        (whatever their shape; ``(1, rows)`` as a rule) with padding behind them.  A document sees itself alone, its positions start
+        at 0, and neither its last token nor padding has a label."""
         B, S = input_ids.shape
-        h = self.hidden_states(input_ids)
+        h = self.hidden_states(input_ids, layout)
         loss, logits = None, None
         if labels is not None:
-            shifted = torch.full_like(labels, -100)
-            shifted[:, :-1] = labels[:, 1:]
+            if layout is not None:
+                shifted = layout.next_ids(labels)
+            else:
+                shifted = torch.full_like(labels, -100)
+                shifted[:, :-1] = labels[:, 1:]
             head = self._head_weight()
             # in-forward accumulation of the head's weight gradient only when a backward pass follows this forward
             scale = self.loss_scale if (self.training and torch.is_grad_enabled()) else None
@@ -210,6 +226,13 @@ class CausalLM(nn.Module):
         if labels is None or return_logits:
             logits = ops.linear(h, self._head_weight()[0]).view(B, S, -1)
         return CausalLMOutput(loss=loss, logits=logits)
+
+    def score(self, input_ids, layout: ops.PackedLayout) -> ops.TokenLogProbs:
+        """Scores the tokens of a packed batch (see ``forward``) under the model: for each row, in the order of
+        ``input_ids.reshape(-1)``, the log probability of the token that follows it in its document (0 where none does) and the entropy
+        of what was predicted there.  Differentiable in both; logits are never kept."""
+        h = self.hidden_states(input_ids, layout)
+        return ops.linear_token_log_probs(h, self._head_weight()[0], layout.next_ids(input_ids))
 
     def _head_weight(self):
         return self.lm_head.weight, None

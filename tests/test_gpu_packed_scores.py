@@ -458,3 +458,41 @@ def test_linear_token_log_probs_slices_and_partial_gradients():
     with torch.no_grad():
         assert torch.equal(ops.linear_token_log_probs(h, w, ids).log_probs, s.log_probs)
     _clean()
+
+
+# ------------------------------------------------------------------------------------------- together, in a model
+@pytest.mark.parametrize("model_type,head_dim", [("qwen3", 128), ("llama", 64)])
+def test_model_scores_of_a_packed_batch(model_type, head_dim):
+    """Packed scores and their gradients on the kernels against the fp32 model on plain operators."""
+    import copy
+
+    ops = _ops()
+    from himuon_b200.models import CausalLM, DecoderConfig
+
+    torch.manual_seed(0)
+    cfg = DecoderConfig(model_type=model_type, vocab_size=2048, hidden_size=256, intermediate_size=512, num_hidden_layers=2,
+                        num_attention_heads=4, num_key_value_heads=2, head_dim=head_dim, rms_norm_eps=1e-6, rope_theta=10000.0,
+                        tie_word_embeddings=model_type == "qwen3", max_position_embeddings=512)
+    plain = CausalLM(cfg).cuda().float()
+    fast = copy.deepcopy(plain).bfloat16()
+    with torch.no_grad():
+        for a, b in zip(plain.parameters(), fast.parameters()):
+            a.copy_(b.float())
+    lengths, pad = [200, 1, 0, 77, 130], 4
+    ids = torch.randint(0, 2048, (1, sum(lengths) + pad), device="cuda")
+    layout = ops.PackedLayout(lengths)
+    advantage = torch.randn(ids.numel(), device="cuda")
+    outs = []
+    for model in (plain, fast):
+        s = model.score(ids, layout)
+        (-(s.log_probs * advantage).sum() / ids.numel() - 0.01 * s.entropy[: sum(lengths)].mean()).backward()
+        outs.append((s, model(ids, labels=ids, layout=layout).loss.item()))
+    _clean()
+    (a, loss_a), (b, loss_b) = outs
+    # bf16 activations through two layers, as in the equal-length model's test
+    assert abs(loss_a - loss_b) < 3e-2
+    assert (a.log_probs - b.log_probs).abs().mean() < 3e-2 and (a.entropy - b.entropy).abs().mean() < 3e-2
+    for (n, p), q in zip(plain.named_parameters(), fast.parameters()):
+        x, y = p.grad.flatten(), q.grad.float().flatten()
+        assert torch.dot(x, y) / (x.norm() * y.norm() + 1e-12) > 0.99, n
+        assert abs(y.norm() / (x.norm() + 1e-12) - 1) < 0.05, n

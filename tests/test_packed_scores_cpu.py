@@ -157,3 +157,61 @@ def test_token_log_probs_refuses():
             ops.linear_token_log_probs(*args)
     s = ops.token_log_probs(x[:0], ids[:0], top_k=2)
     assert s.log_probs.shape == (0,) and s.top_ids.shape == (0, 2)
+
+
+# ------------------------------------------------------------------------------------------- a model's packed batches
+def _model(model_type="qwen3"):
+    from himuon_b200.models import CausalLM, DecoderConfig
+
+    torch.manual_seed(0)
+    return CausalLM(DecoderConfig(model_type=model_type, vocab_size=64, hidden_size=32, intermediate_size=64, num_hidden_layers=2,
+                                  num_attention_heads=4, num_key_value_heads=2, head_dim=16, rms_norm_eps=1e-6, rope_theta=1e4,
+                                  tie_word_embeddings=model_type == "qwen3", max_position_embeddings=64))
+
+
+@pytest.mark.parametrize("model_type", ["qwen3", "llama"])
+@pytest.mark.parametrize("checkpointing", [False, True])
+def test_a_packed_batch_is_its_documents_one_by_one(model_type, checkpointing):
+    model = _model(model_type).train()
+    if checkpointing:
+        model.gradient_checkpointing_enable()
+    lengths, pad = [5, 0, 1, 9], 3
+    ids = torch.randint(0, 64, (1, sum(lengths) + pad))
+    layout = ops.PackedLayout(lengths, device="cpu")
+    out = model(ids, labels=ids, layout=layout, return_logits=True)
+    score = model.score(ids, layout)
+    out.loss.backward()
+    grads = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    total, count, first = 0.0, 0, 0
+    for n in lengths:
+        part = ids[:, first: first + n]
+        if n:
+            one = model(part, labels=part, return_logits=True)
+            assert torch.allclose(out.logits[:, first: first + n], one.logits, atol=1e-5)
+        if n > 1:
+            total, count = total + one.loss * (n - 1), count + n - 1
+            lp = torch.log_softmax(one.logits[0, :-1].float(), -1)
+            assert torch.allclose(score.log_probs[first: first + n - 1], lp.gather(1, part[0, 1:, None])[:, 0], atol=1e-5)
+            assert torch.allclose(score.entropy[first: first + n - 1], -(lp.exp() * lp).sum(-1), atol=1e-5)
+        if n:
+            assert score.log_probs[first + n - 1] == 0
+        first += n
+    assert not score.log_probs[first:].any()
+    assert torch.allclose(out.loss, total / count, atol=1e-6)
+    (total / count).backward()
+    for n, p in model.named_parameters():
+        assert torch.allclose(grads[n], p.grad, atol=1e-6), n
+
+
+def test_scores_of_a_model_train_it():
+    """The gradient of the mean negative log probability is that of the loss."""
+    model = _model()
+    ids = torch.randint(0, 64, (1, 20))
+    layout = ops.PackedLayout([12, 8], device="cpu")
+    model(ids, labels=ids, layout=layout).loss.backward()
+    want = [p.grad.clone() for p in model.parameters()]
+    model.zero_grad()
+    (-model.score(ids, layout).log_probs.sum() / 18).backward()
+    for a, p in zip(want, model.parameters()):
+        assert torch.allclose(a, p.grad, atol=1e-6)
