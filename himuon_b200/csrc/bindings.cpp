@@ -389,6 +389,54 @@ static void token_scores_bwd(const at::Tensor& logits, const at::Tensor& ids, co
   himuon::token_scores_bwd(a, cur_stream());
 }
 
+static himuon::LinearScoreArgs linear_score_args(const char* op, const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, const at::Tensor& entropy,
+                                                 const c10::optional<at::Tensor>& stats, int64_t ignore_index) {
+  const std::string at = std::string("himuon: ") + op;
+  TORCH_CHECK(h.is_cuda() && w.device() == h.device() && is_bf16(h) && is_bf16(w) && h.dim() == 2 && w.dim() == 2 && h.size(1) == w.size(1), at, ": (rows, hidden) and (vocab, hidden) bf16 expected");
+  TORCH_CHECK(h.size(0) > 0 && w.size(0) > 0 && h.size(1) > 0 && h.size(1) % 8 == 0 && h.size(0) < (1LL << 30) && w.size(0) < (1LL << 30) && h.size(1) < (1LL << 30),
+              at, ": rows, vocabulary and a hidden size of a multiple of 8 expected");
+  for (const at::Tensor* t : {&h, &w})
+    TORCH_CHECK(t->stride(1) == 1 && t->stride(0) % 8 == 0 && (t->size(0) <= 1 || t->stride(0) >= t->size(1)) && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
+                at, ": rows must have unit inner stride and start on 16-byte boundaries");
+  TORCH_CHECK(ids.device() == h.device() && ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == h.size(0), at, ": one int64 id for each row");
+  TORCH_CHECK(entropy.device() == h.device() && is_f32(entropy) && entropy.is_contiguous() && entropy.numel() == h.size(0), at, ": entropy must be fp32, one for each row");
+  himuon::LinearScoreArgs a{};
+  a.h = h.data_ptr(); a.w = w.data_ptr(); a.ld_h = h.stride(0); a.ld_w = w.stride(0);
+  a.rows = static_cast<int>(h.size(0)); a.hidden = static_cast<int>(h.size(1)); a.vocab = static_cast<int>(w.size(0));
+  a.ids = reinterpret_cast<const long long*>(ids.data_ptr<int64_t>()); a.ignore = ignore_index;
+  a.entropy = entropy.data_ptr<float>();
+  if (stats.has_value()) {
+    TORCH_CHECK(stats->device() == h.device() && is_f32(*stats) && stats->is_contiguous() && stats->numel() == 2 * a.rows, at, ": stats must be fp32, two for each row");
+    a.stats = stats->data_ptr<float>();
+  }
+  return a;
+}
+static void linear_scores_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, at::Tensor& log_probs, at::Tensor& entropy,
+                              const c10::optional<at::Tensor>& stats, at::Tensor& scratch, int64_t ignore_index) {
+  himuon::LinearScoreArgs a = linear_score_args("linear_scores_fwd", h, w, ids, entropy, stats, ignore_index);
+  HM_CHECK(log_probs.device() == h.device() && is_f32(log_probs) && log_probs.is_contiguous() && log_probs.numel() == a.rows, "linear_scores_fwd: log_probs must be fp32, one for each row");
+  HM_CHECK(scratch.device() == h.device() && is_f32(scratch) && scratch.is_contiguous() && scratch.numel() >= himuon::linear_scores_scratch(a.rows, a.vocab), "linear_scores_fwd: scratch too small");
+  a.log_probs = log_probs.data_ptr<float>();
+  a.scratch = scratch.data_ptr<float>();
+  const c10::cuda::CUDAGuard guard(h.device());
+  himuon::linear_scores_fwd(a, cur_stream());
+}
+static void linear_scores_dlogits(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, const at::Tensor& entropy, const at::Tensor& stats,
+                                  const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy, at::Tensor& grad,
+                                  int64_t ignore_index) {
+  himuon::LinearScoreArgs a = linear_score_args("linear_scores_dlogits", h, w, ids, entropy, stats, ignore_index);
+  for (const auto* g : {&g_log_probs, &g_entropy})
+    if (g->has_value()) HM_CHECK((*g)->device() == h.device() && is_f32(**g) && (*g)->is_contiguous() && (*g)->numel() == a.rows, "linear_scores_dlogits: incoming gradients must be fp32, one for each row");
+  // (whole 16-byte groups of columns are written: the row stride covers them)
+  HM_CHECK(grad.device() == h.device() && is_bf16(grad) && grad.dim() == 2 && grad.size(0) == a.rows && grad.size(1) == (a.vocab + 7) / 8 * 8 && grad.is_contiguous() &&
+               reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0, "linear_scores_dlogits: the gradient must be contiguous bf16, its columns rounded up to a multiple of 8");
+  a.g_log_probs = g_log_probs.has_value() ? g_log_probs->data_ptr<float>() : nullptr;
+  a.g_entropy = g_entropy.has_value() ? g_entropy->data_ptr<float>() : nullptr;
+  a.grad = grad.data_ptr(); a.ld_grad = grad.stride(0);
+  const c10::cuda::CUDAGuard guard(h.device());
+  himuon::linear_scores_dlogits(a, cur_stream());
+}
+
 static bool ns5_fused_supported(int64_t m, int64_t n) { return himuon::ns5_fused_supported((int)m, (int)n); }
 static void ns5_fused(const at::Tensor& x, at::Tensor& out, int64_t steps, double eps, bool normalize) {
   HM_CHECK(x.is_cuda() && is_bf16(x) && is_bf16(out) && x.is_contiguous() && out.is_contiguous() && x.dim() == 3 && x.sizes() == out.sizes(), "ns5_fused: contiguous (B, m, n) bf16 tensors");
@@ -476,6 +524,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("packed_attn_bwd", &packed_attn_bwd);
   m.def("token_scores_fwd", &token_scores_fwd);
   m.def("token_scores_bwd", &token_scores_bwd);
+  m.def("linear_scores_fwd", &linear_scores_fwd);
+  m.def("linear_scores_dlogits", &linear_scores_dlogits);
+  m.def("linear_scores_scratch", [](int64_t rows, int64_t vocab) { return himuon::linear_scores_scratch(rows, (int)vocab); });
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("flash_attn_bwd", &flash_attn_bwd);
   m.def("ns5_fused_supported", &ns5_fused_supported);

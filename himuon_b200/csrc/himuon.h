@@ -192,6 +192,21 @@ struct TokenScoreArgs {
 void token_scores_fwd(const TokenScoreArgs& a, cudaStream_t s);
 void token_scores_bwd(const TokenScoreArgs& a, cudaStream_t s);
 
+// The same from hidden states (rows, hidden) and the head's weight (vocab, hidden), bf16, hidden a multiple of 8, row strides of
+// multiples of 8; logits stay on the chip (linear_scores_sm100.cu).  scratch: linear_scores_scratch() floats, forward only.
+// linear_scores_dlogits writes the logits' gradient, (rows, vocab) bf16 with row stride ld_grad, a multiple of 8 of at least vocab.
+struct LinearScoreArgs {
+  const void* h; const void* w;
+  long long ld_h, ld_w; int rows, hidden, vocab;
+  const long long* ids; long long ignore;
+  float* log_probs; float* entropy; float* stats; float* scratch;
+  const float* g_log_probs; const float* g_entropy;
+  void* grad; long long ld_grad;
+};
+long long linear_scores_scratch(long long rows, int vocab);
+void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s);
+void linear_scores_dlogits(const LinearScoreArgs& a, cudaStream_t s);
+
 // ---------------------------------------------------------------- collectives over peer-mapped memory
 constexpr int kCommMaxBlocks = 256;
 // Flag area of one rank: int[2][kCommMaxBlocks][8] (phase, block slot, writing rank), zero-initialised.

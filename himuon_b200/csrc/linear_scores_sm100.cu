@@ -1,0 +1,352 @@
+// Log probability of given tokens and entropy straight from hidden states and the head's weight, and the gradient of the logits
+// that they never were: a bf16 product on CTA pairs whose epilogue takes the fp32 accumulator's columns for what they are.
+//
+//   forward:   x = h W^T tile by tile; of each row of a tile only m = max x, s = sum e^(x-m), t = sum (x-m) e^(x-m) leave the kernel
+//              (and the logit of the row's own token); linear_scores_join_kernel merges a row's tiles (formulas in token_scores.cu).
+//   gradient:  the same product again, whose epilogue turns x into dx_j = g [j = y] - p_j (g + h (log p_j + H)) and stores it as bf16,
+//              the operand of the products dx W and dx^T h that follow.
+//
+// The product is the pair GEMM's (gemm2_sm100.cu has its protocol): 256 rows by BN vocabulary entries per pair, six stages of 64 along
+// the hidden size, two accumulators, so that the epilogue of one tile runs beside the products of the next.  The tiles of one
+// vocabulary block are neighbours in the schedule: its rows of W come from memory once, the hidden states from the L2.
+#include <stdint.h>
+
+#include "gemm_epilogue.cuh"
+#include "himuon.h"
+#include "pair_common.cuh"
+#include "sm100_common.cuh"
+#include "tma_host.h"
+#include "token_scores.cuh"
+
+namespace himuon {
+
+namespace {
+
+constexpr int LS_THREADS = 384;      // warps 0-3: TMA, MMA, TMEM allocation, none; 4-11: epilogue, two groups of four
+constexpr int LS_STAGES = 6;
+constexpr uint32_t LS_A = BM * BK * 2, LS_STAGE = 2 * LS_A;      // 128 rows of h, and up to 128 of W, a CTA
+
+struct LinScoresDev {
+  const long long* ids;
+  float* part;                       // forward: m, s and t of each (part of the vocabulary, row), in three blocks of n_parts * rows
+  float* target;                     // forward: the logit of each row's own id
+  const float2* stats;               // gradient: as row_grad() takes them
+  const float* entropy;
+  const float* g_log_probs;
+  const float* g_entropy;
+  long long ignore;
+  int rows, vocab, tiles_m, tiles_n, kblocks, bn;
+  int* status;
+};
+
+}  // namespace
+
+template <bool GRAD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LS_THREADS, 1)
+linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmD,
+                     LinScoresDev p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_up_1024(smem_raw);
+  uint8_t* slabs = smem + LS_STAGES * LS_STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(slabs + (GRAD ? 2 * SLAB_BYTES : 0));
+  uint64_t* empty = full + LS_STAGES;
+  uint64_t* tfull = empty + LS_STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id(), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < LS_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 16); }     // eight epilogue warps in each CTA
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 2) tmem_alloc2(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                // the peer's barriers exist before anything signals them
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, total = p.tiles_m * p.tiles_n;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    const uint32_t e = elect_one();
+    tma_prefetch_desc(&tmH);
+    tma_prefetch_desc(&tmW);
+    const uint32_t bytes = 2 * (LS_A + p.bn / 2 * BK * 2);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < total; tile += n_pairs) {
+      const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
+      const int n0 = nt * p.bn + static_cast<int>(rank) * (p.bn / 2);
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
+        uint8_t* sA = smem + stage * LS_STAGE;
+        mbar_expect_tx(&full[stage], bytes, leader ? e : 0);
+        tma2_load_3d(sA, &tmH, &full[stage], kb * BK, m0, 0, e);
+        tma2_load_3d(sA + LS_A, &tmW, &full[stage], kb * BK, n0, 0, e);
+        if (++stage == LS_STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader CTA only)
+    if (leader) {
+      const uint32_t e = elect_one();
+      const uint32_t idesc = umma_idesc_bf16(2 * BM, p.bn, false, false);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < total; tile += n_pairs) {
+        if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1, abort_flag, p.status, 2)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (!mbar_wait_warp(&full[stage], phase, abort_flag, p.status, 2)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(smem + stage * LS_STAGE);
+          const uint64_t a_desc = umma_smem_desc(a_base, 16, 1024), b_desc = umma_smem_desc(a_base + LS_A, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma2_ss(d_tmem, desc_at(a_desc, k * 32), desc_at(b_desc, k * 32), idesc, (kb > 0 || k > 0) ? 1u : 0u, e);
+          const uint32_t e_addr = smem_u32(&empty[stage]);
+          umma2_commit(e_addr, e);                  // this CTA's producer
+          umma2_commit(map_to_cta(e_addr, 1), e);   // the peer's producer
+          if (++stage == LS_STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        const uint32_t f_addr = smem_u32(&tfull[acc]);
+        umma2_commit(f_addr, e);
+        umma2_commit(map_to_cta(f_addr, 1), e);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue (both CTAs, own 128 accumulator rows, one a thread)
+    const int ew = warp & 3, group = (warp - 4) >> 2;
+    const uint32_t tempty_lead = map_to_cta(smem_u32(tempty), 0);
+    const bool issuer = ew == 0 && lane == 0;
+    uint8_t* slab = slabs + group * SLAB_BYTES;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int tile = first; tile < total; tile += n_pairs) {
+      const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
+      const int row = m0 + ew * 32 + lane, n0 = nt * p.bn;
+      const bool row_ok = row < p.rows;
+      RowGrad rg{};
+      long long id = -1;
+      if constexpr (GRAD) {
+        if (row_ok) rg = row_grad(p.stats, p.entropy, p.ids, p.g_log_probs, p.g_entropy, p.ignore, p.vocab, row);
+      } else {
+        if (row_ok) id = p.ids[row];
+      }
+      // the 128 threads of a group meet on named barriers below, so they also leave together when the wait runs out
+      if (!named_barrier_and(1 + 2 * group, 128, mbar_wait(&tfull[acc], acc_phase, abort_flag, p.status, 3))) break;
+      tc_fence_after();
+      const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * 256);
+      if constexpr (!GRAD) {
+        Sums a{-INFINITY, 0.f, 0.f};
+#pragma unroll 1
+        for (int c = group * 32; c < p.bn; c += 64) {
+          if (n0 + c >= p.vocab) break;                       // uniform over the group
+          uint32_t v[32];
+          float x[32];
+          tmem_ld32(t_acc + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = n0 + c + j < p.vocab ? __uint_as_float(v[j]) : -INFINITY;
+          take<32>(a, x, largest<32>(x));
+          const long long at = id - (n0 + c);
+          if (at >= 0 && at < 32 && id < p.vocab) {           // a row's own token: in one of its tiles
+            float mine = x[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) mine = at == j ? x[j] : mine;
+            p.target[row] = mine;
+          }
+        }
+        if (row_ok) {
+          const long long n = static_cast<long long>(p.tiles_n) * 2 * p.rows, i = (static_cast<long long>(nt) * 2 + group) * p.rows + row;
+          p.part[i] = a.m;
+          p.part[n + i] = a.s;
+          p.part[2 * n + i] = a.t;
+        }
+      } else if (m0 < p.rows) {                               // uniform: the second CTA of a ragged last row block has nothing to store
+        uint8_t* my_row = slab + (ew * 32 + lane) * 128;
+#pragma unroll 1
+        for (int c = group * 64; c < p.bn; c += 128) {
+          const int col = n0 + c;
+          if (col >= p.vocab) break;
+          uint32_t o[32];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t v[32];
+            tmem_ld32(t_acc + c + half * 32, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2)
+              o[half * 16 + j / 2] = pack_bf16x2(grad_of(rg, __uint_as_float(v[j]), col + half * 32 + j), grad_of(rg, __uint_as_float(v[j + 1]), col + half * 32 + j + 1));
+          }
+          if (issuer) tma_store_wait_read<0>();
+          named_barrier(1 + 2 * group, 128);                  // the slab is free
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(my_row + ((j ^ (lane & 7)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          fence_proxy_async_smem();
+          named_barrier(2 + 2 * group, 128);                  // the slab is complete
+          if (issuer) {
+            tma_store_3d(&tmD, slab, col, m0, 0);
+            tma_store_commit();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(tempty_lead + acc * 8);
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (GRAD && issuer) tma_store_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                  // neither CTA leaves while the other may still signal or read it
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc2(tmem_base, 512);
+  }
+}
+
+// Merges the parts of RB rows per block (RB neighbouring rows are neighbours in memory), in the same order on every run.
+template <int RB>
+__global__ void __launch_bounds__(256)
+linear_scores_join_kernel(LinScoresDev p, int n_parts, float* log_probs, float* entropy, float2* stats) {
+  constexpr int W = 256 / RB;
+  __shared__ Sums s_sums[256];
+  const int r = threadIdx.x % RB, w = threadIdx.x / RB;
+  const long long row = static_cast<long long>(blockIdx.x) * RB + r;
+  Sums a{-INFINITY, 0.f, 0.f};
+  if (row < p.rows) {
+    const long long n = static_cast<long long>(n_parts) * p.rows;
+#pragma unroll 4
+    for (int i = w; i < n_parts; i += W) {
+      const float* src = p.part + static_cast<long long>(i) * p.rows + row;
+      a = merged(a, Sums{src[0], src[n], src[2 * n]});
+    }
+  }
+  s_sums[threadIdx.x] = a;
+  for (int o = W / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (w < o) s_sums[threadIdx.x] = a = merged(a, s_sums[threadIdx.x + o * RB]);
+  }
+  if (w == 0 && row < p.rows) {
+    const RowScore s = row_score(a);
+    const long long id = p.ids[row];
+    float lp = 0.f;
+    if (id != p.ignore) lp = id >= 0 && id < p.vocab ? (p.target[row] - s.m) - s.log_s : nan_f();
+    log_probs[row] = lp;
+    entropy[row] = s.entropy;
+    if (stats) stats[row] = make_float2(s.m, s.log_s);
+  }
+}
+
+static CUtensorMap rows_tmap(const void* ptr, int rows, int cols, long long ld, int box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), 1};
+  const uint64_t strides[2] = {static_cast<uint64_t>(ld) * 2, static_cast<uint64_t>(ld) * 2 * static_cast<uint64_t>(rows)};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(box_rows), 1};
+  return make_tmap(ptr, 3, dims, strides, box, 2, true);
+}
+
+static int pairs_at_once(size_t smem) {
+  static int most = 0;
+  if (most == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(num_sms());
+    cfg.blockDim = dim3(LS_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, linear_scores_kernel<true>, &cfg) == cudaSuccess && n > 0) most = n;
+    else { cudaGetLastError(); most = num_sms() / 2; }
+  }
+  return most;
+}
+
+// Vocabulary entries per tile.  With one block of rows the weight's bytes bound the call and the last round of tiles counts: the
+// width that needs the fewest of them in sum.  (More rows: 256, the least operand traffic for a product.)
+static int tile_width(int rows, int vocab, int pairs) {
+  if (rows > 2 * BM) return 256;
+  int best = 256;
+  long long least = -1;
+  for (int bn = 256; bn >= 128; bn -= 64) {
+    const long long cost = ((vocab + bn - 1) / bn + pairs - 1) / pairs * static_cast<long long>(bn);
+    if (least < 0 || cost < least) { least = cost; best = bn; }
+  }
+  return best;
+}
+
+template <bool GRAD>
+static void launch(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s) {
+  constexpr size_t SMEM = 1024 + LS_STAGES * LS_STAGE + 2 * SLAB_BYTES + 256;
+  static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
+  for (auto k : {linear_scores_kernel<false>, linear_scores_kernel<true>}) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
+    if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores: ") + cudaGetErrorString(e));
+  }
+  const int pairs = pairs_at_once(SMEM);
+  p.bn = GRAD ? 256 : tile_width(p.rows, p.vocab, pairs);
+  p.tiles_m = (p.rows + 2 * BM - 1) / (2 * BM);
+  p.tiles_n = (p.vocab + p.bn - 1) / p.bn;
+  p.kblocks = (a.hidden + BK - 1) / BK;
+  const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
+  if (total >= (1LL << 30)) throw std::runtime_error("himuon linear_scores: too many tiles for one launch");
+  const CUtensorMap th = rows_tmap(a.h, a.rows, a.hidden, a.ld_h, BM), tw = rows_tmap(a.w, a.vocab, a.hidden, a.ld_w, p.bn / 2),
+                    td = GRAD ? rows_tmap(a.grad, a.rows, static_cast<int>(a.ld_grad), a.ld_grad, BM) : th;
+  const int grid = 2 * static_cast<int>(total < pairs ? total : pairs);
+  linear_scores_kernel<GRAD><<<grid, LS_THREADS, SMEM, s>>>(th, tw, td, p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores launch failed: ") + cudaGetErrorString(e));
+}
+
+static LinScoresDev make_dev(const LinearScoreArgs& a) {
+  if (a.rows <= 0 || a.vocab <= 0 || a.hidden <= 0 || a.hidden % 8) throw std::runtime_error("himuon linear_scores: bad sizes");
+  LinScoresDev p{};
+  p.ids = a.ids; p.ignore = a.ignore;
+  p.rows = a.rows; p.vocab = a.vocab;
+  p.part = a.scratch + a.rows; p.target = a.scratch;
+  p.stats = reinterpret_cast<const float2*>(a.stats);
+  p.entropy = a.entropy;
+  p.g_log_probs = a.g_log_probs; p.g_entropy = a.g_entropy;
+  p.status = status_word_ptr();
+  return p;
+}
+
+// For the narrowest tiles, so that it does not depend on the GPU.
+long long linear_scores_scratch(long long rows, int vocab) { return rows * (1 + 3LL * 2 * ((vocab + 127) / 128)); }
+
+void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {
+  LinScoresDev p = make_dev(a);
+  launch<false>(a, p, s);
+  const int n_parts = 2 * p.tiles_n;
+  float2* stats = reinterpret_cast<float2*>(a.stats);
+  if (a.rows < 512) linear_scores_join_kernel<1><<<a.rows, 256, 0, s>>>(p, n_parts, a.log_probs, a.entropy, stats);
+  else linear_scores_join_kernel<8><<<(a.rows + 7) / 8, 256, 0, s>>>(p, n_parts, a.log_probs, a.entropy, stats);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores join launch failed: ") + cudaGetErrorString(e));
+}
+
+void linear_scores_dlogits(const LinearScoreArgs& a, cudaStream_t s) {
+  LinScoresDev p = make_dev(a);
+  launch<true>(a, p, s);
+}
+
+}  // namespace himuon

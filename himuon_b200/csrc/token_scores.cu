@@ -4,29 +4,30 @@
 // With m = max x, d = x - m:   s = sum e^d,  t = sum d e^d,   log p_j = d_j - log s,   H = log s - t / s.
 // Shifted by the maximum both sums have terms of one sign, so the entropy of a peaked row loses nothing to cancellation, and
 // partial results merge: moving (m1, s1, t1) to a larger m scales s1 by f = e^(m1-m) and turns t1 into f (t1 + (m1-m) s1).
-// Gradient, with the incoming g of log p_y and h of H:   dx_j = g [j = y] - p_j (g + h (log p_j + H)).
+// Gradient, with the incoming g of log p_y and h of H:   dx_j = g [j = y] - p_j (g + h (log p_j + H)).  (token_scores.cuh)
 // A logit of -inf has p = 0 and no part in H.  A row of nothing but -inf has log p = -inf, H = 0 and no gradient.  An id equal to
 // `ignore` has log p = 0 and passes no g on; an id outside the vocabulary has log p = NaN and passes none on either.
 //
-// One pass over the logits; their bytes bound both kernels.  A row goes to a cluster of 1 to 8 blocks, so that a few rows
-// occupy the GPU as well (rule in scores_split()); the blocks' partial results meet in distributed shared memory.
+// One pass over the logits.  fp32 logits run at the rate of memory (2048 x 151936: 178 us, 7.0 TB/s); bf16 ones come close to what the
+// SMs can exponentiate, 16 a clock (2048 x 151936: 105 us, 5.9 TB/s, exponential unit 72 % busy), and alternatives cost half as many
+// instructions again (1024 x 128256 with 8: 72 us, where 46 would do without).  A row goes to a cluster of 1 to 8 blocks, so that a few
+// rows occupy the GPU as well (scores_split()); the blocks' partial results meet in distributed shared memory.  The gradient, one read
+// and one write, takes 215 us at 2048 x 151936 bf16 (5.8 TB/s).
 // Likeliest alternatives: each warp keeps a sorted list of 32, one a lane, as 64-bit keys of value and inverted index, so that equal
-// values go to the lower index.  What passes the list's k-th value is collected in shared memory and merged 32 at a time by a
-// bitonic network; after the first few hundred elements of a row next to nothing passes.
+// values go to the lower index.  What passes a floor that all warps raise together is collected in shared memory and merged 32 at a
+// time by a bitonic network.
 #include <stdint.h>
 
 #include "himuon.h"
 #include "pair_common.cuh"
 #include "sm100_common.cuh"
+#include "token_scores.cuh"
 
 namespace himuon {
 
 namespace {
 
-constexpr int SC_THREADS = 256, SC_WARPS = SC_THREADS / 32;
-constexpr float kLog2eS = 1.4426950408889634f;
-constexpr float kFar = -1.0e4f;                   // d below this: e^d is 0 in fp32, and d * e^d has to be as well
-
+constexpr int NW = 8, NT = NW * 32;              // warps and threads of a block
 template <typename T> struct Vec;                 // one 16-byte group of logits
 template <> struct Vec<float> {
   static constexpr int N = 4;
@@ -43,43 +44,6 @@ template <> struct Vec<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 };
-
-struct Sums { float m, s, t; };
-__device__ __forceinline__ Sums moved(const Sums& a, float m) {     // a's sums relative to m >= a.m
-  if (a.m == -INFINITY) return Sums{m, a.s, a.t};                   // 0, or NaN
-  const float d = fmaxf(a.m - m, kFar), f = exp2f(d * kLog2eS);
-  return Sums{m, a.s * f, f * (a.t + d * a.s)};
-}
-__device__ __forceinline__ Sums merged(const Sums& a, const Sums& b) {
-  const float m = fmaxf(a.m, b.m);
-  const Sums x = moved(a, m), y = moved(b, m);
-  return Sums{m, x.s + y.s, x.t + y.t};
-}
-template <int N>
-__device__ __forceinline__ void take(Sums& a, const float (&x)[N]) {
-  float mx = x[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) mx = fmaxf(mx, x[i]);
-  if (mx > a.m) a = moved(a, mx);
-  const float base = a.m == -INFINITY ? 0.f : a.m;    // nothing but -inf so far: d = -inf, e^d = 0
-  const f32x2 nbase = pack2(-base, -base), l2e = pack2(kLog2eS, kLog2eS);
-  f32x2 s = pack2(0.f, 0.f), t = s;
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const f32x2 d = add2(pack2(x[i], x[i + 1]), nbase);
-    float d0, d1, y0, y1;
-    unpack2(d, d0, d1);
-    unpack2(mul2(d, l2e), y0, y1);
-    const f32x2 e = pack2(exp2f(y0), exp2f(y1));
-    s = add2(s, e);
-    t = fma2(pack2(fmaxf(d0, kFar), fmaxf(d1, kFar)), e, t);
-  }
-  float a0, a1;
-  unpack2(s, a0, a1);
-  a.s += a0 + a1;
-  unpack2(t, a0, a1);
-  a.t += a0 + a1;
-}
 
 // ---------------------------------------------------------------- lists of the largest
 typedef unsigned long long Key;
@@ -125,13 +89,12 @@ __device__ __forceinline__ Key merged_down(Key a, Key b, int lane) {
 
 struct TopList {
   Key best;              // this lane's entry
-  Key kth;               // the k-th of the list, and its value
-  float bar;
+  Key kth;               // the k-th of the list
   int waiting;           // entries of `buf` in use, the same in all lanes
   Key* buf;              // 64 of this warp
   int lane, k;
   __device__ __forceinline__ void start(Key* b, int l, int k_) {
-    best = 0; kth = 0; bar = -INFINITY; waiting = 0; buf = b; lane = l; k = k_;
+    best = 0; kth = 0; waiting = 0; buf = b; lane = l; k = k_;
   }
   __device__ __forceinline__ void flush() {
     __syncwarp();
@@ -141,20 +104,28 @@ struct TopList {
     buf[lane] = rest;
     best = merged_down(best, sorted_down(x, lane), lane);
     kth = __shfl_sync(0xffffffffu, best, k - 1);
-    bar = kth ? key_value(kth) : -INFINITY;
     waiting = waiting > 32 ? waiting - 32 : 0;
   }
-  // One value a lane (live lanes only); called by the whole warp.
-  __device__ __forceinline__ void offer(float x, uint32_t index, bool live) {
-    const Key key = key_of(x, index);
-    const bool in = live && !(x < bar) && key > kth;
+  // One key a lane, 0 for none; called by the whole warp.
+  __device__ __forceinline__ void push(Key key) {
+    const bool in = key > kth;
     const uint32_t who = __ballot_sync(0xffffffffu, in);
-    if (who == 0) return;
     if (in) buf[waiting + __popc(who & ((1u << lane) - 1))] = key;
     waiting += __popc(who);
-    if (waiting >= 32) flush();
+    if (waiting > 32) flush();
   }
 };
+
+// The j-th largest over the lanes (each lane's value counts once).
+__device__ __forceinline__ float jth_largest(float x, int j, int lane) {
+  uint32_t u = static_cast<uint32_t>(key_of(x, 0) >> 32), top = 0;
+  for (int i = 0; i < j; ++i) {
+    top = __reduce_max_sync(0xffffffffu, u);
+    const uint32_t who = __ballot_sync(0xffffffffu, u == top);
+    if (lane == __ffs(who) - 1) u = 0;
+  }
+  return key_value(static_cast<Key>(top) << 32);
+}
 
 }  // namespace
 
@@ -186,16 +157,42 @@ __device__ __forceinline__ V load_remote(const V* p, uint32_t rank) {     // a m
   return out;
 }
 
+// The warps' lists, one entry a lane, merged into warp 0's `best`.
+__device__ __forceinline__ void join_lists(Key& best, Key (*lists)[32], int warp, int lane) {
+#pragma unroll
+  for (int o = NW / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (warp >= o && warp < 2 * o) lists[warp][lane] = best;
+    __syncthreads();
+    if (warp < o) best = merged_down(best, lists[warp + o][lane], lane);
+  }
+}
+
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // Cluster = one row.  Block r of the cluster takes the r-th share of the row's whole 16-byte groups; what lies before the first
 // group and behind the last goes to the first block.
+// With alternatives: a thread's maximum so far is that of an element of its own, so the least of the warps' ceil(k / warps)-th largest
+// thread maxima is a value that k elements reach.  Nothing below it can be among the k; the warps publish and read it as they go (it only
+// grows, so an old one is still true), and after the first pass over the block's threads few groups of logits have a candidate.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(SC_THREADS)
+__global__ void __launch_bounds__(NT)
 token_scores_kernel(ScoreArgsDev p) {
-  constexpr int N = Vec<T>::N, UN = TOP ? 2 : 4;
-  __shared__ Sums s_sums[SC_WARPS];
+  constexpr int N = Vec<T>::N, UN = 4, RING = 2;
+  __shared__ uint4 s_ring[RING][UN][NT];
+  __shared__ Sums s_sums[NW];
   __shared__ Sums s_block;
-  __shared__ Key s_buf[TOP ? SC_WARPS * 64 : 1];
-  __shared__ Key s_list[TOP ? 32 : 1];
+  __shared__ Key s_buf[TOP ? NW * 64 : 1];
+  __shared__ Key s_lists[TOP ? NW : 1][32];
+  __shared__ volatile float s_floor[NW];
+  constexpr int POOL = 96;
+  __shared__ Key s_pool[TOP ? POOL : 1];
+  __shared__ int s_count;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t parts = cluster_nctas(), part = cluster_ctarank();
@@ -208,37 +205,88 @@ token_scores_kernel(ScoreArgsDev p) {
   const int g0 = static_cast<int>(static_cast<long long>(groups) * part / parts), g1 = static_cast<int>(static_cast<long long>(groups) * (part + 1) / parts);
   const uint4* body = reinterpret_cast<const uint4*>(x + head);
 
+  // the row's own token, fetched while the rest is on its way
+  float own = nan_f();
+  bool counted = false;
+  if (part == 0 && threadIdx.x == 0) {
+    const long long y = p.ids[row];
+    counted = y != p.ignore;
+    if (counted && y >= 0 && y < p.vocab) own = Vec<T>::one(x + y);
+  }
   Sums a{-INFINITY, 0.f, 0.f};
   TopList top;
-  if (TOP) top.start(s_buf + warp * 64, lane, p.k);
-  // every lane of a warp makes the same number of passes, with -inf where it is past the end
-  const float none = -INFINITY;
-  for (int g = g0 + warp * 32 * UN; g < g1; g += SC_THREADS * UN) {
-    uint4 raw[UN];
+  float floor = -INFINITY;
+  const int nth = (p.k + NW - 1) / NW;
+  if (TOP) {
+    top.start(s_buf + warp * 64, lane, p.k);
+    if (lane == 0) s_floor[warp] = -INFINITY;
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+  }
+  // Each thread copies its own groups to shared memory ahead of their use and is the only one to read them, so that the copies
+  // wait for nothing but themselves.  (Loads into registers, one pass in flight and then none:
+  // 123 us for 1024 x 128256 with 8 alternatives, 107 this way.)
+  auto group_of = [&](int pass, int u) { return g0 + ((pass * NW + warp) * UN + u) * 32 + lane; };
+  const int passes = (g1 - g0 + NT * UN - 1) / (NT * UN);        // of the block, the same for every warp
+  auto fetch = [&](int pass) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int i = g + u * 32 + lane;
-      if (i < g1) raw[u] = __ldcs(body + i);
+      const int i = group_of(pass, u);
+      if (pass < passes && i < g1) copy_async16(&s_ring[pass % RING][u][threadIdx.x], body + i);
     }
+    copy_async_commit();
+  };
+  for (int pass = 0; pass < RING - 1; ++pass) fetch(pass);
+  for (int pass = 0; pass < passes; ++pass) {
+    fetch(pass + RING - 1);
+    copy_async_wait<RING - 1>();
+    // all groups of a pass at once: their exponentials do not wait for one another
+    float v[UN * N];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int i = g + u * 32 + lane;
-      const bool live = i < g1;
-      float v[N];
-      Vec<T>::unpack(raw[u], v);
-      if (live) take<N>(a, v);
-      if (TOP) {
-        bool any = false;
+      float f[N];
+      Vec<T>::unpack(s_ring[pass % RING][u][threadIdx.x], f);
 #pragma unroll
-        for (int q = 0; q < N; ++q) any = any || !(v[q] < top.bar);
-        if (__any_sync(0xffffffffu, live && any)) {
-#pragma unroll 1
-          for (int q = 0; q < N; ++q) {
-            float xq = none;
+      for (int q = 0; q < N; ++q) v[u * N + q] = f[q];
+    }
+    if (pass == passes - 1) {                         // past the end: whatever the slots hold
 #pragma unroll
-            for (int r = 0; r < N; ++r) if (r == q) xq = v[r];
-            top.offer(xq, static_cast<uint32_t>(head + i * N + q), live);
+      for (int u = 0; u < UN; ++u) {
+        const bool live = group_of(pass, u) < g1;
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[u * N + q] = live ? v[u * N + q] : -INFINITY;
+      }
+    }
+    const float most = largest<UN * N>(v);
+    take<UN * N>(a, v, most);
+    if constexpr (TOP) {
+      if (pass < 2 || (pass & 1) == 0) {
+        const float mine = jth_largest(a.m, nth, lane);
+        if (lane == 0) s_floor[warp] = mine;
+        if (pass == 0) __syncthreads();             // the first value of every warp; later ones may be a little old
+        else __syncwarp();
+        float f = s_floor[lane & (NW - 1)];
+#pragma unroll
+        for (int o = NW / 2; o > 0; o >>= 1) f = fminf(f, __shfl_xor_sync(0xffffffffu, f, o));
+        floor = f;
+      }
+      if (__any_sync(0xffffffffu, most >= floor)) {
+        uint32_t hits = 0;
+#pragma unroll
+        for (int q = 0; q < UN * N; ++q) hits |= v[q] >= floor ? 1u << q : 0u;
+        if (pass == passes - 1) {
+#pragma unroll
+          for (int u = 0; u < UN; ++u) if (group_of(pass, u) >= g1) hits &= ~(((1u << N) - 1) << (u * N));
+        }
+        while (__any_sync(0xffffffffu, hits != 0)) {  // one of each lane at a time: as a rule that is all
+          Key key = 0;
+          if (hits) {
+            const int at = __ffs(hits) - 1, u = at / N, q = at % N;
+            hits &= hits - 1;
+            const T* slot = reinterpret_cast<const T*>(&s_ring[pass % RING][u][threadIdx.x]);
+            key = key_of(Vec<T>::one(slot + q), static_cast<uint32_t>(head + group_of(pass, u) * N + q));
           }
+          top.push(key);
         }
       }
     }
@@ -247,60 +295,95 @@ token_scores_kernel(ScoreArgsDev p) {
     const int tail0 = head + groups * N, loose = head + p.vocab - tail0;
     const bool live = lane < loose;
     const int at = lane < head ? lane : tail0 + lane - head;
-    float v[2] = {none, none};
+    float v[2] = {-INFINITY, -INFINITY};
     if (live) v[0] = Vec<T>::one(x + at);
-    if (live) take<2>(a, v);
-    if (TOP) top.offer(v[0], static_cast<uint32_t>(at), live);
+    if (live) take<2>(a, v, v[0]);
+    if (TOP) top.push(live ? key_of(v[0], static_cast<uint32_t>(at)) : 0);
   }
   // lanes, warps, blocks
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o)};
-    a = merged(a, b);
-  }
-  if (lane == 0) s_sums[warp] = a;
   if (TOP) {
-    while (top.waiting > 0) top.flush();
-    __syncwarp();
-    top.buf[lane] = top.best;
+    const float mine = jth_largest(a.m, nth, lane);
+    if (lane == 0) s_floor[warp] = mine;
+  }
+  a = lanes_merged(a);
+  if (lane == 0) s_sums[warp] = a;
+  if constexpr (TOP) {
+    // NaN and +inf never raise a floor and are not seen by a comparison with one: such a row (its sum is NaN) is looked through again
+    const bool odd = __syncthreads_or(!(a.s >= 0.f));
+    if (odd) {
+      for (int i0 = g0 + warp * 32; i0 < g1; i0 += NT) {
+        const int i = i0 + lane;
+        float v[N];
+        Vec<T>::unpack(i < g1 ? body[i] : make_uint4(0, 0, 0, 0), v);
+        if (i0 == g0 + warp * 32) { top.best = 0; top.kth = 0; top.waiting = 0; }
+#pragma unroll 1
+        for (int q = 0; q < N; ++q) {
+          float xq = v[0];
+#pragma unroll
+          for (int r = 1; r < N; ++r) xq = r == q ? v[r] : xq;
+          top.push(i < g1 ? key_of(xq, static_cast<uint32_t>(head + i * N + q)) : 0);
+        }
+      }
+      if (part == 0 && warp == 0) {
+        const int tail0 = head + groups * N, loose = head + p.vocab - tail0;
+        const int at = lane < head ? lane : tail0 + lane - head;
+        if (g0 + warp * 32 >= g1) { top.best = 0; top.kth = 0; top.waiting = 0; }
+        top.push(lane < loose ? key_of(Vec<T>::one(x + at), static_cast<uint32_t>(at)) : 0);
+      }
+    } else {
+      // what reaches the last floor: a few more than k as a rule, few enough for one warp
+      floor = s_floor[0];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) floor = fminf(floor, s_floor[w]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const Key key = i == 2 ? top.best : lane + 32 * i < top.waiting ? top.buf[lane + 32 * i] : 0;
+        if (key != 0 && key_value(key) >= floor) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < POOL) s_pool[at] = key;
+        }
+      }
+      __syncthreads();
+    }
+    const int n = odd ? POOL + 1 : s_count;           // uniform
+    if (n <= POOL) {
+      if (warp == 0) {
+        top.best = 0;
+        for (int i = 0; i < n; i += 32) top.best = merged_down(top.best, sorted_down(i + lane < n ? s_pool[i + lane] : 0, lane), lane);
+      }
+    } else {
+      while (top.waiting > 0) top.flush();
+      join_lists(top.best, s_lists, warp, lane);
+    }
   }
   __syncthreads();
   if (warp == 0) {
-    a = s_sums[0];
-    for (int w = 1; w < SC_WARPS; ++w) a = merged(a, s_sums[w]);
-    if (TOP) {
-      for (int w = 1; w < SC_WARPS; ++w) top.best = merged_down(top.best, s_buf[w * 64 + lane], lane);
-    }
+    a = lane < NW ? s_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+    a = lanes_merged(a);
   }
   if (parts > 1) {                                  // uniform over the cluster
     if (warp == 0) {
       if (lane == 0) s_block = a;
-      if (TOP) s_list[lane] = top.best;
+      if (TOP) s_lists[0][lane] = top.best;
     }
-    __syncwarp();
     cluster_sync_all();
     if (part == 0 && warp == 0) {
-      for (uint32_t r = 1; r < parts; ++r) {
-        a = merged(a, load_remote(&s_block, r));
-        if (TOP) top.best = merged_down(top.best, load_remote(&s_list[lane], r), lane);
-      }
+      a = static_cast<uint32_t>(lane) < parts ? load_remote(&s_block, lane) : Sums{-INFINITY, 0.f, 0.f};
+      a = lanes_merged(a);
     }
+    if (TOP && part == 0) top.best = static_cast<uint32_t>(warp) < parts ? load_remote(&s_lists[0][lane], warp) : 0;
     cluster_sync_all();                             // no block leaves while it is still read
+    if (TOP && part == 0) join_lists(top.best, s_lists, warp, lane);
   }
   if (part == 0 && warp == 0) {
-    const bool empty = a.s == 0.f;                  // nothing but -inf (a NaN makes s NaN)
-    const float m = empty ? 0.f : a.m;
-    const float log_s = empty ? INFINITY : static_cast<float>(log(static_cast<double>(a.s)));   // (logf is the approximate one in this build)
+    const RowScore r = row_score(a);
     if (lane == 0) {
-      const long long y = p.ids[row];
-      float lp = 0.f;
-      if (y != p.ignore) lp = y >= 0 && y < p.vocab ? (Vec<T>::one(x + y) - m) - log_s : __uint_as_float(0x7FFFFFFFu);
-      p.log_probs[row] = lp;
-      p.entropy[row] = empty ? 0.f : log_s - a.t / a.s;
-      if (p.stats) p.stats[row] = make_float2(m, log_s);
+      p.log_probs[row] = counted ? (own - r.m) - r.log_s : 0.f;
+      p.entropy[row] = r.entropy;
+      if (p.stats) p.stats[row] = make_float2(r.m, r.log_s);
     }
     if (TOP && lane < p.k) {
-      p.top_log_probs[row * p.k + lane] = (key_value(top.best) - m) - log_s;
+      p.top_log_probs[row * p.k + lane] = (key_value(top.best) - r.m) - r.log_s;
       p.top_ids[row * p.k + lane] = key_index(top.best);
     }
   }
@@ -325,33 +408,18 @@ __device__ __forceinline__ void store_one<float>(float* p, float v) { *p = v; }
 template <>
 __device__ __forceinline__ void store_one<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// dx of N logits from column `at` on.
-template <int N>
-__device__ __forceinline__ void grad_of(const float (&x)[N], float (&d)[N], int at, float m, float log_s, float c0, float h, float g, long long y) {
-#pragma unroll
-  for (int q = 0; q < N; ++q) {
-    const float lp = (x[q] - m) - log_s, e = exp2f(lp * kLog2eS);
-    d[q] = -e * fmaf(h, fmaxf(lp, kFar), c0);
-    if (at + q == y) d[q] += g;
-  }
-}
 // T: logits, D: gradient.  Rows that share the offset from 16 bytes with the gradient's are read and written in 16-byte groups of
 // logits; others element by element.
 constexpr int SG_GROUPS = 4;                        // 16-byte groups of logits a thread takes
 template <typename T, typename D>
-__global__ void __launch_bounds__(SC_THREADS)
+__global__ void __launch_bounds__(NT)
 token_scores_grad_kernel(ScoreGradDev p, int blocks_per_row) {
   constexpr int N = Vec<T>::N;
   const long long row = blockIdx.x / blocks_per_row;
   const int piece = static_cast<int>(blockIdx.x - row * blocks_per_row);
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
   D* dx = reinterpret_cast<D*>(p.grad) + row * p.ld_grad;
-  const float2 st = p.stats[row];
-  const long long id = p.ids[row];
-  const bool counted = id != p.ignore && id >= 0 && id < p.vocab;
-  const long long y = counted && st.y != INFINITY ? id : -1;             // (INFINITY: a row of nothing but -inf)
-  const float g = counted && p.g_log_probs ? p.g_log_probs[row] : 0.f;
-  const float h = p.g_entropy ? p.g_entropy[row] : 0.f, c0 = fmaf(h, p.entropy[row], g);
+  const RowGrad r = row_grad(p.stats, p.entropy, p.ids, p.g_log_probs, p.g_entropy, p.ignore, p.vocab, row);
 
   int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T));
   if (head > p.vocab) head = p.vocab;
@@ -359,12 +427,13 @@ token_scores_grad_kernel(ScoreGradDev p, int blocks_per_row) {
   const int groups = (p.vocab - head) / N;
 #pragma unroll
   for (int u = 0; u < SG_GROUPS; ++u) {
-    const int i = (piece * SG_GROUPS + u) * SC_THREADS + static_cast<int>(threadIdx.x);
+    const int i = (piece * SG_GROUPS + u) * NT + static_cast<int>(threadIdx.x);
     if (i >= groups) break;
     const int at = head + i * N;
     float v[N], d[N];
     Vec<T>::unpack(__ldcs(reinterpret_cast<const uint4*>(x + head) + i), v);
-    grad_of<N>(v, d, at, st.x, st.y, c0, h, g, y);
+#pragma unroll
+    for (int q = 0; q < N; ++q) d[q] = grad_of(r, v[q], at + q);
     if (wide) {
       if constexpr (sizeof(D) == 4) {
 #pragma unroll
@@ -382,30 +451,29 @@ token_scores_grad_kernel(ScoreGradDev p, int blocks_per_row) {
   const int tail0 = head + groups * N, loose = head + p.vocab - tail0;
   if (piece == 0 && static_cast<int>(threadIdx.x) < loose) {
     const int at = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail0 + threadIdx.x - head;
-    const float v[1] = {Vec<T>::one(x + at)};
-    float d[1];
-    grad_of<1>(v, d, at, st.x, st.y, c0, h, g, y);
-    store_one<D>(dx + at, d[0]);
+    store_one<D>(dx + at, grad_of(r, Vec<T>::one(x + at), at));
   }
 }
 
-// Blocks per row: doubled while the launch would still not fill the GPU and a share keeps a few thousand logits.
+// Blocks per row, by what a few rows take alone (us, 1 / 2 / 4 / 8 blocks): 1 row of 151936 16.7 / 11.6 / 8.5 / 6.4; 16 rows with 5
+// alternatives 23.6 / 18.6 / 14.6 / 12.9; 64 with 8 24.8 / 18.6 / 16.6 / 23.9; 150 without 20.8 / 18.6 / 18.6 / 22.7.  From 300 rows on
+// a second block only doubles what a block costs at its ends: 333 x 32003 with 5 16.8 / 22.9, 1024 x 128256 with 8 72 / 91.
 static int scores_split(long long rows, int vocab) {
   int parts = 1;
-  while (parts < 8 && rows * parts < 4LL * num_sms() && vocab / (2 * parts) >= 2048) parts *= 2;
+  while (parts < 8 && rows * parts <= num_sms() && vocab / (2 * parts) >= 2048) parts *= 2;
   return parts;
 }
 
 void token_scores_fwd(const TokenScoreArgs& a, cudaStream_t s) {
   if (a.rows <= 0) return;
+  if (a.vocab <= 0 || a.top_k < 0 || a.top_k > kTopMax || a.top_k > a.vocab) throw std::runtime_error("himuon token_scores: bad vocabulary or number of alternatives");
   const ScoreArgsDev p{a.logits, a.ids, a.log_probs, a.entropy, reinterpret_cast<float2*>(a.stats), a.top_log_probs, a.top_ids,
                        a.rows, a.ld, a.ignore, a.vocab, a.top_k};
   const int parts = scores_split(a.rows, a.vocab);
-  if (a.vocab <= 0 || a.top_k < 0 || a.top_k > kTopMax || a.top_k > a.vocab) throw std::runtime_error("himuon token_scores: bad vocabulary or number of alternatives");
   if (a.rows * parts >= (1LL << 31)) throw std::runtime_error("himuon token_scores: too many rows for one launch");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows * parts));
-  cfg.blockDim = dim3(SC_THREADS);
+  cfg.blockDim = dim3(NT);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -423,16 +491,16 @@ void token_scores_bwd(const TokenScoreArgs& a, cudaStream_t s) {
   const ScoreGradDev p{a.logits, a.grad, a.ids, a.entropy, reinterpret_cast<const float2*>(a.stats), a.g_log_probs, a.g_entropy,
                        a.rows, a.ld, a.ld_grad, a.ignore, a.vocab};
   const int n = a.logits_fp32 ? 4 : 8;
-  const long long per_row = (a.vocab / n + SC_THREADS * SG_GROUPS - 1) / (SC_THREADS * SG_GROUPS), blocks_per_row = per_row > 0 ? per_row : 1;
+  const long long per_row = (a.vocab / n + NT * SG_GROUPS - 1) / (NT * SG_GROUPS), blocks_per_row = per_row > 0 ? per_row : 1;
   if (a.vocab <= 0 || a.rows * blocks_per_row >= (1LL << 31)) throw std::runtime_error("himuon token_scores: gradient too large for one launch");
   const unsigned grid = static_cast<unsigned>(a.rows * blocks_per_row);
   const int b = static_cast<int>(blocks_per_row);
   if (a.logits_fp32) {
-    if (a.grad_fp32) token_scores_grad_kernel<float, float><<<grid, SC_THREADS, 0, s>>>(p, b);
-    else token_scores_grad_kernel<float, __nv_bfloat16><<<grid, SC_THREADS, 0, s>>>(p, b);
+    if (a.grad_fp32) token_scores_grad_kernel<float, float><<<grid, NT, 0, s>>>(p, b);
+    else token_scores_grad_kernel<float, __nv_bfloat16><<<grid, NT, 0, s>>>(p, b);
   } else {
     if (a.grad_fp32) throw std::runtime_error("himuon token_scores: bf16 logits have bf16 gradients");
-    token_scores_grad_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, SC_THREADS, 0, s>>>(p, b);
+    token_scores_grad_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, NT, 0, s>>>(p, b);
   }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon token_scores gradient launch failed: ") + cudaGetErrorString(e));

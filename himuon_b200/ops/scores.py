@@ -93,26 +93,30 @@ def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ign
 
 
 class _LinearTokenLogProbsFn(torch.autograd.Function):
-    """Rows in chunks: fp32 logits of a chunk, their scores; the backward pass makes the logits again, turns them into
-    their gradient and multiplies that with both operands."""
+    """The forward pass keeps two numbers a row; the backward pass makes the logits again, as their gradient in bf16, and
+    multiplies that with both operands."""
 
-    CHUNK = 2 ** 29                                   # logits alive at once
+    ROWS = 8192                  # of one launch: their hidden states stay in the L2 while the weight streams by
+    CHUNK = 2 ** 31              # most values of the logits' gradient alive at once (4 GiB)
 
     @staticmethod
     def forward(ctx, h, w, ids, ignore_index):
         ctx.set_materialize_grads(False)
-        rows, vocab = h.shape[0], w.shape[0]
+        rows, vocab, e = h.shape[0], w.shape[0], _ext.ext()
         log_probs = torch.empty(rows, device=h.device, dtype=torch.float32)
         entropy = torch.empty_like(log_probs)
-        stats = torch.empty(rows, 2, device=h.device, dtype=torch.float32)
-        step = max(128, _LinearTokenLogProbsFn.CHUNK // vocab)
+        need = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        stats = torch.empty(rows, 2, device=h.device, dtype=torch.float32) if need else None
+        step = _LinearTokenLogProbsFn.ROWS
+        if rows:
+            scratch = torch.empty(e.linear_scores_scratch(min(rows, step), vocab), device=h.device, dtype=torch.float32)
         for r in range(0, rows, step):
             c = slice(r, min(rows, r + step))
-            logits = gemm(h[c], w, trans_b=True, out_dtype=torch.float32)
-            _ext.ext().token_scores_fwd(logits, ids[c], log_probs[c], entropy[c], stats[c], None, None, ignore_index)
-            _count()
-        ctx.save_for_backward(h, w, ids, entropy, stats)
-        ctx.ignore_index, ctx.step = ignore_index, step
+            e.linear_scores_fwd(h[c], w, ids[c], log_probs[c], entropy[c], stats[c] if need else None, scratch, ignore_index)
+            _count(2)
+        if need:
+            ctx.save_for_backward(h, w, ids, entropy, stats)
+            ctx.ignore_index = ignore_index
         return log_probs, entropy
 
     @staticmethod
@@ -123,18 +127,27 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
         h, w, ids, entropy, stats = ctx.saved_tensors
         rows, vocab = h.shape[0], w.shape[0]
         g, ge = _incoming(g_log_probs), _incoming(g_entropy)
-        dh = torch.empty_like(h)
-        # a sum over several chunks is held in fp32
-        dw = torch.zeros(w.shape, device=w.device, dtype=torch.bfloat16 if rows <= ctx.step else torch.float32)
-        for r in range(0, rows, ctx.step):
-            c = slice(r, min(rows, r + ctx.step))
-            logits = gemm(h[c], w, trans_b=True, out_dtype=torch.float32)
-            dx = torch.empty(logits.shape[0], (vocab + 7) // 8 * 8, device=h.device, dtype=torch.bfloat16)[:, :vocab]
-            _ext.ext().token_scores_bwd(logits, ids[c], entropy[c], stats[c], None if g is None else g[c], None if ge is None else ge[c], dx, ctx.ignore_index)
+        cols = (vocab + 7) // 8 * 8
+        step = max(256, min(_LinearTokenLogProbsFn.ROWS, _LinearTokenLogProbsFn.CHUNK // cols // 256 * 256))
+        dh = torch.empty(h.shape, device=h.device, dtype=h.dtype) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:
+            # a sum over several chunks is held in fp32
+            dw = (torch.zeros if rows == 0 else torch.empty)(w.shape, device=w.device, dtype=torch.bfloat16 if rows <= step else torch.float32)
+        if rows:
+            buf = torch.empty(min(rows, step), cols, device=h.device, dtype=torch.bfloat16)
+        for r in range(0, rows, step):
+            c = slice(r, min(rows, r + step))
+            dx = buf[: c.stop - r]
+            _ext.ext().linear_scores_dlogits(h[c], w, ids[c], entropy[c], stats[c], None if g is None else g[c], None if ge is None else ge[c], dx,
+                                             ctx.ignore_index)
             _count()
-            gemm(dx, w, out=dh[c])
-            gemm(dx, h[c], trans_a=True, out=dw, aux=dw if r else None, beta=1.0 if r else 0.0)
-        return dh, dw.to(w.dtype), None, None
+            dx = dx[:, :vocab]
+            if dh is not None:
+                gemm(dx, w, out=dh[c])
+            if dw is not None:
+                gemm(dx, h[c], trans_a=True, out=dw, aux=dw if r else None, beta=1.0 if r else 0.0)
+        return dh, None if dw is None else dw.to(w.dtype), None, None
 
 
 def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, ignore_index: int = -100) -> TokenLogProbs:
