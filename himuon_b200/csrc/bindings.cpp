@@ -437,6 +437,14 @@ static void linear_scores_dlogits(const at::Tensor& h, const at::Tensor& w, cons
   himuon::linear_scores_dlogits(a, cur_stream());
 }
 
+static void sum_parts(const at::Tensor& parts, at::Tensor& out) {
+  HM_CHECK(parts.is_cuda() && is_f32(parts) && parts.is_contiguous() && parts.dim() == out.dim() + 1 && out.device() == parts.device() && is_bf16(out) && out.is_contiguous() &&
+               parts.numel() == parts.size(0) * out.numel() && out.numel() % 4 == 0 && reinterpret_cast<uintptr_t>(parts.data_ptr()) % 16 == 0 &&
+               reinterpret_cast<uintptr_t>(out.data_ptr()) % 8 == 0, "sum_parts: contiguous fp32 parts of a contiguous bf16 output expected");
+  const c10::cuda::CUDAGuard guard(parts.device());
+  himuon::sum_parts(parts.data_ptr<float>(), out.data_ptr(), out.numel(), (int)parts.size(0), cur_stream());
+}
+
 static bool ns5_fused_supported(int64_t m, int64_t n) { return himuon::ns5_fused_supported((int)m, (int)n); }
 static void ns5_fused(const at::Tensor& x, at::Tensor& out, int64_t steps, double eps, bool normalize) {
   HM_CHECK(x.is_cuda() && is_bf16(x) && is_bf16(out) && x.is_contiguous() && out.is_contiguous() && x.dim() == 3 && x.sizes() == out.sizes(), "ns5_fused: contiguous (B, m, n) bf16 tensors");
@@ -525,6 +533,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("token_scores_fwd", &token_scores_fwd);
   m.def("token_scores_bwd", &token_scores_bwd);
   m.def("linear_scores_fwd", &linear_scores_fwd);
+  m.def("sum_parts", &sum_parts);
   m.def("linear_scores_dlogits", &linear_scores_dlogits);
   m.def("linear_scores_scratch", [](int64_t rows, int64_t vocab) { return himuon::linear_scores_scratch(rows, (int)vocab); });
   m.def("flash_attn_fwd", &flash_attn_fwd);

@@ -206,6 +206,8 @@ struct LinearScoreArgs {
 long long linear_scores_scratch(long long rows, int vocab);
 void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s);
 void linear_scores_dlogits(const LinearScoreArgs& a, cudaStream_t s);
+// out (n bf16) = the sum of n_parts fp32 vectors of n, a multiple of 4, that lie one after the other.
+void sum_parts(const float* parts, void* out, long long n, int n_parts, cudaStream_t s);
 
 // ---------------------------------------------------------------- collectives over peer-mapped memory
 constexpr int kCommMaxBlocks = 256;

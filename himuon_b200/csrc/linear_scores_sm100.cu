@@ -222,6 +222,158 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
   }
 }
 
+// ---------------------------------------------------------------- a few rows
+// Up to 32 rows: the weight's bytes are all that counts, so the weight takes the 128 lanes of the accumulator and the rows its NB
+// columns; a stage carries 16 KB of weight and 2 or 4 of hidden states (the pair kernel spends half of its stages on rows that are not
+// there).  A block streams one share of the vocabulary in tiles of `th` entries; a thread keeps the sums of its lane for
+// every row, and only at the end the 128 lanes meet.  8 rows over 151936 x 1024: NN us, pair kernel 99.
+constexpr int FEW_STAGES = 10, FEW_THREADS = 192;       // warp 0: TMA, 1: MMA, 2-5: epilogue
+struct FewBars {
+  uint64_t full[FEW_STAGES], empty[FEW_STAGES], tfull[2], tempty[2];
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+// One lane's sums for CNT rows against the other lanes': every step halves the rows that a lane keeps.
+template <int CNT, int O>
+__device__ __forceinline__ void share_out(Sums* a, int lane) {
+  if constexpr (O > 0) {
+    constexpr int HALF = CNT > 1 ? CNT / 2 : 1;
+    const bool up = (lane & O) != 0;
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) {
+      const Sums give = CNT > 1 && !up ? a[i + HALF * (CNT > 1)] : a[i], keep = CNT > 1 && up ? a[i + HALF * (CNT > 1)] : a[i];
+      a[i] = merged(keep, Sums{__shfl_xor_sync(0xffffffffu, give.m, O), __shfl_xor_sync(0xffffffffu, give.s, O), __shfl_xor_sync(0xffffffffu, give.t, O)});
+    }
+    share_out<HALF, O / 2>(a, lane);
+  }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(FEW_THREADS, 1)
+linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW, LinScoresDev p, int th) {
+  constexpr uint32_t STAGE = LS_A + NB * BK * 2;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_up_1024(smem_raw);
+  FewBars* bars = reinterpret_cast<FewBars*>(smem + FEW_STAGES * STAGE);
+  Sums* s_warp = reinterpret_cast<Sums*>(bars + 1);      // [4][NB]
+  volatile int* abort_flag = &bars->abort_flag;
+  const int warp = warp_id(), lane = threadIdx.x & 31;
+  // shares of whole groups of eight entries
+  const long long units = (p.vocab + 7) / 8;
+  const int v0 = static_cast<int>(units * blockIdx.x / gridDim.x) * 8, end = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x) * 8;
+  const int v1 = end < p.vocab ? end : p.vocab, tiles = (v1 - v0 + th - 1) / th;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < FEW_STAGES; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars->tfull[i], 1); mbar_init(&bars->tempty[i], 128); }
+    bars->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc(&bars->tmem_slot, 64);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_slot, 0);
+
+  if (warp == 0) {
+    const uint32_t e = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; ok && i < tiles; ++i) {
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&bars->empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
+        uint8_t* sW = smem + stage * STAGE;
+        mbar_expect_tx(&bars->full[stage], (th + NB) * BK * 2, e);
+        tma_load_3d(sW, &tmW, &bars->full[stage], kb * BK, v0 + i * th, 0, e);
+        tma_load_3d(sW + LS_A, &tmH, &bars->full[stage], kb * BK, 0, 0, e);
+        if (++stage == FEW_STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t e = elect_one();
+    constexpr uint32_t idesc = umma_idesc_bf16(128, NB, false, false);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int i = 0; ok && i < tiles; ++i) {
+      if (!mbar_wait_warp(&bars->tempty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, p.status, 2)) break;
+      tc_fence_after();
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&bars->full[stage], phase, abort_flag, p.status, 2)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t base = smem_u32(smem + stage * STAGE);
+        // (lanes from `th` on hold whatever an earlier tile left: rows of the product that nobody reads)
+        const uint64_t w_desc = umma_smem_desc(base, 16, 1024), h_desc = umma_smem_desc(base + LS_A, 16, 1024);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          umma_ss(tmem + (i & 1) * NB, desc_at(w_desc, k * 32), desc_at(h_desc, k * 32), idesc, (kb > 0 || k > 0) ? 1u : 0u, e);
+        umma_commit(&bars->empty[stage], e);
+        if (++stage == FEW_STAGES) { stage = 0; phase ^= 1; }
+      }
+      if (ok) umma_commit(&bars->tfull[i & 1], e);
+    }
+  } else {
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    Sums a[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) a[n] = Sums{-INFINITY, 0.f, 0.f};
+    int own[NB];                                  // the rows' own tokens, -1 where there is none
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const long long id = n < p.rows ? p.ids[n] : -1;
+      own[n] = id >= 0 && id < p.vocab ? static_cast<int>(id) : -1;
+    }
+    for (int i = 0; i < tiles; ++i) {
+      if (!mbar_wait(&bars->tfull[i & 1], (i >> 1) & 1, abort_flag, p.status, 3)) break;
+      tc_fence_after();
+      const int v = v0 + i * th + row;
+      const bool mine = row < th && v < v1;
+#pragma unroll
+      for (int c = 0; c < NB; c += 16) {
+        uint32_t x[16];
+        tmem_ld16(tmem + (i & 1) * NB + lane_off + c, x);
+        tmem_ld_wait();
+        if (mine) {
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            const float y = __uint_as_float(x[n]);
+            Sums& b = a[c + n];
+            const float m = fmaxf(b.m, y), from = fmaxf(b.m - m, kFar), f = exp2f(from * kLog2eS);
+            const float d = y - (m == -INFINITY ? 0.f : m), e = exp2f(d * kLog2eS);
+            b.t = fmaf(fmaxf(d, kFar), e, f * fmaf(from, b.s, b.t));
+            b.s = fmaf(b.s, f, e);
+            b.m = m;
+            if (own[c + n] == v) p.target[c + n] = y;
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&bars->tempty[i & 1]);
+    }
+    share_out<NB, 16>(a, lane);
+    if (NB == 32) s_warp[(warp & 3) * NB + lane] = a[0];
+    else if ((lane & 1) == 0) s_warp[(warp & 3) * NB + (lane >> 1)] = a[0];
+    named_barrier(1, 128);
+    const int n = (warp - 2) * 32 + lane;
+    if (n < p.rows && n < NB) {
+      Sums b = s_warp[n];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) b = merged(b, s_warp[w * NB + n]);
+      const long long all = static_cast<long long>(gridDim.x) * p.rows, at = static_cast<long long>(blockIdx.x) * p.rows + n;
+      p.part[at] = b.m;
+      p.part[all + at] = b.s;
+      p.part[2 * all + at] = b.t;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 64);
+  }
+}
+
 // Merges the parts of RB rows per block (RB neighbouring rows are neighbours in memory), in the same order on every run.
 template <int RB>
 __global__ void __launch_bounds__(256)
@@ -252,6 +404,20 @@ linear_scores_join_kernel(LinScoresDev p, int n_parts, float* log_probs, float* 
     log_probs[row] = lp;
     entropy[row] = s.entropy;
     if (stats) stats[row] = make_float2(s.m, s.log_s);
+  }
+}
+
+// out = sum of n_parts fp32 matrices of n elements, in their order.
+__global__ void __launch_bounds__(256)
+sum_parts_kernel(const float4* __restrict__ parts, uint2* __restrict__ out, long long n4, int n_parts) {
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < n4; i += static_cast<long long>(gridDim.x) * 256) {
+    float4 a = parts[i];
+#pragma unroll 4
+    for (int k = 1; k < n_parts; ++k) {
+      const float4 b = parts[k * n4 + i];
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+    out[i] = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
   }
 }
 
@@ -317,6 +483,23 @@ static void launch(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores launch failed: ") + cudaGetErrorString(e));
 }
 
+// Returns the number of parts.
+template <int NB>
+static int launch_few(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s) {
+  constexpr size_t SMEM = 1024 + FEW_STAGES * (LS_A + NB * BK * 2) + sizeof(FewBars) + 4 * NB * sizeof(Sums);
+  static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
+  const cudaError_t set = cudaFuncSetAttribute(linear_scores_few_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
+  if (set != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores: ") + cudaGetErrorString(set));
+  p.kblocks = (a.hidden + BK - 1) / BK;
+  const int blocks = 2 * ((a.vocab + 127) / 128), grid = blocks < num_sms() ? blocks : num_sms();    // (scratch holds so many parts)
+  const int share = ((a.vocab + 7) / 8 + grid - 1) / grid * 8, tiles = (share + 127) / 128, th = ((share + tiles - 1) / tiles + 7) / 8 * 8;
+  const CUtensorMap thid = rows_tmap(a.h, a.rows, a.hidden, a.ld_h, NB), tw = rows_tmap(a.w, a.vocab, a.hidden, a.ld_w, th);
+  linear_scores_few_kernel<NB><<<grid, FEW_THREADS, SMEM, s>>>(thid, tw, p, th);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores launch failed: ") + cudaGetErrorString(e));
+  return grid;
+}
+
 static LinScoresDev make_dev(const LinearScoreArgs& a) {
   if (a.rows <= 0 || a.vocab <= 0 || a.hidden <= 0 || a.hidden % 8) throw std::runtime_error("himuon linear_scores: bad sizes");
   LinScoresDev p{};
@@ -335,13 +518,27 @@ long long linear_scores_scratch(long long rows, int vocab) { return rows * (1 + 
 
 void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {
   LinScoresDev p = make_dev(a);
-  launch<false>(a, p, s);
-  const int n_parts = 2 * p.tiles_n;
+  int n_parts;
+  if (a.rows <= 32) {
+    n_parts = a.rows <= 16 ? launch_few<16>(a, p, s) : launch_few<32>(a, p, s);
+  } else {
+    launch<false>(a, p, s);
+    n_parts = 2 * p.tiles_n;
+  }
   float2* stats = reinterpret_cast<float2*>(a.stats);
   if (a.rows < 512) linear_scores_join_kernel<1><<<a.rows, 256, 0, s>>>(p, n_parts, a.log_probs, a.entropy, stats);
   else linear_scores_join_kernel<8><<<(a.rows + 7) / 8, 256, 0, s>>>(p, n_parts, a.log_probs, a.entropy, stats);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores join launch failed: ") + cudaGetErrorString(e));
+}
+
+void sum_parts(const float* parts, void* out, long long n, int n_parts, cudaStream_t s) {
+  if (n <= 0 || n_parts <= 0) return;
+  if (n % 4) throw std::runtime_error("himuon sum_parts: a multiple of 4 elements expected");
+  const long long blocks = (n / 4 + 255) / 256, most = static_cast<long long>(num_sms()) * 8;
+  sum_parts_kernel<<<static_cast<int>(blocks < most ? blocks : most), 256, 0, s>>>(reinterpret_cast<const float4*>(parts), reinterpret_cast<uint2*>(out), n / 4, n_parts);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon sum_parts launch failed: ") + cudaGetErrorString(e));
 }
 
 void linear_scores_dlogits(const LinearScoreArgs& a, cudaStream_t s) {

@@ -92,6 +92,38 @@ def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ign
     return TokenLogProbs(*ref.token_log_probs(logits, ids, top_k, ignore_index))
 
 
+def _long_product(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> None:
+    """``out = a @ b`` for a long inner dimension and few output tiles: cut along it into batches whose fp32 results are added up.
+
+    A GEMM's time goes by its rounds of tiles over the SMs, and the cut fills them: 777 x 128256 x 640, 12 tiles of 256 x 256
+    on 74 CTA pairs, NN us in 6 cuts against 567 whole; the fp32 results are what a cut costs."""
+    (rows, inner), cols = a.shape, b.shape[1]
+    pairs = rows > 128 and cols > 192
+    sms = _ext.ext().num_sms()
+    slots, tile = (sms // 2, 256) if pairs else (sms, 128)
+    tiles = -(-rows // tile) * -(-cols // 256)
+    unit = tile * 256 * 2 * inner / (1.4e15 / slots)           # seconds of one tile, whole
+    best, cuts = None, 1
+    for s in range(1, min(16, inner // 4096) + 1):
+        rounds = -(-tiles * s // slots) / s
+        if s == 1 and pairs and tiles > slots // 2 and 0 < tiles % slots <= slots // 2:
+            rounds = tiles / slots                             # (the GEMM cuts such a last round itself)
+        cost = rounds * unit + (8.0 * s * rows * cols / 6e12 + 8e-6 if s > 1 else 0.0)
+        if best is None or cost < best:
+            best, cuts = cost, s
+    if cuts == 1:
+        gemm(a, b, out=out)
+        return
+    step = inner // cuts // 64 * 64
+    rest = inner - cuts * step
+    parts = torch.empty(cuts + (rest > 0), rows, cols, device=a.device, dtype=torch.float32)
+    gemm(a.as_strided((cuts, rows, step), (step, a.stride(0), 1)), b.as_strided((cuts, step, cols), (step * b.stride(0), b.stride(0), 1)), out=parts[:cuts])
+    if rest:
+        gemm(a[:, cuts * step:], b[cuts * step:], out=parts[cuts])
+    _ext.ext().sum_parts(parts, out)
+    _count()
+
+
 class _LinearTokenLogProbsFn(torch.autograd.Function):
     """The forward pass keeps two numbers a row; the backward pass makes the logits again, as their gradient in bf16, and
     multiplies that with both operands."""
@@ -144,7 +176,7 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
             _count()
             dx = dx[:, :vocab]
             if dh is not None:
-                gemm(dx, w, out=dh[c])
+                _long_product(dx, w, dh[c])
             if dw is not None:
                 gemm(dx, h[c], trans_a=True, out=dw, aux=dw if r else None, beta=1.0 if r else 0.0)
         return dh, None if dw is None else dw.to(w.dtype), None, None

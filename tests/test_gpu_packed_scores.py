@@ -390,7 +390,7 @@ def _logit_error(h, w):
     return (h.shape[1] / 16 + 4) * 2.0 ** -22 * (h.double().abs() @ w.double().abs().t()).max().item()
 
 
-@pytest.mark.parametrize("rows,hidden,vocab", [(1, 8, 1), (1, 128, 1000), (8, 256, 5003), (100, 64, 264), (129, 136, 777), (300, 640, 4096), (777, 128, 2050)])
+@pytest.mark.parametrize("rows,hidden,vocab", [(1, 8, 1), (1, 128, 1000), (8, 256, 5003), (3, 72, 40000), (16, 128, 151936), (17, 200, 9000), (32, 640, 128256), (33, 128, 3001), (100, 64, 264), (129, 136, 777), (300, 640, 4096), (777, 128, 2050)])
 def test_linear_token_log_probs(rows, hidden, vocab):
     ops = _ops()
     torch.manual_seed(rows + vocab)
@@ -436,6 +436,25 @@ def test_linear_token_log_probs_in_chunks(monkeypatch):
         assert torch.equal(a, b)
     # the same fp32 terms in another order, then one rounding
     assert ((whole[3].float() - parts[3].float()).abs() <= 2 * U * whole[3].float().abs() + 1e-4).all()
+    _clean()
+
+
+def test_linear_token_log_probs_of_a_long_vocabulary():
+    """Few output tiles and a long inner dimension: the hidden states' gradient is cut along the vocabulary."""
+    ops = _ops()
+    from himuon_b200.ops import scores
+
+    torch.manual_seed(35)
+    for rows, hidden, vocab in [(200, 256, 40000), (40, 136, 50001), (5, 128, 30001)]:
+        a = torch.randn(rows, (vocab + 7) // 8 * 8, device="cuda").bfloat16()[:, :vocab]
+        b = torch.randn(vocab, hidden, device="cuda").bfloat16()
+        out = torch.empty(rows, hidden, device="cuda", dtype=torch.bfloat16)
+        before = ops.launch_count()
+        scores._long_product(a, b, out)
+        assert ops.launch_count() - before >= 2, "one GEMM did it all: the test covers nothing"
+        want = a.double() @ b.double()
+        # an fp32 sum of vocab / 16 steps, then one rounding
+        _within(out, want, U * want.abs() + (vocab / 16 + 64) * 2.0 ** -24 * (a.double().abs() @ b.double().abs()), "product")
     _clean()
 
 
