@@ -279,28 +279,34 @@ static void flash_attn_bwd(const at::Tensor& d_o, const at::Tensor& q, const at:
   himuon::flash_attn_bwd(a, cur_stream());
 }
 
-// `plan`: (2, tiles, 4) int32, the batch's tiles in the two orders (himuon.h); its entries are bounded by the caller, which makes
-// them from the lengths on the host (`tokens` of them).
-static himuon::PackedAttnArgs packed_attn_args(const char* op, const at::Tensor& plan, int64_t tokens, const at::Tensor& q, const at::Tensor& k,
-                                               const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse, int64_t Hq, int64_t Hkv, double scale) {
+// `plan`: (2 * tiles + pairs, 4) int32, the batch's tiles in their three orders (himuon.h); its entries are bounded by the caller, which
+// makes them from the lengths on the host (`tokens` of them).
+static himuon::PackedAttnArgs packed_attn_args(const char* op, const at::Tensor& plan, int64_t tiles, int64_t tokens, const at::Tensor& q, const at::Tensor& k,
+                                               const at::Tensor& v, const at::Tensor& o, const c10::optional<at::Tensor>& lse, int64_t Hq, int64_t Hkv, double scale) {
   const std::string at = std::string("himuon: ") + op;
   TORCH_CHECK(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, at, ": heads");
   TORCH_CHECK(q.dim() == 2 && q.size(1) % Hq == 0, at, ": (tokens, heads*head_dim) views expected");
   const int64_t T = q.size(0), hd = q.size(1) / Hq;
   TORCH_CHECK(hd > 0 && hd % 8 == 0 && hd <= 128, at, ": head_dim must be a multiple of 8 up to 128");
   TORCH_CHECK(T > 0 && T < (1LL << 30) && tokens >= 0 && tokens <= T, at, ": fewer rows than the layout has tokens");
-  TORCH_CHECK(plan.device() == q.device() && plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.dim() == 3 && plan.size(0) == 2 && plan.size(2) == 4,
-              at, ": the plan must be a contiguous (2, tiles, 4) int32 tensor on the device of q");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0, at, ": misaligned plan");
+  TORCH_CHECK(plan.device() == q.device() && plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.dim() == 2 && plan.size(1) == 4 && tiles >= 0 &&
+                  tiles < (1LL << 28) && plan.size(0) >= 2 * tiles && plan.size(0) <= 3 * tiles && reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0,
+              at, ": the plan must be a contiguous (2 * tiles + pairs, 4) int32 tensor on the device of q");
   himuon::PackedAttnArgs a{};
-  a.n_tiles = static_cast<int>(plan.size(1));
+  a.n_tiles = static_cast<int>(tiles);
+  a.n_pairs = static_cast<int>(plan.size(0) - 2 * tiles);
   a.by_keys = reinterpret_cast<const himuon::PackedTile*>(plan.data_ptr<int>());
   a.by_queries = a.by_keys + a.n_tiles;
+  a.pairs = a.by_queries + a.n_tiles;
+  a.tokens = static_cast<int>(tokens);
   a.rows = static_cast<int>(T); a.Hq = static_cast<int>(Hq); a.Hkv = static_cast<int>(Hkv); a.hd = static_cast<int>(hd);
   a.scale = static_cast<float>(scale);
-  TORCH_CHECK(is_f32(lse) && lse.is_contiguous() && lse.device() == q.device() && lse.numel() == Hq * a.n_tiles * 128 &&
-                  reinterpret_cast<uintptr_t>(lse.data_ptr()) % 16 == 0, at, ": lse must be fp32, (heads, tiles * 128)");
-  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr(); a.lse = lse.data_ptr<float>();
+  if (lse.has_value()) {
+    TORCH_CHECK(is_f32(*lse) && lse->is_contiguous() && lse->device() == q.device() && lse->numel() == Hq * a.n_tiles * 128 &&
+                    reinterpret_cast<uintptr_t>(lse->data_ptr()) % 16 == 0, at, ": lse must be fp32, (heads, tiles * 128)");
+    a.lse = lse->data_ptr<float>();
+  }
+  a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr(); a.o = o.data_ptr();
   a.ld_q = q.stride(0); a.ld_k = k.stride(0); a.ld_v = v.stride(0); a.ld_o = o.stride(0);
   return a;
 }
@@ -310,18 +316,18 @@ static void packed_rows(const char* op, const at::Tensor& t, const at::Tensor& q
                   t.stride(0) % 8 == 0 && (t.size(0) <= 1 || t.stride(0) >= cols) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               at, ": bf16 rows of heads * head_dim columns with unit inner stride, each on a 16-byte boundary, expected");
 }
-static void packed_attn_fwd(const at::Tensor& plan, int64_t tokens, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& o,
-                            at::Tensor& lse, int64_t Hq, int64_t Hkv, double scale) {
-  const himuon::PackedAttnArgs a = packed_attn_args("packed_attn_fwd", plan, tokens, q, k, v, o, lse, Hq, Hkv, scale);
+static void packed_attn_fwd(const at::Tensor& plan, int64_t tiles, int64_t tokens, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            at::Tensor& o, const c10::optional<at::Tensor>& lse, int64_t Hq, int64_t Hkv, double scale) {
+  const himuon::PackedAttnArgs a = packed_attn_args("packed_attn_fwd", plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
   packed_rows("packed_attn_fwd", q, q, Hq * a.hd); packed_rows("packed_attn_fwd", k, q, Hkv * a.hd);
   packed_rows("packed_attn_fwd", v, q, Hkv * a.hd); packed_rows("packed_attn_fwd", o, q, Hq * a.hd);
   const c10::cuda::CUDAGuard guard(q.device());
   himuon::packed_attn_fwd(a, cur_stream());
 }
-static void packed_attn_bwd(const at::Tensor& plan, int64_t tokens, const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+static void packed_attn_bwd(const at::Tensor& plan, int64_t tiles, int64_t tokens, const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             const at::Tensor& o, const at::Tensor& lse, at::Tensor& dq, at::Tensor& dk, at::Tensor& dv, at::Tensor& delta,
                             int64_t Hq, int64_t Hkv, double scale) {
-  himuon::PackedAttnArgs a = packed_attn_args("packed_attn_bwd", plan, tokens, q, k, v, o, lse, Hq, Hkv, scale);
+  himuon::PackedAttnArgs a = packed_attn_args("packed_attn_bwd", plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
   for (const at::Tensor* t : {&q, &o, &d_o, static_cast<const at::Tensor*>(&dq)}) packed_rows("packed_attn_bwd", *t, q, Hq * a.hd);
   for (const at::Tensor* t : {&k, &v, static_cast<const at::Tensor*>(&dk), static_cast<const at::Tensor*>(&dv)}) packed_rows("packed_attn_bwd", *t, q, Hkv * a.hd);
   HM_CHECK(is_f32(delta) && delta.is_contiguous() && delta.device() == q.device() && delta.numel() == lse.numel() &&

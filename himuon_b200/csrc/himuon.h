@@ -164,11 +164,12 @@ void flash_attn_bwd(const AttnArgs& a, cudaStream_t s);
 // A tile of up to 128 tokens of one document: the document's first row and length, the tile's number in it and in the batch.
 struct PackedTile { int first, len, index, slot; };
 // q, o and their gradients: (rows, Hq * hd); k, v and theirs: (rows, Hkv * hd); bf16, row strides ld_*.  The tiles are listed
-// twice, by falling number of keys that their queries see and by falling number of queries that see their keys.  lse and delta:
-// (Hq, n_tiles * 128) fp32.  Rows of no document are left alone.
+// by falling number of keys that their queries see, by falling number of queries that see their keys, and (the first of) two and two
+// of a document, by falling number of keys.  lse (may be null in the forward pass) and delta: (Hq, n_tiles * 128) fp32.  Rows from
+// `tokens` on belong to no document: their outputs are zero.
 struct PackedAttnArgs {
-  const PackedTile* by_keys; const PackedTile* by_queries;
-  int n_tiles, rows, Hq, Hkv, hd;
+  const PackedTile* by_keys; const PackedTile* by_queries; const PackedTile* pairs;
+  int n_tiles, n_pairs, tokens, rows, Hq, Hkv, hd;
   const void* q; const void* k; const void* v; void* o; float* lse;
   const void* d_o; void* dq; void* dk; void* dv; float* delta;
   long long ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv;

@@ -22,10 +22,11 @@ from . import reference as ref
 TILE = 128          # tokens of one document that a block of the kernels takes
 
 
-def _tile_plan(lengths: np.ndarray) -> np.ndarray:
-    """``(2, tiles, 4)`` int32: every tile as (first row of its document, length of it, number in the document, number in
-    the batch), in the order of falling work of the passes over a tile's keys and of the pass over its queries."""
-    first = np.concatenate([[0], np.cumsum(lengths)[:-1]]) if lengths.size else lengths
+def _tile_plan(lengths: np.ndarray) -> tuple[np.ndarray, int]:
+    """``(2 * tiles + pairs, 4)`` int32 and the number of tiles.  Every tile as (first row of its document, length of it, number
+    in the document, number in the batch): by falling work of the passes over a tile's keys, by falling work of the pass over
+    its queries, and the first of two and two of a document by falling work of both."""
+    first = np.cumsum(lengths) - lengths
     per_doc = (lengths + TILE - 1) // TILE
     doc = np.repeat(np.arange(lengths.size), per_doc)
     slot = np.arange(doc.size)
@@ -33,7 +34,10 @@ def _tile_plan(lengths: np.ndarray) -> np.ndarray:
     tiles = np.stack([first[doc], lengths[doc], index, slot], axis=1)
     keys = np.minimum((index + 1) * TILE, lengths[doc])
     queries = lengths[doc] - index * TILE
-    return np.stack([tiles[np.argsort(-keys, kind="stable")], tiles[np.argsort(-queries, kind="stable")]]).astype(np.int32)
+    even = np.flatnonzero(index % 2 == 0)
+    both = keys[even] + np.where((index[even] + 1) * TILE < lengths[doc[even]], np.minimum((index[even] + 2) * TILE, lengths[doc[even]]), 0)
+    orders = [np.argsort(-keys, kind="stable"), np.argsort(-queries, kind="stable"), even[np.argsort(-both, kind="stable")]]
+    return np.ascontiguousarray(tiles[np.concatenate(orders)], dtype=np.int32), slot.size
 
 
 class PackedLayout:
@@ -65,16 +69,15 @@ class PackedLayout:
         lens = np.asarray(self.lengths, dtype=np.int64)
         self._position = np.arange(self.tokens) - np.repeat(np.cumsum(lens) - lens, lens)
         self._tables: dict = {}
-        plan = _tile_plan(lens)
-        self.tiles = plan.shape[1]
+        plan, self.tiles = _tile_plan(lens)
         self._table("plan", lambda: plan)
 
-    def _table(self, key, make) -> torch.Tensor:
+    def _table(self, key, make=None) -> torch.Tensor:
         """The device copy of a host table, safe to use on the current stream."""
         entry = self._tables.get(key)
         on_gpu = self.device.type == "cuda"
         if entry is None:
-            host = torch.from_numpy(np.ascontiguousarray(make()))
+            host = torch.from_numpy(make())
             if not on_gpu:
                 entry = (host.to(self.device), None, None)
             else:
@@ -85,17 +88,16 @@ class PackedLayout:
                 entry = (table, stream, event)
             self._tables[key] = entry
         table, stream, event = entry
-        if on_gpu and not torch.cuda.is_current_stream_capturing():
+        if on_gpu and torch._C._cuda_getCurrentRawStream(self.device.index) != stream.cuda_stream and not torch.cuda.is_current_stream_capturing():
             # (a stream that captures a graph has been synchronised with what came before)
             here = torch.cuda.current_stream(self.device)
-            if here != stream:
-                here.wait_event(event)
-                table.record_stream(here)
+            here.wait_event(event)
+            table.record_stream(here)
         return table
 
     @property
     def plan(self) -> torch.Tensor:
-        return self._table("plan", lambda: _tile_plan(np.asarray(self.lengths, dtype=np.int64)))
+        return self._table("plan")
 
     def _check_rows(self, op: str, rows: int) -> None:
         if rows < self.tokens:
@@ -131,16 +133,21 @@ class PackedLayout:
         return cos_sin.index_select(0, self.positions(rows))
 
 
+def _forward(q, k, v, layout, Hq, Hkv, scale, keep: bool):
+    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty(Hq * layout.tiles * TILE, device=q.device, dtype=torch.float32) if keep else None
+    if layout.tiles:
+        _ext.ext().packed_attn_fwd(layout.plan, layout.tiles, layout.tokens, q, k, v, o, lse, Hq, Hkv, scale)
+        _count()
+    else:
+        o.zero_()
+    return o, lse
+
+
 class _PackedAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, layout, Hq, Hkv, scale):
-        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        if q.shape[0] > layout.tokens:
-            o[layout.tokens:].zero_()
-        lse = torch.empty(Hq * layout.tiles * TILE, device=q.device, dtype=torch.float32)
-        if layout.tiles:
-            _ext.ext().packed_attn_fwd(layout.plan, layout.tokens, q, k, v, o, lse, Hq, Hkv, scale)
-            _count()
+        o, lse = _forward(q, k, v, layout, Hq, Hkv, scale, True)
         ctx.save_for_backward(q, k, v, o, lse)
         ctx.layout, ctx.heads, ctx.scale = layout, (Hq, Hkv), scale
         return o
@@ -154,13 +161,13 @@ class _PackedAttnFn(torch.autograd.Function):
         D = q.shape[1] // Hq
         # dq | dk | dv share one buffer, as in attention(): a fused projection sees a single contiguous gradient
         dqkv = torch.empty(q.shape[0], (Hq + 2 * Hkv) * D, device=q.device, dtype=q.dtype)
-        if q.shape[0] > layout.tokens:
-            dqkv[layout.tokens:].zero_()
         dq, dk, dv = dqkv[:, : Hq * D], dqkv[:, Hq * D: (Hq + Hkv) * D], dqkv[:, (Hq + Hkv) * D:]
         if layout.tiles:
             delta = torch.empty_like(lse)
-            _ext.ext().packed_attn_bwd(layout.plan, layout.tokens, do, q, k, v, o, lse, dq, dk, dv, delta, Hq, Hkv, ctx.scale)
+            _ext.ext().packed_attn_bwd(layout.plan, layout.tiles, layout.tokens, do, q, k, v, o, lse, dq, dk, dv, delta, Hq, Hkv, ctx.scale)
             _count(2)
+        else:
+            dqkv.zero_()
         return dq, dk, dv, None, None, None, None
 
 
@@ -185,7 +192,10 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
     if layout.device != q2d.device:
         raise RuntimeError(f"himuon_b200.ops.packed_attention: the layout is on {layout.device}, the tensors on {q2d.device}")
     if use_kernels(q2d) and head_dim <= 128 and head_dim % 8 == 0:
-        return _PackedAttnFn.apply(*(_with_kernel_rows(t) for t in (q2d, k2d, v2d)), layout, Hq, Hkv, scale)
+        q, k, v = _with_kernel_rows(q2d), _with_kernel_rows(k2d), _with_kernel_rows(v2d)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _PackedAttnFn.apply(q, k, v, layout, Hq, Hkv, scale)
+        return _forward(q, k, v, layout, Hq, Hkv, scale, False)[0]
     if use_kernels(q2d):
         _warn_torch_path("packed_attention", f"head_dim {head_dim} (the kernels take multiples of 8 up to 128)")
     return ref.packed_attention(q2d, k2d, v2d, layout.lengths, Hq, Hkv, head_dim, scale)

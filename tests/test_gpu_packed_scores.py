@@ -245,10 +245,10 @@ def test_packed_attention_refusals_of_the_kernel_path():
         ops.packed_attention(q, q, q, ops.PackedLayout([4], device="cpu"), 2, 2, 32)
     from himuon_b200._ext import ext
     plan, lse = ops.PackedLayout([4]).plan, torch.empty(256, device="cuda")
-    ok = (plan, 4, q, q, q, torch.empty_like(q), lse, 2, 2, 0.1)
+    ok = (plan, 1, 4, q, q, q, torch.empty_like(q), lse, 2, 2, 0.1)
     ext().packed_attn_fwd(*ok)
-    for i, bad in [(0, plan.long()), (0, plan[:, :, :2].contiguous()), (0, plan.cpu()), (1, 5), (2, q.float()), (3, q[:, :32]), (4, q[:2]), (5, q.t()),
-                   (6, lse[:128]), (6, lse.double()), (7, 3), (8, 0), (2, torch.randn(5, 64, device="cuda").bfloat16().flatten()[4:260].view(4, 64))]:
+    for i, bad in [(0, plan.long()), (0, plan[:, :2].contiguous()), (0, plan.cpu()), (0, plan[:1]), (1, 2), (1, -1), (2, 5), (3, q.float()), (4, q[:, :32]), (5, q[:2]),
+                   (6, q.t()), (7, lse[:128]), (7, lse.double()), (8, 3), (9, 0), (3, torch.randn(5, 64, device="cuda").bfloat16().flatten()[4:260].view(4, 64))]:
         with pytest.raises(RuntimeError, match="himuon"):
             ext().packed_attn_fwd(*ok[:i], bad, *ok[i + 1:])
     _clean()

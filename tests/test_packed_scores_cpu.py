@@ -18,17 +18,23 @@ def test_layout_lists_every_tile_once_and_heaviest_first(lengths):
     layout = ops.PackedLayout(lengths, device="cpu")
     assert layout.lengths == tuple(lengths) and layout.tokens == sum(lengths)
     plan = layout.plan
-    assert plan.dtype == torch.int32 and plan.shape == (2, layout.tiles, 4)
     want, first = [], 0
     for n in lengths:
         want += [(first, n, i) for i in range(-(-n // TILE))]
         first += n
     want = [(*t, slot) for slot, t in enumerate(want)]
-    for order in plan.tolist():
-        assert sorted(map(tuple, order), key=lambda t: t[3]) == want
-    keys = [min((i + 1) * TILE, n) for _, n, i, _ in plan[0].tolist()]
-    queries = [n - i * TILE for _, n, i, _ in plan[1].tolist()]
-    assert keys == sorted(keys, reverse=True) and queries == sorted(queries, reverse=True)
+    pairs = [t for t in want if t[2] % 2 == 0]
+    assert plan.dtype == torch.int32 and layout.tiles == len(want) and plan.shape == (2 * len(want) + len(pairs), 4)
+    rows = [tuple(t) for t in plan.tolist()]
+    by_keys, by_queries, by_both = rows[: len(want)], rows[len(want): 2 * len(want)], rows[2 * len(want):]
+    for order, all_of in ((by_keys, want), (by_queries, want), (by_both, pairs)):
+        assert sorted(order, key=lambda t: t[3]) == all_of
+
+    def keys(n, i):
+        return min((i + 1) * TILE, n) if i * TILE < n else 0
+
+    for work in ([keys(n, i) for _, n, i, _ in by_keys], [n - i * TILE for _, n, i, _ in by_queries], [keys(n, i) + keys(n, i + 1) for _, n, i, _ in by_both]):
+        assert work == sorted(work, reverse=True)
 
 
 def test_layout_positions_next_ids_and_rope_rows():
