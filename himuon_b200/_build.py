@@ -19,7 +19,7 @@ CUDA_SOURCES = [
     "model_kernels.cu",
     "attention_sm100.cu",
     "attention_kv64_sm100.cu", "attention_bwd_sm100.cu",
-    "packed_attention_sm100.cu", "token_scores.cu", "linear_scores_sm100.cu",
+    "packed_attention_sm100.cu", "packed_attention_bwd_sm100.cu", "token_scores.cu", "linear_scores_sm100.cu",
     "ns5_sm100.cu", "ns_pair_sm100.cu",
     "comm_kernels.cu",
     "soap_kernels.cu",

@@ -326,7 +326,7 @@ static void packed_attn_fwd(const at::Tensor& plan, int64_t tiles, int64_t token
 }
 static void packed_attn_bwd(const at::Tensor& plan, int64_t tiles, int64_t tokens, const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             const at::Tensor& o, const at::Tensor& lse, at::Tensor& dq, at::Tensor& dk, at::Tensor& dv, at::Tensor& delta,
-                            int64_t Hq, int64_t Hkv, double scale) {
+                            const c10::optional<at::Tensor>& dkv_part, int64_t Hq, int64_t Hkv, double scale) {
   himuon::PackedAttnArgs a = packed_attn_args("packed_attn_bwd", plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
   for (const at::Tensor* t : {&q, &o, &d_o, static_cast<const at::Tensor*>(&dq)}) packed_rows("packed_attn_bwd", *t, q, Hq * a.hd);
   for (const at::Tensor* t : {&k, &v, static_cast<const at::Tensor*>(&dk), static_cast<const at::Tensor*>(&dv)}) packed_rows("packed_attn_bwd", *t, q, Hkv * a.hd);
@@ -334,6 +334,11 @@ static void packed_attn_bwd(const at::Tensor& plan, int64_t tiles, int64_t token
                reinterpret_cast<uintptr_t>(delta.data_ptr()) % 16 == 0, "packed_attn_bwd: delta must look like lse");
   a.d_o = d_o.data_ptr(); a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr(); a.delta = delta.data_ptr<float>();
   a.ld_do = d_o.stride(0); a.ld_dq = dq.stride(0); a.ld_dk = dk.stride(0); a.ld_dv = dv.stride(0);
+  if (dkv_part.has_value()) {
+    HM_CHECK(is_f32(*dkv_part) && dkv_part->is_contiguous() && dkv_part->device() == q.device() && dkv_part->numel() == 2 * lse.numel() * a.hd &&
+                 reinterpret_cast<uintptr_t>(dkv_part->data_ptr()) % 16 == 0, "packed_attn_bwd: dkv_part must be fp32, (2, heads, tiles * 128, head_dim)");
+    a.dkv_part = dkv_part->data_ptr<float>();
+  }
   const c10::cuda::CUDAGuard guard(q.device());
   himuon::packed_attn_bwd(a, cur_stream());
 }

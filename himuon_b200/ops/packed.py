@@ -70,6 +70,8 @@ class PackedLayout:
         self._position = np.arange(self.tokens) - np.repeat(np.cumsum(lens) - lens, lens)
         self._tables: dict = {}
         plan, self.tiles = _tile_plan(lens)
+        of = plan[self.tiles: 2 * self.tiles]
+        self._query_steps = int(((of[:, 1] - of[:, 2] * TILE + 63) // 64).sum())   # of 64 queries, over all tiles, for one head
         self._table("plan", lambda: plan)
 
     def _table(self, key, make=None) -> torch.Tensor:
@@ -102,6 +104,14 @@ class PackedLayout:
     def _check_rows(self, op: str, rows: int) -> None:
         if rows < self.tokens:
             raise RuntimeError(f"himuon_b200.ops.{op}: {rows} rows for a layout of {self.tokens} tokens")
+
+    def splits_heads(self, Hq: int, Hkv: int) -> bool:
+        """Whether the pass for dK and dV takes each query head by itself and sums the heads of a group afterwards.  A block
+        otherwise has all heads of a group to go through, and in a small batch the longest block sets the time: NN."""
+        if Hq == Hkv:
+            return False
+        longest = Hq // Hkv * -(-self.max_length // 64)                       # steps of 64 queries
+        return longest > 2 * self._query_steps * Hq / _ext.ext().num_sms()
 
     def positions(self, rows: int | None = None) -> torch.Tensor:
         """Each row's position in its own document (int64), 0 for the padding of a batch of ``rows`` rows."""
@@ -164,8 +174,9 @@ class _PackedAttnFn(torch.autograd.Function):
         dq, dk, dv = dqkv[:, : Hq * D], dqkv[:, Hq * D: (Hq + Hkv) * D], dqkv[:, (Hq + Hkv) * D:]
         if layout.tiles:
             delta = torch.empty_like(lse)
-            _ext.ext().packed_attn_bwd(layout.plan, layout.tiles, layout.tokens, do, q, k, v, o, lse, dq, dk, dv, delta, Hq, Hkv, ctx.scale)
-            _count(2)
+            part = torch.empty(2 * lse.numel() * D, device=q.device, dtype=torch.float32) if layout.splits_heads(Hq, Hkv) else None
+            _ext.ext().packed_attn_bwd(layout.plan, layout.tiles, layout.tokens, do, q, k, v, o, lse, dq, dk, dv, delta, part, Hq, Hkv, ctx.scale)
+            _count(2 if part is None else 3)
         else:
             dqkv.zero_()
         return dq, dk, dv, None, None, None, None

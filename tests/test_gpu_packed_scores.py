@@ -84,7 +84,7 @@ def _attention64(q, k, v, lengths, Hq, Hkv, hd, scale, do=None):
 
 
 SHAPES = [(4, 2, 32), (2, 2, 64), (8, 2, 128), (3, 1, 128), (2, 1, 72), (1, 1, 8), (6, 3, 96)]
-BATCHES = [([1], 0), ([0, 0, 2], 5), ([128], 0), ([127, 1, 0, 64, 65], 7), ([129, 256, 3], 0), ([5, 1, 0, 700, 30, 513], 0), ([1100], 100)]
+BATCHES = [([1], 0), ([0, 0, 2], 5), ([128], 0), ([127, 1, 0, 64, 65], 7), ([129, 256, 3], 0), ([5, 1, 0, 700, 30, 513], 0), ([1100], 100), ([90] * 80, 3)]
 
 
 @pytest.mark.parametrize("Hq,Hkv,hd", SHAPES)
@@ -97,6 +97,8 @@ def test_packed_attention(Hq, Hkv, hd, lengths, pad):
     for t in (q, k, v):
         t.requires_grad_()
     layout = ops.PackedLayout(lengths)
+    # a group's heads one by one in small batches, together in the last one
+    assert layout.splits_heads(Hq, Hkv) == (Hq > Hkv and len(lengths) < 60)
     before = ops.launch_count()
     o = ops.packed_attention(q, k, v, layout, Hq, Hkv, hd)
     dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
