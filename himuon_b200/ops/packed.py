@@ -13,10 +13,9 @@ import operator
 
 import numpy as np
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _ext
-from . import _check_width, _count, _warn_torch_path, _with_kernel_rows, use_kernels
+from . import _check_width, _count, _once, _warn_torch_path, _with_kernel_rows, use_kernels
 from . import reference as ref
 
 TILE = 128          # tokens of one document that a block of the kernels takes
@@ -163,15 +162,15 @@ class _PackedAttnFn(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
+        _once("packed_attention")
         q, k, v, o, lse = ctx.saved_tensors
         layout, (Hq, Hkv) = ctx.layout, ctx.heads
         do = _with_kernel_rows(do)
         D = q.shape[1] // Hq
         # dq | dk | dv share one buffer, as in attention(): a fused projection sees a single contiguous gradient
         dqkv = torch.empty(q.shape[0], (Hq + 2 * Hkv) * D, device=q.device, dtype=q.dtype)
-        dq, dk, dv = dqkv[:, : Hq * D], dqkv[:, Hq * D: (Hq + Hkv) * D], dqkv[:, (Hq + Hkv) * D:]
+        dq, dk, dv = dqkv.split((Hq * D, Hkv * D, Hkv * D), 1)
         if layout.tiles:
             delta = torch.empty_like(lse)
             part = torch.empty(2 * lse.numel() * D, device=q.device, dtype=torch.float32) if layout.splits_heads(Hq, Hkv) else None

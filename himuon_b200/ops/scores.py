@@ -9,10 +9,9 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _ext
-from . import _count, gemm, use_kernels
+from . import _count, _once, _with_kernel_rows, gemm, use_kernels
 from . import reference as ref
 
 MAX_TOP_K = 32
@@ -32,30 +31,34 @@ def _incoming(g: torch.Tensor | None):
     return None if g is None else g.to(torch.float32).contiguous()
 
 
+def _scores(logits, ids, top_k, ignore_index, keep: bool):
+    """log_probs, entropy, alternatives, and with ``keep`` the two numbers a row that the gradient needs."""
+    rows, dev = logits.shape[0], logits.device
+    log_probs = torch.empty(rows, device=dev, dtype=torch.float32)
+    entropy = torch.empty(rows, device=dev, dtype=torch.float32)
+    stats = torch.empty(rows, 2, device=dev, dtype=torch.float32) if keep else None
+    top_lp = torch.empty(rows, top_k, device=dev, dtype=torch.float32) if top_k else None
+    top_ids = torch.empty(rows, top_k, device=dev, dtype=torch.int64) if top_k else None
+    if rows:
+        _ext.ext().token_scores_fwd(logits, ids, log_probs, entropy, stats, top_lp, top_ids, ignore_index)
+        _count()
+    return log_probs, entropy, top_lp, top_ids, stats
+
+
 class _TokenLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, top_k, ignore_index):
         ctx.set_materialize_grads(False)              # the gradient of an unused output arrives as None
-        rows, dev = logits.shape[0], logits.device
-        log_probs = torch.empty(rows, device=dev, dtype=torch.float32)
-        entropy = torch.empty_like(log_probs)
-        need = ctx.needs_input_grad[0]
-        stats = torch.empty(rows, 2, device=dev, dtype=torch.float32) if need else None
-        top_lp = torch.empty(rows, top_k, device=dev, dtype=torch.float32) if top_k else None
-        top_ids = torch.empty(rows, top_k, device=dev, dtype=torch.int64) if top_k else None
-        if rows:
-            _ext.ext().token_scores_fwd(logits, ids, log_probs, entropy, stats, top_lp, top_ids, ignore_index)
-            _count()
-        if need:
-            ctx.save_for_backward(logits, ids, entropy, stats)
-            ctx.ignore_index = ignore_index
+        log_probs, entropy, top_lp, top_ids, stats = _scores(logits, ids, top_k, ignore_index, True)
+        ctx.save_for_backward(logits, ids, entropy, stats)
+        ctx.ignore_index = ignore_index
         if top_k:
             ctx.mark_non_differentiable(top_lp, top_ids)
         return log_probs, entropy, top_lp, top_ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_log_probs, g_entropy, *_):
+        _once("token_log_probs")
         if g_log_probs is None and g_entropy is None:
             return None, None, None, None
         logits, ids, entropy, stats = ctx.saved_tensors
@@ -88,7 +91,9 @@ def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ign
     if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32):
         if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
             logits = logits.contiguous()
-        return TokenLogProbs(*_TokenLogProbsFn.apply(logits, ids, int(top_k), int(ignore_index)))
+        if torch.is_grad_enabled() and logits.requires_grad:
+            return TokenLogProbs(*_TokenLogProbsFn.apply(logits, ids, int(top_k), int(ignore_index)))
+        return TokenLogProbs(*_scores(logits, ids, int(top_k), int(ignore_index), False)[:4])
     return TokenLogProbs(*ref.token_log_probs(logits, ids, top_k, ignore_index))
 
 
@@ -102,6 +107,9 @@ def _long_product(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> None:
     sms = _ext.ext().num_sms()
     slots, tile = (sms // 2, 256) if pairs else (sms, 128)
     tiles = -(-rows // tile) * -(-cols // 256)
+    if tiles >= 4 * slots or inner < 8192:
+        gemm(a, b, out=out)
+        return
     unit = tile * 256 * 2 * inner / (1.4e15 / slots)           # seconds of one tile, whole
     best, cuts = None, 1
     for s in range(1, min(16, inner // 4096) + 1):
@@ -124,43 +132,51 @@ def _long_product(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor) -> None:
     _count()
 
 
+LAUNCH_ROWS = 8192               # of one launch: their hidden states stay in the L2 while the weight streams by
+GRADIENT_VALUES = 2 ** 31        # most values of the logits' gradient alive at once (4 GiB)
+
+
+def _linear_scores(h, w, ids, ignore_index, keep: bool):
+    rows, vocab, e = h.shape[0], w.shape[0], _ext.ext()
+    log_probs = torch.empty(rows, device=h.device, dtype=torch.float32)
+    entropy = torch.empty(rows, device=h.device, dtype=torch.float32)
+    stats = torch.empty(rows, 2, device=h.device, dtype=torch.float32) if keep else None
+    if rows == 0:
+        return log_probs, entropy, stats
+    scratch = torch.empty(e.linear_scores_scratch(min(rows, LAUNCH_ROWS), vocab), device=h.device, dtype=torch.float32)
+    if rows <= LAUNCH_ROWS:
+        e.linear_scores_fwd(h, w, ids, log_probs, entropy, stats, scratch, ignore_index)
+        _count(2)
+        return log_probs, entropy, stats
+    for r in range(0, rows, LAUNCH_ROWS):
+        c = slice(r, min(rows, r + LAUNCH_ROWS))
+        e.linear_scores_fwd(h[c], w, ids[c], log_probs[c], entropy[c], stats[c] if keep else None, scratch, ignore_index)
+        _count(2)
+    return log_probs, entropy, stats
+
+
 class _LinearTokenLogProbsFn(torch.autograd.Function):
     """The forward pass keeps two numbers a row; the backward pass makes the logits again, as their gradient in bf16, and
     multiplies that with both operands."""
 
-    ROWS = 8192                  # of one launch: their hidden states stay in the L2 while the weight streams by
-    CHUNK = 2 ** 31              # most values of the logits' gradient alive at once (4 GiB)
-
     @staticmethod
     def forward(ctx, h, w, ids, ignore_index):
         ctx.set_materialize_grads(False)
-        rows, vocab, e = h.shape[0], w.shape[0], _ext.ext()
-        log_probs = torch.empty(rows, device=h.device, dtype=torch.float32)
-        entropy = torch.empty_like(log_probs)
-        need = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        stats = torch.empty(rows, 2, device=h.device, dtype=torch.float32) if need else None
-        step = _LinearTokenLogProbsFn.ROWS
-        if rows:
-            scratch = torch.empty(e.linear_scores_scratch(min(rows, step), vocab), device=h.device, dtype=torch.float32)
-        for r in range(0, rows, step):
-            c = slice(r, min(rows, r + step))
-            e.linear_scores_fwd(h[c], w, ids[c], log_probs[c], entropy[c], stats[c] if need else None, scratch, ignore_index)
-            _count(2)
-        if need:
-            ctx.save_for_backward(h, w, ids, entropy, stats)
-            ctx.ignore_index = ignore_index
+        log_probs, entropy, stats = _linear_scores(h, w, ids, ignore_index, True)
+        ctx.save_for_backward(h, w, ids, entropy, stats)
+        ctx.ignore_index = ignore_index
         return log_probs, entropy
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_log_probs, g_entropy):
+        _once("linear_token_log_probs")
         if g_log_probs is None and g_entropy is None:
             return None, None, None, None
         h, w, ids, entropy, stats = ctx.saved_tensors
         rows, vocab = h.shape[0], w.shape[0]
         g, ge = _incoming(g_log_probs), _incoming(g_entropy)
         cols = (vocab + 7) // 8 * 8
-        step = max(256, min(_LinearTokenLogProbsFn.ROWS, _LinearTokenLogProbsFn.CHUNK // cols // 256 * 256))
+        step = max(256, min(LAUNCH_ROWS, GRADIENT_VALUES // cols // 256 * 256))
         dh = torch.empty(h.shape, device=h.device, dtype=h.dtype) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:
@@ -169,17 +185,21 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
         if rows:
             buf = torch.empty(min(rows, step), cols, device=h.device, dtype=torch.bfloat16)
         for r in range(0, rows, step):
-            c = slice(r, min(rows, r + step))
-            dx = buf[: c.stop - r]
-            _ext.ext().linear_scores_dlogits(h[c], w, ids[c], entropy[c], stats[c], None if g is None else g[c], None if ge is None else ge[c], dx,
-                                             ctx.ignore_index)
+            part, dx, to = (h, ids, entropy, stats, g, ge), buf, dh
+            if rows > step:
+                c = slice(r, min(rows, r + step))
+                part, dx = tuple(None if t is None else t[c] for t in part), buf[: c.stop - r]
+                to = None if dh is None else dh[c]
+            hc, idc, ec, sc, gc, gec = part
+            _ext.ext().linear_scores_dlogits(hc, w, idc, ec, sc, gc, gec, dx, ctx.ignore_index)
             _count()
-            dx = dx[:, :vocab]
-            if dh is not None:
-                _long_product(dx, w, dh[c])
+            if cols != vocab:
+                dx = dx[:, :vocab]
+            if to is not None:
+                _long_product(dx, w, to)
             if dw is not None:
-                gemm(dx, h[c], trans_a=True, out=dw, aux=dw if r else None, beta=1.0 if r else 0.0)
-        return dh, None if dw is None else dw.to(w.dtype), None, None
+                gemm(dx, hc, trans_a=True, out=dw, aux=dw if r else None, beta=1.0 if r else 0.0)
+        return dh, dw if dw is None or dw.dtype == w.dtype else dw.to(w.dtype), None, None
 
 
 def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, ignore_index: int = -100) -> TokenLogProbs:
@@ -189,8 +209,9 @@ def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor
         raise RuntimeError("himuon_b200.ops.linear_token_log_probs: (rows, hidden) and (vocab, hidden) of one type on one device expected")
     ids = _check_ids("linear_token_log_probs", ids, h2d.shape[0], h2d.device)
     if use_kernels(h2d) and h2d.shape[1] % 8 == 0 and h2d.shape[1] > 0:
-        h2d, w = (t if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-                  for t in (h2d, w))
-        return TokenLogProbs(*_LinearTokenLogProbsFn.apply(h2d, w, ids, int(ignore_index)))
+        h2d, w = _with_kernel_rows(h2d), _with_kernel_rows(w)
+        if torch.is_grad_enabled() and (h2d.requires_grad or w.requires_grad):
+            return TokenLogProbs(*_LinearTokenLogProbsFn.apply(h2d, w, ids, int(ignore_index)))
+        return TokenLogProbs(*_linear_scores(h2d, w, ids, int(ignore_index), False)[:2])
     logits = h2d @ w.t() if h2d.dtype in (torch.float32, torch.float64) else h2d.float() @ w.float().t()
     return TokenLogProbs(*ref.token_log_probs(logits, ids, 0, ignore_index))

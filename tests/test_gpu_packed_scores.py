@@ -149,6 +149,19 @@ def test_packed_attention_gradient_against_differences():
         assert abs(got - slope) <= (want["b" + name] * d.abs()).sum().item() + 1e-5 * abs(slope)
 
 
+def test_gradients_are_not_differentiable_again():
+    ops = _ops()
+    q = torch.randn(20, 64, device="cuda").bfloat16().requires_grad_()
+    x, ids = torch.randn(4, 64, device="cuda", requires_grad=True), torch.zeros(4, dtype=torch.int64, device="cuda")
+    h, w = torch.randn(4, 64, device="cuda").bfloat16().requires_grad_(), torch.randn(100, 64, device="cuda").bfloat16()
+    for out, leaf in ((ops.packed_attention(q, q.detach(), q.detach(), ops.PackedLayout([20]), 1, 1, 64), q), (ops.token_log_probs(x, ids).entropy, x),
+                      (ops.linear_token_log_probs(h, w, ids).entropy, h)):
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            torch.autograd.grad(out.sum(), leaf, create_graph=True)
+        torch.autograd.grad(out.sum(), leaf)
+    _clean()
+
+
 def test_packed_attention_keeps_documents_apart():
     """NaN and infinities in one document and in the padding reach no other document, forward or backward."""
     ops = _ops()
@@ -417,7 +430,7 @@ def test_linear_token_log_probs(rows, hidden, vocab):
 
 
 def test_linear_token_log_probs_in_chunks(monkeypatch):
-    """Row by row nothing depends on how many rows a call has; the weight's gradient is summed over the chunks."""
+    """Nothing of a row depends on the chunk that it is in; the weight's gradient is summed over the chunks."""
     ops = _ops()
     from himuon_b200.ops import scores
 
@@ -432,7 +445,8 @@ def test_linear_token_log_probs_in_chunks(monkeypatch):
         return (s.log_probs, s.entropy, *torch.autograd.grad((s.log_probs, s.entropy), (h, w), (g, g)))
 
     whole = both()
-    monkeypatch.setattr(scores._LinearTokenLogProbsFn, "CHUNK", 256 * 1000)
+    monkeypatch.setattr(scores, "GRADIENT_VALUES", 256 * 1000)
+    monkeypatch.setattr(scores, "LAUNCH_ROWS", 300)      # (up to 256 rows the tiles have another width)
     parts = both()
     for a, b in zip(whole[:3], parts[:3]):
         assert torch.equal(a, b)
