@@ -422,28 +422,41 @@ static himuon::LinearScoreArgs linear_score_args(const char* op, const at::Tenso
   }
   return a;
 }
+// Kept exponentials or the gradient of the logits, and the maxima that belong to the former: `slab_max` (rows, vocab / 64 rounded up).
+static void linear_score_kept(const char* op, himuon::LinearScoreArgs& a, const at::Tensor& h, const at::Tensor& kept, const c10::optional<at::Tensor>& slab_max) {
+  const std::string at = std::string("himuon: ") + op;
+  // (whole 16-byte groups of columns are written: the row stride covers them)
+  TORCH_CHECK(kept.device() == h.device() && is_bf16(kept) && kept.dim() == 2 && kept.size(0) == a.rows && kept.size(1) == (a.vocab + 7) / 8 * 8 && kept.is_contiguous() &&
+                  reinterpret_cast<uintptr_t>(kept.data_ptr()) % 16 == 0, at, ": the gradient must be contiguous bf16, its columns rounded up to a multiple of 8");
+  a.grad = kept.data_ptr(); a.ld_grad = kept.stride(0);
+  if (slab_max.has_value()) {
+    TORCH_CHECK(slab_max->device() == h.device() && is_f32(*slab_max) && slab_max->dim() == 2 && slab_max->size(0) == a.rows && slab_max->size(1) == (a.vocab + 63) / 64 &&
+                    slab_max->is_contiguous(), at, ": slab_max must be fp32, (rows, vocab / 64 rounded up)");
+    a.slab_max = slab_max->data_ptr<float>();
+  }
+}
 static void linear_scores_fwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, at::Tensor& log_probs, at::Tensor& entropy,
-                              const c10::optional<at::Tensor>& stats, at::Tensor& scratch, int64_t ignore_index) {
+                              const c10::optional<at::Tensor>& stats, at::Tensor& scratch, int64_t ignore_index, const c10::optional<at::Tensor>& kept,
+                              const c10::optional<at::Tensor>& slab_max) {
   himuon::LinearScoreArgs a = linear_score_args("linear_scores_fwd", h, w, ids, entropy, stats, ignore_index);
   HM_CHECK(log_probs.device() == h.device() && is_f32(log_probs) && log_probs.is_contiguous() && log_probs.numel() == a.rows, "linear_scores_fwd: log_probs must be fp32, one for each row");
   HM_CHECK(scratch.device() == h.device() && is_f32(scratch) && scratch.is_contiguous() && scratch.numel() >= himuon::linear_scores_scratch(a.rows, a.vocab), "linear_scores_fwd: scratch too small");
   a.log_probs = log_probs.data_ptr<float>();
   a.scratch = scratch.data_ptr<float>();
+  HM_CHECK(kept.has_value() == slab_max.has_value(), "linear_scores_fwd: kept exponentials need their maxima");
+  if (kept.has_value()) linear_score_kept("linear_scores_fwd", a, h, *kept, slab_max);
   const c10::cuda::CUDAGuard guard(h.device());
   himuon::linear_scores_fwd(a, cur_stream());
 }
 static void linear_scores_dlogits(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, const at::Tensor& entropy, const at::Tensor& stats,
                                   const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy, at::Tensor& grad,
-                                  int64_t ignore_index) {
+                                  const c10::optional<at::Tensor>& slab_max, int64_t ignore_index) {
   himuon::LinearScoreArgs a = linear_score_args("linear_scores_dlogits", h, w, ids, entropy, stats, ignore_index);
   for (const auto* g : {&g_log_probs, &g_entropy})
     if (g->has_value()) HM_CHECK((*g)->device() == h.device() && is_f32(**g) && (*g)->is_contiguous() && (*g)->numel() == a.rows, "linear_scores_dlogits: incoming gradients must be fp32, one for each row");
-  // (whole 16-byte groups of columns are written: the row stride covers them)
-  HM_CHECK(grad.device() == h.device() && is_bf16(grad) && grad.dim() == 2 && grad.size(0) == a.rows && grad.size(1) == (a.vocab + 7) / 8 * 8 && grad.is_contiguous() &&
-               reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0, "linear_scores_dlogits: the gradient must be contiguous bf16, its columns rounded up to a multiple of 8");
+  linear_score_kept("linear_scores_dlogits", a, h, grad, slab_max);
   a.g_log_probs = g_log_probs.has_value() ? g_log_probs->data_ptr<float>() : nullptr;
   a.g_entropy = g_entropy.has_value() ? g_entropy->data_ptr<float>() : nullptr;
-  a.grad = grad.data_ptr(); a.ld_grad = grad.stride(0);
   const c10::cuda::CUDAGuard guard(h.device());
   himuon::linear_scores_dlogits(a, cur_stream());
 }

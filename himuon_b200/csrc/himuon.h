@@ -196,7 +196,8 @@ void token_scores_bwd(const TokenScoreArgs& a, cudaStream_t s);
 
 // The same from hidden states (rows, hidden) and the head's weight (vocab, hidden), bf16, hidden a multiple of 8, row strides of
 // multiples of 8; logits stay on the chip (linear_scores_sm100.cu).  scratch: linear_scores_scratch() floats, forward only.
-// linear_scores_dlogits writes the logits' gradient, (rows, vocab) bf16 with row stride ld_grad, a multiple of 8 of at least vocab.
+// linear_scores_dlogits writes the logits' gradient, (rows, ld_grad) bf16, ld_grad the vocabulary rounded up to a multiple of 8.  With `grad` the
+// forward call keeps its exponentials there, as fp16, and with slab_max the other one turns them into the gradient in their place.
 struct LinearScoreArgs {
   const void* h; const void* w;
   long long ld_h, ld_w; int rows, hidden, vocab;
@@ -204,6 +205,7 @@ struct LinearScoreArgs {
   float* log_probs; float* entropy; float* stats; float* scratch;
   const float* g_log_probs; const float* g_entropy;
   void* grad; long long ld_grad;
+  float* slab_max;                           // (rows, vocabulary / 64 rounded up) maxima that kept exponentials are relative to
 };
 long long linear_scores_scratch(long long rows, int vocab);
 void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s);

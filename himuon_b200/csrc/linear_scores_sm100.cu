@@ -3,12 +3,15 @@
 //
 //   forward:   x = h W^T tile by tile; of each row of a tile only m = max x, s = sum e^(x-m), t = sum (x-m) e^(x-m) leave the kernel
 //              (and the logit of the row's own token); linear_scores_join_kernel merges a row's tiles (formulas in token_scores.cu).
-//   gradient:  the same product again, whose epilogue turns x into dx_j = g [j = y] - p_j (g + h (log p_j + H)) and stores it as bf16,
-//              the operand of the products dx W and dx^T h that follow.
+//   gradient:  dx_j = g [j = y] - p_j (g + h (log p_j + H)) as bf16, the operand of the products dx W and dx^T h that follow.  Either from the
+//              same product again, or, where the forward pass could keep them, from its exponentials: e^(x - m of 64 columns), at most 1,
+//              as fp16 (11 bits where the gradient gets 8; below 6e-8 of the largest of 64 they count for nothing), which the gradient then
+//              takes the place of.
 //
 // The product is the pair GEMM's (gemm2_sm100.cu has its protocol): 256 rows by BN vocabulary entries per pair, six stages of 64 along
 // the hidden size, two accumulators, so that the epilogue of one tile runs beside the products of the next.  The tiles of one
 // vocabulary block are neighbours in the schedule: its rows of W come from memory once, the hidden states from the L2.
+#include <cuda_fp16.h>
 #include <stdint.h>
 
 #include "gemm_epilogue.cuh"
@@ -26,8 +29,12 @@ constexpr int LS_THREADS = 384;      // warps 0-3: TMA, MMA, TMEM allocation, no
 constexpr int LS_STAGES = 6;
 constexpr uint32_t LS_A = BM * BK * 2, LS_STAGE = 2 * LS_A;      // 128 rows of h, and up to 128 of W, a CTA
 
+enum { STATS, GRAD, STATS_KEPT };    // what the epilogue makes of the logits; STATS_KEPT: sums, and the exponentials
+
 struct LinScoresDev {
   const long long* ids;
+  float* slab_max;                   // STATS_KEPT: m of each (row, 64 columns)
+  int slabs;
   float* part;                       // forward: m, s and t of each (part of the vocabulary, row), in three blocks of n_parts * rows
   float* target;                     // forward: the logit of each row's own id
   const float2* stats;               // gradient: as row_grad() takes them
@@ -39,16 +46,48 @@ struct LinScoresDev {
   int* status;
 };
 
+// A row's sums over one part of the vocabulary.
+__device__ __forceinline__ void put_sums(const LinScoresDev& p, const Sums& a, int part, int row) {
+  const long long n = static_cast<long long>(p.tiles_n) * 2 * p.rows, i = static_cast<long long>(part) * p.rows + row;
+  p.part[i] = a.m;
+  p.part[n + i] = a.s;
+  p.part[2 * n + i] = a.t;
+}
+// The sums over 64 logits, and their exponentials relative to the largest, as fp16 pairs.
+__device__ __forceinline__ Sums exponentials64(const float (&x)[64], uint32_t (&o)[32]) {
+  const float m = largest<64>(x), base = m == -INFINITY ? 0.f : m;
+  const f32x2 nbase = pack2(-base, -base), l2e = pack2(kLog2eS, kLog2eS);
+  f32x2 s[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)}, t[2] = {s[0], s[0]};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const f32x2 d = add2(pack2(x[2 * i], x[2 * i + 1]), nbase);
+    float y0, y1, d0, d1;
+    unpack2(mul2(d, l2e), y0, y1);
+    unpack2(d, d0, d1);
+    y0 = exp2f(y0);
+    y1 = exp2f(y1);
+    const f32x2 e = pack2(y0, y1);
+    s[i & 1] = add2(s[i & 1], e);
+    t[i & 1] = fma2(pack2(fmaxf(d0, kFar), fmaxf(d1, kFar)), e, t[i & 1]);
+    const __half2 h = __floats2half2_rn(y0, y1);
+    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  float s0, s1, t0, t1;
+  unpack2(add2(s[0], s[1]), s0, s1);
+  unpack2(add2(t[0], t[1]), t0, t1);
+  return Sums{m, s0 + s1, t0 + t1};
+}
+
 }  // namespace
 
-template <bool GRAD>
+template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LS_THREADS, 1)
 linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmD,
                      LinScoresDev p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_up_1024(smem_raw);
   uint8_t* slabs = smem + LS_STAGES * LS_STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(slabs + (GRAD ? 2 * SLAB_BYTES : 0));
+  uint64_t* full = reinterpret_cast<uint64_t*>(slabs + (MODE == STATS ? 0 : 2 * SLAB_BYTES));
   uint64_t* empty = full + LS_STAGES;
   uint64_t* tfull = empty + LS_STAGES;
   uint64_t* tempty = tfull + 2;
@@ -140,7 +179,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
       const bool row_ok = row < p.rows;
       RowGrad rg{};
       long long id = -1;
-      if constexpr (GRAD) {
+      if constexpr (MODE == GRAD) {
         if (row_ok) rg = row_grad(p.stats, p.entropy, p.ids, p.g_log_probs, p.g_entropy, p.ignore, p.vocab, row);
       } else {
         if (row_ok) id = p.ids[row];
@@ -149,39 +188,39 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
       if (!named_barrier_and(1 + 2 * group, 128, mbar_wait(&tfull[acc], acc_phase, abort_flag, p.status, 3))) break;
       tc_fence_after();
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * 256);
-      if constexpr (!GRAD) {
-        Sums a{-INFINITY, 0.f, 0.f};
-#pragma unroll 1
-        for (int c = group * 32; c < p.bn; c += 64) {
-          if (n0 + c >= p.vocab) break;                       // uniform over the group
-          uint32_t v[32];
-          float x[32];
-          tmem_ld32(t_acc + c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = n0 + c + j < p.vocab ? __uint_as_float(v[j]) : -INFINITY;
-          take<32>(a, x, largest<32>(x));
-          const long long at = id - (n0 + c);
-          if (at >= 0 && at < 32 && id < p.vocab) {           // a row's own token: in one of its tiles
-            float mine = x[0];
-#pragma unroll
-            for (int j = 1; j < 32; ++j) mine = at == j ? x[j] : mine;
-            p.target[row] = mine;
-          }
-        }
-        if (row_ok) {
-          const long long n = static_cast<long long>(p.tiles_n) * 2 * p.rows, i = (static_cast<long long>(nt) * 2 + group) * p.rows + row;
-          p.part[i] = a.m;
-          p.part[n + i] = a.s;
-          p.part[2 * n + i] = a.t;
-        }
-      } else if (m0 < p.rows) {                               // uniform: the second CTA of a ragged last row block has nothing to store
+      if (MODE == STATS || m0 < p.rows) {                     // uniform: the second CTA of a ragged last row block has nothing to store
         uint8_t* my_row = slab + (ew * 32 + lane) * 128;
+        Sums a{-INFINITY, 0.f, 0.f};
 #pragma unroll 1
         for (int c = group * 64; c < p.bn; c += 128) {
           const int col = n0 + c;
           if (col >= p.vocab) break;
           uint32_t o[32];
+          if constexpr (MODE != GRAD) {
+            float x[64];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint32_t v[32];
+              tmem_ld32(t_acc + c + half * 32, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[half * 32 + j] = __uint_as_float(v[j]);
+            }
+            if (col + 64 > p.vocab) {
+#pragma unroll
+              for (int j = 0; j < 64; ++j) x[j] = col + j < p.vocab ? x[j] : -INFINITY;
+            }
+            const long long at = id - col;
+            if (at >= 0 && at < 64 && id < p.vocab) {         // a row's own token: in one of its tiles
+              float mine = x[0];
+#pragma unroll
+              for (int j = 1; j < 64; ++j) mine = at == j ? x[j] : mine;
+              p.target[row] = mine;
+            }
+            const Sums b = exponentials64(x, o);
+            a = merged(a, b);
+            if (MODE == STATS_KEPT && row_ok) p.slab_max[static_cast<long long>(row) * p.slabs + col / 64] = b.m;
+          } else {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint32_t v[32];
@@ -191,6 +230,8 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
             for (int j = 0; j < 32; j += 2)
               o[half * 16 + j / 2] = pack_bf16x2(grad_of(rg, __uint_as_float(v[j]), col + half * 32 + j), grad_of(rg, __uint_as_float(v[j + 1]), col + half * 32 + j + 1));
           }
+          }
+          if constexpr (MODE == STATS) continue;
           if (issuer) tma_store_wait_read<0>();
           named_barrier(1 + 2 * group, 128);                  // the slab is free
 #pragma unroll
@@ -203,6 +244,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
             tma_store_commit();
           }
         }
+        if (MODE != GRAD && row_ok) put_sums(p, a, nt * 2 + group, row);
       }
       tc_fence_before();
       __syncwarp();
@@ -210,7 +252,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
-    if (GRAD && issuer) tma_store_wait_all();
+    if (MODE != STATS && issuer) tma_store_wait_all();
   }
 
   tc_fence_before();
@@ -407,6 +449,63 @@ linear_scores_join_kernel(LinScoresDev p, int n_parts, float* log_probs, float* 
   }
 }
 
+// Kept exponentials of a row into the gradient of its logits, in their place.  A thread has 8 columns, which share their 64's maximum.
+__global__ void __launch_bounds__(256)
+kept_to_gradient_kernel(LinScoresDev p, uint4* kept, int groups, int blocks_per_row) {
+  const long long row = blockIdx.x / blocks_per_row;
+  const int piece = static_cast<int>(blockIdx.x - row * blocks_per_row);
+  const RowGrad r = row_grad(p.stats, p.entropy, p.ids, p.g_log_probs, p.g_entropy, p.ignore, p.vocab, row);
+  uint4 raw[4];
+  float f[4];                                         // log p = log e + f,  f = m of the 64 - m of the row - log s
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int i = (piece * 4 + u) * 256 + static_cast<int>(threadIdx.x);
+    if (i < groups) {
+      raw[u] = __ldcs(kept + row * groups + i);
+      f[u] = (p.slab_max[row * p.slabs + (i >> 3)] - r.m) - r.log_s;
+      f[u] = f[u] < kFar ? kFar : f[u];               // (-inf must not meet the 0 that it stands for; NaN stays)
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int i = (piece * 4 + u) * 256 + static_cast<int>(threadIdx.x);
+    if (i >= groups) break;
+    const float scale = exp2f(f[u] * kLog2eS);
+    const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+    f32x2 d[4];
+    const f32x2 by = pack2(-scale, -scale), c0 = pack2(r.c0, r.c0);
+    if (r.h == 0.f) {                                 // uniform
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
+        d[q] = mul2(mul2(pack2(e.x, e.y), by), c0);
+      }
+    } else {
+      const float h2 = r.h / kLog2eS;                 // c0 + h log p = (c0 + h f) + h / log2(e) * log2(e^x)
+      const f32x2 h = pack2(h2, h2), c = pack2(fmaf(r.h, f[u], r.c0), fmaf(r.h, f[u], r.c0));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
+        // (an exponential of 0 gets the log of the least that fp16 has, and the product is 0 all the same)
+        const f32x2 l = pack2(__log2f(fmaxf(e.x, 5.9604645e-8f)), __log2f(fmaxf(e.y, 5.9604645e-8f)));
+        d[q] = mul2(mul2(pack2(e.x, e.y), by), fma2(h, l, c));
+      }
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float d0, d1;
+      unpack2(d[q], d0, d1);
+      if (r.y >> 3 == i) {                            // the group of the row's own token
+        if ((r.y & 7) == 2 * q) d0 += r.g;
+        if ((r.y & 7) == 2 * q + 1) d1 += r.g;
+      }
+      o[q] = pack_bf16x2(d0, d1);
+    }
+    __stcs(kept + row * groups + i, make_uint4(o[0], o[1], o[2], o[3]));
+  }
+}
+
 // out = sum of n_parts fp32 matrices of n elements, in their order.
 __global__ void __launch_bounds__(256)
 sum_parts_kernel(const float4* __restrict__ parts, uint2* __restrict__ out, long long n4, int n_parts) {
@@ -428,6 +527,7 @@ static CUtensorMap rows_tmap(const void* ptr, int rows, int cols, long long ld, 
   return make_tmap(ptr, 3, dims, strides, box, 2, true);
 }
 
+template <int MODE>
 static int pairs_at_once(size_t smem) {
   static int most = 0;
   if (most == 0) {
@@ -441,7 +541,7 @@ static int pairs_at_once(size_t smem) {
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, linear_scores_kernel<true>, &cfg) == cudaSuccess && n > 0) most = n;
+    if (cudaOccupancyMaxActiveClusters(&n, linear_scores_kernel<MODE>, &cfg) == cudaSuccess && n > 0) most = n;
     else { cudaGetLastError(); most = num_sms() / 2; }
   }
   return most;
@@ -460,25 +560,23 @@ static int tile_width(int rows, int vocab, int pairs) {
   return best;
 }
 
-template <bool GRAD>
+template <int MODE>
 static void launch(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + LS_STAGES * LS_STAGE + 2 * SLAB_BYTES + 256;
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
-  for (auto k : {linear_scores_kernel<false>, linear_scores_kernel<true>}) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
-    if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores: ") + cudaGetErrorString(e));
-  }
-  const int pairs = pairs_at_once(SMEM);
-  p.bn = GRAD ? 256 : tile_width(p.rows, p.vocab, pairs);
+  const cudaError_t set = cudaFuncSetAttribute(linear_scores_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
+  if (set != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores: ") + cudaGetErrorString(set));
+  const int pairs = pairs_at_once<MODE>(SMEM);
+  p.bn = MODE == GRAD ? 256 : tile_width(p.rows, p.vocab, pairs);
   p.tiles_m = (p.rows + 2 * BM - 1) / (2 * BM);
   p.tiles_n = (p.vocab + p.bn - 1) / p.bn;
   p.kblocks = (a.hidden + BK - 1) / BK;
   const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
   if (total >= (1LL << 30)) throw std::runtime_error("himuon linear_scores: too many tiles for one launch");
   const CUtensorMap th = rows_tmap(a.h, a.rows, a.hidden, a.ld_h, BM), tw = rows_tmap(a.w, a.vocab, a.hidden, a.ld_w, p.bn / 2),
-                    td = GRAD ? rows_tmap(a.grad, a.rows, static_cast<int>(a.ld_grad), a.ld_grad, BM) : th;
+                    td = MODE == STATS ? th : rows_tmap(a.grad, a.rows, static_cast<int>(a.ld_grad), a.ld_grad, BM);
   const int grid = 2 * static_cast<int>(total < pairs ? total : pairs);
-  linear_scores_kernel<GRAD><<<grid, LS_THREADS, SMEM, s>>>(th, tw, td, p);
+  linear_scores_kernel<MODE><<<grid, LS_THREADS, SMEM, s>>>(th, tw, td, p);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores launch failed: ") + cudaGetErrorString(e));
 }
@@ -519,10 +617,15 @@ long long linear_scores_scratch(long long rows, int vocab) { return rows * (1 + 
 void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {
   LinScoresDev p = make_dev(a);
   int n_parts;
-  if (a.rows <= 32) {
+  if (a.grad != nullptr) {
+    p.slab_max = a.slab_max;
+    p.slabs = (a.vocab + 63) / 64;
+    launch<STATS_KEPT>(a, p, s);
+    n_parts = 2 * p.tiles_n;
+  } else if (a.rows <= 32) {
     n_parts = a.rows <= 16 ? launch_few<16>(a, p, s) : launch_few<32>(a, p, s);
   } else {
-    launch<false>(a, p, s);
+    launch<STATS>(a, p, s);
     n_parts = 2 * p.tiles_n;
   }
   float2* stats = reinterpret_cast<float2*>(a.stats);
@@ -543,7 +646,17 @@ void sum_parts(const float* parts, void* out, long long n, int n_parts, cudaStre
 
 void linear_scores_dlogits(const LinearScoreArgs& a, cudaStream_t s) {
   LinScoresDev p = make_dev(a);
-  launch<true>(a, p, s);
+  if (a.slab_max != nullptr) {
+    p.slab_max = a.slab_max;
+    p.slabs = (a.vocab + 63) / 64;
+    const int groups = static_cast<int>(a.ld_grad / 8), per_row = (groups + 1023) / 1024;
+    if (static_cast<long long>(a.rows) * per_row >= (1LL << 31)) throw std::runtime_error("himuon linear_scores: gradient too large for one launch");
+    kept_to_gradient_kernel<<<a.rows * per_row, 256, 0, s>>>(p, reinterpret_cast<uint4*>(a.grad), groups, per_row);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores gradient launch failed: ") + cudaGetErrorString(e));
+    return;
+  }
+  launch<GRAD>(a, p, s);
 }
 
 }  // namespace himuon

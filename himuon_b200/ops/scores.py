@@ -137,32 +137,38 @@ GRADIENT_VALUES = 2 ** 31        # most values of the logits' gradient alive at 
 
 
 def _linear_scores(h, w, ids, ignore_index, keep: bool):
+    """log_probs, entropy, and with ``keep`` what the gradient needs: two numbers a row, and, where they fit, the exponentials of the
+    logits in the buffer that their gradient will have, with the maxima of each 64 of them."""
     rows, vocab, e = h.shape[0], w.shape[0], _ext.ext()
     log_probs = torch.empty(rows, device=h.device, dtype=torch.float32)
     entropy = torch.empty(rows, device=h.device, dtype=torch.float32)
     stats = torch.empty(rows, 2, device=h.device, dtype=torch.float32) if keep else None
-    if rows == 0:
-        return log_probs, entropy, stats
-    scratch = torch.empty(e.linear_scores_scratch(min(rows, LAUNCH_ROWS), vocab), device=h.device, dtype=torch.float32)
-    if rows <= LAUNCH_ROWS:
-        e.linear_scores_fwd(h, w, ids, log_probs, entropy, stats, scratch, ignore_index)
-        _count(2)
-        return log_probs, entropy, stats
+    cols = (vocab + 7) // 8 * 8
+    kept = slab_max = None
+    if keep and rows > 32 and rows * cols <= GRADIENT_VALUES:        # (a few rows have a kernel that keeps nothing)
+        kept = torch.empty(rows, cols, device=h.device, dtype=torch.bfloat16)
+        slab_max = torch.empty(rows, (vocab + 63) // 64, device=h.device, dtype=torch.float32)
+    if rows:
+        scratch = torch.empty(e.linear_scores_scratch(min(rows, LAUNCH_ROWS), vocab), device=h.device, dtype=torch.float32)
     for r in range(0, rows, LAUNCH_ROWS):
-        c = slice(r, min(rows, r + LAUNCH_ROWS))
-        e.linear_scores_fwd(h[c], w, ids[c], log_probs[c], entropy[c], stats[c] if keep else None, scratch, ignore_index)
+        if rows <= LAUNCH_ROWS:
+            e.linear_scores_fwd(h, w, ids, log_probs, entropy, stats, scratch, ignore_index, kept, slab_max)
+        else:
+            c = slice(r, min(rows, r + LAUNCH_ROWS))
+            e.linear_scores_fwd(h[c], w, ids[c], log_probs[c], entropy[c], stats[c] if keep else None, scratch, ignore_index,
+                                None if kept is None else kept[c], None if kept is None else slab_max[c])
         _count(2)
-    return log_probs, entropy, stats
+    return log_probs, entropy, stats, kept, slab_max
 
 
 class _LinearTokenLogProbsFn(torch.autograd.Function):
-    """The forward pass keeps two numbers a row; the backward pass makes the logits again, as their gradient in bf16, and
-    multiplies that with both operands."""
+    """The backward pass multiplies the logits' gradient with both operands.  It gets it from the exponentials that the forward pass kept, in
+    their place; where there are none (too many, or used up by an earlier backward pass) it makes the logits again."""
 
     @staticmethod
     def forward(ctx, h, w, ids, ignore_index):
         ctx.set_materialize_grads(False)
-        log_probs, entropy, stats = _linear_scores(h, w, ids, ignore_index, True)
+        log_probs, entropy, stats, *ctx.kept = _linear_scores(h, w, ids, ignore_index, True)
         ctx.save_for_backward(h, w, ids, entropy, stats)
         ctx.ignore_index = ignore_index
         return log_probs, entropy
@@ -175,15 +181,17 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
         h, w, ids, entropy, stats = ctx.saved_tensors
         rows, vocab = h.shape[0], w.shape[0]
         g, ge = _incoming(g_log_probs), _incoming(g_entropy)
+        (buf, slab_max), ctx.kept = ctx.kept, (None, None)
         cols = (vocab + 7) // 8 * 8
-        step = max(256, min(LAUNCH_ROWS, GRADIENT_VALUES // cols // 256 * 256))
+        step = rows
+        if buf is None:
+            step = max(256, min(LAUNCH_ROWS, GRADIENT_VALUES // cols // 256 * 256))
+            buf = torch.empty(min(rows, step), cols, device=h.device, dtype=torch.bfloat16)
         dh = torch.empty(h.shape, device=h.device, dtype=h.dtype) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:
             # a sum over several chunks is held in fp32
             dw = (torch.zeros if rows == 0 else torch.empty)(w.shape, device=w.device, dtype=torch.bfloat16 if rows <= step else torch.float32)
-        if rows:
-            buf = torch.empty(min(rows, step), cols, device=h.device, dtype=torch.bfloat16)
         for r in range(0, rows, step):
             part, dx, to = (h, ids, entropy, stats, g, ge), buf, dh
             if rows > step:
@@ -191,7 +199,7 @@ class _LinearTokenLogProbsFn(torch.autograd.Function):
                 part, dx = tuple(None if t is None else t[c] for t in part), buf[: c.stop - r]
                 to = None if dh is None else dh[c]
             hc, idc, ec, sc, gc, gec = part
-            _ext.ext().linear_scores_dlogits(hc, w, idc, ec, sc, gc, gec, dx, ctx.ignore_index)
+            _ext.ext().linear_scores_dlogits(hc, w, idc, ec, sc, gc, gec, dx, slab_max, ctx.ignore_index)
             _count()
             if cols != vocab:
                 dx = dx[:, :vocab]

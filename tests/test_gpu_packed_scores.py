@@ -430,7 +430,8 @@ def test_linear_token_log_probs(rows, hidden, vocab):
 
 
 def test_linear_token_log_probs_in_chunks(monkeypatch):
-    """Nothing of a row depends on the chunk that it is in; the weight's gradient is summed over the chunks."""
+    """Nothing of a row depends on the chunk that it is in; the weight's gradient is summed over the chunks.  A gradient from kept exponentials
+    (the first backward pass) has theirs and one more rounding than one from the logits again (the second)."""
     ops = _ops()
     from himuon_b200.ops import scores
 
@@ -442,16 +443,25 @@ def test_linear_token_log_probs_in_chunks(monkeypatch):
 
     def both():
         s = ops.linear_token_log_probs(h, w, ids)
-        return (s.log_probs, s.entropy, *torch.autograd.grad((s.log_probs, s.entropy), (h, w), (g, g)))
+        passes = [torch.autograd.grad((s.log_probs, s.entropy), (h, w), (g, g), retain_graph=True) for _ in range(2)]
+        return (s.log_probs, s.entropy, *passes)
 
-    whole = both()
+    lp, entropy, kept, again = both()
     monkeypatch.setattr(scores, "GRADIENT_VALUES", 256 * 1000)
     monkeypatch.setattr(scores, "LAUNCH_ROWS", 300)      # (up to 256 rows the tiles have another width)
-    parts = both()
-    for a, b in zip(whole[:3], parts[:3]):
-        assert torch.equal(a, b)
-    # the same fp32 terms in another order, then one rounding
-    assert ((whole[3].float() - parts[3].float()).abs() <= 2 * U * whole[3].float().abs() + 1e-4).all()
+    lp2, entropy2, *parts = both()
+    assert torch.equal(lp, lp2) and torch.equal(entropy, entropy2)
+    for dh, dw in parts:
+        assert torch.equal(dh, again[0])
+        # the same fp32 terms in another order, then one rounding
+        assert ((again[1].float() - dw.float()).abs() <= 2 * U * dw.float().abs() + 1e-4).all()
+    x = h.detach().double() @ w.detach().double().t()
+    l, _, e = _scores64(x, ids)
+    dx, size = _grad64(l, e, ids, g, g)
+    bound = (2 * U) * dx.abs() + 2.0 ** -10 * size       # two roundings to bf16, fp16 exponentials (also of the log in the entropy's part)
+    for i, other in ((0, w), (1, h)):
+        b = bound @ other.detach().double().abs() if i == 0 else bound.t() @ other.detach().double().abs()
+        assert ((kept[i].double() - again[i].double()).abs() <= b + U * again[i].double().abs() * 2).all()
     _clean()
 
 
