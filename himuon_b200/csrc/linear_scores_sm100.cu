@@ -265,11 +265,12 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
 }
 
 // ---------------------------------------------------------------- a few rows
-// Up to 32 rows: the weight's bytes are all that counts, so the weight takes the 128 lanes of the accumulator and the rows its NB
-// columns; a stage carries 16 KB of weight and 2 or 4 of hidden states (the pair kernel spends half of its stages on rows that are not
+// Up to 64 rows: the weight's bytes are all that counts, so the weight takes the 128 lanes of the accumulator and the rows its NB
+// columns; a stage carries 16 KB of weight and 2, 4 or 8 of hidden states (the pair kernel spends half of its stages on rows that are not
 // there).  A block streams one share of the vocabulary in tiles of `th` entries; a thread keeps the sums of its lane for
-// every row, and only at the end the 128 lanes meet.  8 rows over 151936 x 1024: NN us, pair kernel 99.
-constexpr int FEW_STAGES = 10, FEW_THREADS = 192;       // warp 0: TMA, 1: MMA, 2-5: epilogue
+// up to 32 rows, and only at the end the 128 lanes meet.  8 rows over 151936 x 1024: 50 us (6.2 TB/s), pair kernel 99.
+constexpr int FEW_STAGES = 9;
+constexpr int few_threads(int nb) { return 64 + 128 * (nb > 32 ? nb / 32 : 1); }      // warp 0: TMA, 1: MMA, then four for each 32 rows
 struct FewBars {
   uint64_t full[FEW_STAGES], empty[FEW_STAGES], tfull[2], tempty[2];
   uint32_t tmem_slot;
@@ -291,13 +292,14 @@ __device__ __forceinline__ void share_out(Sums* a, int lane) {
 }
 
 template <int NB>
-__global__ void __launch_bounds__(FEW_THREADS, 1)
+__global__ void __launch_bounds__(few_threads(NB), 1)
 linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_constant__ CUtensorMap tmW, LinScoresDev p, int th) {
   constexpr uint32_t STAGE = LS_A + NB * BK * 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_up_1024(smem_raw);
   FewBars* bars = reinterpret_cast<FewBars*>(smem + FEW_STAGES * STAGE);
   Sums* s_warp = reinterpret_cast<Sums*>(bars + 1);      // [4][NB]
+  constexpr int RB = NB < 32 ? NB : 32, GROUPS = NB / RB;      // rows of a thread, groups of four warps
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = warp_id(), lane = threadIdx.x & 31;
   // shares of whole groups of eight entries
@@ -306,11 +308,11 @@ linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_c
   const int v1 = end < p.vocab ? end : p.vocab, tiles = (v1 - v0 + th - 1) / th;
   if (threadIdx.x == 0) {
     for (int i = 0; i < FEW_STAGES; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bars->tfull[i], 1); mbar_init(&bars->tempty[i], 128); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars->tfull[i], 1); mbar_init(&bars->tempty[i], 128 * GROUPS); }
     bars->abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 1) tmem_alloc(&bars->tmem_slot, 64);
+  if (warp == 1) tmem_alloc(&bars->tmem_slot, 128);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -357,13 +359,14 @@ linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_c
   } else {
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    Sums a[NB];
+    const int c0 = (warp - 2) / 4 * RB;                 // the group's first row
+    Sums a[RB];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) a[n] = Sums{-INFINITY, 0.f, 0.f};
-    int own[NB];                                  // the rows' own tokens, -1 where there is none
+    for (int n = 0; n < RB; ++n) a[n] = Sums{-INFINITY, 0.f, 0.f};
+    int own[RB];                                  // the rows' own tokens, -1 where there is none
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const long long id = n < p.rows ? p.ids[n] : -1;
+    for (int n = 0; n < RB; ++n) {
+      const long long id = c0 + n < p.rows ? p.ids[c0 + n] : -1;
       own[n] = id >= 0 && id < p.vocab ? static_cast<int>(id) : -1;
     }
     for (int i = 0; i < tiles; ++i) {
@@ -372,9 +375,9 @@ linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_c
       const int v = v0 + i * th + row;
       const bool mine = row < th && v < v1;
 #pragma unroll
-      for (int c = 0; c < NB; c += 16) {
+      for (int c = 0; c < RB; c += 16) {
         uint32_t x[16];
-        tmem_ld16(tmem + (i & 1) * NB + lane_off + c, x);
+        tmem_ld16(tmem + (i & 1) * NB + lane_off + c0 + c, x);
         tmem_ld_wait();
         if (mine) {
 #pragma unroll
@@ -386,17 +389,17 @@ linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_c
             b.t = fmaf(fmaxf(d, kFar), e, f * fmaf(from, b.s, b.t));
             b.s = fmaf(b.s, f, e);
             b.m = m;
-            if (own[c + n] == v) p.target[c + n] = y;
+            if (own[c + n] == v) p.target[c0 + c + n] = y;
           }
         }
       }
       tc_fence_before();
       mbar_arrive(&bars->tempty[i & 1]);
     }
-    share_out<NB, 16>(a, lane);
-    if (NB == 32) s_warp[(warp & 3) * NB + lane] = a[0];
+    share_out<RB, 16>(a, lane);
+    if (RB == 32) s_warp[(warp & 3) * NB + c0 + lane] = a[0];
     else if ((lane & 1) == 0) s_warp[(warp & 3) * NB + (lane >> 1)] = a[0];
-    named_barrier(1, 128);
+    named_barrier(1, 128 * GROUPS);
     const int n = (warp - 2) * 32 + lane;
     if (n < p.rows && n < NB) {
       Sums b = s_warp[n];
@@ -412,7 +415,7 @@ linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_c
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 64);
+    tmem_dealloc(tmem, 128);
   }
 }
 
@@ -592,7 +595,7 @@ static int launch_few(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s)
   const int blocks = 2 * ((a.vocab + 127) / 128), grid = blocks < num_sms() ? blocks : num_sms();    // (scratch holds so many parts)
   const int share = ((a.vocab + 7) / 8 + grid - 1) / grid * 8, tiles = (share + 127) / 128, th = ((share + tiles - 1) / tiles + 7) / 8 * 8;
   const CUtensorMap thid = rows_tmap(a.h, a.rows, a.hidden, a.ld_h, NB), tw = rows_tmap(a.w, a.vocab, a.hidden, a.ld_w, th);
-  linear_scores_few_kernel<NB><<<grid, FEW_THREADS, SMEM, s>>>(thid, tw, p, th);
+  linear_scores_few_kernel<NB><<<grid, few_threads(NB), SMEM, s>>>(thid, tw, p, th);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores launch failed: ") + cudaGetErrorString(e));
   return grid;
@@ -622,8 +625,8 @@ void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {
     p.slabs = (a.vocab + 63) / 64;
     launch<STATS_KEPT>(a, p, s);
     n_parts = 2 * p.tiles_n;
-  } else if (a.rows <= 32) {
-    n_parts = a.rows <= 16 ? launch_few<16>(a, p, s) : launch_few<32>(a, p, s);
+  } else if (a.rows <= 64) {
+    n_parts = a.rows <= 16 ? launch_few<16>(a, p, s) : a.rows <= 32 ? launch_few<32>(a, p, s) : launch_few<64>(a, p, s);
   } else {
     launch<STATS>(a, p, s);
     n_parts = 2 * p.tiles_n;

@@ -330,13 +330,13 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-// dK and dV of a KV head: the sums over its query heads' parts, in their order.  One block per tile.
+// dK and dV of a KV head: the sums over its query heads' parts, in their order, four columns a thread.  gridDim.y blocks per tile.
 __global__ void __launch_bounds__(256)
 sum_heads_kernel(PackedDev p) {
   const PackedTile t = p.tiles[blockIdx.x];
   const int G = p.Hq / p.Hkv, row0 = t.index * AT, rows = min(AT, t.len - row0), per = p.hd / 4;
   const long long stride = p.stat_rows * p.hd;         // from head to head
-  for (int i = threadIdx.x; i < rows * p.Hkv * per; i += 256) {
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < rows * p.Hkv * per; i += gridDim.y * 256) {
     const int r = i / (p.Hkv * per), y = i - r * (p.Hkv * per), hk = y / per, c = (y - hk * per) * 4;
     const long long src = hk * G * stride + (static_cast<long long>(t.slot) * AT + r) * p.hd + c, at = t.first + row0 + r;
 #pragma unroll
@@ -351,8 +351,10 @@ sum_heads_kernel(PackedDev p) {
       *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
     }
   }
-  zero_padding(p.dk, p.ld_dk, p.tokens, p.rows, p.Hkv * p.hd, threadIdx.x, 256);
-  zero_padding(p.dv, p.ld_dv, p.tokens, p.rows, p.Hkv * p.hd, threadIdx.x, 256);
+  if (blockIdx.y == 0) {
+    zero_padding(p.dk, p.ld_dk, p.tokens, p.rows, p.Hkv * p.hd, threadIdx.x, 256);
+    zero_padding(p.dv, p.ld_dv, p.tokens, p.rows, p.Hkv * p.hd, threadIdx.x, 256);
+  }
 }
 
 // ================================================================================================ dQ
@@ -662,7 +664,7 @@ static void launch_bwd(const PackedAttnArgs& a, cudaStream_t s) {
   packed_dkv_kernel<NH><<<grid(), BWD_THREADS, SMEM_KV, s>>>(tq64, tk, tv, tdo64, tdk, tdv, p);
   check_packed_launch("dK / dV");
   if (p.split_heads) {
-    sum_heads_kernel<<<a.n_tiles, 256, 0, s>>>(p);
+    sum_heads_kernel<<<dim3(a.n_tiles, (AT * a.Hkv * (a.hd / 4) + 255) / 256), 256, 0, s>>>(p);
     check_packed_launch("sum over heads");
   }
 }

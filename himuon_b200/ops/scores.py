@@ -145,7 +145,7 @@ def _linear_scores(h, w, ids, ignore_index, keep: bool):
     stats = torch.empty(rows, 2, device=h.device, dtype=torch.float32) if keep else None
     cols = (vocab + 7) // 8 * 8
     kept = slab_max = None
-    if keep and rows > 32 and rows * cols <= GRADIENT_VALUES:        # (a few rows have a kernel that keeps nothing)
+    if keep and rows > 64 and rows * cols <= GRADIENT_VALUES:        # (a few rows have a kernel that keeps nothing)
         kept = torch.empty(rows, cols, device=h.device, dtype=torch.bfloat16)
         slab_max = torch.empty(rows, (vocab + 63) // 64, device=h.device, dtype=torch.float32)
     if rows:

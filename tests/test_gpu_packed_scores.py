@@ -405,7 +405,7 @@ def _logit_error(h, w):
     return (h.shape[1] / 16 + 4) * 2.0 ** -22 * (h.double().abs() @ w.double().abs().t()).max().item()
 
 
-@pytest.mark.parametrize("rows,hidden,vocab", [(1, 8, 1), (1, 128, 1000), (8, 256, 5003), (3, 72, 40000), (16, 128, 151936), (17, 200, 9000), (32, 640, 128256), (33, 128, 3001), (100, 64, 264), (129, 136, 777), (300, 640, 4096), (777, 128, 2050)])
+@pytest.mark.parametrize("rows,hidden,vocab", [(1, 8, 1), (1, 128, 1000), (8, 256, 5003), (3, 72, 40000), (16, 128, 151936), (17, 200, 9000), (32, 640, 128256), (33, 128, 3001), (64, 256, 5000), (65, 256, 5000), (100, 64, 264), (129, 136, 777), (300, 640, 4096), (777, 128, 2050)])
 def test_linear_token_log_probs(rows, hidden, vocab):
     ops = _ops()
     torch.manual_seed(rows + vocab)
