@@ -11,7 +11,11 @@
 // Scores of sub-block i + 1 are issued ahead of the products that need the softmax of sub-block i; 16 warps share each softmax, 16 of the
 // 64 columns a group of four.  The next item's loads and scores run beside an item's epilogue.
 // A product of 128 x 64 x 16 with both operands in shared memory takes 48 cycles, bound by its operands, one with A in tensor memory 64
-// (N = 128): a sub-block needs 1286 cycles of the dK / dV pass and 1029 of the dQ pass.
+// (N = 128): a sub-block needs 1286 cycles of the dK / dV pass and 1029 of the dQ pass, and shared memory is busy for 1280 and 1152 (the
+// operands and 32 KB of new ones).  Measured, heads of 128: 1580 and 1280 cycles a sub-block; one document of 8192 tokens, 32 heads over 8, 853 and
+// 715 us (802 and 647 TFLOP/s of products, of which P and dP are computed twice), 24 documents of 341 tokens in the mean, 16 over 8, 94 and 82.
+// One block for each item and two sub-blocks' scores in all took 990 and 800, 103 and 105: set-up and epilogue were some 10000
+// cycles an item, and the softmax of a sub-block on half of the warps took longer than the products beside it.
 #include "packed_attention.cuh"
 
 namespace himuon {

@@ -105,12 +105,15 @@ class PackedLayout:
             raise RuntimeError(f"himuon_b200.ops.{op}: {rows} rows for a layout of {self.tokens} tokens")
 
     def splits_heads(self, Hq: int, Hkv: int) -> bool:
-        """Whether the pass for dK and dV takes each query head by itself and sums the heads of a group afterwards.  A block
-        otherwise has all heads of a group to go through, and in a small batch the longest block sets the time: NN."""
-        if Hq == Hkv:
-            return False
-        longest = Hq // Hkv * -(-self.max_length // 64)                       # steps of 64 queries
-        return longest > 2 * self._query_steps * Hq / _ext.ext().num_sms()
+        """Whether the pass for dK and dV takes each query head by itself and sums the heads of a group afterwards.
+
+        A block otherwise goes through all heads of a group, and in a small batch the longest one sets the time: one document of
+        1024 tokens, 32 heads over 8, 61 us whole, 35 + 9 in parts; 2048 tokens, 16 over 8, 62 and 48 + 10.  A larger batch fills the
+        GPU either way and pays for the parts (4096 tokens, 32 over 8, 225 and 264 + 40), a tiny one saves less than their sum
+        costs (300 tokens, 16 over 8, 16.6 and 16.6 + 3)."""
+        steps = -(-self.max_length // 64)                                     # of 64 queries, for one head of the longest tile
+        group = Hq // Hkv
+        return (group - 1) * steps >= 16 and group * steps > 2 * self._query_steps * Hq / _ext.ext().num_sms()
 
     def positions(self, rows: int | None = None) -> torch.Tensor:
         """Each row's position in its own document (int64), 0 for the padding of a batch of ``rows`` rows."""
