@@ -8,7 +8,7 @@
 //              as fp16 (11 bits where the gradient gets 8; below 6e-8 of the largest of 64 they count for nothing), which the gradient then
 //              takes the place of.
 //
-// The product is the pair GEMM's (gemm2_sm100.cu has its protocol): 256 rows by BN vocabulary entries per pair, six stages of 64 along
+// The product is the pair GEMM's (gemm2_sm100.cu has its protocol): 256 rows by 256 vocabulary entries per pair, six stages of 64 along
 // the hidden size, two accumulators, so that the epilogue of one tile runs beside the products of the next.  The tiles of one
 // vocabulary block are neighbours in the schedule: its rows of W come from memory once, the hidden states from the L2.
 #include <cuda_fp16.h>
@@ -27,7 +27,10 @@ namespace {
 
 constexpr int LS_THREADS = 384;      // warps 0-3: TMA, MMA, TMEM allocation, none; 4-11: epilogue, two groups of four
 constexpr int LS_STAGES = 6;
-constexpr uint32_t LS_A = BM * BK * 2, LS_STAGE = 2 * LS_A;      // 128 rows of h, and up to 128 of W, a CTA
+// Vocabulary entries per tile.  Narrower ones fill the last round of tiles better, but cost more than that gives, also where one block
+// of rows has every tile: 65 / 128 / 256 rows at 151936 x 1024 took 72 / 72 / 78 us with 256, 81 / 80 / 86 with 192, 109 / 108 / 111 with 128.
+constexpr int LS_N = 256;
+constexpr uint32_t LS_A = BM * BK * 2, LS_STAGE = 2 * LS_A;      // 128 rows of h and 128 of W, a CTA
 
 enum { STATS, GRAD, STATS_KEPT };    // what the epilogue makes of the logits; STATS_KEPT: sums, and the exponentials
 
@@ -42,7 +45,7 @@ struct LinScoresDev {
   const float* g_log_probs;
   const float* g_entropy;
   long long ignore;
-  int rows, vocab, tiles_m, tiles_n, kblocks, bn;
+  int rows, vocab, tiles_m, tiles_n, kblocks;
   int* status;
 };
 
@@ -116,13 +119,13 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
     const uint32_t e = elect_one();
     tma_prefetch_desc(&tmH);
     tma_prefetch_desc(&tmW);
-    const uint32_t bytes = 2 * (LS_A + p.bn / 2 * BK * 2);
+    const uint32_t bytes = 2 * (LS_A + LS_N / 2 * BK * 2);
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = first; ok && tile < total; tile += n_pairs) {
       const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
-      const int n0 = nt * p.bn + static_cast<int>(rank) * (p.bn / 2);
+      const int n0 = nt * LS_N + static_cast<int>(rank) * (LS_N / 2);
       for (int kb = 0; kb < p.kblocks; ++kb) {
         if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
         uint8_t* sA = smem + stage * LS_STAGE;
@@ -136,7 +139,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
     // ------------------------------------------------------------ MMA issuer (leader CTA only)
     if (leader) {
       const uint32_t e = elect_one();
-      const uint32_t idesc = umma_idesc_bf16(2 * BM, p.bn, false, false);
+      const uint32_t idesc = umma_idesc_bf16(2 * BM, LS_N, false, false);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -175,7 +178,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
     uint32_t acc_phase = 0;
     for (int tile = first; tile < total; tile += n_pairs) {
       const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
-      const int row = m0 + ew * 32 + lane, n0 = nt * p.bn;
+      const int row = m0 + ew * 32 + lane, n0 = nt * LS_N;
       const bool row_ok = row < p.rows;
       RowGrad rg{};
       long long id = -1;
@@ -192,7 +195,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
         uint8_t* my_row = slab + (ew * 32 + lane) * 128;
         Sums a{-INFINITY, 0.f, 0.f};
 #pragma unroll 1
-        for (int c = group * 64; c < p.bn; c += 128) {
+        for (int c = group * 64; c < LS_N; c += 128) {
           const int col = n0 + c;
           if (col >= p.vocab) break;
           uint32_t o[32];
@@ -550,19 +553,6 @@ static int pairs_at_once(size_t smem) {
   return most;
 }
 
-// Vocabulary entries per tile.  With one block of rows the weight's bytes bound the call and the last round of tiles counts: the
-// width that needs the fewest of them in sum.  (More rows: 256, the least operand traffic for a product.)
-static int tile_width(int rows, int vocab, int pairs) {
-  if (rows > 2 * BM) return 256;
-  int best = 256;
-  long long least = -1;
-  for (int bn = 256; bn >= 128; bn -= 64) {
-    const long long cost = ((vocab + bn - 1) / bn + pairs - 1) / pairs * static_cast<long long>(bn);
-    if (least < 0 || cost < least) { least = cost; best = bn; }
-  }
-  return best;
-}
-
 template <int MODE>
 static void launch(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + LS_STAGES * LS_STAGE + 2 * SLAB_BYTES + 256;
@@ -570,13 +560,12 @@ static void launch(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s) {
   const cudaError_t set = cudaFuncSetAttribute(linear_scores_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
   if (set != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores: ") + cudaGetErrorString(set));
   const int pairs = pairs_at_once<MODE>(SMEM);
-  p.bn = MODE == GRAD ? 256 : tile_width(p.rows, p.vocab, pairs);
   p.tiles_m = (p.rows + 2 * BM - 1) / (2 * BM);
-  p.tiles_n = (p.vocab + p.bn - 1) / p.bn;
+  p.tiles_n = (p.vocab + LS_N - 1) / LS_N;
   p.kblocks = (a.hidden + BK - 1) / BK;
   const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
   if (total >= (1LL << 30)) throw std::runtime_error("himuon linear_scores: too many tiles for one launch");
-  const CUtensorMap th = rows_tmap(a.h, a.rows, a.hidden, a.ld_h, BM), tw = rows_tmap(a.w, a.vocab, a.hidden, a.ld_w, p.bn / 2),
+  const CUtensorMap th = rows_tmap(a.h, a.rows, a.hidden, a.ld_h, BM), tw = rows_tmap(a.w, a.vocab, a.hidden, a.ld_w, LS_N / 2),
                     td = MODE == STATS ? th : rows_tmap(a.grad, a.rows, static_cast<int>(a.ld_grad), a.ld_grad, BM);
   const int grid = 2 * static_cast<int>(total < pairs ? total : pairs);
   linear_scores_kernel<MODE><<<grid, LS_THREADS, SMEM, s>>>(th, tw, td, p);
@@ -614,7 +603,7 @@ static LinScoresDev make_dev(const LinearScoreArgs& a) {
   return p;
 }
 
-// For the narrowest tiles, so that it does not depend on the GPU.
+// Room for the most parts that either forward kernel has: one for each 64 entries (launch_few), and the rows' own logits.
 long long linear_scores_scratch(long long rows, int vocab) { return rows * (1 + 3LL * 2 * ((vocab + 127) / 128)); }
 
 void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {

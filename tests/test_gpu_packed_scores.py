@@ -448,7 +448,7 @@ def test_linear_token_log_probs_in_chunks(monkeypatch):
 
     lp, entropy, kept, again = both()
     monkeypatch.setattr(scores, "GRADIENT_VALUES", 256 * 1000)
-    monkeypatch.setattr(scores, "LAUNCH_ROWS", 300)      # (up to 256 rows the tiles have another width)
+    monkeypatch.setattr(scores, "LAUNCH_ROWS", 300)
     lp2, entropy2, *parts = both()
     assert torch.equal(lp, lp2) and torch.equal(entropy, entropy2)
     for dh, dw in parts:
