@@ -44,7 +44,8 @@ class PackedLayout:
 
     ``lengths``: the documents' lengths in tokens, zero included (a sequence of whole numbers, or an integer tensor; one on a
     GPU is read back, which waits for it).  ``device``: where the batch lives.  The device-side tables are copied without a wait on
-    the stream that is current here; calls on other streams wait for them.
+    the stream that is current when they are first needed; calls on other streams wait for them.  A graph may hold calls with a layout
+    whose tables are there before its capture, and needs the layout for as long as it is replayed.
     """
 
     def __init__(self, lengths, device="cuda"):
@@ -78,6 +79,9 @@ class PackedLayout:
         entry = self._tables.get(key)
         on_gpu = self.device.type == "cuda"
         if entry is None:
+            if on_gpu and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("himuon_b200.ops.PackedLayout: a table would be copied from the host while a graph is captured; "
+                                   "make the layout, and call what uses it once, before the capture")
             host = torch.from_numpy(make())
             if not on_gpu:
                 entry = (host.to(self.device), None, None)
@@ -188,7 +192,11 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
     """Causal GQA attention within each document of a packed batch, on ``(rows, heads*head_dim)`` views (``rows`` at least
     ``layout.tokens``; rows behind that are padding); returns ``(rows, Hq*head_dim)``.  ``scale`` defaults to
     ``1/sqrt(head_dim)`` and must be positive.  bf16 CUDA tensors with heads of a multiple of 8 up to 128 run the sm_100a kernels,
-    forward and backward."""
+    forward and backward.
+
+    What is in other documents or in the padding has no part in a row, NaN and infinities included.  Those of a later token of the
+    row's own document have weight 0, which does not take them out: as in :func:`attention`, a token that is not finite may reach
+    neighbours that do not see it."""
     if not isinstance(layout, PackedLayout):
         raise RuntimeError("himuon_b200.ops.packed_attention: layout must be a PackedLayout")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)

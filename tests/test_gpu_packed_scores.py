@@ -238,6 +238,19 @@ def test_packed_attention_on_another_stream_and_in_a_graph():
     _clean()
 
 
+def test_layout_copies_no_table_while_a_graph_is_captured():
+    ops = _ops()
+    layout, graph = ops.PackedLayout([3, 5]), torch.cuda.CUDAGraph()
+    layout.positions()
+    with torch.cuda.graph(graph):
+        there = layout.positions() + 1
+        with pytest.raises(RuntimeError, match="before the capture"):
+            layout.positions(10)
+    graph.replay()
+    assert there.tolist() == [1, 2, 3, 1, 2, 3, 4, 5]
+    assert layout.positions(10).tolist() == [0, 1, 2, 0, 1, 2, 3, 4, 0, 0]
+
+
 def test_packed_attention_repeats_its_bits():
     ops = _ops()
     torch.manual_seed(15)
