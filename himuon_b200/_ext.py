@@ -41,6 +41,10 @@ def ext():
         raise RuntimeError(f"himuon_b200: cannot load the CUDA extension: {e}") from e
 
 
+def loaded() -> bool:
+    return _EXT is not None
+
+
 def available() -> bool:
     try:
         ext()

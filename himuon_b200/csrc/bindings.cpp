@@ -4,6 +4,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
+
 #include "himuon.h"
 #include "symm.h"
 
@@ -343,6 +345,61 @@ static void packed_attn_bwd(const at::Tensor& plan, int64_t tiles, int64_t token
   himuon::packed_attn_bwd(a, cur_stream());
 }
 
+// Autograd functions of calls whose kernels take tens of microseconds are written here and not in Python: a backward pass then runs in
+// the engine's thread without waiting for the interpreter.  (Forward and gradients of the packed attention:
+// 119 us of host time as a Python function, 88 here, of which a function that does nothing takes 63 and 40.)
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+static std::atomic<int64_t> autograd_launched{0};       // kernels launched by them
+
+static void check_once(const char* op) {
+  TORCH_CHECK(!c10::GradMode::is_enabled(), "himuon_b200.ops.", op, ": its gradient cannot be differentiated again (create_graph=True)");
+}
+
+struct PackedAttention : torch::autograd::Function<PackedAttention> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& plan, int64_t tiles,
+                            int64_t tokens, int64_t Hq, int64_t Hkv, double scale, bool split_heads) {
+    at::Tensor o = at::empty(q.sizes(), q.options()), lse = at::empty({Hq * tiles * 128}, q.options().dtype(at::kFloat));
+    if (tiles) {
+      packed_attn_fwd(plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
+      autograd_launched += 1;
+    } else {
+      o.zero_();
+    }
+    ctx->save_for_backward({q, k, v, o, lse, plan});
+    ctx->saved_data["tiles"] = tiles;
+    ctx->saved_data["tokens"] = tokens;
+    ctx->saved_data["Hq"] = Hq;
+    ctx->saved_data["Hkv"] = Hkv;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["split_heads"] = split_heads;
+    return o;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("packed_attention");
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &plan = saved[5];
+    const int64_t tiles = ctx->saved_data["tiles"].toInt(), Hq = ctx->saved_data["Hq"].toInt(), Hkv = ctx->saved_data["Hkv"].toInt(), hd = q.size(1) / Hq;
+    at::Tensor d_o = grads[0];
+    if (d_o.stride(1) != 1 || d_o.stride(0) % 8 || d_o.stride(0) < d_o.size(1) || reinterpret_cast<uintptr_t>(d_o.data_ptr()) % 16)
+      d_o = d_o.clone(at::MemoryFormat::Contiguous);
+    // dq | dk | dv share one buffer, as in attention(): a fused projection sees a single contiguous gradient
+    at::Tensor all = at::empty({q.size(0), (Hq + 2 * Hkv) * hd}, q.options());
+    at::Tensor dq = all.narrow(1, 0, Hq * hd), dk = all.narrow(1, Hq * hd, Hkv * hd), dv = all.narrow(1, (Hq + Hkv) * hd, Hkv * hd);
+    if (tiles) {
+      at::Tensor delta = at::empty_like(lse);
+      c10::optional<at::Tensor> part;
+      if (ctx->saved_data["split_heads"].toBool()) part = at::empty({2 * lse.numel() * hd}, lse.options());
+      packed_attn_bwd(plan, tiles, ctx->saved_data["tokens"].toInt(), d_o, q, k, v, o, lse, dq, dk, dv, delta, part, Hq, Hkv, ctx->saved_data["scale"].toDouble());
+      autograd_launched += part.has_value() ? 3 : 2;
+    } else {
+      all.zero_();
+    }
+    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
 // Checks what the forward and the gradient call share.
 static himuon::TokenScoreArgs token_score_args(const char* op, const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& entropy,
                                                int64_t ignore_index) {
@@ -399,6 +456,54 @@ static void token_scores_bwd(const at::Tensor& logits, const at::Tensor& ids, co
   const c10::cuda::CUDAGuard guard(logits.device());
   himuon::token_scores_bwd(a, cur_stream());
 }
+
+// Outputs of a call: log probabilities, entropy, and values and ids of alternatives where there are any.
+static variable_list score_outputs(const at::Tensor& logits, const at::Tensor& ids, int64_t top_k, int64_t ignore_index, const c10::optional<at::Tensor>& stats) {
+  const int64_t rows = logits.size(0);
+  const auto fp32 = logits.options().dtype(at::kFloat);
+  variable_list out = {at::empty({rows}, fp32), at::empty({rows}, fp32)};
+  c10::optional<at::Tensor> top_log_probs, top_ids;
+  if (top_k) {
+    top_log_probs = at::empty({rows, top_k}, fp32);
+    top_ids = at::empty({rows, top_k}, ids.options());
+    out.push_back(*top_log_probs);
+    out.push_back(*top_ids);
+  }
+  if (rows) {
+    token_scores_fwd(logits, ids, out[0], out[1], stats, top_log_probs, top_ids, ignore_index);
+    autograd_launched += 1;
+  }
+  return out;
+}
+
+struct TokenScores : torch::autograd::Function<TokenScores> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids, int64_t top_k, int64_t ignore_index) {
+    ctx->set_materialize_grads(false);                   // the gradient of an unused output arrives undefined
+    const at::Tensor stats = at::empty({logits.size(0), 2}, logits.options().dtype(at::kFloat));
+    variable_list out = score_outputs(logits, ids, top_k, ignore_index, stats);
+    ctx->save_for_backward({logits, ids, out[1], stats});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    if (top_k) ctx->mark_non_differentiable({out[2], out[3]});
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("token_log_probs");
+    at::Tensor grad;
+    if (grads[0].defined() || grads[1].defined()) {
+      const variable_list saved = ctx->get_saved_variables();
+      grad = at::empty(saved[0].sizes(), saved[0].options());
+      c10::optional<at::Tensor> g[2];
+      for (int i = 0; i < 2; ++i)
+        if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
+      if (grad.numel()) {
+        token_scores_bwd(saved[0], saved[1], saved[2], saved[3], g[0], g[1], grad, ctx->saved_data["ignore_index"].toInt());
+        autograd_launched += 1;
+      }
+    }
+    return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
 
 static himuon::LinearScoreArgs linear_score_args(const char* op, const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, const at::Tensor& entropy,
                                                  const c10::optional<at::Tensor>& stats, int64_t ignore_index) {
@@ -553,7 +658,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("embedding_bwd", &embedding_bwd);
   m.def("cross_entropy", &cross_entropy);
   m.def("packed_attn_fwd", &packed_attn_fwd);
-  m.def("packed_attn_bwd", &packed_attn_bwd);
+  m.def("packed_attention", [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& plan, int64_t tiles, int64_t tokens, int64_t Hq,
+                               int64_t Hkv, double scale, bool split_heads) {
+    return PackedAttention::apply(q, k, v, plan, tiles, tokens, Hq, Hkv, scale, split_heads);
+  });
+  m.def("token_scores", [](const at::Tensor& logits, const at::Tensor& ids, int64_t top_k, int64_t ignore_index) {
+    if (c10::GradMode::is_enabled() && logits.requires_grad()) return TokenScores::apply(logits, ids, top_k, ignore_index);
+    return score_outputs(logits, ids, top_k, ignore_index, c10::nullopt);
+  });
+  m.def("autograd_launched", [] { return autograd_launched.load(); });
   m.def("token_scores_fwd", &token_scores_fwd);
   m.def("token_scores_bwd", &token_scores_bwd);
   m.def("linear_scores_fwd", &linear_scores_fwd);

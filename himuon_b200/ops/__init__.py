@@ -22,7 +22,7 @@ _LAUNCHES = 0
 
 
 def launch_count() -> int:
-    return _LAUNCHES
+    return _LAUNCHES + (_ext.ext().autograd_launched() if _ext.loaded() else 0)
 
 
 def _count(n: int = 1) -> None:

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from .. import _ext
-from . import _check_width, _count, _once, _warn_torch_path, _with_kernel_rows, use_kernels
+from . import _check_width, _count, _warn_torch_path, _with_kernel_rows, use_kernels
 from . import reference as ref
 
 TILE = 128          # tokens of one document that a block of the kernels takes
@@ -149,45 +149,6 @@ class PackedLayout:
         return cos_sin.index_select(0, self.positions(rows))
 
 
-def _forward(q, k, v, layout, Hq, Hkv, scale, keep: bool):
-    o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(Hq * layout.tiles * TILE, device=q.device, dtype=torch.float32) if keep else None
-    if layout.tiles:
-        _ext.ext().packed_attn_fwd(layout.plan, layout.tiles, layout.tokens, q, k, v, o, lse, Hq, Hkv, scale)
-        _count()
-    else:
-        o.zero_()
-    return o, lse
-
-
-class _PackedAttnFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, layout, Hq, Hkv, scale):
-        o, lse = _forward(q, k, v, layout, Hq, Hkv, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse)
-        ctx.layout, ctx.heads, ctx.scale = layout, (Hq, Hkv), scale
-        return o
-
-    @staticmethod
-    def backward(ctx, do):
-        _once("packed_attention")
-        q, k, v, o, lse = ctx.saved_tensors
-        layout, (Hq, Hkv) = ctx.layout, ctx.heads
-        do = _with_kernel_rows(do)
-        D = q.shape[1] // Hq
-        # dq | dk | dv share one buffer, as in attention(): a fused projection sees a single contiguous gradient
-        dqkv = torch.empty(q.shape[0], (Hq + 2 * Hkv) * D, device=q.device, dtype=q.dtype)
-        dq, dk, dv = dqkv.split((Hq * D, Hkv * D, Hkv * D), 1)
-        if layout.tiles:
-            delta = torch.empty_like(lse)
-            part = torch.empty(2 * lse.numel() * D, device=q.device, dtype=torch.float32) if layout.splits_heads(Hq, Hkv) else None
-            _ext.ext().packed_attn_bwd(layout.plan, layout.tiles, layout.tokens, do, q, k, v, o, lse, dq, dk, dv, delta, part, Hq, Hkv, ctx.scale)
-            _count(2 if part is None else 3)
-        else:
-            dqkv.zero_()
-        return dq, dk, dv, None, None, None, None
-
-
 def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, head_dim: int, scale: float | None = None):
     """Causal GQA attention within each document of a packed batch, on ``(rows, heads*head_dim)`` views (``rows`` at least
     ``layout.tokens``; rows behind that are padding); returns ``(rows, Hq*head_dim)``.  ``scale`` defaults to
@@ -215,8 +176,14 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
     if use_kernels(q2d) and head_dim <= 128 and head_dim % 8 == 0:
         q, k, v = _with_kernel_rows(q2d), _with_kernel_rows(k2d), _with_kernel_rows(v2d)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            return _PackedAttnFn.apply(q, k, v, layout, Hq, Hkv, scale)
-        return _forward(q, k, v, layout, Hq, Hkv, scale, False)[0]
+            return _ext.ext().packed_attention(q, k, v, layout.plan, layout.tiles, layout.tokens, Hq, Hkv, scale, layout.splits_heads(Hq, Hkv))
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if layout.tiles:
+            _ext.ext().packed_attn_fwd(layout.plan, layout.tiles, layout.tokens, q, k, v, o, None, Hq, Hkv, scale)
+            _count()
+        else:
+            o.zero_()
+        return o
     if use_kernels(q2d):
         _warn_torch_path("packed_attention", f"head_dim {head_dim} (the kernels take multiples of 8 up to 128)")
     return ref.packed_attention(q2d, k2d, v2d, layout.lengths, Hq, Hkv, head_dim, scale)

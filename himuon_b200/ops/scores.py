@@ -31,44 +31,6 @@ def _incoming(g: torch.Tensor | None):
     return None if g is None else g.to(torch.float32).contiguous()
 
 
-def _scores(logits, ids, top_k, ignore_index, keep: bool):
-    """log_probs, entropy, alternatives, and with ``keep`` the two numbers a row that the gradient needs."""
-    rows, dev = logits.shape[0], logits.device
-    log_probs = torch.empty(rows, device=dev, dtype=torch.float32)
-    entropy = torch.empty(rows, device=dev, dtype=torch.float32)
-    stats = torch.empty(rows, 2, device=dev, dtype=torch.float32) if keep else None
-    top_lp = torch.empty(rows, top_k, device=dev, dtype=torch.float32) if top_k else None
-    top_ids = torch.empty(rows, top_k, device=dev, dtype=torch.int64) if top_k else None
-    if rows:
-        _ext.ext().token_scores_fwd(logits, ids, log_probs, entropy, stats, top_lp, top_ids, ignore_index)
-        _count()
-    return log_probs, entropy, top_lp, top_ids, stats
-
-
-class _TokenLogProbsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, top_k, ignore_index):
-        ctx.set_materialize_grads(False)              # the gradient of an unused output arrives as None
-        log_probs, entropy, top_lp, top_ids, stats = _scores(logits, ids, top_k, ignore_index, True)
-        ctx.save_for_backward(logits, ids, entropy, stats)
-        ctx.ignore_index = ignore_index
-        if top_k:
-            ctx.mark_non_differentiable(top_lp, top_ids)
-        return log_probs, entropy, top_lp, top_ids
-
-    @staticmethod
-    def backward(ctx, g_log_probs, g_entropy, *_):
-        _once("token_log_probs")
-        if g_log_probs is None and g_entropy is None:
-            return None, None, None, None
-        logits, ids, entropy, stats = ctx.saved_tensors
-        grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        if grad.numel():
-            _ext.ext().token_scores_bwd(logits, ids, entropy, stats, _incoming(g_log_probs), _incoming(g_entropy), grad, ctx.ignore_index)
-            _count()
-        return grad, None, None, None
-
-
 def _check_ids(op: str, ids: torch.Tensor, rows: int, device) -> torch.Tensor:
     if ids.dtype != torch.int64 or ids.numel() != rows or ids.dim() != 1 or ids.device != device:
         raise RuntimeError(f"himuon_b200.ops.{op}: ids must be int64, one for each of the {rows} rows, on {device}")
@@ -91,9 +53,7 @@ def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ign
     if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32):
         if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
             logits = logits.contiguous()
-        if torch.is_grad_enabled() and logits.requires_grad:
-            return TokenLogProbs(*_TokenLogProbsFn.apply(logits, ids, int(top_k), int(ignore_index)))
-        return TokenLogProbs(*_scores(logits, ids, int(top_k), int(ignore_index), False)[:4])
+        return TokenLogProbs(*_ext.ext().token_scores(logits, ids, int(top_k), int(ignore_index)))
     return TokenLogProbs(*ref.token_log_probs(logits, ids, top_k, ignore_index))
 
 
