@@ -4,6 +4,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "himuon.h"
@@ -574,6 +575,139 @@ static void sum_parts(const at::Tensor& parts, at::Tensor& out) {
   himuon::sum_parts(parts.data_ptr<float>(), out.data_ptr(), out.numel(), (int)parts.size(0), cur_stream());
 }
 
+// out = a b, for a long inner dimension and few output tiles: cut along it into batches whose fp32 results are added up.
+// A GEMM's time goes by its rounds of tiles over the SMs, and the cut fills them: 777 x 128256 x 640, 12 tiles of 256 x 256
+// on 74 CTA pairs, 130 us in 6 cuts against 567 whole; the fp32 results are what a cut costs.
+static void long_product(const at::Tensor& a, const at::Tensor& b, at::Tensor& out) {
+  const int64_t rows = a.size(0), inner = a.size(1), cols = b.size(1);
+  const bool pairs = rows > 128 && cols > 192;
+  const int64_t slots = pairs ? himuon::num_sms() / 2 : himuon::num_sms(), tile = pairs ? 256 : 128;
+  const int64_t tiles = (rows + tile - 1) / tile * ((cols + 255) / 256);
+  int64_t cuts = 1;
+  if (tiles < 4 * slots && inner >= 8192) {
+    const double unit = tile * 256.0 * 2 * inner / (1.4e15 / slots);                 // seconds of one tile, whole
+    double best = 0;
+    for (int64_t c = 1; c <= std::min<int64_t>(16, inner / 4096); ++c) {
+      double rounds = static_cast<double>((tiles * c + slots - 1) / slots) / c;
+      if (c == 1 && pairs && tiles > slots / 2 && tiles % slots > 0 && tiles % slots <= slots / 2)
+        rounds = static_cast<double>(tiles) / slots;                                 // (the GEMM cuts such a last round itself)
+      const double cost = rounds * unit + (c > 1 ? 8.0 * c * rows * cols / 6e12 + 8e-6 : 0.0);
+      if (c == 1 || cost < best) { best = cost; cuts = c; }
+    }
+  }
+  if (cuts == 1) {
+    gemm(a, b, out, c10::nullopt, false, false, 1.0, 0.0, false, 0, false);
+    autograd_launched += 1;
+    return;
+  }
+  const int64_t step = inner / cuts / 64 * 64, rest = inner - cuts * step;
+  const at::Tensor parts = at::empty({cuts + (rest > 0), rows, cols}, a.options().dtype(at::kFloat));
+  at::Tensor whole = parts.narrow(0, 0, cuts);
+  gemm(a.as_strided({cuts, rows, step}, {step, a.stride(0), 1}), b.as_strided({cuts, step, cols}, {step * b.stride(0), b.stride(0), 1}), whole, c10::nullopt,
+       false, false, 1.0, 0.0, false, 0, false);
+  if (rest) {
+    at::Tensor last = parts.select(0, cuts);
+    gemm(a.narrow(1, cuts * step, rest), b.narrow(0, cuts * step, rest), last, c10::nullopt, false, false, 1.0, 0.0, false, 0, false);
+  }
+  sum_parts(parts, out);
+  autograd_launched += 2 + (rest > 0);
+}
+
+// Log probabilities and entropy, `launch_rows` rows at a time: their hidden states stay in the L2 while the weight streams by.
+static variable_list linear_score_outputs(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, int64_t ignore_index, int64_t launch_rows,
+                                          const c10::optional<at::Tensor>& stats, const c10::optional<at::Tensor>& kept, const c10::optional<at::Tensor>& slab_max) {
+  const int64_t rows = h.size(0);
+  const auto fp32 = h.options().dtype(at::kFloat);
+  variable_list out = {at::empty({rows}, fp32), at::empty({rows}, fp32)};
+  if (!rows) return out;
+  at::Tensor scratch = at::empty({himuon::linear_scores_scratch(std::min(rows, launch_rows), static_cast<int>(w.size(0)))}, fp32);
+  for (int64_t r = 0; r < rows; r += launch_rows) {
+    const int64_t n = std::min(rows - r, launch_rows);
+    auto chunk = [&](const at::Tensor& t) { return n == rows ? t : t.narrow(0, r, n); };
+    auto maybe = [&](const c10::optional<at::Tensor>& t) { return t.has_value() ? c10::optional<at::Tensor>(chunk(*t)) : c10::nullopt; };
+    at::Tensor log_probs = chunk(out[0]), entropy = chunk(out[1]);
+    linear_scores_fwd(chunk(h), w, chunk(ids), log_probs, entropy, maybe(stats), scratch, ignore_index, maybe(kept), maybe(slab_max));
+    autograd_launched += 2;
+  }
+  return out;
+}
+
+// The backward pass multiplies the logits' gradient with both operands.  It gets it from the exponentials that the forward pass kept, in
+// their place; where there are none (more than `gradient_values`, a few rows, whose kernel keeps nothing, or used up by an earlier backward
+// pass) it makes the logits again, for as many rows at a time as that allows.
+struct LinearScores : torch::autograd::Function<LinearScores> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, int64_t ignore_index, int64_t launch_rows,
+                               int64_t gradient_values) {
+    ctx->set_materialize_grads(false);
+    const int64_t rows = h.size(0), vocab = w.size(0), cols = (vocab + 7) / 8 * 8;
+    const auto fp32 = h.options().dtype(at::kFloat);
+    const at::Tensor stats = at::empty({rows, 2}, fp32);
+    c10::optional<at::Tensor> kept, slab_max;
+    if (rows > 64 && rows * cols <= gradient_values) {
+      kept = at::empty({rows, cols}, h.options());
+      slab_max = at::empty({rows, (vocab + 63) / 64}, fp32);
+      ctx->saved_data["kept"] = *kept;
+      ctx->saved_data["slab_max"] = *slab_max;
+    }
+    variable_list out = linear_score_outputs(h, w, ids, ignore_index, launch_rows, stats, kept, slab_max);
+    ctx->save_for_backward({h, w, ids, out[1], stats});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["launch_rows"] = launch_rows;
+    ctx->saved_data["gradient_values"] = gradient_values;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("linear_token_log_probs");
+    variable_list result(6);
+    if (!grads[0].defined() && !grads[1].defined()) return result;
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &h = saved[0], &w = saved[1];
+    const int64_t rows = h.size(0), vocab = w.size(0), cols = (vocab + 7) / 8 * 8, ignore_index = ctx->saved_data["ignore_index"].toInt();
+    c10::optional<at::Tensor> g[2], slab_max;
+    for (int i = 0; i < 2; ++i)
+      if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
+    at::Tensor buf;
+    int64_t step = rows;
+    if (ctx->saved_data.count("kept")) {
+      buf = ctx->saved_data["kept"].toTensor();
+      slab_max = ctx->saved_data["slab_max"].toTensor();
+      ctx->saved_data.erase("kept");
+      ctx->saved_data.erase("slab_max");
+    } else {
+      step = std::max<int64_t>(256, std::min(ctx->saved_data["launch_rows"].toInt(), ctx->saved_data["gradient_values"].toInt() / cols / 256 * 256));
+      buf = at::empty({std::min(rows, step), cols}, h.options());
+    }
+    at::Tensor dh, dw;
+    if (ctx->needs_input_grad(0)) dh = at::empty(h.sizes(), h.options());
+    if (ctx->needs_input_grad(1)) {
+      dw = at::empty(w.sizes(), rows <= step ? w.options() : w.options().dtype(at::kFloat));       // a sum over several chunks is held in fp32
+      if (!rows) dw.zero_();
+    }
+    for (int64_t r = 0; r < rows; r += step) {
+      const int64_t n = std::min(rows - r, step);
+      auto chunk = [&](const at::Tensor& t) { return n == rows ? t : t.narrow(0, r, n); };
+      auto maybe = [&](const c10::optional<at::Tensor>& t) { return t.has_value() ? c10::optional<at::Tensor>(chunk(*t)) : c10::nullopt; };
+      at::Tensor dx = buf.size(0) == n ? buf : buf.narrow(0, 0, n);
+      const at::Tensor hc = chunk(h);
+      linear_scores_dlogits(hc, w, chunk(saved[2]), chunk(saved[3]), chunk(saved[4]), maybe(g[0]), maybe(g[1]), dx, slab_max, ignore_index);
+      autograd_launched += 1;
+      if (cols != vocab) dx = dx.narrow(1, 0, vocab);
+      if (dh.defined()) {
+        at::Tensor to = chunk(dh);
+        long_product(dx, w, to);
+      }
+      if (dw.defined()) {
+        gemm(dx, hc, dw, r ? c10::optional<at::Tensor>(dw) : c10::nullopt, true, false, 1.0, r ? 1.0 : 0.0, false, 0, false);
+        autograd_launched += 1;
+      }
+    }
+    result[0] = dh;
+    if (dw.defined()) result[1] = dw.to(w.scalar_type());
+    return result;
+  }
+};
+
 static bool ns5_fused_supported(int64_t m, int64_t n) { return himuon::ns5_fused_supported((int)m, (int)n); }
 static void ns5_fused(const at::Tensor& x, at::Tensor& out, int64_t steps, double eps, bool normalize) {
   HM_CHECK(x.is_cuda() && is_bf16(x) && is_bf16(out) && x.is_contiguous() && out.is_contiguous() && x.dim() == 3 && x.sizes() == out.sizes(), "ns5_fused: contiguous (B, m, n) bf16 tensors");
@@ -669,10 +803,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("autograd_launched", [] { return autograd_launched.load(); });
   m.def("token_scores_fwd", &token_scores_fwd);
   m.def("token_scores_bwd", &token_scores_bwd);
-  m.def("linear_scores_fwd", &linear_scores_fwd);
-  m.def("sum_parts", &sum_parts);
-  m.def("linear_scores_dlogits", &linear_scores_dlogits);
-  m.def("linear_scores_scratch", [](int64_t rows, int64_t vocab) { return himuon::linear_scores_scratch(rows, (int)vocab); });
+  m.def("long_product", &long_product);
+  m.def("linear_scores", [](const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, int64_t ignore_index, int64_t launch_rows, int64_t gradient_values) {
+    if (c10::GradMode::is_enabled() && (h.requires_grad() || w.requires_grad())) return LinearScores::apply(h, w, ids, ignore_index, launch_rows, gradient_values);
+    return linear_score_outputs(h, w, ids, ignore_index, launch_rows, c10::nullopt, c10::nullopt, c10::nullopt);
+  });
   m.def("flash_attn_fwd", &flash_attn_fwd);
   m.def("flash_attn_bwd", &flash_attn_bwd);
   m.def("ns5_fused_supported", &ns5_fused_supported);
