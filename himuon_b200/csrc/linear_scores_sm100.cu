@@ -433,10 +433,16 @@ linear_scores_join_kernel(LinScoresDev p, int n_parts, float* log_probs, float* 
   Sums a{-INFINITY, 0.f, 0.f};
   if (row < p.rows) {
     const long long n = static_cast<long long>(n_parts) * p.rows;
-#pragma unroll 4
-    for (int i = w; i < n_parts; i += W) {
-      const float* src = p.part + static_cast<long long>(i) * p.rows + row;
-      a = merged(a, Sums{src[0], src[n], src[2 * n]});
+    for (int i = w; i < n_parts; i += 4 * W) {         // (loads of four parts at once: merging one by one waits for each)
+      Sums b[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float* src = p.part + static_cast<long long>(i + u * W) * p.rows + row;
+        b[u] = i + u * W < n_parts ? Sums{src[0], src[n], src[2 * n]} : Sums{-INFINITY, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i + u * W < n_parts) a = merged(a, b[u]);
     }
   }
   s_sums[threadIdx.x] = a;
