@@ -9,7 +9,7 @@
 // `ignore` has log p = 0 and passes no g on; an id outside the vocabulary has log p = NaN and passes none on either.
 //
 // One pass over the logits.  fp32 logits run at the rate of memory (2048 x 151936: 178 us, 7.0 TB/s); bf16 ones come close to what the
-// SMs can exponentiate, 16 a clock (2048 x 151936: 105 us, 5.9 TB/s, exponential unit 72 % busy), and alternatives cost half as many
+// SMs can exponentiate, 16 a clock (2048 x 151936: 105 to 116 us, 5.4 to 5.9 TB/s, exponential unit 63 to 72 % busy), and alternatives cost half as many
 // instructions again (1024 x 128256 with 8: 72 us, where 46 would do without).  A row goes to a cluster of 1 to 8 blocks, so that a few
 // rows occupy the GPU as well (scores_split()); the blocks' partial results meet in distributed shared memory.  The gradient, one read
 // and one write, takes 215 us at 2048 x 151936 bf16 (5.8 TB/s).
