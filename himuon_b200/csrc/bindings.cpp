@@ -646,11 +646,11 @@ struct LinearScores : torch::autograd::Function<LinearScores> {
     if (rows > 64 && rows * cols <= gradient_values) {
       kept = at::empty({rows, cols}, h.options());
       slab_max = at::empty({rows, (vocab + 63) / 64}, fp32);
-      ctx->saved_data["kept"] = *kept;
-      ctx->saved_data["slab_max"] = *slab_max;
     }
     variable_list out = linear_score_outputs(h, w, ids, ignore_index, launch_rows, stats, kept, slab_max);
-    ctx->save_for_backward({h, w, ids, out[1], stats});
+    if (kept.has_value()) ctx->save_for_backward({h, w, ids, out[1], stats, *kept, *slab_max});      // (a checkpoint drops what is saved this way)
+    else ctx->save_for_backward({h, w, ids, out[1], stats});
+    ctx->saved_data["used"] = false;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["launch_rows"] = launch_rows;
     ctx->saved_data["gradient_values"] = gradient_values;
@@ -669,11 +669,10 @@ struct LinearScores : torch::autograd::Function<LinearScores> {
       if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
     at::Tensor buf;
     int64_t step = rows;
-    if (ctx->saved_data.count("kept")) {
-      buf = ctx->saved_data["kept"].toTensor();
-      slab_max = ctx->saved_data["slab_max"].toTensor();
-      ctx->saved_data.erase("kept");
-      ctx->saved_data.erase("slab_max");
+    if (saved.size() == 7 && !ctx->saved_data["used"].toBool()) {
+      buf = saved[5];
+      slab_max = saved[6];
+      ctx->saved_data["used"] = true;
     } else {
       step = std::max<int64_t>(256, std::min(ctx->saved_data["launch_rows"].toInt(), ctx->saved_data["gradient_values"].toInt() / cols / 256 * 256));
       buf = at::empty({std::min(rows, step), cols}, h.options());

@@ -478,6 +478,34 @@ def test_linear_token_log_probs_in_chunks(monkeypatch):
     _clean()
 
 
+def test_operators_under_a_checkpoint():
+    """Recomputed, not kept: the same bits, and no logits' worth of memory between the passes."""
+    from torch.utils.checkpoint import checkpoint
+
+    ops = _ops()
+    torch.manual_seed(43)
+    layout, H, hd, vocab = ops.PackedLayout([150, 3, 60]), 2, 64, 5000
+    x = torch.randn(213, 3 * H * hd, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn(vocab, H * hd, device="cuda") * 0.1).bfloat16().requires_grad_()
+    w2 = (torch.randn(H * hd, 64, device="cuda") * 0.1).requires_grad_()
+    ids = torch.randint(0, vocab, (213,), device="cuda")
+
+    def loss(x, w, w2):
+        h = ops.packed_attention(*x.split(H * hd, 1), layout, H, H, hd)
+        a = ops.linear_token_log_probs(h, w, ids)
+        b = ops.token_log_probs(h.float() @ w2, ids % 64)
+        return (a.log_probs + 0.1 * a.entropy + b.log_probs + 0.1 * b.entropy).sum()
+
+    want = torch.autograd.grad(loss(x, w, w2), (x, w, w2))
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    out = checkpoint(loss, x, w, w2, use_reentrant=False)
+    assert torch.cuda.memory_allocated() - before < 213 * vocab, "what the forward pass kept is still there"
+    got = torch.autograd.grad(out, (x, w, w2))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _clean()
+
+
 def test_linear_token_log_probs_of_a_long_vocabulary():
     """Few output tiles and a long inner dimension: the hidden states' gradient is cut along the vocabulary."""
     ops = _ops()
