@@ -9,8 +9,8 @@
 // `ignore` has log p = 0 and passes no g on; an id outside the vocabulary has log p = NaN and passes none on either.
 //
 // One pass over the logits.  fp32 logits run at the rate of memory (2048 x 151936: 178 us, 7.0 TB/s); bf16 ones come close to what the
-// SMs can exponentiate, 16 a clock (2048 x 151936: 105 to 116 us, 5.4 to 5.9 TB/s, exponential unit 63 to 72 % busy), and alternatives cost half as many
-// instructions again (1024 x 128256 with 8: 72 us, where 46 would do without).  A row goes to a cluster of 1 to 8 blocks, so that a few
+// SMs can exponentiate, 16 a clock (2048 x 151936: 105 to 116 us, 5.4 to 5.9 TB/s, exponential unit 63 to 72 % busy), and alternatives cost half as much
+// again (1024 x 128256 with 8: 66 us, where 46 would do without; of that a third at a row's start and end).  A row goes to a cluster of 1 to 8 blocks, so that a few
 // rows occupy the GPU as well (scores_split()); the blocks' partial results meet in distributed shared memory.  The gradient, one read
 // and one write, takes 215 us at 2048 x 151936 bf16 (5.8 TB/s).
 // Likeliest alternatives: each warp keeps a sorted list of 32, one a lane, as 64-bit keys of value and inverted index, so that equal
@@ -116,15 +116,25 @@ struct TopList {
   }
 };
 
-// The j-th largest over the lanes (each lane's value counts once).
-__device__ __forceinline__ float jth_largest(float x, int j, int lane) {
-  uint32_t u = static_cast<uint32_t>(key_of(x, 0) >> 32), top = 0;
-  for (int i = 0; i < j; ++i) {
-    top = __reduce_max_sync(0xffffffffu, u);
-    const uint32_t who = __ballot_sync(0xffffffffu, u == top);
-    if (lane == __ffs(who) - 1) u = 0;
+// A float in an order that unsigned words have, and a word a lane into descending order.
+__device__ __forceinline__ uint32_t word_of(float x) { return static_cast<uint32_t>(key_of(x, 0) >> 32); }
+__device__ __forceinline__ uint32_t sorted_down(uint32_t k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int j = size >> 1; j > 0; j >>= 1) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, k, j);
+      k = (((lane & j) == 0) == ((lane & size) == 0 || size == 32)) ? max(k, o) : min(k, o);
+    }
   }
-  return key_value(static_cast<Key>(top) << 32);
+  return k;
+}
+
+// The largest over the lanes, taken away from the first lane that has it.
+__device__ __forceinline__ uint32_t take_largest(uint32_t& u, int lane) {
+  const uint32_t top = __reduce_max_sync(0xffffffffu, u), who = __ballot_sync(0xffffffffu, u == top);
+  if (lane == __ffs(who) - 1) u = 0;
+  return top;
 }
 
 }  // namespace
@@ -177,19 +187,24 @@ __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_
 
 // Cluster = one row.  Block r of the cluster takes the r-th share of the row's whole 16-byte groups; what lies before the first
 // group and behind the last goes to the first block.
-// With alternatives: a thread's maximum so far is that of an element of its own, so the least of the warps' ceil(k / warps)-th largest
-// thread maxima is a value that k elements reach.  Nothing below it can be among the k; the warps publish and read it as they go (it only
-// grows, so an old one is still true), and after the first pass over the block's threads few groups of logits have a candidate.
+// With alternatives: a thread's maximum so far is that of an element of its own, so the k-th largest of all warps' four largest thread
+// maxima is a value that k elements reach.  Nothing below it can be among the k; the warps publish and read them as they go (they only
+// grow, so old ones are still true), and after the first pass over the block's threads few threads have a candidate.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(NT)
+__global__ void __launch_bounds__(NT, 4)
 token_scores_kernel(ScoreArgsDev p) {
   constexpr int N = Vec<T>::N, UN = 4, RING = 2;
+  // Up to FEW threads with candidates are looked through one after the other by the whole warp, more than that each through its own: 1024 x 128256
+  // with 8 alternatives 65 us (70 the second way always), 512 x 1024 with 5 12 us (17 the first way always).
+  // A warp looks the floor up again after RENEW threads with candidates: 1024 x 128256 with 1 / 8 / 20 59 / 66 / 71 us (65 / 65 / 74 by every
+  // second pass and the least of the warps' maxima).
+  constexpr int FEW = 2, RENEW = 8;
   __shared__ uint4 s_ring[RING][UN][NT];
   __shared__ Sums s_sums[NW];
   __shared__ Sums s_block;
   __shared__ Key s_buf[TOP ? NW * 64 : 1];
   __shared__ Key s_lists[TOP ? NW : 1][32];
-  __shared__ volatile float s_floor[NW];
+  __shared__ volatile uint32_t s_high[NW * 4];      // each warp's four largest thread maxima
   constexpr int POOL = 96;
   __shared__ Key s_pool[TOP ? POOL : 1];
   __shared__ int s_count;
@@ -216,10 +231,9 @@ token_scores_kernel(ScoreArgsDev p) {
   Sums a{-INFINITY, 0.f, 0.f};
   TopList top;
   float floor = -INFINITY;
-  const int nth = (p.k + NW - 1) / NW;
+  int seen = 0;                                     // candidates' threads since the floor was looked up
   if (TOP) {
     top.start(s_buf + warp * 64, lane, p.k);
-    if (lane == 0) s_floor[warp] = -INFINITY;
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
   }
@@ -235,6 +249,21 @@ token_scores_kernel(ScoreArgsDev p) {
       if (pass < passes && i < g1) copy_async16(&s_ring[pass % RING][u][threadIdx.x], body + i);
     }
     copy_async_commit();
+  };
+  auto publish = [&] {
+    uint32_t rest = word_of(a.m), high = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t most = take_largest(rest, lane);
+      high = lane == i ? most : high;
+    }
+    if (lane < 4) s_high[warp * 4 + lane] = high;
+  };
+  auto kth_published = [&] {
+    uint32_t rest = s_high[lane], kth = 0;
+    if (p.k > 12) kth = __shfl_sync(0xffffffffu, sorted_down(rest, lane), p.k - 1);      // (15 exchanges in a row)
+    else for (int i = 0; i < p.k; ++i) kth = take_largest(rest, lane);
+    return key_value(static_cast<Key>(kth) << 32);
   };
   for (int pass = 0; pass < RING - 1; ++pass) fetch(pass);
   for (int pass = 0; pass < passes; ++pass) {
@@ -260,17 +289,16 @@ token_scores_kernel(ScoreArgsDev p) {
     const float most = largest<UN * N>(v);
     take<UN * N>(a, v, most);
     if constexpr (TOP) {
-      if (pass < 2 || (pass & 1) == 0) {
-        const float mine = jth_largest(a.m, nth, lane);
-        if (lane == 0) s_floor[warp] = mine;
-        if (pass == 0) __syncthreads();             // the first value of every warp; later ones may be a little old
+      if (pass == 0 || seen >= RENEW) {
+        publish();
+        if (pass == 0) __syncthreads();               // the first values of every warp; later ones may be a little old
         else __syncwarp();
-        float f = s_floor[lane & (NW - 1)];
-#pragma unroll
-        for (int o = NW / 2; o > 0; o >>= 1) f = fminf(f, __shfl_xor_sync(0xffffffffu, f, o));
-        floor = f;
+        floor = kth_published();
+        seen = 0;
       }
-      if (__any_sync(0xffffffffu, most >= floor)) {
+      uint32_t who = __ballot_sync(0xffffffffu, most >= floor);
+      seen += __popc(who);
+      if (__popc(who) > FEW) {                        // every lane goes through its own, one at a time
         uint32_t hits = 0;
 #pragma unroll
         for (int q = 0; q < UN * N; ++q) hits |= v[q] >= floor ? 1u << q : 0u;
@@ -278,7 +306,7 @@ token_scores_kernel(ScoreArgsDev p) {
 #pragma unroll
           for (int u = 0; u < UN; ++u) if (group_of(pass, u) >= g1) hits &= ~(((1u << N) - 1) << (u * N));
         }
-        while (__any_sync(0xffffffffu, hits != 0)) {  // one of each lane at a time: as a rule that is all
+        while (__any_sync(0xffffffffu, hits != 0)) {
           Key key = 0;
           if (hits) {
             const int at = __ffs(hits) - 1, u = at / N, q = at % N;
@@ -288,6 +316,15 @@ token_scores_kernel(ScoreArgsDev p) {
           }
           top.push(key);
         }
+      } else if (who) {                               // as a rule: one lane or two, whose logits all lanes look at, one each
+        __syncwarp();
+        const int u = lane / N % UN, q = lane % N;
+        for (; who; who &= who - 1) {
+          const int of = __ffs(who) - 1, i = group_of(pass, u) - lane + of;
+          const float xq = Vec<T>::one(reinterpret_cast<const T*>(&s_ring[pass % RING][u][warp * 32 + of]) + q);
+          top.push(lane < UN * N && i < g1 && xq >= floor ? key_of(xq, static_cast<uint32_t>(head + i * N + q)) : 0);
+        }
+        __syncwarp();                                 // (the slots are copied to again)
       }
     }
   }
@@ -302,8 +339,7 @@ token_scores_kernel(ScoreArgsDev p) {
   }
   // lanes, warps, blocks
   if (TOP) {
-    const float mine = jth_largest(a.m, nth, lane);
-    if (lane == 0) s_floor[warp] = mine;
+    publish();
   }
   a = lanes_merged(a);
   if (lane == 0) s_sums[warp] = a;
@@ -332,9 +368,7 @@ token_scores_kernel(ScoreArgsDev p) {
       }
     } else {
       // what reaches the last floor: a few more than k as a rule, few enough for one warp
-      floor = s_floor[0];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) floor = fminf(floor, s_floor[w]);
+      floor = kth_published();
 #pragma unroll
       for (int i = 0; i < 3; ++i) {
         const Key key = i == 2 ? top.best : lane + 32 * i < top.waiting ? top.buf[lane + 32 * i] : 0;
@@ -348,8 +382,18 @@ token_scores_kernel(ScoreArgsDev p) {
     const int n = odd ? POOL + 1 : s_count;           // uniform
     if (n <= POOL) {
       if (warp == 0) {
-        top.best = 0;
-        for (int i = 0; i < n; i += 32) top.best = merged_down(top.best, sorted_down(i + lane < n ? s_pool[i + lane] : 0, lane), lane);
+        // (no two keys are alike: each finds its place by itself, without the exchanges in a row of a sort)
+        s_lists[0][lane] = 0;
+        __syncwarp();
+        for (int i = lane; i < n; i += 32) {
+          const Key mine = s_pool[i];
+          int before = 0;
+#pragma unroll 4
+          for (int j = 0; j < n; ++j) before += s_pool[j] > mine ? 1 : 0;
+          if (before < 32) s_lists[0][before] = mine;
+        }
+        __syncwarp();
+        top.best = s_lists[0][lane];
       }
     } else {
       while (top.waiting > 0) top.flush();
@@ -455,12 +499,13 @@ token_scores_grad_kernel(ScoreGradDev p, int blocks_per_row) {
   }
 }
 
-// Blocks per row, by what a few rows take alone (us, 1 / 2 / 4 / 8 blocks): 1 row of 151936 16.7 / 11.6 / 8.5 / 6.4; 16 rows with 5
-// alternatives 23.6 / 18.6 / 14.6 / 12.9; 64 with 8 24.8 / 18.6 / 16.6 / 23.9; 150 without 20.8 / 18.6 / 18.6 / 22.7.  From 300 rows on
-// a second block only doubles what a block costs at its ends: 333 x 32003 with 5 16.8 / 22.9, 1024 x 128256 with 8 72 / 91.
+// Blocks per row, by what a few rows take alone (us, 1 / 2 / 4 / 8 blocks): 1 row of 151936 13.0 / 8.8 / 6.1 / 5.1; 16 rows with 5
+// alternatives 21.3 / 15.2 / 11.0 / 10.0; 64 of 128256 with 8 20.2 / 15.1 / 12.7 / 13.3; 150 without 16.0 / 13.3 / 13.1 / 15.0, with 8
+// 24.4 / 21.0 / 22.4 / 27.5; 200 with 8 25.0 / 22.4 / 26.0 / 33.7.  From 300 rows on a second block only doubles what a block costs at its
+// ends: 333 x 32003 with 5 13.3 / 18.8, 1024 x 128256 with 8 67 / 82.
 static int scores_split(long long rows, int vocab) {
   int parts = 1;
-  while (parts < 8 && rows * parts <= num_sms() && vocab / (2 * parts) >= 2048) parts *= 2;
+  while (parts < 8 && 2 * rows * parts <= 3 * num_sms() && vocab / (2 * parts) >= 2048) parts *= 2;
   return parts;
 }
 
