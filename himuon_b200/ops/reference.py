@@ -124,8 +124,9 @@ def packed_attention(q2d, k2d, v2d, lengths, Hq: int, Hkv: int, head_dim: int, s
         first += n
     pad = q2d.shape[0] - first
     if pad or not parts:
-        # (through an empty slice, so that an empty batch has a gradient as well)
-        parts.append(F.pad(q2d[first:first], (0, 0, 0, pad)))
+        # (through empty slices, so that an empty batch has gradients as well)
+        rest = F.pad(q2d[first:first], (0, 0, 0, pad))
+        parts.append(rest if parts else rest + (k2d[first:first].sum() + v2d[first:first].sum()))
     return torch.cat(parts)
 
 

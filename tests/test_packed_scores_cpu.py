@@ -98,6 +98,13 @@ def test_packed_attention_of_no_tokens():
         assert not q.grad.any()
 
 
+def test_an_empty_batch_has_gradients():
+    q, k, v = (torch.randn(3, 2 * 8, requires_grad=True) for _ in range(3))
+    out = ops.packed_attention(q, k, v, ops.PackedLayout([0, 0], device="cpu"), 2, 2, 8)
+    grads = torch.autograd.grad(out.sum(), (q, k, v))
+    assert not out.any() and all(not g.any() for g in grads)
+
+
 def test_packed_attention_refuses():
     layout = ops.PackedLayout([3], device="cpu")
     q, kv = torch.randn(3, 32), torch.randn(3, 16)
