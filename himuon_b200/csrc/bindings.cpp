@@ -319,22 +319,31 @@ static void packed_rows(const char* op, const at::Tensor& t, const at::Tensor& q
                   t.stride(0) % 8 == 0 && (t.size(0) <= 1 || t.stride(0) >= cols) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               at, ": bf16 rows of heads * head_dim columns with unit inner stride, each on a 16-byte boundary, expected");
 }
+// Bytes of O's low bits: rows of a multiple of 16.
+static int64_t packed_low_size(int64_t Hq, int64_t tiles, int64_t hd) { return Hq * tiles * 128 * ((hd + 15) / 16 * 16); }
+static signed char* packed_low(const char* op, const at::Tensor& low, const at::Tensor& q, int64_t Hq, int64_t tiles) {
+  TORCH_CHECK(low.device() == q.device() && low.scalar_type() == at::kChar && low.is_contiguous() && low.numel() == packed_low_size(Hq, tiles, q.size(1) / Hq) &&
+                  reinterpret_cast<uintptr_t>(low.data_ptr()) % 16 == 0, std::string("himuon: ") + op, ": o_low must be int8, (heads, tiles * 128, head_dim rounded up to 16)");
+  return reinterpret_cast<signed char*>(low.data_ptr<int8_t>());
+}
 static void packed_attn_fwd(const at::Tensor& plan, int64_t tiles, int64_t tokens, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                            at::Tensor& o, const c10::optional<at::Tensor>& lse, int64_t Hq, int64_t Hkv, double scale) {
-  const himuon::PackedAttnArgs a = packed_attn_args("packed_attn_fwd", plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
+                            at::Tensor& o, const c10::optional<at::Tensor>& lse, const c10::optional<at::Tensor>& o_low, int64_t Hq, int64_t Hkv, double scale) {
+  himuon::PackedAttnArgs a = packed_attn_args("packed_attn_fwd", plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
   packed_rows("packed_attn_fwd", q, q, Hq * a.hd); packed_rows("packed_attn_fwd", k, q, Hkv * a.hd);
   packed_rows("packed_attn_fwd", v, q, Hkv * a.hd); packed_rows("packed_attn_fwd", o, q, Hq * a.hd);
+  if (o_low.has_value()) a.o_low = packed_low("packed_attn_fwd", *o_low, q, Hq, tiles);
   const c10::cuda::CUDAGuard guard(q.device());
   himuon::packed_attn_fwd(a, cur_stream());
 }
 static void packed_attn_bwd(const at::Tensor& plan, int64_t tiles, int64_t tokens, const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                            const at::Tensor& o, const at::Tensor& lse, at::Tensor& dq, at::Tensor& dk, at::Tensor& dv, at::Tensor& delta,
+                            const at::Tensor& o, const at::Tensor& lse, const at::Tensor& o_low, at::Tensor& dq, at::Tensor& dk, at::Tensor& dv, at::Tensor& delta,
                             const c10::optional<at::Tensor>& dkv_part, int64_t Hq, int64_t Hkv, double scale) {
   himuon::PackedAttnArgs a = packed_attn_args("packed_attn_bwd", plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
   for (const at::Tensor* t : {&q, &o, &d_o, static_cast<const at::Tensor*>(&dq)}) packed_rows("packed_attn_bwd", *t, q, Hq * a.hd);
   for (const at::Tensor* t : {&k, &v, static_cast<const at::Tensor*>(&dk), static_cast<const at::Tensor*>(&dv)}) packed_rows("packed_attn_bwd", *t, q, Hkv * a.hd);
   HM_CHECK(is_f32(delta) && delta.is_contiguous() && delta.device() == q.device() && delta.numel() == lse.numel() &&
                reinterpret_cast<uintptr_t>(delta.data_ptr()) % 16 == 0, "packed_attn_bwd: delta must look like lse");
+  a.o_low = packed_low("packed_attn_bwd", o_low, q, Hq, tiles);
   a.d_o = d_o.data_ptr(); a.dq = dq.data_ptr(); a.dk = dk.data_ptr(); a.dv = dv.data_ptr(); a.delta = delta.data_ptr<float>();
   a.ld_do = d_o.stride(0); a.ld_dq = dq.stride(0); a.ld_dk = dk.stride(0); a.ld_dv = dv.stride(0);
   if (dkv_part.has_value()) {
@@ -361,13 +370,14 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& plan, int64_t tiles,
                             int64_t tokens, int64_t Hq, int64_t Hkv, double scale, bool split_heads) {
     at::Tensor o = at::empty(q.sizes(), q.options()), lse = at::empty({Hq * tiles * 128}, q.options().dtype(at::kFloat));
+    const at::Tensor o_low = at::empty({packed_low_size(Hq, tiles, q.size(1) / Hq)}, q.options().dtype(at::kChar));
     if (tiles) {
-      packed_attn_fwd(plan, tiles, tokens, q, k, v, o, lse, Hq, Hkv, scale);
+      packed_attn_fwd(plan, tiles, tokens, q, k, v, o, lse, o_low, Hq, Hkv, scale);
       autograd_launched += 1;
     } else {
       o.zero_();
     }
-    ctx->save_for_backward({q, k, v, o, lse, plan});
+    ctx->save_for_backward({q, k, v, o, lse, plan, o_low});
     ctx->saved_data["tiles"] = tiles;
     ctx->saved_data["tokens"] = tokens;
     ctx->saved_data["Hq"] = Hq;
@@ -392,7 +402,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       at::Tensor delta = at::empty_like(lse);
       c10::optional<at::Tensor> part;
       if (ctx->saved_data["split_heads"].toBool()) part = at::empty({2 * lse.numel() * hd}, lse.options());
-      packed_attn_bwd(plan, tiles, ctx->saved_data["tokens"].toInt(), d_o, q, k, v, o, lse, dq, dk, dv, delta, part, Hq, Hkv, ctx->saved_data["scale"].toDouble());
+      packed_attn_bwd(plan, tiles, ctx->saved_data["tokens"].toInt(), d_o, q, k, v, o, lse, saved[6], dq, dk, dv, delta, part, Hq, Hkv, ctx->saved_data["scale"].toDouble());
       autograd_launched += part.has_value() ? 3 : 2;
     } else {
       all.zero_();

@@ -172,6 +172,7 @@ struct PackedAttnArgs {
   int n_tiles, n_pairs, tokens, rows, Hq, Hkv, hd;
   const void* q; const void* k; const void* v; void* o; float* lse;
   const void* d_o; void* dq; void* dk; void* dv; float* delta;
+  signed char* o_low;   // (Hq, n_tiles, hd / 16 rounded up, 128, 16): bits of O below its bf16 (low_of); forward: written unless null, backward: needed
   float* dkv_part;      // backward, optional: 2 * Hq * n_tiles * 128 * hd floats; dK and dV are then computed by query head and summed
   long long ld_q, ld_k, ld_v, ld_o, ld_do, ld_dq, ld_dk, ld_dv;
   float scale;

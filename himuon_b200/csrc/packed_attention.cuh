@@ -14,6 +14,8 @@ struct PackedDev {
   const PackedTile* tiles;
   void* o; float* nlse; float* ndelta;               // minus the base-2 log-sum-exp of the scaled scores, minus delta
   const void* o_in; const void* d_o;
+  signed char* o_low;                                // (Hq, tiles, low_ld / 16, 128, 16)
+  int low_ld;
   void* dq; void* dk; void* dv;
   int Hq, Hkv, hd;
   int tokens, rows;                                  // rows from `tokens` on belong to no document
@@ -42,6 +44,28 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, uint32_t half, int row
     for (int i = lane; i < n; i += 32) *reinterpret_cast<uint4*>(tile + j * half + row0 * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
+}
+
+// delta is a difference's second half: for a row whose softmax has one weight near 1, dP - delta is small beside either, and O in bf16 would leave it
+// half a bit of its 8 in error.  So the forward pass of training keeps 8 bits more: what O's fp32 word has above (or lacks) of the word of its
+// bf16, in units of 2^-8 of its last place.  low_of packs four of them, with_low adds one to its bf16.
+__device__ __forceinline__ uint32_t low_of(float f0, float f1, float f2, float f3, uint32_t b01, uint32_t b23) {
+  // (half a place up, rounded down to even, is 128 units, which are one too many)
+  const int d0 = min(__float_as_int(f0) - static_cast<int>(b01 << 16) + 0x80, 0x7FFF), d1 = min(__float_as_int(f1) - static_cast<int>(b01 & 0xFFFF0000u) + 0x80, 0x7FFF);
+  const int d2 = min(__float_as_int(f2) - static_cast<int>(b23 << 16) + 0x80, 0x7FFF), d3 = min(__float_as_int(f3) - static_cast<int>(b23 & 0xFFFF0000u) + 0x80, 0x7FFF);
+  return __byte_perm(__byte_perm(d0, d1, 0x0051), __byte_perm(d2, d3, 0x0051), 0x5410);
+}
+template <int I>
+__device__ __forceinline__ float with_low(uint32_t bf16_word, uint32_t low) {     // bf16_word: a bf16 as the upper half, zeros below
+  uint32_t d;                                        // 0, the byte, and twice its sign
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(d) : "r"(low), "n"(0x0004 | I << 4 | (8 | I) << 8 | (8 | I) << 12));
+  return __uint_as_float(bf16_word + d);
+}
+
+// Where a tile's low bits of a column are: 16 columns of all its rows together, which the threads of the forward pass, one row each, store
+// without gaps (24 documents, 8192 tokens, 16 heads over 8: 62 us against 63 with a row's bytes in one piece).
+__device__ __forceinline__ long long low_at(const PackedDev& p, int head, int slot, int row, int col) {
+  return (head * p.stat_rows + static_cast<long long>(slot) * AT) * p.low_ld + ((col >> 4) * AT + row) * 16 + (col & 15);
 }
 
 // Rows that belong to no document, zeroed by the threads of all blocks.
@@ -82,6 +106,7 @@ inline void check_packed(const PackedAttnArgs& a) {
 inline PackedDev make_dev(const PackedAttnArgs& a) {
   PackedDev p{};
   p.o = a.o; p.o_in = a.o; p.d_o = a.d_o; p.nlse = a.lse; p.ndelta = a.delta; p.dq = a.dq; p.dk = a.dk; p.dv = a.dv;
+  p.o_low = a.o_low; p.low_ld = (a.hd + 15) / 16 * 16;
   p.Hq = a.Hq; p.Hkv = a.Hkv; p.hd = a.hd; p.tokens = a.tokens; p.rows = a.rows;
   p.stat_rows = static_cast<long long>(a.n_tiles) * AT;
   p.ld_o = a.ld_o; p.ld_do = a.ld_do; p.ld_dq = a.ld_dq; p.ld_dk = a.ld_dk; p.ld_dv = a.ld_dv;

@@ -13,7 +13,7 @@
 // A product of 128 x 64 x 16 with both operands in shared memory takes 48 cycles, bound by its operands, one with A in tensor memory 64
 // (N = 128): a sub-block needs 1286 cycles of the dK / dV pass and 1029 of the dQ pass, and shared memory is busy for 1280 and 1152 (the
 // operands and 32 KB of new ones).  Measured, heads of 128: 1580 and 1280 cycles a sub-block; one document of 8192 tokens, 32 heads over 8, 853 and
-// 715 us (802 and 647 TFLOP/s of products, of which P and dP are computed twice), 24 documents of 341 tokens in the mean, 16 over 8, 94 and 82.
+// 715 us (802 and 647 TFLOP/s of products, of which P and dP are computed twice), 24 documents of 341 tokens in the mean, 16 over 8, 93 and 85.
 // One block for each item and two sub-blocks' scores in all took 990 and 800, 103 and 105: set-up and epilogue were some 10000
 // cycles an item, and the softmax of a sub-block on half of the warps took longer than the products beside it.
 #include "packed_attention.cuh"
@@ -570,7 +570,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int part = (warp - 18) >> 2;                 // two warps for the same 32 lanes: 16 rows of delta, 64 columns of dQ each
     uint8_t* stage = sOut + (part * 4 + (warp & 3)) * 4096;
-    // delta = sum over the head of O dO, 8 columns a lane
+    // delta = sum over the head of O dO, 8 columns a lane; O with the bits that its bf16 lacks (low_of)
     auto delta_of = [&](const DqItem& it, int round) {
       constexpr int BATCH = 4;                         // passes whose loads are on their way together
       const int c = (lane % LPR) * 8, r0 = (warp & 3) * 32 + part * 16 + lane / LPR;
@@ -579,13 +579,16 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll 1
       for (int k0 = 0; k0 < 16; k0 += BATCH * RPP) {
         uint4 o4[BATCH], g4[BATCH];
+        uint2 l2[BATCH];
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
           const int at = it.index * AT + r0 + k0 + k * RPP;
           o4[k] = g4[k] = make_uint4(0, 0, 0, 0);
+          l2[k] = make_uint2(0, 0);
           if (at < it.len && c < p.hd) {
             o4[k] = *reinterpret_cast<const uint4*>(o + static_cast<long long>(it.first + at) * p.ld_o);
             g4[k] = *reinterpret_cast<const uint4*>(g + static_cast<long long>(it.first + at) * p.ld_do);
+            l2[k] = *reinterpret_cast<const uint2*>(p.o_low + low_at(p, it.head, it.slot, r0 + k0 + k * RPP, c));
           }
         }
 #pragma unroll
@@ -593,7 +596,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           const uint32_t ow[4] = {o4[k].x, o4[k].y, o4[k].z, o4[k].w}, gw[4] = {g4[k].x, g4[k].y, g4[k].z, g4[k].w};
           float d = 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) d += bf16_lo(ow[q]) * bf16_lo(gw[q]) + bf16_hi(ow[q]) * bf16_hi(gw[q]);
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t low = q < 2 ? l2[k].x : l2[k].y, lo = ow[q] << 16, hi = ow[q] & 0xFFFF0000u;
+            d += (q & 1 ? with_low<2>(lo, low) : with_low<0>(lo, low)) * bf16_lo(gw[q]) + (q & 1 ? with_low<3>(hi, low) : with_low<1>(hi, low)) * bf16_hi(gw[q]);
+          }
 #pragma unroll
           for (int x = LPR / 2; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
           if (lane % LPR == 0) {

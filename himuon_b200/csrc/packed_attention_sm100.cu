@@ -32,7 +32,8 @@ namespace {
 // shared memory is busy for 1280 of them: the operands, and 32 KB of new K and V.  What the issuing warp does beside issuing counts in full,
 // because an MMA is issued about when it starts (the tensor core keeps two more): with a general step, ring positions found by division and
 // item fields that are not uniform the same step took 2200.  24 documents of 341 tokens in the mean, 16 heads over 8: 55 us, where an item has
-// some nine steps and 4300 cycles for its first scores, its last product and its epilogue.
+// some nine steps and 4300 cycles for its first scores, its last product and its epilogue.  What a backward pass needs (KEEP) costs 3 us there, 10 at the
+// one document.
 constexpr int FWD_THREADS = 320;                     // warps 0-3 and 4-7: rows of the tiles, 8: TMA, 9: MMA
 constexpr int BKV = 64;                              // key positions per block
 constexpr uint32_t KV_HALF = BKV * 128;              // one 64-column half of a K or V block: 8 KB
@@ -108,7 +109,8 @@ __device__ __forceinline__ void mask_future(uint32_t (&v)[32], int key0, int row
   for (int k = 0; k < 32; ++k) v[k] = key0 + k > row ? 0xFF800000u : v[k];
 }
 
-template <int NH>
+// KEEP: for a backward pass, with the log-sum-exps and O's low bits.
+template <int NH, bool KEEP>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ CUtensorMap tmO, PackedDev p) {
@@ -367,6 +369,21 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         uint32_t o[32];
         tmem_ld32(tO + c * 32, o);
         tmem_ld_wait();
+        if constexpr (KEEP) {
+          signed char* low = p.o_low + low_at(p, it.head, it.slot, row, c * 32);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float f[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) f[x] = __uint_as_float(o[h * 16 + k * 4 + x]) * inv;
+              w[k] = low_of(f[0], f[1], f[2], f[3], pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+            }
+            if (c * 32 + h * 16 < p.low_ld && lane < rows) *reinterpret_cast<uint4*>(low + h * 16 * AT) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
         if (whole) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
@@ -390,7 +407,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (e) tma_store_commit();
       }
       // minus the base-2 log-sum-exp of the scaled scores; rows past the end: such that their probabilities are 0
-      if (p.nlse) p.nlse[it.head * p.stat_rows + static_cast<long long>(it.slot) * AT + row] = lane < rows ? -m - log2f(l) : -INFINITY;
+      if (KEEP) p.nlse[it.head * p.stat_rows + static_cast<long long>(it.slot) * AT + row] = lane < rows ? -m - log2f(l) : -INFINITY;
       it = next;
     }
     tma_store_wait_all();
@@ -414,12 +431,12 @@ static CUtensorMap piece_tmap(const void* ptr, int rows, int H, int hd, long lon
   return make_tmap(ptr, 4, dims, strides, box, 2, true);
 }
 
-template <int NH>
+template <int NH, bool KEEP>
 static void launch_fwd(const PackedAttnArgs& a, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + 2 * NH * HALF_BYTES + FWD_SLOTS * NH * KV_HALF + 8 * NH * 4096 + sizeof(FwdBars);
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
   static std::atomic<uint64_t> done{0};
-  allow_smem(packed_fwd_kernel<NH>, SMEM, done);
+  allow_smem(packed_fwd_kernel<NH, KEEP>, SMEM, done);
   PackedDev p = make_dev(a);
   p.pair_heads = a.Hq / a.Hkv % 2 == 0 ? 1 : 0;
   p.tiles = p.pair_heads ? a.by_keys : a.pairs;
@@ -427,13 +444,15 @@ static void launch_fwd(const PackedAttnArgs& a, cudaStream_t s) {
   const CUtensorMap tq = head_tmap(a.q, 1, a.rows, a.Hq, a.hd, a.ld_q), tk = head_tmap(a.k, 1, a.rows, a.Hkv, a.hd, a.ld_k, BKV),
                     tv = head_tmap(a.v, 1, a.rows, a.Hkv, a.hd, a.ld_v, BKV), to = piece_tmap(a.o, a.rows, a.Hq, a.hd, a.ld_o);
   const int grid = p.n_items < num_sms() ? p.n_items : num_sms();
-  packed_fwd_kernel<NH><<<grid, FWD_THREADS, SMEM, s>>>(tq, tk, tv, to, p);
+  packed_fwd_kernel<NH, KEEP><<<grid, FWD_THREADS, SMEM, s>>>(tq, tk, tv, to, p);
 }
 void packed_attn_fwd(const PackedAttnArgs& a, cudaStream_t s) {
   check_packed(a);
   if (a.n_tiles == 0) return;
-  if (head_halves(a.hd) == 1) launch_fwd<1>(a, s);
-  else launch_fwd<2>(a, s);
+  if ((a.lse == nullptr) != (a.o_low == nullptr)) throw std::runtime_error("himuon packed attention: log-sum-exps and low bits go together");
+  const bool one = head_halves(a.hd) == 1;
+  if (a.lse) one ? launch_fwd<1, true>(a, s) : launch_fwd<2, true>(a, s);
+  else one ? launch_fwd<1, false>(a, s) : launch_fwd<2, false>(a, s);
   check_packed_launch("forward");
 }
 

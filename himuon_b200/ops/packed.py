@@ -179,7 +179,7 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
             return _ext.ext().packed_attention(q, k, v, layout.plan, layout.tiles, layout.tokens, Hq, Hkv, scale, layout.splits_heads(Hq, Hkv))
         o = torch.empty_like(q, memory_format=torch.contiguous_format)
         if layout.tiles:
-            _ext.ext().packed_attn_fwd(layout.plan, layout.tiles, layout.tokens, q, k, v, o, None, Hq, Hkv, scale)
+            _ext.ext().packed_attn_fwd(layout.plan, layout.tiles, layout.tokens, q, k, v, o, None, None, Hq, Hkv, scale)
             _count()
         else:
             o.zero_()

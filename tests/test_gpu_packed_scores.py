@@ -129,6 +129,35 @@ def test_packed_attention_of_peaked_scores_and_another_scale():
         _within(got, want[name], want["b" + name], name)
 
 
+def test_gradients_of_nearly_certain_rows():
+    """One weight near 1 in a row: dP - delta is small beside both, and what delta loses by O's rounding would be a multiple of it."""
+    ops = _ops()
+    torch.manual_seed(47)
+    H, hd, n = 3, 128, 400
+    layout = ops.PackedLayout([2] * n)
+    q, k, v = (torch.randn(2 * n, H * hd, device="cuda").bfloat16().requires_grad_() for _ in range(3))
+    do = torch.randn(2 * n, H * hd, device="cuda").bfloat16()
+    grads = torch.autograd.grad(ops.packed_attention(q, k, v, layout, H, H, hd, scale=0.5), (q, k, v), do)
+    a, b, c = (t.detach().double().view(n, 2, H, hd) for t in (q, k, v))
+    g = do.double().view(n, 2, H, hd)[:, 1]
+    # the second token of two: weights p and 1 - p, dS = p (1 - p) (dO v0 - dO v1) on the first and its negative on the second
+    p = torch.sigmoid(0.5 * (a[:, 1] * (b[:, 0] - b[:, 1])).sum(-1))
+    ds = p * (1 - p) * (g * (c[:, 0] - c[:, 1])).sum(-1)
+    dq = 0.5 * ds[..., None] * (b[:, 0] - b[:, 1])
+    # P and dS in bf16, O and delta to 2^-16 (and fp32 sums of 128 terms): relative to dS, and what is lost beside it, p of it on the
+    # first token and 1 - p on the second
+    lost = (2 * 2.0 ** -16 + 300 * 2.0 ** -24) * (g.abs() * (c[:, 0].abs() + c[:, 1].abs())).sum(-1)
+    lost = lost + 2.0 ** -8 * torch.minimum(p, 1 - p) * (g * (c[:, 0] - c[:, 1])).sum(-1).abs()
+    bound = 3 * 2.0 ** -8 * dq.abs() + 0.5 * (2 * 2.0 ** -8 * ds.abs() + 2 * lost)[..., None] * (b[:, 0].abs() + b[:, 1].abs()) + 1e-6
+    got = grads[0].double().view(n, 2, H, hd)
+    assert ((got[:, 1] - dq).abs() <= bound).all()
+    certain = torch.minimum(p, 1 - p) < 1e-3
+    assert certain.any()
+    err = (got[:, 1] - dq)[certain].norm() / dq[certain].norm()
+    assert err < 0.02, err
+    _clean()
+
+
 def test_packed_attention_gradient_against_differences():
     """The kernels' gradient along a direction against a central difference of the 64-bit formula."""
     ops = _ops()
@@ -272,11 +301,11 @@ def test_packed_attention_refusals_of_the_kernel_path():
     with pytest.raises(RuntimeError, match="layout is on"):
         ops.packed_attention(q, q, q, ops.PackedLayout([4], device="cpu"), 2, 2, 32)
     from himuon_b200._ext import ext
-    plan, lse = ops.PackedLayout([4]).plan, torch.empty(256, device="cuda")
-    ok = (plan, 1, 4, q, q, q, torch.empty_like(q), lse, 2, 2, 0.1)
+    plan, lse, low = ops.PackedLayout([4]).plan, torch.empty(256, device="cuda"), torch.empty(256 * 32, device="cuda", dtype=torch.int8)
+    ok = (plan, 1, 4, q, q, q, torch.empty_like(q), lse, low, 2, 2, 0.1)
     ext().packed_attn_fwd(*ok)
     for i, bad in [(0, plan.long()), (0, plan[:, :2].contiguous()), (0, plan.cpu()), (0, plan[:1]), (1, 2), (1, -1), (2, 5), (3, q.float()), (4, q[:, :32]), (5, q[:2]),
-                   (6, q.t()), (7, lse[:128]), (7, lse.double()), (8, 3), (9, 0), (3, torch.randn(5, 64, device="cuda").bfloat16().flatten()[4:260].view(4, 64))]:
+                   (6, q.t()), (7, lse[:128]), (7, lse.double()), (7, None), (8, low[:64]), (8, low.int()), (8, low.cpu()), (9, 3), (10, 0), (3, torch.randn(5, 64, device="cuda").bfloat16().flatten()[4:260].view(4, 64))]:
         with pytest.raises(RuntimeError, match="himuon"):
             ext().packed_attn_fwd(*ok[:i], bad, *ok[i + 1:])
     _clean()
