@@ -65,8 +65,14 @@ static GemmArgs gemm_args(const at::Tensor& a, const at::Tensor& b, const at::Te
 static void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, const c10::optional<at::Tensor>& aux,
                  bool trans_a, bool trans_b, double alpha, double beta, bool round_acc, int64_t max_ctas,
                  bool symmetric) {
-  const GemmArgs g = gemm_args(a, b, out, aux, trans_a, trans_b, alpha, beta, round_acc, max_ctas, symmetric);
+  GemmArgs g = gemm_args(a, b, out, aux, trans_a, trans_b, alpha, beta, round_acc, max_ctas, symmetric);
   const c10::cuda::CUDAGuard guard(a.device());
+  // (of this call's stream: calls on different streams share nothing)
+  at::Tensor parts;
+  if (const int64_t floats = himuon::gemm_parts_floats(g)) {
+    parts = at::empty({floats}, a.options().dtype(at::kFloat));
+    g.parts = parts.data_ptr<float>();
+  }
   himuon::gemm_bf16(g, cur_stream());
 }
 // Whether gemm() with these arguments runs on CTA pairs.

@@ -178,10 +178,10 @@ gemm2_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * BN2);
       const long long aux_row = static_cast<long long>(b) * p.strideAux + static_cast<long long>(m0 + row_in_tile) * p.ldaux;
       if (w.split) {
-        // K-slice of a last-wave tile: add the fp32 partial into the scratch tile (rows tail*256 + rank*128 ..);
-        // a follow-up kernel applies the epilogue to the complete sums
-        epilogue_tile_tma<BN2, true>(&tmW, slab, group, t_acc, row_in_tile, w.tail * 2 * BM + static_cast<int>(rank) * BM, 0, 0, nullptr, 0,
-                                     1 << 30, BN2, 1.f, 0.f, 0, issuer, true);
+        // K-slice of a last-wave tile: the fp32 partial goes to the slice's scratch tile (256 rows each, rank*128 ..); a follow-up
+        // kernel adds them up and applies the epilogue
+        epilogue_tile_tma<BN2, true>(&tmW, slab, group, t_acc, row_in_tile, (w.tail * p.nslices + w.slice) * 2 * BM + static_cast<int>(rank) * BM,
+                                     0, 0, nullptr, 0, 1 << 30, BN2, 1.f, 0.f, 0, issuer);
       } else if (m0 < p.M) {              // uniform: the second CTA of a ragged last row block has nothing to store
         if (p.reduce_out && p.out_fp32)   // C += alpha*acc without reading C: the L2 adds the staged slabs
           epilogue_tile_tma<BN2, true>(&tmC, slab, group, t_acc, row_in_tile, m0, nt * BN2, b, nullptr, 0, p.M, p.N, p.alpha,
@@ -202,7 +202,7 @@ gemm2_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
-    if (issuer) tma_store_wait_all();      // reductions into the scratch tiles are complete before the kernel ends
+    if (issuer) tma_store_wait_all();      // the scratch tiles are complete before the kernel ends
   }
 
   tc_fence_before();
@@ -214,11 +214,13 @@ gemm2_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   }
 }
 
-// Second half of the split-K tail: turns the complete fp32 sums of the last-wave tiles into outputs (alpha, beta*aux,
-// optional bf16 rounding point, cast) and leaves the scratch zeroed for the next launch.
+// Second half of the split-K tail: adds the slices' fp32 partials of the last-wave tiles, first to last whatever order they came in, and
+// turns the sums into outputs (alpha, beta*aux, optional bf16 rounding point, cast).  (Partials that meet by reductions in one zeroed
+// tile cost as much or more, reduced / added here: 2048 x 2560 x 9728 83.6 / 82.9 us, 2560 x 2048 x 6144 61.9 / 57.8, 8192 x 2560 x 9728 337 / 326,
+// 11520 x 2560 x 4096 202 / 205, and the order of three or more changes bits from run to run.)
 template <typename T>
 __global__ void __launch_bounds__(256)
-gemm2_finish_kernel(float* __restrict__ ws, GemmDev p, int first_tail_tile, int n_tail) {
+gemm2_finish_kernel(const float* __restrict__ ws, GemmDev p, int first_tail_tile, int n_tail) {
   const int tiles_per_batch = p.tiles_m * p.tiles_n;
   const long long per_tile = 256LL * 256 / 4;            // float4 groups per tile
   const long long total = per_tile * n_tail;
@@ -227,9 +229,13 @@ gemm2_finish_kernel(float* __restrict__ ws, GemmDev p, int first_tail_tile, int 
     const int t = static_cast<int>(i / per_tile);
     const int e = static_cast<int>(i - t * per_tile);
     const int r = e >> 6, c = (e & 63) * 4;
-    float4* src = reinterpret_cast<float4*>(ws + (static_cast<long long>(t) * 256 + r) * 256 + c);
-    const float4 v = *src;
-    *src = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4* src = reinterpret_cast<const float4*>(ws + (static_cast<long long>(t) * p.nslices * 256 + r) * 256 + c);
+    float4 v = src[0];
+#pragma unroll 4
+    for (int s = 1; s < p.nslices; ++s) {
+      const float4 u = src[s * per_tile];
+      v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+    }
     const int tile = first_tail_tile + t;
     const int b = tile / tiles_per_batch;
     const int rr = tile - b * tiles_per_batch;
@@ -254,23 +260,6 @@ gemm2_finish_kernel(float* __restrict__ ws, GemmDev p, int first_tail_tile, int 
       else reinterpret_cast<float*>(cp)[j] = o;
     }
   }
-}
-
-// fp32 scratch for the split-K tail of the pair kernel: up to kPairTailMax tiles of 256 x 256, zero between launches.
-// One buffer per device, shared by every GEMM of that device (GEMMs that split must not overlap on different streams).
-constexpr int kPairTailMax = 40;
-static float* pair_scratch() {
-  static float* per_device[64] = {nullptr};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) dev = 0;
-  if (per_device[dev] == nullptr) {
-    void* ptr = nullptr;
-    const size_t bytes = static_cast<size_t>(kPairTailMax) * 256 * 256 * sizeof(float);
-    if (cudaMalloc(&ptr, bytes) == cudaSuccess && cudaMemset(ptr, 0, bytes) == cudaSuccess) per_device[dev] = static_cast<float*>(ptr);
-    else cudaGetLastError();
-  }
-  return per_device[dev];
 }
 
 static CUtensorMap operand_tmap(const void* ptr, bool mn, int extent, int K, long long ld, int batch, long long stride) {
@@ -335,17 +324,15 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   }
   int cap = max_pairs;
   if (a.max_ctas > 0 && a.max_ctas / 2 < cap) cap = a.max_ctas / 2 > 0 ? a.max_ctas / 2 : 1;
-  // Split the tiles of a mostly idle last wave along K: each K-slice adds its fp32 partial tile into a scratch tile
-  // with TMA reductions and a small follow-up kernel applies the epilogue.
+  // Split the tiles of a mostly idle last wave along K: each K-slice stores its fp32 partial in the caller's scratch and a small
+  // follow-up kernel adds them and applies the epilogue.
   CUtensorMap tmW = tmC;
   const int rem = static_cast<int>(total % cap);
-  float* scratch = nullptr;
   // Accumulating fp32 outputs need no scratch to split a tile along K (every part just adds into C), so their work is
   // dealt out in equal contiguous (tile, k-block) ranges whenever whole tiles would not fill the last wave.
   const bool want_stream = p.reduce_out && total % cap != 0 && p.kblocks >= 8 &&
                            total * p.kblocks >= 8LL * cap;
-  if (!want_stream && total > cap / 2 && rem > 0 && rem * 2 <= cap && rem <= kPairTailMax && p.kblocks >= 16 &&
-      (scratch = pair_scratch()) != nullptr) {
+  if (!want_stream && a.parts != nullptr && total > cap / 2 && rem > 0 && rem * 2 <= cap && p.kblocks >= 16) {
     int sl = cap / rem;
     if (sl > p.kblocks / 8) sl = p.kblocks / 8;
     // worth it only when the K-blocks saved outweigh the fp32 reduction traffic and the second launch (~12 us)
@@ -353,10 +340,11 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
       p.nslices = sl;
       p.full_items = static_cast<int>(total) - rem;
       p.total_items = p.full_items + rem * sl;
-      const uint64_t dimsW[3] = {256, static_cast<uint64_t>(kPairTailMax) * 256, 1};
-      const uint64_t strW[2] = {256 * sizeof(float), static_cast<uint64_t>(kPairTailMax) * 256 * 256 * sizeof(float)};
+      const uint64_t rows = static_cast<uint64_t>(rem) * sl * 256;      // (rem * sl <= cap tiles)
+      const uint64_t dimsW[3] = {256, rows, 1};
+      const uint64_t strW[2] = {256 * sizeof(float), rows * 256 * sizeof(float)};
       const uint32_t boxW[3] = {32, BM, 1};
-      tmW = make_tmap(scratch, 3, dimsW, strW, boxW, 4, true);
+      tmW = make_tmap(a.parts, 3, dimsW, strW, boxW, 4, true);
     }
   }
   long long pairs = p.total_items < cap ? p.total_items : cap;
@@ -368,8 +356,8 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   if (p.nslices > 1) {
     const long long groups = 256LL * 256 / 4 * rem;
     const int blocks = static_cast<int>((groups + 255) / 256 < num_sms() * 4 ? (groups + 255) / 256 : num_sms() * 4);
-    if (a.out_fp32) gemm2_finish_kernel<float><<<blocks, 256, 0, stream>>>(scratch, p, p.full_items, rem);
-    else gemm2_finish_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(scratch, p, p.full_items, rem);
+    if (a.out_fp32) gemm2_finish_kernel<float><<<blocks, 256, 0, stream>>>(a.parts, p, p.full_items, rem);
+    else gemm2_finish_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(a.parts, p, p.full_items, rem);
   }
 }
 
@@ -407,6 +395,10 @@ static bool pairs_win(const GemmArgs& a) {
   if ((wide == 1 && (a.aux || a.out_fp32)) || (a.aux && a.K < 768)) return false;
   const int slack = (a.out_fp32 ? (a.aux ? -1024 : -256) : (a.aux ? -512 : 1024)) + (a_off ? 512 : 0);
   return (a.K + slack) * wide >= 1536;
+}
+long long gemm_parts_floats(const GemmArgs& a) {
+  // (a tile for each pair at most, where the plan may cut a last wave: reductions of 16 blocks or more)
+  return gemm2_supported(a) && a.K > 15 * BK ? static_cast<long long>(num_sms() / 2) * 256 * 256 : 0;
 }
 // True when the pair kernel can run this problem and is expected to win: TMA-storable output (whole 16-byte groups of
 // columns: a TMA store writes those whole, past the output's last column if need be) and more than one CTA tile of rows.

@@ -19,7 +19,7 @@ struct GemmDev {
   int tma_store;    // 1: epilogue goes through shared-memory slabs and TMA stores (needs 16-byte aligned C rows)
   int n_store;      // columns that TMA stores: N rounded down to whole 16-byte groups, because a TMA store writes those whole
   // Work list: items [0, full_items) are whole tiles; in the pair kernel each tile of a mostly empty last wave is cut
-  // into `nslices` K-ranges, one item each, whose fp32 partial sums meet in a scratch tile.
+  // into `nslices` K-ranges, one item each, whose fp32 partial sums go to a scratch tile each.
   int full_items, total_items, nslices;
   int reduce_out;   // pair kernel, C += alpha*acc (aux == C, beta == 1; fp32 or bf16): tiles add into C with TMA reductions
   int stream_k;     // with reduce_out: every CTA pair takes an equal, contiguous range of (tile, k-block) units and
@@ -286,7 +286,7 @@ __device__ __forceinline__ void epilogue_tile_tma(const CUtensorMap* tmC, uint8_
     fence_proxy_async_smem();
     named_barrier(2 + 2 * group, 128);                     // the slab is complete
     if (issuer) {
-      if (reduce_add) tma_reduce_add_3d(tmC, slab, col, m0, b);    // split-K: accumulate into the fp32 scratch tile
+      if (reduce_add) tma_reduce_add_3d(tmC, slab, col, m0, b);
       else tma_store_3d(tmC, slab, col, m0, b);
       tma_store_commit();
     }

@@ -36,7 +36,9 @@ struct GemmArgs {
   int max_ctas = 0;   // 0 = one CTA per SM
   int symmetric = 0;  // the caller guarantees C = C^T (X X^T, or c A A + b A with A symmetric): the one-CTA kernel then
                       // computes only the tiles that touch the lower triangle and mirrors the rest
+  float* parts = nullptr;   // gemm_parts_floats() floats for the partials of tiles that are cut along K; none are cut without
 };
+long long gemm_parts_floats(const GemmArgs& args);
 void gemm_bf16(const GemmArgs& args, cudaStream_t stream);
 // CTA-pair (cta_group::2) variant for 256 x 256 tiles; gemm_bf16 dispatches to it when gemm2_supported().
 bool gemm2_supported(const GemmArgs& args);

@@ -90,3 +90,35 @@ def test_optimizer_step_is_bitwise_reproducible():
         return [p.detach() for p in model.parameters()]
 
     _same_bits(run, runs=3)
+
+
+@pytest.mark.parametrize("M,N,K", [(2048, 2560, 9728), (2560, 2048, 6144), (11520, 2560, 4096)])
+def test_gemm_split_tail_is_bitwise_reproducible(M, N, K):
+    """A last wave of tiles cut into three or more K-slices: they are added in their order, not in that of their arrival."""
+    from himuon_b200 import ops
+
+    torch.manual_seed(4)
+    a = torch.randn(M, K, device="cuda", dtype=torch.bfloat16)
+    b = torch.randn(N, K, device="cuda", dtype=torch.bfloat16)
+    _same_bits(lambda: ops.gemm(a, b, trans_b=True), runs=6)
+    ops.check_status()
+
+
+def test_split_gemms_on_two_streams_do_not_meet():
+    """Two products whose last waves are cut run at the same time; neither finds the other's partial sums."""
+    from himuon_b200 import ops
+
+    torch.manual_seed(5)
+    operands = [(torch.randn(2048, 9728, device="cuda", dtype=torch.bfloat16), torch.randn(2560, 9728, device="cuda", dtype=torch.bfloat16)) for _ in range(2)]
+    want = [ops.gemm(a, b, trans_b=True) for a, b in operands]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in operands]
+    got = [[], []]
+    for _ in range(10):
+        for i, (a, b) in enumerate(operands):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.gemm(a, b, trans_b=True))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in outs)
+    ops.check_status()

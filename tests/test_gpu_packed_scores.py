@@ -611,3 +611,19 @@ def test_model_scores_of_a_packed_batch(model_type, head_dim):
         x, y = p.grad.flatten(), q.grad.float().flatten()
         assert torch.dot(x, y) / (x.norm() * y.norm() + 1e-12) > 0.99, n
         assert abs(y.norm() / (x.norm() + 1e-12) - 1) < 0.05, n
+
+
+def test_linear_token_log_probs_repeats_its_bits():
+    """Gradients whose products leave a last wave of tiles that is cut along the sum (2048 rows by 2560 columns: 80 tiles on 74 pairs)."""
+    ops = _ops()
+    torch.manual_seed(51)
+    h = torch.randn(2048, 2560, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn(9728, 2560, device="cuda") * 0.04).bfloat16().requires_grad_()
+    ids = torch.randint(0, 9728, (2048,), device="cuda")
+    g, seen = torch.randn(2048, device="cuda"), None
+    for _ in range(5):
+        s = ops.linear_token_log_probs(h, w, ids)
+        got = (s.log_probs.detach(), s.entropy.detach(), *torch.autograd.grad((s.log_probs, s.entropy), (h, w), (g, g)))
+        assert seen is None or all(torch.equal(a, b) for a, b in zip(seen, got))
+        seen = got
+    _clean()
