@@ -64,9 +64,10 @@ static GemmArgs gemm_args(const at::Tensor& a, const at::Tensor& b, const at::Te
 }
 static void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, const c10::optional<at::Tensor>& aux,
                  bool trans_a, bool trans_b, double alpha, double beta, bool round_acc, int64_t max_ctas,
-                 bool symmetric) {
+                 bool symmetric, bool ordered = false) {
   GemmArgs g = gemm_args(a, b, out, aux, trans_a, trans_b, alpha, beta, round_acc, max_ctas, symmetric);
   const c10::cuda::CUDAGuard guard(a.device());
+  g.ordered = ordered ? 1 : 0;
   // (of this call's stream: calls on different streams share nothing)
   at::Tensor parts;
   if (const int64_t floats = himuon::gemm_parts_floats(g)) {
@@ -713,7 +714,7 @@ struct LinearScores : torch::autograd::Function<LinearScores> {
         long_product(dx, w, to);
       }
       if (dw.defined()) {
-        gemm(dx, hc, dw, r ? c10::optional<at::Tensor>(dw) : c10::nullopt, true, false, 1.0, r ? 1.0 : 0.0, false, 0, false);
+        gemm(dx, hc, dw, r ? c10::optional<at::Tensor>(dw) : c10::nullopt, true, false, 1.0, r ? 1.0 : 0.0, false, 0, false, true);
         autograd_launched += 1;
       }
     }
@@ -781,7 +782,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("soap_ratio", &soap_ratio);
   m.def("gemm", &gemm, py::arg("a"), py::arg("b"), py::arg("out"), py::arg("aux") = py::none(), py::arg("trans_a") = false,
         py::arg("trans_b") = false, py::arg("alpha") = 1.0, py::arg("beta") = 0.0, py::arg("round_acc") = false,
-        py::arg("max_ctas") = 0, py::arg("symmetric") = false);
+        py::arg("max_ctas") = 0, py::arg("symmetric") = false, py::arg("ordered") = false);
   m.def("gemm_on_pairs", &gemm_on_pairs, py::arg("a"), py::arg("b"), py::arg("out"), py::arg("aux") = py::none(), py::arg("trans_a") = false,
         py::arg("trans_b") = false, py::arg("alpha") = 1.0, py::arg("beta") = 0.0, py::arg("round_acc") = false,
         py::arg("max_ctas") = 0, py::arg("symmetric") = false);

@@ -301,7 +301,7 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   p.tma_store = 1;
   p.nslices = 1;
   // (a bf16 C takes one rounding more that way, of the partial: long reductions only, as ever)
-  p.reduce_out = (a.K >= 2048 && a.aux == a.C && a.beta == 1.f && !a.round_acc &&
+  p.reduce_out = (!a.ordered && a.K >= 2048 && a.aux == a.C && a.beta == 1.f && !a.round_acc &&
                   a.ldaux == a.ldc && a.strideAux == a.strideC) ? 1 : 0;
   p.status = status_word_ptr();
   const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n * a.batch;
@@ -332,7 +332,8 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   // dealt out in equal contiguous (tile, k-block) ranges whenever whole tiles would not fill the last wave.
   const bool want_stream = p.reduce_out && total % cap != 0 && p.kblocks >= 8 &&
                            total * p.kblocks >= 8LL * cap;
-  if (!want_stream && a.parts != nullptr && total > cap / 2 && rem > 0 && rem * 2 <= cap && p.kblocks >= 16) {
+  // (Few tiles with ordered sums, which have no stream-K: all of them are the last wave.)
+  if (!want_stream && a.parts != nullptr && (total > cap / 2 || a.ordered) && rem > 0 && rem * 2 <= cap && p.kblocks >= 16) {
     int sl = cap / rem;
     if (sl > p.kblocks / 8) sl = p.kblocks / 8;
     // worth it only when the K-blocks saved outweigh the fp32 reduction traffic and the second launch (~12 us)

@@ -36,6 +36,7 @@ struct GemmArgs {
   int max_ctas = 0;   // 0 = one CTA per SM
   int symmetric = 0;  // the caller guarantees C = C^T (X X^T, or c A A + b A with A symmetric): the one-CTA kernel then
                       // computes only the tiles that touch the lower triangle and mirrors the rest
+  int ordered = 0;    // C += alpha*acc reads C and adds each tile once: no reductions into C, whose order is the schedule's
   float* parts = nullptr;   // gemm_parts_floats() floats for the partials of tiles that are cut along K; none are cut without
 };
 long long gemm_parts_floats(const GemmArgs& args);

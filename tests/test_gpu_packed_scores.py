@@ -627,3 +627,22 @@ def test_linear_token_log_probs_repeats_its_bits():
         assert seen is None or all(torch.equal(a, b) for a, b in zip(seen, got))
         seen = got
     _clean()
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [(6144, 2560, 2304), (24576, 640, 1024)])
+def test_linear_token_log_probs_in_chunks_repeats_its_bits(monkeypatch, rows, hidden, vocab):
+    """The weight's gradient summed over three chunks of rows, with tiles that do not fill their last round (9 by 10 on 74 pairs) or
+    are too few for one (4 by 3)."""
+    ops = _ops()
+    from himuon_b200.ops import scores
+
+    monkeypatch.setattr(scores, "GRADIENT_VALUES", rows // 3 * vocab)
+    torch.manual_seed(53)
+    h = torch.randn(rows, hidden, device="cuda").bfloat16().requires_grad_()
+    w = (torch.randn(vocab, hidden, device="cuda") * 0.04).bfloat16().requires_grad_()
+    ids, g, seen = torch.randint(0, vocab, (rows,), device="cuda"), torch.randn(rows, device="cuda"), None
+    for _ in range(6):
+        got = torch.autograd.grad(ops.linear_token_log_probs(h, w, ids).log_probs, (h, w), g)
+        assert seen is None or all(torch.equal(a, b) for a, b in zip(seen, got))
+        seen = got
+    _clean()
