@@ -102,6 +102,7 @@ struct TopList {
     const Key rest = lane + 32 < waiting ? buf[lane + 32] : 0;
     __syncwarp();
     buf[lane] = rest;
+    __syncwarp();                // (the exchanges below order no memory, and the next push of another lane may go to this slot)
     best = merged_down(best, sorted_down(x, lane), lane);
     kth = __shfl_sync(0xffffffffu, best, k - 1);
     waiting = waiting > 32 ? waiting - 32 : 0;

@@ -51,3 +51,14 @@ def test_no_unbounded_barrier_in_a_loop_that_threads_leave_one_by_one(name):
     for body in _loops(_code(CSRC / name)):
         if re.search(r"if \(!mbar_wait\(", body) and "break;" in body:
             assert not re.search(rf"\b(?:{barriers})\s*(?:<[^;()]*>)?\(|\bbar\.sync\b", body), body[:400]
+
+
+def test_the_waiting_list_of_a_warp_is_ordered_by_warp_barriers():
+    """`buf` is shared memory that every lane of a warp reads and writes at other lanes' places: exchanges and votes between lanes
+    order no memory, so that `flush` has a warp barrier before, between and behind its accesses (a push follows it)."""
+    code = _code(CSRC / "token_scores.cu")
+    body = code[code.index("void flush()"):]
+    body = body[: body.index("void push(")]
+    accesses = re.findall(r"__syncwarp\(\)|buf\[[^\]]*\](?: = )?", body)
+    kinds = ["barrier" if a.startswith("__") else "write" if a.endswith(" = ") else "read" for a in accesses]
+    assert kinds == ["barrier", "read", "read", "barrier", "write", "barrier"], kinds
