@@ -13,9 +13,10 @@ import operator
 
 import numpy as np
 import torch
+from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from .. import _ext
-from . import _check_width, _count, _warn_torch_path, _with_kernel_rows, use_kernels
+from . import _check_width, _count, _transformed, _warn_torch_path, _with_kernel_rows, use_kernels
 from . import reference as ref
 
 TILE = 128          # tokens of one document that a block of the kernels takes
@@ -153,7 +154,7 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
     """Causal GQA attention within each document of a packed batch, on ``(rows, heads*head_dim)`` views (``rows`` at least
     ``layout.tokens``; rows behind that are padding); returns ``(rows, Hq*head_dim)``.  ``scale`` defaults to
     ``1/sqrt(head_dim)`` and must be positive.  bf16 CUDA tensors with heads of a multiple of 8 up to 128 run the sm_100a kernels,
-    forward and backward.
+    forward and backward; under vmap and forward-mode differentiation, for which those have no rules, the PyTorch formulation runs.
 
     What is in other documents or in the padding has no part in a row, NaN and infinities included.  Those of a later token of the
     row's own document have weight 0, which does not take them out: as in :func:`attention`, a token that is not finite may reach
@@ -173,7 +174,8 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
     layout._check_rows("packed_attention", rows)
     if layout.device != q2d.device:
         raise RuntimeError(f"himuon_b200.ops.packed_attention: the layout is on {layout.device}, the tensors on {q2d.device}")
-    if use_kernels(q2d) and head_dim <= 128 and head_dim % 8 == 0:
+    transformed = any(map(_transformed, (q2d, k2d, v2d)))
+    if use_kernels(q2d) and head_dim <= 128 and head_dim % 8 == 0 and not transformed:
         q, k, v = _with_kernel_rows(q2d), _with_kernel_rows(k2d), _with_kernel_rows(v2d)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             return _ext.ext().packed_attention(q, k, v, layout.plan, layout.tiles, layout.tokens, Hq, Hkv, scale, layout.splits_heads(Hq, Hkv))
@@ -185,5 +187,8 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
             o.zero_()
         return o
     if use_kernels(q2d):
-        _warn_torch_path("packed_attention", f"head_dim {head_dim} (the kernels take multiples of 8 up to 128)")
+        _warn_torch_path("packed_attention", "under vmap or forward-mode differentiation" if transformed else f"head_dim {head_dim} (the kernels take multiples of 8 up to 128)")
+    if transformed:
+        with sdpa_kernel(SDPBackend.MATH):               # (the fused implementations have no forward-mode rule)
+            return ref.packed_attention(q2d, k2d, v2d, layout.lengths, Hq, Hkv, head_dim, scale)
     return ref.packed_attention(q2d, k2d, v2d, layout.lengths, Hq, Hkv, head_dim, scale)

@@ -646,3 +646,65 @@ def test_linear_token_log_probs_in_chunks_repeats_its_bits(monkeypatch, rows, hi
         assert seen is None or all(torch.equal(a, b) for a, b in zip(seen, got))
         seen = got
     _clean()
+
+
+# ------------------------------------------------------------------------------------------- transforms
+def _calls(dtype=torch.bfloat16):
+    """Each operator as a function of its first operand, with that operand and a direction; the results are tensors."""
+    ops = _ops()
+    torch.manual_seed(57)
+    layout = ops.PackedLayout([5, 0, 9])
+    k, v = (torch.randn(14, 64, device="cuda").to(dtype) for _ in range(2))
+    w, ids = (torch.randn(40, 64, device="cuda") * 0.3).to(dtype), torch.randint(0, 40, (14,), device="cuda")
+    fns = {"packed_attention": lambda t: (ops.packed_attention(t, k, v, layout, 2, 2, 32),),
+           "token_log_probs": lambda t: ops.token_log_probs(t, ids, top_k=3)[:2],
+           "linear_token_log_probs": lambda t: ops.linear_token_log_probs(t, w, ids)[:2]}
+    return fns, torch.randn(14, 64, device="cuda").to(dtype), torch.randn(14, 64, device="cuda").to(dtype)
+
+
+@pytest.mark.filterwarnings("ignore:himuon_b200.ops")
+@pytest.mark.parametrize("name", ["packed_attention", "token_log_probs", "linear_token_log_probs"])
+def test_forward_mode_tangents_are_not_lost(name):
+    """A dual tensor asks for no gradient and still has a derivative: that of a central difference, in 32 bits."""
+    from torch.autograd import forward_ad
+
+    fns, x, d = _calls(torch.float32)
+    h = 1e-2
+    slopes = [((a - b) / (2 * h)) for a, b in zip(fns[name](x + h * d), fns[name](x - h * d))]
+    for dtype in (torch.float32, torch.bfloat16):
+        fn, a, t = _calls(dtype)[0][name], x.to(dtype), d.to(dtype)
+        with forward_ad.dual_level():
+            duals = [forward_ad.unpack_dual(o) for o in fn(forward_ad.make_dual(a, t))]
+        for (_, tangent), slope in zip(duals, slopes):
+            assert tangent is not None
+            # bf16: operands and result rounded; the difference itself is good to a third derivative times h^2 / 6
+            assert (tangent.double() - slope.double()).norm() <= (0.05 if dtype == torch.bfloat16 else 1e-2) * slope.double().norm()
+        if dtype == torch.bfloat16:
+            _, tangents = torch.func.jvp(fn, (a,), (t,))
+            assert all(torch.equal(u, o.tangent) for u, o in zip(tangents, duals))
+    _clean()
+
+
+@pytest.mark.filterwarnings("ignore:himuon_b200.ops")
+@pytest.mark.parametrize("name", ["packed_attention", "token_log_probs", "linear_token_log_probs"])
+def test_operators_under_vmap(name):
+    """A batch of calls at once returns what the calls return one by one."""
+    fns, x, d = _calls()
+    got = torch.vmap(fns[name])(torch.stack([x, d]))
+    for i, a in enumerate((x, d)):
+        for one, all_of in zip(fns[name](a), got):
+            # the kernels and the plain formulation: bf16 roundings of values around 1, and of fp32 log probabilities of bf16 logits
+            assert (one.double() - all_of[i].double()).abs().max() <= (8 * U if name == "packed_attention" else 1e-4)
+    _clean()
+
+
+@pytest.mark.filterwarnings("ignore:himuon_b200.ops")
+def test_scores_under_vmap_over_ids_alone():
+    ops = _ops()
+    torch.manual_seed(59)
+    x, h, w = torch.randn(6, 40, device="cuda"), torch.randn(6, 64, device="cuda").bfloat16(), torch.randn(40, 64, device="cuda").bfloat16()
+    ids = torch.randint(0, 40, (3, 6), device="cuda")
+    for fn in (lambda i: ops.token_log_probs(x, i).log_probs, lambda i: ops.linear_token_log_probs(h, w, i).log_probs):
+        got = torch.vmap(fn)(ids)
+        assert all((fn(i) - g).abs().max() <= 1e-4 for i, g in zip(ids, got))
+    _clean()

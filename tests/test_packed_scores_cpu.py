@@ -228,3 +228,17 @@ def test_scores_of_a_model_train_it():
     (-model.score(ids, layout).log_probs.sum() / 18).backward()
     for a, p in zip(want, model.parameters()):
         assert torch.allclose(a, p.grad, atol=1e-6)
+
+
+def test_packed_attention_has_forward_mode_tangents_and_takes_vmap():
+    torch.manual_seed(5)
+    layout = ops.PackedLayout([3, 0, 6], device="cpu")
+    q, k, v, d = (torch.randn(10, 16, dtype=torch.float64) for _ in range(4))
+
+    def f(t):
+        return ops.packed_attention(t, k, v, layout, 2, 2, 8)
+
+    _, tangent = torch.func.jvp(f, (q,), (d,))
+    slope = (f(q + 1e-4 * d) - f(q - 1e-4 * d)) / 2e-4
+    assert torch.allclose(tangent, slope, rtol=1e-6, atol=1e-8)
+    assert torch.allclose(torch.vmap(f)(torch.stack([q, d])), torch.stack([f(q), f(d)]))
