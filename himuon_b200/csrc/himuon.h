@@ -201,7 +201,7 @@ void token_scores_bwd(const TokenScoreArgs& a, cudaStream_t s);
 // The same from hidden states (rows, hidden) and the head's weight (vocab, hidden), bf16, hidden a multiple of 8, row strides of
 // multiples of 8; logits stay on the chip (linear_scores_sm100.cu).  scratch: linear_scores_scratch() floats, forward only.
 // linear_scores_dlogits writes the logits' gradient, (rows, ld_grad) bf16, ld_grad the vocabulary rounded up to a multiple of 8.  With `grad` the
-// forward call keeps its exponentials there, as fp16, and with slab_max the other one turns them into the gradient in their place.
+// forward call keeps its exponentials there, 16 bits each, and with slab_max the other one turns them into the gradient in their place.
 struct LinearScoreArgs {
   const void* h; const void* w;
   long long ld_h, ld_w; int rows, hidden, vocab;

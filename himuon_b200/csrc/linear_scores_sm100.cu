@@ -4,14 +4,12 @@
 //   forward:   x = h W^T tile by tile; of each row of a tile only m = max x, s = sum e^(x-m), t = sum (x-m) e^(x-m) leave the kernel
 //              (and the logit of the row's own token); linear_scores_join_kernel merges a row's tiles (formulas in token_scores.cu).
 //   gradient:  dx_j = g [j = y] - p_j (g + h (log p_j + H)) as bf16, the operand of the products dx W and dx^T h that follow.  Either from the
-//              same product again, or, where the forward pass could keep them, from its exponentials: e^(x - m of 64 columns), at most 1,
-//              as fp16 (11 bits where the gradient gets 8; below 6e-8 of the largest of 64 they count for nothing), which the gradient then
-//              takes the place of.
+//              same product again, or, where the forward pass could keep them, from its exponentials: e^(x - m of 64 columns) in 16 bits
+//              (kept_pair: 10 bits at any size where the gradient gets 8), which the gradient then takes the place of.
 //
 // The product is the pair GEMM's (gemm2_sm100.cu has its protocol): 256 rows by 256 vocabulary entries per pair, six stages of 64 along
 // the hidden size, two accumulators, so that the epilogue of one tile runs beside the products of the next.  The tiles of one
 // vocabulary block are neighbours in the schedule: its rows of W come from memory once, the hidden states from the L2.
-#include <cuda_fp16.h>
 #include <stdint.h>
 
 #include "gemm_epilogue.cuh"
@@ -56,7 +54,16 @@ __device__ __forceinline__ void put_sums(const LinScoresDev& p, const Sums& a, i
   p.part[n + i] = a.s;
   p.part[2 * n + i] = a.t;
 }
-// The sums over 64 logits, and their exponentials relative to the largest, as fp16 pairs.
+// Two exponentials in 16 bits each.  They lie in 0..1, so that an fp32 word's sign and the first bit of its exponent are 0; the next 16
+// are kept, 7 of the exponent and 9 of the mantissa, rounded.  (fp16 has a bit more from 1 to 6e-5, loses one with each factor of 2 below and has nothing
+// under 3e-8: 17 nats beside a confident row's token.  A NaN may become a number: its row's sums are NaN, and so is the gradient.)
+__device__ __forceinline__ uint32_t kept_pair(float a, float b) {
+  return __byte_perm((__float_as_uint(a) << 2) + 0x8000u, (__float_as_uint(b) << 2) + 0x8000u, 0x7632);
+}
+__device__ __forceinline__ float2 from_kept(uint32_t w) {
+  return make_float2(__uint_as_float((w << 14) & 0x3FFFC000u), __uint_as_float((w >> 2) & 0x3FFFC000u));
+}
+// The sums over 64 logits, and their exponentials relative to the largest, as kept_pair()s.
 __device__ __forceinline__ Sums exponentials64(const float (&x)[64], uint32_t (&o)[32]) {
   const float m = largest<64>(x), base = m == -INFINITY ? 0.f : m;
   const f32x2 nbase = pack2(-base, -base), l2e = pack2(kLog2eS, kLog2eS);
@@ -72,8 +79,7 @@ __device__ __forceinline__ Sums exponentials64(const float (&x)[64], uint32_t (&
     const f32x2 e = pack2(y0, y1);
     s[i & 1] = add2(s[i & 1], e);
     t[i & 1] = fma2(pack2(fmaxf(d0, kFar), fmaxf(d1, kFar)), e, t[i & 1]);
-    const __half2 h = __floats2half2_rn(y0, y1);
-    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+    o[i] = kept_pair(y0, y1);
   }
   float s0, s1, t0, t1;
   unpack2(add2(s[0], s[1]), s0, s1);
@@ -489,7 +495,7 @@ kept_to_gradient_kernel(LinScoresDev p, uint4* kept, int groups, int blocks_per_
     if (r.h == 0.f) {                                 // uniform
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
+        const float2 e = from_kept(w[q]);
         d[q] = mul2(mul2(pack2(e.x, e.y), by), c0);
       }
     } else {
@@ -497,9 +503,9 @@ kept_to_gradient_kernel(LinScoresDev p, uint4* kept, int groups, int blocks_per_
       const f32x2 h = pack2(h2, h2), c = pack2(fmaf(r.h, f[u], r.c0), fmaf(r.h, f[u], r.c0));
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
-        // (an exponential of 0 gets the log of the least that fp16 has, and the product is 0 all the same)
-        const f32x2 l = pack2(__log2f(fmaxf(e.x, 5.9604645e-8f)), __log2f(fmaxf(e.y, 5.9604645e-8f)));
+        const float2 e = from_kept(w[q]);
+        // (an exponential of 0 gets the log of the least normal number, and the product is 0 all the same)
+        const f32x2 l = pack2(__log2f(fmaxf(e.x, 1.17549435e-38f)), __log2f(fmaxf(e.y, 1.17549435e-38f)));
         d[q] = mul2(mul2(pack2(e.x, e.y), by), fma2(h, l, c));
       }
     }

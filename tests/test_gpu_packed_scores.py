@@ -708,3 +708,38 @@ def test_scores_under_vmap_over_ids_alone():
         got = torch.vmap(fn)(ids)
         assert all((fn(i) - g).abs().max() <= 1e-4 for i, g in zip(ids, got))
     _clean()
+
+
+def _peaked_head(rows=128, vocab=1000):
+    """Hidden states that are unit vectors, so that a row's logits stand in a column of the weight and its logits' gradient in one of dw;
+    within 64 neighbours they spread over 50 nats, as beside the token of a confident row, and the neighbours' maxima over 30."""
+    torch.manual_seed(61)
+    top = -30 * torch.rand(rows, (vocab + 63) // 64, device="cuda")
+    top[:, 3] = 0
+    x = top.repeat_interleave(64, 1)[:, :vocab] - 50 * torch.rand(rows, vocab, device="cuda")
+    x.scatter_(1, torch.randint(3 * 64, 4 * 64, (rows, 1), device="cuda"), 0.0)
+    return torch.eye(rows, device="cuda").bfloat16().requires_grad_(), x.t().contiguous().bfloat16().requires_grad_()
+
+
+@pytest.mark.parametrize("with_entropy", [False, True])
+def test_head_gradient_of_peaked_rows_at_any_size(with_entropy):
+    """Each entry of the logits' gradient to its own size, from kept exponentials (the first backward pass) and from the logits
+    again (the second): an optimizer that normalises entries sees the error of the small ones too."""
+    ops = _ops()
+    h, w = _peaked_head()
+    ids, rows = torch.randint(0, w.shape[0], (h.shape[0],), device="cuda"), h.shape[0]
+    g, e = 0.5 + torch.rand(rows, device="cuda"), (torch.rand(rows, device="cuda") if with_entropy else torch.zeros(rows, device="cuda"))
+    s = ops.linear_token_log_probs(h, w, ids)
+    lp, _, entropy = _scores64(w.detach().double().t(), ids)
+    dx, size = _grad64(lp, entropy, ids, g, e)
+    p = lp.exp()
+    part = -p * (g.double() + e.double() * entropy)[:, None] - p * e.double()[:, None] * lp          # without the own token's g
+    # kept exponentials to 2^-10 (and as much of their logarithm in the entropy's part), fp32 exponents of up to 80 to 2^-17, then one
+    # rounding to bf16; what is below the normal numbers may be 0
+    bound = 2.0 ** -10 * (part.abs() + p * e.double()[:, None]) + 2.0 ** -13 * size
+    bound = bound + 2.0 ** -8 * (dx.abs() + bound) + 1e-37
+    outs = (s.log_probs, s.entropy) if with_entropy else (s.log_probs,)
+    for _ in range(2):
+        dw, = torch.autograd.grad(outs, w, (g, e)[: len(outs)], retain_graph=True)
+        _within(dw.t(), dx, bound, "gradient of the logits")
+    _clean()
