@@ -12,7 +12,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _ext
-from . import _transformed, _warn_torch_path, _with_kernel_rows, use_kernels
+from . import _any_transformed, _warn_torch_path, _with_kernel_rows, use_kernels
 from . import reference as ref
 
 MAX_TOP_K = 32
@@ -47,7 +47,7 @@ def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ign
     if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[1]):
         raise RuntimeError(f"himuon_b200.ops.token_log_probs: top_k must lie in 0..{min(MAX_TOP_K, logits.shape[1])}, got {top_k}")
     ids = _check_ids("token_log_probs", ids, logits.shape[0], logits.device)
-    transformed = any(map(_transformed, (logits, ids)))
+    transformed = _any_transformed(logits, ids)
     if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32) and not transformed:
         if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
             logits = logits.contiguous()
@@ -70,7 +70,7 @@ def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor
     if h2d.dim() != 2 or w.dim() != 2 or h2d.shape[1] != w.shape[1] or w.shape[0] == 0 or h2d.dtype != w.dtype or h2d.device != w.device:
         raise RuntimeError("himuon_b200.ops.linear_token_log_probs: (rows, hidden) and (vocab, hidden) of one type on one device expected")
     ids = _check_ids("linear_token_log_probs", ids, h2d.shape[0], h2d.device)
-    transformed = any(map(_transformed, (h2d, w, ids)))
+    transformed = _any_transformed(h2d, w, ids)
     if use_kernels(h2d) and h2d.shape[1] % 8 == 0 and h2d.shape[1] > 0 and not transformed:
         h2d, w = _with_kernel_rows(h2d), _with_kernel_rows(w)
         return TokenLogProbs(*_ext.ext().linear_scores(h2d, w, ids, int(ignore_index), LAUNCH_ROWS, GRADIENT_VALUES))
