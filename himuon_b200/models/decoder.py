@@ -182,7 +182,9 @@ class CausalLM(nn.Module):
     def hidden_states(self, input_ids, layout: ops.PackedLayout | None = None):
         B, S = input_ids.shape
         if layout is not None:
-            cos_sin = layout.rope_table(self._rope(max(layout.max_length, 1), input_ids.device), B * S)
+            # (tables of whole powers of two: batches differ in their longest document, and every length asked for is kept)
+            positions = 1 << (max(layout.max_length, 1) - 1).bit_length()
+            cos_sin = layout.rope_table(self._rope(positions, input_ids.device), B * S)
         else:
             cos_sin = self._rope(S, input_ids.device)
         h = ops.embedding(input_ids, self.model.embed_tokens.weight).reshape(B * S, -1)

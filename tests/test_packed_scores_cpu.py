@@ -242,3 +242,13 @@ def test_packed_attention_has_forward_mode_tangents_and_takes_vmap():
     slope = (f(q + 1e-4 * d) - f(q - 1e-4 * d)) / 2e-4
     assert torch.allclose(tangent, slope, rtol=1e-6, atol=1e-8)
     assert torch.allclose(torch.vmap(f)(torch.stack([q, d])), torch.stack([f(q), f(d)]))
+
+
+def test_a_model_keeps_few_rotary_tables_for_many_longest_documents():
+    model = _model()
+    with torch.no_grad():
+        for n in range(1, 60):
+            ids = torch.randint(0, 64, (1, n + 2))
+            model.score(ids, ops.PackedLayout([2, n], device="cpu"))
+    assert len(model._rope_cache) <= 6                     # 2, 4, ... 64 positions
+    assert sum(t.shape[0] for t in model._rope_cache.values()) <= 4 * 59
