@@ -474,6 +474,12 @@ def _with_kernel_rows(t: torch.Tensor) -> torch.Tensor:
     return t if _kernel_rows(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+def _with_rows_apart(t: torch.Tensor) -> torch.Tensor:
+    # The same for kernels that also want every row to have memory of its own: expanded and overlapping ones are copied.
+    apart = t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
+    return t if apart and _kernel_rows(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def _transformed(t: torch.Tensor) -> bool:
     """vmap / functorch wrappers and forward-mode duals, which an autograd function without those rules cannot take."""
     return torch._C._functorch.is_functorch_wrapped_tensor(t) or torch.autograd.forward_ad._current_level >= 0

@@ -16,7 +16,7 @@ import torch
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from .. import _ext
-from . import _any_transformed, _check_width, _count, _warn_torch_path, _with_kernel_rows, use_kernels
+from . import _any_transformed, _check_width, _count, _warn_torch_path, _with_rows_apart, use_kernels
 from . import reference as ref
 
 TILE = 128          # tokens of one document that a block of the kernels takes
@@ -176,7 +176,7 @@ def packed_attention(q2d, k2d, v2d, layout: PackedLayout, Hq: int, Hkv: int, hea
         raise RuntimeError(f"himuon_b200.ops.packed_attention: the layout is on {layout.device}, the tensors on {q2d.device}")
     transformed = _any_transformed(q2d, k2d, v2d)
     if use_kernels(q2d) and head_dim <= 128 and head_dim % 8 == 0 and not transformed:
-        q, k, v = _with_kernel_rows(q2d), _with_kernel_rows(k2d), _with_kernel_rows(v2d)
+        q, k, v = _with_rows_apart(q2d), _with_rows_apart(k2d), _with_rows_apart(v2d)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             return _ext.ext().packed_attention(q, k, v, layout.plan, layout.tiles, layout.tokens, Hq, Hkv, scale, layout.splits_heads(Hq, Hkv))
         o = torch.empty_like(q, memory_format=torch.contiguous_format)

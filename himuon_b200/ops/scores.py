@@ -12,7 +12,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _ext
-from . import _any_transformed, _warn_torch_path, _with_kernel_rows, use_kernels
+from . import _any_transformed, _warn_torch_path, _with_rows_apart, use_kernels
 from . import reference as ref
 
 MAX_TOP_K = 32
@@ -72,7 +72,7 @@ def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor
     ids = _check_ids("linear_token_log_probs", ids, h2d.shape[0], h2d.device)
     transformed = _any_transformed(h2d, w, ids)
     if use_kernels(h2d) and h2d.shape[1] % 8 == 0 and h2d.shape[1] > 0 and not transformed:
-        h2d, w = _with_kernel_rows(h2d), _with_kernel_rows(w)
+        h2d, w = _with_rows_apart(h2d), _with_rows_apart(w)
         return TokenLogProbs(*_ext.ext().linear_scores(h2d, w, ids, int(ignore_index), LAUNCH_ROWS, GRADIENT_VALUES))
     if use_kernels(h2d) and transformed:
         _warn_torch_path("linear_token_log_probs", "under vmap or forward-mode differentiation")

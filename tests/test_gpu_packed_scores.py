@@ -743,3 +743,32 @@ def test_head_gradient_of_peaked_rows_at_any_size(with_entropy):
         dw, = torch.autograd.grad(outs, w, (g, e)[: len(outs)], retain_graph=True)
         _within(dw.t(), dx, bound, "gradient of the logits")
     _clean()
+
+
+def test_operands_whose_rows_share_memory():
+    """Expanded and overlapping rows are results of ordinary calls: one state scored against many candidates, keys that all documents share."""
+    ops = _ops()
+    torch.manual_seed(63)
+    h, w = torch.randn(1, 64, device="cuda").bfloat16().requires_grad_(), torch.randn(90, 64, device="cuda").bfloat16().requires_grad_()
+    flat = torch.randn(64 + 8 * 69, device="cuda").bfloat16()
+    ids = torch.randint(0, 90, (70,), device="cuda")
+    for rows in (h.expand(70, 64), flat.as_strided((70, 64), (8, 1)).requires_grad_()):
+        got = []
+        for t in (rows, rows.contiguous()):
+            s = ops.linear_token_log_probs(t, w, ids)
+            got.append((s.log_probs, s.entropy, *torch.autograd.grad(s.log_probs.sum(), (rows, w))))
+            with torch.no_grad():
+                assert (ops.linear_token_log_probs(t, w, ids).log_probs - s.log_probs).abs().max() <= 1e-4
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+    layout = ops.PackedLayout([40, 30])
+    q, k, v = (torch.randn(n, 128, device="cuda").bfloat16().requires_grad_() for n in (70, 1, 1))
+    got = []
+    for kk, vv in ((k.expand(70, 128), v.expand(70, 128)), (k.repeat(70, 1), v.repeat(70, 1))):
+        o = ops.packed_attention(q, kk, vv, layout, 2, 2, 64)
+        with torch.no_grad():
+            assert torch.equal(ops.packed_attention(q, kk, vv, layout, 2, 2, 64), o)
+        got.append((o, *torch.autograd.grad(o, (q, kk, vv), torch.ones_like(o))))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    got = [ops.packed_attention(t, k.expand(70, 128), v.expand(70, 128), layout, 2, 2, 64) for t in (q[:1].expand(70, 128), q[:1].repeat(70, 1))]
+    assert torch.equal(*got)
+    _clean()
