@@ -50,7 +50,7 @@ def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ign
     transformed = _any_transformed(logits, ids)
     if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32) and not transformed:
         if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
-            logits = logits.contiguous()
+            logits = logits.clone(memory_format=torch.contiguous_format)      # (one column is contiguous at any stride)
         return TokenLogProbs(*_ext.ext().token_scores(logits, ids, int(top_k), int(ignore_index)))
     if logits.is_cuda and transformed:
         _warn_torch_path("token_log_probs", "under vmap or forward-mode differentiation")

@@ -772,3 +772,14 @@ def test_operands_whose_rows_share_memory():
     got = [ops.packed_attention(t, k.expand(70, 128), v.expand(70, 128), layout, 2, 2, 64) for t in (q[:1].expand(70, 128), q[:1].repeat(70, 1))]
     assert torch.equal(*got)
     _clean()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_token_log_probs_of_one_token_in_a_transposed_matrix(dtype):
+    ops = _ops()
+    x = torch.randn(1, 6, device="cuda").to(dtype).t().requires_grad_()
+    assert x.stride() == (1, 6)
+    s = ops.token_log_probs(x, torch.zeros(6, dtype=torch.int64, device="cuda"), top_k=1)
+    assert not s.log_probs.any() and not s.entropy.any() and not s.top_ids.any()
+    assert not torch.autograd.grad((s.log_probs.sum(), s.entropy.sum()), x)[0].any()
+    _clean()
