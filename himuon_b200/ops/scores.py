@@ -74,7 +74,8 @@ def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor
     if use_kernels(h2d) and h2d.shape[1] % 8 == 0 and h2d.shape[1] > 0 and not transformed:
         h2d, w = _with_rows_apart(h2d), _with_rows_apart(w)
         return TokenLogProbs(*_ext.ext().linear_scores(h2d, w, ids, int(ignore_index), LAUNCH_ROWS, GRADIENT_VALUES))
-    if use_kernels(h2d) and transformed:
-        _warn_torch_path("linear_token_log_probs", "under vmap or forward-mode differentiation")
+    if use_kernels(h2d):
+        _warn_torch_path("linear_token_log_probs", "under vmap or forward-mode differentiation" if transformed else
+                         f"hidden size {h2d.shape[1]} (the kernels take multiples of 8)")
     logits = h2d @ w.t() if h2d.dtype in (torch.float32, torch.float64) else h2d.float() @ w.float().t()
     return TokenLogProbs(*ref.token_log_probs(logits, ids, 0, ignore_index))

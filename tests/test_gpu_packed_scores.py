@@ -783,3 +783,11 @@ def test_token_log_probs_of_one_token_in_a_transposed_matrix(dtype):
     assert not s.log_probs.any() and not s.entropy.any() and not s.top_ids.any()
     assert not torch.autograd.grad((s.log_probs.sum(), s.entropy.sum()), x)[0].any()
     _clean()
+
+
+def test_an_odd_hidden_size_is_said_to_run_without_the_kernels():
+    ops = _ops()
+    ops._WARNED.discard(("linear_token_log_probs", "hidden size 63 (the kernels take multiples of 8)"))
+    h, w = torch.randn(4, 63, device="cuda").bfloat16(), torch.randn(20, 63, device="cuda").bfloat16()
+    with pytest.warns(UserWarning, match="linear_token_log_probs: hidden size 63"):
+        ops.linear_token_log_probs(h, w, torch.zeros(4, dtype=torch.int64, device="cuda"))
