@@ -12,6 +12,8 @@
 // vocabulary block are neighbours in the schedule: its rows of W come from memory once, the hidden states from the L2.
 #include <stdint.h>
 
+#include <atomic>
+
 #include "gemm_epilogue.cuh"
 #include "himuon.h"
 #include "pair_common.cuh"
@@ -545,10 +547,15 @@ static CUtensorMap rows_tmap(const void* ptr, int rows, int cols, long long ld, 
   return make_tmap(ptr, 3, dims, strides, box, 2, true);
 }
 
+// CTA pairs that can be resident at once on the current device.  (Callers and the autograd engine's threads may ask at the same time.)
 template <int MODE>
 static int pairs_at_once(size_t smem) {
-  static int most = 0;
-  if (most == 0) {
+  static std::atomic<int> most[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < 64;
+  int n = known ? most[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(num_sms());
     cfg.blockDim = dim3(LS_THREADS);
@@ -558,11 +565,13 @@ static int pairs_at_once(size_t smem) {
     attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, linear_scores_kernel<MODE>, &cfg) == cudaSuccess && n > 0) most = n;
-    else { cudaGetLastError(); most = num_sms() / 2; }
+    if (cudaOccupancyMaxActiveClusters(&n, linear_scores_kernel<MODE>, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = num_sms() / 2;
+    }
+    if (known) most[dev].store(n, std::memory_order_relaxed);
   }
-  return most;
+  return n;
 }
 
 template <int MODE>

@@ -62,3 +62,11 @@ def test_the_waiting_list_of_a_warp_is_ordered_by_warp_barriers():
     accesses = re.findall(r"__syncwarp\(\)|buf\[[^\]]*\](?: = )?", body)
     kinds = ["barrier" if a.startswith("__") else "write" if a.endswith(" = ") else "read" for a in accesses]
     assert kinds == ["barrier", "read", "read", "barrier", "write", "barrier"], kinds
+
+
+@pytest.mark.parametrize("name", ["packed_attention_sm100.cu", "packed_attention_bwd_sm100.cu", "packed_attention.cuh", "token_scores.cu", "token_scores.cuh",
+                                  "linear_scores_sm100.cu"])
+def test_what_launches_remember_is_safe_to_ask_from_two_threads(name):
+    """Callers and the autograd engine's threads launch these kernels at the same time: what a function keeps between calls is atomic."""
+    kept = re.findall(r"^[ \t]+static (?!__device__|constexpr|const |_assert|_cast)([^;(=]*)", _code(CSRC / name), re.M)
+    assert all(k.startswith("std::atomic<") for k in kept), kept
