@@ -637,7 +637,8 @@ static variable_list linear_score_outputs(const at::Tensor& h, const at::Tensor&
   const auto fp32 = h.options().dtype(at::kFloat);
   variable_list out = {at::empty({rows}, fp32), at::empty({rows}, fp32)};
   if (!rows) return out;
-  at::Tensor scratch = at::empty({himuon::linear_scores_scratch(std::min(rows, launch_rows), static_cast<int>(w.size(0)))}, fp32);
+  const int vocab = static_cast<int>(w.size(0));       // (a last launch of a few rows may need more than the others: its kernel has more parts)
+  at::Tensor scratch = at::empty({std::max(himuon::linear_scores_scratch(std::min(rows, launch_rows), vocab), himuon::linear_scores_scratch(rows % launch_rows, vocab))}, fp32);
   for (int64_t r = 0; r < rows; r += launch_rows) {
     const int64_t n = std::min(rows - r, launch_rows);
     auto chunk = [&](const at::Tensor& t) { return n == rows ? t : t.narrow(0, r, n); };

@@ -281,6 +281,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
 // there).  A block streams one share of the vocabulary in tiles of `th` entries; a thread keeps the sums of its lane for
 // up to 32 rows, and only at the end the 128 lanes meet.  8 rows over 151936 x 1024: 50 us (6.2 TB/s), pair kernel 99.
 constexpr int FEW_STAGES = 9;
+constexpr int FEW_ROWS = 64;
 constexpr int few_threads(int nb) { return 64 + 128 * (nb > 32 ? nb / 32 : 1); }      // warp 0: TMA, 1: MMA, then four for each 32 rows
 struct FewBars {
   uint64_t full[FEW_STAGES], empty[FEW_STAGES], tfull[2], tempty[2];
@@ -624,8 +625,11 @@ static LinScoresDev make_dev(const LinearScoreArgs& a) {
   return p;
 }
 
-// Room for the most parts that either forward kernel has: one for each 64 entries (launch_few), and the rows' own logits.
-long long linear_scores_scratch(long long rows, int vocab) { return rows * (1 + 3LL * 2 * ((vocab + 127) / 128)); }
+// Room for the parts of the forward kernel that takes so many rows, one for each 64 entries (launch_few) or 128, and the rows' own logits.
+long long linear_scores_scratch(long long rows, int vocab) {
+  const int per = rows <= FEW_ROWS ? 128 : LS_N;
+  return rows * (1 + 3LL * 2 * ((vocab + per - 1) / per));
+}
 
 void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {
   LinScoresDev p = make_dev(a);
@@ -635,7 +639,7 @@ void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {
     p.slabs = (a.vocab + 63) / 64;
     launch<STATS_KEPT>(a, p, s);
     n_parts = 2 * p.tiles_n;
-  } else if (a.rows <= 64) {
+  } else if (a.rows <= FEW_ROWS) {
     n_parts = a.rows <= 16 ? launch_few<16>(a, p, s) : a.rows <= 32 ? launch_few<32>(a, p, s) : launch_few<64>(a, p, s);
   } else {
     launch<STATS>(a, p, s);

@@ -791,3 +791,26 @@ def test_an_odd_hidden_size_is_said_to_run_without_the_kernels():
     h, w = torch.randn(4, 63, device="cuda").bfloat16(), torch.randn(20, 63, device="cuda").bfloat16()
     with pytest.warns(UserWarning, match="linear_token_log_probs: hidden size 63"):
         ops.linear_token_log_probs(h, w, torch.zeros(4, dtype=torch.int64, device="cuda"))
+
+
+def test_scores_of_a_head_take_no_more_scratch_than_their_parts(monkeypatch):
+    """Three floats for each row and 128 tokens above 64 rows, for each 64 below; a last launch of a few rows fits in as well."""
+    ops = _ops()
+    from himuon_b200.ops import scores
+
+    w, ids = torch.randn(60000, 64, device="cuda").bfloat16(), torch.zeros(1024, dtype=torch.int64, device="cuda")
+    h = torch.randn(1024, 64, device="cuda").bfloat16()
+    with torch.no_grad():
+        for rows, per in ((1024, 128), (65, 128), (64, 64), (8, 64)):
+            ops.linear_token_log_probs(h[:rows], w, ids[:rows])
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            ops.linear_token_log_probs(h[:rows], w, ids[:rows])
+            # (two results, roundings of a block of memory, and the scratch of two tiles that the vocabulary ends in)
+            assert torch.cuda.max_memory_allocated() - before <= 12 * rows * (60000 / per + 4) + 2 ** 16
+        want = ops.linear_token_log_probs(h[:129], w, ids[:129])
+        monkeypatch.setattr(scores, "LAUNCH_ROWS", 65)
+        got = ops.linear_token_log_probs(h[:129], w, ids[:129])
+        assert (got.log_probs - want.log_probs).abs().max() <= 1e-4 and torch.equal(got.log_probs[:65], want.log_probs[:65])
+    _clean()
