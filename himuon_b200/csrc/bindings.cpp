@@ -1,6 +1,7 @@
 // PyTorch bindings: tensors in, raw pointers + current stream out.  All checks that would
 // otherwise become device faults (dtype, contiguity, alignment, shape agreement) happen here.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -573,10 +574,14 @@ static void linear_scores_fwd(const at::Tensor& h, const at::Tensor& w, const at
 }
 static void linear_scores_dlogits(const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, const at::Tensor& entropy, const at::Tensor& stats,
                                   const c10::optional<at::Tensor>& g_log_probs, const c10::optional<at::Tensor>& g_entropy, at::Tensor& grad,
-                                  const c10::optional<at::Tensor>& slab_max, int64_t ignore_index) {
+                                  const c10::optional<at::Tensor>& kept, const c10::optional<at::Tensor>& slab_max, int64_t ignore_index) {
   himuon::LinearScoreArgs a = linear_score_args("linear_scores_dlogits", h, w, ids, entropy, stats, ignore_index);
   for (const auto* g : {&g_log_probs, &g_entropy})
     if (g->has_value()) HM_CHECK((*g)->device() == h.device() && is_f32(**g) && (*g)->is_contiguous() && (*g)->numel() == a.rows, "linear_scores_dlogits: incoming gradients must be fp32, one for each row");
+  if (kept.has_value()) {
+    linear_score_kept("linear_scores_dlogits", a, h, *kept, slab_max);
+    a.kept = a.grad;
+  }
   linear_score_kept("linear_scores_dlogits", a, h, grad, slab_max);
   a.g_log_probs = g_log_probs.has_value() ? g_log_probs->data_ptr<float>() : nullptr;
   a.g_entropy = g_entropy.has_value() ? g_entropy->data_ptr<float>() : nullptr;
@@ -651,7 +656,7 @@ static variable_list linear_score_outputs(const at::Tensor& h, const at::Tensor&
 }
 
 // The backward pass multiplies the logits' gradient with both operands.  It gets it from the exponentials that the forward pass kept, in
-// their place; where there are none (more than `gradient_values`, a few rows, whose kernel keeps nothing, or used up by an earlier backward
+// their place (one that a graph captures, elsewhere); where there are none (more than `gradient_values`, a few rows, whose kernel keeps nothing, or used up by an earlier backward
 // pass) it makes the logits again, for as many rows at a time as that allows.
 struct LinearScores : torch::autograd::Function<LinearScores> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& ids, int64_t ignore_index, int64_t launch_rows,
@@ -669,6 +674,7 @@ struct LinearScores : torch::autograd::Function<LinearScores> {
     if (kept.has_value()) ctx->save_for_backward({h, w, ids, out[1], stats, *kept, *slab_max});      // (a checkpoint drops what is saved this way)
     else ctx->save_for_backward({h, w, ids, out[1], stats});
     ctx->saved_data["used"] = false;
+    ctx->saved_data["captured"] = false;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["launch_rows"] = launch_rows;
     ctx->saved_data["gradient_values"] = gradient_values;
@@ -682,15 +688,22 @@ struct LinearScores : torch::autograd::Function<LinearScores> {
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor &h = saved[0], &w = saved[1];
     const int64_t rows = h.size(0), vocab = w.size(0), cols = (vocab + 7) / 8 * 8, ignore_index = ctx->saved_data["ignore_index"].toInt();
-    c10::optional<at::Tensor> g[2], slab_max;
+    c10::optional<at::Tensor> g[2], kept, slab_max;
     for (int i = 0; i < 2; ++i)
       if (grads[i].defined()) g[i] = grads[i].to(at::kFloat).contiguous();
     at::Tensor buf;
     int64_t step = rows;
     if (saved.size() == 7 && !ctx->saved_data["used"].toBool()) {
-      buf = saved[5];
       slab_max = saved[6];
-      ctx->saved_data["used"] = true;
+      const bool captured = c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+      if (captured) ctx->saved_data["captured"] = true;    // may be replayed, and again for one forward pass: what was kept stays
+      if (ctx->saved_data["captured"].toBool()) {
+        kept = saved[5];
+        buf = at::empty_like(*kept);
+      } else {
+        buf = saved[5];
+        ctx->saved_data["used"] = true;
+      }
     } else {
       step = std::max<int64_t>(256, std::min(ctx->saved_data["launch_rows"].toInt(), ctx->saved_data["gradient_values"].toInt() / cols / 256 * 256));
       buf = at::empty({std::min(rows, step), cols}, h.options());
@@ -707,7 +720,7 @@ struct LinearScores : torch::autograd::Function<LinearScores> {
       auto maybe = [&](const c10::optional<at::Tensor>& t) { return t.has_value() ? c10::optional<at::Tensor>(chunk(*t)) : c10::nullopt; };
       at::Tensor dx = buf.size(0) == n ? buf : buf.narrow(0, 0, n);
       const at::Tensor hc = chunk(h);
-      linear_scores_dlogits(hc, w, chunk(saved[2]), chunk(saved[3]), chunk(saved[4]), maybe(g[0]), maybe(g[1]), dx, slab_max, ignore_index);
+      linear_scores_dlogits(hc, w, chunk(saved[2]), chunk(saved[3]), chunk(saved[4]), maybe(g[0]), maybe(g[1]), dx, kept, slab_max, ignore_index);
       autograd_launched += 1;
       if (cols != vocab) dx = dx.narrow(1, 0, vocab);
       if (dh.defined()) {

@@ -201,7 +201,8 @@ void token_scores_bwd(const TokenScoreArgs& a, cudaStream_t s);
 // The same from hidden states (rows, hidden) and the head's weight (vocab, hidden), bf16, hidden a multiple of 8, row strides of
 // multiples of 8; logits stay on the chip (linear_scores_sm100.cu).  scratch: linear_scores_scratch() floats, forward only.
 // linear_scores_dlogits writes the logits' gradient, (rows, ld_grad) bf16, ld_grad the vocabulary rounded up to a multiple of 8.  With `grad` the
-// forward call keeps its exponentials there, 16 bits each, and with slab_max the other one turns them into the gradient in their place.
+// forward call keeps its exponentials there, 16 bits each, and with slab_max the other one turns them into the gradient, from `kept` or, where
+// that is null, in their place.
 struct LinearScoreArgs {
   const void* h; const void* w;
   long long ld_h, ld_w; int rows, hidden, vocab;
@@ -209,6 +210,7 @@ struct LinearScoreArgs {
   float* log_probs; float* entropy; float* stats; float* scratch;
   const float* g_log_probs; const float* g_entropy;
   void* grad; long long ld_grad;
+  const void* kept;                          // gradient only: exponentials that are to stay as they are, laid out as grad
   float* slab_max;                           // (rows, vocabulary / 64 rounded up) maxima that kept exponentials are relative to
 };
 long long linear_scores_scratch(long long rows, int vocab);

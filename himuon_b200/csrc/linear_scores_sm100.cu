@@ -470,9 +470,9 @@ linear_scores_join_kernel(LinScoresDev p, int n_parts, float* log_probs, float* 
   }
 }
 
-// Kept exponentials of a row into the gradient of its logits, in their place.  A thread has 8 columns, which share their 64's maximum.
+// Kept exponentials of a row into the gradient of its logits, in their place as a rule.  A thread has 8 columns, which share their 64's maximum.
 __global__ void __launch_bounds__(256)
-kept_to_gradient_kernel(LinScoresDev p, uint4* kept, int groups, int blocks_per_row) {
+kept_to_gradient_kernel(LinScoresDev p, const uint4* kept, uint4* grad, int groups, int blocks_per_row) {
   const long long row = blockIdx.x / blocks_per_row;
   const int piece = static_cast<int>(blockIdx.x - row * blocks_per_row);
   const RowGrad r = row_grad(p.stats, p.entropy, p.ids, p.g_log_probs, p.g_entropy, p.ignore, p.vocab, row);
@@ -523,7 +523,7 @@ kept_to_gradient_kernel(LinScoresDev p, uint4* kept, int groups, int blocks_per_
       }
       o[q] = pack_bf16x2(d0, d1);
     }
-    __stcs(kept + row * groups + i, make_uint4(o[0], o[1], o[2], o[3]));
+    __stcs(grad + row * groups + i, make_uint4(o[0], o[1], o[2], o[3]));
   }
 }
 
@@ -668,7 +668,7 @@ void linear_scores_dlogits(const LinearScoreArgs& a, cudaStream_t s) {
     p.slabs = (a.vocab + 63) / 64;
     const int groups = static_cast<int>(a.ld_grad / 8), per_row = (groups + 1023) / 1024;
     if (static_cast<long long>(a.rows) * per_row >= (1LL << 31)) throw std::runtime_error("himuon linear_scores: gradient too large for one launch");
-    kept_to_gradient_kernel<<<a.rows * per_row, 256, 0, s>>>(p, reinterpret_cast<uint4*>(a.grad), groups, per_row);
+    kept_to_gradient_kernel<<<a.rows * per_row, 256, 0, s>>>(p, reinterpret_cast<const uint4*>(a.kept ? a.kept : a.grad), reinterpret_cast<uint4*>(a.grad), groups, per_row);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores gradient launch failed: ") + cudaGetErrorString(e));
     return;

@@ -814,3 +814,43 @@ def test_scores_of_a_head_take_no_more_scratch_than_their_parts(monkeypatch):
         got = ops.linear_token_log_probs(h[:129], w, ids[:129])
         assert (got.log_probs - want.log_probs).abs().max() <= 1e-4 and torch.equal(got.log_probs[:65], want.log_probs[:65])
     _clean()
+
+
+def test_head_gradients_replayed_twice_for_one_forward_pass():
+    """Captured apart, the backward pass runs as often as it is replayed: it must not use up what the forward pass kept."""
+    ops = _ops()
+    torch.manual_seed(67)
+    h, w = torch.randn(100, 64, device="cuda").bfloat16().requires_grad_(), torch.randn(500, 64, device="cuda").bfloat16().requires_grad_()
+    ids, g = torch.randint(0, 500, (100,), device="cuda"), torch.randn(100, device="cuda")
+
+    def scores(a, b):
+        return ops.linear_token_log_probs(a, b, ids).log_probs
+
+    want = torch.autograd.grad(scores(h, w), (h, w), g)
+    graphed = torch.cuda.make_graphed_callables(scores, (h, w))
+    out = graphed(h, w)
+    for _ in range(3):
+        got = torch.autograd.grad(out, (h, w), g, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _clean()
+
+
+def test_head_gradients_replayed_after_an_eager_pass_on_the_same_graph():
+    ops = _ops()
+    torch.manual_seed(69)
+    h, w = torch.randn(100, 64, device="cuda").bfloat16().requires_grad_(), torch.randn(500, 64, device="cuda").bfloat16().requires_grad_()
+    ids, g = torch.randint(0, 500, (100,), device="cuda"), torch.randn(100, device="cuda")
+    want = torch.autograd.grad(ops.linear_token_log_probs(h, w, ids).log_probs, (h, w), g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        out = ops.linear_token_log_probs(h, w, ids).log_probs
+        with torch.cuda.graph(graph, stream=side):
+            captured = torch.autograd.grad(out, (h, w), g, retain_graph=True)
+        eager = torch.autograd.grad(out, (h, w), g, retain_graph=True)
+        graph.replay()
+    side.synchronize()
+    for got in (eager, captured):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    _clean()
