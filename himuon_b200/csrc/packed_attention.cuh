@@ -101,7 +101,8 @@ __device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
 inline void check_packed(const PackedAttnArgs& a) {
   if (a.Hq <= 0 || a.Hkv <= 0 || a.Hq % a.Hkv || a.rows <= 0 || a.n_tiles < 0) throw std::runtime_error("himuon packed attention: bad sizes");
   if (a.hd <= 0 || a.hd > 128 || a.hd % 8) throw std::runtime_error("himuon packed attention: head_dim must be a multiple of 8 up to 128");
-  if (static_cast<long long>(a.n_tiles) * a.Hq >= (1LL << 31)) throw std::runtime_error("himuon packed attention: too many tiles for one launch");
+  // (blocks look two turns past the last item, in 32 bits: my_turn)
+  if (static_cast<long long>(a.n_tiles) * a.Hq >= (1LL << 31) - (1 << 16)) throw std::runtime_error("himuon packed attention: too many tiles for one launch");
 }
 inline PackedDev make_dev(const PackedAttnArgs& a) {
   PackedDev p{};

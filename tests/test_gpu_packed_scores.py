@@ -854,3 +854,16 @@ def test_head_gradients_replayed_after_an_eager_pass_on_the_same_graph():
     for got in (eager, captured):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     _clean()
+
+
+def test_packed_attention_refuses_more_items_than_its_turns_count():
+    """Blocks look up to two turns past the last (tile, head) item, whose number has to fit in 32 bits; nothing is launched."""
+    from himuon_b200._ext import ext
+
+    tiles, Hq = 1024, 2 ** 21 - 16
+    assert 2 ** 31 - 2 ** 16 <= tiles * Hq < 2 ** 31
+    plan = torch.zeros(2 * tiles, 4, device="cuda", dtype=torch.int32)
+    q, k = torch.zeros(1, Hq * 8, device="cuda", dtype=torch.bfloat16), torch.zeros(1, 8, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="too many tiles"):
+        ext().packed_attn_fwd(plan, tiles, 1, q, k, k, torch.empty_like(q), None, None, Hq, 1, 0.1)
+    _clean()
