@@ -476,8 +476,10 @@ def _with_kernel_rows(t: torch.Tensor) -> torch.Tensor:
 
 def _with_rows_apart(t: torch.Tensor) -> torch.Tensor:
     # The same for kernels that also want every row to have memory of its own: expanded and overlapping ones are copied.
-    apart = t.shape[0] <= 1 or t.stride(0) >= t.shape[1]
-    return t if apart and _kernel_rows(t) else t.clone(memory_format=torch.contiguous_format)
+    (rows, cols), (ld, inner) = t.shape, t.stride()
+    if inner == 1 and ld % 8 == 0 and (ld >= cols or rows <= 1) and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _transformed(t: torch.Tensor) -> bool:
