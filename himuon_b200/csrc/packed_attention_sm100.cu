@@ -81,8 +81,9 @@ __device__ __forceinline__ FwdRow fwd_row(const PackedDev& p, int i, int t) {
   const FwdItem it = fwd_item(p, i);
   return t ? FwdRow{it.first, it.len, it.index[1], it.head[1], it.n[1], it.slot[1]} : FwdRow{it.first, it.len, it.index[0], it.head[0], it.n[0], it.slot[0]};
 }
-// e^(scaled score - maximum) of 32 scores as bf16, and their sums.  (A part of the exponentials as polynomials on the FMA units only costs:
+// e^(scaled score - maximum) of 32 scores as bf16, and the sums of what was not rounded yet.  (A part of the exponentials as polynomials on the FMA units only costs:
 // 447 us for one document of 8192 tokens without, 448, 465 and 492 with an eighth, three and five eighths.)
+template <bool SUM>
 __device__ __forceinline__ void to_probabilities(const uint32_t (&v)[32], f32x2 scale2, f32x2 m2, f32x2 (&sum)[2], uint32_t (&pk)[16]) {
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
@@ -90,9 +91,26 @@ __device__ __forceinline__ void to_probabilities(const uint32_t (&v)[32], f32x2 
     unpack2(fma2(pack2(v[2 * k], v[2 * k + 1]), scale2, m2), p0, p1);
     p0 = exp2f(p0);                                  // (of a masked score, -inf, 0)
     p1 = exp2f(p1);
-    sum[k & 1] = add2(sum[k & 1], pack2(p0, p1));
+    if (SUM) sum[k & 1] = add2(sum[k & 1], pack2(p0, p1));
     pk[k] = pack_bf16x2(p0, p1);
   }
+}
+// Sums of the rounded ones.  O is divided by these: its weights then add up to 1, and a row with one weight near 1 keeps what delta has beside it.
+// (Divided by the others O is off by up to 2^-8 of that one's V where its weight is relative to an older maximum: gradients of rows with 1e-3 to 1e-2 beside a
+// weight were off by 4 to 6 % in documents of 700 to 2000 tokens, of others by 0.25.)  An addition takes a bf16 as it is: 2 instructions a pair for 3 with
+// shifts and packed sums, 447 us for 455 over five documents of 16384 tokens, 439 with the unrounded sums, which the exponentials hide better.
+__device__ __forceinline__ void add_rounded(const uint32_t (&pk)[16], float (&sum)[4]) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const unsigned short lo = static_cast<unsigned short>(pk[k]), hi = static_cast<unsigned short>(pk[k] >> 16);
+    asm("add.f32.bf16 %0, %1, %0;" : "+f"(sum[(2 * k) & 3]) : "h"(lo));
+    asm("add.f32.bf16 %0, %1, %0;" : "+f"(sum[(2 * k + 1) & 3]) : "h"(hi));
+  }
+}
+__device__ __forceinline__ float total(const f32x2 (&sum)[2]) {
+  float s0, s1;
+  unpack2(add2(sum[0], sum[1]), s0, s1);
+  return s0 + s1;
 }
 __device__ __forceinline__ float largest32(const uint32_t (&v)[32]) {
   float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
@@ -309,7 +327,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const FwdRow next = my_item(my_turn(round + 1));      // (looked up early)
       const int n = it.n, diag0 = it.index * (AT / BKV);
       if (n == 0) { it = next; continue; }
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, l_rounded = 0.f;      // (l only where the log-sum-exps are kept)
       for (int j = 0; j < n; ++j, ++steps) {
         const int b = steps & 1;
         if (!mbar_wait(&bars->s_full[t][b], (steps >> 1) & 1, abort_flag, p.status, 4)) { ok = false; break; }
@@ -343,23 +361,26 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_st16(tO + c * 16, o);
           }
           l *= alpha;
+          l_rounded *= alpha;
         }
         const f32x2 m2 = pack2(-m, -m);
         f32x2 sum[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-        to_probabilities(v[0], scale2, m2, sum, pk[0]);
-        to_probabilities(v[1], scale2, m2, sum, pk[1]);
+        to_probabilities<KEEP>(v[0], scale2, m2, sum, pk[0]);
+        to_probabilities<KEEP>(v[1], scale2, m2, sum, pk[1]);
         tmem_st16(tS, pk[0]);                            // over scores that are in registers
         tmem_st16(tS + 16, pk[1]);
-        float s0, s1;
-        unpack2(add2(sum[0], sum[1]), s0, s1);
-        l += s0 + s1;
+        if (KEEP) l += total(sum);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bars->p_ready[t][b]);
+        float rounded[4] = {0.f, 0.f, 0.f, 0.f};      // (beside the product)
+        add_rounded(pk[0], rounded);
+        add_rounded(pk[1], rounded);
+        l_rounded += (rounded[0] + rounded[1]) + (rounded[2] + rounded[3]);
       }
       if (!ok || !mbar_wait(&bars->acc_done[t], items++ & 1, abort_flag, p.status, 4)) { ok = false; break; }
       tc_fence_after();
-      const float inv = 1.f / l;
+      const float inv = 1.f / l_rounded;
       const int q0 = it.index * AT + (warp & 3) * 32, rows = it.len - q0;
       const bool whole = rows >= 32;                     // uniform over the warp
       tma_store_wait_read<0>();                          // the item before has left the buffer (whichever lane sent it)

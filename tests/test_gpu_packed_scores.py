@@ -867,3 +867,64 @@ def test_packed_attention_refuses_more_items_than_its_turns_count():
     with pytest.raises(RuntimeError, match="too many tiles"):
         ext().packed_attn_fwd(plan, tiles, 1, q, k, k, torch.empty_like(q), None, None, Hq, 1, 0.1)
     _clean()
+
+
+def _certain_bounds(q, k, v, do, lengths, Hq, Hkv, hd, scale):
+    """Results in 64 bits and bounds that hold for rows with one weight near 1 as well.
+
+    With a = 2^-8 (a weight rounded to bf16), a row's weights are p_j (1 + e_j) over their sum, so that O is off by sum p_j e_j (v_j - o)
+    and delta by sum p_j e_j (dP_j - delta), at most a sum |dS|.  Scores are off by the tensor core's fp32 sums, which move p alike.  Beside
+    that delta has O to 2^-16, and fp32 sums of hd terms."""
+    T, G, a = q.shape[0], Hq // Hkv, U
+    step = (hd / 16 + 4) * 2.0 ** -22                            # of a sum of hd products, relative to their absolute values
+    q, k, v, do = (_heads(t, hd) for t in (q, k, v, do))
+    out = {n: torch.zeros(h, T, hd, dtype=torch.float64, device=q.device) for n, h in
+           (("o", Hq), ("dq", Hq), ("dk", Hkv), ("bo", Hq), ("bdq", Hq), ("bdk", Hkv))}
+    largest = torch.zeros(Hq, T, dtype=torch.float64, device=q.device)
+    first = 0
+    for n in lengths:
+        c = slice(first, first + n)
+        first += n
+        if n == 0:
+            continue
+        kk, vv = (t[:, c].repeat_interleave(G, 0) for t in (k, v))
+        qq, g = q[:, c], do[:, c]
+        s = scale * qq @ kk.transpose(1, 2)
+        p = torch.softmax(s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1), -math.inf), -1)
+        o = p @ vv
+        e = 2 * (step * scale * (qq.abs() @ kk.abs().transpose(1, 2)).amax(-1, keepdim=True) + 2.0 ** -22 * (2 + s.abs().amax(-1, keepdim=True)))
+        dp = g @ vv.transpose(1, 2)
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+        size, osize = g.abs() @ vv.abs().transpose(1, 2), (g.abs() * o.abs()).sum(-1, keepdim=True)
+        off = (a + e) * ds.abs().sum(-1, keepdim=True) + (2.0 ** -16 + (hd + 40) * 2.0 ** -23) * osize
+        bds = (2 * a + 2 * e) * ds.abs() + p * (off + step * size)
+        far = torch.stack([(p[h][..., None] * (vv[h][None] - o[h][:, None]).abs()).sum(1) for h in range(Hq)])
+        bo = (a + e) * far + 2.0 ** -20 * (p @ vv.abs())
+        per = {"o": (o, bo), "dq": (scale * ds @ kk, scale * bds @ kk.abs()), "dk": (scale * ds.transpose(1, 2) @ qq, scale * bds.transpose(1, 2) @ qq.abs())}
+        for name, (val, bound) in per.items():
+            if name == "dk":
+                val, bound = (t.view(Hkv, G, n, hd).sum(1) for t in (val, bound))
+            out[name][:, c] = val
+            out["b" + name][:, c] = bound * (1 + 2.0 ** -8) + a * val.abs() * (1 + 2.0 ** -6) + 1e-30
+        largest[:, c] = p.amax(-1)
+    return {n: _flat(t) for n, t in out.items()}, largest
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", SHAPES)
+@pytest.mark.parametrize("lengths", [[2] * 60 + [1, 64, 65], [300, 129], [700]])
+def test_gradients_of_nearly_certain_rows_of_any_head_and_length(Hq, Hkv, hd, lengths):
+    """Scores that spread by 6, so that many rows have one weight near 1, of a key that the running maximum may have met late."""
+    ops = _ops()
+    torch.manual_seed(71 + hd)
+    T, scale = sum(lengths), 6 / math.sqrt(hd)
+    q, k, v = (torch.randn(T, h * hd, device="cuda").bfloat16().requires_grad_() for h in (Hq, Hkv, Hkv))
+    do = torch.randn(T, Hq * hd, device="cuda").bfloat16()
+    o = ops.packed_attention(q, k, v, ops.PackedLayout(lengths), Hq, Hkv, hd, scale=scale)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    want, largest = _certain_bounds(q, k, v, do, lengths, Hq, Hkv, hd, scale)
+    assert ((largest < 1) & (largest > 0.99)).sum() > 20
+    for name, got in zip(("o", "dq", "dk"), (o, *grads)):
+        _within(got, want[name], want["b" + name], name)
+    with torch.no_grad():
+        _within(ops.packed_attention(q, k, v, ops.PackedLayout(lengths), Hq, Hkv, hd, scale=scale), want["o"], want["bo"], "o without a graph")
+    _clean()
