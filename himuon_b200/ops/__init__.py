@@ -52,12 +52,6 @@ def _warn_torch_path(op: str, why: str) -> None:
                       stacklevel=3)
 
 
-def _once(op: str) -> None:
-    """Called by a backward pass that kernels compute: what they return has no graph of its own."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"himuon_b200.ops.{op}: its gradient cannot be differentiated again (create_graph=True)")
-
-
 def check_status() -> None:
     """Raise if any kernel's bounded wait ran out since the last check (synchronises)."""
     code = _ext.ext().status(True)
