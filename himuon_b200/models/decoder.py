@@ -232,7 +232,8 @@ class CausalLM(nn.Module):
     def score(self, input_ids, layout: ops.PackedLayout) -> ops.TokenLogProbs:
         """Scores the tokens of a packed batch (see ``forward``) under the model: for each row, in the order of
         ``input_ids.reshape(-1)``, the log probability of the token that follows it in its document (0 where none does) and the entropy
-        of what was predicted there.  Differentiable in both; logits are never kept."""
+        of what was predicted there.  Differentiable in both.  Logits never exist as a whole; for a gradient two bytes for each may be kept
+        until the backward pass (:func:`ops.linear_token_log_probs`)."""
         h = self.hidden_states(input_ids, layout)
         return ops.linear_token_log_probs(h, self._head_weight()[0], layout.next_ids(input_ids))
 

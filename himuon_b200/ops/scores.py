@@ -1,8 +1,9 @@
 """Log probabilities of given tokens, with the entropy of their distribution and the likeliest alternatives.
 
-:func:`token_log_probs` takes logits, :func:`linear_token_log_probs` hidden states and the head's weight, whose logits it never
-keeps.  Both are differentiable in the log probabilities and the entropy (policy gradients, entropy bonuses, distillation); under vmap
-and forward-mode differentiation, for which the kernels have no rules, the PyTorch formulation runs.
+:func:`token_log_probs` takes logits, :func:`linear_token_log_probs` hidden states and the head's weight, whose logits never exist as
+a whole; for a gradient it may keep two bytes for each.  Both are differentiable in the log probabilities and the entropy (policy
+gradients, entropy bonuses, distillation); under vmap and forward-mode differentiation, for which the kernels have no rules, the
+PyTorch formulation runs.
 """
 
 from __future__ import annotations
@@ -66,7 +67,7 @@ def linear_token_log_probs(h2d: torch.Tensor, w: torch.Tensor, ids: torch.Tensor
     hidden)`` head, without alternatives.  bf16 CUDA tensors whose hidden size is a multiple of 8 run the sm_100a kernels.
 
     Where a gradient is asked for, more than 64 rows keep two bytes for each logit until the backward pass, which needs them for the
-    logits' gradient anyway, as long as that is no more than 4 GiB; beyond, it makes the logits again, some thousand rows at a time.  A backward pass that
+    logits' gradient anyway, as long as that is no more than 4 GiB; a checkpoint around the call drops them.  Beyond, the backward pass makes the logits again, some thousand rows at a time.  A backward pass that
     a graph captures leaves what was kept as it is and takes as much again, because it may be replayed more than once."""
     if h2d.dim() != 2 or w.dim() != 2 or h2d.shape[1] != w.shape[1] or w.shape[0] == 0 or h2d.dtype != w.dtype or h2d.device != w.device:
         raise RuntimeError("himuon_b200.ops.linear_token_log_probs: (rows, hidden) and (vocab, hidden) of one type on one device expected")

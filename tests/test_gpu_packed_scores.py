@@ -928,3 +928,65 @@ def test_gradients_of_nearly_certain_rows_of_any_head_and_length(Hq, Hkv, hd, le
     with torch.no_grad():
         _within(ops.packed_attention(q, k, v, ops.PackedLayout(lengths), Hq, Hkv, hd, scale=scale), want["o"], want["bo"], "o without a graph")
     _clean()
+
+
+@pytest.mark.parametrize("lengths,rows", [([], 0), ([0, 0], 0), ([], 5), ([0], 5)])
+def test_a_batch_without_tokens_on_the_gpu(lengths, rows):
+    ops = _ops()
+    q, k, v = (torch.randn(rows, n * 64, device="cuda").bfloat16().requires_grad_() for n in (4, 2, 2))
+    layout = ops.PackedLayout(lengths)
+    o = ops.packed_attention(q, k, v, layout, 4, 2, 64)
+    grads = torch.autograd.grad(o, (q, k, v), torch.ones_like(o))
+    assert o.shape == q.shape and not o.any()
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, (q, k, v)))
+    with torch.no_grad():
+        assert not ops.packed_attention(q, k, v, layout, 4, 2, 64).any()
+    h, w, ids = torch.randn(0, 64, device="cuda").bfloat16().requires_grad_(), torch.randn(9, 64, device="cuda").bfloat16().requires_grad_(), torch.zeros(0, dtype=torch.int64, device="cuda")
+    x = torch.randn(0, 9, device="cuda", requires_grad=True)
+    dh, dw = torch.autograd.grad(ops.linear_token_log_probs(h, w, ids).log_probs.sum(), (h, w))
+    dx, = torch.autograd.grad(ops.token_log_probs(x, ids, top_k=2).entropy.sum(), x)
+    assert dh.shape == (0, 64) and dw.shape == (9, 64) and not dw.any() and dx.shape == (0, 9)
+    _clean()
+
+
+def test_token_log_probs_fp32_gradient_over_several_blocks_from_strided_gradients():
+    ops = _ops()
+    torch.manual_seed(73)
+    rows, vocab = 5, 40001
+    x = (3 * torch.randn(rows, vocab + 3, device="cuda"))[:, 3:].requires_grad_()
+    ids = torch.tensor([0, 40000, -100, 4096, 16383], device="cuda")
+    both = torch.randn(rows, 2, device="cuda")
+    s = ops.token_log_probs(x, ids)
+    dx, = torch.autograd.grad((s.log_probs, s.entropy), x, (both[:, 0], both[:, 1]))
+    lp, _, entropy = _scores64(x.detach(), ids)
+    want, size = _grad64(lp, entropy, ids, both[:, 0], both[:, 1])
+    tol = _log_tolerance(vocab)
+    _within(dx, want, 2.0 ** -22 * want.abs() + (4 * tol * (1 + entropy[:, None]) + 2.0 ** -18) * size + 1e-30, "gradient")
+    _clean()
+
+
+def test_two_threads_on_one_retained_graph():
+    """Each gets a gradient that a single caller gets: from what was kept, or from the logits again."""
+    import threading
+
+    ops = _ops()
+    torch.manual_seed(75)
+    h, w = torch.randn(300, 128, device="cuda").bfloat16().requires_grad_(), torch.randn(2000, 128, device="cuda").bfloat16().requires_grad_()
+    ids, g = torch.randint(0, 2000, (300,), device="cuda"), torch.randn(300, device="cuda")
+
+    def call():
+        return ops.linear_token_log_probs(h, w, ids).log_probs
+
+    out = call()
+    one_by_one = [torch.autograd.grad(out, (h, w), g, retain_graph=True) for _ in range(2)]
+    for _ in range(10):
+        out, got = call(), []
+        threads = [threading.Thread(target=lambda: got.append(torch.autograd.grad(out, (h, w), g, retain_graph=True))) for _ in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        kinds = sorted(next(i for i, want in enumerate(one_by_one) if all(torch.equal(a, b) for a, b in zip(x, want))) for x in got)
+        assert kinds == [0, 1]
+    _clean()
