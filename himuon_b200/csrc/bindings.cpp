@@ -642,10 +642,14 @@ static variable_list linear_score_outputs(const at::Tensor& h, const at::Tensor&
   const auto fp32 = h.options().dtype(at::kFloat);
   variable_list out = {at::empty({rows}, fp32), at::empty({rows}, fp32)};
   if (!rows) return out;
-  const int vocab = static_cast<int>(w.size(0));       // (a last launch of a few rows may need more than the others: its kernel has more parts)
-  at::Tensor scratch = at::empty({std::max(himuon::linear_scores_scratch(std::min(rows, launch_rows), vocab), himuon::linear_scores_scratch(rows % launch_rows, vocab))}, fp32);
-  for (int64_t r = 0; r < rows; r += launch_rows) {
-    const int64_t n = std::min(rows - r, launch_rows);
+  // a rest that the kernel for a few rows would take goes along with the launch before: its order of sums is another, and no result may depend
+  // on the launch that a row is in
+  auto of_launch = [&](int64_t r) { return rows - r <= launch_rows + himuon::kFewRows ? rows - r : launch_rows; };
+  const int64_t rest = rows % launch_rows, most = std::max(of_launch(0), rows > launch_rows && rest <= himuon::kFewRows ? launch_rows + rest : 0);
+  at::Tensor scratch = at::empty({himuon::linear_scores_scratch(most, static_cast<int>(w.size(0)))}, fp32);
+  int64_t n;
+  for (int64_t r = 0; r < rows; r += n) {
+    n = of_launch(r);
     auto chunk = [&](const at::Tensor& t) { return n == rows ? t : t.narrow(0, r, n); };
     auto maybe = [&](const c10::optional<at::Tensor>& t) { return t.has_value() ? c10::optional<at::Tensor>(chunk(*t)) : c10::nullopt; };
     at::Tensor log_probs = chunk(out[0]), entropy = chunk(out[1]);
@@ -666,7 +670,7 @@ struct LinearScores : torch::autograd::Function<LinearScores> {
     const auto fp32 = h.options().dtype(at::kFloat);
     const at::Tensor stats = at::empty({rows, 2}, fp32);
     c10::optional<at::Tensor> kept, slab_max;
-    if (rows > 64 && rows * cols <= gradient_values) {
+    if (rows > himuon::kFewRows && rows * cols <= gradient_values) {
       kept = at::empty({rows, cols}, h.options());
       slab_max = at::empty({rows, (vocab + 63) / 64}, fp32);
     }

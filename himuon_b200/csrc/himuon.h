@@ -213,6 +213,7 @@ struct LinearScoreArgs {
   const void* kept;                          // gradient only: exponentials that are to stay as they are, laid out as grad
   float* slab_max;                           // (rows, vocabulary / 64 rounded up) maxima that kept exponentials are relative to
 };
+constexpr int kFewRows = 64;               // up to so many rows have a forward kernel of their own, which keeps nothing
 long long linear_scores_scratch(long long rows, int vocab);
 void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s);
 void linear_scores_dlogits(const LinearScoreArgs& a, cudaStream_t s);

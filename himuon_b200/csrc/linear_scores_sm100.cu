@@ -281,7 +281,6 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
 // there).  A block streams one share of the vocabulary in tiles of `th` entries; a thread keeps the sums of its lane for
 // up to 32 rows, and only at the end the 128 lanes meet.  8 rows over 151936 x 1024: 50 us (6.2 TB/s), pair kernel 99.
 constexpr int FEW_STAGES = 9;
-constexpr int FEW_ROWS = 64;
 constexpr int few_threads(int nb) { return 64 + 128 * (nb > 32 ? nb / 32 : 1); }      // warp 0: TMA, 1: MMA, then four for each 32 rows
 struct FewBars {
   uint64_t full[FEW_STAGES], empty[FEW_STAGES], tfull[2], tempty[2];
@@ -627,7 +626,7 @@ static LinScoresDev make_dev(const LinearScoreArgs& a) {
 
 // Room for the parts of the forward kernel that takes so many rows, one for each 64 entries (launch_few) or 128, and the rows' own logits.
 long long linear_scores_scratch(long long rows, int vocab) {
-  const int per = rows <= FEW_ROWS ? 128 : LS_N;
+  const int per = rows <= kFewRows ? 128 : LS_N;
   return rows * (1 + 3LL * 2 * ((vocab + per - 1) / per));
 }
 
@@ -639,7 +638,7 @@ void linear_scores_fwd(const LinearScoreArgs& a, cudaStream_t s) {
     p.slabs = (a.vocab + 63) / 64;
     launch<STATS_KEPT>(a, p, s);
     n_parts = 2 * p.tiles_n;
-  } else if (a.rows <= FEW_ROWS) {
+  } else if (a.rows <= kFewRows) {
     n_parts = a.rows <= 16 ? launch_few<16>(a, p, s) : a.rows <= 32 ? launch_few<32>(a, p, s) : launch_few<64>(a, p, s);
   } else {
     launch<STATS>(a, p, s);

@@ -990,3 +990,20 @@ def test_two_threads_on_one_retained_graph():
         kinds = sorted(next(i for i, want in enumerate(one_by_one) if all(torch.equal(a, b) for a, b in zip(x, want))) for x in got)
         assert kinds == [0, 1]
     _clean()
+
+
+@pytest.mark.parametrize("rows", [301, 364, 365, 640, 664])
+def test_a_row_of_the_head_does_not_depend_on_its_launch(monkeypatch, rows):
+    """Launches of 300 rows and one, with a gradient and without: the same bits, also where a few rows are left for the last launch."""
+    ops = _ops()
+    from himuon_b200.ops import scores
+
+    torch.manual_seed(77)
+    h, w = torch.randn(rows, 128, device="cuda").bfloat16(), (torch.randn(3000, 128, device="cuda") * 0.2).bfloat16()
+    ids = torch.randint(0, 3000, (rows,), device="cuda")
+    want = ops.linear_token_log_probs(h, w, ids)
+    monkeypatch.setattr(scores, "LAUNCH_ROWS", 300)
+    for t in (h, h.clone().requires_grad_()):
+        got = ops.linear_token_log_probs(t, w, ids)
+        assert torch.equal(got.log_probs, want.log_probs) and torch.equal(got.entropy, want.entropy)
+    _clean()
