@@ -32,6 +32,12 @@ constexpr int LS_STAGES = 6;
 constexpr int LS_N = 256;
 constexpr uint32_t LS_A = BM * BK * 2, LS_STAGE = 2 * LS_A;      // 128 rows of h and 128 of W, a CTA
 
+// The tensor core cuts its fp32 sums off toward 0, 16 elements at a time, so that a logit comes out too small by about so much of itself for each element of the
+// hidden size.  Measured, slope of the accumulators against 64 bits: 7.4e-10 to 9.6e-10 at hidden sizes of 64 to 8192 (normal operands, also with a part in
+// common), 1.0e-9 to 1.4e-9 with heavy tails, 1.2e-9 to 3.9e-9 where all products are positive.  What all of them share is put back; the rest of the error has no sign.
+// At 2560 the entropy was off by 1.0e-6 of itself without.
+constexpr float kShrink = 7.5e-10f;
+
 enum { STATS, GRAD, STATS_KEPT };    // what the epilogue makes of the logits; STATS_KEPT: sums, and the exponentials
 
 struct LinScoresDev {
@@ -45,6 +51,7 @@ struct LinScoresDev {
   const float* g_log_probs;
   const float* g_entropy;
   long long ignore;
+  float regrow;                      // accumulator to logit (kShrink)
   int rows, vocab, tiles_m, tiles_n, kblocks;
   int* status;
 };
@@ -181,6 +188,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
     const int ew = warp & 3, group = (warp - 4) >> 2;
     const uint32_t tempty_lead = map_to_cta(smem_u32(tempty), 0);
     const bool issuer = ew == 0 && lane == 0;
+    const f32x2 regrow = pack2(p.regrow, p.regrow);
     uint8_t* slab = slabs + group * SLAB_BYTES;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -215,7 +223,7 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
               tmem_ld32(t_acc + c + half * 32, v);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[half * 32 + j] = __uint_as_float(v[j]);
+              for (int j = 0; j < 32; j += 2) unpack2(mul2(pack2(v[j], v[j + 1]), regrow), x[half * 32 + j], x[half * 32 + j + 1]);
             }
             if (col + 64 > p.vocab) {
 #pragma unroll
@@ -238,8 +246,11 @@ linear_scores_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_const
             tmem_ld32(t_acc + c + half * 32, v);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 2)
-              o[half * 16 + j / 2] = pack_bf16x2(grad_of(rg, __uint_as_float(v[j]), col + half * 32 + j), grad_of(rg, __uint_as_float(v[j + 1]), col + half * 32 + j + 1));
+            for (int j = 0; j < 32; j += 2) {
+              float x0, x1;
+              unpack2(mul2(pack2(v[j], v[j + 1]), regrow), x0, x1);
+              o[half * 16 + j / 2] = pack_bf16x2(grad_of(rg, x0, col + half * 32 + j), grad_of(rg, x1, col + half * 32 + j + 1));
+            }
           }
           }
           if constexpr (MODE == STATS) continue;
@@ -393,7 +404,7 @@ linear_scores_few_kernel(const __grid_constant__ CUtensorMap tmH, const __grid_c
         if (mine) {
 #pragma unroll
           for (int n = 0; n < 16; ++n) {
-            const float y = __uint_as_float(x[n]);
+            const float y = __uint_as_float(x[n]) * p.regrow;
             Sums& b = a[c + n];
             const float m = fmaxf(b.m, y), from = fmaxf(b.m - m, kFar), f = exp2f(from * kLog2eS);
             const float d = y - (m == -INFINITY ? 0.f : m), e = exp2f(d * kLog2eS);
@@ -616,6 +627,7 @@ static LinScoresDev make_dev(const LinearScoreArgs& a) {
   LinScoresDev p{};
   p.ids = a.ids; p.ignore = a.ignore;
   p.rows = a.rows; p.vocab = a.vocab;
+  p.regrow = 1.f + kShrink * static_cast<float>(a.hidden);
   p.part = a.scratch + a.rows; p.target = a.scratch;
   p.stats = reinterpret_cast<const float2*>(a.stats);
   p.entropy = a.entropy;
