@@ -45,12 +45,14 @@ def token_log_probs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ign
     """
     if logits.dim() != 2 or logits.shape[1] == 0 or not logits.is_floating_point():
         raise RuntimeError("himuon_b200.ops.token_log_probs: logits must be a (rows, vocab) matrix of floating point")
-    if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[1]):
-        raise RuntimeError(f"himuon_b200.ops.token_log_probs: top_k must lie in 0..{min(MAX_TOP_K, logits.shape[1])}, got {top_k}")
-    ids = _check_ids("token_log_probs", ids, logits.shape[0], logits.device)
+    rows, vocab = logits.shape
+    if not 0 <= top_k <= min(MAX_TOP_K, vocab):
+        raise RuntimeError(f"himuon_b200.ops.token_log_probs: top_k must lie in 0..{min(MAX_TOP_K, vocab)}, got {top_k}")
+    ids = _check_ids("token_log_probs", ids, rows, logits.device)
     transformed = _any_transformed(logits, ids)
     if logits.is_cuda and logits.dtype in (torch.bfloat16, torch.float32) and not transformed:
-        if logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        ld, inner = logits.stride()
+        if inner != 1 or (rows > 1 and ld < vocab):
             logits = logits.clone(memory_format=torch.contiguous_format)      # (one column is contiguous at any stride)
         return TokenLogProbs(*_ext.ext().token_scores(logits, ids, int(top_k), int(ignore_index)))
     if logits.is_cuda and transformed:
