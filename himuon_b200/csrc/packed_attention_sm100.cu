@@ -26,14 +26,14 @@ namespace {
 // that they find scores when they are done.  Probabilities are taken relative to an older maximum of the row, and only where it has grown
 // by more than 2^8 (in base-2 units) is O rescaled.  The block's loads run ahead of its products across items; O leaves by TMA.
 //
-// Measured, one document of 8192 tokens, 32 heads over 8 of 128: 433 us, 1270 TFLOP/s (one tile a block, two blocks per SM, 580; blocks of 128
-// keys with one S a tile, where scores, probabilities, P V and the next scores follow one another, 501).  A step of 64 keys takes 1650
-// cycles.  Its products alone take 1239 (products of 128 x 64 x 16 with both operands in shared memory 48, those of P V 64 each), and
+// Measured, one document of 8192 tokens, 32 heads over 8 of 128: 440 us, 1250 TFLOP/s (one tile a block, two blocks per SM, 580; blocks of 128
+// keys with one S a tile, where scores, probabilities, P V and the next scores follow one another, 501).  A step of 64 keys took 1650
+// cycles without the sums of rounded weights (435 us).  Its products alone take 1239 (products of 128 x 64 x 16 with both operands in shared memory 48, those of P V 64 each), and
 // shared memory is busy for 1280 of them: the operands, and 32 KB of new K and V.  What the issuing warp does beside issuing counts in full,
 // because an MMA is issued about when it starts (the tensor core keeps two more): with a general step, ring positions found by division and
-// item fields that are not uniform the same step took 2200.  24 documents of 341 tokens in the mean, 16 heads over 8: 55 us, where an item has
-// some nine steps and 4300 cycles for its first scores, its last product and its epilogue.  What a backward pass needs (KEEP) costs 3 us there, 10 at the
-// one document.
+// item fields that are not uniform the same step took 2200.  24 documents of 341 tokens in the mean, 16 heads over 8: 57 us, where an item has
+// some nine steps and 4300 cycles for its first scores, its last product and its epilogue.  What a backward pass needs (KEEP) costs 3 us there, 22 at the
+// one document (in a training step; 60 where this kernel alone runs, at the power limit).
 constexpr int FWD_THREADS = 320;                     // warps 0-3 and 4-7: rows of the tiles, 8: TMA, 9: MMA
 constexpr int BKV = 64;                              // key positions per block
 constexpr uint32_t KV_HALF = BKV * 128;              // one 64-column half of a K or V block: 8 KB
