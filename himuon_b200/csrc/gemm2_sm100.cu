@@ -334,14 +334,14 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
                            total * p.kblocks >= 8LL * cap;
   // (Few tiles with ordered sums, which have no stream-K: all of them are the last wave.)
   if (!want_stream && a.parts != nullptr && (total > cap / 2 || a.ordered) && rem > 0 && rem * 2 <= cap && p.kblocks >= 16) {
-    int sl = cap / rem;
+    int sl = (cap < num_sms() / 2 ? cap : num_sms() / 2) / rem;      // (as many tiles as gemm_parts_floats() counts)
     if (sl > p.kblocks / 8) sl = p.kblocks / 8;
     // worth it only when the K-blocks saved outweigh the fp32 reduction traffic and the second launch (~12 us)
     if (sl >= 2 && (sl - 1) * p.kblocks / sl >= 40) {
       p.nslices = sl;
       p.full_items = static_cast<int>(total) - rem;
       p.total_items = p.full_items + rem * sl;
-      const uint64_t rows = static_cast<uint64_t>(rem) * sl * 256;      // (rem * sl <= cap tiles)
+      const uint64_t rows = static_cast<uint64_t>(rem) * sl * 256;
       const uint64_t dimsW[3] = {256, rows, 1};
       const uint64_t strW[2] = {256 * sizeof(float), rows * 256 * sizeof(float)};
       const uint32_t boxW[3] = {32, BM, 1};

@@ -34,7 +34,7 @@ constexpr uint32_t LS_A = BM * BK * 2, LS_STAGE = 2 * LS_A;      // 128 rows of 
 
 // The tensor core cuts its fp32 sums off toward 0, 16 elements at a time, so that a logit comes out too small by about so much of itself for each element of the
 // hidden size.  Measured, slope of the accumulators against 64 bits: 7.4e-10 to 9.6e-10 at hidden sizes of 64 to 8192 (normal operands, also with a part in
-// common), 1.0e-9 to 1.4e-9 with heavy tails, 1.2e-9 to 3.9e-9 where all products are positive.  What all of them share is put back; the rest of the error has no sign.
+// common), 1.0e-9 to 1.4e-9 with heavy tails, 1.2e-9 to 3.9e-9 where all products are positive.  What all of them share is put back.
 // At 2560 the entropy was off by 1.0e-6 of itself without.
 constexpr float kShrink = 7.5e-10f;
 
