@@ -20,12 +20,13 @@ CUDA_SOURCES = [
     "attention_sm100.cu",
     "attention_kv64_sm100.cu", "attention_bwd_sm100.cu",
     "packed_attention_sm100.cu", "packed_attention_bwd_sm100.cu", "token_scores.cu", "linear_scores_sm100.cu",
+    "rotary_kernels.cu", "gated_mlp_sm100.cu", "fp8_quantize.cu", "fp8_sm100.cu", "few_rows_sm100.cu",
     "ns5_sm100.cu", "ns_pair_sm100.cu",
     "comm_kernels.cu",
     "soap_kernels.cu",
     "rmsnorm_bwd_noalloc.cu",
 ]
-CPP_SOURCES = ["bindings.cpp", "symm.cpp", "vmm.cpp"]
+CPP_SOURCES = ["bindings.cpp", "layer_ops.cpp", "symm.cpp", "vmm.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "bindings.h"
 #include "himuon.h"
 #include "symm.h"
 
@@ -76,6 +77,9 @@ static void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, cons
     g.parts = parts.data_ptr<float>();
   }
   himuon::gemm_bf16(g, cur_stream());
+}
+void gemm_into(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool trans_a, bool trans_b) {
+  gemm(a, b, out, c10::nullopt, trans_a, trans_b, 1.0, 0.0, false, 0, false);
 }
 // Whether gemm() with these arguments runs on CTA pairs.
 static bool gemm_on_pairs(const at::Tensor& a, const at::Tensor& b, const at::Tensor& out, const c10::optional<at::Tensor>& aux,
@@ -368,7 +372,7 @@ static void packed_attn_bwd(const at::Tensor& plan, int64_t tiles, int64_t token
 // 119 us of host time as a Python function, 88 here, of which a function that does nothing takes 63 and 40.)
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-static std::atomic<int64_t> autograd_launched{0};       // kernels launched by them
+std::atomic<int64_t> autograd_launched{0};       // kernels launched by them
 
 static void check_once(const char* op) {
   TORCH_CHECK(!c10::GradMode::is_enabled(), "himuon_b200.ops.", op, ": its gradient cannot be differentiated again (create_graph=True)");
@@ -855,4 +859,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return std::vector<int64_t>{(int64_t)sizeof(himuon::MomTileEntry), (int64_t)sizeof(himuon::ApplyEntry), (int64_t)sizeof(himuon::AdamEntry)};
   });
   himuon::bind_symm(m);
+  bind_layer_ops(m);
 }

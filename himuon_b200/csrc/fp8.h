@@ -1,0 +1,37 @@
+// Host-side interface of the 8-bit kernels (fp8_quantize.cu, fp8_sm100.cu, few_rows_sm100.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+
+namespace himuon {
+
+// One 8-bit copy of a matrix: e4m3 values with rows of `ld` bytes, and the scales of blocks of (block_rows, 128).
+struct Fp8Out {
+  void* values = nullptr;          // null: this copy is not wanted
+  float* scales = nullptr;
+  long long ld = 0, scale_row = 0, scale_col = 0;      // strides between the scales of neighbouring blocks
+  int block_rows = 1;              // 1 or 128
+};
+// `rows` x `cols` values of bf16 or fp32 as they lie, and turned around.
+struct Fp8QuantizeArgs {
+  const void* x = nullptr;
+  long long rows = 0, cols = 0, ld = 0;
+  int fp32 = 0;
+  Fp8Out straight, turned;
+};
+void fp8_quantize(const Fp8QuantizeArgs& a, cudaStream_t s);
+
+struct Fp8Matrix {
+  const void* values = nullptr;
+  const float* scales = nullptr;
+  long long ld = 0, scale_row = 0, scale_col = 0;
+  int rows = 0, cols = 0, block_rows = 1;
+};
+void fp8_dequantize(const Fp8Matrix& m, void* out, long long ld_out, int out_fp32, cudaStream_t s);
+
+// c = a b^T, bf16 or fp32.  a has blocks of 1 or 128 rows, b of 128.  Rows of c are multiples of 16 bytes apart and written in whole groups of 16.
+void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c, int out_fp32, cudaStream_t s);
+// The same for up to kFewProductRows rows of a (gated_mlp.h) and an inner dimension of multiples of 16; c is contiguous.
+void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, cudaStream_t s);
+
+}  // namespace himuon

@@ -1,0 +1,390 @@
+// The gated feed-forward block  y = (act(x Wg^T) * (x Wu^T)) Wd^T  on CTA pairs: its two products with an activation in between.
+//
+//   UP:         g = x Wg^T and u = x Wu^T for the same 256 rows and 128 features meet in one accumulator (one CTA of the pair stages rows of
+//               Wg, the other of Wu), whose epilogue writes h = act(g) * u; g and u only where a gradient will want them, 24 bits of each.
+//   DOWN_GRAD:  dh = dy Wd, from whose fp32 accumulator the epilogue writes dg = dh u act'(g) and du = dh act(g), operands of the products
+//               that follow, in bf16.  dh itself is never written.
+//
+// h, dg and du are rounded to bf16: they are the operands of the next products, and each is off by at most 2^-8 of itself, as the results are.
+// Everything between two products is fp32.
+//
+// The main loop is the pair GEMM's (gemm2_sm100.cu has its protocol): six stages of 64 along the inner dimension, two accumulators of 256
+// columns, so that one tile's epilogue runs beside the products of the next.
+#include "activations.cuh"
+#include "gated_mlp.h"
+#include "gemm_epilogue.cuh"
+#include "himuon.h"
+#include "pair_common.cuh"
+#include "sm100_common.cuh"
+#include "tma_host.h"
+
+#include <atomic>
+
+namespace himuon {
+
+namespace {
+
+constexpr int GM_THREADS = 384;      // warps 0-3: TMA, MMA, TMEM allocation, none; 4-11: epilogue, two groups of four
+constexpr int GM_STAGES = 6;
+// Registers of a thread at launch, and after the first four warps have given some to the others.
+constexpr int GM_REGS = 168, GM_REGS_FEW = 104, GM_REGS_EPILOGUE = 200;
+static_assert(GM_REGS_FEW + 2 * GM_REGS_EPILOGUE <= 3 * GM_REGS, "more registers than the block was launched with");
+constexpr uint32_t GM_A = BM * BK * 2, GM_STAGE = 2 * GM_A;      // 128 rows of each operand, a CTA
+
+enum { UP, DOWN_GRAD };
+
+struct GatedDev {
+  const uint16_t* gu;                  // DOWN_GRAD: g | u, upper bits
+  uint8_t* gu_low;                     // the bits below; UP: null where g and u are not wanted
+  int rows, inter, low, tiles_m, tiles_n, kblocks;
+  int* status;
+};
+
+// A slab of 128 rows by 64 columns on its way to global memory by TMA: the 128 threads of a group, one row each.
+__device__ __forceinline__ void slab_free(int group, bool issuer) {
+  if (issuer) tma_store_wait_read<0>();
+  named_barrier(1 + 2 * group, 128);
+}
+// Columns 16 q to 16 q + 15 of a thread's row.
+__device__ __forceinline__ void put16(uint8_t* slab, int row, int q, const uint32_t (&o)[8]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    *reinterpret_cast<uint4*>(slab + row * 128 + (((2 * q + j) ^ (row & 7)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+}
+__device__ __forceinline__ void slab_store(const CUtensorMap* tm, const uint8_t* slab, int group, int col, int row0, bool issuer) {
+  fence_proxy_async_smem();
+  named_barrier(2 + 2 * group, 128);                  // the slab is complete
+  if (issuer) {
+    tma_store_3d(tm, slab, col, row0, 0);
+    tma_store_commit();
+  }
+}
+__device__ __forceinline__ void load16(const uint16_t* p, int valid, uint4 (&v)[2]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) v[j] = 8 * j < valid ? reinterpret_cast<const uint4*>(p)[j] : make_uint4(0, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// Two kept values from a word of upper bits and the word that has their lower ones (in its first or second half).
+__device__ __forceinline__ void from_kept(uint32_t upper, uint32_t low, int half, float& a, float& b) {
+  a = __uint_as_float(__byte_perm(upper, low, half ? 0x1062 : 0x1040) & 0xFFFFFF00u);
+  b = __uint_as_float(__byte_perm(upper, low, half ? 0x3272 : 0x3252) & 0xFFFFFF00u);
+}
+
+}  // namespace
+
+// tmA: rows of x or dy.  UP: tmB0 and tmB1 rows of Wg and Wu along the inner dimension, tmO h, tmG and tmU the halves of g | u.
+// DOWN_GRAD: tmB0 = tmB1 = Wd, its features along its rows; tmG and tmU the halves of dg | du.  (Halves have a map each: what a box has behind
+// the last feature of one must not go to the first of the other.)
+template <int MODE, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GM_THREADS, 1)
+gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                 const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmU, GatedDev p) {
+  constexpr int FEATURES = MODE == UP ? 128 : 256;    // of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_up_1024(smem_raw);
+  uint8_t* slabs = smem + GM_STAGES * GM_STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(slabs + 2 * SLAB_BYTES);
+  uint64_t* empty = full + GM_STAGES;
+  uint64_t* tfull = empty + GM_STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = warp_id(), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < GM_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 16); }     // eight epilogue warps in each CTA
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 2) tmem_alloc2(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                // the peer's barriers exist before anything signals them
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, total = p.tiles_m * p.tiles_n;
+
+  if (warp < 4) {
+  registers_down<GM_REGS_FEW>();
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    const uint32_t e = elect_one();
+    const CUtensorMap* tmB = rank == 0 ? &tmB0 : &tmB1;
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(tmB);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < total; tile += n_pairs) {
+      const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
+      const int n0 = MODE == UP ? nt * 128 : nt * 256 + static_cast<int>(rank) * 128;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
+        uint8_t* sA = smem + stage * GM_STAGE;
+        mbar_expect_tx(&full[stage], 2 * GM_STAGE, leader ? e : 0);
+        tma2_load_3d(sA, &tmA, &full[stage], kb * BK, m0, 0, e);
+        if (MODE == UP) {
+          tma2_load_3d(sA + GM_A, tmB, &full[stage], kb * BK, n0, 0, e);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) tma2_load_3d(sA + GM_A + j * BK * 128, tmB, &full[stage], n0 + j * 64, kb * BK, 0, e);
+        }
+        if (++stage == GM_STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader CTA only)
+    if (leader) {
+      const uint32_t e = elect_one();
+      constexpr uint32_t idesc = umma_idesc_bf16(2 * BM, 256, false, MODE == DOWN_GRAD);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < total; tile += n_pairs) {
+        if (!mbar_wait_warp(&tempty[acc], acc_phase ^ 1, abort_flag, p.status, 2)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * 256);
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (!mbar_wait_warp(&full[stage], phase, abort_flag, p.status, 2)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_base = smem_u32(smem + stage * GM_STAGE);
+          const uint64_t a_desc = umma_smem_desc(a_base, 16, 1024);
+          const uint64_t b_desc = umma_smem_desc(a_base + GM_A, MODE == DOWN_GRAD ? BK * 128 : 16, 1024);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma2_ss(d_tmem, desc_at(a_desc, k * 32), desc_at(b_desc, k * (MODE == DOWN_GRAD ? 2048 : 32)), idesc, (kb > 0 || k > 0) ? 1u : 0u, e);
+          const uint32_t e_addr = smem_u32(&empty[stage]);
+          umma2_commit(e_addr, e);                  // this CTA's producer
+          umma2_commit(map_to_cta(e_addr, 1), e);   // the peer's producer
+          if (++stage == GM_STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        const uint32_t f_addr = smem_u32(&tfull[acc]);
+        umma2_commit(f_addr, e);
+        umma2_commit(map_to_cta(f_addr, 1), e);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+    }
+  }
+  } else {
+    registers_up<GM_REGS_EPILOGUE>();
+    // ------------------------------------------------------------ epilogue (both CTAs, own 128 accumulator rows, one a thread)
+    const int ew = warp & 3, group = (warp - 4) >> 2, row_in_tile = ew * 32 + lane;
+    const uint32_t tempty_lead = map_to_cta(smem_u32(tempty), 0);
+    const bool issuer = ew == 0 && lane == 0;
+    uint8_t* slab = slabs + group * SLAB_BYTES;
+    if (issuer) tma_prefetch_desc(MODE == UP ? &tmO : &tmG);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int tile = first; tile < total; tile += n_pairs) {
+      const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
+      const int n0 = nt * FEATURES;
+      // the 128 threads of a group meet on named barriers below, so they also leave together when the wait runs out
+      if (!named_barrier_and(1 + 2 * group, 128, mbar_wait(&tfull[acc], acc_phase, abort_flag, p.status, 3))) break;
+      tc_fence_after();
+      const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(acc * 256);
+      if (m0 < p.rows) {                            // uniform: the second CTA of a ragged last row block has nothing to store
+        if constexpr (MODE == UP) {
+          const int col = n0 + group * 64;
+          if (col < p.inter) {
+            // (values go to the slab as they come: 64 of them at once are more registers than there are)
+            const uint32_t t_slab = t_acc + group * 64;
+            slab_free(group, issuer);
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              uint32_t g[16], u[16], o[8];
+              tmem_ld16(t_slab + q * 16, g);
+              tmem_ld16(t_slab + 128 + q * 16, u);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                o[j] = pack_bf16x2(activate<ACT>(__uint_as_float(g[2 * j])) * __uint_as_float(u[2 * j]),
+                                   activate<ACT>(__uint_as_float(g[2 * j + 1])) * __uint_as_float(u[2 * j + 1]));
+              put16(slab, row_in_tile, q, o);
+            }
+            slab_store(&tmO, slab, group, col, m0, issuer);
+            if (p.gu_low) {
+              uint8_t* low = p.gu_low + static_cast<long long>(m0 + row_in_tile) * 2 * p.low + col;
+              const bool row_ok = m0 + row_in_tile < p.rows;
+#pragma unroll 1
+              for (int part = 0; part < 2; ++part) {
+                slab_free(group, issuer);
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                  uint32_t v[16], o[8], l[4];
+                  tmem_ld16(t_slab + part * 128 + q * 16, v);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) o[j] = __byte_perm(v[2 * j], v[2 * j + 1], 0x7632);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    l[j] = __byte_perm(__byte_perm(v[4 * j], v[4 * j + 1], 0x0051), __byte_perm(v[4 * j + 2], v[4 * j + 3], 0x0051), 0x5410);
+                  put16(slab, row_in_tile, q, o);
+                  if (row_ok && col + q * 16 < p.inter) *reinterpret_cast<uint4*>(low + part * p.low + q * 16) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+                slab_store(part ? &tmU : &tmG, slab, group, col, m0, issuer);
+              }
+            }
+          }
+        } else {
+          const uint16_t* gu = p.gu + static_cast<long long>(m0 + row_in_tile) * 2 * p.inter;
+          const uint8_t* low = p.gu_low + static_cast<long long>(m0 + row_in_tile) * 2 * p.low;
+          const bool row_ok = m0 + row_in_tile < p.rows;
+#pragma unroll 1
+          for (int c = group * 64; c < 256; c += 128) {
+            const int col = n0 + c;
+            if (col >= p.inter) break;                // uniform over the group
+            uint32_t du[4][8];
+            slab_free(group, issuer);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4 gv[2], uv[2];
+              const int valid = row_ok ? p.inter - col - q * 16 : 0;
+              load16(gu + col + q * 16, valid, gv);
+              load16(gu + p.inter + col + q * 16, valid, uv);
+              const uint4 none = make_uint4(0, 0, 0, 0);
+              const uint4 gl = valid > 0 ? *reinterpret_cast<const uint4*>(low + col + q * 16) : none;
+              const uint4 ul = valid > 0 ? *reinterpret_cast<const uint4*>(low + p.low + col + q * 16) : none;
+              uint32_t d[16], dg[8];
+              tmem_ld16(t_acc + c + q * 16, d);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                float g0, g1, u0, u1, a0, a1, s0, s1;
+                from_kept(word(gv[j / 4], j & 3), word(gl, j / 2), j & 1, g0, g1);
+                from_kept(word(uv[j / 4], j & 3), word(ul, j / 2), j & 1, u0, u1);
+                activate_grad<ACT>(g0, a0, s0);
+                activate_grad<ACT>(g1, a1, s1);
+                const float d0 = __uint_as_float(d[2 * j]), d1 = __uint_as_float(d[2 * j + 1]);
+                dg[j] = pack_bf16x2(d0 * u0 * s0, d1 * u1 * s1);
+                du[q][j] = pack_bf16x2(d0 * a0, d1 * a1);
+              }
+              put16(slab, row_in_tile, q, dg);
+            }
+            slab_store(&tmG, slab, group, col, m0, issuer);
+            slab_free(group, issuer);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) put16(slab, row_in_tile, q, du[q]);
+            slab_store(&tmU, slab, group, col, m0, issuer);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(tempty_lead + acc * 8);
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1;
+    }
+    if (issuer) tma_store_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                  // neither CTA leaves while the other may still signal or read it
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc2(tmem_base, 512);
+  }
+}
+
+// Rows of `cols` bf16 values, boxes of 64 columns.
+static CUtensorMap rows_map(const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), 1};
+  const uint64_t strides[2] = {static_cast<uint64_t>(ld) * 2, static_cast<uint64_t>(ld) * 2 * static_cast<uint64_t>(rows)};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(box_rows), 1};
+  return make_tmap(ptr, 3, dims, strides, box, 2, true);
+}
+
+// CTA pairs that can be resident at once on the current device.  (Callers and the autograd engine's threads may ask at the same time.)
+template <class Kernel>
+static int pairs_at_once(Kernel kernel, size_t smem, std::atomic<int>* most) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < 64;
+  int n = known ? most[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(num_sms());
+    cfg.blockDim = dim3(GM_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = num_sms() / 2;
+    }
+    if (known) most[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+template <int MODE, int ACT>
+static void launch(const CUtensorMap& a, const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& o, const CUtensorMap& g, const CUtensorMap& u,
+                   GatedDev p, int inner, cudaStream_t s) {
+  constexpr size_t SMEM = 1024 + GM_STAGES * GM_STAGE + 2 * SLAB_BYTES + 256;
+  static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
+  static std::atomic<int> most[64] = {};
+  const auto kernel = gated_mlp_kernel<MODE, ACT>;
+  const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
+  if (set != cudaSuccess) throw std::runtime_error(std::string("himuon gated_mlp: ") + cudaGetErrorString(set));
+  const int pairs = pairs_at_once(kernel, SMEM, most);
+  constexpr int FEATURES = MODE == UP ? 128 : 256;
+  p.tiles_m = (p.rows + 2 * BM - 1) / (2 * BM);
+  p.tiles_n = (p.inter + FEATURES - 1) / FEATURES;
+  p.kblocks = (inner + BK - 1) / BK;
+  p.status = status_word_ptr();
+  const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n;
+  if (total >= (1LL << 30)) throw std::runtime_error("himuon gated_mlp: too many tiles for one launch");
+  kernel<<<2 * static_cast<int>(total < pairs ? total : pairs), GM_THREADS, SMEM, s>>>(a, b0, b1, o, g, u, p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon gated_mlp launch failed: ") + cudaGetErrorString(e));
+}
+template <int MODE, class... Args>
+static void launch_activation(int activation, const Args&... args) {
+  switch (activation) {
+    case kSilu: return launch<MODE, kSilu>(args...);
+    case kGelu: return launch<MODE, kGelu>(args...);
+    case kGeluTanh: return launch<MODE, kGeluTanh>(args...);
+    case kRelu: return launch<MODE, kRelu>(args...);
+  }
+  throw std::runtime_error("himuon gated_mlp: unknown activation");
+}
+
+void gated_up(const GatedUpArgs& a, cudaStream_t s) {
+  if (a.rows <= 0 || a.inter <= 0 || a.hidden <= 0 || a.hidden % 8 || a.inter % 8) throw std::runtime_error("himuon gated_mlp: bad sizes");
+  const long long ld = 2LL * a.inter;
+  GatedDev p{};
+  if ((a.gu == nullptr) != (a.gu_low == nullptr)) throw std::runtime_error("himuon gated_mlp: upper and lower bits go together");
+  p.gu_low = static_cast<uint8_t*>(a.gu_low);
+  p.rows = a.rows;
+  p.inter = a.inter;
+  p.low = gated_low(a.inter);
+  const CUtensorMap o = rows_map(a.h, a.rows, a.inter, a.inter, BM);
+  launch_activation<UP>(a.activation, rows_map(a.x, a.rows, a.hidden, a.ld_x, BM), rows_map(a.wg, a.inter, a.hidden, a.ld_wg, BM),
+                        rows_map(a.wu, a.inter, a.hidden, a.ld_wu, BM), o, a.gu ? rows_map(a.gu, a.rows, a.inter, ld, BM) : o,
+                        a.gu ? rows_map(static_cast<char*>(a.gu) + 2LL * a.inter, a.rows, a.inter, ld, BM) : o, p, a.hidden, s);
+}
+
+void gated_down_grad(const GatedDownGradArgs& a, cudaStream_t s) {
+  if (a.rows <= 0 || a.inter <= 0 || a.hidden <= 0 || a.hidden % 8 || a.inter % 8) throw std::runtime_error("himuon gated_mlp: bad sizes");
+  const long long ld = 2LL * a.inter;
+  GatedDev p{};
+  p.gu = static_cast<const uint16_t*>(a.gu);
+  p.gu_low = static_cast<uint8_t*>(const_cast<void*>(a.gu_low));
+  p.rows = a.rows;
+  p.inter = a.inter;
+  p.low = gated_low(a.inter);
+  const CUtensorMap w = rows_map(a.wd, a.hidden, a.inter, a.ld_wd, BK), g = rows_map(a.dgu, a.rows, a.inter, ld, BM);
+  launch_activation<DOWN_GRAD>(a.activation, rows_map(a.dy, a.rows, a.hidden, a.ld_dy, BM), w, w, g, g,
+                               rows_map(static_cast<char*>(a.dgu) + 2LL * a.inter, a.rows, a.inter, ld, BM), p, a.hidden, s);
+}
+
+}  // namespace himuon

@@ -17,16 +17,22 @@
 #include "sm100_common.cuh"
 #include "tma_host.h"
 
+#include <type_traits>
+
 namespace himuon {
 
 constexpr int BN2 = 256;     // tile width
 constexpr int BNH = 128;     // rows of B staged by each CTA
 
 constexpr int GEMM2_THREADS = 384;   // warps 0-3: TMA, MMA, TMEM allocation, none; 4-11: epilogue, two groups of four
-template <int STAGES, bool A_MN, bool B_MN>
+// A second product that the first one's accumulator goes on with: blocks of K from `kblocks` on are its own.
+struct NoSecond {};
+struct SecondProduct { CUtensorMap tmA, tmB; int kblocks; };
+template <int STAGES, bool A_MN, bool B_MN, class Second>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM2_THREADS, 1)
 gemm2_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmW, GemmDev p) {
+                  const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmW, GemmDev p,
+                  const __grid_constant__ Second second) {
   constexpr uint32_t A_BYTES = BM * BK * 2;
   constexpr uint32_t B_BYTES = BNH * BK * 2;
   constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
@@ -95,6 +101,17 @@ gemm2_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           uint8_t* sA = smem + stage * STAGE_BYTES;
           uint8_t* sB = sA + A_BYTES;
           mbar_expect_tx(&full[stage], 2 * STAGE_BYTES, leader ? e : 0);
+          if constexpr (!std::is_same_v<Second, NoSecond>) {
+            static_assert(!A_MN && B_MN, "the form that the feed-forward block's gradient has");
+            const bool two = kb >= second.kblocks;
+            const int k0 = (two ? kb - second.kblocks : kb) * BK;
+            const CUtensorMap *ma = two ? &second.tmA : &tmA, *mb = two ? &second.tmB : &tmB;
+            tma2_load_3d(sA, ma, &full[stage], k0, m0, b, e);
+#pragma unroll
+            for (int j = 0; j < BNH / 64; ++j) tma2_load_3d(sB + j * CHUNK_BYTES, mb, &full[stage], n0 + j * 64, k0, b, e);
+            if (++stage == STAGES) { stage = 0; phase ^= 1; }
+            continue;
+          }
           if (!A_MN) {
             tma2_load_3d(sA, &tmA, &full[stage], kb * BK, m0, b, e);
           } else {
@@ -270,12 +287,12 @@ static CUtensorMap operand_tmap(const void* ptr, bool mn, int extent, int K, lon
   return make_tmap(ptr, 3, dims, strides, box, 2, true);
 }
 
-template <int STAGES, bool A_MN, bool B_MN>
+template <int STAGES, bool A_MN, bool B_MN, class Second = NoSecond>
 static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   constexpr uint32_t STAGE_BYTES = (BM + BNH) * BK * 2;
   constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + 2 * SLAB_BYTES + 256;
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
-  auto kern = gemm2_bf16_kernel<STAGES, A_MN, B_MN>;
+  auto kern = gemm2_bf16_kernel<STAGES, A_MN, B_MN, Second>;
   static bool attr_done = false;
   if (!attr_done) {
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
@@ -298,6 +315,13 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   p.tiles_m = (a.M + 2 * BM - 1) / (2 * BM);
   p.tiles_n = (a.N + BN2 - 1) / BN2;
   p.kblocks = (a.K + BK - 1) / BK;
+  Second second{};
+  if constexpr (!std::is_same_v<Second, NoSecond>) {
+    second.tmA = operand_tmap(a.A2, A_MN, a.M, a.K, a.lda, a.batch, a.strideA);
+    second.tmB = operand_tmap(a.B2, B_MN, a.N, a.K, a.ldb2, a.batch, a.strideB);
+    second.kblocks = p.kblocks;
+    p.kblocks *= 2;
+  }
   p.tma_store = 1;
   p.nslices = 1;
   // (a bf16 C takes one rounding more that way, of the partial: long reductions only, as ever)
@@ -353,7 +377,7 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
     p.stream_k = 1;
     pairs = cap;
   }
-  kern<<<static_cast<int>(2 * pairs), GEMM2_THREADS, SMEM, stream>>>(tmA, tmB, tmC, tmW, p);
+  kern<<<static_cast<int>(2 * pairs), GEMM2_THREADS, SMEM, stream>>>(tmA, tmB, tmC, tmW, p, second);
   if (p.nslices > 1) {
     const long long groups = 256LL * 256 / 4 * rem;
     const int blocks = static_cast<int>((groups + 255) / 256 < num_sms() * 4 ? (groups + 255) / 256 : num_sms() * 4);
@@ -401,6 +425,10 @@ long long gemm_parts_floats(const GemmArgs& a) {
   // (a tile for each pair at most, where the plan may cut a last wave: reductions of 16 blocks or more)
   return gemm2_supported(a) && a.K > 15 * BK ? static_cast<long long>(num_sms() / 2) * 256 * 256 : 0;
 }
+// The same for a gemm2_bf16() that is asked for as such.
+long long gemm2_parts_floats(const GemmArgs& a) {
+  return (a.A2 != nullptr ? 2 : 1) * ((a.K + BK - 1) / BK) >= 16 ? static_cast<long long>(num_sms() / 2) * 256 * 256 : 0;
+}
 // True when the pair kernel can run this problem and is expected to win: TMA-storable output (whole 16-byte groups of
 // columns: a TMA store writes those whole, past the output's last column if need be) and more than one CTA tile of rows.
 bool gemm2_supported(const GemmArgs& a) {
@@ -411,6 +439,13 @@ bool gemm2_supported(const GemmArgs& a) {
 }
 
 void gemm2_bf16(const GemmArgs& a, cudaStream_t stream) {
+  if (a.A2 != nullptr) {
+    if (a.a_mn || !a.b_mn || a.N % 8 || a.ldc % 8 || a.aux != nullptr || a.out_fp32) throw std::runtime_error("himuon gemm (pair): two products are a b + a2 b2 of rows of a along K, in bf16");
+    launch_gemm2<6, false, true, SecondProduct>(a, stream);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) throw std::runtime_error(std::string("himuon gemm (pair) launch failed: ") + cudaGetErrorString(e));
+    return;
+  }
   const int sel = (a.a_mn ? 2 : 0) | (a.b_mn ? 1 : 0);
   switch (sel) {
     case 0: launch_gemm2<6, false, false>(a, stream); break;

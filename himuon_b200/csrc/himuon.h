@@ -37,9 +37,12 @@ struct GemmArgs {
   int symmetric = 0;  // the caller guarantees C = C^T (X X^T, or c A A + b A with A symmetric): the one-CTA kernel then
                       // computes only the tiles that touch the lower triangle and mirrors the rest
   int ordered = 0;    // C += alpha*acc reads C and adds each tile once: no reductions into C, whose order is the schedule's
+  const void *A2 = nullptr, *B2 = nullptr;      // gemm2_bf16 alone: C = A B + A2 B2, rounded once; A2 laid out as A, B2 as B but for
+  long long ldb2 = 0;                           // its own stride
   float* parts = nullptr;   // gemm_parts_floats() floats for the partials of tiles that are cut along K; none are cut without
 };
 long long gemm_parts_floats(const GemmArgs& args);
+long long gemm2_parts_floats(const GemmArgs& args);
 void gemm_bf16(const GemmArgs& args, cudaStream_t stream);
 // CTA-pair (cta_group::2) variant for 256 x 256 tiles; gemm_bf16 dispatches to it when gemm2_supported().
 bool gemm2_supported(const GemmArgs& args);

@@ -1,0 +1,197 @@
+// Rotary positions: the first `rotary_dim` values of every head are pairs (a, b), turned by the angle of their position,
+//     a' = c a - s b,   b' = c b + s a,   c = m cos(pos f_i), s = m sin(pos f_i);
+// the values behind them pass through.  Pairs are (i, i + rotary_dim / 2) or, interleaved, (2i, 2i + 1).  The gradient is the same with -s.
+//
+// Angles.  fp32 angles of far positions are off by pos * 2^-24 of a radian and more (0.008 at 131071).  Here a frequency is a whole
+// number of 2^-64 turns a position, so that pos * f modulo 2^64 is the angle's place within its turn, exact to pos * 2^-65 of a turn at any
+// position, with no table to make, keep or read.  Its upper 32 bits go to sincospif.
+//
+// Bounded by memory: every value is read and written once.  A thread takes two vectors of 16 bytes of a head (a's and b's of the same pairs,
+// or two that pass through), works out their sines once and keeps them for all the heads that it goes through.
+#include "rotary.h"
+
+#include <algorithm>
+
+#include "himuon.h"
+#include "sm100_common.cuh"
+
+namespace himuon {
+
+namespace {
+
+struct RotaryDev {
+  RotaryArgs a;
+  int units;                 // pairs of vectors in a head
+  int lanes;                 // heads that neighbouring threads take, of the `heads`
+  long long threads;         // rows * lanes * units
+};
+
+__device__ __forceinline__ float2 wave(const RotaryArgs& a, long long pos, int i) {
+  const unsigned long long t = static_cast<unsigned long long>(pos) * a.turns[i];
+  float s, c;
+  sincospif(static_cast<float>(static_cast<int>(t >> 32)) * 0x1p-31f, &s, &c);      // (2^32 is a turn, pi half of one)
+  return make_float2(c * a.cos_factor, s * a.sin_factor);
+}
+// One pair, with the same roundings in every kernel.
+__device__ __forceinline__ void turn(const float2& w, float& a, float& b) {
+  const float was = a;
+  a = fmaf(w.x, was, -__fmul_rn(w.y, b));
+  b = fmaf(w.x, b, __fmul_rn(w.y, was));
+}
+__device__ __forceinline__ long long position(const RotaryArgs& a, long long row) { return a.positions ? a.positions[row] : row % a.seq_len; }
+
+template <typename T> struct Vec;
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void get(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = bf16_lo(w[i]); f[2 * i + 1] = bf16_hi(w[i]); }
+  }
+  static __device__ __forceinline__ uint4 put(const float (&f)[8]) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+};
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void get(const uint4& v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 put(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+
+// Whole vectors: heads of whole vectors, rows on 16-byte boundaries, and no vector with both halves of a pair unless interleaved.
+template <typename T, bool INTERLEAVED>
+__global__ void __launch_bounds__(256) rotary_vec_kernel(RotaryDev p) {
+  constexpr int N = Vec<T>::N;
+  const RotaryArgs& a = p.a;
+  const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= p.threads) return;
+  const int unit = static_cast<int>(id % p.units);
+  const long long rest = id / p.units;
+  const int first = static_cast<int>(rest % p.lanes);
+  const long long row = rest / p.lanes;
+  // the unit's two vectors, and whether they are turned
+  const int vecs = a.head_dim / N, turned = a.rotary_dim / N;
+  int v0, v1;
+  bool r0, r1;
+  if (INTERLEAVED) {
+    v0 = unit; v1 = unit + p.units;
+    r0 = v0 < turned; r1 = v1 < turned;
+  } else if (unit < turned / 2) {
+    v0 = unit; v1 = unit + turned / 2;
+    r0 = r1 = true;
+  } else {
+    const int half = (vecs - turned + 1) / 2;
+    v0 = unit - turned / 2 + turned; v1 = v0 + half;
+    r0 = r1 = false;
+  }
+  const bool second = v1 < vecs;
+  constexpr int W = N;                                   // waves of a thread: N pairs, or two times N / 2
+  float2 w[W];
+  if (r0) {
+    const long long pos = position(a, row);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      int pair = v0 * N + i;
+      if (INTERLEAVED) pair = (i < N / 2 ? v0 * N / 2 + i : v1 * N / 2 + i - N / 2);
+      w[i] = !INTERLEAVED || i < N / 2 || r1 ? wave(a, pos, pair) : make_float2(1.f, 0.f);
+    }
+  }
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
+  T* y = reinterpret_cast<T*>(a.y) + row * a.ld_y;
+#pragma unroll 4
+  for (int h = first; h < a.heads; h += p.lanes) {
+    const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<long long>(h) * a.head_dim);
+    uint4* dst = reinterpret_cast<uint4*>(y + static_cast<long long>(h) * a.head_dim);
+    uint4 q0 = src[v0], q1 = second ? src[v1] : make_uint4(0, 0, 0, 0);
+    if (r0) {
+      float f0[N], f1[N];
+      Vec<T>::get(q0, f0);
+      Vec<T>::get(q1, f1);
+      if (INTERLEAVED) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          turn(w[i], f0[2 * i], f0[2 * i + 1]);
+          turn(w[i + N / 2], f1[2 * i], f1[2 * i + 1]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) turn(w[i], f0[i], f1[i]);
+      }
+      q0 = Vec<T>::put(f0);
+      if (!INTERLEAVED || r1) q1 = Vec<T>::put(f1);       // (what passes through keeps its bits)
+    }
+    dst[v0] = q0;
+    if (second) dst[v1] = q1;
+  }
+}
+
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void put(float* p, float x) { *p = x; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// Any even rotary_dim, any row stride: a thread has one pair, or one value that passes through, of all the heads.
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_any_kernel(RotaryDev p) {
+  const RotaryArgs& a = p.a;
+  const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (id >= p.threads) return;
+  const int unit = static_cast<int>(id % p.units);
+  const long long rest = id / p.units;
+  const int first = static_cast<int>(rest % p.lanes), half = a.rotary_dim / 2;
+  const long long row = rest / p.lanes;
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
+  T* y = reinterpret_cast<T*>(a.y) + row * a.ld_y;
+  if (unit >= half) {
+    for (int h = first; h < a.heads; h += p.lanes) {
+      const long long at = static_cast<long long>(h) * a.head_dim + half + unit;
+      y[at] = x[at];
+    }
+    return;
+  }
+  const float2 w = wave(a, position(a, row), unit);
+  const int i0 = a.interleaved ? 2 * unit : unit, i1 = a.interleaved ? 2 * unit + 1 : unit + half;
+  for (int h = first; h < a.heads; h += p.lanes) {
+    const long long at = static_cast<long long>(h) * a.head_dim;
+    float f0 = as_float(x[at + i0]), f1 = as_float(x[at + i1]);
+    turn(w, f0, f1);
+    put(y + at + i0, f0);
+    put(y + at + i1, f1);
+  }
+}
+
+template <typename T>
+void launch(const RotaryArgs& a, cudaStream_t s) {
+  constexpr int N = Vec<T>::N;
+  auto grid16 = [](const void* p, long long ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % N == 0; };
+  const bool whole = a.head_dim % N == 0 && a.rotary_dim % (a.interleaved ? N : 2 * N) == 0 && a.rotary_dim > 0 && grid16(a.x, a.ld_x) && grid16(a.y, a.ld_y);
+  RotaryDev p{};
+  p.a = a;
+  const int vecs = a.head_dim / N;
+  p.units = whole ? (vecs + 1) / 2 : a.head_dim - a.rotary_dim / 2;
+  p.lanes = std::min(a.heads, 4);
+  p.threads = a.rows * p.lanes * p.units;
+  const long long blocks = (p.threads + 255) / 256;
+  if (blocks >= (1LL << 31)) throw std::runtime_error("himuon rotary: too many rows for one launch");
+  const int grid = static_cast<int>(blocks);
+  if (!whole) rotary_any_kernel<T><<<grid, 256, 0, s>>>(p);
+  else if (a.interleaved) rotary_vec_kernel<T, true><<<grid, 256, 0, s>>>(p);
+  else rotary_vec_kernel<T, false><<<grid, 256, 0, s>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon rotary launch failed: ") + cudaGetErrorString(e));
+}
+
+}  // namespace
+
+void rotary(const RotaryArgs& a, cudaStream_t s) {
+  if (a.rows <= 0 || a.heads <= 0 || a.head_dim <= 0) return;
+  if (a.rotary_dim < 0 || a.rotary_dim % 2 || a.rotary_dim > a.head_dim || (a.positions == nullptr && a.seq_len <= 0)) throw std::runtime_error("himuon rotary: bad sizes");
+  if (a.fp32) launch<float>(a, s);
+  else launch<__nv_bfloat16>(a, s);
+}
+
+}  // namespace himuon

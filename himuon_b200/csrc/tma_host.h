@@ -55,7 +55,7 @@ struct TmapKeyHash {
   }
 };
 
-// Encodes (and caches) a tiled tensor map of rank 3 or 4 over 16-bit or 32-bit elements.
+// Encodes (and caches) a tiled tensor map of rank 3 or 4 over 8-bit, 16-bit or 32-bit elements.
 // dims/box are innermost-first; strides[i] is the byte stride of dimension i+1.
 // Requirements checked here: base 16-byte aligned, strides multiples of 16 bytes,
 // inner box extent * element size a multiple of 16 bytes and at most 128 bytes when swizzled.
@@ -83,7 +83,7 @@ inline CUtensorMap make_tmap(const void* ptr, int rank, const uint64_t* dims, co
   for (int i = 0; i < rank; ++i) { gdim[i] = dims[i]; gbox[i] = box[i]; }
   for (int i = 0; i < rank - 1; ++i) gstr[i] = strides_bytes[i];
   CUtensorMap tm;
-  CUtensorMapDataType dt = elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  CUtensorMapDataType dt = elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = get_encode_fn()(&tm, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(ptr), gdim, gstr, gbox, estr,
                                CU_TENSOR_MAP_INTERLEAVE_NONE,
                                swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,

@@ -783,3 +783,8 @@ def linear_cross_entropy(h2d, w, labels, ignore_index: int = -100, chunk: int = 
 # ------------------------------------------------------------------------------------------- packed documents, token scores
 from .packed import PackedLayout, packed_attention  # noqa: E402
 from .scores import TokenLogProbs, linear_token_log_probs, token_log_probs  # noqa: E402
+
+# ------------------------------------------------------------------------------------------- rotary positions, feed-forward block, 8 bits
+from .fp8 import Fp8Blocks, fp8_linear, fp8_matmul, quantize_fp8  # noqa: E402
+from .positions import RotaryFrequencies, rotary  # noqa: E402
+from .gated import gated_mlp  # noqa: E402

@@ -1,0 +1,43 @@
+"""The gated feed-forward block: ``(act(x Wg^T) * (x Wu^T)) Wd^T``."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _ext
+from . import _any_transformed, _warn_torch_path, _with_rows_apart, use_kernels
+from . import reference as ref
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T`` for ``(..., hidden)`` inputs, ``(inter, hidden)`` gate and up weights (which may be
+    slices of one matrix) and a ``(hidden, inter)`` down weight.  ``activation``: ``"silu"``, ``"gelu"`` (exact), ``"gelu_tanh"`` or ``"relu"``.
+
+    bf16 CUDA tensors whose sizes are multiples of 8 run the sm_100a kernels: both projections, the activation and the product are one of them,
+    as are the down projection's gradient and the gates' on the way back.  The activation sees the projections before they are rounded, so that
+    the result is nearer to the exact one than that of :func:`swiglu` on finished projections, and not its bits.  Up to 64 rows run kernels
+    that stream the weights.  Differentiable once in all four; the backward pass needs ``x``, and keeps 8 bytes for each row and
+    intermediate feature until then.  Under vmap and forward-mode differentiation the PyTorch formulation runs."""
+    if activation not in ACTIVATIONS:
+        raise RuntimeError(f"himuon_b200.ops.gated_mlp: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
+    if x.dim() < 1 or w_gate.dim() != 2 or not x.is_floating_point():
+        raise RuntimeError("himuon_b200.ops.gated_mlp: (..., hidden) inputs and (inter, hidden) weights of floating point expected")
+    inter, hidden = w_gate.shape
+    if x.shape[-1] != hidden or w_up.shape != (inter, hidden) or w_down.shape != (hidden, inter) or hidden == 0 or inter == 0:
+        raise RuntimeError(f"himuon_b200.ops.gated_mlp: sizes disagree: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, "
+                           f"w_down {tuple(w_down.shape)}")
+    if any(w.dtype != x.dtype or w.device != x.device for w in (w_gate, w_up, w_down)):
+        raise RuntimeError("himuon_b200.ops.gated_mlp: inputs and weights must be of one type on one device")
+    transformed = _any_transformed(x, w_gate, w_up, w_down)
+    if use_kernels(x) and hidden % 8 == 0 and inter % 8 == 0 and not transformed:
+        x2d = _with_rows_apart(x.reshape(math.prod(x.shape[:-1]), hidden))
+        y = _ext.ext().gated_mlp(x2d, _with_rows_apart(w_gate), _with_rows_apart(w_up), _with_rows_apart(w_down), ACTIVATIONS[activation])
+        return y.view(x.shape)
+    if use_kernels(x):
+        _warn_torch_path("gated_mlp", "under vmap or forward-mode differentiation" if transformed else
+                         f"sizes of {hidden} and {inter} (the kernels take multiples of 8)")
+    return ref.gated_mlp(x, w_gate, w_up, w_down, activation)

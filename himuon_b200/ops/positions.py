@@ -1,0 +1,145 @@
+"""Rotary positions: both layouts of the pairs, any part of the head, any position, frequencies scaled for long contexts.
+
+:func:`head_norm_rope` turns whole heads by a table of the positions of one sequence, with the heads' norm on the way.
+:func:`rotary` takes the positions themselves and needs no table: the angle of a position is exact wherever it lies.
+"""
+
+from __future__ import annotations
+
+import math
+from fractions import Fraction
+
+import torch
+
+from .. import _ext
+from . import _any_transformed, _check_width, _warn_torch_path
+from . import reference as ref
+
+TWO_PI = 2 * Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)
+SCALINGS = ("linear", "ntk", "yarn", "llama3")
+
+
+def _number(op: str, d: dict, key: str, default=None, least: float = 0.0) -> float:
+    value = d.get(key, default)
+    if value is None:
+        raise RuntimeError(f"himuon_b200.ops.{op}: scaling needs {key}")
+    value = float(value)
+    if not (math.isfinite(value) and value > least):
+        raise RuntimeError(f"himuon_b200.ops.{op}: {key} must be above {least}, got {value}")
+    return value
+
+
+def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[list[float], float]:
+    """(angle of each pair at position 1 in 64 bits, factor of cosine and sine)."""
+    op, pairs = "RotaryFrequencies", rotary_dim // 2
+    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
+    if kind in (None, "default"):
+        if scaling is not None and kind is None:
+            raise RuntimeError(f"himuon_b200.ops.{op}: scaling needs rope_type, one of {SCALINGS}")
+        return [theta ** (-2.0 * i / rotary_dim) for i in range(pairs)], 1.0
+    if kind not in SCALINGS:
+        raise RuntimeError(f"himuon_b200.ops.{op}: rope_type must be one of {SCALINGS}, got {kind!r}")
+    factor = _number(op, scaling, "factor")
+    if kind == "ntk":                    # a larger base: the last pair ends up `factor` times as long, the first as it was
+        if rotary_dim > 2:
+            theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+        return [theta ** (-2.0 * i / rotary_dim) for i in range(pairs)], 1.0
+    inv = [theta ** (-2.0 * i / rotary_dim) for i in range(pairs)]
+    if kind == "linear":
+        return [f / factor for f in inv], 1.0
+    length = _number(op, scaling, "original_max_position_embeddings")
+    if kind == "yarn":
+        # pairs that turn often within the original length stay, those that do not turn once are stretched, a ramp between them
+        fast, slow = _number(op, scaling, "beta_fast", 32.0), _number(op, scaling, "beta_slow", 1.0)
+
+        def pair_of(turns: float) -> float:
+            return rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
+        span = float(hi - lo) if hi != lo else 0.001
+        attention = scaling.get("attention_factor")
+        if attention is None:
+            attention = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        else:
+            attention = _number(op, scaling, "attention_factor")
+        out = []
+        for i, f in enumerate(inv):
+            ramp = min(max((i - lo) / span, 0.0), 1.0)
+            out.append(f / factor * ramp + f * (1.0 - ramp))
+        return out, attention
+    low, high = _number(op, scaling, "low_freq_factor"), _number(op, scaling, "high_freq_factor")
+    if high <= low:
+        raise RuntimeError(f"himuon_b200.ops.{op}: high_freq_factor must be above low_freq_factor")
+    out = []
+    for f in inv:                        # by how often a pair turns within the original length
+        kept = min(max((length * f / (2 * math.pi) - low) / (high - low), 0.0), 1.0)
+        out.append(f / factor * (1.0 - kept) + f * kept)
+    return out, 1.0
+
+
+class RotaryFrequencies:
+    """How fast the pairs of a head turn.  Made once for a model; every layer uses it.
+
+    ``rotary_dim``: how many values of a head are turned, the first ones (even, 0 included).  Pair ``i`` turns by
+    ``theta ** (-2 i / rotary_dim)`` a position.  ``scaling``: as ``rope_scaling`` in a model's configuration, with ``rope_type``
+    ``"linear"`` (all frequencies divided by ``factor``), ``"ntk"`` (a larger ``theta``, by ``factor ** (d / (d - 2))``), ``"yarn"``
+    (``factor``, ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``attention_factor``) or ``"llama3"`` (``factor``,
+    ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``).
+
+    ``frequencies``: the angles at position 1 as floats; ``factor``: what cosine and sine are multiplied by (other than 1 with yarn).
+    """
+
+    def __init__(self, rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None, device="cuda"):
+        if not isinstance(rotary_dim, int) or rotary_dim < 0 or rotary_dim % 2:
+            raise RuntimeError(f"himuon_b200.ops.RotaryFrequencies: rotary_dim must be an even number of values, got {rotary_dim!r}")
+        if not (math.isfinite(theta) and theta > 1.0):
+            raise RuntimeError(f"himuon_b200.ops.RotaryFrequencies: theta must be above 1, got {theta}")
+        self.rotary_dim, self.theta, self.scaling = rotary_dim, float(theta), None if scaling is None else dict(scaling)
+        self.frequencies, self.factor = _frequencies(rotary_dim, self.theta, self.scaling)
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        # whole numbers of 2^-64 turns a position: position times this, modulo 2^64, is the place within a turn
+        turns = [round(Fraction(f) / TWO_PI * 2 ** 64) % 2 ** 64 for f in self.frequencies]
+        self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64).to(self.device)
+        if self.device.type == "cuda":
+            torch.cuda.current_stream(self.device).synchronize()       # calls on any stream find it there
+
+
+def rotary(x2d, positions, freqs: RotaryFrequencies, heads: int, head_dim: int, interleaved: bool = False):
+    """Turns the first ``freqs.rotary_dim`` values of every head of ``(rows, heads*head_dim)`` rows (which may be a column slice: queries and
+    keys of one projection are turned by one call) by their position; the values behind them pass through.
+
+    ``positions``: int64, one for each row (any value; ``PackedLayout.positions`` has those of a packed batch), or the length ``S`` of
+    sequences that lie one after the other, whose rows have positions ``0..S-1``.  Pairs are ``(i, i + rotary_dim / 2)``, or ``(2 i, 2 i + 1)`` with
+    ``interleaved``.  Returns a new contiguous tensor of the type of ``x2d``; differentiable in ``x2d``, any number of times.  bf16 and fp32 CUDA
+    tensors run the sm_100a kernel, in fp32; under vmap and forward-mode differentiation the PyTorch formulation runs."""
+    if not isinstance(freqs, RotaryFrequencies):
+        raise RuntimeError("himuon_b200.ops.rotary: freqs must be a RotaryFrequencies")
+    if x2d.dim() != 2 or not x2d.is_floating_point() or heads <= 0 or head_dim <= 0:
+        raise RuntimeError("himuon_b200.ops.rotary: (rows, heads*head_dim) of floating point expected")
+    _check_width("rotary", x2d, heads * head_dim)
+    if freqs.rotary_dim > head_dim:
+        raise RuntimeError(f"himuon_b200.ops.rotary: {freqs.rotary_dim} values to be turned in heads of {head_dim}")
+    if freqs.device != x2d.device:
+        raise RuntimeError(f"himuon_b200.ops.rotary: the frequencies are on {freqs.device}, the tensor on {x2d.device}")
+    rows, seq_len = x2d.shape[0], 1
+    if isinstance(positions, torch.Tensor):
+        if positions.dtype != torch.int64 or positions.dim() != 1 or positions.shape[0] != rows or positions.device != x2d.device:
+            raise RuntimeError(f"himuon_b200.ops.rotary: positions must be int64, one for each of the {rows} rows, on {x2d.device}")
+        positions = positions.contiguous()
+    else:
+        seq_len, positions = positions, None
+        if not isinstance(seq_len, int) or seq_len <= 0 or rows % seq_len:
+            raise RuntimeError(f"himuon_b200.ops.rotary: positions must be a tensor or the length of sequences that {rows} rows hold, got {seq_len!r}")
+    transformed = _any_transformed(x2d)
+    if x2d.is_cuda and x2d.dtype in (torch.bfloat16, torch.float32) and not transformed:
+        if x2d.stride(1) != 1 and x2d.shape[1] > 1:
+            x2d = x2d.clone(memory_format=torch.contiguous_format)
+        return _ext.ext().rotary(x2d, positions, freqs.turns, seq_len, heads, freqs.rotary_dim, bool(interleaved), freqs.factor)
+    if x2d.is_cuda and transformed:
+        _warn_torch_path("rotary", "under vmap or forward-mode differentiation")
+    if positions is None:
+        positions = torch.arange(rows, device=x2d.device) % seq_len
+    inv = torch.tensor(freqs.frequencies, dtype=torch.float64, device=x2d.device)
+    return ref.rotary(x2d, positions, inv, freqs.factor, heads, head_dim, bool(interleaved))

@@ -150,3 +150,78 @@ def token_log_probs(logits, ids, top_k: int = 0, ignore_index: int = -100):
         return log_probs, entropy, None, None
     top_ids = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[:, :top_k].contiguous()
     return log_probs, entropy, lp.detach().gather(1, top_ids), top_ids
+
+
+def rotary(x2d, positions, inv, factor: float, heads: int, head_dim: int, interleaved: bool):
+    """Turns the first ``2 * len(inv)`` values of every head by ``positions * inv`` (angles in fp64), products in fp32 (fp64 for fp64)."""
+    acc = torch.float64 if x2d.dtype == torch.float64 else torch.float32
+    angles = positions.to(torch.float64)[:, None] * inv
+    cos, sin = ((f(angles) * factor).to(acc)[:, None, :] for f in (torch.cos, torch.sin))
+    x = x2d.to(acc).reshape(x2d.shape[0], heads, head_dim)
+    r = 2 * inv.numel()
+    head, rest = x[..., :r], x[..., r:]
+    a, b = (head[..., 0::2], head[..., 1::2]) if interleaved else (head[..., : r // 2], head[..., r // 2:])
+    a, b = a * cos - b * sin, b * cos + a * sin
+    head = torch.stack((a, b), -1).flatten(-2) if interleaved else torch.cat((a, b), -1)
+    return torch.cat((head, rest), -1).reshape(x2d.shape).to(x2d.dtype)
+
+
+def gated_mlp(x, w_gate, w_up, w_down, activation: str = "silu"):
+    act = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda g: F.gelu(g, approximate="tanh"), "relu": F.relu}[activation]
+    if x.dtype in (torch.float32, torch.float64):
+        return (act(x @ w_gate.t()) * (x @ w_up.t())) @ w_down.t()
+    x, dtype = x.float(), x.dtype
+    h = act(x @ w_gate.float().t()) * (x @ w_up.float().t())
+    return (h.to(dtype).float() @ w_down.float().t()).to(dtype)
+
+
+def quantize_fp8(x, block_rows: int):
+    """``(values, scales)``: e4m3 and a power of two for each block of ``(block_rows, 128)``: see ``ops.quantize_fp8``."""
+    rows, cols = x.shape
+    nr, nc = -(-rows // block_rows), -(-cols // 128)
+    padded = F.pad(x.float(), (0, nc * 128 - cols, 0, nr * block_rows - rows)).view(nr, block_rows, nc, 128)
+    size = torch.where(padded.isfinite(), padded.abs(), torch.zeros_like(padded))
+    mantissa, exponent = torch.frexp(size.amax((1, 3)) if size.numel() else size.new_zeros(nr, nc))
+    exponent = torch.where(mantissa == 0, torch.zeros_like(exponent), exponent - 9 + (mantissa > 0.875).int()).clamp(min=-110)
+    scales = torch.ldexp(torch.ones_like(mantissa), exponent)
+    q = padded / scales[:, None, :, None]
+    q = torch.where(q.isfinite(), q, torch.full_like(q, float("nan"))).to(torch.float8_e4m3fn)
+    return q.view(nr * block_rows, nc * 128)[:rows, :cols].contiguous(), scales
+
+
+def fp8_dequantize(values, scales, block_rows: int):
+    rows, cols = values.shape
+    return values.float() * scales.repeat_interleave(block_rows, 0)[:rows].repeat_interleave(128, 1)[:, :cols]
+
+
+class _Fp8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w):
+        ctx.save_for_backward(x, w)
+        return (_in_fp8(x, 1) @ _in_fp8(w, 128).t()).to(x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        dx = (_in_fp8(dy, 1) @ _in_fp8(w, 128)).to(x.dtype) if ctx.needs_input_grad[0] else None
+        dw = (_in_fp8(dy.t(), 1) @ _in_fp8(x.t(), 128).t()).to(w.dtype) if ctx.needs_input_grad[1] else None
+        return dx, dw
+
+
+def _in_fp8(x, block_rows):
+    return fp8_dequantize(*quantize_fp8(x, block_rows), block_rows)
+
+
+def fp8_linear(x2d, w):
+    """``x2d @ w.T`` with operands rounded to 8 bits, and so the gradients' products: see ``ops.fp8_linear``."""
+    return _Fp8LinearFn.apply(x2d, w)
+
+
+def fp8_linear_any(x2d, w):
+    """The same for any transform: rounding has the derivative of doing nothing, and the gradients' products round ``w`` and ``x`` alone."""
+    def rounded(t, block_rows):
+        t = t.float()
+        return t + (_in_fp8(t.detach(), block_rows) - t.detach())
+
+    return (rounded(x2d, 1) @ rounded(w, 128).t()).to(x2d.dtype)
