@@ -6,8 +6,9 @@
 // hangs on the rounding of a quotient; it costs up to one bit of range at the lower end, of 17.  A value that is not finite becomes NaN and has no part
 // in its block's scale.  Below 2^-110 * 2^-10 there is nothing left, also not what this build's arithmetic would flush.
 //
-// Bounded by memory: a block of 256 threads has 128 x 128 values, 8 x 8 a thread, reads them once and writes each wanted copy, as they lie
-// and turned around (through shared memory), with the same scales' maxima from one pass.
+// Bounded by memory: every value is read once, for all the copies that are wanted.  Where a row's blocks are all that is wanted, 16 threads take a block of
+// 128 values.  Otherwise a block of 256 threads has 128 x 128 values, 8 x 8 a thread, and turns them around in shared memory; it holds them as they
+// came (a bf16 pair in a register), since as fp32 they left room for one block to an SM (8192 x 9728 by rows 190 us so).
 #include <cuda_fp8.h>
 
 #include "fp8.h"
@@ -28,120 +29,194 @@ __device__ __forceinline__ int scale_exponent(uint32_t bits) {
   return k < -110 ? -110 : k;
 }
 __device__ __forceinline__ float power_of_two(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? b : 0u;
-}
-__device__ __forceinline__ float nan_for_infinite(float x) {
-  return (__float_as_uint(x) & 0x7FFFFFFFu) >= 0x7F800000u ? __uint_as_float(0x7FFFFFFFu) : x;
-}
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
-
+__device__ __forceinline__ uint32_t two(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return two(a, b) | (two(c, d) << 16); }
 __device__ __forceinline__ float as_float(float x) { return x; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int valid, bool whole, float (&f)[8]) {
-  if (whole) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+constexpr uint32_t kInfinite = 0x7F800000u;
+
+// Eight neighbouring values as they came.
+template <typename T> struct Eight {
+  static constexpr int W = sizeof(T) * 2;
+  uint32_t w[W];
+  // `valid` of them (none: zeros); `whole`: all eight, on a 16-byte boundary.
+  __device__ __forceinline__ void load(const T* p, int valid, bool whole) {
+    if (whole) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { f[2 * j] = bf16_lo(w[j]); f[2 * j + 1] = bf16_hi(w[j]); }
+      for (int i = 0; i < W / 4; ++i) reinterpret_cast<uint4*>(w)[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
     } else {
-      const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    }
-  } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = j < valid ? as_float(p[j]) : 0.f;
+      for (int i = 0; i < W; ++i) w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < valid) {
+          if constexpr (sizeof(T) == 2) w[j / 2] |= static_cast<uint32_t>(__bfloat16_as_ushort(p[j])) << (16 * (j & 1));
+          else w[j] = __float_as_uint(p[j]);
+        }
+    }
+  }
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (sizeof(T) == 2) return (j & 1) ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]);
+    else return __uint_as_float(w[j]);
+  }
+  // Bits of the largest absolute value, as of an fp32 number; of kInfinite or more where one is not finite.
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+      return max(m << 16, m & 0xFFFF0000u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+      return m;
+    }
+  }
+  // The same of the finite ones.
+  __device__ __forceinline__ uint32_t largest_finite() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = __float_as_uint(at(j)) & 0x7FFFFFFFu;
+      m = max(m, b < kInfinite ? b : 0u);
+    }
+    return m;
+  }
+  __device__ __forceinline__ uint2 quantized(float by) const {
+    return make_uint2(pack4(at(0) * by, at(1) * by, at(2) * by, at(3) * by), pack4(at(4) * by, at(5) * by, at(6) * by, at(7) * by));
+  }
+  // Infinities become NaN.
+  __device__ __forceinline__ void mark() {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if ((w[i] & 0x7F80u) == 0x7F80u) w[i] |= 0x7Fu;
+        if ((w[i] & 0x7F800000u) == kInfinite) w[i] |= 0x7F0000u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if ((w[i] & kInfinite) == kInfinite) w[i] |= 0x7FFFFFu;
+    }
+  }
+};
+
+template <int LANES>
+__device__ __forceinline__ uint32_t largest_of(uint32_t m) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+// Rows by themselves: 16 threads take RUN neighbouring blocks of a row.
+constexpr int RUN = 4;
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(Fp8QuantizeArgs a, int runs, int blocks_c, long long total, int aligned) {
+  const long long id = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const bool mine = id < total;                        // (all 32 lanes meet in the shuffles)
+  const long long row = mine ? id / runs : 0;
+  const int b0 = static_cast<int>(id - row * runs) * RUN, lane = threadIdx.x & 15;
+  const Fp8Out& o = a.straight;
+  Eight<T> v[RUN];
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    const long long c = static_cast<long long>(b0 + i) * QT + lane * 8;
+    const int valid = mine && c < a.cols ? static_cast<int>(a.cols - c < 8 ? a.cols - c : 8) : 0;
+    v[i].load(reinterpret_cast<const T*>(a.x) + row * a.ld + c, valid, valid == 8 && aligned);
+  }
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
+    uint32_t m = largest_of<16>(v[i].largest());
+    if (__any_sync(0xffffffffu, m >= kInfinite)) {
+      m = largest_of<16>(v[i].largest_finite());
+      v[i].mark();
+    }
+    const int k = scale_exponent(m);
+    const long long c = static_cast<long long>(b0 + i) * QT + lane * 8;
+    if (mine && b0 + i < blocks_c) {
+      if (c < o.ld) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(o.values) + row * o.ld + c) = v[i].quantized(power_of_two(-k));      // (zeros behind the last column)
+      if (lane == 0) o.scales[row * o.scale_row + (b0 + i) * o.scale_col] = power_of_two(k);
+    }
   }
 }
 
-template <typename T>
+// Any copies: STRAIGHT and TURNED are the rows of their blocks, or 0 for none.
+template <typename T, int STRAIGHT, int TURNED>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(Fp8QuantizeArgs a, int tiles_c, int aligned) {
   __shared__ uint32_t s_col[QT];
   __shared__ uint32_t s_all;
-  __shared__ uint2 s_turned[QT * 16];                  // [column][group of 8 rows, swizzled]
+  __shared__ uint2 s_turned[TURNED ? QT * 16 : 1];     // [column][group of 8 rows, swizzled]
   const int tr = threadIdx.x >> 4, tc = threadIdx.x & 15;
   const long long rblk = blockIdx.x / tiles_c, cblk = blockIdx.x - rblk * tiles_c;
   const long long r0 = rblk * QT + tr * 8, c0 = cblk * QT + tc * 8;
-  const bool turn = a.turned.values != nullptr;
-  float v[8][8];
-  const int valid = static_cast<int>(a.cols - c0 < 8 ? a.cols - c0 : 8);
+  Eight<T> v[8];
+  const int valid = a.cols <= c0 ? 0 : static_cast<int>(a.cols - c0 < 8 ? a.cols - c0 : 8);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const bool in = r0 + i < a.rows;
-    load8(reinterpret_cast<const T*>(a.x) + (r0 + i) * a.ld + c0, in ? valid : 0, in && valid == 8 && aligned, v[i]);
+    v[i].load(reinterpret_cast<const T*>(a.x) + (r0 + i) * a.ld + c0, in ? valid : 0, in && valid == 8 && aligned);
   }
-  const bool whole_scale = (a.straight.values && a.straight.block_rows == QT) || (turn && a.turned.block_rows == QT);
-  if (threadIdx.x < QT) s_col[threadIdx.x] = 0;
-  if (threadIdx.x == 0) s_all = 0;
-  __syncthreads();
-  uint32_t row_max[8];
+  constexpr bool WHOLE = STRAIGHT == QT || TURNED == QT;
+  if (TURNED == 1 && threadIdx.x < QT) s_col[threadIdx.x] = 0;
+  if (WHOLE && threadIdx.x == 0) s_all = 0;
+  uint32_t row_max[8], m_all = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t m = 0;
+  for (int i = 0; i < 8; ++i) m_all = max(m_all, row_max[i] = v[i].largest());
+  const bool finite = !__syncthreads_or(m_all >= kInfinite);
+  if (!finite) {
+    m_all = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, finite_bits(v[i][j]));
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    row_max[i] = m;
+    for (int i = 0; i < 8; ++i) m_all = max(m_all, row_max[i] = v[i].largest_finite());
   }
-  if (whole_scale) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, row_max[i]);
-    if (tc == 0) atomicMax(&s_all, m);
+  if constexpr (WHOLE) {
+    const uint32_t m = largest_of<32>(m_all);
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_all, m);
   }
-  if (turn && a.turned.block_rows == 1) {
+  if constexpr (TURNED == 1) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, finite_bits(v[i][j]));
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t b = __float_as_uint(v[i].at(j)) & 0x7FFFFFFFu;
+        m = max(m, finite || b < kInfinite ? b : 0u);
+      }
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
       if ((threadIdx.x & 16) == 0) atomicMax(&s_col[tc * 8 + j], m);
     }
   }
-  __syncthreads();
-  const int all = whole_scale ? scale_exponent(s_all) : 0;
+  if (WHOLE || TURNED) __syncthreads();
+  const int all = WHOLE ? scale_exponent(s_all) : 0;
+  if (!finite) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = nan_for_infinite(v[i][j]);
-
-  if (a.straight.values) {
+    for (int i = 0; i < 8; ++i) v[i].mark();
+  }
+  if constexpr (STRAIGHT != 0) {
     const Fp8Out& o = a.straight;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int k = o.block_rows == QT ? all : scale_exponent(row_max[i]);
-      const float by = power_of_two(-k);
+      const int k = STRAIGHT == QT ? all : scale_exponent(largest_of<16>(row_max[i]));
       if (r0 + i < a.rows) {
         if (c0 < o.ld)                                 // (behind the last column, up to the row's end, are zeros)
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(o.values) + (r0 + i) * o.ld + c0) =
-              make_uint2(pack4(v[i][0] * by, v[i][1] * by, v[i][2] * by, v[i][3] * by), pack4(v[i][4] * by, v[i][5] * by, v[i][6] * by, v[i][7] * by));
-        if (tc == 0 && o.block_rows == 1) o.scales[(r0 + i) * o.scale_row + cblk * o.scale_col] = power_of_two(k);
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(o.values) + (r0 + i) * o.ld + c0) = v[i].quantized(power_of_two(-k));
+        if (tc == 0 && STRAIGHT == 1) o.scales[(r0 + i) * o.scale_row + cblk * o.scale_col] = power_of_two(k);
       }
     }
-    if (threadIdx.x == 0 && o.block_rows == QT) o.scales[rblk * o.scale_row + cblk * o.scale_col] = power_of_two(all);
+    if (threadIdx.x == 0 && STRAIGHT == QT) o.scales[rblk * o.scale_row + cblk * o.scale_col] = power_of_two(all);
   }
-  if (turn) {
+  if constexpr (TURNED != 0) {
     const Fp8Out& o = a.turned;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = tc * 8 + j;
-      const float by = power_of_two(-(o.block_rows == QT ? all : scale_exponent(s_col[c])));
-      s_turned[c * 16 + (tr ^ tc)] =
-          make_uint2(pack4(v[0][j] * by, v[1][j] * by, v[2][j] * by, v[3][j] * by), pack4(v[4][j] * by, v[5][j] * by, v[6][j] * by, v[7][j] * by));
+      const float by = power_of_two(-(TURNED == QT ? all : scale_exponent(s_col[c])));
+      s_turned[c * 16 + (tr ^ tc)] = make_uint2(pack4(v[0].at(j) * by, v[1].at(j) * by, v[2].at(j) * by, v[3].at(j) * by),
+                                                pack4(v[4].at(j) * by, v[5].at(j) * by, v[6].at(j) * by, v[7].at(j) * by));
     }
-    if (o.block_rows == 1) {
+    if (TURNED == 1) {
       if (threadIdx.x < QT && cblk * QT + threadIdx.x < a.cols)
         o.scales[(cblk * QT + threadIdx.x) * o.scale_row + rblk * o.scale_col] = power_of_two(scale_exponent(s_col[threadIdx.x]));
     } else if (threadIdx.x == 0) {
@@ -158,30 +233,47 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(Fp8QuantizeArgs a, in
   }
 }
 
-// Four values a thread and turn, so that 32 threads write 512 bytes in a row.
+// Four values a thread and group, so that 32 threads write 512 bytes in a row; GROUPS groups of a row whose loads are under way together.
+constexpr int GROUPS = 4;
 template <typename T>
-__global__ void __launch_bounds__(256) fp8_dequantize_kernel(Fp8Matrix m, T* out, long long ld_out, int groups, int fast, long long total) {
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * 256) {
-    const long long row = i / groups;
-    const int col = static_cast<int>(i - row * groups) * 4;
-    const uint8_t* src = static_cast<const uint8_t*>(m.values) + row * m.ld + col;
-    T* dst = out + row * ld_out + col;
-    const float scale = m.scales[(m.block_rows == 1 ? row : row / QT) * m.scale_row + (col / QT) * m.scale_col];
-    const int valid = m.cols - col < 4 ? m.cols - col : 4;
-    uint32_t q = 0;
-    if (fast) q = *reinterpret_cast<const uint32_t*>(src);
-    else
-      for (int j = 0; j < valid; ++j) q |= static_cast<uint32_t>(src[j]) << (8 * j);
-    const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q & 0xFFFFu), __NV_E4M3)));
-    const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q >> 16), __NV_E4M3)));
-    const float f[4] = {lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale};
+__global__ void __launch_bounds__(256) fp8_dequantize_kernel(Fp8Matrix m, T* out, long long ld_out, int pieces, int fast) {
+  const long long row = blockIdx.x / pieces;
+  const int col0 = (static_cast<int>(blockIdx.x - row * pieces) * GROUPS * 256 + static_cast<int>(threadIdx.x)) * 4;
+  const uint8_t* src = static_cast<const uint8_t*>(m.values) + row * m.ld;
+  const float* scales = m.scales + (m.block_rows == 1 ? row : row / QT) * m.scale_row;
+  T* dst = out + row * ld_out;
+  uint32_t q[GROUPS];
+  float scale[GROUPS];
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int col = col0 + g * 1024;
+    q[g] = 0;
+    scale[g] = 0.f;
+    if (col < m.cols) {
+      scale[g] = scales[(col / QT) * m.scale_col];
+      if (fast) {
+        q[g] = __ldcs(reinterpret_cast<const uint32_t*>(src + col));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < m.cols) q[g] |= static_cast<uint32_t>(src[col + j]) << (8 * j);
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int col = col0 + g * 1024;
+    if (col >= m.cols) break;
+    const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[g] & 0xFFFFu), __NV_E4M3)));
+    const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(q[g] >> 16), __NV_E4M3)));
+    const float f[4] = {lo.x * scale[g], lo.y * scale[g], hi.x * scale[g], hi.y * scale[g]};
     if (fast) {
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(f[0], f[1], f[2], f[3]);
-      else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+      if constexpr (sizeof(T) == 4) __stcs(reinterpret_cast<float4*>(dst + col), make_float4(f[0], f[1], f[2], f[3]));
+      else __stcs(reinterpret_cast<uint2*>(dst + col), make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])));
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (j < valid) put(dst + j, f[j]);
+        if (col + j < m.cols) put(dst + col + j, f[j]);
     }
   }
 }
@@ -191,6 +283,20 @@ void check(const char* what) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon ") + what + " launch failed: " + cudaGetErrorString(e));
 }
 
+template <typename T>
+void launch_quantize(const Fp8QuantizeArgs& a, int tiles, int tiles_c, int runs, long long groups, cudaStream_t s) {
+  const int aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ld % (16 / static_cast<int>(sizeof(T))) == 0;
+  const int straight = a.straight.values ? a.straight.block_rows : 0, turned = a.turned.values ? a.turned.block_rows : 0;
+  if (straight == 1 && !turned) fp8_quantize_rows_kernel<T><<<static_cast<int>((groups + 15) / 16), 256, 0, s>>>(a, runs, tiles_c, groups, aligned);
+  else if (straight == QT && !turned) fp8_quantize_kernel<T, QT, 0><<<tiles, 256, 0, s>>>(a, tiles_c, aligned);
+  else if (!straight && turned == 1) fp8_quantize_kernel<T, 0, 1><<<tiles, 256, 0, s>>>(a, tiles_c, aligned);
+  else if (!straight && turned == QT) fp8_quantize_kernel<T, 0, QT><<<tiles, 256, 0, s>>>(a, tiles_c, aligned);
+  else if (straight == 1 && turned == 1) fp8_quantize_kernel<T, 1, 1><<<tiles, 256, 0, s>>>(a, tiles_c, aligned);
+  else if (straight == 1 && turned == QT) fp8_quantize_kernel<T, 1, QT><<<tiles, 256, 0, s>>>(a, tiles_c, aligned);
+  else if (straight == QT && turned == QT) fp8_quantize_kernel<T, QT, QT><<<tiles, 256, 0, s>>>(a, tiles_c, aligned);
+  else throw std::runtime_error("himuon fp8_quantize: no such pair of copies");
+}
+
 }  // namespace
 
 void fp8_quantize(const Fp8QuantizeArgs& a, cudaStream_t s) {
@@ -198,23 +304,22 @@ void fp8_quantize(const Fp8QuantizeArgs& a, cudaStream_t s) {
   for (const Fp8Out* o : {&a.straight, &a.turned})
     if (o->values && ((o->block_rows != 1 && o->block_rows != QT) || o->ld % 16 || reinterpret_cast<uintptr_t>(o->values) % 16))
       throw std::runtime_error("himuon fp8_quantize: blocks of 1 or 128 rows, rows of multiples of 16 bytes");
-  const long long tiles_c = (a.cols + QT - 1) / QT, tiles = (a.rows + QT - 1) / QT * tiles_c;
-  if (tiles >= (1LL << 31)) throw std::runtime_error("himuon fp8_quantize: matrix too large for one launch");
-  const int aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ld % (a.fp32 ? 4 : 8) == 0;
-  if (a.fp32) fp8_quantize_kernel<float><<<static_cast<int>(tiles), 256, 0, s>>>(a, static_cast<int>(tiles_c), aligned);
-  else fp8_quantize_kernel<__nv_bfloat16><<<static_cast<int>(tiles), 256, 0, s>>>(a, static_cast<int>(tiles_c), aligned);
+  const long long tiles_c = (a.cols + QT - 1) / QT, tiles = (a.rows + QT - 1) / QT * tiles_c, runs = (tiles_c + RUN - 1) / RUN, groups = a.rows * runs;
+  if (tiles >= (1LL << 31) || groups >= (1LL << 34)) throw std::runtime_error("himuon fp8_quantize: matrix too large for one launch");
+  if (a.fp32) launch_quantize<float>(a, static_cast<int>(tiles), static_cast<int>(tiles_c), static_cast<int>(runs), groups, s);
+  else launch_quantize<__nv_bfloat16>(a, static_cast<int>(tiles), static_cast<int>(tiles_c), static_cast<int>(runs), groups, s);
   check("fp8_quantize");
 }
 
 void fp8_dequantize(const Fp8Matrix& m, void* out, long long ld_out, int out_fp32, cudaStream_t s) {
   if (m.rows <= 0 || m.cols <= 0) return;
-  const int groups = (m.cols + 3) / 4;
   const int fast = m.cols % 4 == 0 && m.ld % 4 == 0 && reinterpret_cast<uintptr_t>(m.values) % 4 == 0 && ld_out % 4 == 0 &&
                    reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  const long long total = static_cast<long long>(m.rows) * groups, blocks = (total + 255) / 256, most = static_cast<long long>(num_sms()) * 32;
-  const int grid = static_cast<int>(blocks < most ? blocks : most);
-  if (out_fp32) fp8_dequantize_kernel<float><<<grid, 256, 0, s>>>(m, static_cast<float*>(out), ld_out, groups, fast, total);
-  else fp8_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(m, static_cast<__nv_bfloat16*>(out), ld_out, groups, fast, total);
+  const int pieces = (m.cols + GROUPS * 1024 - 1) / (GROUPS * 1024);
+  const long long blocks = static_cast<long long>(m.rows) * pieces;
+  if (blocks >= (1LL << 31)) throw std::runtime_error("himuon fp8_dequantize: matrix too large for one launch");
+  if (out_fp32) fp8_dequantize_kernel<float><<<static_cast<int>(blocks), 256, 0, s>>>(m, static_cast<float*>(out), ld_out, pieces, fast);
+  else fp8_dequantize_kernel<__nv_bfloat16><<<static_cast<int>(blocks), 256, 0, s>>>(m, static_cast<__nv_bfloat16*>(out), ld_out, pieces, fast);
   check("fp8_dequantize");
 }
 

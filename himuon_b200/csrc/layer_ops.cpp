@@ -202,7 +202,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
 };
 
 // ------------------------------------------------------------------------------------------------ 8 bits
-struct Fp8 { at::Tensor values, scales; int64_t block_rows = 1; };
+struct Fp8 { at::Tensor values, scales; int64_t block_rows = 1; bool powers = false; };      // powers: scales known to be powers of two
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
@@ -210,6 +210,7 @@ int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 Fp8 fp8_empty(const at::Tensor& like, int64_t rows, int64_t cols, int64_t block_rows) {
   Fp8 m;
   m.block_rows = block_rows;
+  m.powers = true;                                       // (that is what it will be filled with)
   m.values = at::empty({rows, up(cols, 16) * 16}, like.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, cols);
   const auto fp32 = like.options().dtype(at::kFloat);
   m.scales = block_rows == 1 ? at::empty({up(cols, 128), rows}, fp32).t() : at::empty({up(rows, 128), up(cols, 128)}, fp32);
@@ -287,11 +288,12 @@ at::Tensor product(const char* op, Fp8 a, Fp8 b, bool out_fp32) {
   // (rows of the result are stored in groups of 16 bytes)
   const int64_t group = out_fp32 ? 4 : 8, ld = up(cols, group) * group;
   at::Tensor c = at::empty({rows, ld}, type);
-  himuon::fp8_product(fp8_matrix(a), fp8_matrix(b), c.data_ptr(), ld, out_fp32, cur_stream());
+  himuon::fp8_product(fp8_matrix(a), fp8_matrix(b), c.data_ptr(), ld, out_fp32, a.powers && b.powers, cur_stream());
   return ld == cols ? c : c.narrow(1, 0, cols).contiguous();
 }
-at::Tensor fp8_matmul(const at::Tensor& a, const at::Tensor& a_scales, int64_t a_block, const at::Tensor& b, const at::Tensor& b_scales, int64_t b_block, bool out_fp32) {
-  return product("fp8_matmul", Fp8{a, a_scales, a_block}, Fp8{b, b_scales, b_block}, out_fp32);
+at::Tensor fp8_matmul(const at::Tensor& a, const at::Tensor& a_scales, int64_t a_block, bool a_powers, const at::Tensor& b, const at::Tensor& b_scales, int64_t b_block,
+                      bool b_powers, bool out_fp32) {
+  return product("fp8_matmul", Fp8{a, a_scales, a_block, a_powers}, Fp8{b, b_scales, b_block, b_powers}, out_fp32);
 }
 at::Tensor fp8_dequantize(const at::Tensor& values, const at::Tensor& scales, int64_t block_rows, bool out_fp32) {
   const Fp8 m{values, scales, block_rows};
@@ -307,11 +309,11 @@ at::Tensor fp8_dequantize(const at::Tensor& values, const at::Tensor& scales, in
 }
 
 // x w^T with w kept in 8 bits.
-at::Tensor fp8_linear_kept(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scales, int64_t w_block) {
+at::Tensor fp8_linear_kept(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scales, int64_t w_block, bool w_powers) {
   HM_CHECK(x.dim() == 2 && x.scalar_type() == at::kBFloat16, "fp8_linear: bf16 rows expected");
   const Fp8 q = fp8_empty(x, x.size(0), x.size(1), 1);
   quantize(x, &q, nullptr);
-  return product("fp8_linear", q, Fp8{w, w_scales, w_block}, false);
+  return product("fp8_linear", q, Fp8{w, w_scales, w_block, w_powers}, false);
 }
 // x w^T with both put into 8 bits; copies turned around for the gradients' products are made on the way.
 at::Tensor fp8_linear_forward(const at::Tensor& x, const at::Tensor& w, Fp8* xt, Fp8* wt) {
@@ -352,8 +354,8 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     if (need_w) qt = fp8_empty(dy, dy.size(1), dy.size(0), 1);
     quantize(dy, need_x ? &q : nullptr, need_w ? &qt : nullptr);
     variable_list out(2);
-    if (need_x) out[0] = product("fp8_linear", q, Fp8{saved[0], saved[1], 128}, false);
-    if (need_w) out[1] = product("fp8_linear", qt, Fp8{saved[kept_x ? 2 : 0], saved[kept_x ? 3 : 1], 128}, false);
+    if (need_x) out[0] = product("fp8_linear", q, Fp8{saved[0], saved[1], 128, true}, false);
+    if (need_w) out[1] = product("fp8_linear", qt, Fp8{saved[kept_x ? 2 : 0], saved[kept_x ? 3 : 1], 128, true}, false);
     return out;
   }
 };

@@ -20,11 +20,14 @@ BLOCK = 128
 
 class Fp8Blocks(NamedTuple):
     """A matrix in 8 bits.  ``values``: ``(rows, cols)`` of ``float8_e4m3fn``.  ``scales``: fp32, one for each block of ``(block_rows, 128)`` values,
-    ``(ceil(rows / block_rows), ceil(cols / 128))`` with any strides; ``block_rows`` is 1 or 128."""
+    ``(ceil(rows / block_rows), ceil(cols / 128))`` with any strides; ``block_rows`` is 1 or 128.  ``powers``: every scale is known to be a power of
+    two (from ``2**-126`` on), as those of :func:`quantize_fp8` are; products of two such matrices leave the scales to the tensor core.  Nobody looks at the
+    scales: where it is set and they are others, results are wrong."""
 
     values: torch.Tensor
     scales: torch.Tensor
     block_rows: int = 1
+    powers: bool = False
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the 8 bits stand for, in fp32 or rounded to bf16."""
@@ -61,8 +64,8 @@ def quantize_fp8(x2d: torch.Tensor, block_rows: int = 1, transpose: bool = False
         raise RuntimeError("himuon_b200.ops.quantize_fp8: not under vmap or forward-mode differentiation")
     x2d = x2d.detach()
     if x2d.is_cuda:
-        return Fp8Blocks(*_ext.ext().quantize_fp8(_rows(x2d), int(block_rows), bool(transpose)), int(block_rows))
-    return Fp8Blocks(*ref.quantize_fp8(x2d.t() if transpose else x2d, int(block_rows)), int(block_rows))
+        return Fp8Blocks(*_ext.ext().quantize_fp8(_rows(x2d), int(block_rows), bool(transpose)), int(block_rows), True)
+    return Fp8Blocks(*ref.quantize_fp8(x2d.t() if transpose else x2d, int(block_rows)), int(block_rows), True)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -86,8 +89,8 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"himuon_b200.ops.fp8_matmul: bfloat16 or float32 expected, got {out_dtype}")
     if a.values.is_cuda:
-        return _ext.ext().fp8_matmul(a.values, a.scales, a.block_rows, b.values, b.scales, b.block_rows, out_dtype == torch.float32)
-    return (ref.fp8_dequantize(*a) @ ref.fp8_dequantize(*b).t()).to(out_dtype)
+        return _ext.ext().fp8_matmul(*a, *b, out_dtype == torch.float32)
+    return (ref.fp8_dequantize(*a[:3]) @ ref.fp8_dequantize(*b[:3]).t()).to(out_dtype)
 
 
 def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
@@ -122,5 +125,5 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
         _warn_torch_path("fp8_linear", "under vmap or forward-mode differentiation")
     x2d = x.reshape(math.prod(x.shape[:-1]), shape[1])
     if kept:
-        return (ref.fp8_dequantize(*ref.quantize_fp8(x2d.detach(), 1), 1) @ ref.fp8_dequantize(*w).t()).to(x.dtype).view(out)
+        return (ref.fp8_dequantize(*ref.quantize_fp8(x2d.detach(), 1), 1) @ ref.fp8_dequantize(*w[:3]).t()).to(x.dtype).view(out)
     return (ref.fp8_linear_any if transformed else ref.fp8_linear)(x2d, w).view(out)

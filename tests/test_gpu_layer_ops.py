@@ -359,14 +359,14 @@ def test_quantisation_has_the_bits_of_the_plain_one(dtype, block_rows):
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 128, 128), (5, 40, 144), (8, 352, 128), (16, 130, 512), (31, 640, 1000), (64, 200, 2560), (65, 128, 640), (3, 20, 77), (129, 8, 8),
                                    (130, 1000, 1729), (300, 257, 256), (777, 1728, 640), (513, 300, 4096)])
 def test_fp8_matmul(M, N, K):
-    """Any fp32 scales, blocks of either kind in a, every row length."""
+    """Powers of two and any other fp32 scales, different from block to block, blocks of either kind in a, every row length."""
     ops = _ops()
     torch.manual_seed(M + N + K)
-    for a_block, dtype in ((1, torch.float32), (128, torch.bfloat16), (1, torch.bfloat16)):
+    for a_block, dtype, powers in ((1, torch.float32, False), (128, torch.bfloat16, False), (1, torch.bfloat16, True), (128, torch.float32, True)):
         a = ops.quantize_fp8(torch.randn(M, K, device="cuda"), a_block)
         b = ops.quantize_fp8(torch.randn(N, K, device="cuda"), 128)
-        a = ops.Fp8Blocks(a.values, a.scales * (0.5 + torch.rand_like(a.scales)), a_block)
-        b = ops.Fp8Blocks(b.values, (b.scales * (0.5 + torch.rand_like(b.scales))).t().contiguous().t(), 128)
+        sa, sb = (torch.exp2(torch.randint(-9, 9, s.shape, device="cuda").float()) if powers else s * (0.5 + torch.rand_like(s)) for s in (a.scales, b.scales))
+        a, b = ops.Fp8Blocks(a.values, sa, a_block, powers), ops.Fp8Blocks(b.values, sb.t().contiguous().t(), 128, powers)
         before = ops.launch_count()
         c = ops.fp8_matmul(a, b, out_dtype=dtype)
         assert ops.launch_count() == before + 1 and c.dtype == dtype and c.is_contiguous()
@@ -374,7 +374,7 @@ def test_fp8_matmul(M, N, K):
         want, size = va @ vb.t(), va.abs() @ vb.abs().t()
         bound = _sums(K) * size                                        # (and two roundings of a scale)
         _within(c, want, bound + (U if dtype == torch.bfloat16 else 2.0 ** -24) * (want.abs() + bound), "c")
-        again = ops.Fp8Blocks(a.values.contiguous(), a.scales.contiguous(), a_block), ops.Fp8Blocks(b.values.t().contiguous().t(), b.scales.contiguous(), 128)
+        again = ops.Fp8Blocks(a.values.contiguous(), a.scales.contiguous(), a_block, powers), ops.Fp8Blocks(b.values.t().contiguous().t(), b.scales.contiguous(), 128, powers)
         assert torch.equal(ops.fp8_matmul(*again, out_dtype=dtype), c)
     _clean()
 
@@ -555,7 +555,7 @@ def test_layer_operators_refusals_on_the_gpu():
         e.gated_mlp(x[:, :4], wg[:, :4], wu[:, :4], wd[:4], 0)
     q = ops.quantize_fp8(x)
     with pytest.raises(RuntimeError, match="one for each block"):
-        e.fp8_matmul(q.values, q.scales[:1], 1, q.values, q.scales, 128, False)
+        e.fp8_matmul(q.values, q.scales[:1], 1, False, q.values, q.scales, 128, False, False)
     with pytest.raises(RuntimeError, match="scales must be"):
         ops.fp8_matmul(q, ops.Fp8Blocks(q.values, q.scales.cpu(), 128))
     with pytest.raises(RuntimeError, match="one device"):
