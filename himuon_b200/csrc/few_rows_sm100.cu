@@ -1,273 +1,333 @@
 // Products of a few rows (newest tokens) with a large weight, whose bytes are all that counts:  y = x W^T  in bf16, the same of two
 // weights with the gated activation between them, and the same in 8 bits with a scale for each block of 128.
 //
-// Rows of W are streamed from memory straight into the registers that mma.sync takes them from: 16 rows of W are the A operand, up to 8 rows of x the
-// B operand.  (tcgen05.mma takes its operands from shared memory and leaves its sums in tensor memory; both detours cost more here than the tensor core's rate
-// gives, which is not needed: 16 x 8 x 16 products for every 512 bytes of weight.)  The sum over the inner dimension may take it in any order, as long
-// as both operands use the same: so a thread loads 16 bytes that lie together, and gives them to two products.  Lane l has row l / 4 and bytes 16 (l % 4) of a
-// step of 64 bytes, of W and of x alike.
+// A block streams `th` rows of W (of both weights) through a ring of stages in shared memory, 128 bytes or more of each row and of each row of x a
+// stage, by TMA; two blocks to an SM, so that some 190 KB are on the way at any time.  Warps take 16 rows of W each from there: rows of W are the A operand of
+// mma.sync, up to 8 rows of x the B operand.  (tcgen05.mma leaves its sums in tensor memory, and blocks with scales of their own would have to be fetched from
+// there one by one; its rate is not needed here.)  A block has as few rows of W as it takes to keep all SMs busy, so that often two or seven groups of warps take
+// the stages in turn, and their parts meet in shared memory: a stage costs its warps some 500 cycles whatever is in it.  Everything is added up in one order, which
+// goes by the weight's sizes: bits repeat, and a row's do not depend on how many rows come with it.
 //
-// A block has 16 rows of W; its eight warps share the inner dimension, and a cluster of up to eight blocks again, where 16 rows a block would leave SMs
-// idle.  The parts meet in shared memory, in one order, so that bits repeat, and a row's do not depend on how many rows come with it.
-#include <cooperative_groups.h>
-
+// Weights loaded from memory straight into the operands' registers, 64 bytes of 16 rows a warp, took longer: 24 rows of 2560 x 9728 gated and back
+// 38 + 30 us (22 + 17 now) with eight warps on one group of 16 rows, 57 + 47 with a group a warp.  So did clusters that share the inner dimension (25 + 21), and stages that all warps
+// of a block wait for (25 + 47).
 #include "activations.cuh"
 #include "fp8.h"
 #include "gated_mlp.h"
 #include "himuon.h"
 #include "sm100_common.cuh"
+#include "tma_host.h"
 
 namespace himuon {
-
-namespace cg = cooperative_groups;
 
 namespace {
 
 enum { PLAIN, GATED, EIGHT_BITS };
 
-constexpr int FEW_WARPS = 8;
+constexpr int FEW_WARPS = 7, FEW_THREADS = 32 * (1 + FEW_WARPS);      // warp 0: TMA; then 16 rows of W each (with one more, threads would have 96 registers)
+constexpr int FEW_ROWS = 16 * FEW_WARPS;
+constexpr int FEW_STAGES = 24;
+constexpr uint32_t FEW_RING = 96 * 1024;
 
 struct FewDev {
-  const uint8_t *x, *w0, *w1;          // rows of bytes
-  long long ld_x, ld_w0, ld_w1;
   const float *sx, *sw;                // EIGHT_BITS
   long long sx_row, sx_col, sw_row, sw_col;
   int x_block;
   void *y, *gu;                        // (rows, outer) in bf16 or fp32; GATED: g | u or null (gated_mlp.h)
   uint8_t* gu_low;
-  int rows, outer, inner_bytes, out_fp32;
+  int rows, outer, out_fp32, activation;
+  int blocks, kblocks;                 // of 128 bytes, and stages
+  int th, tiles, stages;               // rows of W of a tile, tiles of a block, stages of the ring
+  int sub;                             // times 128 bytes of every row in a stage
+  int warps, groups;                   // warps that a tile's rows take, and groups of so many, which take stages in turn
+  int* status;
 };
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 stream16(const uint8_t* p, bool ok) {
-  return ok ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void ldmatrix4(uint32_t (&v)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+// 16 bytes of a row of 128, where the swizzle has put them.
+__device__ __forceinline__ uint32_t cell(uint32_t base, int row, int chunk) { return base + row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+__device__ __forceinline__ float activate_any(int activation, float g) {
+  return activation == kSilu ? activate<kSilu>(g) : activation == kGelu ? activate<kGelu>(g) : activation == kGeluTanh ? activate<kGeluTanh>(g) : activate<kRelu>(g);
+}
+// The result of one row of W (of both) and one of x.
+template <int KIND>
+__device__ __forceinline__ void put_result(const FewDev& p, int feature, int row, float v, float u) {
+  if (feature >= p.outer || row >= p.rows) return;
+  const long long at = static_cast<long long>(row) * p.outer + feature;
+  if constexpr (KIND == GATED) {
+    reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(activate_any(p.activation, v) * u);
+    if (p.gu) {
+      uint16_t* gu = static_cast<uint16_t*>(p.gu) + 2LL * row * p.outer + feature;
+      uint8_t* low = p.gu_low + 2LL * row * gated_low(p.outer) + feature;
+      gu[0] = static_cast<uint16_t>(__float_as_uint(v) >> 16);
+      gu[p.outer] = static_cast<uint16_t>(__float_as_uint(u) >> 16);
+      low[0] = static_cast<uint8_t>(__float_as_uint(v) >> 8);
+      low[gated_low(p.outer)] = static_cast<uint8_t>(__float_as_uint(u) >> 8);
+    }
+  } else if (p.out_fp32) {
+    reinterpret_cast<float*>(p.y)[at] = v;
+  } else {
+    reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+  }
 }
 
-// NT: groups of eight rows of x.  ACT: of GATED.
-template <int KIND, int NT, int ACT>
-__global__ void __launch_bounds__(FEW_WARPS * 32) few_rows_kernel(FewDev p) {
-  constexpr int MATS = KIND == GATED ? 2 : 1;
-  constexpr int NX = NT * 8;
-  constexpr int UNROLL = NT >= 4 ? 2 : 4;              // steps of 64 bytes whose loads are under way together
-  extern __shared__ float s_part[];                    // [warp][matrix][16][NX], then [matrix][16][NX] of the block
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int S = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
-  const int f0 = static_cast<int>(blockIdx.x / S) * 16;
-  // this warp's share of the inner dimension, in blocks of 128 values where they have scales of their own and steps else
-  constexpr int UNIT = KIND == EIGHT_BITS ? 128 : 64;
-  const int units = (p.inner_bytes + UNIT - 1) / UNIT, shares = S * FEW_WARPS, share = part * FEW_WARPS + warp;
-  const int u0 = static_cast<int>(static_cast<long long>(units) * share / shares), u1 = static_cast<int>(static_cast<long long>(units) * (share + 1) / shares);
-  const bool ok0 = f0 + r < p.outer, ok1 = f0 + r + 8 < p.outer;
-  const uint8_t *wa[MATS], *wb[MATS];
-  wa[0] = p.w0 + (ok0 ? f0 + r : 0) * p.ld_w0 + t * 16;
-  wb[0] = p.w0 + (ok1 ? f0 + r + 8 : 0) * p.ld_w0 + t * 16;
-  if constexpr (MATS == 2) {
-    wa[1] = p.w1 + (ok0 ? f0 + r : 0) * p.ld_w1 + t * 16;
-    wb[1] = p.w1 + (ok1 ? f0 + r + 8 : 0) * p.ld_w1 + t * 16;
+struct FewBars {
+  uint64_t full[FEW_STAGES], empty[FEW_STAGES];
+  int abort_flag;
+};
+
+// NT: groups of eight rows of x.
+template <int KIND, int NT>
+__global__ void __launch_bounds__(FEW_THREADS, 2)
+few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1, FewDev p) {
+  constexpr int MATS = KIND == GATED ? 2 : 1, NX = NT * 8;
+  constexpr int PER_SUB = KIND == EIGHT_BITS ? 128 : 64;        // values in 128 bytes
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_up_1024(smem_raw);
+  FewBars* bars = reinterpret_cast<FewBars*>(smem + FEW_RING);
+  volatile int* abort_flag = &bars->abort_flag;
+  const bool joined = p.groups > 1;
+  const int warp = warp_id(), lane = threadIdx.x & 31;
+  const int first = static_cast<int>(blockIdx.x) * p.th * p.tiles;
+  const uint32_t w_bytes = static_cast<uint32_t>(p.th) * 128, sub_bytes = MATS * w_bytes + NX * 128, stage_bytes = p.sub * sub_bytes;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], p.warps); }
+    bars->abort_flag = 0;
+    mbar_fence_init();
   }
-  float acc[MATS][NT][4] = {};
-  if constexpr (KIND == EIGHT_BITS) {
-    const float* sw = p.sw + static_cast<long long>(f0 / 128) * p.sw_row;
-    for (int u = u0; u < u1; u += UNROLL / 2) {        // two steps a block
-      uint4 va[UNROLL], vb[UNROLL];
-#pragma unroll
-      for (int i = 0; i < UNROLL; ++i) {
-        const int at = u * 128 + i * 64;
-        const bool in = u + i / 2 < u1 && at + t * 16 < p.inner_bytes;
-        va[i] = stream16(wa[0] + at, in && ok0);
-        vb[i] = stream16(wb[0] + at, in && ok1);
-      }
-#pragma unroll
-      for (int b = 0; b < UNROLL / 2; ++b) {
-        if (u + b >= u1) break;
-        const float w_scale = sw[(u + b) * p.sw_col];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int row = n * 8 + r;
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 2 * b; i < 2 * b + 2; ++i) {
-            const int at = u * 128 + i * 64 + t * 16;
-            const uint4 x = row < p.rows && at < p.inner_bytes ? *reinterpret_cast<const uint4*>(p.x + row * p.ld_x + at) : make_uint4(0, 0, 0, 0);
-            mma_e4m3(c, va[i].x, vb[i].x, va[i].y, vb[i].y, x.x, x.y);
-            mma_e4m3(c, va[i].z, vb[i].z, va[i].w, vb[i].w, x.z, x.w);
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {                // columns 2t and 2t + 1 of the product are rows of x
-            const int col = n * 8 + 2 * t + j;
-            const float s = col < p.rows ? w_scale * p.sx[(col / p.x_block) * p.sx_row + (u + b) * p.sx_col] : 0.f;
-            acc[0][n][j] = fmaf(c[j], s, acc[0][n][j]);
-            acc[0][n][2 + j] = fmaf(c[2 + j], s, acc[0][n][2 + j]);
-          }
+  __syncthreads();
+
+  if (warp == 0) {
+    const uint32_t e = elect_one();
+    tma_prefetch_desc(&tmW0);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = 0; ok && tile < p.tiles && first + tile * p.th < p.outer; ++tile) {
+      const int f0 = first + tile * p.th;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&bars->empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
+        uint8_t* at = smem + stage * stage_bytes;
+        mbar_expect_tx(&bars->full[stage], stage_bytes, e);
+#pragma unroll 1
+        for (int u = 0; u < p.sub; ++u, at += sub_bytes) {
+          const int k = (kb * p.sub + u) * PER_SUB;      // (behind the last value: zeros)
+          tma_load_3d(at, &tmW0, &bars->full[stage], k, f0, 0, e);
+          if (MATS == 2) tma_load_3d(at + w_bytes, &tmW1, &bars->full[stage], k, f0, 0, e);
+          tma_load_3d(at + MATS * w_bytes, &tmX, &bars->full[stage], k, 0, 0, e);
         }
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
       }
     }
   } else {
-    for (int u = u0; u < u1; u += UNROLL) {
-      uint4 va[MATS][UNROLL], vb[MATS][UNROLL];
+    const int group = (warp - 1) / p.warps, m0 = (warp - 1 - group * p.warps) * 16, r = lane >> 2, t = lane & 3;
+    const uint32_t ring = smem_u32(smem);
+    // the lane's addresses of ldmatrix: rows 0-7 and 8-15 of W by bytes 0-15 and 16-31; eight rows of x by four times 16 bytes
+    const int a_row = m0 + (lane & 15), a_chunk = lane >> 4, b_row = lane & 7, b_chunk = lane >> 3;
+    int stage = group;                                   // (groups take turns; stages are a multiple of them)
+    uint32_t phase = 0;
+    bool ok = group < p.groups;
+    for (int tile = 0; tile < p.tiles && first + tile * p.th < p.outer; ++tile) {
+      const int f0 = first + tile * p.th;
+      float acc[MATS][NT][4] = {};
+      const float *sw0 = nullptr, *sw1 = nullptr;
+      float by_w[2] = {}, by_x[NT][2] = {};
+      const bool x_blocks = p.x_block > 1;                 // (of 128 rows: the first has them all)
+      auto load_scales = [&](int block) {
+        const int at = min(block, p.blocks - 1);
+        by_w[0] = __ldg(sw0 + at * p.sw_col);
+        by_w[1] = __ldg(sw1 + at * p.sw_col);
 #pragma unroll
-      for (int i = 0; i < UNROLL; ++i) {
-        const int at = (u + i) * 64;
-        const bool in = u + i < u1 && at + t * 16 < p.inner_bytes;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-          va[m][i] = stream16(wa[m] + at, in && ok0);
-          vb[m][i] = stream16(wb[m] + at, in && ok1);
-        }
+          for (int j = 0; j < 2; ++j) by_x[n][j] = __ldg(p.sx + (x_blocks ? 0 : min(n * 8 + 2 * t + j, p.rows - 1)) * p.sx_row + at * p.sx_col);
+      };
+      if constexpr (KIND == EIGHT_BITS) {
+        sw0 = p.sw + static_cast<long long>(min(f0 + m0 + r, p.outer - 1) / 128) * p.sw_row;
+        sw1 = p.sw + static_cast<long long>(min(f0 + m0 + r + 8, p.outer - 1) / 128) * p.sw_row;
       }
+      for (int kb = group; ok && kb < p.kblocks; kb += p.groups) {
+        if constexpr (KIND == EIGHT_BITS) load_scales(kb * p.sub);           // (on their way while the stage is waited for)
+        if (!mbar_wait_warp(&bars->full[stage], phase, abort_flag, p.status, 3)) { ok = false; break; }
+        constexpr int NN = NT < 4 ? NT : KIND == EIGHT_BITS ? 2 : 4;              // groups of x at a time: more would not fit in the registers of two blocks
+#pragma unroll 1
+        for (int u = 0; u < p.sub; ++u) {
+          if (KIND == EIGHT_BITS && u > 0) load_scales(kb * p.sub + u);
+          const uint32_t base = ring + stage * stage_bytes + u * sub_bytes, x_base = base + MATS * w_bytes;
 #pragma unroll
-      for (int i = 0; i < UNROLL; ++i) {
-        if (u + i >= u1) break;
-        const int at = (u + i) * 64 + t * 16;
+          for (int n0 = 0; n0 < NT; n0 += NN) {
+            float c[NN][4] = {};
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+              uint32_t b[NN][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int row = n * 8 + r;
-          const uint4 x = row < p.rows && at < p.inner_bytes ? *reinterpret_cast<const uint4*>(p.x + row * p.ld_x + at) : make_uint4(0, 0, 0, 0);
+              for (int n = 0; n < NN; ++n) ldmatrix4(b[n], cell(x_base, (n0 + n) * 8 + b_row, half * 4 + b_chunk));
 #pragma unroll
-          for (int m = 0; m < MATS; ++m) {
-            mma_bf16(acc[m][n], va[m][i].x, vb[m][i].x, va[m][i].y, vb[m][i].y, x.x, x.y);
-            mma_bf16(acc[m][n], va[m][i].z, vb[m][i].z, va[m][i].w, vb[m][i].w, x.z, x.w);
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                  uint32_t a[4];
+                  ldmatrix4(a, cell(base + m * w_bytes, a_row, half * 4 + k * 2 + a_chunk));
+#pragma unroll
+                  for (int n = 0; n < NN; ++n) {
+                    if constexpr (KIND == EIGHT_BITS) mma_e4m3(c[n], a, b[n][2 * k], b[n][2 * k + 1]);
+                    else mma_bf16(acc[m][n0 + n], a, b[n][2 * k], b[n][2 * k + 1]);
+                  }
+                }
+            }
+            if constexpr (KIND == EIGHT_BITS) {
+#pragma unroll
+              for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[0][n0 + n][j] = fmaf(c[n][j], by_w[j >> 1] * by_x[n0 + n][j & 1], acc[0][n0 + n][j]);
+            }
           }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->empty[stage]);
+        stage += p.groups;
+        if (stage >= p.stages) { stage -= p.stages; phase ^= 1; }
       }
+      if (!joined) {                                     // (one group: it has them all)
+        if (ok) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int f = m0 + r + 8 * (j >> 1);
+              if (f < p.th) put_result<KIND>(p, f0 + f, n * 8 + 2 * t + (j & 1), acc[0][n][j], acc[MATS - 1][n][j]);
+            }
+        }
+      } else {                                           // (one tile: the ring has been read to its end by all warps that the barrier waits for)
+        named_barrier(1, 32 * FEW_WARPS);
+        if (group < p.groups) {
+          float* s_part = reinterpret_cast<float*>(smem) + group * MATS * p.warps * 16 * (NX + 1);
+#pragma unroll
+          for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s_part[(m * p.warps * 16 + m0 + r + 8 * (j >> 1)) * (NX + 1) + n * 8 + 2 * t + (j & 1)] = acc[m][n][j];
+        }
+      }
+      if (!ok && group < p.groups) break;
     }
   }
-  // the warps' parts: row r (and r + 8) of W, rows 2t and 2t + 1 of each group of x
-#pragma unroll
-  for (int m = 0; m < MATS; ++m)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* dst = s_part + ((warp * MATS + m) * 16 + r) * NX + n * 8 + 2 * t;
-      dst[0] = acc[m][n][0];
-      dst[1] = acc[m][n][1];
-      dst[8 * NX] = acc[m][n][2];
-      dst[8 * NX + 1] = acc[m][n][3];
-    }
+  if (!joined) return;
+  // the groups' parts, neighbouring features next to one another
   __syncthreads();
-  constexpr int VALUES = MATS * 16 * NX;
-  float* s_sum = s_part + FEW_WARPS * VALUES;
-  for (int i = threadIdx.x; i < VALUES; i += FEW_WARPS * 32) {
-    float v = s_part[i];
-#pragma unroll
-    for (int w = 1; w < FEW_WARPS; ++w) v += s_part[w * VALUES + i];
-    s_sum[i] = v;
-  }
-  if (S > 1) cluster.sync();
-  else __syncthreads();
-  // the blocks' parts: each block has its share of the values, neighbouring features next to one another
-  constexpr int OUT = 16 * NX;
-  const int o0 = OUT * part / S, o1 = OUT * (part + 1) / S;
-  for (int o = o0 + threadIdx.x; o < o1; o += FEW_WARPS * 32) {
-    const int f = o & 15, row = o >> 4;
+  const float* s_part = reinterpret_cast<const float*>(smem);
+  const int out = p.th * p.rows, high = p.warps * 16;
+  for (int o = static_cast<int>(threadIdx.x); o < out; o += FEW_THREADS) {
+    const int row = o / p.th, f = o - row * p.th;
     float v[MATS];
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) {
-      const int at = (m * 16 + f) * NX + row;
-      v[m] = 0.f;
-      for (int k = 0; k < S; ++k) v[m] += S > 1 ? cluster.map_shared_rank(s_sum, k)[at] : s_sum[at];
-    }
-    if (row < p.rows && f0 + f < p.outer) {
-      const long long at = static_cast<long long>(row) * p.outer + f0 + f;
-      if constexpr (KIND == GATED) {
-        reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(activate<ACT>(v[0]) * v[1]);
-        if (p.gu) {
-          uint16_t* gu = static_cast<uint16_t*>(p.gu) + 2LL * row * p.outer + f0 + f;
-          uint8_t* low = p.gu_low + 2LL * row * gated_low(p.outer) + f0 + f;
+    for (int m = 0; m < MATS; ++m) v[m] = 0.f;
+    for (int g = 0; g < p.groups; ++g)
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            gu[m * p.outer] = static_cast<uint16_t>(__float_as_uint(v[m]) >> 16);
-            low[m * gated_low(p.outer)] = static_cast<uint8_t>(__float_as_uint(v[m]) >> 8);
-          }
-        }
-      } else if (p.out_fp32) {
-        reinterpret_cast<float*>(p.y)[at] = v[0];
-      } else {
-        reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v[0]);
-      }
-    }
+      for (int m = 0; m < MATS; ++m) v[m] += s_part[((g * MATS + m) * high + f) * (NX + 1) + row];
+    put_result<KIND>(p, first + f, row, v[0], v[MATS - 1]);
   }
-  if (S > 1) cluster.sync();                           // no block leaves while another may still read its sums
 }
 
-template <int KIND, int NT, int ACT>
-void launch(const FewDev& p, cudaStream_t s) {
-  constexpr size_t SMEM = sizeof(float) * (FEW_WARPS + 1) * (KIND == GATED ? 2 : 1) * 16 * NT * 8;
-  const auto kernel = few_rows_kernel<KIND, NT, ACT>;
+struct FewOperands {
+  const void *x = nullptr, *w0 = nullptr, *w1 = nullptr;
+  long long ld_x = 0, ld_w0 = 0, ld_w1 = 0;              // bytes between rows
+  int inner = 0, esz = 2;                                // values of a row and their bytes
+};
+CUtensorMap few_map(const void* ptr, int rows, const FewOperands& o, long long ld, int box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(o.inner), static_cast<uint64_t>(rows), 1};
+  const uint64_t strides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(ld) * static_cast<uint64_t>(rows)};
+  const uint32_t box[3] = {static_cast<uint32_t>(128 / o.esz), static_cast<uint32_t>(box_rows), 1};
+  return make_tmap(ptr, 3, dims, strides, box, o.esz, true);
+}
+
+template <int KIND, int NT>
+void launch(const FewOperands& o, FewDev p, cudaStream_t s) {
+  constexpr int MATS = KIND == GATED ? 2 : 1, NX = NT * 8;
+  constexpr size_t SMEM = 1024 + FEW_RING + sizeof(FewBars);
+  static_assert(2 * SMEM <= 232448 && MATS * FEW_ROWS * (NX + 1) * sizeof(float) <= FEW_RING &&
+                    (MATS * FEW_ROWS + kFewProductRows) * 128 <= FEW_RING, "shared memory of two blocks exceeded");
+  const auto kernel = few_rows_kernel<KIND, NT>;
+  p.blocks = (o.inner * o.esz + 127) / 128;
+  // Rows of W in equal shares over two blocks a SM, in tiles of up to FEW_ROWS.
+  const int slots = 2 * num_sms(), share = ((p.outer + slots - 1) / slots + 7) / 8 * 8;
+  p.tiles = (share + FEW_ROWS - 1) / FEW_ROWS;
+  p.th = ((share + p.tiles - 1) / p.tiles + 7) / 8 * 8;
+  p.warps = (p.th + 15) / 16;
+  // Bytes of a stage and groups go by the weight alone (with the most rows of x that there may be), since what a group has, and with it the order of sums, does.
+  const int weight = MATS * p.th * 128;
+  p.sub = weight >= 4096 ? 1 : 2;
+  const int least = static_cast<int>(FEW_RING) / (p.sub * (weight + kFewProductRows * 128));
+  p.groups = p.tiles > 1 ? 1 : FEW_WARPS / p.warps < least ? FEW_WARPS / p.warps : least;
+  const int sub_bytes = weight + NX * 128;
+  p.kblocks = (p.blocks + p.sub - 1) / p.sub;
+  const int fit = static_cast<int>(FEW_RING) / (p.sub * sub_bytes);
+  p.stages = fit < FEW_STAGES ? fit : FEW_STAGES;
+  // (A stage is always the same group's: a group that met another's could be a whole round ahead of it, where a barrier's phases look alike.)
+  p.stages -= p.stages % p.groups;
+  p.status = status_word_ptr();
+  const long long group = static_cast<long long>(p.th) * p.tiles;
+  const CUtensorMap tx = few_map(o.x, p.rows, o, o.ld_x, NX), t0 = few_map(o.w0, p.outer, o, o.ld_w0, p.th), t1 = MATS == 2 ? few_map(o.w1, p.outer, o, o.ld_w1, p.th) : t0;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
   if (e == cudaSuccess) {
-    const int groups = (p.outer + 15) / 16, steps = (p.inner_bytes + 63) / 64;
-    int S = 1;                                         // blocks that share a group's inner dimension: about four a SM, of two steps a warp or more
-    while (S < 8 && groups * S < 3 * num_sms() && steps >= 2 * S * FEW_WARPS * 2) S *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(groups * S);
-    cfg.blockDim = dim3(FEW_WARPS * 32);
-    cfg.dynamicSmemBytes = SMEM;
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = S; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    kernel<<<static_cast<int>((p.outer + group - 1) / group), FEW_THREADS, SMEM, s>>>(tx, t0, t1, p);
+    e = cudaGetLastError();
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon product of few rows: launch failed: ") + cudaGetErrorString(e));
 }
-template <int KIND, int ACT = 0>
-void launch_rows(const FewDev& p, cudaStream_t s) {
-  if (p.rows <= 0 || p.rows > kFewProductRows || p.outer <= 0 || p.inner_bytes <= 0 || p.inner_bytes % 16) throw std::runtime_error("himuon product of few rows: bad sizes");
-  if (p.rows <= 8) launch<KIND, 1, ACT>(p, s);
-  else if (p.rows <= 16) launch<KIND, 2, ACT>(p, s);
-  else if (p.rows <= 32) launch<KIND, 4, ACT>(p, s);
-  else launch<KIND, 8, ACT>(p, s);
+template <int KIND>
+void launch_rows(const FewOperands& o, const FewDev& p, cudaStream_t s) {
+  if (p.rows <= 0 || p.rows > (KIND == EIGHT_BITS ? kFewFp8Rows : kFewProductRows) || p.outer <= 0 || o.inner <= 0) throw std::runtime_error("himuon product of few rows: bad sizes");
+  if (p.rows <= 8) launch<KIND, 1>(o, p, s);
+  else if (p.rows <= 16) launch<KIND, 2>(o, p, s);
+  else if (p.rows <= 32) launch<KIND, 4>(o, p, s);
+  else if constexpr (KIND != EIGHT_BITS) launch<KIND, 8>(o, p, s);
 }
 
 }  // namespace
 
 void few_rows_product(const void* x, long long ld_x, const void* w, long long ld_w, void* y, int rows, int inner, int outer, cudaStream_t s) {
+  FewOperands o;
+  o.x = x; o.ld_x = 2 * ld_x; o.w0 = w; o.ld_w0 = 2 * ld_w; o.inner = inner;
   FewDev p{};
-  p.x = static_cast<const uint8_t*>(x); p.ld_x = 2 * ld_x;
-  p.w0 = static_cast<const uint8_t*>(w); p.ld_w0 = 2 * ld_w;
-  p.y = y;
-  p.rows = rows; p.outer = outer; p.inner_bytes = 2 * inner;
-  launch_rows<PLAIN>(p, s);
+  p.y = y; p.rows = rows; p.outer = outer;
+  launch_rows<PLAIN>(o, p, s);
 }
 
 void few_rows_gated_up(const GatedUpArgs& a, cudaStream_t s) {
+  FewOperands o;
+  o.x = a.x; o.ld_x = 2 * a.ld_x; o.w0 = a.wg; o.ld_w0 = 2 * a.ld_wg; o.w1 = a.wu; o.ld_w1 = 2 * a.ld_wu; o.inner = a.hidden;
   FewDev p{};
-  p.x = static_cast<const uint8_t*>(a.x); p.ld_x = 2 * a.ld_x;
-  p.w0 = static_cast<const uint8_t*>(a.wg); p.ld_w0 = 2 * a.ld_wg;
-  p.w1 = static_cast<const uint8_t*>(a.wu); p.ld_w1 = 2 * a.ld_wu;
   p.y = a.h; p.gu = a.gu; p.gu_low = static_cast<uint8_t*>(a.gu_low);
-  p.rows = a.rows; p.outer = a.inter; p.inner_bytes = 2 * a.hidden;
-  switch (a.activation) {
-    case kSilu: return launch_rows<GATED, kSilu>(p, s);
-    case kGelu: return launch_rows<GATED, kGelu>(p, s);
-    case kGeluTanh: return launch_rows<GATED, kGeluTanh>(p, s);
-    case kRelu: return launch_rows<GATED, kRelu>(p, s);
-  }
-  throw std::runtime_error("himuon gated_mlp: unknown activation");
+  p.rows = a.rows; p.outer = a.inter; p.activation = a.activation;
+  if (a.activation < kSilu || a.activation > kRelu) throw std::runtime_error("himuon gated_mlp: unknown activation");
+  launch_rows<GATED>(o, p, s);
 }
 
 void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, cudaStream_t s) {
   if (a.cols != b.cols || b.block_rows != 128) throw std::runtime_error("himuon fp8_product: bad sizes");
+  FewOperands o;
+  o.x = a.values; o.ld_x = a.ld; o.w0 = b.values; o.ld_w0 = b.ld; o.inner = a.cols; o.esz = 1;
   FewDev p{};
-  p.x = static_cast<const uint8_t*>(a.values); p.ld_x = a.ld;
-  p.w0 = static_cast<const uint8_t*>(b.values); p.ld_w0 = b.ld;
   p.sx = a.scales; p.sx_row = a.scale_row; p.sx_col = a.scale_col; p.x_block = a.block_rows;
   p.sw = b.scales; p.sw_row = b.scale_row; p.sw_col = b.scale_col;
   p.y = c; p.out_fp32 = out_fp32;
-  p.rows = a.rows; p.outer = b.rows; p.inner_bytes = a.cols;
-  launch_rows<EIGHT_BITS>(p, s);
+  p.rows = a.rows; p.outer = b.rows;
+  launch_rows<EIGHT_BITS>(o, p, s);
 }
 
 }  // namespace himuon

@@ -32,7 +32,8 @@ void fp8_dequantize(const Fp8Matrix& m, void* out, long long ld_out, int out_fp3
 // c = a b^T, bf16 or fp32.  a has blocks of 1 or 128 rows, b of 128.  Rows of c are multiples of 16 bytes apart and written in whole groups of 16.
 // `powers`: all scales are powers of two (of normal numbers), as fp8_quantize() makes them.
 void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c, int out_fp32, int powers, cudaStream_t s);
-// The same for up to kFewProductRows rows of a (gated_mlp.h) and an inner dimension of multiples of 16; c is contiguous.
+// The same for a few rows of a; c is contiguous.  (33 to 64 rows have as many accumulators as a thread has registers: they are the large kernel's.)
+constexpr int kFewFp8Rows = 32;
 void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, cudaStream_t s);
 
 }  // namespace himuon

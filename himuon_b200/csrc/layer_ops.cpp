@@ -280,7 +280,7 @@ at::Tensor product(const char* op, Fp8 a, Fp8 b, bool out_fp32) {
   a.values = fp8_rows(a.values);
   b.values = fp8_rows(b.values);
   autograd_launched += 1;
-  if (rows <= himuon::kFewProductRows && inner % 16 == 0) {
+  if (rows <= himuon::kFewFp8Rows) {
     at::Tensor c = at::empty({rows, cols}, type);
     himuon::few_rows_fp8_product(fp8_matrix(a), fp8_matrix(b), c.data_ptr(), out_fp32, cur_stream());
     return c;
