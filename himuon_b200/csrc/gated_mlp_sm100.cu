@@ -8,8 +8,9 @@
 // h, dg and du are rounded to bf16: they are the operands of the next products, and each is off by at most 2^-8 of itself, as the results are.
 // Everything between two products is fp32.
 //
-// The main loop is the pair GEMM's (gemm2_sm100.cu has its protocol): six stages of 64 along the inner dimension, two accumulators of 256
-// columns, so that one tile's epilogue runs beside the products of the next.
+// The main loop is the pair GEMM's (gemm2_sm100.cu has its protocol): six stages of 64 along the inner dimension (five in DOWN_GRAD), two accumulators of 256
+// columns, so that one tile's epilogue runs beside the products of the next.  In DOWN_GRAD the epilogue's g and u come by TMA, a slab ahead, into the
+// shared memory that dg and du leave from: with loads by the threads, which have a row each, it took longer than the products (8192 x 2560 x 9728 482 us).
 #include "activations.cuh"
 #include "gated_mlp.h"
 #include "gemm_epilogue.cuh"
@@ -25,7 +26,8 @@ namespace himuon {
 namespace {
 
 constexpr int GM_THREADS = 384;      // warps 0-3: TMA, MMA, TMEM allocation, none; 4-11: epilogue, two groups of four
-constexpr int GM_STAGES = 6;
+constexpr int stages_of(int mode) { return mode == 0 ? 6 : 5; }
+constexpr int slabs_of(int mode) { return mode == 0 ? 1 : 2; }      // of each epilogue group
 // Registers of a thread at launch, and after the first four warps have given some to the others.
 constexpr int GM_REGS = 168, GM_REGS_FEW = 104, GM_REGS_EPILOGUE = 200;
 static_assert(GM_REGS_FEW + 2 * GM_REGS_EPILOGUE <= 3 * GM_REGS, "more registers than the block was launched with");
@@ -34,8 +36,7 @@ constexpr uint32_t GM_A = BM * BK * 2, GM_STAGE = 2 * GM_A;      // 128 rows of 
 enum { UP, DOWN_GRAD };
 
 struct GatedDev {
-  const uint16_t* gu;                  // DOWN_GRAD: g | u, upper bits
-  uint8_t* gu_low;                     // the bits below; UP: null where g and u are not wanted
+  uint8_t* gu_low;                     // the lower bits of g | u; UP: null where g and u are not wanted
   int rows, inter, low, tiles_m, tiles_n, kblocks;
   int* status;
 };
@@ -45,11 +46,13 @@ __device__ __forceinline__ void slab_free(int group, bool issuer) {
   if (issuer) tma_store_wait_read<0>();
   named_barrier(1 + 2 * group, 128);
 }
+// Columns 8 j to 8 j + 7 of a row.
+__device__ __forceinline__ uint4* slab_cell(uint8_t* slab, int row, int j) { return reinterpret_cast<uint4*>(slab + row * 128 + ((j ^ (row & 7)) << 4)); }
 // Columns 16 q to 16 q + 15 of a thread's row.
 __device__ __forceinline__ void put16(uint8_t* slab, int row, int q, const uint32_t (&o)[8]) {
 #pragma unroll
   for (int j = 0; j < 2; ++j)
-    *reinterpret_cast<uint4*>(slab + row * 128 + (((2 * q + j) ^ (row & 7)) << 4)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+    *slab_cell(slab, row, 2 * q + j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
 }
 __device__ __forceinline__ void slab_store(const CUtensorMap* tm, const uint8_t* slab, int group, int col, int row0, bool issuer) {
   fence_proxy_async_smem();
@@ -59,11 +62,6 @@ __device__ __forceinline__ void slab_store(const CUtensorMap* tm, const uint8_t*
     tma_store_commit();
   }
 }
-__device__ __forceinline__ void load16(const uint16_t* p, int valid, uint4 (&v)[2]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) v[j] = 8 * j < valid ? reinterpret_cast<const uint4*>(p)[j] : make_uint4(0, 0, 0, 0);
-}
-
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 // Two kept values from a word of upper bits and the word that has their lower ones (in its first or second half).
 __device__ __forceinline__ void from_kept(uint32_t upper, uint32_t low, int half, float& a, float& b) {
@@ -74,27 +72,30 @@ __device__ __forceinline__ void from_kept(uint32_t upper, uint32_t low, int half
 }  // namespace
 
 // tmA: rows of x or dy.  UP: tmB0 and tmB1 rows of Wg and Wu along the inner dimension, tmO h, tmG and tmU the halves of g | u.
-// DOWN_GRAD: tmB0 = tmB1 = Wd, its features along its rows; tmG and tmU the halves of dg | du.  (Halves have a map each: what a box has behind
-// the last feature of one must not go to the first of the other.)
+// DOWN_GRAD: tmB0 Wd, its features along its rows; tmO and tmB1 the halves of what is kept of g | u, tmG and tmU those of dg | du.  (Halves have a map each: what
+// a box has behind the last feature of one must not go to the first of the other.)
 template <int MODE, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GM_THREADS, 1)
 gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
                  const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmU, GatedDev p) {
   constexpr int FEATURES = MODE == UP ? 128 : 256;    // of a tile
+  constexpr int GM_STAGES = stages_of(MODE), SLABS = slabs_of(MODE);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_up_1024(smem_raw);
   uint8_t* slabs = smem + GM_STAGES * GM_STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(slabs + 2 * SLAB_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(slabs + 2 * SLABS * SLAB_BYTES);
   uint64_t* empty = full + GM_STAGES;
   uint64_t* tfull = empty + GM_STAGES;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* kept = tempty + 2;         // DOWN_GRAD: a slab's g and u are there, one for each epilogue group
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kept + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = warp_id(), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
+    for (int g = 0; g < 2; ++g) mbar_init(&kept[g], 1);
     for (int s = 0; s < GM_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 16); }     // eight epilogue warps in each CTA
     *abort_flag = 0;
@@ -113,7 +114,7 @@ gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
     const uint32_t e = elect_one();
-    const CUtensorMap* tmB = rank == 0 ? &tmB0 : &tmB1;
+    const CUtensorMap* tmB = MODE == DOWN_GRAD || rank == 0 ? &tmB0 : &tmB1;
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(tmB);
     int stage = 0;
@@ -177,10 +178,26 @@ gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int ew = warp & 3, group = (warp - 4) >> 2, row_in_tile = ew * 32 + lane;
     const uint32_t tempty_lead = map_to_cta(smem_u32(tempty), 0);
     const bool issuer = ew == 0 && lane == 0;
-    uint8_t* slab = slabs + group * SLAB_BYTES;
-    if (issuer) tma_prefetch_desc(MODE == UP ? &tmO : &tmG);
+    bool ok = true;
+    uint8_t* slab = slabs + group * SLABS * SLAB_BYTES;
+    if (issuer) tma_prefetch_desc(&tmO);
     int acc = 0;
-    uint32_t acc_phase = 0;
+    uint32_t acc_phase = 0, kept_phase = 0;
+    // DOWN_GRAD: has g and u of the group's next slab loaded, from columns c of a tile on (a tile may have none)
+    auto load_kept = [&](int tile, int c) {
+      int row, col;
+      for (;; tile += n_pairs, c = group * 64) {
+        if (tile >= total) return;
+        const int nt = tile / p.tiles_m;
+        row = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
+        col = nt * FEATURES + c;
+        if (c < 256 && row < p.rows && col < p.inter) break;
+      }
+      mbar_expect_tx(&kept[group], 2 * SLAB_BYTES);
+      tma_load_3d(slab, &tmO, &kept[group], col, row, 0);
+      tma_load_3d(slab + SLAB_BYTES, &tmB1, &kept[group], col, row, 0);
+    };
+    if (MODE == DOWN_GRAD && issuer) load_kept(first, group * 64);
     for (int tile = first; tile < total; tile += n_pairs) {
       const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
       const int n0 = nt * FEATURES;
@@ -232,46 +249,57 @@ gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
         } else {
-          const uint16_t* gu = p.gu + static_cast<long long>(m0 + row_in_tile) * 2 * p.inter;
           const uint8_t* low = p.gu_low + static_cast<long long>(m0 + row_in_tile) * 2 * p.low;
           const bool row_ok = m0 + row_in_tile < p.rows;
 #pragma unroll 1
           for (int c = group * 64; c < 256; c += 128) {
             const int col = n0 + c;
             if (col >= p.inter) break;                // uniform over the group
-            uint32_t du[4][8];
-            slab_free(group, issuer);
+            uint4 gl[4], ul[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const bool in = row_ok && col + q * 16 < p.inter;
+              gl[q] = in ? *reinterpret_cast<const uint4*>(low + col + q * 16) : make_uint4(0, 0, 0, 0);
+              ul[q] = in ? *reinterpret_cast<const uint4*>(low + p.low + col + q * 16) : make_uint4(0, 0, 0, 0);
+            }
+            if (!named_barrier_and(1 + 2 * group, 128, mbar_wait(&kept[group], kept_phase, abort_flag, p.status, 3))) { ok = false; break; }
+            kept_phase ^= 1;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               uint4 gv[2], uv[2];
-              const int valid = row_ok ? p.inter - col - q * 16 : 0;
-              load16(gu + col + q * 16, valid, gv);
-              load16(gu + p.inter + col + q * 16, valid, uv);
-              const uint4 none = make_uint4(0, 0, 0, 0);
-              const uint4 gl = valid > 0 ? *reinterpret_cast<const uint4*>(low + col + q * 16) : none;
-              const uint4 ul = valid > 0 ? *reinterpret_cast<const uint4*>(low + p.low + col + q * 16) : none;
-              uint32_t d[16], dg[8];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                gv[j] = *slab_cell(slab, row_in_tile, 2 * q + j);
+                uv[j] = *slab_cell(slab + SLAB_BYTES, row_in_tile, 2 * q + j);
+              }
+              uint32_t d[16], dg[8], du[8];
               tmem_ld16(t_acc + c + q * 16, d);
               tmem_ld_wait();
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 float g0, g1, u0, u1, a0, a1, s0, s1;
-                from_kept(word(gv[j / 4], j & 3), word(gl, j / 2), j & 1, g0, g1);
-                from_kept(word(uv[j / 4], j & 3), word(ul, j / 2), j & 1, u0, u1);
+                from_kept(word(gv[j / 4], j & 3), word(gl[q], j / 2), j & 1, g0, g1);
+                from_kept(word(uv[j / 4], j & 3), word(ul[q], j / 2), j & 1, u0, u1);
                 activate_grad<ACT>(g0, a0, s0);
                 activate_grad<ACT>(g1, a1, s1);
                 const float d0 = __uint_as_float(d[2 * j]), d1 = __uint_as_float(d[2 * j + 1]);
                 dg[j] = pack_bf16x2(d0 * u0 * s0, d1 * u1 * s1);
-                du[q][j] = pack_bf16x2(d0 * a0, d1 * a1);
+                du[j] = pack_bf16x2(d0 * a0, d1 * a1);
               }
               put16(slab, row_in_tile, q, dg);
+              put16(slab + SLAB_BYTES, row_in_tile, q, du);
             }
-            slab_store(&tmG, slab, group, col, m0, issuer);
-            slab_free(group, issuer);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) put16(slab, row_in_tile, q, du[q]);
-            slab_store(&tmU, slab, group, col, m0, issuer);
+            fence_proxy_async_smem();
+            named_barrier(2 + 2 * group, 128);        // both slabs are complete
+            if (issuer) {
+              tma_store_3d(&tmG, slab, col, m0, 0);
+              tma_store_3d(&tmU, slab + SLAB_BYTES, col, m0, 0);
+              tma_store_commit();
+              tma_store_wait_read<0>();
+              load_kept(tile, c + 128);
+            }
           }
+          if (!ok) break;
         }
       }
       tc_fence_before();
@@ -329,7 +357,7 @@ static int pairs_at_once(Kernel kernel, size_t smem, std::atomic<int>* most) {
 template <int MODE, int ACT>
 static void launch(const CUtensorMap& a, const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& o, const CUtensorMap& g, const CUtensorMap& u,
                    GatedDev p, int inner, cudaStream_t s) {
-  constexpr size_t SMEM = 1024 + GM_STAGES * GM_STAGE + 2 * SLAB_BYTES + 256;
+  constexpr size_t SMEM = 1024 + stages_of(MODE) * GM_STAGE + 2 * slabs_of(MODE) * SLAB_BYTES + 256;
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
   static std::atomic<int> most[64] = {};
   const auto kernel = gated_mlp_kernel<MODE, ACT>;
@@ -377,14 +405,13 @@ void gated_down_grad(const GatedDownGradArgs& a, cudaStream_t s) {
   if (a.rows <= 0 || a.inter <= 0 || a.hidden <= 0 || a.hidden % 8 || a.inter % 8) throw std::runtime_error("himuon gated_mlp: bad sizes");
   const long long ld = 2LL * a.inter;
   GatedDev p{};
-  p.gu = static_cast<const uint16_t*>(a.gu);
   p.gu_low = static_cast<uint8_t*>(const_cast<void*>(a.gu_low));
   p.rows = a.rows;
   p.inter = a.inter;
   p.low = gated_low(a.inter);
   const CUtensorMap w = rows_map(a.wd, a.hidden, a.inter, a.ld_wd, BK), g = rows_map(a.dgu, a.rows, a.inter, ld, BM);
-  launch_activation<DOWN_GRAD>(a.activation, rows_map(a.dy, a.rows, a.hidden, a.ld_dy, BM), w, w, g, g,
-                               rows_map(static_cast<char*>(a.dgu) + 2LL * a.inter, a.rows, a.inter, ld, BM), p, a.hidden, s);
+  launch_activation<DOWN_GRAD>(a.activation, rows_map(a.dy, a.rows, a.hidden, a.ld_dy, BM), w, rows_map(static_cast<const char*>(a.gu) + 2LL * a.inter, a.rows, a.inter, ld, BM),
+                               rows_map(a.gu, a.rows, a.inter, ld, BM), g, rows_map(static_cast<char*>(a.dgu) + 2LL * a.inter, a.rows, a.inter, ld, BM), p, a.hidden, s);
 }
 
 }  // namespace himuon
