@@ -183,21 +183,39 @@ gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     if (issuer) tma_prefetch_desc(&tmO);
     int acc = 0;
     uint32_t acc_phase = 0, kept_phase = 0;
-    // DOWN_GRAD: has g and u of the group's next slab loaded, from columns c of a tile on (a tile may have none)
-    auto load_kept = [&](int tile, int c) {
-      int row, col;
-      for (;; tile += n_pairs, c = group * 64) {
-        if (tile >= total) return;
+    // DOWN_GRAD: the group's next slab, from columns c of a tile on (a tile may have none), and its g and u, which are on their way a slab ahead
+    auto next_slab = [&](int tile, int c, int& row, int& col) {
+      for (; tile < total; tile += n_pairs, c = group * 64) {
         const int nt = tile / p.tiles_m;
         row = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
         col = nt * FEATURES + c;
-        if (c < 256 && row < p.rows && col < p.inter) break;
+        if (c < 256 && row < p.rows && col < p.inter) return true;
       }
+      return false;
+    };
+    uint4 gl[4], ul[4];
+    auto load_low = [&](int tile, int c) {
+      int row, col;
+      const bool there = next_slab(tile, c, row, col) && row + row_in_tile < p.rows;
+      const uint8_t* low = p.gu_low + static_cast<long long>(there ? row + row_in_tile : 0) * 2 * p.low + (there ? col : 0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool in = there && col + q * 16 < p.inter;
+        gl[q] = in ? *reinterpret_cast<const uint4*>(low + q * 16) : make_uint4(0, 0, 0, 0);
+        ul[q] = in ? *reinterpret_cast<const uint4*>(low + p.low + q * 16) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto load_kept = [&](int tile, int c) {
+      int row, col;
+      if (!next_slab(tile, c, row, col)) return;
       mbar_expect_tx(&kept[group], 2 * SLAB_BYTES);
       tma_load_3d(slab, &tmO, &kept[group], col, row, 0);
       tma_load_3d(slab + SLAB_BYTES, &tmB1, &kept[group], col, row, 0);
     };
-    if (MODE == DOWN_GRAD && issuer) load_kept(first, group * 64);
+    if constexpr (MODE == DOWN_GRAD) {
+      if (issuer) load_kept(first, group * 64);
+      load_low(first, group * 64);
+    }
     for (int tile = first; tile < total; tile += n_pairs) {
       const int nt = tile / p.tiles_m, m0 = (tile - nt * p.tiles_m) * 2 * BM + static_cast<int>(rank) * BM;
       const int n0 = nt * FEATURES;
@@ -249,19 +267,10 @@ gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             }
           }
         } else {
-          const uint8_t* low = p.gu_low + static_cast<long long>(m0 + row_in_tile) * 2 * p.low;
-          const bool row_ok = m0 + row_in_tile < p.rows;
 #pragma unroll 1
           for (int c = group * 64; c < 256; c += 128) {
             const int col = n0 + c;
             if (col >= p.inter) break;                // uniform over the group
-            uint4 gl[4], ul[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const bool in = row_ok && col + q * 16 < p.inter;
-              gl[q] = in ? *reinterpret_cast<const uint4*>(low + col + q * 16) : make_uint4(0, 0, 0, 0);
-              ul[q] = in ? *reinterpret_cast<const uint4*>(low + p.low + col + q * 16) : make_uint4(0, 0, 0, 0);
-            }
             if (!named_barrier_and(1 + 2 * group, 128, mbar_wait(&kept[group], kept_phase, abort_flag, p.status, 3))) { ok = false; break; }
             kept_phase ^= 1;
 #pragma unroll
@@ -289,6 +298,7 @@ gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               put16(slab, row_in_tile, q, dg);
               put16(slab + SLAB_BYTES, row_in_tile, q, du);
             }
+            load_low(tile, c + 128);
             fence_proxy_async_smem();
             named_barrier(2 + 2 * group, 128);        // both slabs are complete
             if (issuer) {

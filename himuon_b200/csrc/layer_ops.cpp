@@ -66,12 +66,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
                             int64_t rotary_dim, bool interleaved, double cos_factor, double sin_factor) {
     if (positions.has_value()) ctx->save_for_backward({turns, *positions});
     else ctx->save_for_backward({turns});
-    ctx->saved_data["seq_len"] = seq_len;
-    ctx->saved_data["heads"] = heads;
-    ctx->saved_data["rotary_dim"] = rotary_dim;
-    ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["cos_factor"] = cos_factor;
-    ctx->saved_data["sin_factor"] = sin_factor;
+    ctx->saved_data["sizes"] = std::vector<int64_t>{seq_len, heads, rotary_dim, interleaved};
+    ctx->saved_data["factors"] = std::vector<double>{cos_factor, sin_factor};
     return rotate(x, positions, turns, seq_len, heads, rotary_dim, interleaved, cos_factor, sin_factor);
   }
 
@@ -81,9 +77,11 @@ struct Rotary : torch::autograd::Function<Rotary> {
     at::Tensor dy = grads[0];
     if (dy.stride(1) != 1 && dy.size(1) > 1) dy = dy.contiguous();
     variable_list out(9);
-    out[0] = apply(dy, saved.size() > 1 ? c10::optional<at::Tensor>(saved[1]) : c10::nullopt, saved[0], ctx->saved_data["seq_len"].toInt(), ctx->saved_data["heads"].toInt(),
-                   ctx->saved_data["rotary_dim"].toInt(), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["cos_factor"].toDouble(),
-                   -ctx->saved_data["sin_factor"].toDouble());
+    const c10::optional<at::Tensor> positions = saved.size() > 1 ? c10::optional<at::Tensor>(saved[1]) : c10::nullopt;
+    const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();
+    const std::vector<double> f = ctx->saved_data["factors"].toDoubleVector();
+    out[0] = c10::GradMode::is_enabled() ? apply(dy, positions, saved[0], n[0], n[1], n[2], n[3] != 0, f[0], -f[1])
+                                         : rotate(dy, positions, saved[0], n[0], n[1], n[2], n[3] != 0, f[0], -f[1]);
     return out;
   }
 };

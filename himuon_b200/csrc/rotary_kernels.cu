@@ -6,8 +6,10 @@
 // number of 2^-64 turns a position, so that pos * f modulo 2^64 is the angle's place within its turn, exact to pos * 2^-65 of a turn at any
 // position, with no table to make, keep or read.  Its upper 32 bits go to sincospif.
 //
-// Bounded by memory: every value is read and written once.  A thread takes two vectors of 16 bytes of a head (a's and b's of the same pairs,
-// or two that pass through), works out their sines once and keeps them for all the heads that it goes through.
+// Bounded by memory: every value is read and written once.  A block has some rows, of all heads or of a share of them.  Its threads ask for their first
+// values, work out a sine and cosine each while those are on their way, and leave them in shared memory for all the heads; then they take pairs of vectors of 16
+// bytes (a's and b's of the same pairs, or two that pass through), two pairs at a time.  With every thread working out the eight sines of its own vectors, for a
+// quarter of the heads: 4071 rows of 20 heads of 64 7.1 us.
 #include "rotary.h"
 
 #include <algorithm>
@@ -19,10 +21,13 @@ namespace himuon {
 
 namespace {
 
+constexpr int ROT_WAVES = 1024;      // sines and cosines that a block has room for
+
 struct RotaryDev {
   RotaryArgs a;
   int units;                 // pairs of vectors in a head
-  int lanes;                 // heads that neighbouring threads take, of the `heads`
+  int rows, heads;           // of a block
+  int lanes;                 // rotary_any_kernel: heads that neighbouring threads take, of the `heads`
   long long threads;         // rows * lanes * units
 };
 
@@ -65,67 +70,79 @@ template <> struct Vec<float> {
 // Whole vectors: heads of whole vectors, rows on 16-byte boundaries, and no vector with both halves of a pair unless interleaved.
 template <typename T, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_vec_kernel(RotaryDev p) {
-  constexpr int N = Vec<T>::N;
+  constexpr int N = Vec<T>::N, BATCH = 2;
+  __shared__ float2 s_wave[ROT_WAVES];
   const RotaryArgs& a = p.a;
-  const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (id >= p.threads) return;
-  const int unit = static_cast<int>(id % p.units);
-  const long long rest = id / p.units;
-  const int first = static_cast<int>(rest % p.lanes);
-  const long long row = rest / p.lanes;
-  // the unit's two vectors, and whether they are turned
-  const int vecs = a.head_dim / N, turned = a.rotary_dim / N;
-  int v0, v1;
-  bool r0, r1;
-  if (INTERLEAVED) {
-    v0 = unit; v1 = unit + p.units;
-    r0 = v0 < turned; r1 = v1 < turned;
-  } else if (unit < turned / 2) {
-    v0 = unit; v1 = unit + turned / 2;
-    r0 = r1 = true;
-  } else {
-    const int half = (vecs - turned + 1) / 2;
-    v0 = unit - turned / 2 + turned; v1 = v0 + half;
-    r0 = r1 = false;
-  }
-  const bool second = v1 < vecs;
-  constexpr int W = N;                                   // waves of a thread: N pairs, or two times N / 2
-  float2 w[W];
-  if (r0) {
-    const long long pos = position(a, row);
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      int pair = v0 * N + i;
-      if (INTERLEAVED) pair = (i < N / 2 ? v0 * N / 2 + i : v1 * N / 2 + i - N / 2);
-      w[i] = !INTERLEAVED || i < N / 2 || r1 ? wave(a, pos, pair) : make_float2(1.f, 0.f);
+  const int vecs = a.head_dim / N, turned = a.rotary_dim / N, pairs = a.rotary_dim / 2;
+  const long long row0 = static_cast<long long>(blockIdx.x) * p.rows;
+  const int h0 = static_cast<int>(blockIdx.y) * p.heads, nh = min(p.heads, a.heads - h0), nr = static_cast<int>(min(static_cast<long long>(p.rows), a.rows - row0));
+  const int items = nr * nh * p.units;
+  struct Item {
+    uint4 q0, q1;
+    long long to;            // of the head, in the result
+    int v0, v1, row;         // its two vectors, and the row
+    bool there, second, turn0, turn1;
+  };
+  auto fetch = [&](int i, Item& it) {
+    it.there = i < items;
+    if (!it.there) return;
+    const int unit = i % p.units, rest = i / p.units, h = h0 + rest % nh;
+    it.row = rest / nh;
+    if (INTERLEAVED) {
+      it.v0 = unit; it.v1 = unit + p.units;
+      it.turn0 = it.v0 < turned; it.turn1 = it.v1 < turned;
+    } else if (unit < turned / 2) {
+      it.v0 = unit; it.v1 = unit + turned / 2;
+      it.turn0 = it.turn1 = true;
+    } else {
+      it.v0 = unit + turned / 2; it.v1 = it.v0 + (vecs - turned + 1) / 2;
+      it.turn0 = it.turn1 = false;
     }
-  }
-  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld_x;
-  T* y = reinterpret_cast<T*>(a.y) + row * a.ld_y;
-#pragma unroll 4
-  for (int h = first; h < a.heads; h += p.lanes) {
-    const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<long long>(h) * a.head_dim);
-    uint4* dst = reinterpret_cast<uint4*>(y + static_cast<long long>(h) * a.head_dim);
-    uint4 q0 = src[v0], q1 = second ? src[v1] : make_uint4(0, 0, 0, 0);
-    if (r0) {
+    it.second = it.v1 < vecs;
+    it.to = (row0 + it.row) * a.ld_y + static_cast<long long>(h) * a.head_dim;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + (row0 + it.row) * a.ld_x + static_cast<long long>(h) * a.head_dim);
+    it.q0 = src[it.v0];
+    it.q1 = it.second ? src[it.v1] : make_uint4(0, 0, 0, 0);
+  };
+  auto finish = [&](Item& it) {
+    if (!it.there) return;
+    if (it.turn0) {
+      const float2* w = s_wave + it.row * pairs;
       float f0[N], f1[N];
-      Vec<T>::get(q0, f0);
-      Vec<T>::get(q1, f1);
+      Vec<T>::get(it.q0, f0);
+      Vec<T>::get(it.q1, f1);
       if (INTERLEAVED) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-          turn(w[i], f0[2 * i], f0[2 * i + 1]);
-          turn(w[i + N / 2], f1[2 * i], f1[2 * i + 1]);
+          turn(w[it.v0 * (N / 2) + i], f0[2 * i], f0[2 * i + 1]);
+          if (it.turn1) turn(w[it.v1 * (N / 2) + i], f1[2 * i], f1[2 * i + 1]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) turn(w[i], f0[i], f1[i]);
+        for (int i = 0; i < N; ++i) turn(w[it.v0 * N + i], f0[i], f1[i]);
       }
-      q0 = Vec<T>::put(f0);
-      if (!INTERLEAVED || r1) q1 = Vec<T>::put(f1);       // (what passes through keeps its bits)
+      it.q0 = Vec<T>::put(f0);
+      if (!INTERLEAVED || it.turn1) it.q1 = Vec<T>::put(f1);       // (what passes through keeps its bits)
     }
-    dst[v0] = q0;
-    if (second) dst[v1] = q1;
+    uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.y) + it.to);
+    dst[it.v0] = it.q0;
+    if (it.second) dst[it.v1] = it.q1;
+  };
+  Item batch[BATCH];
+#pragma unroll
+  for (int b = 0; b < BATCH; ++b) fetch(threadIdx.x + b * 256, batch[b]);
+  for (int i = threadIdx.x; i < nr * pairs; i += 256) {
+    const int r = i / pairs;
+    s_wave[i] = wave(a, position(a, row0 + r), i - r * pairs);
+  }
+  __syncthreads();
+  for (int at = threadIdx.x;; ) {
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) finish(batch[b]);
+    at += BATCH * 256;
+    if (at >= items) break;
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) fetch(at + b * 256, batch[b]);
   }
 }
 
@@ -168,19 +185,29 @@ template <typename T>
 void launch(const RotaryArgs& a, cudaStream_t s) {
   constexpr int N = Vec<T>::N;
   auto grid16 = [](const void* p, long long ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % N == 0; };
-  const bool whole = a.head_dim % N == 0 && a.rotary_dim % (a.interleaved ? N : 2 * N) == 0 && a.rotary_dim > 0 && grid16(a.x, a.ld_x) && grid16(a.y, a.ld_y);
+  const bool whole = a.head_dim % N == 0 && a.rotary_dim % (a.interleaved ? N : 2 * N) == 0 && a.rotary_dim / 2 <= ROT_WAVES && grid16(a.x, a.ld_x) && grid16(a.y, a.ld_y);
   RotaryDev p{};
   p.a = a;
-  const int vecs = a.head_dim / N;
-  p.units = whole ? (vecs + 1) / 2 : a.head_dim - a.rotary_dim / 2;
-  p.lanes = std::min(a.heads, 4);
-  p.threads = a.rows * p.lanes * p.units;
-  const long long blocks = (p.threads + 255) / 256;
-  if (blocks >= (1LL << 31)) throw std::runtime_error("himuon rotary: too many rows for one launch");
-  const int grid = static_cast<int>(blocks);
-  if (!whole) rotary_any_kernel<T><<<grid, 256, 0, s>>>(p);
-  else if (a.interleaved) rotary_vec_kernel<T, true><<<grid, 256, 0, s>>>(p);
-  else rotary_vec_kernel<T, false><<<grid, 256, 0, s>>>(p);
+  if (whole) {
+    const int pairs = std::max(a.rotary_dim / 2, 1);
+    p.units = (a.head_dim / N + 1) / 2;
+    // as many rows as there are sines for the threads, but four blocks a SM, if need be with a share of the heads each
+    const long long want = 4LL * num_sms();
+    p.rows = static_cast<int>(std::max(1LL, std::min<long long>(256 / pairs, a.rows / want)));
+    const long long blocks = (a.rows + p.rows - 1) / p.rows, shares = std::max(1LL, std::min<long long>(want / blocks, a.heads * p.units / 64));
+    p.heads = static_cast<int>((a.heads + shares - 1) / shares);
+    if (blocks >= (1LL << 31)) throw std::runtime_error("himuon rotary: too many rows for one launch");
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((a.heads + p.heads - 1) / p.heads));
+    if (a.interleaved) rotary_vec_kernel<T, true><<<grid, 256, 0, s>>>(p);
+    else rotary_vec_kernel<T, false><<<grid, 256, 0, s>>>(p);
+  } else {
+    p.units = a.head_dim - a.rotary_dim / 2;
+    p.lanes = std::min(a.heads, 4);
+    p.threads = a.rows * p.lanes * p.units;
+    const long long blocks = (p.threads + 255) / 256;
+    if (blocks >= (1LL << 31)) throw std::runtime_error("himuon rotary: too many rows for one launch");
+    rotary_any_kernel<T><<<static_cast<int>(blocks), 256, 0, s>>>(p);
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon rotary launch failed: ") + cudaGetErrorString(e));
 }
