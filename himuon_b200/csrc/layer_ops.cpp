@@ -92,7 +92,13 @@ void check_rows(const char* op, const char* name, const at::Tensor& t, const at:
                   t.stride(0) % 8 == 0 && (rows <= 1 || t.stride(0) >= cols) && aligned16(t),
               std::string("himuon: ") + op + ": " + name + " must be (" + std::to_string(rows) + ", " + std::to_string(cols) + ") bf16, its rows on 16-byte boundaries with unit inner stride");
 }
-// The same, for a gradient: copied where it lies otherwise.
+// Rows of all dimensions but the last.
+int64_t flat_rows(const at::Tensor& t) {
+  int64_t n = 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
+  return n;
+}
+// Rows as check_rows() wants them: copied where they lie otherwise.
 at::Tensor with_rows(const at::Tensor& t) {
   if (t.stride(1) == 1 && t.stride(0) % 8 == 0 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) && aligned16(t)) return t;
   return t.clone(at::MemoryFormat::Contiguous);
@@ -200,26 +206,42 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
 };
 
 // ------------------------------------------------------------------------------------------------ 8 bits
-struct Fp8 { at::Tensor values, scales; int64_t block_rows = 1; bool powers = false; };      // powers: scales known to be powers of two
-
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to; }
 
-// Room for (rows, cols) values, their rows padded to 16 bytes, and their scales: of rows along rows, which is how a product reads them.
-Fp8 fp8_empty(const at::Tensor& like, int64_t rows, int64_t cols, int64_t block_rows) {
-  Fp8 m;
-  m.block_rows = block_rows;
-  m.powers = true;                                       // (that is what it will be filled with)
-  m.values = at::empty({rows, up(cols, 16) * 16}, like.options().dtype(at::kFloat8_e4m3fn)).narrow(1, 0, cols);
-  const auto fp32 = like.options().dtype(at::kFloat);
-  m.scales = block_rows == 1 ? at::empty({up(cols, 128), rows}, fp32).t() : at::empty({up(rows, 128), up(cols, 128)}, fp32);
-  return m;
+// A matrix in 8 bits and what holds its memory.  `powers`: its scales are known to be powers of two.
+struct Fp8 {
+  himuon::Fp8Matrix m;
+  bool powers = false;
+  at::Tensor values, scales;             // or all in `values`
+};
+
+// Where values, with rows padded to 16 bytes, and scales of a matrix lie in one piece of memory; scales of rows one behind the other, which is how a
+// product reads them.
+int64_t fp8_scales_at(int64_t rows, int64_t cols) { return rows * up(cols, 16) * 16; }
+int64_t fp8_scale_count(int64_t rows, int64_t cols, int64_t block_rows) { return up(rows, block_rows) * up(cols, 128); }
+Fp8 fp8_in(const at::Tensor& piece, int64_t rows, int64_t cols, int64_t block_rows) {
+  Fp8 q;
+  char* at = static_cast<char*>(piece.data_ptr());
+  q.m.values = at;
+  q.m.scales = reinterpret_cast<float*>(at + fp8_scales_at(rows, cols));
+  q.m.ld = up(cols, 16) * 16;
+  q.m.scale_row = block_rows == 1 ? 1 : up(cols, 128);
+  q.m.scale_col = block_rows == 1 ? rows : 1;
+  q.m.rows = static_cast<int>(rows); q.m.cols = static_cast<int>(cols); q.m.block_rows = static_cast<int>(block_rows);
+  q.powers = true;                       // (that is what it will be filled with)
+  q.values = piece;
+  return q;
 }
-himuon::Fp8Out fp8_out(const Fp8& m) {
+Fp8 fp8_piece(const at::Tensor& like, int64_t rows, int64_t cols, int64_t block_rows) {
+  HM_CHECK(rows < (1LL << 30) && cols < (1LL << 30), "a matrix in 8 bits is too large");
+  return fp8_in(at::empty({fp8_scales_at(rows, cols) + 4 * fp8_scale_count(rows, cols, block_rows)}, like.options().dtype(at::kByte)), rows, cols, block_rows);
+}
+himuon::Fp8Out fp8_out(const himuon::Fp8Matrix& m) {
   himuon::Fp8Out o;
-  o.values = m.values.data_ptr();
-  o.scales = m.scales.data_ptr<float>();
-  o.ld = m.values.stride(0); o.scale_row = m.scales.stride(0); o.scale_col = m.scales.stride(1);
-  o.block_rows = static_cast<int>(m.block_rows);
+  o.values = const_cast<void*>(m.values);
+  o.scales = const_cast<float*>(m.scales);
+  o.ld = m.ld; o.scale_row = m.scale_row; o.scale_col = m.scale_col;
+  o.block_rows = m.block_rows;
   return o;
 }
 // Fills the copies that are given.
@@ -230,77 +252,89 @@ void quantize(const at::Tensor& x, const Fp8* straight, const Fp8* turned) {
   const c10::cuda::CUDAGuard guard(x.device());
   himuon::Fp8QuantizeArgs a;
   a.x = x.data_ptr(); a.rows = x.size(0); a.cols = x.size(1); a.ld = x.stride(0); a.fp32 = x.scalar_type() == at::kFloat;
-  if (straight) a.straight = fp8_out(*straight);
-  if (turned) a.turned = fp8_out(*turned);
+  if (straight) a.straight = fp8_out(straight->m);
+  if (turned) a.turned = fp8_out(turned->m);
   himuon::fp8_quantize(a, cur_stream());
   autograd_launched += 1;
 }
-std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor& x, int64_t block_rows, bool transpose) {
-  HM_CHECK(x.dim() == 2 && (block_rows == 1 || block_rows == 128), "quantize_fp8: a matrix and blocks of 1 or 128 rows expected");
-  const Fp8 m = transpose ? fp8_empty(x, x.size(1), x.size(0), block_rows) : fp8_empty(x, x.size(0), x.size(1), block_rows);
-  quantize(x, transpose ? nullptr : &m, transpose ? &m : nullptr);
-  return {m.values, m.scales};
+// Rows with unit inner stride that share no memory: copied where they lie otherwise.
+at::Tensor apart(const at::Tensor& t) {
+  if ((t.stride(1) == 1 || t.size(1) <= 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1))) return t;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+std::tuple<at::Tensor, at::Tensor> quantize_fp8(const at::Tensor& given, int64_t block_rows, bool transpose) {
+  HM_CHECK(given.dim() == 2 && (block_rows == 1 || block_rows == 128), "quantize_fp8: a matrix and blocks of 1 or 128 rows expected");
+  const at::Tensor x = apart(given);
+  const int64_t rows = transpose ? x.size(1) : x.size(0), cols = transpose ? x.size(0) : x.size(1), ld = up(cols, 16) * 16;
+  HM_CHECK(rows < (1LL << 30) && cols < (1LL << 30), "quantize_fp8: matrix too large");
+  const auto fp32 = x.options().dtype(at::kFloat);
+  const std::vector<int64_t> blocks = {up(rows, block_rows), up(cols, 128)};
+  at::Tensor values = at::empty({rows, ld}, x.options().dtype(at::kFloat8_e4m3fn));
+  const at::Tensor scales = block_rows == 1 ? at::empty_strided(blocks, {1, std::max<int64_t>(rows, 1)}, fp32) : at::empty(blocks, fp32);
+  Fp8 q;
+  q.m.values = values.data_ptr(); q.m.scales = scales.data_ptr<float>();
+  q.m.ld = ld; q.m.scale_row = scales.stride(0); q.m.scale_col = scales.stride(1);
+  q.m.block_rows = static_cast<int>(block_rows);
+  quantize(x, transpose ? nullptr : &q, transpose ? &q : nullptr);
+  return {ld == cols ? values : values.narrow(1, 0, cols), scales};
 }
 
-void check_fp8(const char* op, const Fp8& m, const at::Device& device) {
-  TORCH_CHECK((m.block_rows == 1 || m.block_rows == 128) && m.values.device() == device && m.values.is_cuda() && m.values.scalar_type() == at::kFloat8_e4m3fn && m.values.dim() == 2 &&
-                  m.values.size(0) < (1LL << 30) && m.values.size(1) < (1LL << 30),
+// A matrix as a caller has it, checked.  `rows16`: with its rows on 16-byte boundaries, each with memory of its own; copied where they lie otherwise.
+Fp8 fp8_given(const char* op, const at::Tensor& values, const at::Tensor& scales, int64_t block_rows, bool powers, const at::Device& device, bool rows16) {
+  TORCH_CHECK((block_rows == 1 || block_rows == 128) && values.device() == device && values.is_cuda() && values.scalar_type() == at::kFloat8_e4m3fn && values.dim() == 2 &&
+                  values.size(0) < (1LL << 30) && values.size(1) < (1LL << 30),
               std::string("himuon: ") + op + ": a float8_e4m3fn matrix on " + device.str() + " with blocks of 1 or 128 rows expected");
-  TORCH_CHECK(m.scales.device() == device && m.scales.scalar_type() == at::kFloat && m.scales.dim() == 2 && m.scales.size(0) == up(m.values.size(0), m.block_rows) &&
-                  m.scales.size(1) == up(m.values.size(1), 128),
-              std::string("himuon: ") + op + ": scales must be fp32, one for each block of (" + std::to_string(m.block_rows) + ", 128) values");
-}
-// Rows on 16-byte boundaries, each with memory of its own; copied where they lie otherwise.
-at::Tensor fp8_rows(const at::Tensor& v) {
-  if (v.stride(1) == 1 && v.stride(0) % 16 == 0 && (v.size(0) <= 1 || v.stride(0) >= v.size(1)) && aligned16(v)) return v;
-  at::Tensor to = at::empty({v.size(0), up(v.size(1), 16) * 16}, v.options()).narrow(1, 0, v.size(1));
-  to.copy_(v);
-  return to;
-}
-himuon::Fp8Matrix fp8_matrix(const Fp8& m) {
-  himuon::Fp8Matrix a;
-  a.values = m.values.data_ptr(); a.scales = m.scales.data_ptr<float>();
-  a.ld = m.values.stride(0); a.scale_row = m.scales.stride(0); a.scale_col = m.scales.stride(1);
-  a.rows = static_cast<int>(m.values.size(0)); a.cols = static_cast<int>(m.values.size(1)); a.block_rows = static_cast<int>(m.block_rows);
-  return a;
+  TORCH_CHECK(scales.device() == device && scales.scalar_type() == at::kFloat && scales.dim() == 2 && scales.size(0) == up(values.size(0), block_rows) &&
+                  scales.size(1) == up(values.size(1), 128),
+              std::string("himuon: ") + op + ": scales must be fp32, one for each block of (" + std::to_string(block_rows) + ", 128) values");
+  Fp8 q;
+  q.values = values;
+  const bool unit = values.stride(1) == 1 || (!rows16 && values.size(1) <= 1);
+  if (rows16 && !(unit && values.stride(0) % 16 == 0 && (values.size(0) <= 1 || values.stride(0) >= values.size(1)) && aligned16(values))) {
+    q.values = at::empty({values.size(0), up(values.size(1), 16) * 16}, values.options()).narrow(1, 0, values.size(1));
+    q.values.copy_(values);
+  } else if (!unit) {
+    q.values = values.contiguous();
+  }
+  q.scales = scales;
+  q.powers = powers;
+  q.m.values = q.values.data_ptr(); q.m.scales = scales.data_ptr<float>();
+  q.m.ld = q.values.stride(0); q.m.scale_row = scales.stride(0); q.m.scale_col = scales.stride(1);
+  q.m.rows = static_cast<int>(values.size(0)); q.m.cols = static_cast<int>(values.size(1)); q.m.block_rows = static_cast<int>(block_rows);
+  return q;
 }
 // a b^T in bf16 or fp32.
-at::Tensor product(const char* op, Fp8 a, Fp8 b, bool out_fp32) {
-  check_fp8(op, a, a.values.device());
-  check_fp8(op, b, a.values.device());
-  TORCH_CHECK(a.values.size(1) == b.values.size(1), "himuon: ", op, ": inner dimensions disagree");
-  TORCH_CHECK(b.block_rows == 128, "himuon: ", op, ": the second operand needs blocks of 128 rows");
+at::Tensor product(const char* op, const Fp8& a, const Fp8& b, bool out_fp32) {
+  TORCH_CHECK(a.m.cols == b.m.cols, "himuon: ", op, ": inner dimensions disagree");
+  TORCH_CHECK(b.m.block_rows == 128, "himuon: ", op, ": the second operand needs blocks of 128 rows");
   const c10::cuda::CUDAGuard guard(a.values.device());
-  const int64_t rows = a.values.size(0), cols = b.values.size(0), inner = a.values.size(1);
+  const int64_t rows = a.m.rows, cols = b.m.rows;
   const auto type = a.values.options().dtype(out_fp32 ? at::kFloat : at::kBFloat16);
   if (!rows || !cols) return at::empty({rows, cols}, type);
-  if (!inner) return at::zeros({rows, cols}, type);
-  a.values = fp8_rows(a.values);
-  b.values = fp8_rows(b.values);
+  if (!a.m.cols) return at::zeros({rows, cols}, type);
   autograd_launched += 1;
   if (rows <= himuon::kFewFp8Rows) {
     at::Tensor c = at::empty({rows, cols}, type);
-    himuon::few_rows_fp8_product(fp8_matrix(a), fp8_matrix(b), c.data_ptr(), out_fp32, cur_stream());
+    himuon::few_rows_fp8_product(a.m, b.m, c.data_ptr(), out_fp32, cur_stream());
     return c;
   }
   // (rows of the result are stored in groups of 16 bytes)
   const int64_t group = out_fp32 ? 4 : 8, ld = up(cols, group) * group;
   at::Tensor c = at::empty({rows, ld}, type);
-  himuon::fp8_product(fp8_matrix(a), fp8_matrix(b), c.data_ptr(), ld, out_fp32, a.powers && b.powers, cur_stream());
+  himuon::fp8_product(a.m, b.m, c.data_ptr(), ld, out_fp32, a.powers && b.powers, cur_stream());
   return ld == cols ? c : c.narrow(1, 0, cols).contiguous();
 }
 at::Tensor fp8_matmul(const at::Tensor& a, const at::Tensor& a_scales, int64_t a_block, bool a_powers, const at::Tensor& b, const at::Tensor& b_scales, int64_t b_block,
                       bool b_powers, bool out_fp32) {
-  return product("fp8_matmul", Fp8{a, a_scales, a_block, a_powers}, Fp8{b, b_scales, b_block, b_powers}, out_fp32);
+  return product("fp8_matmul", fp8_given("fp8_matmul", a, a_scales, a_block, a_powers, a.device(), true), fp8_given("fp8_matmul", b, b_scales, b_block, b_powers, a.device(), true),
+                 out_fp32);
 }
 at::Tensor fp8_dequantize(const at::Tensor& values, const at::Tensor& scales, int64_t block_rows, bool out_fp32) {
-  const Fp8 m{values, scales, block_rows};
-  check_fp8("dequantize", m, values.device());
-  HM_CHECK((values.stride(1) == 1 || values.size(1) <= 1), "dequantize: unit inner stride expected");
+  const Fp8 q = fp8_given("dequantize", values, scales, block_rows, false, values.device(), false);
   const c10::cuda::CUDAGuard guard(values.device());
   at::Tensor out = at::empty(values.sizes(), values.options().dtype(out_fp32 ? at::kFloat : at::kBFloat16));
   if (out.numel()) {
-    himuon::fp8_dequantize(fp8_matrix(m), out.data_ptr(), out.size(1), out_fp32, cur_stream());
+    himuon::fp8_dequantize(q.m, out.data_ptr(), out.size(1), out_fp32, cur_stream());
     autograd_launched += 1;
   }
   return out;
@@ -308,18 +342,15 @@ at::Tensor fp8_dequantize(const at::Tensor& values, const at::Tensor& scales, in
 
 // x w^T with w kept in 8 bits.
 at::Tensor fp8_linear_kept(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scales, int64_t w_block, bool w_powers) {
-  HM_CHECK(x.dim() == 2 && x.scalar_type() == at::kBFloat16, "fp8_linear: bf16 rows expected");
-  const Fp8 q = fp8_empty(x, x.size(0), x.size(1), 1);
+  HM_CHECK(x.dim() == 2 && x.is_cuda() && x.scalar_type() == at::kBFloat16, "fp8_linear: bf16 rows expected");
+  const Fp8 v = fp8_given("fp8_linear", w, w_scales, w_block, w_powers, x.device(), true);
+  const Fp8 q = fp8_piece(x, x.size(0), x.size(1), 1);
   quantize(x, &q, nullptr);
-  return product("fp8_linear", q, Fp8{w, w_scales, w_block, w_powers}, false);
+  return product("fp8_linear", q, v, false);
 }
 // x w^T with both put into 8 bits; copies turned around for the gradients' products are made on the way.
-at::Tensor fp8_linear_forward(const at::Tensor& x, const at::Tensor& w, Fp8* xt, Fp8* wt) {
-  HM_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1) && x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16 && x.device() == w.device(),
-           "fp8_linear: (rows, in) and (out, in) of bf16 on one device expected");
-  const Fp8 q = fp8_empty(x, x.size(0), x.size(1), 1), v = fp8_empty(w, w.size(0), w.size(1), 128);
-  if (xt) *xt = fp8_empty(x, x.size(1), x.size(0), 128);
-  if (wt) *wt = fp8_empty(w, w.size(1), w.size(0), 128);
+at::Tensor fp8_linear_forward(const at::Tensor& x, const at::Tensor& w, const Fp8* xt, const Fp8* wt) {
+  const Fp8 q = fp8_piece(x, x.size(0), x.size(1), 1), v = fp8_piece(w, w.size(0), w.size(1), 128);
   quantize(x, &q, xt);
   quantize(w, &v, wt);
   return product("fp8_linear", q, v, false);
@@ -327,36 +358,43 @@ at::Tensor fp8_linear_forward(const at::Tensor& x, const at::Tensor& w, Fp8* xt,
 
 struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w) {
-    Fp8 xt, wt;
     const bool need_x = x.requires_grad(), need_w = w.requires_grad();
+    Fp8 xt, wt;
+    if (need_w) xt = fp8_piece(x, x.size(1), x.size(0), 128);
+    if (need_x) wt = fp8_piece(w, w.size(1), w.size(0), 128);
     const at::Tensor y = fp8_linear_forward(x, w, need_w ? &xt : nullptr, need_x ? &wt : nullptr);
     variable_list keep;
-    if (need_x) keep.insert(keep.end(), {wt.values, wt.scales});
-    if (need_w) keep.insert(keep.end(), {xt.values, xt.scales});
+    if (need_x) keep.push_back(wt.values);
+    if (need_w) keep.push_back(xt.values);
     ctx->save_for_backward(keep);
-    ctx->saved_data["need_x"] = need_x;
-    ctx->saved_data["need_w"] = need_w;
+    ctx->saved_data["sizes"] = std::vector<int64_t>{x.size(0), x.size(1), w.size(0), need_x, need_w};
     return y;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_once("fp8_linear");
     const variable_list saved = ctx->get_saved_variables();
-    const bool kept_x = ctx->saved_data["need_x"].toBool(), kept_w = ctx->saved_data["need_w"].toBool();
-    const bool need_x = kept_x && ctx->needs_input_grad(0), need_w = kept_w && ctx->needs_input_grad(1);
-    at::Tensor dy = grads[0];
-    if ((dy.stride(1) != 1 && dy.size(1) > 1) || (dy.size(0) > 1 && dy.stride(0) < dy.size(1))) dy = dy.clone(at::MemoryFormat::Contiguous);
+    const std::vector<int64_t> n = ctx->saved_data["sizes"].toIntVector();       // rows, in, out, and what was kept
+    const int64_t rows = n[0], in = n[1], out = n[2];
+    const bool need_x = n[3] && ctx->needs_input_grad(0), need_w = n[4] && ctx->needs_input_grad(1);
+    const at::Tensor dy = apart(grads[0]);
     const c10::cuda::CUDAGuard guard(dy.device());
     Fp8 q, qt;
-    if (need_x) q = fp8_empty(dy, dy.size(0), dy.size(1), 1);
-    if (need_w) qt = fp8_empty(dy, dy.size(1), dy.size(0), 1);
+    if (need_x) q = fp8_piece(dy, rows, out, 1);
+    if (need_w) qt = fp8_piece(dy, out, rows, 1);
     quantize(dy, need_x ? &q : nullptr, need_w ? &qt : nullptr);
-    variable_list out(2);
-    if (need_x) out[0] = product("fp8_linear", q, Fp8{saved[0], saved[1], 128, true}, false);
-    if (need_w) out[1] = product("fp8_linear", qt, Fp8{saved[kept_x ? 2 : 0], saved[kept_x ? 3 : 1], 128, true}, false);
-    return out;
+    variable_list result(2);
+    if (need_x) result[0] = product("fp8_linear", q, fp8_in(saved[0], in, out, 128), false);
+    if (need_w) result[1] = product("fp8_linear", qt, fp8_in(saved[n[3] ? 1 : 0], in, rows, 128), false);
+    return result;
   }
 };
+
+std::vector<int64_t> shape_of(const at::Tensor& x, const at::Tensor& w) {
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = w.size(0);
+  return shape;
+}
 
 }  // namespace
 
@@ -367,15 +405,26 @@ void bind_layer_ops(pybind11::module& m) {
     return rotate(x, positions, turns, seq_len, heads, rotary_dim, interleaved, factor, factor);
   });
   m.def("gated_mlp", [](const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t activation) {
-    if (any_grad({&x, &wg, &wu, &wd})) return GatedMlp::apply(x, wg, wu, wd, activation);
-    return gated_forward(x, wg, wu, wd, activation, nullptr);
+    HM_CHECK(x.dim() >= 1 && wg.dim() == 2 && wu.dim() == 2 && wd.dim() == 2 && x.size(-1) == wg.size(1), "gated_mlp: (..., hidden) and (inter, hidden) expected");
+    const bool flat = x.dim() == 2;
+    const at::Tensor x2 = with_rows(flat ? x : x.reshape({flat_rows(x), x.size(-1)})), g = with_rows(wg), u = with_rows(wu), d = with_rows(wd);
+    at::Tensor y = any_grad({&x2, &g, &u, &d}) ? GatedMlp::apply(x2, g, u, d, activation) : gated_forward(x2, g, u, d, activation, nullptr);
+    return flat ? y : y.view(x.sizes());
   });
   m.def("quantize_fp8", &quantize_fp8);
   m.def("fp8_dequantize", &fp8_dequantize);
   m.def("fp8_matmul", &fp8_matmul);
-  m.def("fp8_linear_kept", &fp8_linear_kept);
+  m.def("fp8_linear_kept", [](const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scales, int64_t w_block, bool w_powers) {
+    HM_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1), "fp8_linear: (..., in) inputs and an (out, in) weight expected");
+    if (x.dim() == 2) return fp8_linear_kept(apart(x), w, w_scales, w_block, w_powers);
+    return fp8_linear_kept(apart(x.reshape({flat_rows(x), x.size(-1)})), w, w_scales, w_block, w_powers).view(shape_of(x, w));
+  });
   m.def("fp8_linear", [](const at::Tensor& x, const at::Tensor& w) {
-    if (any_grad({&x, &w})) return Fp8Linear::apply(x, w);
-    return fp8_linear_forward(x, w, nullptr, nullptr);
+    HM_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && x.is_cuda() && x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16 && x.device() == w.device(),
+             "fp8_linear: (..., in) and (out, in) of bf16 on one device expected");
+    const bool flat = x.dim() == 2;
+    const at::Tensor x2 = apart(flat ? x : x.reshape({flat_rows(x), x.size(-1)})), w2 = apart(w);
+    at::Tensor y = any_grad({&x2, &w2}) ? Fp8Linear::apply(x2, w2) : fp8_linear_forward(x2, w2, nullptr, nullptr);
+    return flat ? y : y.view(shape_of(x, w));
   });
 }

@@ -35,8 +35,7 @@ class Fp8Blocks(NamedTuple):
         if dtype not in (torch.float32, torch.bfloat16):
             raise RuntimeError(f"himuon_b200.ops.Fp8Blocks.dequantize: float32 or bfloat16 expected, got {dtype}")
         if self.values.is_cuda:
-            v = self.values if self.values.stride(1) == 1 or self.values.shape[1] <= 1 else self.values.contiguous()
-            return _ext.ext().fp8_dequantize(v, self.scales, self.block_rows, dtype == torch.float32)
+            return _ext.ext().fp8_dequantize(self.values, self.scales, self.block_rows, dtype == torch.float32)
         return ref.fp8_dequantize(self.values, self.scales, self.block_rows).to(dtype)
 
 
@@ -62,18 +61,10 @@ def quantize_fp8(x2d: torch.Tensor, block_rows: int = 1, transpose: bool = False
         raise RuntimeError(f"himuon_b200.ops.quantize_fp8: blocks of 1 or {BLOCK} rows, got {block_rows}")
     if _any_transformed(x2d):
         raise RuntimeError("himuon_b200.ops.quantize_fp8: not under vmap or forward-mode differentiation")
-    x2d = x2d.detach()
     if x2d.is_cuda:
-        return Fp8Blocks(*_ext.ext().quantize_fp8(_rows(x2d), int(block_rows), bool(transpose)), int(block_rows), True)
-    return Fp8Blocks(*ref.quantize_fp8(x2d.t() if transpose else x2d, int(block_rows)), int(block_rows), True)
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    # unit inner stride, and rows that share no memory
-    (rows, cols), (ld, inner) = t.shape, t.stride()
-    if (inner == 1 or cols <= 1) and (ld >= cols or rows <= 1):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+        return Fp8Blocks(*_ext.ext().quantize_fp8(x2d, block_rows, bool(transpose)), block_rows, True)
+    x2d = x2d.detach()
+    return Fp8Blocks(*ref.quantize_fp8(x2d.t() if transpose else x2d, block_rows), block_rows, True)
 
 
 def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -116,14 +107,12 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
     if x.dim() < 1 or len(shape) != 2 or x.shape[-1] != shape[1] or device != x.device or not x.is_floating_point() or not (kept or w.dtype == x.dtype):
         raise RuntimeError("himuon_b200.ops.fp8_linear: (..., in) inputs and an (out, in) weight of one floating point type on one device expected")
     transformed = _any_transformed(x) if kept else _any_transformed(x, w)
-    out = (*x.shape[:-1], shape[0])
-    if x.is_cuda and x.dtype == torch.bfloat16 and not transformed:
-        x2d = _rows(x.reshape(math.prod(x.shape[:-1]), shape[1]))
-        y = _ext.ext().fp8_linear_kept(x2d, *w) if kept else _ext.ext().fp8_linear(x2d, _rows(w))
-        return y.view(out)
-    if x.is_cuda and x.dtype == torch.bfloat16:
+    kernels = x.is_cuda and x.dtype == torch.bfloat16
+    if kernels and not transformed:
+        return _ext.ext().fp8_linear_kept(x, *w) if kept else _ext.ext().fp8_linear(x, w)
+    if kernels:
         _warn_torch_path("fp8_linear", "under vmap or forward-mode differentiation")
-    x2d = x.reshape(math.prod(x.shape[:-1]), shape[1])
+    x2d, out = x.reshape(math.prod(x.shape[:-1]), shape[1]), (*x.shape[:-1], shape[0])
     if kept:
         return (ref.fp8_dequantize(*ref.quantize_fp8(x2d.detach(), 1), 1) @ ref.fp8_dequantize(*w[:3]).t()).to(x.dtype).view(out)
     return (ref.fp8_linear_any if transformed else ref.fp8_linear)(x2d, w).view(out)

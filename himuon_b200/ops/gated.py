@@ -2,12 +2,10 @@
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from .. import _ext
-from . import _any_transformed, _warn_torch_path, _with_rows_apart, use_kernels
+from . import _any_transformed, _warn_torch_path, use_kernels
 from . import reference as ref
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
@@ -22,21 +20,22 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     the result is nearer to the exact one than that of :func:`swiglu` on finished projections, and not its bits.  Up to 64 rows run kernels
     that stream the weights.  Differentiable once in all four; the backward pass needs ``x``, and keeps 8 bytes for each row and
     intermediate feature until then.  Under vmap and forward-mode differentiation the PyTorch formulation runs."""
-    if activation not in ACTIVATIONS:
+    number = ACTIVATIONS.get(activation)
+    if number is None:
         raise RuntimeError(f"himuon_b200.ops.gated_mlp: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
     if x.dim() < 1 or w_gate.dim() != 2 or not x.is_floating_point():
         raise RuntimeError("himuon_b200.ops.gated_mlp: (..., hidden) inputs and (inter, hidden) weights of floating point expected")
-    inter, hidden = w_gate.shape
-    if x.shape[-1] != hidden or w_up.shape != (inter, hidden) or w_down.shape != (hidden, inter) or hidden == 0 or inter == 0:
+    shape = w_gate.shape
+    inter, hidden = shape
+    if x.shape[-1] != hidden or w_up.shape != shape or w_down.shape != (hidden, inter) or not hidden or not inter:
         raise RuntimeError(f"himuon_b200.ops.gated_mlp: sizes disagree: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)}, "
                            f"w_down {tuple(w_down.shape)}")
-    if any(w.dtype != x.dtype or w.device != x.device for w in (w_gate, w_up, w_down)):
+    dtype, device = x.dtype, x.device
+    if w_gate.dtype != dtype or w_up.dtype != dtype or w_down.dtype != dtype or w_gate.device != device or w_up.device != device or w_down.device != device:
         raise RuntimeError("himuon_b200.ops.gated_mlp: inputs and weights must be of one type on one device")
     transformed = _any_transformed(x, w_gate, w_up, w_down)
     if use_kernels(x) and hidden % 8 == 0 and inter % 8 == 0 and not transformed:
-        x2d = _with_rows_apart(x.reshape(math.prod(x.shape[:-1]), hidden))
-        y = _ext.ext().gated_mlp(x2d, _with_rows_apart(w_gate), _with_rows_apart(w_up), _with_rows_apart(w_down), ACTIVATIONS[activation])
-        return y.view(x.shape)
+        return _ext.ext().gated_mlp(x, w_gate, w_up, w_down, number)
     if use_kernels(x):
         _warn_torch_path("gated_mlp", "under vmap or forward-mode differentiation" if transformed else
                          f"sizes of {hidden} and {inter} (the kernels take multiples of 8)")
