@@ -10,8 +10,9 @@
 //
 // Other scales: the tensor core sums the 128 products of a block, and each block's sums are read from tensor memory, scaled and added up in registers, in
 // fp32.  As b has blocks of 128 rows, a thread, which has one row of a and 128 columns, needs one factor a block.  Two accumulators, so that one block is added
-// up beside the products of the next.  219 and 217 us: it takes the hand-on of a block between the tensor core and both CTAs' warps, there and back, for each 512
-// cycles of products (187 us with nothing but the hand-on).  Sixteen warps with 64 columns each were slower (302 for 262, at an earlier state).
+// up beside the products of the next.  210 and 212 us: it takes the hand-on of a block between the tensor core and both CTAs' warps, there and back, for each 512
+// cycles of products (187 us with nothing but the hand-on).  Commits of their own for the producer and for the sums 219; sixteen warps with 64 columns each 302 for
+// 262, at an earlier state; columns on their way while others are added up, no difference.
 #include "fp8.h"
 #include "gemm_epilogue.cuh"
 #include "himuon.h"
@@ -70,9 +71,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   uint8_t* smem = align_up_1024(smem_raw);
   uint8_t* slabs = smem + F8_STAGES * F8_STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(slabs + 2 * SLAB_BYTES);
-  uint64_t* empty = full + F8_STAGES;
-  uint64_t* tfull = empty + F8_STAGES;
-  uint64_t* tempty = tfull + 2;
+  uint64_t* done = full + F8_STAGES;       // a stage's products are in tensor memory, and the stage is free: to the producer and to the sums
+  uint64_t* tempty = done + F8_STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -80,8 +80,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < F8_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 16); }     // eight summing warps in each CTA
+    for (int s = 0; s < F8_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&done[s], 1); }
+    for (int a = 0; a < 2; ++a) { mbar_init(&tempty[a], 16); }     // eight summing warps in each CTA
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -108,7 +108,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         tile_at(p, tile, mt, nt);
         const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + static_cast<int>(rank) * BM;
       for (int kb = 0; kb < p.kblocks; ++kb) {
-        if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
+        if (!mbar_wait_warp(&done[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
         uint8_t* sA = smem + stage * F8_STAGE;
         mbar_expect_tx(&full[stage], 2 * F8_STAGE, leader ? e : 0);
         tma2_load_3d(sA, &tmA, &full[stage], kb * F8_K, m0, 0, e);
@@ -122,7 +122,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const uint32_t e = elect_one();
       constexpr uint32_t idesc = idesc_e4m3(256, 256);
       const uint64_t a_desc0 = umma_smem_desc(smem_u32(smem), 16, 1024), b_desc0 = desc_at(a_desc0, F8_A);
-      const uint32_t empty0 = smem_u32(empty), empty1 = map_to_cta(empty0, 1), tfull0 = smem_u32(tfull), tfull1 = map_to_cta(tfull0, 1);
+      const uint32_t done0 = smem_u32(done), done1 = map_to_cta(done0, 1);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
@@ -134,10 +134,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
           for (int k = 0; k < 4; ++k)                // 32 values an instruction
             umma2_f8(tmem_base + static_cast<uint32_t>(acc * 256), desc_at(a_desc, k * 32), desc_at(b_desc, k * 32), idesc, k > 0 ? 1u : 0u, e);
-          umma2_commit(tfull0 + acc * 8, e);
-          umma2_commit(tfull1 + acc * 8, e);
-          umma2_commit(empty0 + stage * 8, e);       // this CTA's producer
-          umma2_commit(empty1 + stage * 8, e);       // the peer's
+          umma2_commit(done0 + stage * 8, e);        // to this CTA's producer and sums
+          umma2_commit(done1 + stage * 8, e);        // and to the peer's
           if (++stage == F8_STAGES) { stage = 0; phase ^= 1; }
           acc ^= 1;
           if (acc == 0) acc_phase ^= 1;
@@ -155,8 +153,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     uint8_t* my_row = slab + row_in_tile * 128;
     const uint32_t t_group = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(group * 128);
     if (issuer) tma_prefetch_desc(&tmC);
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    int acc = 0, stage = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int tile = first; ok && tile < total; tile += n_pairs) {
       int mt, nt;
@@ -177,7 +175,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         const int ahead = min(kb + 1, p.kblocks - 1);
         next_a = __ldg(sa + ahead * p.sa_col);
         next_b = __ldg(sb + ahead * p.sb_col);
-        ok = mbar_wait(&tfull[acc], acc_phase, abort_flag, p.status, 3);
+        ok = mbar_wait(&done[stage], phase, abort_flag, p.status, 3);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
@@ -192,7 +190,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive_remote(tempty_lead + acc * 8);
         acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
+        if (++stage == F8_STAGES) { stage = 0; phase ^= 1; }
       }
       // the 128 threads of a group meet on named barriers below, so they also leave together when a wait runs out
       ok = named_barrier_and(1 + 2 * group, 128, ok);

@@ -7,7 +7,6 @@
 from __future__ import annotations
 
 import math
-from fractions import Fraction
 
 import torch
 
@@ -15,7 +14,7 @@ from .. import _ext
 from . import _any_transformed, _check_width, _warn_torch_path
 from . import reference as ref
 
-TWO_PI = 2 * Fraction(314159265358979323846264338327950288419716939937510, 10 ** 50)
+TWO_PI_E50 = 628318530717958647692528676655900576839433879875021      # 2 pi * 10^50
 SCALINGS = ("linear", "ntk", "yarn", "llama3")
 
 
@@ -100,7 +99,8 @@ class RotaryFrequencies:
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         # whole numbers of 2^-64 turns a position: position times this, modulo 2^64, is the place within a turn
-        turns = [round(Fraction(f) / TWO_PI * 2 ** 64) % 2 ** 64 for f in self.frequencies]
+        ratios = (f.as_integer_ratio() for f in self.frequencies)
+        turns = [((n * 2 ** 65 * 10 ** 50) // (d * TWO_PI_E50) + 1) // 2 % 2 ** 64 for n, d in ratios]
         self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64).to(self.device)
         if self.device.type == "cuda":
             torch.cuda.current_stream(self.device).synchronize()       # calls on any stream find it there
