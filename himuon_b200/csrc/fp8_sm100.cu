@@ -21,6 +21,7 @@
 #include "tma_host.h"
 
 #include <atomic>
+#include <type_traits>
 
 namespace himuon {
 
@@ -41,6 +42,7 @@ struct Fp8Dev {
   long long sa_row, sa_col, sb_row, sb_col;
   int a_block;                       // rows of a block of a
   int rows, cols, tiles_m, tiles_n, kblocks, band;
+  int whole, items, cuts;            // fp8_powers_kernel: tiles that are taken whole, and each of the others in so many parts along the inner dimension
   int* status;
 };
 
@@ -58,6 +60,22 @@ __device__ __forceinline__ void tile_at(const Fp8Dev& p, int tile, int& mt, int&
   const int per = p.band * p.tiles_n, b = tile / per, at = tile - b * per, first = b * p.band, size = min(p.tiles_m - first, p.band);
   nt = at / size;
   mt = first + at - nt * size;
+}
+// One of the `items`: blocks kb0 to kb1 - 1 of a tile, and where its sums go if they are a part (-1 else).
+struct F8Item { int mt, nt, kb0, kb1, part; };
+__device__ __forceinline__ F8Item item_at(const Fp8Dev& p, int item) {
+  F8Item w;
+  const int t = item - p.whole, tile = t < 0 ? item : p.whole + t / p.cuts;
+  tile_at(p, tile, w.mt, w.nt);
+  w.part = t < 0 ? -1 : t;
+  w.kb0 = 0;
+  w.kb1 = p.kblocks;
+  if (t >= 0) {                      // (cut between groups of four blocks, which share a word of scales)
+    const int cut = t % p.cuts, groups = (p.kblocks + 3) / 4;
+    w.kb0 = groups * cut / p.cuts * 4;
+    w.kb1 = cut + 1 < p.cuts ? groups * (cut + 1) / p.cuts * 4 : p.kblocks;
+  }
+  return w;
 }
 // fp32 sums of e4m3 values (format 0), both operands along K.
 constexpr uint32_t idesc_e4m3(int m, int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
@@ -277,7 +295,8 @@ __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&v)[4])
 
 template <bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MX_THREADS, 1)
-fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC, Fp8Dev p) {
+fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+                  const __grid_constant__ CUtensorMap tmParts, Fp8Dev p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_up_1024(smem_raw);
   uint8_t* slabs = smem + MX_STAGES * MX_STAGE;
@@ -307,7 +326,7 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   cluster_sync_all();                // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, total = p.tiles_m * p.tiles_n;
+  const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
 
   if (warp < 4) {
     registers_down<MX_REGS_FEW>();
@@ -319,11 +338,10 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = first; ok && tile < total; tile += n_pairs) {
-        int mt, nt;
-        tile_at(p, tile, mt, nt);
-        const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + static_cast<int>(rank) * BM;
-        for (int kb = 0; kb < p.kblocks; kb += 2) {
+      for (int item = first; ok && item < p.items; item += n_pairs) {
+        const F8Item w = item_at(p, item);
+        const int m0 = w.mt * 256 + static_cast<int>(rank) * BM, n0 = w.nt * 256 + static_cast<int>(rank) * BM;
+        for (int kb = w.kb0; kb < w.kb1; kb += 2) {
           if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
           uint8_t* sA = smem + stage * MX_STAGE;
           mbar_expect_tx(&full[stage], 2 * MX_STAGE, leader ? e : 0);
@@ -345,15 +363,16 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       int stage = 0, slot = 0;
       uint32_t phase = 0, slot_phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = first; ok && tile < total; tile += n_pairs) {
+      for (int item = first; ok && item < p.items; item += n_pairs) {
+        const F8Item w = item_at(p, item);
         if (!mbar_wait_warp(tempty, acc_phase ^ 1, abort_flag, p.status, 2)) break;
         uint32_t more = 0;
-        for (int kb = 0; kb < p.kblocks; kb += 4) {
+        for (int kb = w.kb0; kb < w.kb1; kb += 4) {
           if (!mbar_wait_warp(&sfull[slot], slot_phase, abort_flag, p.status, 2)) { ok = false; break; }
           const uint32_t t_scales = tmem_base + MX_SCALES + static_cast<uint32_t>(slot) * MX_SLOT;
 #pragma unroll
           for (int pair = 0; pair < 2; ++pair) {
-            if (pair == 1 && kb + 2 >= p.kblocks) break;
+            if (pair == 1 && kb + 2 >= w.kb1) break;
             if (!mbar_wait_warp(&full[stage], phase, abort_flag, p.status, 2)) { ok = false; break; }
             tc_fence_after();
             const uint64_t a_desc = desc_at(a_desc0, stage * MX_STAGE), b_desc = desc_at(b_desc0, stage * MX_STAGE);
@@ -388,10 +407,9 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     int slot = 0;
     uint32_t slot_phase = 0;
     bool ok = true;
-    for (int tile = first; ok && tile < total; tile += n_pairs) {
-      int mt, nt;
-        tile_at(p, tile, mt, nt);
-        const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256;
+    for (int item = first; ok && item < p.items; item += n_pairs) {
+      const F8Item it = item_at(p, item);
+      const int m0 = it.mt * 256 + static_cast<int>(rank) * BM, n0 = it.nt * 256;
       // (loads without conditions, of places that exist, and a group ahead: each would otherwise wait for the one before.  What a row or a
       // block that is not there is scaled by does not matter, as its values are zeros, as long as it is a number.)
       const float *sa[4], *sb[2];
@@ -412,13 +430,13 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           for (int i = 0; i < 2; ++i) next[16 + i * 4 + j] = __float_as_uint(__ldg(sb[i] + ob));
         }
       };
-      load(0);
-      for (int kb = 0; ok && kb < p.kblocks; kb += 4) {
+      load(it.kb0);
+      for (int kb = it.kb0; ok && kb < it.kb1; kb += 4) {
         uint32_t w[6];                               // four exponents each
 #pragma unroll
         for (int i = 0; i < 6; ++i)
           w[i] = (next[4 * i] >> 23 & 255u) | (next[4 * i + 1] >> 23 & 255u) << 8 | (next[4 * i + 2] >> 23 & 255u) << 16 | (next[4 * i + 3] >> 23 & 255u) << 24;
-        if (kb + 4 < p.kblocks) load(kb + 4);
+        if (kb + 4 < it.kb1) load(kb + 4);
         ok = mbar_wait_warp(&sempty[slot], slot_phase ^ 1, abort_flag, p.status, 3);
         if (!ok) break;
         tc_fence_after();
@@ -445,10 +463,9 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     const uint32_t t_group = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(group * 128);
     if (issuer) tma_prefetch_desc(&tmC);
     uint32_t acc_phase = 0;
-    for (int tile = first; tile < total; tile += n_pairs) {
-      int mt, nt;
-        tile_at(p, tile, mt, nt);
-        const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + group * 128;
+    for (int item = first; item < p.items; item += n_pairs) {
+      const F8Item w = item_at(p, item);
+      const int m0 = w.mt * 256 + static_cast<int>(rank) * BM, n0 = w.nt * 256 + group * 128;
       // the 128 threads of a group meet on named barriers below, so they also leave together when the wait runs out
       if (!named_barrier_and(1 + 2 * group, 128, mbar_wait(tfull, acc_phase, abort_flag, p.status, 3))) break;
       acc_phase ^= 1;
@@ -461,27 +478,42 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(tempty_lead);
       if (m0 >= p.rows) continue;                              // uniform
+      if (F32 || w.part >= 0) {
+        const bool part = w.part >= 0;                         // (all of a part is stored, which costs less than to ask)
 #pragma unroll
-      for (int sl = 0; sl < (F32 ? 4 : 2); ++sl) {             // slabs of 32 or 64 columns
-        const int col = n0 + sl * (F32 ? 32 : 64);
+        for (int sl = 0; sl < 4; ++sl) {                       // slabs of 32 columns
+          const int col = sl * 32;
+          if (!part && n0 + col >= p.cols) break;
+          if (issuer) tma_store_wait_read<0>();
+          named_barrier(1 + 2 * group, 128);                   // the slab is free
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(my_row + ((j ^ (row_in_tile & 7)) << 4)) = make_uint4(c[sl][4 * j], c[sl][4 * j + 1], c[sl][4 * j + 2], c[sl][4 * j + 3]);
+          fence_proxy_async_smem();
+          named_barrier(2 + 2 * group, 128);                   // the slab is complete
+          if (issuer) {
+            if (part) tma_store_3d(&tmParts, slab, group * 128 + col, w.part * 256 + static_cast<int>(rank) * BM, 0);
+            else tma_store_3d(&tmC, slab, n0 + col, m0, 0);
+            tma_store_commit();
+          }
+        }
+        continue;
+      }
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {                         // slabs of 64 columns
+        const int col = n0 + sl * 64;
         if (col >= p.cols) break;
         if (issuer) tma_store_wait_read<0>();
         named_barrier(1 + 2 * group, 128);                     // the slab is free
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          uint4 o;
-          if constexpr (F32) {
-            o = make_uint4(c[sl][4 * j], c[sl][4 * j + 1], c[sl][4 * j + 2], c[sl][4 * j + 3]);
-          } else {
-            uint32_t w[4];
+          uint32_t o[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const int at = 8 * j + 2 * t;
-              w[t] = pack_bf16x2(__uint_as_float(c[2 * sl + at / 32][at % 32]), __uint_as_float(c[2 * sl + at / 32][at % 32 + 1]));
-            }
-            o = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int t = 0; t < 4; ++t) {
+            const int at = 8 * j + 2 * t;
+            o[t] = pack_bf16x2(__uint_as_float(c[2 * sl + at / 32][at % 32]), __uint_as_float(c[2 * sl + at / 32][at % 32 + 1]));
           }
-          *reinterpret_cast<uint4*>(my_row + ((j ^ (row_in_tile & 7)) << 4)) = o;
+          *reinterpret_cast<uint4*>(my_row + ((j ^ (row_in_tile & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         named_barrier(2 + 2 * group, 128);                     // the slab is complete
@@ -501,6 +533,28 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     tc_fence_after();
     tmem_dealloc2(tmem_base, 512);
   }
+}
+
+// The tiles that were cut: their parts, of 256 x 256, added up first to last.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__ parts, T* __restrict__ c, long long ld_c, Fp8Dev p) {
+  constexpr int PER_TILE = 256 * 64;                           // groups of four columns
+  const int at = blockIdx.x * 256 + threadIdx.x, tile = at / PER_TILE, e = at - tile * PER_TILE;
+  int mt, nt;
+  tile_at(p, p.whole + tile, mt, nt);
+  const int r = e >> 6, col = nt * 256 + (e & 63) * 4;
+  const long long row = mt * 256LL + r;
+  if (row >= p.rows || col >= p.cols) return;
+  const float4* src = reinterpret_cast<const float4*>(parts) + static_cast<long long>(tile) * p.cuts * PER_TILE + e;
+  float4 v = src[0];
+#pragma unroll 4
+  for (int k = 1; k < p.cuts; ++k) {
+    const float4 u = src[static_cast<long long>(k) * PER_TILE];
+    v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+  }
+  // (rows of c hold whole groups of 16 bytes)
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(c + row * ld_c + col) = v;
+  else *reinterpret_cast<uint2*>(c + row * ld_c + col) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
 }
 
 static CUtensorMap bytes_map(const Fp8Matrix& m) {
@@ -540,21 +594,63 @@ static void check(cudaError_t e) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon fp8_product: ") + cudaGetErrorString(e));
 }
 
+// How the last round of tiles is cut along the inner dimension, where less than half of the pairs would have one: into as many parts as there are pairs
+// for, of 8 blocks or more.  Writing the parts and adding them up takes about as long as 20 blocks of products.  256 x 2560 x 9728 (10 tiles) 31 -> 20 us,
+// 9728 x 2560 x 8192 (380 tiles on 74 pairs) 155 -> 151: large products are held back by power more than by their last round.
+static void plan_cuts(Fp8Dev& p, int pairs) {
+  const int total = p.tiles_m * p.tiles_n, rest = total % pairs;
+  p.whole = p.items = total;
+  p.cuts = 1;
+  if (rest == 0 || 2 * rest > pairs) return;
+  const int cuts = pairs / rest < p.kblocks / 8 ? pairs / rest : p.kblocks / 8;
+  if (cuts < 2 || p.kblocks - p.kblocks / cuts < 20) return;
+  p.whole = total - rest;
+  p.cuts = cuts;
+  p.items = p.whole + rest * cuts;
+}
+
 template <bool POWERS, bool F32>
-static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Fp8Dev& p, cudaStream_t s) {
+static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, Fp8Dev p, void* c, long long ld_c, float* parts, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + F8_STAGES * F8_STAGE + 2 * SLAB_BYTES + 256;
   static_assert(MX_STAGES * MX_STAGE == F8_STAGES * F8_STAGE);
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
   static std::atomic<int> most[64] = {};
-  const auto kernel = POWERS ? fp8_powers_kernel<F32> : fp8_product_kernel<F32>;
+  const auto kernel = [] {
+    if constexpr (POWERS) return fp8_powers_kernel<F32>;
+    else return fp8_product_kernel<F32>;
+  }();
   constexpr int THREADS = POWERS ? MX_THREADS : F8_THREADS;
   check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM)));
-  const int pairs = pairs_at_once(kernel, THREADS, SMEM, most), total = p.tiles_m * p.tiles_n;
-  kernel<<<2 * (total < pairs ? total : pairs), THREADS, SMEM, s>>>(ta, tb, tc, p);
-  check(cudaGetLastError());
+  const int pairs = pairs_at_once(kernel, THREADS, SMEM, most), most_pairs = pairs < num_sms() / 2 ? pairs : num_sms() / 2;
+  if constexpr (POWERS) {
+    plan_cuts(p, parts ? most_pairs : 1);                // (as many parts as fp8_parts_floats() counts)
+    CUtensorMap tp = tc;
+    const int n = p.items - p.whole;
+    if (n) {
+      const uint64_t dims[3] = {256, static_cast<uint64_t>(n) * 256, 1};
+      const uint64_t strides[2] = {256 * sizeof(float), dims[1] * 256 * sizeof(float)};
+      const uint32_t box[3] = {32, BM, 1};
+      tp = make_tmap(parts, 3, dims, strides, box, 4, true);
+    }
+    kernel<<<2 * (p.items < pairs ? p.items : pairs), THREADS, SMEM, s>>>(ta, tb, tc, tp, p);
+    check(cudaGetLastError());
+    if (n) {
+      using T = std::conditional_t<F32, float, __nv_bfloat16>;
+      fp8_join_kernel<T><<<n / p.cuts * 64, 256, 0, s>>>(parts, static_cast<T*>(c), ld_c, p);
+      check(cudaGetLastError());
+    }
+  } else {
+    const int total = p.tiles_m * p.tiles_n;
+    kernel<<<2 * (total < pairs ? total : pairs), THREADS, SMEM, s>>>(ta, tb, tc, p);
+    check(cudaGetLastError());
+  }
 }
 
-void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c, int out_fp32, int powers, cudaStream_t s) {
+long long fp8_parts_floats(const Fp8Matrix& a, const Fp8Matrix& b) {
+  return a.cols > 20 * F8_K && a.rows > 0 && b.rows > 0 ? static_cast<long long>(num_sms() / 2) * 256 * 256 : 0;
+}
+
+void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c, int out_fp32, int powers, float* parts, cudaStream_t s) {
   const int esz = out_fp32 ? 4 : 2;
   if (a.rows <= 0 || b.rows <= 0 || a.cols <= 0 || a.cols != b.cols || b.block_rows != 128 || ld_c < b.rows || ld_c * esz % 16)
     throw std::runtime_error("himuon fp8_product: bad sizes");
@@ -573,8 +669,8 @@ void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c
   const uint64_t strides[2] = {static_cast<uint64_t>(ld_c) * esz, static_cast<uint64_t>(ld_c) * esz * dims[1]};
   const uint32_t box[3] = {static_cast<uint32_t>(128 / esz), BM, 1};
   const CUtensorMap ta = bytes_map(a), tb = bytes_map(b), tc = make_tmap(c, 3, dims, strides, box, esz, true);
-  if (powers) out_fp32 ? launch<true, true>(ta, tb, tc, p, s) : launch<true, false>(ta, tb, tc, p, s);
-  else out_fp32 ? launch<false, true>(ta, tb, tc, p, s) : launch<false, false>(ta, tb, tc, p, s);
+  const auto run = powers ? (out_fp32 ? launch<true, true> : launch<true, false>) : (out_fp32 ? launch<false, true> : launch<false, false>);
+  run(ta, tb, tc, p, c, ld_c, parts, s);
 }
 
 }  // namespace himuon

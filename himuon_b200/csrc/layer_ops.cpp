@@ -321,7 +321,10 @@ at::Tensor product(const char* op, const Fp8& a, const Fp8& b, bool out_fp32) {
   // (rows of the result are stored in groups of 16 bytes)
   const int64_t group = out_fp32 ? 4 : 8, ld = up(cols, group) * group;
   at::Tensor c = at::empty({rows, ld}, type);
-  himuon::fp8_product(a.m, b.m, c.data_ptr(), ld, out_fp32, a.powers && b.powers, cur_stream());
+  const bool powers = a.powers && b.powers;
+  at::Tensor parts;
+  if (const int64_t floats = powers ? himuon::fp8_parts_floats(a.m, b.m) : 0) parts = at::empty({floats}, a.values.options().dtype(at::kFloat));
+  himuon::fp8_product(a.m, b.m, c.data_ptr(), ld, out_fp32, powers, parts.defined() ? parts.data_ptr<float>() : nullptr, cur_stream());
   return ld == cols ? c : c.narrow(1, 0, cols).contiguous();
 }
 at::Tensor fp8_matmul(const at::Tensor& a, const at::Tensor& a_scales, int64_t a_block, bool a_powers, const at::Tensor& b, const at::Tensor& b_scales, int64_t b_block,

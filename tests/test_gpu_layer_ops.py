@@ -357,7 +357,8 @@ def test_quantisation_has_the_bits_of_the_plain_one(dtype, block_rows):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 128, 128), (5, 40, 144), (8, 352, 128), (16, 130, 512), (31, 640, 1000), (64, 200, 2560), (65, 128, 640), (3, 20, 77), (129, 8, 8),
-                                   (130, 1000, 1729), (300, 257, 256), (777, 1728, 640), (513, 300, 4096)])
+                                   (130, 1000, 1729), (300, 257, 256), (777, 1728, 640), (513, 300, 4096),
+                                   (70, 520, 9728), (6400, 700, 4096), (200, 12, 5000)])
 def test_fp8_matmul(M, N, K):
     """Powers of two and any other fp32 scales, different from block to block, blocks of either kind in a, every row length."""
     ops = _ops()
