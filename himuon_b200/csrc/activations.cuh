@@ -29,9 +29,11 @@ __device__ __forceinline__ void activate_grad(float g, float& a, float& d) {
     a = g * phi;
     d = phi + g * 0.3989422804f * __expf(-0.5f * g * g);
   } else if constexpr (ACT == kGeluTanh) {
-    const float e = __expf(fminf(-2.f * kGeluC * g * (1.f + kGeluA * g * g), 80.f)), s = __fdividef(1.f, 1.f + e);
+    // (beyond 30 the sigmoid is what it is there, while the polynomial would run over; NaN stays)
+    const float z = fminf(fmaxf(g, -30.f), 30.f), e = __expf(fminf(-2.f * kGeluC * z * (1.f + kGeluA * z * z), 80.f)), s = __fdividef(1.f, 1.f + e);
     a = g * s;
-    d = s + g * (e * s) * s * (2.f * kGeluC * (1.f + 3.f * kGeluA * g * g));
+    d = s + z * (e * s) * s * (2.f * kGeluC * (1.f + 3.f * kGeluA * z * z));
+    if (g != g) d = g;
   } else {
     a = g < 0.f ? 0.f : g;
     d = g <= 0.f ? 0.f : 1.f;

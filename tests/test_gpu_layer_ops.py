@@ -245,10 +245,11 @@ def test_gated_mlp(T, H, I, activation):
 
 @pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "relu"])
 def test_gated_mlp_of_large_gates(activation):
-    """Gates of hundreds, where sigmoids are 0 and 1 and exponentials would run over."""
+    """Gates of hundreds, where sigmoids are 0 and 1 and exponentials would run over, and of 1e12, where their cubes would."""
     ops = _ops()
-    for T in (20, 200):
+    for T, spread in ((20, 120.0), (200, 120.0), (20, 1e12), (200, 1e12)):
         x, wg, wu, wd, dy = _block(T, 256, 384, spread=120.0)
+        wg = (wg.float() * (spread / 120.0)).bfloat16()
         leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
         y = ops.gated_mlp(*leaves, activation=activation)
         grads = torch.autograd.grad(y, leaves, dy)
