@@ -36,7 +36,6 @@ constexpr int F8_BAND = 8;           // rows of tiles in a band (tile_at)
 constexpr int F8_K = 128;            // values of a block, a 128-byte row of shared memory
 constexpr uint32_t F8_A = BM * F8_K, F8_STAGE = 2 * F8_A;
 
-
 struct Fp8Dev {
   const float *sa, *sb;
   long long sa_row, sa_col, sb_row, sb_col;
@@ -123,8 +122,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     bool ok = true;
     for (int tile = first; ok && tile < total; tile += n_pairs) {
       int mt, nt;
-        tile_at(p, tile, mt, nt);
-        const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + static_cast<int>(rank) * BM;
+      tile_at(p, tile, mt, nt);
+      const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + static_cast<int>(rank) * BM;
       for (int kb = 0; kb < p.kblocks; ++kb) {
         if (!mbar_wait_warp(&done[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
         uint8_t* sA = smem + stage * F8_STAGE;
@@ -176,8 +175,8 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     bool ok = true;
     for (int tile = first; ok && tile < total; tile += n_pairs) {
       int mt, nt;
-        tile_at(p, tile, mt, nt);
-        const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + group * 128;
+      tile_at(p, tile, mt, nt);
+      const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + group * 128;
       const int row = m0 + row_in_tile;
       const bool mine = row < p.rows && n0 < p.cols;           // (else there is nothing to scale: zeros)
       const float* sa = p.sa + static_cast<long long>(mine ? row / p.a_block : 0) * p.sa_row;

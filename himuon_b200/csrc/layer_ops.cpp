@@ -89,7 +89,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
 // ------------------------------------------------------------------------------------------------ gated feed-forward block
 void check_rows(const char* op, const char* name, const at::Tensor& t, const at::Tensor& like, int64_t rows, int64_t cols) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1 &&
-                  t.stride(0) % 8 == 0 && (rows <= 1 || t.stride(0) >= cols) && aligned16(t),
+                  t.stride(0) % 8 == 0 && t.stride(0) >= cols && aligned16(t),
               std::string("himuon: ") + op + ": " + name + " must be (" + std::to_string(rows) + ", " + std::to_string(cols) + ") bf16, its rows on 16-byte boundaries with unit inner stride");
 }
 // Rows of all dimensions but the last.
@@ -98,9 +98,9 @@ int64_t flat_rows(const at::Tensor& t) {
   for (int64_t i = 0; i + 1 < t.dim(); ++i) n *= t.size(i);
   return n;
 }
-// Rows as check_rows() wants them: copied where they lie otherwise.
+// Rows as check_rows() wants them: copied where they lie otherwise (a single row too, whose stride may be anything: a tensor map takes none below its width).
 at::Tensor with_rows(const at::Tensor& t) {
-  if (t.stride(1) == 1 && t.stride(0) % 8 == 0 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) && aligned16(t)) return t;
+  if (t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && aligned16(t)) return t;
   return t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -153,8 +153,13 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_once("gated_mlp");
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &wd = saved[3], &h = saved[4], &gu = saved[5];
-    const GatedSizes n{x.size(0), x.size(1), wg.size(0)};
+    const at::Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &wd = saved[3], &h = saved[4], &gu = saved[5], &low = saved[6];
+    const int64_t activation = ctx->saved_data["activation"].toInt();
+    const GatedSizes n = gated_sizes(x, wg, wu, wd, activation);       // (hooks may have moved what was kept)
+    check_rows("gated_mlp", "what is kept of h", h, x, n.rows, n.inter);
+    check_rows("gated_mlp", "what is kept of the gates", gu, x, n.rows, 2 * n.inter);
+    HM_CHECK(gu.is_contiguous() && low.device() == x.device() && low.scalar_type() == at::kByte && low.is_contiguous() &&
+                 low.numel() == n.rows * 2 * himuon::gated_low(static_cast<int>(n.inter)) && aligned16(low), "gated_mlp: what was kept of the gates has changed");
     const c10::cuda::CUDAGuard guard(x.device());
     variable_list out(5);
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
@@ -172,10 +177,10 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     if (!need_x && !need_w) return out;
     at::Tensor dgu = at::empty_like(gu);
     himuon::GatedDownGradArgs a;
-    a.dy = dy.data_ptr(); a.wd = wd.data_ptr(); a.gu = gu.data_ptr(); a.gu_low = saved[6].data_ptr(); a.dgu = dgu.data_ptr();
+    a.dy = dy.data_ptr(); a.wd = wd.data_ptr(); a.gu = gu.data_ptr(); a.gu_low = low.data_ptr(); a.dgu = dgu.data_ptr();
     a.ld_dy = dy.stride(0); a.ld_wd = wd.stride(0);
     a.rows = static_cast<int>(n.rows); a.hidden = static_cast<int>(n.hidden); a.inter = static_cast<int>(n.inter);
-    a.activation = static_cast<int>(ctx->saved_data["activation"].toInt());
+    a.activation = static_cast<int>(activation);
     himuon::gated_down_grad(a, cur_stream());
     autograd_launched += 1;
     if (need_x) {
@@ -290,7 +295,7 @@ Fp8 fp8_given(const char* op, const at::Tensor& values, const at::Tensor& scales
   Fp8 q;
   q.values = values;
   const bool unit = values.stride(1) == 1 || (!rows16 && values.size(1) <= 1);
-  if (rows16 && !(unit && values.stride(0) % 16 == 0 && (values.size(0) <= 1 || values.stride(0) >= values.size(1)) && aligned16(values))) {
+  if (rows16 && !(unit && values.stride(0) % 16 == 0 && values.stride(0) >= values.size(1) && aligned16(values))) {
     q.values = at::empty({values.size(0), up(values.size(1), 16) * 16}, values.options()).narrow(1, 0, values.size(1));
     q.values.copy_(values);
   } else if (!unit) {
@@ -382,13 +387,19 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     const bool need_x = n[3] && ctx->needs_input_grad(0), need_w = n[4] && ctx->needs_input_grad(1);
     const at::Tensor dy = apart(grads[0]);
     const c10::cuda::CUDAGuard guard(dy.device());
+    auto kept = [&](int64_t i, int64_t cols) {           // (hooks may have moved it)
+      const at::Tensor& t = saved[i];
+      HM_CHECK(t.device() == dy.device() && t.scalar_type() == at::kByte && t.is_contiguous() && t.numel() == fp8_scales_at(in, cols) + 4 * fp8_scale_count(in, cols, 128) &&
+                   aligned16(t), "fp8_linear: what was kept has changed");
+      return fp8_in(t, in, cols, 128);
+    };
     Fp8 q, qt;
     if (need_x) q = fp8_piece(dy, rows, out, 1);
     if (need_w) qt = fp8_piece(dy, out, rows, 1);
     quantize(dy, need_x ? &q : nullptr, need_w ? &qt : nullptr);
     variable_list result(2);
-    if (need_x) result[0] = product("fp8_linear", q, fp8_in(saved[0], in, out, 128), false);
-    if (need_w) result[1] = product("fp8_linear", qt, fp8_in(saved[n[3] ? 1 : 0], in, rows, 128), false);
+    if (need_x) result[0] = product("fp8_linear", q, kept(0, out), false);
+    if (need_w) result[1] = product("fp8_linear", qt, kept(n[3] ? 1 : 0, rows), false);
     return result;
   }
 };

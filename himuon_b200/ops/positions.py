@@ -77,7 +77,7 @@ def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[l
 
 
 class RotaryFrequencies:
-    """How fast the pairs of a head turn.  Made once for a model; every layer uses it.
+    """How fast the pairs of a head turn.  Made once for a model, outside of a graph's capture; every layer uses it.
 
     ``rotary_dim``: how many values of a head are turned, the first ones (even, 0 included).  Pair ``i`` turns by
     ``theta ** (-2 i / rotary_dim)`` a position.  ``scaling``: as ``rope_scaling`` in a model's configuration, with ``rope_type``
@@ -98,6 +98,8 @@ class RotaryFrequencies:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("himuon_b200.ops.RotaryFrequencies: they would be copied from the host while a graph is captured; make them before the capture")
         # whole numbers of 2^-64 turns a position: position times this, modulo 2^64, is the place within a turn
         ratios = (f.as_integer_ratio() for f in self.frequencies)
         turns = [((n * 2 ** 65 * 10 ** 50) // (d * TWO_PI_E50) + 1) // 2 % 2 ** 64 for n, d in ratios]

@@ -568,6 +568,189 @@ def test_layer_operators_refusals_on_the_gpu():
     _clean()
 
 
+def test_single_rows_of_any_stride():
+    """A row's stride means nothing where there is one row; tensor maps take none below a row's width."""
+    ops = _ops()
+    torch.manual_seed(71)
+    fns, x, _ = _calls()
+    f = ops.RotaryFrequencies(32, 10000.0)
+    fns["rotary"] = lambda t: ops.rotary(t, 1, f, 2, 32)
+    kept = ops.quantize_fp8((torch.randn(40, 64, device="cuda") * 0.2).bfloat16(), 128)
+    fns["kept"] = lambda t: ops.fp8_linear(t, kept)
+    row = x[:1].contiguous()
+    for name, fn in fns.items():
+        for stride in (0, 8, 1000):
+            odd = torch.as_strided(x.clone(), (1, 64), (stride, 1))
+            assert torch.equal(fn(odd), fn(row)), (name, stride)
+            if name == "kept":
+                continue
+            grads = []
+            for t in (odd, row):
+                leaf = t.detach().requires_grad_()
+                y = fn(leaf)
+                grads.append(torch.autograd.grad(y, leaf, torch.as_strided(torch.ones(40 * 64, device="cuda", dtype=y.dtype), y.shape, (stride % 16, 1)))[0])
+            assert torch.equal(*grads), (name, stride)
+    a, b = ops.quantize_fp8(row), ops.quantize_fp8(row, 128)
+    for stride in (0, 16):
+        odd = torch.as_strided(a.values.clone(), (1, 64), (stride, 1))
+        assert torch.equal(ops.fp8_matmul(a._replace(values=odd), b._replace(values=odd)), ops.fp8_matmul(a, b))
+        assert torch.equal(a._replace(values=odd).dequantize(), a.dequantize())
+    _clean()
+
+
+def test_what_is_kept_goes_through_hooks():
+    """What hooks bring back is used where it is what was kept, and refused where it lies otherwise."""
+    fns, x, _ = _calls()
+    for name, fn in fns.items():
+        leaf = x.clone().requires_grad_()
+        want, = torch.autograd.grad(fn(leaf).sum(), leaf)
+        with torch.autograd.graph.save_on_cpu():
+            y = fn(leaf)
+        assert torch.equal(torch.autograd.grad(y.sum(), leaf)[0], want), name
+        for unpack in (lambda t: t[:-1] if t.dim() else t, lambda t: t.cpu(), lambda t: t.float(), lambda t: torch.cat([t, t])):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                y = fn(leaf)
+            with pytest.raises(RuntimeError, match="himuon"):
+                torch.autograd.grad(y.sum(), leaf)
+    _clean()
+
+
+def test_what_changes_before_the_backward_pass_is_noticed():
+    ops = _ops()
+    torch.manual_seed(73)
+    f, at = ops.RotaryFrequencies(32, 10000.0), torch.arange(14, device="cuda")
+    w = [(torch.randn(*s, device="cuda") * 0.2).bfloat16().requires_grad_() for s in ((40, 64), (40, 64), (64, 40))]
+    x = torch.randn(14, 64, device="cuda").bfloat16().requires_grad_()
+    for y, changed in ((ops.rotary(x, at, f, 2, 32), at), (ops.gated_mlp(x, *w), w[2]), (ops.gated_mlp(x, *w), x)):
+        with torch.no_grad():
+            changed.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    _clean()
+
+
+def test_frequencies_are_not_made_while_a_graph_is_captured():
+    ops = _ops()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    t = torch.zeros(8, device="cuda")
+    with torch.cuda.graph(graph, stream=side):
+        t.add_(1)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            ops.RotaryFrequencies(32)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (t == 1).all()
+
+
+def test_one_matrix_for_gate_and_up():
+    """Gradients of a matrix that is used twice are added up, and again over two passes."""
+    ops = _ops()
+    torch.manual_seed(79)
+    for rows in (20, 100):
+        x = torch.randn(rows, 64, device="cuda").bfloat16()
+        w, d = ((torch.randn(*s, device="cuda") * 0.2).bfloat16() for s in ((40, 64), (64, 40)))
+        v = w.clone()
+        for t in (w, v, d):
+            t.requires_grad_()
+        apart = torch.autograd.grad(ops.gated_mlp(x, w, v, d).sum(), (w, v, d))
+        ops.gated_mlp(x, w, w, d).sum().backward()
+        assert torch.equal(w.grad, apart[0] + apart[1]) and torch.equal(d.grad, apart[2])
+        once = w.grad.clone()
+        ops.gated_mlp(x, w, w, d).sum().backward()
+        assert torch.equal(w.grad, once + once)
+    _clean()
+
+
+def test_layer_operators_from_two_threads():
+    """Two threads on streams of their own, at once."""
+    import threading
+
+    ops = _ops()
+    torch.manual_seed(83)
+    f = ops.RotaryFrequencies(32, 10000.0)
+    jobs = []
+    for rows in (24, 700):
+        x = torch.randn(rows, 640, device="cuda").bfloat16()
+        w = [(torch.randn(*s, device="cuda") * 0.05).bfloat16() for s in ((1728, 640), (1728, 640), (640, 1728))]
+
+        def step(x=x, w=w):
+            leaves = [t.detach().requires_grad_() for t in (x, *w)]
+            y = ops.gated_mlp(ops.rotary(leaves[0], x.shape[0], f, 20, 32), *leaves[1:]) + ops.fp8_linear(ops.fp8_linear(leaves[0], leaves[1]), leaves[3])
+            return torch.autograd.grad(y.sum(), leaves)
+
+        jobs.append((step, step()))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(step, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got = [step() for _ in range(10)]
+                torch.cuda.current_stream().synchronize()
+            wrong.extend(1 for g in got if not _same(g, want))
+        except Exception as e:                             # (a thread's own would be lost)
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    _clean()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values: the last rows are those of a call with nothing else."""
+    ops = _ops()
+    torch.manual_seed(89)
+    rows, cols, tail = 547 * 128, 258 * 128, 256
+    assert rows * cols > 2 ** 31
+    x = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    x[-tail:] = torch.randn(tail, cols, device="cuda")
+    for block in (1, 128):
+        for turned in (False, True):
+            got, want = ops.quantize_fp8(x, block, turned), ops.quantize_fp8(x[-tail:], block, turned)
+            if turned:
+                assert torch.equal(got.values[:, -tail:].view(torch.uint8), want.values.view(torch.uint8)) and torch.equal(got.scales[:, -tail // 128:], want.scales)
+            else:
+                assert torch.equal(got.values[-tail:].view(torch.uint8), want.values.view(torch.uint8)) and torch.equal(got.scales[-tail // block:], want.scales)
+                assert torch.equal(got.dequantize(torch.bfloat16)[-tail:], want.dequantize(torch.bfloat16))
+            del got, want
+    f = ops.RotaryFrequencies(96, 10000.0)
+    at = torch.arange(rows, device="cuda")
+    assert torch.equal(ops.rotary(x, at, f, 258, 128)[-tail:], ops.rotary(x[-tail:], at[-tail:], f, 258, 128))
+    odd = ops.RotaryFrequencies(20, 10000.0)
+    assert torch.equal(ops.rotary(x, at, odd, 258, 128)[-tail:], ops.rotary(x[-tail:], at[-tail:], odd, 258, 128))
+    del x
+    a, b = ops.quantize_fp8(torch.randn(rows, 136, device="cuda")), ops.quantize_fp8(torch.randn(cols, 136, device="cuda"), 128)
+    for powers in (True, False):
+        got = ops.fp8_matmul(a._replace(powers=powers), b)[-tail:, -tail:]
+        last = ops.Fp8Blocks(a.values[-tail:], a.scales[-tail:], 1, powers), ops.Fp8Blocks(b.values[-tail:], b.scales[-tail // 128:], 128, True)
+        assert torch.equal(got, ops.fp8_matmul(*last))
+    _clean()
+
+
+def test_gated_mlp_offsets_beyond_32_bits():
+    ops = _ops()
+    torch.manual_seed(97)
+    rows, hidden, inter, tail = 65536, 64, 17408, 300
+    assert rows * 2 * inter > 2 ** 31
+    w = [(torch.randn(*s, device="cuda") * s[1] ** -0.5).bfloat16().requires_grad_() for s in ((inter, hidden), (inter, hidden), (hidden, inter))]
+    x = torch.randn(rows, hidden, device="cuda").bfloat16().requires_grad_()
+    g = torch.zeros(rows, hidden, device="cuda", dtype=torch.bfloat16)
+    g[-tail:] = torch.randn(tail, hidden, device="cuda")
+    y = ops.gated_mlp(x, *w)
+    got = [y[-tail:].detach()] + [t[-tail:] if i == 0 else t for i, t in enumerate(torch.autograd.grad(y, (x, *w), g))]
+    last = x[-tail:].detach().requires_grad_()
+    z = ops.gated_mlp(last, *w)
+    want = [z.detach(), *torch.autograd.grad(z, (last, *w), g[-tail:])]
+    for a, b in zip(got, want):
+        # sums may be cut elsewhere: two results rounded to bf16, and as much again for fp32 sums in another order
+        assert (a.double() - b.double()).norm() <= 4 * U * b.double().norm()
+    _clean()
+
+
 @pytest.mark.parametrize("rows", [20, 300])
 def test_a_decoder_layer_of_them(rows):
     """Queries and keys of one projection in 8 bits, turned, packed attention, and the feed-forward block: forward and backward against 64 bits."""
