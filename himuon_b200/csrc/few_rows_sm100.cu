@@ -15,8 +15,11 @@
 #include "fp8.h"
 #include "gated_mlp.h"
 #include "himuon.h"
+#include "pair_common.cuh"
 #include "sm100_common.cuh"
 #include "tma_host.h"
+
+#include <type_traits>
 
 namespace himuon {
 
@@ -27,6 +30,7 @@ enum { PLAIN, GATED, EIGHT_BITS };
 constexpr int FEW_WARPS = 7, FEW_THREADS = 32 * (1 + FEW_WARPS);      // warp 0: TMA; then 16 rows of W each (with one more, threads would have 96 registers)
 constexpr int FEW_ROWS = 16 * FEW_WARPS;
 constexpr int FEW_STAGES = 24;
+constexpr int FEW_CUT = 4;               // blocks that share a tile, at most
 constexpr uint32_t FEW_RING = 96 * 1024;
 
 struct FewDev {
@@ -36,9 +40,10 @@ struct FewDev {
   void *y, *gu;                        // (rows, outer) in bf16 or fp32; GATED: g | u or null (gated_mlp.h)
   uint8_t* gu_low;
   int rows, outer, out_fp32, activation;
-  int blocks, kblocks;                 // of 128 bytes, and stages
+  int blocks;                          // of 128 bytes of a row
   int th, tiles, stages;               // rows of W of a tile, tiles of a block, stages of the ring
-  int sub;                             // times 128 bytes of every row in a stage
+  int cut;                             // blocks (a cluster) that a tile's inner dimension is dealt out to
+  int early;                           // W was there before the launch before this one
   int warps, groups;                   // warps that a tile's rows take, and groups of so many, which take stages in turn
   int* status;
 };
@@ -55,6 +60,19 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], 
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&v)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[1]) { asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[0]) : "r"(addr) : "memory"); }
+__device__ __forceinline__ void ld_cluster(uint32_t addr, float (&v)[4]) {
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes, uint32_t e) {
+  asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes), "r"(e) : "memory");
+}
+__device__ __forceinline__ void load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int x, int y, uint32_t e) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}" ::"r"(dst), "l"(tm), "r"(bar), "r"(x), "r"(y), "r"(e)
+      : "memory");
 }
 // 16 bytes of a row of 128, where the swizzle has put them.
 __device__ __forceinline__ uint32_t cell(uint32_t base, int row, int chunk) { return base + row * 128 + ((chunk ^ (row & 7)) << 4); }
@@ -99,37 +117,45 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
   uint8_t* smem = align_up_1024(smem_raw);
   FewBars* bars = reinterpret_cast<FewBars*>(smem + FEW_RING);
   volatile int* abort_flag = &bars->abort_flag;
-  const bool joined = p.groups > 1;
+  const bool joined = p.groups > 1 || p.cut > 1;
+  const int line = p.warps * 16 + 4;                   // of parts: a row of x by all rows of W (4 more, so that a warp's values lie in 32 banks)
   const int warp = warp_id(), lane = threadIdx.x & 31;
-  const int first = static_cast<int>(blockIdx.x) * p.th * p.tiles;
-  const uint32_t w_bytes = static_cast<uint32_t>(p.th) * 128, sub_bytes = MATS * w_bytes + NX * 128, stage_bytes = p.sub * sub_bytes;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < p.stages; ++i) { mbar_init(&bars->full[i], 1); mbar_init(&bars->empty[i], p.warps); }
-    bars->abort_flag = 0;
-    mbar_fence_init();
-  }
+  const int rank = p.cut > 1 ? static_cast<int>(blockIdx.x) % p.cut : 0, first = static_cast<int>(blockIdx.x) / p.cut * p.th * p.tiles;
+  const int kb0 = p.blocks * rank / p.cut, kb1 = p.blocks * (rank + 1) / p.cut;
+  const uint32_t w_bytes = static_cast<uint32_t>(p.th) * 128, stage_bytes = MATS * w_bytes + NX * 128;
+  launch_dependents();
+  if (static_cast<int>(threadIdx.x) < p.stages) { mbar_init(&bars->full[threadIdx.x], 1); mbar_init(&bars->empty[threadIdx.x], p.warps); }
+  if (threadIdx.x == 0) bars->abort_flag = 0;
+  if (warp == 0) mbar_fence_init();
   __syncthreads();
 
   if (warp == 0) {
-    const uint32_t e = elect_one();
-    tma_prefetch_desc(&tmW0);
-    int stage = 0;
-    uint32_t phase = 0;
+    // (a stage costs its bytes' time or this loop's instructions, which take some five cycles each: addresses go along, nothing is worked out anew)
+    const uint32_t e = elect_one(), bytes = MATS * w_bytes + p.rows * 128, ring = smem_u32(smem), full0 = smem_u32(bars->full);
+    const int n = kb1 - kb0, ahead = p.early ? min(p.stages, n) : 0;
+    for (int i = 0; i < ahead; ++i) {                    // W while the kernel before may still be writing x
+      expect(full0 + i * 8, bytes, e);
+      load(ring + i * stage_bytes, &tmW0, full0 + i * 8, (kb0 + i) * PER_SUB, first, e);
+      if (MATS == 2) load(ring + i * stage_bytes + w_bytes, &tmW1, full0 + i * 8, (kb0 + i) * PER_SUB, first, e);
+    }
+    wait_for_previous();
+    for (int i = 0; i < ahead; ++i) load(ring + i * stage_bytes + MATS * w_bytes, &tmX, full0 + i * 8, (kb0 + i) * PER_SUB, 0, e);
+    int stage = ahead;
+    uint32_t phase = 1, at = ring + ahead * stage_bytes, bar = full0 + ahead * 8;
     bool ok = true;
-    for (int tile = 0; ok && tile < p.tiles && first + tile * p.th < p.outer; ++tile) {
-      const int f0 = first + tile * p.th;
-      for (int kb = 0; kb < p.kblocks; ++kb) {
-        if (!mbar_wait_warp(&bars->empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
-        uint8_t* at = smem + stage * stage_bytes;
-        mbar_expect_tx(&bars->full[stage], stage_bytes, e);
+    for (int tile = 0, f0 = first; ok && tile < p.tiles && f0 < p.outer; ++tile, f0 += p.th) {
+      int k = (kb0 + (tile == 0 ? ahead : 0)) * PER_SUB;
 #pragma unroll 1
-        for (int u = 0; u < p.sub; ++u, at += sub_bytes) {
-          const int k = (kb * p.sub + u) * PER_SUB;      // (behind the last value: zeros)
-          tma_load_3d(at, &tmW0, &bars->full[stage], k, f0, 0, e);
-          if (MATS == 2) tma_load_3d(at + w_bytes, &tmW1, &bars->full[stage], k, f0, 0, e);
-          tma_load_3d(at + MATS * w_bytes, &tmX, &bars->full[stage], k, 0, 0, e);
-        }
-        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      for (int left = n - (tile == 0 ? ahead : 0); left > 0; --left, k += PER_SUB) {      // (behind the last value: zeros)
+        if (stage == p.stages) { stage = 0; phase ^= 1; at = ring; bar = full0; }
+        if (!mbar_wait_warp(&bars->empty[stage], phase, abort_flag, p.status, 1)) { ok = false; break; }
+        expect(bar, bytes, e);
+        load(at, &tmW0, bar, k, f0, e);
+        if (MATS == 2) load(at + w_bytes, &tmW1, bar, k, f0, e);
+        load(at + MATS * w_bytes, &tmX, bar, k, 0, e);
+        ++stage;
+        at += stage_bytes;
+        bar += 8;
       }
     }
   } else {
@@ -140,60 +166,84 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     int stage = group;                                   // (groups take turns; stages are a multiple of them)
     uint32_t phase = 0;
     bool ok = group < p.groups;
+    if (KIND == EIGHT_BITS) wait_for_previous();         // (scales of x)
     for (int tile = 0; tile < p.tiles && first + tile * p.th < p.outer; ++tile) {
       const int f0 = first + tile * p.th;
       float acc[MATS][NT][4] = {};
       const float *sw0 = nullptr, *sw1 = nullptr;
-      float by_w[2] = {}, by_x[NT][2] = {};
+      float by_w[2] = {}, by_x[NT][2] = {}, next_w[2] = {}, next_x[NT][2] = {};
       const bool x_blocks = p.x_block > 1;                 // (of 128 rows: the first has them all)
       auto load_scales = [&](int block) {
         const int at = min(block, p.blocks - 1);
-        by_w[0] = __ldg(sw0 + at * p.sw_col);
-        by_w[1] = __ldg(sw1 + at * p.sw_col);
+        next_w[0] = __ldg(sw0 + at * p.sw_col);
+        next_w[1] = __ldg(sw1 + at * p.sw_col);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) by_x[n][j] = __ldg(p.sx + (x_blocks ? 0 : min(n * 8 + 2 * t + j, p.rows - 1)) * p.sx_row + at * p.sx_col);
+          for (int j = 0; j < 2; ++j) next_x[n][j] = __ldg(p.sx + (x_blocks ? 0 : min(n * 8 + 2 * t + j, p.rows - 1)) * p.sx_row + at * p.sx_col);
       };
       if constexpr (KIND == EIGHT_BITS) {
         sw0 = p.sw + static_cast<long long>(min(f0 + m0 + r, p.outer - 1) / 128) * p.sw_row;
         sw1 = p.sw + static_cast<long long>(min(f0 + m0 + r + 8, p.outer - 1) / 128) * p.sw_row;
+        load_scales(kb0 + group);
       }
-      for (int kb = group; ok && kb < p.kblocks; kb += p.groups) {
-        if constexpr (KIND == EIGHT_BITS) load_scales(kb * p.sub);           // (on their way while the stage is waited for)
+      for (int kb = kb0 + group; ok && kb < kb1; kb += p.groups) {
+        if constexpr (KIND == EIGHT_BITS) {                  // (those of a turn are on their way during the one before)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            by_w[j] = next_w[j];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) by_x[n][j] = next_x[n][j];
+          }
+          load_scales(kb + p.groups);
+        }
         if (!mbar_wait_warp(&bars->full[stage], phase, abort_flag, p.status, 3)) { ok = false; break; }
         constexpr int NN = NT < 4 ? NT : KIND == EIGHT_BITS ? 2 : 4;              // groups of x at a time: more would not fit in the registers of two blocks
+        const uint32_t base = ring + stage * stage_bytes, x_base = base + MATS * w_bytes;
+        // With few rows a turn is latency: all of its operands are asked for before the first product, and 8-bit products go to two sums.
+        constexpr int HALVES = NT <= 2 ? 2 : 1, AHEAD = NT <= 2 ? 4 : 1, CHAINS = NT <= 2 ? 2 : 1;
+#pragma unroll
+        for (int n0 = 0; n0 < NT; n0 += NN) {
+          float c[CHAINS][NN][4] = {};
 #pragma unroll 1
-        for (int u = 0; u < p.sub; ++u) {
-          if (KIND == EIGHT_BITS && u > 0) load_scales(kb * p.sub + u);
-          const uint32_t base = ring + stage * stage_bytes + u * sub_bytes, x_base = base + MATS * w_bytes;
+          for (int half = 0; half < 2; half += HALVES) {
+            uint32_t b[HALVES][NN][4];
 #pragma unroll
-          for (int n0 = 0; n0 < NT; n0 += NN) {
-            float c[NN][4] = {};
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-              uint32_t b[NN][4];
+            for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-              for (int n = 0; n < NN; ++n) ldmatrix4(b[n], cell(x_base, (n0 + n) * 8 + b_row, half * 4 + b_chunk));
+              for (int n = 0; n < NN; ++n) ldmatrix4(b[h][n], cell(x_base, (n0 + n) * 8 + b_row, (half + h) * 4 + b_chunk));
 #pragma unroll
-              for (int k = 0; k < 2; ++k)
+            for (int k0 = 0; k0 < 2 * HALVES; k0 += AHEAD) {
+              uint32_t a[AHEAD][MATS][4];
+              auto products = [&](int m, int k) {
 #pragma unroll
-                for (int m = 0; m < MATS; ++m) {
-                  uint32_t a[4];
-                  ldmatrix4(a, cell(base + m * w_bytes, a_row, half * 4 + k * 2 + a_chunk));
-#pragma unroll
-                  for (int n = 0; n < NN; ++n) {
-                    if constexpr (KIND == EIGHT_BITS) mma_e4m3(c[n], a, b[n][2 * k], b[n][2 * k + 1]);
-                    else mma_bf16(acc[m][n0 + n], a, b[n][2 * k], b[n][2 * k + 1]);
-                  }
+                for (int n = 0; n < NN; ++n) {
+                  const uint32_t b0 = b[(k0 + k) / 2][n][2 * ((k0 + k) % 2)], b1 = b[(k0 + k) / 2][n][2 * ((k0 + k) % 2) + 1];
+                  if constexpr (KIND == EIGHT_BITS) mma_e4m3(c[k % CHAINS][n], a[k][m], b0, b1);
+                  else mma_bf16(acc[m][n0 + n], a[k][m], b0, b1);
                 }
-            }
-            if constexpr (KIND == EIGHT_BITS) {
+              };
 #pragma unroll
-              for (int n = 0; n < NN; ++n)
+              for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[0][n0 + n][j] = fmaf(c[n][j], by_w[j >> 1] * by_x[n0 + n][j & 1], acc[0][n0 + n][j]);
+                for (int k = 0; k < AHEAD; ++k) {
+                  ldmatrix4(a[k][m], cell(base + m * w_bytes, a_row, half * 4 + (k0 + k) * 2 + a_chunk));
+                  if (AHEAD == 1) products(m, k);
+                }
+              if (AHEAD > 1) {
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+                  for (int m = 0; m < MATS; ++m) products(m, k);
+              }
             }
+          }
+          if constexpr (KIND == EIGHT_BITS) {
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                acc[0][n0 + n][j] = fmaf(CHAINS == 2 ? c[0][n][j] + c[CHAINS - 1][n][j] : c[0][n][j], by_w[j >> 1] * by_x[n0 + n][j & 1], acc[0][n0 + n][j]);
           }
         }
         __syncwarp();
@@ -214,33 +264,53 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
       } else {                                           // (one tile: the ring has been read to its end by all warps that the barrier waits for)
         named_barrier(1, 32 * FEW_WARPS);
         if (group < p.groups) {
-          float* s_part = reinterpret_cast<float*>(smem) + group * MATS * p.warps * 16 * (NX + 1);
+          float* s_part = reinterpret_cast<float*>(smem) + group * MATS * NX * line;
 #pragma unroll
           for (int m = 0; m < MATS; ++m)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) s_part[(m * p.warps * 16 + m0 + r + 8 * (j >> 1)) * (NX + 1) + n * 8 + 2 * t + (j & 1)] = acc[m][n][j];
+              for (int j = 0; j < 4; ++j) s_part[(m * NX + n * 8 + 2 * t + (j & 1)) * line + m0 + r + 8 * (j >> 1)] = acc[m][n][j];
         }
       }
       if (!ok && group < p.groups) break;
     }
   }
   if (!joined) return;
-  // the groups' parts, neighbouring features next to one another
-  __syncthreads();
-  const float* s_part = reinterpret_cast<const float*>(smem);
-  const int out = p.th * p.rows, high = p.warps * 16;
-  for (int o = static_cast<int>(threadIdx.x); o < out; o += FEW_THREADS) {
-    const int row = o / p.th, f = o - row * p.th;
-    float v[MATS];
+  // the groups' parts, of all blocks of the cluster, neighbouring features next to one another; the blocks share the results
+  __syncwarp();
+  if (p.cut > 1) cluster_sync_all();
+  else __syncthreads();
+  const uint32_t parts = smem_u32(smem), step = MATS * NX * line * 4, of_w1 = (MATS - 1) * NX * line * 4;
+  // V neighbouring features a thread: four where that leaves one for each thread (24 rows of 40 features: 1.2 us for 2.4 one by one), else one
+  auto join = [&](auto width) {
+    constexpr int V = decltype(width)::value;
+    const int line_of = p.th / V, out = line_of * p.rows;
+    for (int o = rank * FEW_THREADS + static_cast<int>(threadIdx.x); o < out; o += p.cut * FEW_THREADS) {
+      const int row = o / line_of, f = (o - row * line_of) * V;
+      float v[MATS][V] = {};
+      const uint32_t at = parts + (row * line + f) * 4;
+      for (int g = 0; g < p.groups; ++g)
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) v[m] = 0.f;
-    for (int g = 0; g < p.groups; ++g)
+        for (int m = 0; m < MATS; ++m) {
+          float u[FEW_CUT][V];
 #pragma unroll
-      for (int m = 0; m < MATS; ++m) v[m] += s_part[((g * MATS + m) * high + f) * (NX + 1) + row];
-    put_result<KIND>(p, first + f, row, v[0], v[MATS - 1]);
-  }
+          for (int c = 0; c < FEW_CUT; ++c)
+            if (c < p.cut) ld_cluster((p.cut > 1 ? map_to_cta(at, c) : at) + g * step + m * of_w1, u[c]);
+#pragma unroll
+          for (int c = 0; c < FEW_CUT; ++c)
+            if (c < p.cut)
+#pragma unroll
+              for (int i = 0; i < V; ++i) v[m][i] += u[c][i];
+        }
+#pragma unroll
+      for (int i = 0; i < V; ++i) put_result<KIND>(p, first + f + i, row, v[0][i], v[MATS - 1][i]);
+    }
+  };
+  if (p.th * p.rows >= 2 * FEW_THREADS * p.cut) join(std::integral_constant<int, 4>{});
+  else join(std::integral_constant<int, 1>{});
+  __syncwarp();
+  if (p.cut > 1) cluster_sync_all();   // (nobody leaves while others read its parts)
 }
 
 struct FewOperands {
@@ -249,43 +319,60 @@ struct FewOperands {
   int inner = 0, esz = 2;                                // values of a row and their bytes
 };
 CUtensorMap few_map(const void* ptr, int rows, const FewOperands& o, long long ld, int box_rows) {
-  const uint64_t dims[3] = {static_cast<uint64_t>(o.inner), static_cast<uint64_t>(rows), 1};
-  const uint64_t strides[2] = {static_cast<uint64_t>(ld), static_cast<uint64_t>(ld) * static_cast<uint64_t>(rows)};
-  const uint32_t box[3] = {static_cast<uint32_t>(128 / o.esz), static_cast<uint32_t>(box_rows), 1};
-  return make_tmap(ptr, 3, dims, strides, box, o.esz, true);
+  const uint64_t dims[2] = {static_cast<uint64_t>(o.inner), static_cast<uint64_t>(rows)}, strides[1] = {static_cast<uint64_t>(ld)};
+  const uint32_t box[2] = {static_cast<uint32_t>(128 / o.esz), static_cast<uint32_t>(box_rows)};
+  return make_tmap(ptr, 2, dims, strides, box, o.esz, true);
 }
 
 template <int KIND, int NT>
 void launch(const FewOperands& o, FewDev p, cudaStream_t s) {
   constexpr int MATS = KIND == GATED ? 2 : 1, NX = NT * 8;
   constexpr size_t SMEM = 1024 + FEW_RING + sizeof(FewBars);
-  static_assert(2 * SMEM <= 232448 && MATS * FEW_ROWS * (NX + 1) * sizeof(float) <= FEW_RING &&
+  static_assert(2 * SMEM <= 232448 && MATS * NX * (FEW_ROWS + 4 * FEW_WARPS) * sizeof(float) <= FEW_RING &&
                     (MATS * FEW_ROWS + kFewProductRows) * 128 <= FEW_RING, "shared memory of two blocks exceeded");
   const auto kernel = few_rows_kernel<KIND, NT>;
   p.blocks = (o.inner * o.esz + 127) / 128;
   // Rows of W in equal shares over two blocks a SM, in tiles of up to FEW_ROWS.
-  const int slots = 2 * num_sms(), share = ((p.outer + slots - 1) / slots + 7) / 8 * 8;
+  // Where that leaves a block fewer than 32 rows, so that x would be as much to load as W, blocks share tiles instead.
+  const int slots = 2 * num_sms();
+  p.cut = 1;
+  while (p.cut < FEW_CUT && static_cast<long long>(p.outer) * p.cut < 24LL * slots && p.blocks >= 32 * p.cut) p.cut *= 2;
+  const int share = static_cast<int>((static_cast<long long>(p.outer) * p.cut + slots - 1) / slots + 7) / 8 * 8;
   p.tiles = (share + FEW_ROWS - 1) / FEW_ROWS;
   p.th = ((share + p.tiles - 1) / p.tiles + 7) / 8 * 8;
   p.warps = (p.th + 15) / 16;
   // Bytes of a stage and groups go by the weight alone (with the most rows of x that there may be), since what a group has, and with it the order of sums, does.
   const int weight = MATS * p.th * 128;
-  p.sub = weight >= 4096 ? 1 : 2;
-  const int least = static_cast<int>(FEW_RING) / (p.sub * (weight + kFewProductRows * 128));
+  const int least = static_cast<int>(FEW_RING) / (weight + kFewProductRows * 128);
   p.groups = p.tiles > 1 ? 1 : FEW_WARPS / p.warps < least ? FEW_WARPS / p.warps : least;
   const int sub_bytes = weight + NX * 128;
-  p.kblocks = (p.blocks + p.sub - 1) / p.sub;
-  const int fit = static_cast<int>(FEW_RING) / (p.sub * sub_bytes);
+  const int fit = static_cast<int>(FEW_RING) / sub_bytes;
   p.stages = fit < FEW_STAGES ? fit : FEW_STAGES;
   // (A stage is always the same group's: a group that met another's could be a whole round ahead of it, where a barrier's phases look alike.)
   p.stages -= p.stages % p.groups;
   p.status = status_word_ptr();
-  const long long group = static_cast<long long>(p.th) * p.tiles;
-  const CUtensorMap tx = few_map(o.x, p.rows, o, o.ld_x, NX), t0 = few_map(o.w0, p.outer, o, o.ld_w0, p.th), t1 = MATS == 2 ? few_map(o.w1, p.outer, o, o.ld_w1, p.th) : t0;
+  const long long group = static_cast<long long>(p.th) * p.tiles, grid = (p.outer + group - 1) / group * p.cut;
+  const CUtensorMap tx = few_map(o.x, p.rows, o, o.ld_x, p.rows), t0 = few_map(o.w0, p.outer, o, o.ld_w0, p.th), t1 = MATS == 2 ? few_map(o.w1, p.outer, o, o.ld_w1, p.th) : t0;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
   if (e == cudaSuccess) {
-    kernel<<<static_cast<int>((p.outer + group - 1) / group), FEW_THREADS, SMEM, s>>>(tx, t0, t1, p);
-    e = cudaGetLastError();
+    cudaLaunchAttribute attrs[2];
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(FEW_THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = s;
+    cfg.attrs = attrs;
+    if (p.early) {
+      attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (p.cut > 1) {
+      attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+      attrs[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(p.cut);
+      attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
+      ++cfg.numAttrs;
+    }
+    e = cudaLaunchKernelEx(&cfg, kernel, tx, t0, t1, p);
   }
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon product of few rows: launch failed: ") + cudaGetErrorString(e));
 }
@@ -300,11 +387,11 @@ void launch_rows(const FewOperands& o, const FewDev& p, cudaStream_t s) {
 
 }  // namespace
 
-void few_rows_product(const void* x, long long ld_x, const void* w, long long ld_w, void* y, int rows, int inner, int outer, cudaStream_t s) {
+void few_rows_product(const void* x, long long ld_x, const void* w, long long ld_w, void* y, int rows, int inner, int outer, bool early, cudaStream_t s) {
   FewOperands o;
   o.x = x; o.ld_x = 2 * ld_x; o.w0 = w; o.ld_w0 = 2 * ld_w; o.inner = inner;
   FewDev p{};
-  p.y = y; p.rows = rows; p.outer = outer;
+  p.y = y; p.rows = rows; p.outer = outer; p.early = early;
   launch_rows<PLAIN>(o, p, s);
 }
 
@@ -318,14 +405,14 @@ void few_rows_gated_up(const GatedUpArgs& a, cudaStream_t s) {
   launch_rows<GATED>(o, p, s);
 }
 
-void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, cudaStream_t s) {
+void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, bool early, cudaStream_t s) {
   if (a.cols != b.cols || b.block_rows != 128) throw std::runtime_error("himuon fp8_product: bad sizes");
   FewOperands o;
   o.x = a.values; o.ld_x = a.ld; o.w0 = b.values; o.ld_w0 = b.ld; o.inner = a.cols; o.esz = 1;
   FewDev p{};
   p.sx = a.scales; p.sx_row = a.scale_row; p.sx_col = a.scale_col; p.x_block = a.block_rows;
   p.sw = b.scales; p.sw_row = b.scale_row; p.sw_col = b.scale_col;
-  p.y = c; p.out_fp32 = out_fp32;
+  p.y = c; p.out_fp32 = out_fp32; p.early = early;
   p.rows = a.rows; p.outer = b.rows;
   launch_rows<EIGHT_BITS>(o, p, s);
 }

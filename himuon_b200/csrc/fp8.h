@@ -34,8 +34,9 @@ void fp8_dequantize(const Fp8Matrix& m, void* out, long long ld_out, int out_fp3
 // tiles that are cut along the inner dimension (none are without).
 void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c, int out_fp32, int powers, float* parts, cudaStream_t s);
 long long fp8_parts_floats(const Fp8Matrix& a, const Fp8Matrix& b);
-// The same for a few rows of a; c is contiguous.  (33 to 64 rows have as many accumulators as a thread has registers: they are the large kernel's.)
+// The same for a few rows of a; c is contiguous.  `early`: b was there before the launch that comes before this one on the stream, and may be read while that still
+// runs.  (33 to 64 rows have as many accumulators as a thread has registers: they are the large kernel's.)
 constexpr int kFewFp8Rows = 32;
-void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, cudaStream_t s);
+void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, bool early, cudaStream_t s);
 
 }  // namespace himuon

@@ -115,6 +115,7 @@ __device__ __forceinline__ uint32_t largest_of(uint32_t m) {
 constexpr int RUN = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(Fp8QuantizeArgs a, int runs, int blocks_c, long long total, int aligned) {
+  launch_dependents();
   const long long id = static_cast<long long>(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const bool mine = id < total;                        // (all 32 lanes meet in the shuffles)
   const long long row = mine ? id / runs : 0;
@@ -146,6 +147,7 @@ __global__ void __launch_bounds__(256) fp8_quantize_rows_kernel(Fp8QuantizeArgs 
 // Any copies: STRAIGHT and TURNED are the rows of their blocks, or 0 for none.
 template <typename T, int STRAIGHT, int TURNED>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(Fp8QuantizeArgs a, int tiles_c, int aligned) {
+  launch_dependents();
   __shared__ uint32_t s_col[QT];
   __shared__ uint32_t s_all;
   __shared__ uint2 s_turned[TURNED ? QT * 16 : 1];     // [column][group of 8 rows, swizzled]

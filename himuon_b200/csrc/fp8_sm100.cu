@@ -108,6 +108,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   cluster_sync_all();                // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  wait_for_previous();               // (launched while what makes the operands may still run)
   const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, total = p.tiles_m * p.tiles_n;
 
   if (warp < 4) {
@@ -325,6 +326,7 @@ fp8_powers_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   cluster_sync_all();                // the peer's barriers exist before anything signals them
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  wait_for_previous();               // (launched while what makes the operands may still run)
   const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
 
   if (warp < 4) {
@@ -589,6 +591,21 @@ static int pairs_at_once(Kernel kernel, int threads, size_t smem, std::atomic<in
   return n;
 }
 
+// A launch that may begin before the kernel before it has ended (it waits for it itself).
+template <class... Params, class... Args>
+static cudaError_t launch_over(void (*kernel)(Params...), int blocks, int threads, size_t smem, cudaStream_t s, const Args&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 static void check(cudaError_t e) {
   if (e != cudaSuccess) throw std::runtime_error(std::string("himuon fp8_product: ") + cudaGetErrorString(e));
 }
@@ -631,8 +648,7 @@ static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
       const uint32_t box[3] = {32, BM, 1};
       tp = make_tmap(parts, 3, dims, strides, box, 4, true);
     }
-    kernel<<<2 * (p.items < pairs ? p.items : pairs), THREADS, SMEM, s>>>(ta, tb, tc, tp, p);
-    check(cudaGetLastError());
+    check(launch_over(kernel, 2 * (p.items < pairs ? p.items : pairs), THREADS, SMEM, s, ta, tb, tc, tp, p));
     if (n) {
       using T = std::conditional_t<F32, float, __nv_bfloat16>;
       fp8_join_kernel<T><<<n / p.cuts * 64, 256, 0, s>>>(parts, static_cast<T*>(c), ld_c, p);
@@ -640,8 +656,7 @@ static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
     }
   } else {
     const int total = p.tiles_m * p.tiles_n;
-    kernel<<<2 * (total < pairs ? total : pairs), THREADS, SMEM, s>>>(ta, tb, tc, p);
-    check(cudaGetLastError());
+    check(launch_over(kernel, 2 * (total < pairs ? total : pairs), THREADS, SMEM, s, ta, tb, tc, p));
   }
 }
 

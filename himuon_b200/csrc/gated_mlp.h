@@ -31,8 +31,9 @@ struct GatedDownGradArgs {
 void gated_down_grad(const GatedDownGradArgs& a, cudaStream_t s);
 
 // Products with a few rows (up to kFewProductRows), whose weight is all that counts: y = x w^T in bf16, or gated_up().
+// `early`: w was there before the launch that comes before this one on the stream, and may be read while that still runs.
 constexpr int kFewProductRows = 64;
-void few_rows_product(const void* x, long long ld_x, const void* w, long long ld_w, void* y, int rows, int inner, int outer, cudaStream_t s);
+void few_rows_product(const void* x, long long ld_x, const void* w, long long ld_w, void* y, int rows, int inner, int outer, bool early, cudaStream_t s);
 void few_rows_gated_up(const GatedUpArgs& a, cudaStream_t s);
 
 }  // namespace himuon

@@ -132,7 +132,7 @@ at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Te
   a.rows = static_cast<int>(n.rows); a.hidden = static_cast<int>(n.hidden); a.inter = static_cast<int>(n.inter); a.activation = static_cast<int>(activation);
   if (n.rows <= himuon::kFewProductRows) {
     himuon::few_rows_gated_up(a, cur_stream());
-    himuon::few_rows_product(h.data_ptr(), n.inter, wd.data_ptr(), wd.stride(0), y.data_ptr(), a.rows, a.inter, a.hidden, cur_stream());
+    himuon::few_rows_product(h.data_ptr(), n.inter, wd.data_ptr(), wd.stride(0), y.data_ptr(), a.rows, a.inter, a.hidden, true, cur_stream());
   } else {
     himuon::gated_up(a, cur_stream());
     gemm_into(h, wd, y, false, true);
@@ -191,6 +191,7 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
       g.M = a.rows; g.N = a.hidden; g.K = a.inter;
       g.lda = 2 * n.inter; g.ldb = wg.stride(0); g.ldb2 = wu.stride(0); g.ldc = n.hidden;
       g.b_mn = true;
+      g.ordered = 1;                                     // (so that few tiles are cut along the inner dimension too)
       at::Tensor parts;
       if (const int64_t floats = himuon::gemm2_parts_floats(g)) {
         parts = at::empty({floats}, x.options().dtype(at::kFloat));
@@ -309,7 +310,8 @@ Fp8 fp8_given(const char* op, const at::Tensor& values, const at::Tensor& scales
   return q;
 }
 // a b^T in bf16 or fp32.
-at::Tensor product(const char* op, const Fp8& a, const Fp8& b, bool out_fp32) {
+// `early`: b was there before the launch before this one, which makes a.
+at::Tensor product(const char* op, const Fp8& a, const Fp8& b, bool out_fp32, bool early = false) {
   TORCH_CHECK(a.m.cols == b.m.cols, "himuon: ", op, ": inner dimensions disagree");
   TORCH_CHECK(b.m.block_rows == 128, "himuon: ", op, ": the second operand needs blocks of 128 rows");
   const c10::cuda::CUDAGuard guard(a.values.device());
@@ -320,7 +322,7 @@ at::Tensor product(const char* op, const Fp8& a, const Fp8& b, bool out_fp32) {
   autograd_launched += 1;
   if (rows <= himuon::kFewFp8Rows) {
     at::Tensor c = at::empty({rows, cols}, type);
-    himuon::few_rows_fp8_product(a.m, b.m, c.data_ptr(), out_fp32, cur_stream());
+    himuon::few_rows_fp8_product(a.m, b.m, c.data_ptr(), out_fp32, early, cur_stream());
     return c;
   }
   // (rows of the result are stored in groups of 16 bytes)
@@ -354,7 +356,7 @@ at::Tensor fp8_linear_kept(const at::Tensor& x, const at::Tensor& w, const at::T
   const Fp8 v = fp8_given("fp8_linear", w, w_scales, w_block, w_powers, x.device(), true);
   const Fp8 q = fp8_piece(x, x.size(0), x.size(1), 1);
   quantize(x, &q, nullptr);
-  return product("fp8_linear", q, v, false);
+  return product("fp8_linear", q, v, false, true);
 }
 // x w^T with both put into 8 bits; copies turned around for the gradients' products are made on the way.
 at::Tensor fp8_linear_forward(const at::Tensor& x, const at::Tensor& w, const Fp8* xt, const Fp8* wt) {

@@ -106,6 +106,12 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes, ui
                : "memory");
 }
 
+// ---------------------------------------------------------------- launches that overlap
+// The next kernel of the stream, if it was launched for it, may start from here on; it has to wait for this one before it touches what this one writes.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Returns when the kernels before have ended and what they wrote can be seen (at once in a kernel that was not launched for overlap).
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- TMA (no multicast anywhere)
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* tmap, uint64_t* bar, int x, int y,
                                             int z) {
