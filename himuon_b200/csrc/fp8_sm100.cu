@@ -41,7 +41,7 @@ struct Fp8Dev {
   long long sa_row, sa_col, sb_row, sb_col;
   int a_block;                       // rows of a block of a
   int rows, cols, tiles_m, tiles_n, kblocks, band;
-  int whole, items, cuts;            // fp8_powers_kernel: tiles that are taken whole, and each of the others in so many parts along the inner dimension
+  int whole, items, cuts;            // tiles that are taken whole, and each of the others in so many parts along the inner dimension
   int* status;
 };
 
@@ -83,7 +83,8 @@ constexpr uint32_t idesc_e4m3(int m, int n) { return (1u << 4) | (static_cast<ui
 
 template <bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
-fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC, Fp8Dev p) {
+fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+                   const __grid_constant__ CUtensorMap tmParts, Fp8Dev p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_up_1024(smem_raw);
   uint8_t* slabs = smem + F8_STAGES * F8_STAGE;
@@ -109,7 +110,7 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   wait_for_previous();               // (launched while what makes the operands may still run)
-  const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, total = p.tiles_m * p.tiles_n;
+  const int first = blockIdx.x >> 1, n_pairs = gridDim.x >> 1;
 
   if (warp < 4) {
   registers_down<F8_REGS_FEW>();
@@ -121,11 +122,10 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = first; ok && tile < total; tile += n_pairs) {
-      int mt, nt;
-      tile_at(p, tile, mt, nt);
-      const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + static_cast<int>(rank) * BM;
-      for (int kb = 0; kb < p.kblocks; ++kb) {
+    for (int item = first; ok && item < p.items; item += n_pairs) {
+      const F8Item w = item_at(p, item);
+      const int m0 = w.mt * 256 + static_cast<int>(rank) * BM, n0 = w.nt * 256 + static_cast<int>(rank) * BM;
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
         if (!mbar_wait_warp(&done[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
         uint8_t* sA = smem + stage * F8_STAGE;
         mbar_expect_tx(&full[stage], 2 * F8_STAGE, leader ? e : 0);
@@ -144,8 +144,9 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = first; ok && tile < total; tile += n_pairs) {
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+      for (int item = first; ok && item < p.items; item += n_pairs) {
+        const F8Item w = item_at(p, item);
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait_warp(&full[stage], phase, abort_flag, p.status, 2) || !mbar_wait_warp(&tempty[acc], acc_phase ^ 1, abort_flag, p.status, 2)) { ok = false; break; }
           tc_fence_after();
           const uint64_t a_desc = desc_at(a_desc0, stage * F8_STAGE), b_desc = desc_at(b_desc0, stage * F8_STAGE);
@@ -174,23 +175,22 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     int acc = 0, stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = first; ok && tile < total; tile += n_pairs) {
-      int mt, nt;
-      tile_at(p, tile, mt, nt);
-      const int m0 = mt * 256 + static_cast<int>(rank) * BM, n0 = nt * 256 + group * 128;
+    for (int item = first; ok && item < p.items; item += n_pairs) {
+      const F8Item w = item_at(p, item);
+      const int m0 = w.mt * 256 + static_cast<int>(rank) * BM, n0 = w.nt * 256 + group * 128;
       const int row = m0 + row_in_tile;
       const bool mine = row < p.rows && n0 < p.cols;           // (else there is nothing to scale: zeros)
       const float* sa = p.sa + static_cast<long long>(mine ? row / p.a_block : 0) * p.sa_row;
       const float* sb = p.sb + static_cast<long long>(mine ? n0 / 128 : 0) * p.sb_row;
-      float next_a = sa[0], next_b = sb[0];                    // (multiplied when they are used, a block later: they take their time)
+      float next_a = sa[w.kb0 * p.sa_col], next_b = sb[w.kb0 * p.sb_col];                    // (multiplied when they are used, a block later: they take their time)
       f32x2 c[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) c[j] = pack2(0.f, 0.f);
 #pragma unroll 1
-      for (int kb = 0; kb < p.kblocks; ++kb) {
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
         const float by = mine ? next_a * next_b : 0.f;
         const f32x2 scale = pack2(by, by);
-        const int ahead = min(kb + 1, p.kblocks - 1);
+        const int ahead = min(kb + 1, w.kb1 - 1);
         next_a = __ldg(sa + ahead * p.sa_col);
         next_b = __ldg(sb + ahead * p.sb_col);
         ok = mbar_wait(&done[stage], phase, abort_flag, p.status, 3);
@@ -214,31 +214,47 @@ fp8_product_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       ok = named_barrier_and(1 + 2 * group, 128, ok);
       if (!ok) break;
       if (m0 >= p.rows) continue;                              // uniform
+      const bool part = w.part >= 0;                           // (all of a part is stored, which costs less than to ask)
+      if (F32 || part) {
 #pragma unroll
-      for (int sl = 0; sl < (F32 ? 4 : 2); ++sl) {             // slabs of 32 or 64 columns
-        const int col = n0 + sl * (F32 ? 32 : 64);
+        for (int sl = 0; sl < 4; ++sl) {                       // slabs of 32 columns
+          const int col = sl * 32;
+          if (!part && n0 + col >= p.cols) break;
+          if (issuer) tma_store_wait_read<0>();
+          named_barrier(1 + 2 * group, 128);                   // the slab is free
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float f[4];
+            unpack2(c[sl * 16 + 2 * j], f[0], f[1]);
+            unpack2(c[sl * 16 + 2 * j + 1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(my_row + ((j ^ (row_in_tile & 7)) << 4)) = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+          }
+          fence_proxy_async_smem();
+          named_barrier(2 + 2 * group, 128);                   // the slab is complete
+          if (issuer) {
+            if (part) tma_store_3d(&tmParts, slab, group * 128 + col, w.part * 256 + static_cast<int>(rank) * BM, 0);
+            else tma_store_3d(&tmC, slab, n0 + col, m0, 0);
+            tma_store_commit();
+          }
+        }
+        continue;
+      }
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {                         // slabs of 64 columns
+        const int col = n0 + sl * 64;
         if (col >= p.cols) break;
         if (issuer) tma_store_wait_read<0>();
         named_barrier(1 + 2 * group, 128);                     // the slab is free
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          uint4 o;
-          if constexpr (F32) {
-            float f[4];
-            unpack2(c[sl * 16 + 2 * j], f[0], f[1]);
-            unpack2(c[sl * 16 + 2 * j + 1], f[2], f[3]);
-            o = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-          } else {
-            uint32_t w[4];
+          uint32_t o[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              float lo, hi;
-              unpack2(c[sl * 32 + 4 * j + t], lo, hi);
-              w[t] = pack_bf16x2(lo, hi);
-            }
-            o = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int t = 0; t < 4; ++t) {
+            float lo, hi;
+            unpack2(c[sl * 32 + 4 * j + t], lo, hi);
+            o[t] = pack_bf16x2(lo, hi);
           }
-          *reinterpret_cast<uint4*>(my_row + ((j ^ (row_in_tile & 7)) << 4)) = o;
+          *reinterpret_cast<uint4*>(my_row + ((j ^ (row_in_tile & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         named_barrier(2 + 2 * group, 128);                     // the slab is complete
@@ -638,25 +654,20 @@ static void launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
   constexpr int THREADS = POWERS ? MX_THREADS : F8_THREADS;
   check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM)));
   const int pairs = pairs_at_once(kernel, THREADS, SMEM, most), most_pairs = pairs < num_sms() / 2 ? pairs : num_sms() / 2;
-  if constexpr (POWERS) {
-    plan_cuts(p, parts ? most_pairs : 1);                // (as many parts as fp8_parts_floats() counts)
-    CUtensorMap tp = tc;
-    const int n = p.items - p.whole;
-    if (n) {
-      const uint64_t dims[3] = {256, static_cast<uint64_t>(n) * 256, 1};
-      const uint64_t strides[2] = {256 * sizeof(float), dims[1] * 256 * sizeof(float)};
-      const uint32_t box[3] = {32, BM, 1};
-      tp = make_tmap(parts, 3, dims, strides, box, 4, true);
-    }
-    check(launch_over(kernel, 2 * (p.items < pairs ? p.items : pairs), THREADS, SMEM, s, ta, tb, tc, tp, p));
-    if (n) {
-      using T = std::conditional_t<F32, float, __nv_bfloat16>;
-      fp8_join_kernel<T><<<n / p.cuts * 64, 256, 0, s>>>(parts, static_cast<T*>(c), ld_c, p);
-      check(cudaGetLastError());
-    }
-  } else {
-    const int total = p.tiles_m * p.tiles_n;
-    check(launch_over(kernel, 2 * (total < pairs ? total : pairs), THREADS, SMEM, s, ta, tb, tc, p));
+  plan_cuts(p, parts ? most_pairs : 1);                  // (as many parts as fp8_parts_floats() counts)
+  CUtensorMap tp = tc;
+  const int n = p.items - p.whole;
+  if (n) {
+    const uint64_t dims[3] = {256, static_cast<uint64_t>(n) * 256, 1};
+    const uint64_t strides[2] = {256 * sizeof(float), dims[1] * 256 * sizeof(float)};
+    const uint32_t box[3] = {32, BM, 1};
+    tp = make_tmap(parts, 3, dims, strides, box, 4, true);
+  }
+  check(launch_over(kernel, 2 * (p.items < pairs ? p.items : pairs), THREADS, SMEM, s, ta, tb, tc, tp, p));
+  if (n) {
+    using T = std::conditional_t<F32, float, __nv_bfloat16>;
+    fp8_join_kernel<T><<<n / p.cuts * 64, 256, 0, s>>>(parts, static_cast<T*>(c), ld_c, p);
+    check(cudaGetLastError());
   }
 }
 

@@ -117,6 +117,21 @@ GatedSizes gated_sizes(const at::Tensor& x, const at::Tensor& wg, const at::Tens
   check_rows("gated_mlp", "w_down", wd, x, n.hidden, n.inter);
   return n;
 }
+// y = h wd^T.  Where the pair GEMM has tiles for less than half of the pairs it goes there, which cuts them along the long inner dimension (139 rows, 5648 to
+// 472: TODO us); else where gemm() sends it.
+void down_product(const at::Tensor& h, const at::Tensor& wd, at::Tensor& y) {
+  const int64_t tiles = (h.size(0) + 255) / 256 * ((wd.size(0) + 255) / 256), pairs = himuon::num_sms() / 2, blocks = (h.size(1) + 63) / 64;
+  const int64_t cuts = std::min(pairs / tiles, blocks / 8);
+  if (2 * tiles > pairs || cuts < 2 || (cuts - 1) * blocks / cuts < 40) return gemm_into(h, wd, y, false, true);
+  himuon::GemmArgs g;
+  g.A = h.data_ptr(); g.B = wd.data_ptr(); g.C = y.data_ptr();
+  g.M = static_cast<int>(h.size(0)); g.N = static_cast<int>(wd.size(0)); g.K = static_cast<int>(h.size(1));
+  g.lda = h.stride(0); g.ldb = wd.stride(0); g.ldc = y.stride(0);
+  g.ordered = 1;
+  const at::Tensor parts = at::empty({himuon::gemm2_parts_floats(g)}, y.options().dtype(at::kFloat));
+  g.parts = parts.data_ptr<float>();
+  himuon::gemm2_bf16(g, cur_stream());
+}
 // y; with `kept`, h and what is kept of g | u are left there.
 struct GatedKept { at::Tensor h, gu, gu_low; };
 at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t activation, GatedKept* kept) {
@@ -135,7 +150,7 @@ at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Te
     himuon::few_rows_product(h.data_ptr(), n.inter, wd.data_ptr(), wd.stride(0), y.data_ptr(), a.rows, a.inter, a.hidden, true, cur_stream());
   } else {
     himuon::gated_up(a, cur_stream());
-    gemm_into(h, wd, y, false, true);
+    down_product(h, wd, y);
   }
   autograd_launched += 2;
   return y;
@@ -330,7 +345,7 @@ at::Tensor product(const char* op, const Fp8& a, const Fp8& b, bool out_fp32, bo
   at::Tensor c = at::empty({rows, ld}, type);
   const bool powers = a.powers && b.powers;
   at::Tensor parts;
-  if (const int64_t floats = powers ? himuon::fp8_parts_floats(a.m, b.m) : 0) parts = at::empty({floats}, a.values.options().dtype(at::kFloat));
+  if (const int64_t floats = himuon::fp8_parts_floats(a.m, b.m)) parts = at::empty({floats}, a.values.options().dtype(at::kFloat));
   himuon::fp8_product(a.m, b.m, c.data_ptr(), ld, out_fp32, powers, parts.defined() ? parts.data_ptr<float>() : nullptr, cur_stream());
   return ld == cols ? c : c.narrow(1, 0, cols).contiguous();
 }

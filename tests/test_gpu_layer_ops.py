@@ -226,7 +226,8 @@ GATED = ("y", "dx", "dwg", "dwu", "dwd")
 
 
 @pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "relu"])
-@pytest.mark.parametrize("T,H,I", [(1, 8, 8), (3, 40, 24), (8, 128, 352), (17, 200, 136), (33, 64, 1000), (64, 640, 264), (65, 640, 264), (129, 72, 128), (300, 264, 520), (777, 640, 1728)])
+@pytest.mark.parametrize("T,H,I", [(1, 8, 8), (3, 40, 24), (8, 128, 352), (17, 200, 136), (33, 64, 1000), (64, 640, 264), (65, 640, 264), (129, 72, 128), (300, 264, 520), (777, 640, 1728),
+                                   (5, 264, 4104), (24, 320, 2056), (40, 72, 4096), (64, 2048, 8), (200, 264, 5648)])
 def test_gated_mlp(T, H, I, activation):
     ops = _ops()
     x, wg, wu, wd, dy = _block(T, H, I)
@@ -359,7 +360,7 @@ def test_quantisation_has_the_bits_of_the_plain_one(dtype, block_rows):
 
 @pytest.mark.parametrize("M,N,K", [(1, 1, 16), (1, 128, 128), (5, 40, 144), (8, 352, 128), (16, 130, 512), (31, 640, 1000), (64, 200, 2560), (65, 128, 640), (3, 20, 77), (129, 8, 8),
                                    (130, 1000, 1729), (300, 257, 256), (777, 1728, 640), (513, 300, 4096),
-                                   (70, 520, 9728), (6400, 700, 4096), (200, 12, 5000)])
+                                   (70, 520, 9728), (6400, 700, 4096), (200, 12, 5000), (8, 200, 9000), (20, 301, 5000), (32, 4000, 8192)])
 def test_fp8_matmul(M, N, K):
     """Powers of two and any other fp32 scales, different from block to block, blocks of either kind in a, every row length."""
     ops = _ops()
