@@ -78,9 +78,6 @@ static void gemm(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, cons
   }
   himuon::gemm_bf16(g, cur_stream());
 }
-void gemm_into(const at::Tensor& a, const at::Tensor& b, at::Tensor& out, bool trans_a, bool trans_b) {
-  gemm(a, b, out, c10::nullopt, trans_a, trans_b, 1.0, 0.0, false, 0, false);
-}
 // Whether gemm() with these arguments runs on CTA pairs.
 static bool gemm_on_pairs(const at::Tensor& a, const at::Tensor& b, const at::Tensor& out, const c10::optional<at::Tensor>& aux,
                           bool trans_a, bool trans_b, double alpha, double beta, bool round_acc, int64_t max_ctas,

@@ -1,16 +1,22 @@
 // Products of a few rows (newest tokens) with a large weight, whose bytes are all that counts:  y = x W^T  in bf16, the same of two
 // weights with the gated activation between them, and the same in 8 bits with a scale for each block of 128.
 //
-// A block streams `th` rows of W (of both weights) through a ring of stages in shared memory, 128 bytes or more of each row and of each row of x a
+// A block streams `th` rows of W (of both weights) through a ring of stages in shared memory, 128 bytes of each row and of each row of x a
 // stage, by TMA; two blocks to an SM, so that some 190 KB are on the way at any time.  Warps take 16 rows of W each from there: rows of W are the A operand of
 // mma.sync, up to 8 rows of x the B operand.  (tcgen05.mma leaves its sums in tensor memory, and blocks with scales of their own would have to be fetched from
-// there one by one; its rate is not needed here.)  A block has as few rows of W as it takes to keep all SMs busy, so that often two or seven groups of warps take
-// the stages in turn, and their parts meet in shared memory: a stage costs its warps some 500 cycles whatever is in it.  Everything is added up in one order, which
-// goes by the weight's sizes: bits repeat, and a row's do not depend on how many rows come with it.
+// there one by one; its rate is not needed here.)  A block has as few rows of W as it takes to keep all SMs busy, so that often two or three groups of warps take
+// the stages in turn, and their parts meet in shared memory.  Where that would be fewer than 24 rows (a narrow weight, whose inner dimension is long), so that x
+// would be as much to load as W, up to four blocks, a cluster, have a part of the inner dimension each, and read one another's parts.  Everything is added
+// up in one order, which goes by the weight's sizes: bits repeat, and a row's do not depend on how many rows come with it.
 //
-// Weights loaded from memory straight into the operands' registers, 64 bytes of 16 rows a warp, took longer: 24 rows of 2560 x 9728 gated and back
-// 38 + 30 us (22 + 17 now) with eight warps on one group of 16 rows, 57 + 47 with a group a warp.  So did clusters that share the inner dimension (25 + 21), and stages that all warps
-// of a block wait for (25 + 47).
+// A kernel of this kind is over in 8 to 20 us, of which its start is one or two.  So the second of two (the down projection; the product behind a quantisation)
+// is launched over the first: it sets up, and fills its ring with W, while that still runs, and waits for it before it asks for x.
+//
+// What bounds it: memory while the ring is full (6.3 TB/s of W at 24 rows of 2560 x 9728 gated), the start, and the loading warp, whose every instruction costs
+// some five cycles: with addresses worked out at each stage it took 500 cycles a stage.  One row, 2048 x 8192 gated and back: 22.5 us for 100.7 MB; 24 rows, 2560 x 9728:
+// 36.3 us for 149.4 MB; 8 rows, 2560 -> 9728 in 8 bits with x's quantisation: 14 us for 24.9 MB.  Without the clusters and the overlap 30.7, 41.9 and 14.4.
+// W loaded from memory straight into the operands' registers took longer (24 rows 38 + 30 us, at that time 22 + 17), so did stages that all warps of a
+// block wait for (25 + 47), and loads issued by the group that has emptied a stage (28.8 for 24.4 gated).
 #include "activations.cuh"
 #include "fp8.h"
 #include "gated_mlp.h"

@@ -117,50 +117,69 @@ GatedSizes gated_sizes(const at::Tensor& x, const at::Tensor& wg, const at::Tens
   check_rows("gated_mlp", "w_down", wd, x, n.hidden, n.inter);
   return n;
 }
-// y = h wd^T.  Where the pair GEMM has tiles for less than half of the pairs it goes there, which cuts them along the long inner dimension (139 rows, 5648 to
-// 472: TODO us); else where gemm() sends it.
-void down_product(const at::Tensor& h, const at::Tensor& wd, at::Tensor& y) {
-  const int64_t tiles = (h.size(0) + 255) / 256 * ((wd.size(0) + 255) / 256), pairs = himuon::num_sms() / 2, blocks = (h.size(1) + 63) / 64;
-  const int64_t cuts = std::min(pairs / tiles, blocks / 8);
-  if (2 * tiles > pairs || cuts < 2 || (cuts - 1) * blocks / cuts < 40) return gemm_into(h, wd, y, false, true);
-  himuon::GemmArgs g;
-  g.A = h.data_ptr(); g.B = wd.data_ptr(); g.C = y.data_ptr();
-  g.M = static_cast<int>(h.size(0)); g.N = static_cast<int>(wd.size(0)); g.K = static_cast<int>(h.size(1));
-  g.lda = h.stride(0); g.ldb = wd.stride(0); g.ldc = y.stride(0);
-  g.ordered = 1;
-  const at::Tensor parts = at::empty({himuon::gemm2_parts_floats(g)}, y.options().dtype(at::kFloat));
-  g.parts = parts.data_ptr<float>();
-  himuon::gemm2_bf16(g, cur_stream());
+// A product with rows of c one behind the other, on CTA pairs or where gemm() sends it.
+void product_into(himuon::GemmArgs& g, bool pairs, const at::Tensor& like) {
+  at::Tensor parts;
+  if (const int64_t floats = pairs ? himuon::gemm2_parts_floats(g) : himuon::gemm_parts_floats(g)) {
+    parts = at::empty({floats}, like.options().dtype(at::kFloat));
+    g.parts = parts.data_ptr<float>();
+  }
+  if (pairs) himuon::gemm2_bf16(g, cur_stream());
+  else himuon::gemm_bf16(g, cur_stream());
+  autograd_launched += 1;
 }
-// y; with `kept`, h and what is kept of g | u are left there.
-struct GatedKept { at::Tensor h, gu, gu_low; };
-at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t activation, GatedKept* kept) {
+himuon::GemmArgs product_of(const void* a, int64_t lda, bool a_mn, const void* b, int64_t ldb, bool b_mn, const at::Tensor& c, int64_t inner) {
+  himuon::GemmArgs g;
+  g.A = a; g.B = b; g.C = c.data_ptr();
+  g.M = static_cast<int>(c.size(0)); g.N = static_cast<int>(c.size(1)); g.K = static_cast<int>(inner);
+  g.lda = lda; g.ldb = ldb; g.ldc = c.size(1);
+  g.a_mn = a_mn; g.b_mn = b_mn;
+  return g;
+}
+// h and, for a backward pass, what is kept of g | u, in one piece of memory.
+struct GatedKept {
+  char *h, *gu, *low;
+  static int64_t bytes(const GatedSizes& n, bool all) { return n.rows * (2 * n.inter + (all ? 4 * n.inter + 2 * himuon::gated_low(static_cast<int>(n.inter)) : 0)); }
+  GatedKept(const at::Tensor& piece, const GatedSizes& n)
+      : h(static_cast<char*>(piece.data_ptr())), gu(h + 2 * n.rows * n.inter), low(gu + 4 * n.rows * n.inter) {}
+};
+// y; `piece` is left there if it is asked for.
+at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t activation, at::Tensor* piece) {
   const GatedSizes n = gated_sizes(x, wg, wu, wd, activation);
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor h = at::empty({n.rows, n.inter}, x.options()), y = at::empty({n.rows, n.hidden}, x.options());
-  if (kept) *kept = {h, at::empty({n.rows, 2 * n.inter}, x.options()), at::empty({n.rows, 2 * himuon::gated_low(static_cast<int>(n.inter))}, x.options().dtype(at::kByte))};
+  const at::Tensor memory = at::empty({GatedKept::bytes(n, piece != nullptr)}, x.options().dtype(at::kByte));
+  const GatedKept kept(memory, n);
+  at::Tensor y = at::empty({n.rows, n.hidden}, x.options());
+  if (piece) *piece = memory;
   if (!n.rows) return y;
   himuon::GatedUpArgs a;
   a.x = x.data_ptr(); a.wg = wg.data_ptr(); a.wu = wu.data_ptr();
-  a.h = h.data_ptr(); a.gu = kept ? kept->gu.data_ptr() : nullptr; a.gu_low = kept ? kept->gu_low.data_ptr() : nullptr;
+  a.h = kept.h; a.gu = piece ? kept.gu : nullptr; a.gu_low = piece ? kept.low : nullptr;
   a.ld_x = x.stride(0); a.ld_wg = wg.stride(0); a.ld_wu = wu.stride(0);
   a.rows = static_cast<int>(n.rows); a.hidden = static_cast<int>(n.hidden); a.inter = static_cast<int>(n.inter); a.activation = static_cast<int>(activation);
+  autograd_launched += 1;
   if (n.rows <= himuon::kFewProductRows) {
     himuon::few_rows_gated_up(a, cur_stream());
-    himuon::few_rows_product(h.data_ptr(), n.inter, wd.data_ptr(), wd.stride(0), y.data_ptr(), a.rows, a.inter, a.hidden, true, cur_stream());
-  } else {
-    himuon::gated_up(a, cur_stream());
-    down_product(h, wd, y);
+    himuon::few_rows_product(kept.h, n.inter, wd.data_ptr(), wd.stride(0), y.data_ptr(), a.rows, a.inter, a.hidden, true, cur_stream());
+    autograd_launched += 1;
+    return y;
   }
-  autograd_launched += 2;
+  himuon::gated_up(a, cur_stream());
+  himuon::GemmArgs g = product_of(kept.h, n.inter, false, wd.data_ptr(), wd.stride(0), false, y, n.inter);
+  // Where the pair GEMM has tiles for less than half of the pairs it is taken all the same, as it cuts them along the inner dimension.
+  // Gated and back, 80 rows of 4096 x 12288: 94 us for 109 where gemm() sends it, 139 rows of 472 x 5648 30 for 45.
+  const int64_t tiles = (n.rows + 255) / 256 * ((n.hidden + 255) / 256), pairs = himuon::num_sms() / 2, blocks = (n.inter + 63) / 64, cuts = std::min(pairs / tiles, blocks / 8);
+  const bool cut = 2 * tiles <= pairs && cuts >= 2 && (cuts - 1) * blocks / cuts >= 40;
+  g.ordered = cut;
+  product_into(g, cut, x);
   return y;
 }
 
 struct GatedMlp : torch::autograd::Function<GatedMlp> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const at::Tensor& wd, int64_t activation) {
-    GatedKept kept;
-    const at::Tensor y = gated_forward(x, wg, wu, wd, activation, &kept);
-    ctx->save_for_backward({x, wg, wu, wd, kept.h, kept.gu, kept.gu_low});
+    at::Tensor piece;
+    const at::Tensor y = gated_forward(x, wg, wu, wd, activation, &piece);
+    ctx->save_for_backward({x, wg, wu, wd, piece});
     ctx->saved_data["activation"] = activation;
     return y;
   }
@@ -168,13 +187,12 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_once("gated_mlp");
     const variable_list saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &wd = saved[3], &h = saved[4], &gu = saved[5], &low = saved[6];
+    const at::Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &wd = saved[3], &piece = saved[4];
     const int64_t activation = ctx->saved_data["activation"].toInt();
     const GatedSizes n = gated_sizes(x, wg, wu, wd, activation);       // (hooks may have moved what was kept)
-    check_rows("gated_mlp", "what is kept of h", h, x, n.rows, n.inter);
-    check_rows("gated_mlp", "what is kept of the gates", gu, x, n.rows, 2 * n.inter);
-    HM_CHECK(gu.is_contiguous() && low.device() == x.device() && low.scalar_type() == at::kByte && low.is_contiguous() &&
-                 low.numel() == n.rows * 2 * himuon::gated_low(static_cast<int>(n.inter)) && aligned16(low), "gated_mlp: what was kept of the gates has changed");
+    HM_CHECK(piece.device() == x.device() && piece.scalar_type() == at::kByte && piece.is_contiguous() && piece.numel() == GatedKept::bytes(n, true) && aligned16(piece),
+             "gated_mlp: what was kept has changed");
+    const GatedKept kept(piece, n);
     const c10::cuda::CUDAGuard guard(x.device());
     variable_list out(5);
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
@@ -185,40 +203,31 @@ struct GatedMlp : torch::autograd::Function<GatedMlp> {
     }
     const at::Tensor dy = with_rows(grads[0]);
     if (ctx->needs_input_grad(3)) {
-      out[3] = at::empty(wd.sizes(), wd.options());
-      gemm_into(dy, h, out[3], true, false);
-      autograd_launched += 1;
+      out[3] = at::empty({n.hidden, n.inter}, wd.options());
+      himuon::GemmArgs g = product_of(dy.data_ptr(), dy.stride(0), true, kept.h, n.inter, true, out[3], n.rows);
+      product_into(g, false, x);
     }
     if (!need_x && !need_w) return out;
-    at::Tensor dgu = at::empty_like(gu);
+    const at::Tensor dgu = at::empty({n.rows, 2 * n.inter}, x.options());
     himuon::GatedDownGradArgs a;
-    a.dy = dy.data_ptr(); a.wd = wd.data_ptr(); a.gu = gu.data_ptr(); a.gu_low = low.data_ptr(); a.dgu = dgu.data_ptr();
+    a.dy = dy.data_ptr(); a.wd = wd.data_ptr(); a.gu = kept.gu; a.gu_low = kept.low; a.dgu = dgu.data_ptr();
     a.ld_dy = dy.stride(0); a.ld_wd = wd.stride(0);
     a.rows = static_cast<int>(n.rows); a.hidden = static_cast<int>(n.hidden); a.inter = static_cast<int>(n.inter);
     a.activation = static_cast<int>(activation);
     himuon::gated_down_grad(a, cur_stream());
     autograd_launched += 1;
-    if (need_x) {
-      out[0] = at::empty(x.sizes(), x.options());
-      himuon::GemmArgs g;                                // dx = dg Wg + du Wu
-      g.A = dgu.data_ptr(); g.A2 = static_cast<char*>(dgu.data_ptr()) + 2 * n.inter;
-      g.B = wg.data_ptr(); g.B2 = wu.data_ptr(); g.C = out[0].data_ptr();
-      g.M = a.rows; g.N = a.hidden; g.K = a.inter;
-      g.lda = 2 * n.inter; g.ldb = wg.stride(0); g.ldb2 = wu.stride(0); g.ldc = n.hidden;
-      g.b_mn = true;
-      g.ordered = 1;                                     // (so that few tiles are cut along the inner dimension too)
-      at::Tensor parts;
-      if (const int64_t floats = himuon::gemm2_parts_floats(g)) {
-        parts = at::empty({floats}, x.options().dtype(at::kFloat));
-        g.parts = parts.data_ptr<float>();
-      }
-      himuon::gemm2_bf16(g, cur_stream());
-      autograd_launched += 1;
+    if (need_x) {                                        // dx = dg Wg + du Wu
+      out[0] = at::empty({n.rows, n.hidden}, x.options());
+      himuon::GemmArgs g = product_of(dgu.data_ptr(), 2 * n.inter, false, wg.data_ptr(), wg.stride(0), true, out[0], n.inter);
+      g.A2 = static_cast<char*>(dgu.data_ptr()) + 2 * n.inter;
+      g.B2 = wu.data_ptr(); g.ldb2 = wu.stride(0);
+      g.ordered = 1;                                     // (so that few tiles are cut along the inner dimension too: 777 rows, 640 x 1728 17 us for 23)
+      product_into(g, true, x);
     }
     if (need_w) {
-      at::Tensor dw = at::empty({2 * n.inter, n.hidden}, x.options());
-      gemm_into(dgu, x, dw, true, false);
-      autograd_launched += 1;
+      const at::Tensor dw = at::empty({2 * n.inter, n.hidden}, x.options());
+      himuon::GemmArgs g = product_of(dgu.data_ptr(), 2 * n.inter, true, x.data_ptr(), x.stride(0), true, dw, n.rows);
+      product_into(g, false, x);
       if (ctx->needs_input_grad(1)) out[1] = dw.narrow(0, 0, n.inter);
       if (ctx->needs_input_grad(2)) out[2] = dw.narrow(0, n.inter, n.inter);
     }
