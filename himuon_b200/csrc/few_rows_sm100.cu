@@ -3,7 +3,7 @@
 //
 // A block streams `th` rows of W (of both weights) through a ring of stages in shared memory, 128 bytes of each row and of each row of x a
 // stage, by TMA; two blocks to an SM, so that some 190 KB are on the way at any time.  Warps take 16 rows of W each from there: rows of W are the A operand of
-// mma.sync, up to 8 rows of x the B operand.  (tcgen05.mma leaves its sums in tensor memory, and blocks with scales of their own would have to be fetched from
+// mma.sync, up to 8 rows of x the B operand (8-bit values as fp16, which is what they cost anyway: 21.3 us for 24 rows of 2560 -> 9728 as e4m3, 19.4 so).  (tcgen05.mma leaves its sums in tensor memory, and blocks with scales of their own would have to be fetched from
 // there one by one; its rate is not needed here.)  A block has as few rows of W as it takes to keep all SMs busy, so that often two or three groups of warps take
 // the stages in turn, and their parts meet in shared memory.  Where that would be fewer than 24 rows (a narrow weight, whose inner dimension is long), so that x
 // would be as much to load as W, up to four blocks, a cluster, have a part of the inner dimension each, and read one another's parts.  Everything is added
@@ -59,10 +59,24 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four e4m3 values as fp16, which holds them all.
+__device__ __forceinline__ void widen(uint32_t v, uint32_t (&w)[2]) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(w[0]), "=r"(w[1]) : "r"(v));
+}
+// 32 products of e4m3 values, as two times 16 of fp16: lanes have four neighbouring values along the sum, which may come in any order that is the same in a and b.
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  uint32_t w[4][2], v[2][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) widen(a[i], w[i]);
+  widen(b0, v[0]);
+  widen(b1, v[1]);
+  mma_f16(c, w[0][0], w[1][0], w[0][1], w[1][1], v[0][0], v[0][1]);
+  mma_f16(c, w[2][0], w[3][0], w[2][1], w[3][1], v[1][0], v[1][1]);
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&v)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
@@ -204,10 +218,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
           load_scales(kb + p.groups);
         }
         if (!mbar_wait_warp(&bars->full[stage], phase, abort_flag, p.status, 3)) { ok = false; break; }
-        constexpr int NN = NT < 4 ? NT : KIND == EIGHT_BITS ? 2 : 4;              // groups of x at a time: more would not fit in the registers of two blocks
+        constexpr int NN = NT < 4 ? NT : 4;                  // groups of x at a time: more would not fit in the registers of two blocks
         const uint32_t base = ring + stage * stage_bytes, x_base = base + MATS * w_bytes;
-        // With few rows a turn is latency: all of its operands are asked for before the first product, and 8-bit products go to two sums.
-        constexpr int HALVES = NT <= 2 ? 2 : 1, AHEAD = NT <= 2 ? 4 : 1, CHAINS = NT <= 2 ? 2 : 1;
+        // A turn is latency: as many operands as there are registers for are asked for before the first product, and few rows' 8-bit products go to two sums.
+        constexpr int HALVES = NT <= 2 ? 2 : 1, AHEAD = NT <= 2 ? 4 : NT <= 4 ? 2 : 1, CHAINS = NT <= 2 ? 2 : 1;
 #pragma unroll
         for (int n0 = 0; n0 < NT; n0 += NN) {
           float c[CHAINS][NN][4] = {};

@@ -36,7 +36,12 @@ void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c
 long long fp8_parts_floats(const Fp8Matrix& a, const Fp8Matrix& b);
 // The same for a few rows of a; c is contiguous.  `early`: b was there before the launch that comes before this one on the stream, and may be read while that still
 // runs.  (33 to 64 rows have as many accumulators as a thread has registers: they are the large kernel's.)
+// Which of the two: up to 16 rows always; up to 32 of a weight of 16 MB at most, whose time is its launch (24 rows, 2048 -> 2048 7.6 us, 11.7 in the other; 2560 ->
+// 9728 17.6 and 14.8, as each of the few products has its scales to load and apply).
 constexpr int kFewFp8Rows = 32;
+inline bool few_fp8_rows(const Fp8Matrix& a, const Fp8Matrix& b) {
+  return a.rows <= kFewFp8Rows / 2 || (a.rows <= kFewFp8Rows && static_cast<long long>(b.rows) * b.cols <= 1LL << 24);
+}
 void few_rows_fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, int out_fp32, bool early, cudaStream_t s);
 
 }  // namespace himuon

@@ -344,7 +344,7 @@ at::Tensor product(const char* op, const Fp8& a, const Fp8& b, bool out_fp32, bo
   if (!rows || !cols) return at::empty({rows, cols}, type);
   if (!a.m.cols) return at::zeros({rows, cols}, type);
   autograd_launched += 1;
-  if (rows <= himuon::kFewFp8Rows) {
+  if (himuon::few_fp8_rows(a.m, b.m)) {
     at::Tensor c = at::empty({rows, cols}, type);
     himuon::few_rows_fp8_product(a.m, b.m, c.data_ptr(), out_fp32, early, cur_stream());
     return c;

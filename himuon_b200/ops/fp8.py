@@ -70,7 +70,8 @@ def quantize_fp8(x2d: torch.Tensor, block_rows: int = 1, transpose: bool = False
 def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a @ b.T`` of two 8-bit matrices ``(rows, inner)`` and ``(cols, inner)``, in bf16 or fp32.  ``a`` has blocks of 1 or 128 rows, ``b`` of 128
     (as a weight has).  The products of a block are summed by the tensor core, the blocks, scaled, in fp32 (by the product of two scales, which has to be a
-    normal fp32 number).  Up to 32 rows run a kernel that streams ``b``.  Not differentiable: see :func:`fp8_linear`."""
+    normal fp32 number).  Few rows (up to 16, or 32 of a small ``b``) run a kernel that streams
+    ``b``.  Not differentiable: see :func:`fp8_linear`."""
     _check("fp8_matmul", a)
     _check("fp8_matmul", b)
     if a.values.shape[1] != b.values.shape[1] or a.values.device != b.values.device:

@@ -701,6 +701,40 @@ def test_layer_operators_from_two_threads():
     _clean()
 
 
+@pytest.mark.parametrize("rows", [3, 24, 300])
+def test_launches_over_one_another_see_what_came_before(rows):
+    """Inputs and weights are overwritten just before each call, eagerly and in a graph: kernels that start early must not read them early."""
+    ops = _ops()
+    torch.manual_seed(rows + 101)
+    xs = [torch.randn(rows, 640, device="cuda").bfloat16() for _ in range(4)]
+    ws = [[(torch.randn(*s, device="cuda") * 0.05).bfloat16() for s in ((1728, 640), (1728, 640), (640, 1728))] for _ in range(4)]
+    kept = [ops.quantize_fp8(w[2], 128) for w in ws]
+    x, w = torch.empty_like(xs[0]), [torch.empty_like(t) for t in ws[0]]
+    q = ops.Fp8Blocks(torch.empty_like(kept[0].values), torch.empty_like(kept[0].scales), 128, True)
+
+    def step(i):
+        x.copy_(xs[i])
+        for a, b in zip((*w, q.values.view(torch.uint8), q.scales), (*ws[i], kept[i].values.view(torch.uint8), kept[i].scales)):
+            a.copy_(b)
+        h = ops.gated_mlp(x, *w)
+        y = ops.fp8_linear(ops.fp8_linear(h, w[0]), q)
+        return h, y, ops.fp8_matmul(ops.quantize_fp8(w[1]), q._replace(values=q.values[:, :640], scales=q.scales[:, :5]))
+
+    want = []
+    for i in range(4):
+        want.append(step(i))
+        torch.cuda.synchronize()
+    got = [step(i % 4) for i in range(40)]
+    assert all(_same(g, want[i % 4]) for i, g in enumerate(got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = [step(i) for i in range(4)]
+    for _ in range(3):
+        graph.replay()
+    assert all(_same(a, b) for a, b in zip(captured, want))
+    _clean()
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^31 values: the last rows are those of a call with nothing else."""
     ops = _ops()
