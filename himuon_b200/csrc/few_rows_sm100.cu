@@ -3,18 +3,22 @@
 //
 // A block streams `th` rows of W (of both weights) through a ring of stages in shared memory, 128 bytes of each row and of each row of x a
 // stage, by TMA; two blocks to an SM, so that some 190 KB are on the way at any time.  Warps take 16 rows of W each from there: rows of W are the A operand of
-// mma.sync, up to 8 rows of x the B operand (8-bit values as fp16, which is what they cost anyway: 21.3 us for 24 rows of 2560 -> 9728 as e4m3, 19.4 so).  (tcgen05.mma leaves its sums in tensor memory, and blocks with scales of their own would have to be fetched from
-// there one by one; its rate is not needed here.)  A block has as few rows of W as it takes to keep all SMs busy, so that often two or three groups of warps take
-// the stages in turn, and their parts meet in shared memory.  Where that would be fewer than 24 rows (a narrow weight, whose inner dimension is long), so that x
-// would be as much to load as W, up to four blocks, a cluster, have a part of the inner dimension each, and read one another's parts.  Everything is added
-// up in one order, which goes by the weight's sizes: bits repeat, and a row's do not depend on how many rows come with it.
+// mma.sync, up to 8 rows of x the B operand; 8-bit values go there as fp16 (24 rows of 2560 -> 9728 19.4 us, 21.3 as e4m3).  (tcgen05.mma leaves its sums in tensor
+// memory, and blocks with scales of their own would have to be fetched from there one by one; its rate is not needed here.)
+//
+// A block has as few rows of W as it takes to keep all SMs busy, so that often two or three groups of warps take the stages in turn, and their parts meet in
+// shared memory.  Where that would be fewer than 24 rows (a narrow weight, whose inner dimension is long), so that x would be as much to load as W, up to four
+// blocks, a cluster, have a part of the inner dimension each, and read one another's parts.  From 33 rows on blocks with 32 rows each have a tile together, which
+// takes W from memory once and from the L2 for the others, and has more rows of W for that (64 rows, 2560 x 9728 gated and back: 51 us, 59 in one block with 64
+// rows, whose sums fill the registers).  Everything is added up in one order, which goes by the weight's sizes and, from 33 rows on, by the number of such blocks: bits
+// repeat, and a row's do not depend on how many rows up to 32 come with it.
 //
 // A kernel of this kind is over in 8 to 20 us, of which its start is one or two.  So the second of two (the down projection; the product behind a quantisation)
 // is launched over the first: it sets up, and fills its ring with W, while that still runs, and waits for it before it asks for x.
 //
 // What bounds it: memory while the ring is full (6.3 TB/s of W at 24 rows of 2560 x 9728 gated), the start, and the loading warp, whose every instruction costs
 // some five cycles: with addresses worked out at each stage it took 500 cycles a stage.  One row, 2048 x 8192 gated and back: 22.5 us for 100.7 MB; 24 rows, 2560 x 9728:
-// 36.3 us for 149.4 MB; 8 rows, 2560 -> 9728 in 8 bits with x's quantisation: 14 us for 24.9 MB.  Without the clusters and the overlap 30.7, 41.9 and 14.4.
+// 36.5 us for 149.4 MB; 8 rows, 2560 -> 9728 in 8 bits with x's quantisation: 12.6 us for 24.9 MB.  Without the clusters and the overlap 30.7, 41.9 and 14.4.
 // W loaded from memory straight into the operands' registers took longer (24 rows 38 + 30 us, at that time 22 + 17), so did stages that all warps of a
 // block wait for (25 + 47), and loads issued by the group that has emptied a stage (28.8 for 24.4 gated).
 #include "activations.cuh"
@@ -49,6 +53,7 @@ struct FewDev {
   int blocks;                          // of 128 bytes of a row
   int th, tiles, stages;               // rows of W of a tile, tiles of a block, stages of the ring
   int cut;                             // blocks (a cluster) that a tile's inner dimension is dealt out to
+  int chunks, x_rows;                  // blocks that have a tile with 32 rows of x each, and rows of x in a load
   int early;                           // W was there before the launch before this one
   int warps, groups;                   // warps that a tile's rows take, and groups of so many, which take stages in turn
   int* status;
@@ -103,7 +108,7 @@ __device__ __forceinline__ float activate_any(int activation, float g) {
 // The result of one row of W (of both) and one of x.
 template <int KIND>
 __device__ __forceinline__ void put_result(const FewDev& p, int feature, int row, float v, float u) {
-  if (feature >= p.outer || row >= p.rows) return;
+  if (feature >= p.outer) return;
   const long long at = static_cast<long long>(row) * p.outer + feature;
   if constexpr (KIND == GATED) {
     reinterpret_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(activate_any(p.activation, v) * u);
@@ -140,10 +145,11 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
   const bool joined = p.groups > 1 || p.cut > 1;
   const int line = p.warps * 16 + 4;                   // of parts: a row of x by all rows of W (4 more, so that a warp's values lie in 32 banks)
   const int warp = warp_id(), lane = threadIdx.x & 31;
-  const int rank = p.cut > 1 ? static_cast<int>(blockIdx.x) % p.cut : 0, first = static_cast<int>(blockIdx.x) / p.cut * p.th * p.tiles;
+  const int of = static_cast<int>(blockIdx.x) / p.cut, rank = static_cast<int>(blockIdx.x) - of * p.cut, first = of / p.chunks * p.th * p.tiles;
+  const int row0 = of % p.chunks * 32, rows = min(p.rows - row0, 32);
   const int kb0 = p.blocks * rank / p.cut, kb1 = p.blocks * (rank + 1) / p.cut;
   const uint32_t w_bytes = static_cast<uint32_t>(p.th) * 128, stage_bytes = MATS * w_bytes + NX * 128;
-  launch_dependents();
+  if (KIND == GATED) launch_dependents();              // (the down projection, whose W is not made here; nothing is launched over one that was launched so itself)
   if (static_cast<int>(threadIdx.x) < p.stages) { mbar_init(&bars->full[threadIdx.x], 1); mbar_init(&bars->empty[threadIdx.x], p.warps); }
   if (threadIdx.x == 0) bars->abort_flag = 0;
   if (warp == 0) mbar_fence_init();
@@ -151,7 +157,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
 
   if (warp == 0) {
     // (a stage costs its bytes' time or this loop's instructions, which take some five cycles each: addresses go along, nothing is worked out anew)
-    const uint32_t e = elect_one(), bytes = MATS * w_bytes + p.rows * 128, ring = smem_u32(smem), full0 = smem_u32(bars->full);
+    const uint32_t e = elect_one(), bytes = MATS * w_bytes + p.x_rows * 128, ring = smem_u32(smem), full0 = smem_u32(bars->full);
     const int n = kb1 - kb0, ahead = p.early ? min(p.stages, n) : 0;
     for (int i = 0; i < ahead; ++i) {                    // W while the kernel before may still be writing x
       expect(full0 + i * 8, bytes, e);
@@ -159,7 +165,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
       if (MATS == 2) load(ring + i * stage_bytes + w_bytes, &tmW1, full0 + i * 8, (kb0 + i) * PER_SUB, first, e);
     }
     wait_for_previous();
-    for (int i = 0; i < ahead; ++i) load(ring + i * stage_bytes + MATS * w_bytes, &tmX, full0 + i * 8, (kb0 + i) * PER_SUB, 0, e);
+    for (int i = 0; i < ahead; ++i) load(ring + i * stage_bytes + MATS * w_bytes, &tmX, full0 + i * 8, (kb0 + i) * PER_SUB, row0, e);
     int stage = ahead;
     uint32_t phase = 1, at = ring + ahead * stage_bytes, bar = full0 + ahead * 8;
     bool ok = true;
@@ -172,7 +178,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         expect(bar, bytes, e);
         load(at, &tmW0, bar, k, f0, e);
         if (MATS == 2) load(at + w_bytes, &tmW1, bar, k, f0, e);
-        load(at + MATS * w_bytes, &tmX, bar, k, 0, e);
+        load(at + MATS * w_bytes, &tmX, bar, k, row0, e);
         ++stage;
         at += stage_bytes;
         bar += 8;
@@ -218,53 +224,39 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
           load_scales(kb + p.groups);
         }
         if (!mbar_wait_warp(&bars->full[stage], phase, abort_flag, p.status, 3)) { ok = false; break; }
-        constexpr int NN = NT < 4 ? NT : 4;                  // groups of x at a time: more would not fit in the registers of two blocks
         const uint32_t base = ring + stage * stage_bytes, x_base = base + MATS * w_bytes;
         // A turn is latency: as many operands as there are registers for are asked for before the first product, and few rows' 8-bit products go to two sums.
-        constexpr int HALVES = NT <= 2 ? 2 : 1, AHEAD = NT <= 2 ? 4 : NT <= 4 ? 2 : 1, CHAINS = NT <= 2 ? 2 : 1;
-#pragma unroll
-        for (int n0 = 0; n0 < NT; n0 += NN) {
-          float c[CHAINS][NN][4] = {};
+        constexpr int HALVES = NT <= 2 ? 2 : 1, STEPS = 2 * HALVES, CHAINS = HALVES;
+        float c[CHAINS][NT][4] = {};
 #pragma unroll 1
-          for (int half = 0; half < 2; half += HALVES) {
-            uint32_t b[HALVES][NN][4];
+        for (int half = 0; half < 2; half += HALVES) {
+          uint32_t b[HALVES][NT][4];
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
+          for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-              for (int n = 0; n < NN; ++n) ldmatrix4(b[h][n], cell(x_base, (n0 + n) * 8 + b_row, (half + h) * 4 + b_chunk));
+            for (int n = 0; n < NT; ++n) ldmatrix4(b[h][n], cell(x_base, n * 8 + b_row, (half + h) * 4 + b_chunk));
+          uint32_t a[STEPS][MATS][4];
 #pragma unroll
-            for (int k0 = 0; k0 < 2 * HALVES; k0 += AHEAD) {
-              uint32_t a[AHEAD][MATS][4];
-              auto products = [&](int m, int k) {
+          for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                for (int n = 0; n < NN; ++n) {
-                  const uint32_t b0 = b[(k0 + k) / 2][n][2 * ((k0 + k) % 2)], b1 = b[(k0 + k) / 2][n][2 * ((k0 + k) % 2) + 1];
-                  if constexpr (KIND == EIGHT_BITS) mma_e4m3(c[k % CHAINS][n], a[k][m], b0, b1);
-                  else mma_bf16(acc[m][n0 + n], a[k][m], b0, b1);
-                }
-              };
+            for (int k = 0; k < STEPS; ++k) ldmatrix4(a[k][m], cell(base + m * w_bytes, a_row, half * 4 + k * 2 + a_chunk));
 #pragma unroll
-              for (int m = 0; m < MATS; ++m)
+          for (int k = 0; k < STEPS; ++k)
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k) {
-                  ldmatrix4(a[k][m], cell(base + m * w_bytes, a_row, half * 4 + (k0 + k) * 2 + a_chunk));
-                  if (AHEAD == 1) products(m, k);
-                }
-              if (AHEAD > 1) {
+            for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                for (int k = 0; k < AHEAD; ++k)
-#pragma unroll
-                  for (int m = 0; m < MATS; ++m) products(m, k);
+              for (int n = 0; n < NT; ++n) {
+                const uint32_t b0 = b[k / 2][n][2 * (k % 2)], b1 = b[k / 2][n][2 * (k % 2) + 1];
+                if constexpr (KIND == EIGHT_BITS) mma_e4m3(c[k % CHAINS][n], a[k][m], b0, b1);
+                else mma_bf16(acc[m][n], a[k][m], b0, b1);
               }
-            }
-          }
-          if constexpr (KIND == EIGHT_BITS) {
+        }
+        if constexpr (KIND == EIGHT_BITS) {
 #pragma unroll
-            for (int n = 0; n < NN; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                acc[0][n0 + n][j] = fmaf(CHAINS == 2 ? c[0][n][j] + c[CHAINS - 1][n][j] : c[0][n][j], by_w[j >> 1] * by_x[n0 + n][j & 1], acc[0][n0 + n][j]);
-          }
+            for (int j = 0; j < 4; ++j)
+              acc[0][n][j] = fmaf(CHAINS == 2 ? c[0][n][j] + c[CHAINS - 1][n][j] : c[0][n][j], by_w[j >> 1] * by_x[n][j & 1], acc[0][n][j]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->empty[stage]);
@@ -278,7 +270,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int f = m0 + r + 8 * (j >> 1);
-              if (f < p.th) put_result<KIND>(p, f0 + f, n * 8 + 2 * t + (j & 1), acc[0][n][j], acc[MATS - 1][n][j]);
+              if (f < p.th && n * 8 + 2 * t + (j & 1) < rows) put_result<KIND>(p, f0 + f, row0 + n * 8 + 2 * t + (j & 1), acc[0][n][j], acc[MATS - 1][n][j]);
             }
         }
       } else {                                           // (one tile: the ring has been read to its end by all warps that the barrier waits for)
@@ -305,7 +297,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
   // V neighbouring features a thread: four where that leaves one for each thread (24 rows of 40 features: 1.2 us for 2.4 one by one), else one
   auto join = [&](auto width) {
     constexpr int V = decltype(width)::value;
-    const int line_of = p.th / V, out = line_of * p.rows;
+    const int line_of = p.th / V, out = line_of * rows;
     for (int o = rank * FEW_THREADS + static_cast<int>(threadIdx.x); o < out; o += p.cut * FEW_THREADS) {
       const int row = o / line_of, f = (o - row * line_of) * V;
       float v[MATS][V] = {};
@@ -324,10 +316,10 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
               for (int i = 0; i < V; ++i) v[m][i] += u[c][i];
         }
 #pragma unroll
-      for (int i = 0; i < V; ++i) put_result<KIND>(p, first + f + i, row, v[0][i], v[MATS - 1][i]);
+      for (int i = 0; i < V; ++i) put_result<KIND>(p, first + f + i, row0 + row, v[0][i], v[MATS - 1][i]);
     }
   };
-  if (p.th * p.rows >= 2 * FEW_THREADS * p.cut) join(std::integral_constant<int, 4>{});
+  if (p.th * rows >= 2 * FEW_THREADS * p.cut) join(std::integral_constant<int, 4>{});
   else join(std::integral_constant<int, 1>{});
   __syncwarp();
   if (p.cut > 1) cluster_sync_all();   // (nobody leaves while others read its parts)
@@ -349,12 +341,14 @@ void launch(const FewOperands& o, FewDev p, cudaStream_t s) {
   constexpr int MATS = KIND == GATED ? 2 : 1, NX = NT * 8;
   constexpr size_t SMEM = 1024 + FEW_RING + sizeof(FewBars);
   static_assert(2 * SMEM <= 232448 && MATS * NX * (FEW_ROWS + 4 * FEW_WARPS) * sizeof(float) <= FEW_RING &&
-                    (MATS * FEW_ROWS + kFewProductRows) * 128 <= FEW_RING, "shared memory of two blocks exceeded");
+                    (MATS * FEW_ROWS + 32) * 128 <= FEW_RING, "shared memory of two blocks exceeded");
   const auto kernel = few_rows_kernel<KIND, NT>;
   p.blocks = (o.inner * o.esz + 127) / 128;
   // Rows of W in equal shares over two blocks a SM, in tiles of up to FEW_ROWS.
   // Where that leaves a block fewer than 32 rows, so that x would be as much to load as W, blocks share tiles instead.
-  const int slots = 2 * num_sms();
+  p.chunks = (p.rows + 31) / 32;
+  p.x_rows = p.rows < 32 ? p.rows : 32;
+  const int slots = 2 * num_sms() / p.chunks;
   p.cut = 1;
   while (p.cut < FEW_CUT && static_cast<long long>(p.outer) * p.cut < 24LL * slots && p.blocks >= 32 * p.cut) p.cut *= 2;
   const int share = static_cast<int>((static_cast<long long>(p.outer) * p.cut + slots - 1) / slots + 7) / 8 * 8;
@@ -363,7 +357,7 @@ void launch(const FewOperands& o, FewDev p, cudaStream_t s) {
   p.warps = (p.th + 15) / 16;
   // Bytes of a stage and groups go by the weight alone (with the most rows of x that there may be), since what a group has, and with it the order of sums, does.
   const int weight = MATS * p.th * 128;
-  const int least = static_cast<int>(FEW_RING) / (weight + kFewProductRows * 128);
+  const int least = static_cast<int>(FEW_RING) / (weight + 32 * 128);
   p.groups = p.tiles > 1 ? 1 : FEW_WARPS / p.warps < least ? FEW_WARPS / p.warps : least;
   const int sub_bytes = weight + NX * 128;
   const int fit = static_cast<int>(FEW_RING) / sub_bytes;
@@ -371,8 +365,8 @@ void launch(const FewOperands& o, FewDev p, cudaStream_t s) {
   // (A stage is always the same group's: a group that met another's could be a whole round ahead of it, where a barrier's phases look alike.)
   p.stages -= p.stages % p.groups;
   p.status = status_word_ptr();
-  const long long group = static_cast<long long>(p.th) * p.tiles, grid = (p.outer + group - 1) / group * p.cut;
-  const CUtensorMap tx = few_map(o.x, p.rows, o, o.ld_x, p.rows), t0 = few_map(o.w0, p.outer, o, o.ld_w0, p.th), t1 = MATS == 2 ? few_map(o.w1, p.outer, o, o.ld_w1, p.th) : t0;
+  const long long group = static_cast<long long>(p.th) * p.tiles, grid = (p.outer + group - 1) / group * p.chunks * p.cut;
+  const CUtensorMap tx = few_map(o.x, p.rows, o, o.ld_x, p.x_rows), t0 = few_map(o.w0, p.outer, o, o.ld_w0, p.th), t1 = MATS == 2 ? few_map(o.w1, p.outer, o, o.ld_w1, p.th) : t0;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
   if (e == cudaSuccess) {
     cudaLaunchAttribute attrs[2];
@@ -401,8 +395,7 @@ void launch_rows(const FewOperands& o, const FewDev& p, cudaStream_t s) {
   if (p.rows <= 0 || p.rows > (KIND == EIGHT_BITS ? kFewFp8Rows : kFewProductRows) || p.outer <= 0 || o.inner <= 0) throw std::runtime_error("himuon product of few rows: bad sizes");
   if (p.rows <= 8) launch<KIND, 1>(o, p, s);
   else if (p.rows <= 16) launch<KIND, 2>(o, p, s);
-  else if (p.rows <= 32) launch<KIND, 4>(o, p, s);
-  else if constexpr (KIND != EIGHT_BITS) launch<KIND, 8>(o, p, s);
+  else launch<KIND, 4>(o, p, s);
 }
 
 }  // namespace

@@ -158,7 +158,7 @@ at::Tensor gated_forward(const at::Tensor& x, const at::Tensor& wg, const at::Te
   a.ld_x = x.stride(0); a.ld_wg = wg.stride(0); a.ld_wu = wu.stride(0);
   a.rows = static_cast<int>(n.rows); a.hidden = static_cast<int>(n.hidden); a.inter = static_cast<int>(n.inter); a.activation = static_cast<int>(activation);
   autograd_launched += 1;
-  if (n.rows <= himuon::kFewProductRows) {
+  if (himuon::few_gated_rows(n.rows, n.hidden, n.inter)) {
     himuon::few_rows_gated_up(a, cur_stream());
     himuon::few_rows_product(kept.h, n.inter, wd.data_ptr(), wd.stride(0), y.data_ptr(), a.rows, a.inter, a.hidden, true, cur_stream());
     autograd_launched += 1;

@@ -227,7 +227,8 @@ GATED = ("y", "dx", "dwg", "dwu", "dwd")
 
 @pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "relu"])
 @pytest.mark.parametrize("T,H,I", [(1, 8, 8), (3, 40, 24), (8, 128, 352), (17, 200, 136), (33, 64, 1000), (64, 640, 264), (65, 640, 264), (129, 72, 128), (300, 264, 520), (777, 640, 1728),
-                                   (5, 264, 4104), (24, 320, 2056), (40, 72, 4096), (64, 2048, 8), (200, 264, 5648)])
+                                   (5, 264, 4104), (24, 320, 2056), (40, 72, 4096), (64, 2048, 8), (200, 264, 5648), (384, 8, 264),
+                                   (385, 264, 520), (390, 8, 8), (400, 72, 128), (513, 640, 264), (65, 4096, 2056), (129, 2048, 2056), (200, 520, 5648)])
 def test_gated_mlp(T, H, I, activation):
     ops = _ops()
     x, wg, wu, wd, dy = _block(T, H, I)
@@ -248,7 +249,7 @@ def test_gated_mlp(T, H, I, activation):
 def test_gated_mlp_of_large_gates(activation):
     """Gates of hundreds, where sigmoids are 0 and 1 and exponentials would run over, and of 1e12, where their cubes would."""
     ops = _ops()
-    for T, spread in ((20, 120.0), (200, 120.0), (20, 1e12), (200, 1e12)):
+    for T, spread in ((20, 120.0), (400, 120.0), (20, 1e12), (400, 1e12)):
         x, wg, wu, wd, dy = _block(T, 256, 384, spread=120.0)
         wg = (wg.float() * (spread / 120.0)).bfloat16()
         leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
@@ -263,7 +264,7 @@ def test_gated_mlp_of_large_gates(activation):
 def test_gated_mlp_gradient_against_differences():
     """The kernels' gradients along a direction against a central difference of the 64-bit formula."""
     ops = _ops()
-    for T in (30, 150):
+    for T in (30, 150, 400):
         x, wg, wu, wd, dy = _block(T, 128, 352)
         leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
         grads = torch.autograd.grad(ops.gated_mlp(*leaves), leaves, dy)
@@ -279,7 +280,7 @@ def test_gated_mlp_gradient_against_differences():
 def test_gated_mlp_of_slices_shapes_and_some_gradients():
     """Halves of one weight, rows off the 16-byte grid, expanded gradients, leading dimensions; each gradient alone has the same bits."""
     ops = _ops()
-    for T in (24, 150):
+    for T in (24, 150, 400):
         x, wg, wu, wd, dy = _block(T, 128, 200)
         leaves = [t.requires_grad_() for t in (x, wg, wu, wd)]
         y = ops.gated_mlp(*leaves)
@@ -309,16 +310,14 @@ def test_gated_mlp_of_slices_shapes_and_some_gradients():
 
 
 def test_gated_mlp_rows_do_not_depend_on_one_another():
-    """Up to 64 rows a row has the same bits however many come with it, and above as well; NaN stays in its row and in the weights' gradients."""
+    """Up to 32 rows a row has the same bits however many come with it, so it has from 33 to 64, and by tiles; NaN stays in its row and in the weights' gradients."""
     ops = _ops()
-    x, wg, wu, wd, dy = _block(64, 640, 1728)
-    whole = ops.gated_mlp(x, wg, wu, wd)
-    for n in (1, 7, 8, 9, 16, 30, 33):
-        assert torch.equal(ops.gated_mlp(x[:n], wg, wu, wd), whole[:n])
-    x, wg, wu, wd, dy = _block(400, 640, 1728)
-    whole = ops.gated_mlp(x, wg, wu, wd)
-    assert torch.equal(ops.gated_mlp(x[:300], wg, wu, wd), whole[:300])
-    for n in (60, 300):
+    for rows, some in ((32, (1, 7, 8, 9, 16, 30)), (64, (33, 50)), (400, (385, 390))):
+        x, wg, wu, wd, dy = _block(rows, 640, 1728)
+        whole = ops.gated_mlp(x, wg, wu, wd)
+        for n in some:
+            assert torch.equal(ops.gated_mlp(x[:n], wg, wu, wd), whole[:n])
+    for n in (60, 300, 400):
         got = []
         for t in (x[:n], x[:n].clone()):
             if got:
@@ -476,7 +475,7 @@ def test_layer_operators_under_transforms(name):
 def test_layer_operators_on_streams_and_in_graphs():
     """Another stream, two graphs in turn, gradients captured, and new inputs at each replay."""
     torch.manual_seed(61)
-    for rows in (14, 140):
+    for rows in (14, 140, 400):
         fns, _, _ = _calls()
         at = torch.randint(0, 10000, (rows,), device="cuda")
         ops, f = _ops(), _ops().RotaryFrequencies(32, 10000.0)
@@ -647,7 +646,7 @@ def test_one_matrix_for_gate_and_up():
     """Gradients of a matrix that is used twice are added up, and again over two passes."""
     ops = _ops()
     torch.manual_seed(79)
-    for rows in (20, 100):
+    for rows in (20, 100, 400):
         x = torch.randn(rows, 64, device="cuda").bfloat16()
         w, d = ((torch.randn(*s, device="cuda") * 0.2).bfloat16() for s in ((40, 64), (64, 40)))
         v = w.clone()
@@ -701,7 +700,7 @@ def test_layer_operators_from_two_threads():
     _clean()
 
 
-@pytest.mark.parametrize("rows", [3, 24, 300])
+@pytest.mark.parametrize("rows", [3, 24, 300, 400])
 def test_launches_over_one_another_see_what_came_before(rows):
     """Inputs and weights are overwritten just before each call, eagerly and in a graph: kernels that start early must not read them early."""
     ops = _ops()
@@ -786,7 +785,7 @@ def test_gated_mlp_offsets_beyond_32_bits():
     _clean()
 
 
-@pytest.mark.parametrize("rows", [20, 300])
+@pytest.mark.parametrize("rows", [20, 300, 400])
 def test_a_decoder_layer_of_them(rows):
     """Queries and keys of one projection in 8 bits, turned, packed attention, and the feed-forward block: forward and backward against 64 bits."""
     ops = _ops()
