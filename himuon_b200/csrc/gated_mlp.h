@@ -33,10 +33,10 @@ void gated_down_grad(const GatedDownGradArgs& a, cudaStream_t s);
 // Products with a few rows (up to kFewProductRows), whose weight is all that counts: y = x w^T in bf16, or gated_up().
 // `early`: w was there before the launch that comes before this one on the stream, and may be read while that still runs.
 constexpr int kFewProductRows = 384;
-// Which of the two the gated block takes.  Up to 64 rows always (64 of 2560 x 9728, gated and back: 51 us, 58 by tiles; 64 of 4096 x 12288: 85 either way), and up to 384 of
-// small weights, whose tiles would be few (128 rows of 640 x 1728 12.9 and 18.8 us, of 1360 x 2472 22 and 33, 384 of 640 x 1728 18 and 19; but 512 of those 22 and 19).
+// Whether the gated block takes them: up to 32 rows always, up to 64 unless the weights are large (64 rows of 2048 x 6144, gated and back: 29 us, 31 in tiles of all rows,
+// of 2560 x 9728 51 and 45), and up to 384 of small ones (128 rows of 640 x 1728 13 and 19, of 1360 x 2472 22 and 31, 384 of 640 x 1728 18 and 19; but 192 of 472 x 5648 33 and 24).
 inline bool few_gated_rows(long long rows, long long hidden, long long inter) {
-  return rows <= 64 || (rows <= kFewProductRows && rows * hidden * inter <= 1LL << 29);
+  return rows <= 32 || (rows <= 64 && hidden * inter <= 1LL << 24) || (rows <= kFewProductRows && rows * hidden * inter <= 400000000);
 }
 void few_rows_product(const void* x, long long ld_x, const void* w, long long ld_w, void* y, int rows, int inner, int outer, bool early, cudaStream_t s);
 void few_rows_gated_up(const GatedUpArgs& a, cudaStream_t s);

@@ -69,6 +69,24 @@ __device__ __forceinline__ void from_kept(uint32_t upper, uint32_t low, int half
   b = __uint_as_float(__byte_perm(upper, low, half ? 0x3272 : 0x3252) & 0xFFFFFF00u);
 }
 
+// 8 consecutive fp32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr)
+               : "memory");
+}
+// What is kept of eight values.
+__device__ __forceinline__ void put_kept(uint16_t* upper, uint8_t* low, const uint32_t (&v)[8]) {
+  uint32_t o[4], l[2];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = __byte_perm(v[2 * j], v[2 * j + 1], 0x7632);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) l[j] = __byte_perm(__byte_perm(v[4 * j], v[4 * j + 1], 0x0051), __byte_perm(v[4 * j + 2], v[4 * j + 3], 0x0051), 0x5410);
+  *reinterpret_cast<uint4*>(upper) = make_uint4(o[0], o[1], o[2], o[3]);
+  *reinterpret_cast<uint2*>(low) = make_uint2(l[0], l[1]);
+}
+
 }  // namespace
 
 // tmA: rows of x or dy.  UP: tmB0 and tmB1 rows of Wg and Wu along the inner dimension, tmO h, tmG and tmU the halves of g | u.
@@ -330,6 +348,133 @@ gated_mlp_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   }
 }
 
+// UP for up to 256 rows, whose weights are all that counts.  Tiles of 128 features would be a little more than there are pairs (76 on 74 for 9728), and the second round as
+// long as the first; so a CTA by itself takes as many features as give every SM a tile (`features`, a multiple of 8), for all the rows: MT tiles of 128, which
+// share the rows of Wg and Wu that it has staged.  g and u of a feature are columns of one accumulator row.  The results are few, and go straight to memory.
+// 2560 x 9728 gated and back: 100 rows 45 us, 59 in tiles for pairs, 192 rows 50 and 60.
+constexpr int GR_STAGES = 8, GR_SMEM = 1024 + 216 * 1024 + 256;
+struct GatedRowsDev {
+  void *h, *gu;
+  uint8_t* gu_low;                     // null where g and u are not wanted
+  int rows, inter, low, features, tiles, kblocks, stages;
+  int* status;
+};
+template <int ACT, int MT>
+__global__ void __launch_bounds__(GM_THREADS, 1)
+gated_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmU, GatedRowsDev p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_up_1024(smem_raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + 216 * 1024);
+  uint64_t* empty = full + GR_STAGES;
+  uint64_t *tfull = empty + GR_STAGES, *tempty = tfull + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = warp_id(), lane = threadIdx.x & 31;
+  const uint32_t w_bytes = static_cast<uint32_t>(p.features) * 128, stage_bytes = MT * GM_A + 2 * w_bytes;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    mbar_init(tfull, 1);
+    mbar_init(tempty, 8);              // epilogue warps
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 2) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  if (warp == 0) {
+    const uint32_t e = elect_one();
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmG);
+    tma_prefetch_desc(&tmU);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+      const int n0 = tile * p.features;
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&empty[stage], phase ^ 1, abort_flag, p.status, 1)) { ok = false; break; }
+        uint8_t* at = smem + stage * stage_bytes;
+        mbar_expect_tx(&full[stage], stage_bytes, e);
+        tma_load_3d(at + MT * GM_A, &tmG, &full[stage], kb * BK, n0, 0, e);
+        tma_load_3d(at + MT * GM_A + w_bytes, &tmU, &full[stage], kb * BK, n0, 0, e);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) tma_load_3d(at + t * GM_A, &tmX, &full[stage], kb * BK, t * BM, 0, e);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t e = elect_one(), idesc = umma_idesc_bf16(BM, 2 * p.features, false, false);
+    int stage = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < p.tiles; tile += gridDim.x) {
+      if (!mbar_wait_warp(tempty, acc_phase ^ 1, abort_flag, p.status, 2)) break;
+      tc_fence_after();
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        if (!mbar_wait_warp(&full[stage], phase, abort_flag, p.status, 2)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t a_desc = umma_smem_desc(smem_u32(smem + stage * stage_bytes), 16, 1024), b_desc = desc_at(a_desc, MT * GM_A);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            umma_ss(tmem_base + static_cast<uint32_t>(t * 256), desc_at(a_desc, t * GM_A + k * 32), desc_at(b_desc, k * 32), idesc, (kb > 0 || k > 0) ? 1u : 0u, e);
+        umma_commit(&empty[stage], e);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+      if (!ok) break;
+      umma_commit(tfull, e);
+      acc_phase ^= 1;
+    }
+  } else if (warp >= 4) {
+    // one row a thread; two groups of warps have a tile of rows each, or every other eight features of the one
+    const int ew = warp & 3, group = (warp - 4) >> 2, mt = MT == 2 ? group : 0, row = mt * BM + ew * 32 + lane;
+    const bool row_ok = row < p.rows;
+    const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(ew * 32) << 16) + static_cast<uint32_t>(mt * 256);
+    uint32_t acc_phase = 0;
+    for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+      if (!mbar_wait_warp(tfull, acc_phase, abort_flag, p.status, 3)) break;
+      acc_phase ^= 1;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = MT == 2 ? 0 : group * 8; c < p.features; c += MT == 2 ? 8 : 16) {
+        const int col = tile * p.features + c;
+        if (col >= p.inter) break;                       // uniform
+        uint32_t g[8], u[8];
+        tmem_ld8(t_acc + c, g);
+        tmem_ld8(t_acc + p.features + c, u);
+        tmem_ld_wait();
+        if (row_ok) {
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[j] = pack_bf16x2(activate<ACT>(__uint_as_float(g[2 * j])) * __uint_as_float(u[2 * j]), activate<ACT>(__uint_as_float(g[2 * j + 1])) * __uint_as_float(u[2 * j + 1]));
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.h) + static_cast<long long>(row) * p.inter + col) = make_uint4(o[0], o[1], o[2], o[3]);
+          if (p.gu_low) {
+            uint16_t* upper = static_cast<uint16_t*>(p.gu) + 2LL * row * p.inter + col;
+            uint8_t* low = p.gu_low + 2LL * row * p.low + col;
+            put_kept(upper, low, g);
+            put_kept(upper + p.inter, low + p.low, u);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
 // Rows of `cols` bf16 values, boxes of 64 columns.
 static CUtensorMap rows_map(const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
   const uint64_t dims[3] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows), 1};
@@ -396,6 +541,38 @@ static void launch_activation(int activation, const Args&... args) {
   throw std::runtime_error("himuon gated_mlp: unknown activation");
 }
 
+template <int ACT, int MT>
+static void launch_rows(const GatedUpArgs& a, cudaStream_t s) {
+  const auto kernel = gated_rows_kernel<ACT, MT>;
+  GatedRowsDev p{};
+  p.h = a.h; p.gu = a.gu; p.gu_low = static_cast<uint8_t*>(a.gu_low);
+  p.rows = a.rows; p.inter = a.inter; p.low = gated_low(a.inter);
+  const int sms = num_sms(), share = (a.inter + sms - 1) / sms;
+  p.features = ((share + (share + 127) / 128 - 1) / ((share + 127) / 128) + 7) / 8 * 8;
+  p.tiles = (a.inter + p.features - 1) / p.features;
+  p.kblocks = (a.hidden + BK - 1) / BK;
+  const int fit = 216 * 1024 / (MT * static_cast<int>(GM_A) + 2 * p.features * 128);
+  p.stages = fit < GR_STAGES ? fit : GR_STAGES;
+  p.status = status_word_ptr();
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GR_SMEM);
+  if (e == cudaSuccess) {
+    kernel<<<p.tiles < sms ? p.tiles : sms, GM_THREADS, GR_SMEM, s>>>(rows_map(a.x, a.rows, a.hidden, a.ld_x, BM), rows_map(a.wg, a.inter, a.hidden, a.ld_wg, p.features),
+                                                                     rows_map(a.wu, a.inter, a.hidden, a.ld_wu, p.features), p);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon gated_mlp launch failed: ") + cudaGetErrorString(e));
+}
+template <int MT>
+static void launch_rows(const GatedUpArgs& a, cudaStream_t s) {
+  switch (a.activation) {
+    case kSilu: return launch_rows<kSilu, MT>(a, s);
+    case kGelu: return launch_rows<kGelu, MT>(a, s);
+    case kGeluTanh: return launch_rows<kGeluTanh, MT>(a, s);
+    case kRelu: return launch_rows<kRelu, MT>(a, s);
+  }
+  throw std::runtime_error("himuon gated_mlp: unknown activation");
+}
+
 void gated_up(const GatedUpArgs& a, cudaStream_t s) {
   if (a.rows <= 0 || a.inter <= 0 || a.hidden <= 0 || a.hidden % 8 || a.inter % 8) throw std::runtime_error("himuon gated_mlp: bad sizes");
   const long long ld = 2LL * a.inter;
@@ -405,6 +582,8 @@ void gated_up(const GatedUpArgs& a, cudaStream_t s) {
   p.rows = a.rows;
   p.inter = a.inter;
   p.low = gated_low(a.inter);
+  if (a.rows <= BM) return launch_rows<1>(a, s);
+  if (a.rows <= 2 * BM) return launch_rows<2>(a, s);
   const CUtensorMap o = rows_map(a.h, a.rows, a.inter, a.inter, BM);
   launch_activation<UP>(a.activation, rows_map(a.x, a.rows, a.hidden, a.ld_x, BM), rows_map(a.wg, a.inter, a.hidden, a.ld_wg, BM),
                         rows_map(a.wu, a.inter, a.hidden, a.ld_wu, BM), o, a.gu ? rows_map(a.gu, a.rows, a.inter, ld, BM) : o,

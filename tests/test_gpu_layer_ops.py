@@ -228,7 +228,8 @@ GATED = ("y", "dx", "dwg", "dwu", "dwd")
 @pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "relu"])
 @pytest.mark.parametrize("T,H,I", [(1, 8, 8), (3, 40, 24), (8, 128, 352), (17, 200, 136), (33, 64, 1000), (64, 640, 264), (65, 640, 264), (129, 72, 128), (300, 264, 520), (777, 640, 1728),
                                    (5, 264, 4104), (24, 320, 2056), (40, 72, 4096), (64, 2048, 8), (200, 264, 5648), (384, 8, 264),
-                                   (385, 264, 520), (390, 8, 8), (400, 72, 128), (513, 640, 264), (65, 4096, 2056), (129, 2048, 2056), (200, 520, 5648)])
+                                   (385, 264, 520), (390, 8, 8), (400, 72, 128), (513, 640, 264), (65, 4096, 2056), (129, 2048, 2056), (200, 520, 5648),
+                                   (100, 4104, 1000), (256, 1000, 2000), (70, 320, 19008), (48, 2056, 8200)])
 def test_gated_mlp(T, H, I, activation):
     ops = _ops()
     x, wg, wu, wd, dy = _block(T, H, I)
@@ -312,19 +313,20 @@ def test_gated_mlp_of_slices_shapes_and_some_gradients():
 def test_gated_mlp_rows_do_not_depend_on_one_another():
     """Up to 32 rows a row has the same bits however many come with it, so it has from 33 to 64, and by tiles; NaN stays in its row and in the weights' gradients."""
     ops = _ops()
-    for rows, some in ((32, (1, 7, 8, 9, 16, 30)), (64, (33, 50)), (400, (385, 390))):
-        x, wg, wu, wd, dy = _block(rows, 640, 1728)
+    for rows, some, H, I in ((32, (1, 7, 8, 9, 16, 30), 640, 1728), (64, (33, 50), 640, 1728), (128, (101, 120), 1360, 3200), (256, (129, 200), 1360, 3200), (400, (385, 390), 640, 1728)):
+        x, wg, wu, wd, dy = _block(rows, H, I)
         whole = ops.gated_mlp(x, wg, wu, wd)
         for n in some:
             assert torch.equal(ops.gated_mlp(x[:n], wg, wu, wd), whole[:n])
-    for n in (60, 300, 400):
+    for n in (60, 120, 200, 400):
+        x, wg, wu, wd, dy = _block(n, *((640, 1728) if n in (60, 400) else (1360, 3200)))
         got = []
-        for t in (x[:n], x[:n].clone()):
+        for t in (x, x.clone()):
             if got:
                 t[3], t[5, 7] = math.nan, math.inf
             t = t.detach().requires_grad_()
             y = ops.gated_mlp(t, wg, wu, wd)
-            got.append((y.detach(), torch.autograd.grad(y, t, dy[:n])[0]))
+            got.append((y.detach(), torch.autograd.grad(y, t, dy)[0]))
         others = torch.ones(n, dtype=torch.bool, device="cuda")
         others[3] = others[5] = False
         for a, b in zip(*got):
