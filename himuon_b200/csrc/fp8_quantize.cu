@@ -75,7 +75,25 @@ template <typename T> struct Eight {
       return m;
     }
   }
-  // The same of the finite ones.
+  // The same of the eight columns of eight rows.
+  static __device__ __forceinline__ void largest_of_columns(const Eight (&rows)[8], uint32_t (&out)[8]) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) m = __vmaxu2(m, rows[r].w[i] & 0x7FFF7FFFu);
+        out[2 * i] = m << 16;
+        out[2 * i + 1] = m & 0xFFFF0000u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) out[i] = max(out[i], rows[r].w[i] & 0x7FFFFFFFu);
+    }
+  }
+  // largest() of the finite ones.
   __device__ __forceinline__ uint32_t largest_finite() const {
     uint32_t m = 0;
 #pragma unroll
@@ -109,6 +127,18 @@ __device__ __forceinline__ uint32_t largest_of(uint32_t m) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
+}
+
+// Of eight values in each of 16 lanes, the largest of all lanes: of the value tc / 2 in lane tc.  (Lanes halve what they have as they go: 8 shuffles, not 32.)
+__device__ __forceinline__ uint32_t largest_of_rows(const uint32_t (&m)[8], int tc) {
+  uint32_t a[4], b[2];
+  const bool h = tc & 8, q = tc & 4, e = tc & 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = max(h ? m[i + 4] : m[i], __shfl_xor_sync(0xffffffffu, h ? m[i] : m[i + 4], 8));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) b[i] = max(q ? a[i + 2] : a[i], __shfl_xor_sync(0xffffffffu, q ? a[i] : a[i + 2], 4));
+  const uint32_t c = max(e ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, e ? b[0] : b[1], 2));
+  return max(c, __shfl_xor_sync(0xffffffffu, c, 1));
 }
 
 // Rows by themselves: 16 threads take RUN neighbouring blocks of a row; the 16 rows of a block of threads have their scales one behind the other, as products read them
@@ -178,52 +208,63 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(Fp8QuantizeArgs a, in
     if ((threadIdx.x & 31) == 0) atomicMax(&s_all, m);
   }
   if constexpr (TURNED == 1) {
+    uint32_t col_max[8] = {};
+    if (finite) {
+      Eight<T>::largest_of_columns(v, col_max);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t b = __float_as_uint(v[i].at(j)) & 0x7FFFFFFFu;
+          col_max[j] = max(col_max[j], b < kInfinite ? b : 0u);
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t b = __float_as_uint(v[i].at(j)) & 0x7FFFFFFFu;
-        m = max(m, finite || b < kInfinite ? b : 0u);
-      }
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      const uint32_t m = max(col_max[j], __shfl_xor_sync(0xffffffffu, col_max[j], 16));
       if ((threadIdx.x & 16) == 0) atomicMax(&s_col[tc * 8 + j], m);
     }
   }
   if (WHOLE || TURNED) __syncthreads();
   const int all = WHOLE ? scale_exponent(s_all) : 0;
+  if constexpr (TURNED == 1) {                         // (once for each column, not by all threads that have values of it)
+    if (threadIdx.x < QT) {
+      const int k = scale_exponent(s_col[threadIdx.x]);
+      if (cblk * QT + threadIdx.x < a.cols) a.turned.scales[(cblk * QT + threadIdx.x) * a.turned.scale_row + rblk * a.turned.scale_col] = power_of_two(k);
+      s_col[threadIdx.x] = __float_as_uint(power_of_two(-k));
+    }
+  }
   if (!finite) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i].mark();
   }
   if constexpr (STRAIGHT != 0) {
     const Fp8Out& o = a.straight;
+    int k_own = 0;
+    if constexpr (STRAIGHT == 1) {
+      k_own = scale_exponent(largest_of_rows(row_max, tc));
+      if ((tc & 1) == 0 && r0 + tc / 2 < a.rows) o.scales[(r0 + tc / 2) * o.scale_row + cblk * o.scale_col] = power_of_two(k_own);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int k = STRAIGHT == QT ? all : scale_exponent(largest_of<16>(row_max[i]));
-      if (r0 + i < a.rows) {
-        if (c0 < o.ld)                                 // (behind the last column, up to the row's end, are zeros)
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(o.values) + (r0 + i) * o.ld + c0) = v[i].quantized(power_of_two(-k));
-        if (tc == 0 && STRAIGHT == 1) o.scales[(r0 + i) * o.scale_row + cblk * o.scale_col] = power_of_two(k);
-      }
+      const int k = STRAIGHT == QT ? all : __shfl_sync(0xffffffffu, k_own, (threadIdx.x & 16) | (2 * i));
+      if (r0 + i < a.rows && c0 < o.ld)                // (behind the last column, up to the row's end, are zeros)
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(o.values) + (r0 + i) * o.ld + c0) = v[i].quantized(power_of_two(-k));
     }
     if (threadIdx.x == 0 && STRAIGHT == QT) o.scales[rblk * o.scale_row + cblk * o.scale_col] = power_of_two(all);
   }
   if constexpr (TURNED != 0) {
     const Fp8Out& o = a.turned;
+    if (TURNED == 1) __syncthreads();                  // (s_col has factors)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = tc * 8 + j;
-      const float by = power_of_two(-(TURNED == QT ? all : scale_exponent(s_col[c])));
+      const float by = TURNED == QT ? power_of_two(-all) : __uint_as_float(s_col[c]);
       s_turned[c * 16 + (tr ^ tc)] = make_uint2(pack4(v[0].at(j) * by, v[1].at(j) * by, v[2].at(j) * by, v[3].at(j) * by),
                                                 pack4(v[4].at(j) * by, v[5].at(j) * by, v[6].at(j) * by, v[7].at(j) * by));
     }
-    if (TURNED == 1) {
-      if (threadIdx.x < QT && cblk * QT + threadIdx.x < a.cols)
-        o.scales[(cblk * QT + threadIdx.x) * o.scale_row + rblk * o.scale_col] = power_of_two(scale_exponent(s_col[threadIdx.x]));
-    } else if (threadIdx.x == 0) {
-      o.scales[cblk * o.scale_row + rblk * o.scale_col] = power_of_two(all);
-    }
+    if (TURNED == QT && threadIdx.x == 0) o.scales[cblk * o.scale_row + rblk * o.scale_col] = power_of_two(all);
     __syncthreads();
     const long long at = rblk * QT + tc * 8;           // now 16 threads for the 128 rows of a column
 #pragma unroll
