@@ -79,18 +79,20 @@ def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[l
 class RotaryFrequencies:
     """How fast the pairs of a head turn.  Made once for a model, outside of a graph's capture; every layer uses it.
 
-    ``rotary_dim``: how many values of a head are turned, the first ones (even, 0 included).  Pair ``i`` turns by
-    ``theta ** (-2 i / rotary_dim)`` a position.  ``scaling``: as ``rope_scaling`` in a model's configuration, with ``rope_type``
-    ``"linear"`` (all frequencies divided by ``factor``), ``"ntk"`` (a larger ``theta``, by ``factor ** (d / (d - 2))``), ``"yarn"``
-    (``factor``, ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``attention_factor``) or ``"llama3"`` (``factor``,
+    ``rotary_dim``: how many values of a head are turned, the first ones (even, 0 included).  Pair ``i`` turns by ``theta ** (-2 i
+    / rotary_dim)`` a position.  ``scaling``: as ``rope_scaling`` in a model's configuration, with ``rope_type`` ``"linear"`` (all
+    frequencies divided by ``factor``), ``"ntk"`` (a larger ``theta``, by ``factor ** (d / (d - 2))``), ``"yarn"`` (``factor``,
+    ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``attention_factor``) or ``"llama3"`` (``factor``,
     ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``).
 
-    ``frequencies``: the angles at position 1 as floats; ``factor``: what cosine and sine are multiplied by (other than 1 with yarn).
+    ``frequencies``: the angles at position 1 as floats; ``factor``: what cosine and sine are multiplied by (other than 1 with
+    yarn).
     """
 
     def __init__(self, rotary_dim: int, theta: float = 10000.0, scaling: dict | None = None, device="cuda"):
         if not isinstance(rotary_dim, int) or rotary_dim < 0 or rotary_dim % 2:
-            raise RuntimeError(f"himuon_b200.ops.RotaryFrequencies: rotary_dim must be an even number of values, got {rotary_dim!r}")
+            raise RuntimeError("himuon_b200.ops.RotaryFrequencies: rotary_dim must be an even number of values, "
+                               f"got {rotary_dim!r}")
         if not (math.isfinite(theta) and theta > 1.0):
             raise RuntimeError(f"himuon_b200.ops.RotaryFrequencies: theta must be above 1, got {theta}")
         self.rotary_dim, self.theta, self.scaling = rotary_dim, float(theta), None if scaling is None else dict(scaling)
@@ -99,7 +101,8 @@ class RotaryFrequencies:
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("himuon_b200.ops.RotaryFrequencies: they would be copied from the host while a graph is captured; make them before the capture")
+            raise RuntimeError("himuon_b200.ops.RotaryFrequencies: they would be copied from the host while a graph is captured; "
+                               "make them before the capture")
         # whole numbers of 2^-64 turns a position: position times this, modulo 2^64, is the place within a turn
         ratios = (f.as_integer_ratio() for f in self.frequencies)
         turns = [((n * 2 ** 65 * 10 ** 50) // (d * TWO_PI_E50) + 1) // 2 % 2 ** 64 for n, d in ratios]
@@ -109,13 +112,14 @@ class RotaryFrequencies:
 
 
 def rotary(x2d, positions, freqs: RotaryFrequencies, heads: int, head_dim: int, interleaved: bool = False):
-    """Turns the first ``freqs.rotary_dim`` values of every head of ``(rows, heads*head_dim)`` rows (which may be a column slice: queries and
-    keys of one projection are turned by one call) by their position; the values behind them pass through.
+    """Turns the first ``freqs.rotary_dim`` values of every head of ``(rows, heads*head_dim)`` rows (which may be a column slice:
+    queries and keys of one projection are turned by one call) by their position; the values behind them pass through.
 
-    ``positions``: int64, one for each row (any value; ``PackedLayout.positions`` has those of a packed batch), or the length ``S`` of
-    sequences that lie one after the other, whose rows have positions ``0..S-1``.  Pairs are ``(i, i + rotary_dim / 2)``, or ``(2 i, 2 i + 1)`` with
-    ``interleaved``.  Returns a new contiguous tensor of the type of ``x2d``; differentiable in ``x2d``, any number of times.  bf16 and fp32 CUDA
-    tensors run the sm_100a kernel, in fp32; under vmap and forward-mode differentiation the PyTorch formulation runs."""
+    ``positions``: int64, one for each row (any value; ``PackedLayout.positions`` has those of a packed batch), or the length
+    ``S`` of sequences that lie one after the other, whose rows have positions ``0..S-1``.  Pairs are ``(i, i + rotary_dim / 2)``,
+    or ``(2 i, 2 i + 1)`` with ``interleaved``.  Returns a new contiguous tensor of the type of ``x2d``; differentiable in
+    ``x2d``, any number of times.  bf16 and fp32 CUDA tensors run the sm_100a kernel, in fp32; under vmap and forward-mode
+    differentiation the PyTorch formulation runs."""
     if not isinstance(freqs, RotaryFrequencies):
         raise RuntimeError("himuon_b200.ops.rotary: freqs must be a RotaryFrequencies")
     if x2d.dim() != 2 or not x2d.is_floating_point() or heads <= 0 or head_dim <= 0:
@@ -128,12 +132,14 @@ def rotary(x2d, positions, freqs: RotaryFrequencies, heads: int, head_dim: int, 
     rows, seq_len = x2d.shape[0], 1
     if isinstance(positions, torch.Tensor):
         if positions.dtype != torch.int64 or positions.dim() != 1 or positions.shape[0] != rows or positions.device != x2d.device:
-            raise RuntimeError(f"himuon_b200.ops.rotary: positions must be int64, one for each of the {rows} rows, on {x2d.device}")
+            raise RuntimeError(f"himuon_b200.ops.rotary: positions must be int64, one for each of the {rows} rows, "
+                               f"on {x2d.device}")
         positions = positions.contiguous()
     else:
         seq_len, positions = positions, None
         if not isinstance(seq_len, int) or seq_len <= 0 or rows % seq_len:
-            raise RuntimeError(f"himuon_b200.ops.rotary: positions must be a tensor or the length of sequences that {rows} rows hold, got {seq_len!r}")
+            raise RuntimeError("himuon_b200.ops.rotary: positions must be a tensor or the length of sequences that "
+                               f"{rows} rows hold, got {seq_len!r}")
     transformed = _any_transformed(x2d)
     if x2d.is_cuda and x2d.dtype in (torch.bfloat16, torch.float32) and not transformed:
         if x2d.stride(1) != 1 and x2d.shape[1] > 1:
