@@ -736,6 +736,43 @@ def test_launches_over_one_another_see_what_came_before(rows):
     _clean()
 
 
+@pytest.mark.parametrize("rows", [8, 300])
+def test_products_in_branches_of_a_graph(rows):
+    """First in a graph, behind copies and fills, on a branch that joins again, behind two branches."""
+    ops = _ops()
+    torch.manual_seed(rows + 103)
+    x = torch.randn(rows, 640, device="cuda").bfloat16()
+    q = [ops.quantize_fp8((torch.randn(1728, 640, device="cuda") * 0.05).bfloat16(), 128) for _ in range(2)]
+    w = [(torch.randn(*s, device="cuda") * 0.05).bfloat16() for s in ((1728, 640), (1728, 640), (640, 1728))]
+    a = ops.quantize_fp8(x)
+    want = [ops.fp8_matmul(a, q[0]), ops.fp8_linear(x, q[1]), ops.gated_mlp(x, *w)]
+    torch.cuda.synchronize()
+    values, scales, y = torch.zeros_like(a.values), torch.zeros_like(a.scales), torch.zeros_like(x)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = ops.fp8_matmul(a, q[0])
+        main = torch.cuda.current_stream()
+        values.view(torch.uint8).copy_(a.values.view(torch.uint8))
+        scales.zero_()
+        scales.copy_(a.scales)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            y.copy_(x)
+            other = ops.fp8_linear(y, q[1])
+            block = ops.gated_mlp(y, *w)
+        second = ops.fp8_matmul(a._replace(values=values, scales=scales), q[0])
+        main.wait_stream(side)
+        joined = ops.fp8_matmul(a._replace(values=values, scales=scales), q[0])
+        last = ops.gated_mlp(y, *w)
+    for _ in range(3):
+        for t in (first, second, joined, other, block, last):
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(t, want[0]) for t in (first, second, joined)) and torch.equal(other, want[1])
+        assert torch.equal(block, want[2]) and torch.equal(last, want[2])
+    _clean()
+
+
 def test_offsets_beyond_32_bits():
     """More than 2^31 values: the last rows are those of a call with nothing else."""
     ops = _ops()
