@@ -246,6 +246,12 @@ gemm2_finish_kernel(const float* __restrict__ ws, GemmDev p, int first_tail_tile
     const int t = static_cast<int>(i / per_tile);
     const int e = static_cast<int>(i - t * per_tile);
     const int r = e >> 6, c = (e & 63) * 4;
+    const int tile = first_tail_tile + t;
+    const int b = tile / tiles_per_batch;
+    const int rr = tile - b * tiles_per_batch;
+    const int row = (rr % p.tiles_m) * 256 + r;
+    const int col = (rr / p.tiles_m) * 256 + c;
+    if (row >= p.M || col >= p.N) continue;              // (before the parts are read: of few rows most of a tile is not there)
     const float4* src = reinterpret_cast<const float4*>(ws + (static_cast<long long>(t) * p.nslices * 256 + r) * 256 + c);
     float4 v = src[0];
 #pragma unroll 4
@@ -253,12 +259,6 @@ gemm2_finish_kernel(const float* __restrict__ ws, GemmDev p, int first_tail_tile
       const float4 u = src[s * per_tile];
       v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
     }
-    const int tile = first_tail_tile + t;
-    const int b = tile / tiles_per_batch;
-    const int rr = tile - b * tiles_per_batch;
-    const int row = (rr % p.tiles_m) * 256 + r;
-    const int col = (rr / p.tiles_m) * 256 + c;
-    if (row >= p.M) continue;
     const float vals[4] = {v.x, v.y, v.z, v.w};
     T* cp = reinterpret_cast<T*>(p.C) + static_cast<long long>(b) * p.strideC + static_cast<long long>(row) * p.ldc + col;
     const T* xp = p.aux ? reinterpret_cast<const T*>(p.aux) + static_cast<long long>(b) * p.strideAux +
