@@ -55,7 +55,7 @@ struct TmapKeyHash {
   }
 };
 
-// Encodes (and caches) a tiled tensor map of rank 3 or 4 over 8-bit, 16-bit or 32-bit elements.
+// Encodes (and caches) a tiled tensor map of rank 2 to 4 over 8-bit, 16-bit or 32-bit elements.
 // dims/box are innermost-first; strides[i] is the byte stride of dimension i+1.
 // Requirements checked here: base 16-byte aligned, strides multiples of 16 bytes,
 // inner box extent * element size a multiple of 16 bytes and at most 128 bytes when swizzled.
