@@ -1,0 +1,96 @@
+"""The rotary positions, the gated feed-forward block and the 8-bit products on the GPU where they have been wrong: far gates, rows that come
+with others, transforms of operands that are not the first, angles next to half a turn (GPU tier).
+
+Bounds follow from the kernels' roundings and stand where they are used; U = 2^-8 is what rounding to bf16 changes a value by at most.
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -8
+
+
+def _ops():
+    from himuon_b200 import ops
+
+    return ops
+
+
+def _clean():
+    from himuon_b200._ext import ext
+
+    torch.cuda.synchronize()
+    assert ext().status(True) == 0, "a bounded device wait ran out (status word set)"
+
+
+# ------------------------------------------------------------------------------------------- far gates
+SIDE = 1448                       # hidden and intermediate features: 20, 200 and 400 rows of them go to different kernels
+
+
+def _gates_as_given(rows, gates, up):
+    """Leaves whose gate projections are `gates` (one for each feature) and up projections `up`, exactly, in every row; the down projection
+    passes features through."""
+    x = torch.zeros(rows, SIDE, device="cuda")
+    x[:, 0], x[:, 1] = 1.0, 2.0 ** (math.frexp(up)[1] // 2)
+    wg, wu = (torch.zeros(SIDE, SIDE, device="cuda") for _ in range(2))
+    wg[:, 0] = gates
+    wu[:, 1] = up / x[0, 1]
+    leaves = [t.bfloat16().requires_grad_() for t in (x, wg, wu, torch.eye(SIDE, device="cuda"))]
+    assert (leaves[1][:, 0].double() == gates.double()).all() and (x[0, 1].double() * leaves[2][:, 1].double() == up).all()
+    return leaves
+
+
+@pytest.mark.parametrize("rows", [20, 200, 400])
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_far_negative_gates_are_nothing(activation, rows):
+    """Below -120 an activation is smaller than fp32's least number: results and gradients are 0, up to the least gate that bf16 has."""
+    ops = _ops()
+    gates = -torch.exp2(torch.linspace(7.0, 127.0, SIDE, device="cuda")).bfloat16().float()
+    gates[-1] = torch.finfo(torch.bfloat16).min
+    leaves = _gates_as_given(rows, gates, 3.0)
+    y = ops.gated_mlp(*leaves, activation=activation)
+    grads = torch.autograd.grad(y, leaves, torch.randn_like(y))
+    for name, t in zip(("y", "dx", "dwg", "dwu", "dwd"), (y, *grads)):
+        assert not t.any(), (name, t.abs().max().item())
+    _clean()
+
+
+@pytest.mark.parametrize("rows", [20, 200, 400])
+def test_gates_where_the_sigmoid_leaves_the_range_of_numbers(rows):
+    """silu of -60 to -100, seen through an up projection of 2^100.  The sigmoid is 0 below 2^-126; an exponential of 127 ln 2 is good to 2^-16 (its
+    argument's rounding, 2^-18, and the constant's) as is what is made of it."""
+    ops = _ops()
+    gates = torch.linspace(-100.0, -60.0, SIDE, device="cuda").bfloat16().float()
+    up = 2.0 ** 100
+    leaves = _gates_as_given(rows, gates, up)
+    y = ops.gated_mlp(*leaves)
+    _, dwg, dwu, _ = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    g = gates.double()
+    s = torch.sigmoid(g)
+    a, d = g * s, s * (1.0 + g * torch.sigmoid(-g))
+    near, least = 2.0 ** -16, 101.0 * 2.0 ** -126
+    h, side = a * up, leaves[0][0, 1].double()
+    # h, or dg and du, are rounded to bf16 and so is the result
+    for name, got, want, scale in (("y", y.double(), h.expand(rows, -1), up), ("dwg", dwg[:, 0].double(), rows * up * d, rows * up), ("dwu", dwu[:, 1].double(), rows * side * a, rows * side)):
+        bound = (2 * U + U * U + 2 * near) * want.abs() + 1.01 * least * scale
+        over = (got - want).abs() - bound
+        assert (over <= 0).all(), (name, over.max().item())
+    _clean()
+
+
+@pytest.mark.parametrize("rows", [20, 200, 400])
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+def test_gates_that_are_no_numbers(activation, rows):
+    """-inf times a sigmoid of 0 is no number, and NaN stays."""
+    ops = _ops()
+    for gate in (-math.inf, math.nan):
+        x = torch.zeros(rows, SIDE, device="cuda")
+        wg, wu = (torch.zeros(SIDE, SIDE, device="cuda") for _ in range(2))
+        x[:, 0], wg[:, 0], wu[:, 0] = 1.0, gate, 1.0
+        y = ops.gated_mlp(*(t.bfloat16() for t in (x, wg, wu, torch.ones(SIDE, SIDE, device="cuda"))), activation=activation)
+        assert y.isnan().all()
+    _clean()
