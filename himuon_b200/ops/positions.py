@@ -54,7 +54,13 @@ def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[l
         def pair_of(turns: float) -> float:
             return rotary_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(theta))
 
-        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rotary_dim - 1)
+        truncate = scaling.get("truncate", True)
+        if not isinstance(truncate, bool):
+            raise RuntimeError(f"himuon_b200.ops.{op}: truncate must be true or false, got {truncate!r}")
+        lo, hi = pair_of(fast), pair_of(slow)
+        if truncate:                     # the ramp starts and ends at whole pairs
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
         span = float(hi - lo) if hi != lo else 0.001
         attention = scaling.get("attention_factor")
         if attention is None:
@@ -82,7 +88,7 @@ class RotaryFrequencies:
     ``rotary_dim``: how many values of a head are turned, the first ones (even, 0 included).  Pair ``i`` turns by ``theta ** (-2 i
     / rotary_dim)`` a position.  ``scaling``: as ``rope_scaling`` in a model's configuration, with ``rope_type`` ``"linear"`` (all
     frequencies divided by ``factor``), ``"ntk"`` (a larger ``theta``, by ``factor ** (d / (d - 2))``), ``"yarn"`` (``factor``,
-    ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``attention_factor``) or ``"llama3"`` (``factor``,
+    ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``truncate``, ``attention_factor``) or ``"llama3"`` (``factor``,
     ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``).
 
     ``frequencies``: the angles at position 1 as floats; ``factor``: what cosine and sine are multiplied by (other than 1 with
