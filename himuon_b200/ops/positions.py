@@ -62,11 +62,16 @@ def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[l
             lo, hi = math.floor(lo), math.ceil(hi)
         lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
         span = float(hi - lo) if hi != lo else 0.001
-        attention = scaling.get("attention_factor")
-        if attention is None:
-            attention = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
-        else:
+
+        def stretch(k: float) -> float:
+            return 0.1 * k * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+
+        if scaling.get("attention_factor") is not None:
             attention = _number(op, scaling, "attention_factor")
+        elif scaling.get("mscale") is None and scaling.get("mscale_all_dim") is None:
+            attention = stretch(1.0)
+        else:                            # (both or none: readers differ on what one of them means)
+            attention = stretch(_number(op, scaling, "mscale")) / stretch(_number(op, scaling, "mscale_all_dim"))
         out = []
         for i, f in enumerate(inv):
             ramp = min(max((i - lo) / span, 0.0), 1.0)
@@ -88,8 +93,8 @@ class RotaryFrequencies:
     ``rotary_dim``: how many values of a head are turned, the first ones (even, 0 included).  Pair ``i`` turns by ``theta ** (-2 i
     / rotary_dim)`` a position.  ``scaling``: as ``rope_scaling`` in a model's configuration, with ``rope_type`` ``"linear"`` (all
     frequencies divided by ``factor``), ``"ntk"`` (a larger ``theta``, by ``factor ** (d / (d - 2))``), ``"yarn"`` (``factor``,
-    ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``truncate``, ``attention_factor``) or ``"llama3"`` (``factor``,
-    ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``).
+    ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``truncate``, and ``attention_factor`` or ``mscale`` with
+    ``mscale_all_dim``) or ``"llama3"`` (``factor``, ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``).
 
     ``frequencies``: the angles at position 1 as floats; ``factor``: what cosine and sine are multiplied by (other than 1 with
     yarn).

@@ -47,3 +47,23 @@ def test_yarn_with_and_without_whole_pairs(d, theta):
     for wrong in (1, 0.0, "false"):
         with pytest.raises(RuntimeError, match="truncate"):
             _freqs(d, theta, {**YARN, "truncate": wrong})
+
+
+def test_yarn_factor_of_cosine_and_sine():
+    """0.1 k ln factor + 1 for k = 1, or the quotient of two of them, or as given; 1 where nothing is stretched."""
+    def m(k, factor):
+        return 0.1 * k * math.log(factor) + 1.0
+
+    for factor in (40.0, 1.5):
+        s = {**YARN, "factor": factor}
+        assert math.isclose(_freqs(64, 1e4, s)[1], m(1.0, factor), rel_tol=1e-15)
+        for k, all_dim in ((1.0, 1.0), (0.707, 0.707), (1.0, 0.8), (0.4, 1.2)):
+            got, scale = _freqs(64, 1e4, {**s, "mscale": k, "mscale_all_dim": all_dim})
+            assert math.isclose(scale, m(k, factor) / m(all_dim, factor), rel_tol=1e-15) and got == _freqs(64, 1e4, s)[0]
+        assert _freqs(64, 1e4, {**s, "mscale": 1.0, "mscale_all_dim": 1.0})[1] == 1.0
+        assert _freqs(64, 1e4, {**s, "mscale": 1.0, "mscale_all_dim": 2.0, "attention_factor": 1.25})[1] == 1.25
+        # one of them alone means different things to different readers
+        for alone in ({"mscale": 1.0}, {"mscale_all_dim": 1.0}, {"mscale": 0.707, "mscale_all_dim": None}, {"mscale": 0.707, "mscale_all_dim": 0}):
+            with pytest.raises(RuntimeError, match="mscale"):
+                _freqs(64, 1e4, {**s, **alone})
+    assert _freqs(64, 1e4, {**YARN, "factor": 0.5, "mscale": 1.0, "mscale_all_dim": 0.5})[1] == 1.0 == _freqs(64, 1e4, {**YARN, "factor": 1.0})[1]
