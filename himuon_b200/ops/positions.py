@@ -31,6 +31,8 @@ def _number(op: str, d: dict, key: str, default=None, least: float = 0.0) -> flo
 def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[list[float], float]:
     """(angle of each pair at position 1 in 64 bits, factor of cosine and sine)."""
     op, pairs = "RotaryFrequencies", rotary_dim // 2
+    if scaling is not None:
+        scaling = {k: v for k, v in scaling.items() if v is not None}      # (a key without a value is not there)
     kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
     if kind in (None, "default"):
         if scaling is not None and kind is None:
@@ -66,12 +68,12 @@ def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[l
         def stretch(k: float) -> float:
             return 0.1 * k * math.log(factor) + 1.0 if factor > 1.0 else 1.0
 
-        if scaling.get("attention_factor") is not None:
+        if "attention_factor" in scaling:
             attention = _number(op, scaling, "attention_factor")
-        elif scaling.get("mscale") is None and scaling.get("mscale_all_dim") is None:
-            attention = stretch(1.0)
-        else:                            # (both or none: readers differ on what one of them means)
+        elif "mscale" in scaling or "mscale_all_dim" in scaling:      # (both: readers differ on what one of them means)
             attention = stretch(_number(op, scaling, "mscale")) / stretch(_number(op, scaling, "mscale_all_dim"))
+        else:
+            attention = stretch(1.0)
         out = []
         for i, f in enumerate(inv):
             ramp = min(max((i - lo) / span, 0.0), 1.0)

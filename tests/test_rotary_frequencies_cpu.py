@@ -67,3 +67,11 @@ def test_yarn_factor_of_cosine_and_sine():
             with pytest.raises(RuntimeError, match="mscale"):
                 _freqs(64, 1e4, {**s, **alone})
     assert _freqs(64, 1e4, {**YARN, "factor": 0.5, "mscale": 1.0, "mscale_all_dim": 0.5})[1] == 1.0 == _freqs(64, 1e4, {**YARN, "factor": 1.0})[1]
+
+
+def test_keys_without_a_value_are_not_there():
+    absent = dict.fromkeys(("beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"))
+    assert _freqs(64, 1e4, {**YARN, **absent}) == _freqs(64, 1e4, YARN)
+    assert _freqs(64, 1e4, {"rope_type": None, "type": "linear", "factor": 4.0}) == _freqs(64, 1e4, {"rope_type": "linear", "factor": 4.0})
+    with pytest.raises(RuntimeError, match="needs factor"):
+        _freqs(64, 1e4, {"rope_type": "linear", "factor": None})
