@@ -16,6 +16,13 @@ from . import reference as ref
 
 TWO_PI_E50 = 628318530717958647692528676655900576839433879875021      # 2 pi * 10^50
 SCALINGS = ("linear", "ntk", "yarn", "llama3")
+# What each of them is made of.  Any other key is refused: it may change the frequencies, and nothing would say so.
+LENGTH = "original_max_position_embeddings"
+SCALING_KEYS = {
+    "default": (), "linear": ("factor",), "ntk": ("factor",),
+    "yarn": ("factor", LENGTH, "beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"),
+    "llama3": ("factor", LENGTH, "low_freq_factor", "high_freq_factor"),
+}
 
 
 def _number(op: str, d: dict, key: str, default=None, least: float = 0.0) -> float:
@@ -28,18 +35,31 @@ def _number(op: str, d: dict, key: str, default=None, least: float = 0.0) -> flo
     return value
 
 
+def _form(op: str, theta: float, scaling: dict) -> tuple[str, dict]:
+    """The form of a scaling and what it is made of."""
+    scaling = {k: v for k, v in scaling.items() if v is not None}      # (a key without a value is not there)
+    names = [scaling[k] for k in ("rope_type", "type") if k in scaling]
+    if not names:
+        raise RuntimeError(f"himuon_b200.ops.{op}: scaling needs rope_type, one of {SCALINGS}")
+    kind = names[0]
+    if names[-1] != kind or kind not in ("default", *SCALINGS):
+        raise RuntimeError(f"himuon_b200.ops.{op}: rope_type must be one of {SCALINGS}, got {' and '.join(map(repr, names))}")
+    if float(scaling.get("rope_theta", theta)) != theta:
+        raise RuntimeError(f"himuon_b200.ops.{op}: rope_theta of the scaling is {scaling['rope_theta']}, theta is {theta}")
+    # (a length may always be there: the forms that do not name it have no use for one)
+    unknown = [str(k) for k in scaling if k not in (*SCALING_KEYS[kind], "rope_type", "type", "rope_theta", LENGTH)]
+    if unknown:
+        raise RuntimeError(f"himuon_b200.ops.{op}: a scaling of rope_type {kind} takes {SCALING_KEYS[kind]}, got {', '.join(unknown)}")
+    return kind, scaling
+
+
 def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[list[float], float]:
     """(angle of each pair at position 1 in 64 bits, factor of cosine and sine)."""
-    op, pairs = "RotaryFrequencies", rotary_dim // 2
+    op, pairs, kind = "RotaryFrequencies", rotary_dim // 2, "default"
     if scaling is not None:
-        scaling = {k: v for k, v in scaling.items() if v is not None}      # (a key without a value is not there)
-    kind = None if scaling is None else scaling.get("rope_type", scaling.get("type"))
-    if kind in (None, "default"):
-        if scaling is not None and kind is None:
-            raise RuntimeError(f"himuon_b200.ops.{op}: scaling needs rope_type, one of {SCALINGS}")
+        kind, scaling = _form(op, theta, scaling)
+    if kind == "default":
         return [theta ** (-2.0 * i / rotary_dim) for i in range(pairs)], 1.0
-    if kind not in SCALINGS:
-        raise RuntimeError(f"himuon_b200.ops.{op}: rope_type must be one of {SCALINGS}, got {kind!r}")
     factor = _number(op, scaling, "factor")
     if kind == "ntk":                    # a larger base: the last pair ends up `factor` times as long, the first as it was
         if rotary_dim > 2:
@@ -48,7 +68,7 @@ def _frequencies(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[l
     inv = [theta ** (-2.0 * i / rotary_dim) for i in range(pairs)]
     if kind == "linear":
         return [f / factor for f in inv], 1.0
-    length = _number(op, scaling, "original_max_position_embeddings")
+    length = _number(op, scaling, LENGTH)
     if kind == "yarn":
         # pairs that turn often within the original length stay, those that do not turn once are stretched, a ramp between them
         fast, slow = _number(op, scaling, "beta_fast", 32.0), _number(op, scaling, "beta_slow", 1.0)
@@ -97,6 +117,7 @@ class RotaryFrequencies:
     frequencies divided by ``factor``), ``"ntk"`` (a larger ``theta``, by ``factor ** (d / (d - 2))``), ``"yarn"`` (``factor``,
     ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``truncate``, and ``attention_factor`` or ``mscale`` with
     ``mscale_all_dim``) or ``"llama3"`` (``factor``, ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``).
+    Other keys are refused, as is a ``rope_theta`` other than ``theta``.
 
     ``frequencies``: the angles at position 1 as floats; ``factor``: what cosine and sine are multiplied by (other than 1 with
     yarn).

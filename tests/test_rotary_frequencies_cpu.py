@@ -75,3 +75,37 @@ def test_keys_without_a_value_are_not_there():
     assert _freqs(64, 1e4, {"rope_type": None, "type": "linear", "factor": 4.0}) == _freqs(64, 1e4, {"rope_type": "linear", "factor": 4.0})
     with pytest.raises(RuntimeError, match="needs factor"):
         _freqs(64, 1e4, {"rope_type": "linear", "factor": None})
+
+
+LLAMA3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_max_position_embeddings": 8192}
+
+
+def test_keys_that_are_not_known_are_refused():
+    """Whatever a form does not take may change its frequencies."""
+    linear, ntk, default = {"rope_type": "linear", "factor": 4.0}, {"rope_type": "ntk", "factor": 4.0}, {"rope_type": "default"}
+    for s in (linear, ntk, default, LLAMA3):
+        for key, value in (("beta_fast", 16.0), ("mscale", 1.0), ("truncate", False), ("attention_factor", 1.0)):
+            with pytest.raises(RuntimeError, match=f"RotaryFrequencies: .*{key}"):
+                _freqs(64, 1e4, {**s, key: value})
+    for s in (linear, ntk, default, YARN, LLAMA3):
+        for key, value in (("partial_rotary_factor", 0.5), ("mrope_section", [16, 24, 24]), ("short_factor", [1.0] * 32), ("Factor", 2.0), (5, 2.0)):
+            with pytest.raises(RuntimeError, match=f"RotaryFrequencies: .*{key}"):
+                _freqs(64, 1e4, {**s, key: value})
+    for s in (default, YARN):
+        with pytest.raises(RuntimeError, match="low_freq_factor"):
+            _freqs(64, 1e4, {**s, "low_freq_factor": 1.0})
+    with pytest.raises(RuntimeError, match="factor"):
+        _freqs(64, 1e4, {**default, "factor": 4.0})
+
+
+def test_keys_that_say_the_same_twice_have_to_agree():
+    """Configurations have the form under both of its names, and the base beside the scaling."""
+    for s in (YARN, LLAMA3, {"rope_type": "default"}):
+        want = _freqs(64, 1e4, s)
+        assert _freqs(64, 1e4, {**s, "type": s["rope_type"], "rope_theta": 10000}) == want
+        with pytest.raises(RuntimeError, match="rope_type"):
+            _freqs(64, 1e4, {**s, "type": "mrope"})
+        with pytest.raises(RuntimeError, match="rope_theta"):
+            _freqs(64, 1e4, {**s, "rope_theta": 500000.0})
+    # lengths have no part in these
+    assert _freqs(64, 1e4, {"rope_type": "linear", "factor": 4.0, "original_max_position_embeddings": 4096}) == _freqs(64, 1e4, {"rope_type": "linear", "factor": 4.0})
