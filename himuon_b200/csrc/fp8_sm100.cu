@@ -16,6 +16,7 @@
 #include "fp8.h"
 #include "gemm_epilogue.cuh"
 #include "himuon.h"
+#include "kernel_host.h"
 #include "pair_common.cuh"
 #include "sm100_common.cuh"
 #include "tma_host.h"
@@ -579,32 +580,6 @@ static CUtensorMap bytes_map(const Fp8Matrix& m) {
   const uint64_t strides[2] = {static_cast<uint64_t>(m.ld), static_cast<uint64_t>(m.ld) * static_cast<uint64_t>(m.rows)};
   const uint32_t box[3] = {F8_K, BM, 1};
   return make_tmap(m.values, 3, dims, strides, box, 1, true);
-}
-
-// CTA pairs that can be resident at once on the current device.  (Callers and the autograd engine's threads may ask at the same time.)
-template <class Kernel>
-static int pairs_at_once(Kernel kernel, int threads, size_t smem, std::atomic<int>* most) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const bool known = dev >= 0 && dev < 64;
-  int n = known ? most[dev].load(std::memory_order_relaxed) : 0;
-  if (n == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_sms());
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
-      cudaGetLastError();
-      n = num_sms() / 2;
-    }
-    if (known) most[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
 }
 
 // A launch that may begin before the kernel before it has ended (it waits for it itself).

@@ -15,6 +15,7 @@
 #include "gated_mlp.h"
 #include "gemm_epilogue.cuh"
 #include "himuon.h"
+#include "kernel_host.h"
 #include "pair_common.cuh"
 #include "sm100_common.cuh"
 #include "tma_host.h"
@@ -483,32 +484,6 @@ static CUtensorMap rows_map(const void* ptr, long long rows, long long cols, lon
   return make_tmap(ptr, 3, dims, strides, box, 2, true);
 }
 
-// CTA pairs that can be resident at once on the current device.  (Callers and the autograd engine's threads may ask at the same time.)
-template <class Kernel>
-static int pairs_at_once(Kernel kernel, size_t smem, std::atomic<int>* most) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const bool known = dev >= 0 && dev < 64;
-  int n = known ? most[dev].load(std::memory_order_relaxed) : 0;
-  if (n == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_sms());
-    cfg.blockDim = dim3(GM_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
-      cudaGetLastError();
-      n = num_sms() / 2;
-    }
-    if (known) most[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 template <int MODE, int ACT>
 static void launch(const CUtensorMap& a, const CUtensorMap& b0, const CUtensorMap& b1, const CUtensorMap& o, const CUtensorMap& g, const CUtensorMap& u,
                    GatedDev p, int inner, cudaStream_t s) {
@@ -518,7 +493,7 @@ static void launch(const CUtensorMap& a, const CUtensorMap& b0, const CUtensorMa
   const auto kernel = gated_mlp_kernel<MODE, ACT>;
   const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
   if (set != cudaSuccess) throw std::runtime_error(std::string("himuon gated_mlp: ") + cudaGetErrorString(set));
-  const int pairs = pairs_at_once(kernel, SMEM, most);
+  const int pairs = pairs_at_once(kernel, GM_THREADS, SMEM, most);
   constexpr int FEATURES = MODE == UP ? 128 : 256;
   p.tiles_m = (p.rows + 2 * BM - 1) / (2 * BM);
   p.tiles_n = (p.inter + FEATURES - 1) / FEATURES;

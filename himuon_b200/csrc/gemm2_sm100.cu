@@ -13,6 +13,7 @@
 // Every wait is bounded; both CTAs always reach the closing cluster barrier.
 #include "gemm_epilogue.cuh"
 #include "himuon.h"
+#include "kernel_host.h"
 #include "pair_common.cuh"
 #include "sm100_common.cuh"
 #include "tma_host.h"
@@ -293,11 +294,8 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + 2 * SLAB_BYTES + 256;
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
   auto kern = gemm2_bf16_kernel<STAGES, A_MN, B_MN, Second>;
-  static bool attr_done = false;
-  if (!attr_done) {
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
-    attr_done = true;
-  }
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(kern, SMEM, allowed);
   const CUtensorMap tmA = operand_tmap(a.A, A_MN, a.M, a.K, a.lda, a.batch, a.strideA);
   const CUtensorMap tmB = operand_tmap(a.B, B_MN, a.N, a.K, a.ldb, a.batch, a.strideB);
   const int esz = a.out_fp32 ? 4 : 2;
@@ -330,23 +328,8 @@ static void launch_gemm2(const GemmArgs& a, cudaStream_t stream) {
   p.status = status_word_ptr();
   const long long total = static_cast<long long>(p.tiles_m) * p.tiles_n * a.batch;
   p.full_items = p.total_items = static_cast<int>(total);
-  // Clusters that can be resident at once (GPCs with an odd number of free SMs leave one SM unpaired).
-  static int max_pairs = 0;
-  if (max_pairs == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_sms());
-    cfg.blockDim = dim3(GEMM2_THREADS);
-    cfg.dynamicSmemBytes = SMEM;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) max_pairs = n;
-    else { cudaGetLastError(); max_pairs = num_sms() / 2; }
-  }
-  int cap = max_pairs;
+  static std::atomic<int> most[64] = {};
+  int cap = pairs_at_once(kern, GEMM2_THREADS, SMEM, most);
   if (a.max_ctas > 0 && a.max_ctas / 2 < cap) cap = a.max_ctas / 2 > 0 ? a.max_ctas / 2 : 1;
   // Split the tiles of a mostly idle last wave along K: each K-slice stores its fp32 partial in the caller's scratch and a small
   // follow-up kernel adds them and applies the epilogue.

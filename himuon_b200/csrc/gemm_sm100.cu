@@ -20,6 +20,7 @@
 // and the cuBLAS calls behind F.linear / torch.addmm.
 #include "gemm_epilogue.cuh"
 #include "himuon.h"
+#include "kernel_host.h"
 #include "sm100_common.cuh"
 #include "tma_host.h"
 
@@ -384,11 +385,8 @@ static void launch_gemm(const GemmArgs& a, cudaStream_t stream) {
   constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + NSTG * SLAB_BYTES + 256;
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
   auto kern = gemm_bf16_kernel<BN, STAGES, NSTG, A_MN, B_MN, AUX_TMA>;
-  static bool attr_done = false;
-  if (!attr_done) {
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
-    attr_done = true;
-  }
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(kern, SMEM, allowed);
   // A: K-major storage (M rows x K) or MN-major storage (K rows x M).
   uint64_t dimsA[3], strA[2], dimsB[3], strB[2];
   uint32_t boxA[3], boxB[3];

@@ -16,6 +16,7 @@
 
 #include "gemm_epilogue.cuh"
 #include "himuon.h"
+#include "kernel_host.h"
 #include "pair_common.cuh"
 #include "sm100_common.cuh"
 #include "tma_host.h"
@@ -558,40 +559,14 @@ static CUtensorMap rows_tmap(const void* ptr, int rows, int cols, long long ld, 
   return make_tmap(ptr, 3, dims, strides, box, 2, true);
 }
 
-// CTA pairs that can be resident at once on the current device.  (Callers and the autograd engine's threads may ask at the same time.)
-template <int MODE>
-static int pairs_at_once(size_t smem) {
-  static std::atomic<int> most[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const bool known = dev >= 0 && dev < 64;
-  int n = known ? most[dev].load(std::memory_order_relaxed) : 0;
-  if (n == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_sms());
-    cfg.blockDim = dim3(LS_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, linear_scores_kernel<MODE>, &cfg) != cudaSuccess || n <= 0) {
-      cudaGetLastError();
-      n = num_sms() / 2;
-    }
-    if (known) most[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 template <int MODE>
 static void launch(const LinearScoreArgs& a, LinScoresDev& p, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + LS_STAGES * LS_STAGE + 2 * SLAB_BYTES + 256;
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
   const cudaError_t set = cudaFuncSetAttribute(linear_scores_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SMEM));
   if (set != cudaSuccess) throw std::runtime_error(std::string("himuon linear_scores: ") + cudaGetErrorString(set));
-  const int pairs = pairs_at_once<MODE>(SMEM);
+  static std::atomic<int> most[64] = {};
+  const int pairs = pairs_at_once(linear_scores_kernel<MODE>, LS_THREADS, SMEM, most);
   p.tiles_m = (p.rows + 2 * BM - 1) / (2 * BM);
   p.tiles_n = (p.vocab + LS_N - 1) / LS_N;
   p.kblocks = (a.hidden + BK - 1) / BK;

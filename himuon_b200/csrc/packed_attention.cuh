@@ -1,11 +1,11 @@
 // What the forward and the backward kernels of packed attention share (packed_attention_sm100.cu has the formulas and the tiles).
 #pragma once
 
-#include <atomic>
 #include <string>
 #include <type_traits>
 
 #include "attention_common.cuh"
+#include "kernel_host.h"
 
 namespace himuon {
 
@@ -114,17 +114,6 @@ inline PackedDev make_dev(const PackedAttnArgs& a) {
   p.scale = a.scale; p.scale_log2 = a.scale * kLog2e;
   p.status = status_word_ptr();
   return p;
-}
-// Once for each kernel and device.
-template <typename K>
-void allow_smem(K kern, size_t bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-  if (e != cudaSuccess) throw std::runtime_error(std::string("himuon packed attention: ") + cudaGetErrorString(e));
-  done.fetch_or(bit, std::memory_order_relaxed);
 }
 inline void check_packed_launch(const char* what) {
   const cudaError_t e = cudaGetLastError();

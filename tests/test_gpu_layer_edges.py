@@ -94,3 +94,20 @@ def test_gates_that_are_no_numbers(activation, rows):
         y = ops.gated_mlp(*(t.bfloat16() for t in (x, wg, wu, torch.ones(SIDE, SIDE, device="cuda"))), activation=activation)
         assert y.isnan().all()
     _clean()
+
+
+# ------------------------------------------------------------------------------------------- more than one device
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_products_on_a_second_device_of_the_process():
+    """What a kernel is allowed, and how many of its blocks fit, is asked on each device: the same calls on the first and then on another."""
+    ops = _ops()
+    torch.manual_seed(5)
+    for rows in (24, 100, 200, 400):
+        x, wg, wu, wd = (torch.randn(*s).bfloat16() * 0.1 for s in ((rows, 640), (1728, 640), (1728, 640), (640, 1728)))
+        got = []
+        for device in ("cuda:0", "cuda:1"):
+            leaves = [t.to(device).requires_grad_() for t in (x, wg, wu, wd)]
+            y = ops.gated_mlp(*leaves) + ops.fp8_linear(ops.linear(leaves[0], leaves[1]), leaves[3])
+            got.append([t.cpu() for t in (y.detach(), *torch.autograd.grad(y.sum(), leaves))])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+    _clean()
