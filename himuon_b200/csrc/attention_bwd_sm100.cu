@@ -26,6 +26,7 @@
 // with 16 heads over 8 191 -> 139 us, 4 x 1000 with 32 over 8 373 -> 270 us, 2 x 1984 with 16 over 8 304 -> 205 us;
 // 4 x 1024 (whole sub-blocks) 149 us before and after.
 #include "attention_common.cuh"
+#include "kernel_host.h"
 
 #include <string>
 
@@ -471,8 +472,8 @@ flash_bwd_dq_t_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 template <int NH, bool RAGGED>
 static void launch_dkv_t(const AttnArgs& a, const AttnDev& p, int heads_y, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + 2 * NH * HALF_BYTES + 2 * NST * NH * Q_HALF + NST * STAT_BYTES + sizeof(DkvBars) + 64;
-  static bool attr = false;
-  if (!attr) { cudaFuncSetAttribute(flash_bwd_dkv_t_kernel<NH, RAGGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM); attr = true; }
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(flash_bwd_dkv_t_kernel<NH, RAGGED>, SMEM, allowed);
   const CUtensorMap tq = head_tmap(a.q, a.B, a.S, a.Hq, a.hd, a.ld_q, BQ), tk = head_tmap(a.k, a.B, a.S, a.Hkv, a.hd, a.ld_k),
                     tv = head_tmap(a.v, a.B, a.S, a.Hkv, a.hd, a.ld_v), tdo = head_tmap(a.d_o, a.B, a.S, a.Hq, a.hd, a.ld_do, BQ);
   flash_bwd_dkv_t_kernel<NH, RAGGED><<<dim3(p.nblk, heads_y, a.B), BWD_THREADS, SMEM, s>>>(tq, tk, tv, tdo, p);
@@ -494,8 +495,8 @@ template <int NH>
 static void launch_dq_t(const AttnArgs& a, const AttnDev& p, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + 3 * NH * HALF_BYTES + 2 * NST * NH * Q_HALF + sizeof(DqBars) + 64;
   static_assert(SMEM <= 232448, "shared memory budget of one CTA exceeded");
-  static bool attr = false;
-  if (!attr) { cudaFuncSetAttribute(flash_bwd_dq_t_kernel<NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM); attr = true; }
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(flash_bwd_dq_t_kernel<NH>, SMEM, allowed);
   const CUtensorMap tq = head_tmap(a.q, a.B, a.S, a.Hq, a.hd, a.ld_q), tk = head_tmap(a.k, a.B, a.S, a.Hkv, a.hd, a.ld_k, BQ),
                     tv = head_tmap(a.v, a.B, a.S, a.Hkv, a.hd, a.ld_v, BQ), tdo = head_tmap(a.d_o, a.B, a.S, a.Hq, a.hd, a.ld_do);
   flash_bwd_dq_t_kernel<NH><<<dim3(p.nblk, a.Hq, a.B), BWD_THREADS, SMEM, s>>>(tq, tk, tv, tdo, p);

@@ -3,6 +3,7 @@
 // K/V arrive in blocks of 64 positions: shared memory stays at 96 KB and the TMEM footprint at 256 columns, so two
 // CTAs run on every SM and one CTA's tensor-core work overlaps the other's softmax.
 #include "attention_common.cuh"
+#include "kernel_host.h"
 
 #include <string>
 
@@ -248,11 +249,8 @@ static AttnDev make_dev(const AttnArgs& a) {
 template <int NH>
 static void launch_fwd(const AttnArgs& a, cudaStream_t s) {
   constexpr size_t SMEM = 1024 + NH * HALF_BYTES + 4 * NH * KV_HALF + 256;
-  static bool attr = false;
-  if (!attr) {
-    cudaFuncSetAttribute(flash_fwd64_t_kernel<NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
-    attr = true;
-  }
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(flash_fwd64_t_kernel<NH>, SMEM, allowed);
   const AttnDev p = make_dev(a);
   const CUtensorMap tq = head_tmap(a.q, a.B, a.S, a.Hq, a.hd, a.ld_q), tk = head_tmap(a.k, a.B, a.S, a.Hkv, a.hd, a.ld_k, BKV),
                     tv = head_tmap(a.v, a.B, a.S, a.Hkv, a.hd, a.ld_v, BKV);

@@ -449,12 +449,16 @@ static void launch_gemm(const GemmArgs& a, cudaStream_t stream) {
 }
 
 int num_sms() {
-  static int sms[64] = {0};
+  static std::atomic<int> sms[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
-  if (sms[dev] == 0) cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev);
-  return sms[dev];
+  int n = sms[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    sms[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 // Tiles of width bn that the one-CTA kernel computes for this problem (launch_gemm's own count).
@@ -530,7 +534,7 @@ void gemm_bf16(const GemmArgs& a, cudaStream_t stream) {
 }
 
 int* status_word_ptr() {
-  static int* ptrs[64] = {nullptr};
+  static std::atomic<int*> ptrs[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;

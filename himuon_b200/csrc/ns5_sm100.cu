@@ -15,6 +15,7 @@
 // Rows are padded to the 128-row UMMA shape by TMA zero fill, so short tiles cost a full
 // 128-row MMA but need no separate code path.
 #include "himuon.h"
+#include "kernel_host.h"
 #include "sm100_common.cuh"
 #include "tma_host.h"
 
@@ -248,8 +249,8 @@ static void launch_ns5(const void* x_in, void* x_out, long long n_tiles, int m, 
   constexpr size_t SMEM = 1024 + (NCH + 2) * NS_HALF + 256;
   constexpr int TM_COLS = N <= 128 ? 128 : 256;
   auto kern = ns5_fused_kernel<NCH, HALVES>;
-  static bool attr = false;
-  if (!attr) { cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM); attr = true; }
+  static std::atomic<uint64_t> allowed{0};
+  allow_smem(kern, SMEM, allowed);
   const uint64_t dims[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(m), static_cast<uint64_t>(n_tiles)};
   const uint64_t strides[2] = {static_cast<uint64_t>(N) * 2, static_cast<uint64_t>(N) * 2 * m};
   const uint32_t box[3] = {64, 128, 1};

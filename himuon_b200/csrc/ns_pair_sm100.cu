@@ -29,6 +29,7 @@
 // Measured, this kernel against the GEMM launches, us: 592 of 512 x 512 1656 / 2485, 128 of them 384 / 664, 28 127 / 234,
 // 396 of 256 x 256 309 / 563, 6 of 336 x 504 110 / 165, 64 of 256 x 1024 139 / 270.  The results have the same bits.
 #include "himuon.h"
+#include "kernel_host.h"
 #include "pair_common.cuh"
 #include "sm100_common.cuh"
 #include "tma_host.h"
@@ -534,7 +535,7 @@ static cudaLaunchConfig_t nsp_config(int clusters, int P, cudaLaunchAttribute* a
 }
 
 static int nsp_max_clusters(int P) {
-  static int cache[64][NSP_MAXP + 1] = {};
+  static std::atomic<int> cache[64][NSP_MAXP + 1] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;

@@ -21,3 +21,12 @@ def test_products_are_set_up_on_every_device(name):
     assert "cudaFuncSetAttribute" not in code and re.search(r"\ballow_smem\(", code)
     kept = [k for k in _kept(code) if not re.search(r"\[64\]", k)]
     assert kept and all(k.startswith("std::atomic<uint64_t>") for k in kept), kept
+
+
+@pytest.mark.parametrize("name", LAUNCHERS)
+def test_what_launches_keep_is_atomic_and_belongs_to_a_device(name):
+    code = LAUNCHERS[name]
+    kept = _kept(code)
+    assert all(k.startswith("std::atomic<") for k in kept), kept
+    for k in kept:                                       # a bit, or a place, for each device
+        assert k.startswith("std::atomic<uint64_t>") or "[64]" in k, k
