@@ -11,7 +11,7 @@
 // blocks, a cluster, have a part of the inner dimension each, and read one another's parts.  From 33 rows on blocks with 32 rows each have a tile together, which
 // takes W from memory once and from the L2 for the others, and has more rows of W for that (64 rows, 2560 x 9728 gated and back: 51 us, 59 in one block with 64
 // rows, whose sums fill the registers).  Everything is added up in one order, which goes by the weight's sizes and, from 33 rows on, by the number of such blocks: bits
-// repeat, and a row's do not depend on how many rows up to 32 come with it.
+// repeat, and a row's do not depend on how many rows up to 32 come with it (in 8 bits, up to 16 where the weight is large: more are another kernel's, fp8.h).
 //
 // A kernel of this kind is over in 8 to 20 us, of which its start is one or two.  So the second of two (the down projection; the product behind a quantisation)
 // is launched over the first: it sets up, and fills its ring with W, while that still runs, and waits for it before it asks for x.
@@ -225,21 +225,26 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         }
         if (!mbar_wait_warp(&bars->full[stage], phase, abort_flag, p.status, 3)) { ok = false; break; }
         const uint32_t base = ring + stage * stage_bytes, x_base = base + MATS * w_bytes;
-        // A turn is latency: as many operands as there are registers for are asked for before the first product, and few rows' 8-bit products go to two sums.
-        constexpr int HALVES = NT <= 2 ? 2 : 1, STEPS = 2 * HALVES, CHAINS = HALVES;
-        float c[CHAINS][NT][4] = {};
+        // A turn is latency: as many operands as there are registers for are asked for before the first product.  In 8 bits every other product goes to another
+        // sum, and the two are scaled and added one after the other: with many rows there are registers for one of them at a time, and the order is the same.
+        constexpr int HALVES = NT <= 2 ? 2 : 1, STEPS = 2 * HALVES;
+        constexpr bool ONE_SUM = KIND == EIGHT_BITS && HALVES == 1;
+        // products 2 half and 2 half + 1 of the four, or (ONE_SUM) half and half + 2
+        const int b_at = ONE_SUM ? (b_chunk & 1) + (b_chunk >> 1) * 4 : b_chunk;
+        constexpr int B_HALF = ONE_SUM ? 2 : 4, A_STEP = ONE_SUM ? 4 : 2, A_HALF = ONE_SUM ? 2 : 4;
 #pragma unroll 1
         for (int half = 0; half < 2; half += HALVES) {
+          float c[HALVES][NT][4] = {};
           uint32_t b[HALVES][NT][4];
 #pragma unroll
           for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) ldmatrix4(b[h][n], cell(x_base, n * 8 + b_row, (half + h) * 4 + b_chunk));
+            for (int n = 0; n < NT; ++n) ldmatrix4(b[h][n], cell(x_base, n * 8 + b_row, (half + h) * B_HALF + b_at));
           uint32_t a[STEPS][MATS][4];
 #pragma unroll
           for (int m = 0; m < MATS; ++m)
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k) ldmatrix4(a[k][m], cell(base + m * w_bytes, a_row, half * 4 + k * 2 + a_chunk));
+            for (int k = 0; k < STEPS; ++k) ldmatrix4(a[k][m], cell(base + m * w_bytes, a_row, half * A_HALF + k * A_STEP + a_chunk));
 #pragma unroll
           for (int k = 0; k < STEPS; ++k)
 #pragma unroll
@@ -247,16 +252,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 const uint32_t b0 = b[k / 2][n][2 * (k % 2)], b1 = b[k / 2][n][2 * (k % 2) + 1];
-                if constexpr (KIND == EIGHT_BITS) mma_e4m3(c[k % CHAINS][n], a[k][m], b0, b1);
+                if constexpr (KIND == EIGHT_BITS) mma_e4m3(c[k % HALVES][n], a[k][m], b0, b1);
                 else mma_bf16(acc[m][n], a[k][m], b0, b1);
               }
-        }
-        if constexpr (KIND == EIGHT_BITS) {
+          if constexpr (KIND == EIGHT_BITS) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+            for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[0][n][j] = fmaf(CHAINS == 2 ? c[0][n][j] + c[CHAINS - 1][n][j] : c[0][n][j], by_w[j >> 1] * by_x[n][j & 1], acc[0][n][j]);
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[0][n][j] = fmaf(c[h][n][j], by_w[j >> 1] * by_x[n][j & 1], acc[0][n][j]);
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->empty[stage]);

@@ -96,6 +96,44 @@ def test_gates_that_are_no_numbers(activation, rows):
     _clean()
 
 
+# ------------------------------------------------------------------------------------------- rows that come with others
+def _rows(m, n):
+    return m._replace(values=m.values[:n], scales=m.scales[:n])
+
+
+@pytest.mark.parametrize("powers", [True, False])
+@pytest.mark.parametrize("outer,inner", [(2048, 2048), (200, 1000), (24, 16400)])
+def test_few_8_bit_rows_do_not_depend_on_one_another(outer, inner, powers):
+    """In fp32, which hides no order of sums: a row has the same bits alone and with up to 31 others."""
+    ops = _ops()
+    torch.manual_seed(outer + inner)
+    a, b = ops.quantize_fp8(torch.randn(32, inner, device="cuda")), ops.quantize_fp8(torch.randn(outer, inner, device="cuda"), 128)
+    if not powers:
+        a, b = (m._replace(scales=m.scales * (0.5 + torch.rand_like(m.scales)), powers=False) for m in (a, b))
+    whole = ops.fp8_matmul(a, b, out_dtype=torch.float32)
+    for n in (1, 7, 8, 9, 16, 17, 31):
+        assert torch.equal(ops.fp8_matmul(_rows(a, n), b, out_dtype=torch.float32), whole[:n]), n
+    _clean()
+
+
+def test_few_8_bit_rows_of_a_large_weight():
+    """Above 2^24 values rows come in groups of up to 16 or more, each with one order of sums; the two differ by fp32 roundings of the terms: 2^-23 of
+    their absolute values for each sum of 16 products and each of what is done to them."""
+    ops = _ops()
+    torch.manual_seed(7)
+    outer, inner = 4104, 4096
+    a, b = ops.quantize_fp8(torch.randn(32, inner, device="cuda")), ops.quantize_fp8(torch.randn(outer, inner, device="cuda"), 128)
+    few, many = (ops.fp8_matmul(_rows(a, n), b, out_dtype=torch.float32) for n in (16, 32))
+    for n in (1, 8, 9):
+        assert torch.equal(ops.fp8_matmul(_rows(a, n), b, out_dtype=torch.float32), few[:n]), n
+    for n in (17, 31):
+        assert torch.equal(ops.fp8_matmul(_rows(a, n), b, out_dtype=torch.float32), many[:n]), n
+    va, vb = (m.dequantize().double() for m in (a, b))
+    want, bound = va @ vb.t(), 2.0 ** -23 * (inner / 16 + 17) * (va.abs() @ vb.abs().t())
+    assert ((many.double() - want).abs() <= bound).all() and ((few.double() - want[:16]).abs() <= bound[:16]).all()
+    _clean()
+
+
 # ------------------------------------------------------------------------------------------- more than one device
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
 def test_products_on_a_second_device_of_the_process():
