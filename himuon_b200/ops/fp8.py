@@ -32,11 +32,11 @@ class Fp8Blocks(NamedTuple):
     powers: bool = False
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        """The values that the 8 bits stand for, in fp32 or rounded to bf16."""
+        """The values that the 8 bits stand for, in fp32 or rounded to bf16.  Under vmap the PyTorch formulation runs."""
         _check("Fp8Blocks.dequantize", self)
         if dtype not in (torch.float32, torch.bfloat16):
             raise RuntimeError(f"himuon_b200.ops.Fp8Blocks.dequantize: float32 or bfloat16 expected, got {dtype}")
-        if self.values.is_cuda:
+        if self.values.is_cuda and _kernels("Fp8Blocks.dequantize", self.values, self.scales):
             return _ext.ext().fp8_dequantize(self.values, self.scales, self.block_rows, dtype == torch.float32)
         return ref.fp8_dequantize(self.values, self.scales, self.block_rows).to(dtype)
 
@@ -51,6 +51,14 @@ def _check(op: str, m: Fp8Blocks) -> None:
     if m.scales.dtype != torch.float32 or tuple(m.scales.shape) != blocks or m.scales.device != m.values.device:
         raise RuntimeError(f"himuon_b200.ops.{op}: scales must be fp32 of {blocks} on {m.values.device}, "
                            f"got {m.scales.dtype} of {tuple(m.scales.shape)}")
+
+
+def _kernels(op: str, *tensors: torch.Tensor) -> bool:
+    """Whether the kernels can have them: not under a transform, which gives tensors without memory."""
+    if not _any_transformed(*tensors):
+        return True
+    _warn_torch_path(op, "under vmap or forward-mode differentiation")
+    return False
 
 
 def quantize_fp8(x2d: torch.Tensor, block_rows: int = 1, transpose: bool = False) -> Fp8Blocks:
@@ -76,7 +84,7 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
     """``a @ b.T`` of two 8-bit matrices ``(rows, inner)`` and ``(cols, inner)``, in bf16 or fp32.  ``a`` has blocks of 1 or 128
     rows, ``b`` of 128 (as a weight has).  The products of a block are summed by the tensor core, the blocks, scaled, in fp32 (by
     the product of two scales, which has to be a normal fp32 number).  Few rows (up to 16, or 32 of a small ``b``) run a kernel
-    that streams ``b``.  Not differentiable: see :func:`fp8_linear`."""
+    that streams ``b``.  Not differentiable: see :func:`fp8_linear`.  Under vmap the PyTorch formulation runs."""
     _check("fp8_matmul", a)
     _check("fp8_matmul", b)
     if a.values.shape[1] != b.values.shape[1] or a.values.device != b.values.device:
@@ -85,7 +93,7 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, out_dtype: torch.dtype = torch.bfloat
         raise RuntimeError(f"himuon_b200.ops.fp8_matmul: the second operand needs blocks of {BLOCK} rows")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise RuntimeError(f"himuon_b200.ops.fp8_matmul: bfloat16 or float32 expected, got {out_dtype}")
-    if a.values.is_cuda:
+    if a.values.is_cuda and _kernels("fp8_matmul", a.values, a.scales, b.values, b.scales):
         return _ext.ext().fp8_matmul(*a, *b, out_dtype == torch.float32)
     return (ref.fp8_dequantize(*a[:3]) @ ref.fp8_dequantize(*b[:3]).t()).to(out_dtype)
 
@@ -116,7 +124,7 @@ def fp8_linear(x: torch.Tensor, w) -> torch.Tensor:
             or not (kept or w.dtype == x.dtype)):
         raise RuntimeError("himuon_b200.ops.fp8_linear: (..., in) inputs and an (out, in) weight of one floating point type "
                            "on one device expected")
-    transformed = _any_transformed(x) if kept else _any_transformed(x, w)
+    transformed = _any_transformed(x, w.values, w.scales) if kept else _any_transformed(x, w)
     kernels = x.is_cuda and x.dtype == torch.bfloat16
     if kernels and not transformed:
         return _ext.ext().fp8_linear_kept(x, *w) if kept else _ext.ext().fp8_linear(x, w)

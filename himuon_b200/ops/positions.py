@@ -174,7 +174,7 @@ def rotary(x2d, positions, freqs: RotaryFrequencies, heads: int, head_dim: int, 
         if not isinstance(seq_len, int) or seq_len <= 0 or rows % seq_len:
             raise RuntimeError("himuon_b200.ops.rotary: positions must be a tensor or the length of sequences that "
                                f"{rows} rows hold, got {seq_len!r}")
-    transformed = _any_transformed(x2d)
+    transformed = _any_transformed(x2d) if positions is None else _any_transformed(x2d, positions)
     if x2d.is_cuda and x2d.dtype in (torch.bfloat16, torch.float32) and not transformed:
         if x2d.stride(1) != 1 and x2d.shape[1] > 1:
             x2d = x2d.clone(memory_format=torch.contiguous_format)

@@ -134,6 +134,59 @@ def test_few_8_bit_rows_of_a_large_weight():
     _clean()
 
 
+# ------------------------------------------------------------------------------------------- transforms of any operand
+@pytest.mark.filterwarnings("ignore:himuon_b200.ops")
+def test_vmap_over_positions():
+    """Rows that stay and positions that do not: what calls one by one return, but for two roundings to bf16."""
+    ops = _ops()
+    torch.manual_seed(11)
+    f, x, at = ops.RotaryFrequencies(16), torch.randn(6, 64, device="cuda").bfloat16(), torch.randint(0, 10000, (3, 6), device="cuda")
+    got = torch.vmap(lambda p: ops.rotary(x, p, f, 2, 32))(at)
+    for i in range(3):
+        want = ops.rotary(x, at[i], f, 2, 32).double()
+        assert (got[i].double() - want).abs().max() <= 2.01 * U * want.abs().max()
+    y = torch.vmap(lambda t, p: ops.rotary(t, p, f, 2, 32))(torch.stack([x] * 3), at)
+    assert torch.equal(y, got)
+    _clean()
+
+
+@pytest.mark.filterwarnings("ignore:himuon_b200.ops")
+@pytest.mark.parametrize("over", ["values", "scales", "both"])
+def test_vmap_over_8_bit_operands(over):
+    """Values, scales or both of either operand, of a kept weight, and of what is put back to fp32."""
+    ops = _ops()
+    torch.manual_seed(13)
+    x = torch.randn(5, 200, device="cuda").bfloat16()
+    a, b = ops.quantize_fp8(x), ops.quantize_fp8(torch.randn(140, 200, device="cuda"), 128)
+
+    def forms(m):
+        values = torch.stack([m.values.view(torch.uint8), m.values.flip(0).contiguous().view(torch.uint8)]).view(torch.float8_e4m3fn)
+        scales = torch.stack([m.scales, m.scales * 4])
+        return (values if over != "scales" else m.values.expand(2, -1, -1), scales if over != "values" else m.scales.expand(2, -1, -1))
+
+    def each(m, fn):
+        values, scales = forms(m)
+        mapped = (values if over != "scales" else values[0], scales if over != "values" else scales[0])
+        dims = (0 if over != "scales" else None, 0 if over != "values" else None)
+        got = torch.vmap(lambda v, s: fn(m._replace(values=v, scales=s)), in_dims=dims)(*mapped)
+        return [(got[i], m._replace(values=values[i].contiguous(), scales=scales[i].contiguous())) for i in range(2)]
+
+    def size(p, q):
+        return p.dequantize().double().abs() @ q.dequantize().double().abs().t()
+
+    sums = 2 * 2.0 ** -23 * (200 / 16 + 17)                # two fp32 sums of the terms
+    for got, m in each(b, lambda m: m.dequantize()):
+        assert torch.equal(got, m.dequantize())
+    for got, m in each(b, lambda m: ops.fp8_matmul(a, m, out_dtype=torch.float32)):
+        assert ((got - ops.fp8_matmul(a, m, out_dtype=torch.float32)).abs() <= sums * size(a, m)).all()
+    for got, m in each(a, lambda m: ops.fp8_matmul(m, b, out_dtype=torch.float32)):
+        assert ((got - ops.fp8_matmul(m, b, out_dtype=torch.float32)).abs() <= sums * size(m, b)).all()
+    for got, m in each(b, lambda m: ops.fp8_linear(x, m)):
+        want = ops.fp8_linear(x, m).double()
+        assert ((got.double() - want).abs() <= sums * size(a, m) + 2.01 * U * (want.abs() + sums * size(a, m))).all()
+    _clean()
+
+
 # ------------------------------------------------------------------------------------------- more than one device
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
 def test_products_on_a_second_device_of_the_process():
