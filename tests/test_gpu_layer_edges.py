@@ -96,6 +96,28 @@ def test_gates_that_are_no_numbers(activation, rows):
     _clean()
 
 
+# ------------------------------------------------------------------------------------------- sines and cosines
+@pytest.mark.parametrize("heads,hd,interleaved", [(1, 128, False), (3, 128, True), (1, 130, False)])
+def test_sines_of_every_place_in_a_turn(heads, hd, interleaved):
+    """Pairs (1, 0) come out as cosine and sine.  A place in the turn has 32 bits, so an angle is off by pi * 2^-32; a sine or cosine is good to a unit of its last
+    place, 2^-23 of it, and half of one for what the angle's low bits add.  So results near 0 are as good as near 1."""
+    ops = _ops()
+    torch.manual_seed(17)
+    f = ops.RotaryFrequencies(128, 10000.0)
+    x = torch.zeros(20000, heads, hd, device="cuda")
+    x[..., 0:128:2] = 1.0
+    if not interleaved:
+        x[..., :128] = torch.cat([torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")])
+    at = torch.randint(0, 131072, (20000,), device="cuda")
+    y = ops.rotary(x.view(20000, -1), at, f, heads, hd, interleaved=interleaved).view(20000, heads, hd)[..., :128].double()
+    cos, sin = (y[..., 0::2], y[..., 1::2]) if interleaved else y.chunk(2, -1)
+    angles = at.double()[:, None] * torch.tensor(f.frequencies, dtype=torch.float64, device="cuda")
+    for got, want in ((cos, angles.cos()), (sin, angles.sin())):
+        over = (got - want[:, None]).abs() - (math.pi * 2.0 ** -32 + 1e-10 + 1.5 * 2.0 ** -23 * want[:, None].abs())
+        assert (over <= 0).all(), over.max().item()
+    _clean()
+
+
 # ------------------------------------------------------------------------------------------- rows that come with others
 def _rows(m, n):
     return m._replace(values=m.values[:n], scales=m.scales[:n])
