@@ -351,7 +351,7 @@ void launch(const FewOperands& o, FewDev p, cudaStream_t s) {
   const auto kernel = few_rows_kernel<KIND, NT>;
   p.blocks = (o.inner * o.esz + 127) / 128;
   // Rows of W in equal shares over two blocks a SM, in tiles of up to FEW_ROWS.
-  // Where that leaves a block fewer than 32 rows, so that x would be as much to load as W, blocks share tiles instead.
+  // Where that leaves a block fewer than 24 rows, so that up to 32 of x would be as much to load as W, blocks share tiles instead.
   p.chunks = (p.rows + 31) / 32;
   p.x_rows = p.rows < 32 ? p.rows : 32;
   const int slots = 2 * num_sms() / p.chunks;

@@ -30,8 +30,8 @@ struct Fp8Matrix {
 void fp8_dequantize(const Fp8Matrix& m, void* out, long long ld_out, int out_fp32, cudaStream_t s);
 
 // c = a b^T, bf16 or fp32.  a has blocks of 1 or 128 rows, b of 128.  Rows of c are multiples of 16 bytes apart and written in whole groups of 16.
-// `powers`: all scales are powers of two (of normal numbers), as fp8_quantize() makes them; then `parts` may be fp8_parts_floats() floats of the call's own, for
-// tiles that are cut along the inner dimension (none are without).
+// `powers`: all scales are powers of two (of normal numbers), as fp8_quantize() makes them.  `parts`: fp8_parts_floats() floats of the call's own, for tiles that are
+// cut along the inner dimension, whatever the scales are (none are without).
 void fp8_product(const Fp8Matrix& a, const Fp8Matrix& b, void* c, long long ld_c, int out_fp32, int powers, float* parts, cudaStream_t s);
 long long fp8_parts_floats(const Fp8Matrix& a, const Fp8Matrix& b);
 // The same for a few rows of a; c is contiguous.  `early`: b was there before the launch that comes before this one on the stream, and may be read while that still

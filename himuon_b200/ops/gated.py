@@ -20,9 +20,11 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     bf16 CUDA tensors whose sizes are multiples of 8 run the sm_100a kernels: both projections, the activation and the product are
     one of them, as are the down projection's gradient and the gates' on the way back.  The activation sees the projections before
     they are rounded, so that the result is nearer to the exact one than that of :func:`swiglu` on finished projections, and not
-    its bits.  Few rows (up to 32, or 384 of a small block) run kernels that stream the weights.  Differentiable once in all four;
-    the backward pass needs ``x``, and keeps 8 bytes for each row and intermediate feature until then.  Under vmap and
-    forward-mode differentiation the PyTorch formulation runs."""
+    its bits.  Few rows (up to 32, 64 where a weight has 2 ** 24 values or fewer, 384 where rows times those are 4e8 or less)
+    run kernels that stream the weights.  Differentiable once in all four; the backward pass needs ``x``, and keeps 8 bytes for each
+    row and intermediate feature until then.  The gradients of ``w_gate`` and ``w_up`` are made together, as the halves of one tensor,
+    whichever of them is asked for: either keeps the memory of both.  Under vmap and forward-mode differentiation the PyTorch
+    formulation runs."""
     number = ACTIVATIONS.get(activation)
     if number is None:
         raise RuntimeError(f"himuon_b200.ops.gated_mlp: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")

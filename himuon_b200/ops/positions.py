@@ -49,7 +49,8 @@ def _form(op: str, theta: float, scaling: dict) -> tuple[str, dict]:
     # (a length may always be there: the forms that do not name it have no use for one)
     unknown = [str(k) for k in scaling if k not in (*SCALING_KEYS[kind], "rope_type", "type", "rope_theta", LENGTH)]
     if unknown:
-        raise RuntimeError(f"himuon_b200.ops.{op}: a scaling of rope_type {kind} takes {SCALING_KEYS[kind]}, got {', '.join(unknown)}")
+        raise RuntimeError(f"himuon_b200.ops.{op}: a scaling of rope_type {kind} takes {SCALING_KEYS[kind]}, "
+                           f"got {', '.join(unknown)}")
     return kind, scaling
 
 
@@ -116,8 +117,9 @@ class RotaryFrequencies:
     / rotary_dim)`` a position.  ``scaling``: as ``rope_scaling`` in a model's configuration, with ``rope_type`` ``"linear"`` (all
     frequencies divided by ``factor``), ``"ntk"`` (a larger ``theta``, by ``factor ** (d / (d - 2))``), ``"yarn"`` (``factor``,
     ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``truncate``, and ``attention_factor`` or ``mscale`` with
-    ``mscale_all_dim``) or ``"llama3"`` (``factor``, ``low_freq_factor``, ``high_freq_factor``, ``original_max_position_embeddings``).
-    Other keys are refused, as is a ``rope_theta`` other than ``theta``.
+    ``mscale_all_dim``) or ``"llama3"`` (``factor``, ``low_freq_factor``, ``high_freq_factor``,
+    ``original_max_position_embeddings``).  Keys whose value is ``None`` count as absent; other keys are refused, as is a
+    ``rope_theta`` other than ``theta``.
 
     ``frequencies``: the angles at position 1 as floats; ``factor``: what cosine and sine are multiplied by (other than 1 with
     yarn).
