@@ -9,6 +9,8 @@ import math
 import pytest
 import torch
 
+from test_gpu_layer_ops import GATED, SCALINGS, TURN, _gated64, _rotary64, _sums, _values64, _within
+
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -8
@@ -207,6 +209,53 @@ def test_vmap_over_8_bit_operands(over):
         want = ops.fp8_linear(x, m).double()
         assert ((got.double() - want).abs() <= sums * size(a, m) + 2.01 * U * (want.abs() + sums * size(a, m))).all()
     _clean()
+
+
+# ------------------------------------------------------------------------------------------- one behind the other
+@pytest.mark.parametrize("rows", [20, 300])
+def test_a_layer_operator_by_operator(rows):
+    """Each operator of a decoder layer against 64 bits on what it was really given, forward and backward, under its own bound: column slices of one projection as
+    operands, gradients that come as slices, sums of branches, 8-bit copies of what another kernel has just written."""
+    ops = _ops()
+    torch.manual_seed(rows + 19)
+    H, heads, kv, hd, I = 256, 4, 2, 64, 352
+    layout, f = ops.PackedLayout([rows // 2, rows - rows // 2 - 3]), ops.RotaryFrequencies(hd, 10000.0, SCALINGS[5])
+    at = layout.positions(rows)
+    x = torch.randn(rows, H, device="cuda").bfloat16().requires_grad_()
+    w = [(torch.randn(n, m, device="cuda") / math.sqrt(m)).bfloat16().requires_grad_() for n, m in (((heads + 2 * kv) * hd, H), (H, heads * hd), (I, H), (I, H), (H, I))]
+    calls = []
+
+    def call(fn, t, *weights):
+        given = t.view_as(t)                               # its gradient is this operator's alone
+        out = fn(given, *weights)
+        for s in (given, out):
+            s.retain_grad()
+        calls.append((given, out, weights))
+        return out
+
+    qkv = call(ops.fp8_linear, x, w[0])
+    qk = call(lambda t: ops.rotary(t, at, f, heads + kv, hd), qkv[:, : (heads + kv) * hd])
+    o = ops.packed_attention(qk[:, : heads * hd], qk[:, heads * hd:], qkv[:, (heads + kv) * hd:], layout, heads, kv, hd)
+    a = x + call(ops.fp8_linear, o, w[1])
+    y = a + call(ops.gated_mlp, a, *w[2:])
+    y.backward(torch.randn_like(y))
+    _clean()
+    for given, out, weights in (calls[0], calls[2]):
+        t, m, g = given.detach(), weights[0].detach(), out.grad
+        q = {n: _values64(ops.quantize_fp8(s, b, transpose=tr)) for n, s, b, tr in
+             (("x", t, 1, False), ("w", m, 128, False), ("dy", g, 1, False), ("dyt", g, 1, True), ("xt", t, 128, True))}
+        for what, got, p, r in (("y", out, q["x"], q["w"].t()), ("dx", given.grad, q["dy"], q["w"]), ("dw", weights[0].grad, q["dyt"], q["xt"].t())):
+            want, bound = p @ r, _sums(p.shape[1]) * (p.abs() @ r.abs())
+            _within(got, want, bound + U * (want.abs() + bound), what)
+    given, out, _ = calls[1]
+    angles = at.double()[:, None] * torch.tensor(f.frequencies, dtype=torch.float64, device="cuda")
+    for got, t, sign in ((out, given, 1.0), (given.grad, out.grad, -1.0)):
+        want, size = _rotary64(t, angles.cos(), sign * angles.sin(), heads + kv, hd, False)
+        _within(got, want, U * want.abs() + TURN * (1 + U) * size, "rotary")
+    given, out, weights = calls[3]
+    exact = _gated64(given, *weights, "silu", out.grad)
+    for name, got in zip(GATED, (out, given.grad, *(m.grad for m in weights))):
+        _within(got, *exact[name], name)
 
 
 # ------------------------------------------------------------------------------------------- more than one device
